@@ -648,6 +648,71 @@ int32_t mk_k_bf16_matmul(const float* w, int64_t rows, int64_t cols, const int64
 int32_t mk_k_q4k_matmul_tc_noalloc_dev(const void* w_q4k_dev, int64_t rows, int64_t cols, const float* x_dev, int32_t T, float* y_dev,
                                        void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators over the caller's device buffers, for serving many continuations of one prompt: sampling several answers,
+ * requests behind one long prefix, drafted tokens.  The reference has no counterparts (it decodes every lane's history by itself
+ * and one token at a time).
+ *
+ * All pointers that end in _dev are device pointers of the current device.  A call only enqueues work on cuda_stream (a
+ * cudaStream_t, NULL for the default stream): it allocates nothing, copies nothing to the host and does not wait, so it may be
+ * captured into a graph, in which sizes, pointers and host scalars are fixed and what the buffers hold is not.  The workspace is
+ * the caller's, holds nothing between calls and is not shared by calls that may overlap.  status_dev (may be NULL) points to one
+ * word into which the kernels OR what they met; nobody clears it but the caller.  No out-of-range page, length or position leads
+ * to an access outside the buffers; what the call leaves for the lanes concerned is not specified.
+ * ---------------------------------------------------------------------------------------------- */
+#define MK_DEV_BAD_PAGE 1  /* a page number outside the pool */
+#define MK_DEV_WAIT 2      /* a bounded wait inside a kernel gave up: results hold NaN */
+#define MK_DEV_BAD_RANGE 4 /* a length, count, position or setting outside what the call allows */
+#define MK_DEV_BAD_ROW 8   /* a row of logits that is no distribution: NaN, +inf, or nothing above -inf */
+
+/* Attention of a batch whose lanes share their first pages.  Lane i has lengths[i] tokens in the pages tables[i][..] (the new ones
+ * written already) and rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of q, at most `rows`, which are its last positions; cu_seqlens NULL:
+ * `rows` each, total = lanes * rows.  A row at position p attends to max(0, p - window + 1) .. p (window 0: from the first);
+ * scores are scale * q.k, with softcap > 0 then softcap * tanh(score / softcap).  A row that sees nothing becomes zeros; rows of q
+ * that belong to no lane are left as they were in out.  The first shared_len tokens (whole pages; 0 is allowed) are the same
+ * pages in every lane's table, and are read once for all lanes, through lane 0's: the result is what attention lane by lane
+ * gives.  They must hold finite values.  Values behind a lane's length may be anything.
+ * q, out [total] rows of q_heads x head_dim values, q_stride / out_stride values apart; pools of one layer, pages [kv_heads]
+ * [block_tokens][head_dim] page_stride values apart (a layer of the model's arena: kv_heads * block_tokens * head_dim); all
+ * f16 or all bf16 (type).  Rows, strides and pools are 16-byte aligned.  head_dim 64, 128 or 256; any group size up to 128.  Scores, softmax
+ * statistics and sums are 32-bit, weights are rounded to `type`. */
+int32_t mk_k_shared_attention_workspace(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_tokens, int32_t table_width, int32_t lanes, int32_t rows,
+                                        int32_t total, int32_t shared_len, int64_t* bytes);
+int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_stride, const void* k_pool_dev, const void* v_pool_dev, int64_t pool_pages, int64_t page_stride,
+                                  int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_tokens, const int32_t* tables_dev, int64_t table_stride, int32_t table_width,
+                                  const int32_t* lengths_dev, const int32_t* cu_seqlens_dev, int32_t lanes, int32_t rows, int32_t total, int32_t shared_len, float scale,
+                                  float softcap, int32_t window, void* out_dev, int64_t out_stride, void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev,
+                                  void* cuda_stream);
+
+/* Verification of drafted tokens.  logits [lanes][drafts + 1] rows of vocab values (logits_stride apart): row i of a lane is the
+ * target's answer behind its first i drafts.  Its distribution p_i is the sampler's (mk_k_sample): logits / temperature over the
+ * top_k best tokens (lower token first among equals; top_k 0: all), of those the head that adds up to top_p (below 1 only with
+ * top_k >= 1; top_k at most 1024); temperature 0: the best token.  drafts [lanes][drafts], a negative one ends a lane's;
+ * draft_probs [lanes][drafts][vocab] f32: the distributions q_i that they were drawn from, NULL: drafts without one (looked up), q_i = 1
+ * on the draft.  u [lanes][drafts + 1] uniform in [0, 1).  Draft i is kept while u_i q_i(d_i) < p_i(d_i); the first that is not is
+ * replaced by a token of max(p_i - q_i, 0), and behind the last one a token of p is added, both drawn by u_drafts: the first token, in
+ * their order, whose cumulative weight exceeds u times the whole.  tokens [lanes][drafts + 1]: the kept drafts, that token, -1 behind;
+ * accepted [lanes]: how many were kept.  A row that is no distribution ends the lane with token -1 and MK_DEV_BAD_ROW. */
+int32_t mk_k_verify_drafts_workspace(int32_t lanes, int32_t drafts, int64_t* bytes);
+int32_t mk_k_verify_drafts_dev(int32_t type, const void* logits_dev, int64_t logits_stride, int32_t lanes, int32_t drafts, int32_t vocab, const int32_t* drafts_dev,
+                               const float* draft_probs_dev, const float* u_dev, const float* temperature_dev, const int32_t* top_k_dev, const float* top_p_dev,
+                               int32_t* tokens_dev, int32_t* accepted_dev, void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev, void* cuda_stream);
+
+/* Copies inside pools [layers][pages][kv_heads][block_tokens] of rows of row_bytes: copies [n][3] of (from page, to page, rows) - the first
+ * `rows` tokens of a page, in every layer and head, K and V.  What a fork does to the page it continues, and what moves pages
+ * together.  No page is written by two copies, or written by one and read by another. */
+int32_t mk_k_copy_pages_dev(void* k_pool_dev, void* v_pool_dev, int64_t layers, int64_t pages, int32_t kv_heads, int32_t block_tokens, int32_t row_bytes,
+                            const int32_t* copies_dev, int32_t n, int32_t* status_dev, void* cuda_stream);
+
+/* Kept tokens of lanes moved together: token keep[i][j] of the pages from_tables[i] becomes token first[i] + j of the pages
+ * to_tables[i], for j < counts[i], in every layer and head, K and V.  keep ascends.  The two tables may name the same pages (then
+ * first[i] <= keep[i][0], and what has been kept stays where it is read until it has moved); otherwise no page of one lane's
+ * destination is read or written by another copy.  Accepted branches of drafted trees, and contexts thinned out. */
+int32_t mk_k_gather_tokens_dev(void* k_pool_dev, void* v_pool_dev, int64_t layers, int64_t pages, int32_t kv_heads, int32_t block_tokens, int32_t row_bytes,
+                               const int32_t* from_tables_dev, int64_t from_stride, int32_t from_width, const int32_t* keep_dev, int64_t keep_stride, int32_t keep_width,
+                               const int32_t* counts_dev, const int32_t* to_tables_dev, int64_t to_stride, int32_t to_width, const int32_t* first_dev, int32_t lanes,
+                               int32_t* status_dev, void* cuda_stream);
+
 /* TokenEmbedding::forward_validated (src/model_weights.rs:489-502). */
 int32_t mk_k_embed(int32_t type, const void* w, int64_t rows, int64_t cols, const uint32_t* ids, int32_t T, float scale, float* out);
 

@@ -6,6 +6,7 @@ through :func:`__graft_entry__.load_package` (or any importlib call that gives i
 Submodules
   _capi    ctypes binding of libmacllm_b200.so (C ABI in include/macllm_b200.h)
   ops      NumPy wrappers of the kernel-level entry points
+  device_ops  operators over CUDA tensors: shared-prefix attention, verification of drafts, moves inside the paged cache
   kv       host-only paged-KV pool / block tables / prefix cache (mirrors crates/macllm-kv)
   model    CausalLm-shaped model / session / reservation objects
   engine   the continuous-batching engine (ServingScheduler-shaped)

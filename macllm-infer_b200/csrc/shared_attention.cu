@@ -1,0 +1,433 @@
+// Attention of a batch whose lanes share their first pages.
+//
+// Row t of lane i has position p = length_i - n_i + t and sees the keys max(0, p - window + 1) .. p of the lane's pages:
+//   o = sum_j w_j v_j / sum_j w_j,   w_j = exp(cap(scale q . k_j) - m).
+// Sums over disjoint parts of the keys join exactly: with (m_a, l_a, o_a) and (m_b, l_b, o_b) of two parts and m = max(m_a, m_b), l = l_a e^(m_a - m) +
+// l_b e^(m_b - m), o likewise.  Maxima, sums and outputs of parts are 32-bit; weights are rounded to the pools' type for the product with V, as the
+// result itself is at the end.
+#include "shared_attention.h"
+#include "hgemm_tc.h"
+#include "kernels.h"
+#include "umma.cuh"
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <algorithm>
+
+namespace mk {
+
+namespace {
+
+using namespace umma;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)).
+__device__ __forceinline__ float capped(float v, float cap, float two_over_cap) {
+    return cap - __fdividef(2.0f * cap, 1.0f + __expf(fminf(v * two_over_cap, 80.0f)));
+}
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+// The 8 x 8 tile of 16-bit numbers that a warp holds as (row lane / 4, columns 2 (lane % 4), + 1), transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ void tell(int32_t* status, int bit) {
+    if (status != nullptr) atomicOr(status, bit);
+}
+
+// Where a lane's rows and keys are; whatever the arrays hold, rows stay inside [0, total) and keys inside the table.
+struct LaneRange {
+    int first, n;       // rows
+    int position;       // of its first row
+    int keys;           // length, at most what the table holds
+};
+__device__ __forceinline__ LaneRange lane_range(const SharedAttnArgs& a, int lane) {
+    LaneRange r;
+    r.first = a.cu != nullptr ? a.cu[lane] : lane * a.rows;
+    r.n = a.cu != nullptr ? a.cu[lane + 1] - r.first : a.rows;
+    const int length = a.lengths[lane];
+    r.keys = min(max(length, 0), a.width << a.bt_shift);
+    if (r.first < 0 || r.first > a.total || r.n < 0 || r.n > a.rows || r.n > a.total - r.first || r.keys != length) {
+        tell(a.status, kDevBadRange);
+        if (r.first < 0 || r.first > a.total) r.first = 0, r.n = 0;
+        r.n = min(max(r.n, 0), min(a.rows, a.total - r.first));
+    }
+    r.position = r.keys - r.n;
+    return r;
+}
+
+// ---- a lane's keys -----------------------------------------------------------------------------------------------
+//
+// A CTA takes a share of one lane's keys for NT * 8 (row, head) items of one KV head.  Each of its four warps walks tiles of 16 keys, which TMA brings
+// into a ring of its own; the items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.
+constexpr int kWarps = 4;
+constexpr int kTile = 16;
+
+template <int D>
+struct LaneSmem {
+    static constexpr int PANELS = D / 64, K_BYTES = kTile * D * 2, STAGE = 2 * K_BYTES;
+    static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? 3 : 4);
+    static constexpr int QP = D + 8, OP = D + 4;
+    static constexpr size_t bytes(int nt) { return 1024 + (size_t)kWarps * std::max(STAGES * STAGE, nt * 8 * (OP + 2) * 4) + (size_t)nt * 8 * QP * 2; }
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
+                                                               int first_key, int chunk, int shares, int first_part) {
+    using L = LaneSmem<D>;
+    using P = Pair<T>;
+    constexpr int ITEMS = NT * 8, RING = (L::STAGES * L::STAGE > ITEMS * (L::OP + 2) * 4 ? L::STAGES * L::STAGE : ITEMS * (L::OP + 2) * 4);
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[kWarps * L::STAGES];
+    uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    T* qs = reinterpret_cast<T*>(rings + kWarps * RING);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
+    const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y, g = a.q_heads / a.kv_heads;
+    const LaneRange at = lane_range(a, lane_id);
+    const int item0 = blockIdx.z * ITEMS, n_items = min(ITEMS, at.n * g - item0);
+    if (n_items <= 0) return;
+    if (tid == 0) {
+        for (int i = 0; i < kWarps * L::STAGES; ++i) bar_init(&bars[i], 1);
+        bar_init_fence();
+    }
+    const int p0 = at.position + item0 / g, p1 = at.position + (item0 + n_items - 1) / g;
+    const int lo = max(first_key + share * chunk, attention_first_key(max(p0, 0), a.window, 0)), hi = min(min(p1 + 1, at.keys), shares > 1 ? first_key + (share + 1) * chunk : INT_MAX);
+    const int begin = lo / kTile * kTile, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0;
+    const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
+
+    for (int i = tid; i < ITEMS * (D / 8); i += kWarps * 32) {
+        const int item = i / (D / 8), c = (i - item * (D / 8)) * 8;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (item < n_items) {
+            const int r = (item0 + item) / g, hq = (item0 + item) - r * g;
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(at.first + r) * a.ldq + (kvh * g + hq) * D + c);
+        }
+        *reinterpret_cast<uint4*>(qs + item * L::QP + c) = v;
+    }
+    __syncthreads();
+
+    uint8_t* ring = rings + warp * RING;
+    uint64_t* full = bars + warp * L::STAGES;
+    const int32_t* table = a.tables + lane_id * a.ld_table;
+    auto load_tile = [&](int i) {   // one lane
+        const int pos = begin + (warp + kWarps * i) * kTile;
+        int32_t page = table[pos >> a.bt_shift];
+        if ((uint32_t)page >= (uint64_t)a.pool_pages) {
+            tell(a.status, kDevBadPage);
+            page = 0;
+        }
+        const int row = (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
+        const int st = i % L::STAGES;
+        const uint32_t dst = smem_u32(ring) + st * L::STAGE;
+        bar_expect_tx(&full[st], L::STAGE);
+#pragma unroll
+        for (int p = 0; p < L::PANELS; ++p) {
+            tma_load_2d(dst + p * (kTile * 128), &tm_k, p * 64, row, &full[st]);
+            tma_load_2d(dst + L::K_BYTES + p * (kTile * 128), &tm_v, p * 64, row, &full[st]);
+        }
+    };
+    if (lane == 0)
+        for (int i = 0; i < L::STAGES && i < my_tiles; ++i) load_tile(i);
+
+    float o_acc[NT][D / 16][4], m_run[NT][2], l_run[NT][2];
+    int see_lo[NT][2], see_hi[NT][2];   // keys that the lane's two items of a group of eight see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) o_acc[n][j][0] = o_acc[n][j][1] = o_acc[n][j][2] = o_acc[n][j][3] = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            m_run[n][h] = -INFINITY;
+            l_run[n][h] = 0.f;
+            const int p = at.position + (item0 + n * 8 + 2 * tq + h) / g;
+            see_lo[n][h] = max(lo, attention_first_key(max(p, 0), a.window, 0));
+            see_hi[n][h] = min(hi, p + 1);
+        }
+    }
+    const int all_lo = max(lo, attention_first_key(max(p1, 0), a.window, 0)), all_hi = min(hi, p0 + 1);   // keys that every item sees
+    const float two_over_cap = a.softcap != 0.f ? 2.0f / a.softcap : 0.f, unit = a.softcap != 0.f ? a.scale : a.scale * kLog2e;
+    const uint32_t q_at = smem_u32(qs) + (uint32_t)((lane & 7) * L::QP + (lane >> 3) * 8) * 2;
+    bool ok = true;
+    for (int i = 0; i < my_tiles; ++i) {
+        const int st = i % L::STAGES;
+        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i / L::STAGES & 1));
+        if (!ok) {
+            if (lane == 0) tell(a.status, kDevWait);
+            break;
+        }
+        const uint32_t kt = smem_u32(ring) + st * L::STAGE, vt = kt + L::K_BYTES;
+        const int pos0 = begin + (warp + kWarps * i) * kTile;
+        if (pos0 + kTile > hi) {   // rows behind the last key hold whatever the page held: weights of 0 need finite values there
+            for (int j = lane; j < (kTile - (hi - pos0)) * 8 * L::PANELS; j += 32) {
+                const int r = hi - pos0 + j / (8 * L::PANELS), c = j % (8 * L::PANELS);
+                *reinterpret_cast<uint4*>(ring + st * L::STAGE + L::K_BYTES + (c >> 3) * (kTile * 128) + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            __syncwarp();
+        }
+        float sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        const int kr = lane & 15;
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {
+            uint32_t a0[4], a1[4];
+            const uint32_t base = kt + (kk >> 1) * (kTile * 128) + kr * 128;
+            const int cb = (kk & 1) * 64 + (lane >> 4) * 16;
+            ldmatrix_x4(a0, base + (cb ^ ((kr & 7) << 4)));
+            ldmatrix_x4(a1, base + ((cb + 32) ^ ((kr & 7) << 4)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t b[4];
+                ldmatrix_x4(b, q_at + (uint32_t)(n * 8 * L::QP + kk * 32) * 2);
+                P::mma(sc[n], a0, b[0], b[1]);
+                P::mma(sc[n], a1, b[2], b[3]);
+            }
+        }
+        const bool whole = pos0 >= all_lo && pos0 + kTile <= all_hi;
+        uint32_t b0[NT], b1[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int pos = pos0 + gid + 8 * (e >> 1);
+                float v = sc[n][e] * unit;
+                if (a.softcap != 0.f) v = capped(v, a.softcap, two_over_cap) * kLog2e;
+                sc[n][e] = whole || (pos >= see_lo[n][e & 1] && pos < see_hi[n][e & 1]) ? v : -INFINITY;
+            }
+            float alpha[2], m_use[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = fmaxf(sc[n][h], sc[n][2 + h]);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float m_new = fmaxf(m_run[n][h], top);
+                m_use[h] = m_new == -INFINITY ? 0.f : m_new;
+                alpha[h] = ex2(m_run[n][h] - m_use[h]);
+                m_run[n][h] = m_new;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] = ex2(sc[n][e] - m_use[e & 1]);
+            l_run[n][0] = l_run[n][0] * alpha[0] + (sc[n][0] + sc[n][2]);
+            l_run[n][1] = l_run[n][1] * alpha[1] + (sc[n][1] + sc[n][3]);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                o_acc[n][j][0] *= alpha[0];
+                o_acc[n][j][1] *= alpha[1];
+                o_acc[n][j][2] *= alpha[0];
+                o_acc[n][j][3] *= alpha[1];
+            }
+            b0[n] = transpose_8x8(P::pack(sc[n][0], sc[n][1]));
+            b1[n] = transpose_8x8(P::pack(sc[n][2], sc[n][3]));
+        }
+        const int vr = (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+            uint32_t af[4];
+            ldmatrix_x4_trans(af, vt + (j >> 2) * (kTile * 128) + vr * 128 + (((j & 3) * 32 + ((lane >> 3) & 1) * 16) ^ ((vr & 7) << 4)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) P::mma(o_acc[n][j], af, b0[n], b1[n]);
+        }
+        __syncwarp();
+        if (lane == 0 && i + L::STAGES < my_tiles) load_tile(i + L::STAGES);
+    }
+    if (!ok) {   // what this warp still has under way lands before the CTA ends; the result says so
+        for (int i = 0; i < L::STAGES; ++i)
+            if (i < my_tiles) bar_wait(&full[i], 0), bar_wait(&full[i], 1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) l_run[n][0] = l_run[n][1] = m_run[n][0] = m_run[n][1] = __int_as_float(0x7fffffff);
+    }
+    __syncwarp();
+    // the warps' results meet in the rings
+    float* w_o = reinterpret_cast<float*>(ring);
+    float* w_ml = w_o + ITEMS * L::OP;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float l = l_run[n][h];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int item = n * 8 + 2 * tq + h;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                w_o[item * L::OP + j * 16 + gid] = o_acc[n][j][h];
+                w_o[item * L::OP + j * 16 + gid + 8] = o_acc[n][j][2 + h];
+            }
+            if (gid == 0) {
+                w_ml[item * 2] = m_run[n][h];
+                w_ml[item * 2 + 1] = l;
+            }
+        }
+    __syncthreads();
+    constexpr int STEP = RING / 4;
+    const float* first = reinterpret_cast<const float*>(rings);
+    for (int i = tid; i < n_items * (D / 4); i += kWarps * 32) {
+        const int item = i / (D / 4), c = (i - item * (D / 4)) * 4, r = (item0 + item) / g, hq = item0 + item - r * g;
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float mw = first[w * STEP + ITEMS * L::OP + item * 2];
+            m = mw > m || mw != mw ? mw : m;
+        }
+        const float m_use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = ex2(first[w * STEP + ITEMS * L::OP + item * 2] - m_use);
+            const float4 x = *reinterpret_cast<const float4*>(first + w * STEP + item * L::OP + c);
+            l += first[w * STEP + ITEMS * L::OP + item * 2 + 1] * f;
+            o[0] += x.x * f; o[1] += x.y * f; o[2] += x.z * f; o[3] += x.w * f;
+        }
+        const int64_t row = at.first + r;
+        if (first_part < 0) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * a.ldo + (kvh * g + hq) * D + c) = make_uint2(P::pack(o[0] * inv, o[1] * inv), P::pack(o[2] * inv, o[3] * inv));
+        } else {
+            const int64_t slot = ((int64_t)(first_part + share) * a.total + row) * a.q_heads + kvh * g + hq;
+            if (l != 0.f) *reinterpret_cast<float4*>(a.part_o + slot * D + c) = make_float4(o[0], o[1], o[2], o[3]);
+            if (c == 0) a.part_ml[slot] = make_float2(m, l);
+        }
+    }
+}
+
+// The parts of a row, joined: a warp per (row, head).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ SharedAttnArgs a, int parts) {
+    constexpr int V = D / 32;   // values of a thread
+    pdl_wait();
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), n_rows = (int64_t)a.total * a.q_heads;
+    const int lane = threadIdx.x & 31;
+    if (row >= n_rows) return;
+    const int token = (int)(row / a.q_heads);
+    if (a.cu != nullptr && (token < a.cu[0] || token >= a.cu[a.lanes])) return;
+    float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += 32) {
+        const float2 ml = s0 + lane < parts ? a.part_ml[(s0 + lane) * n_rows + row] : make_float2(-INFINITY, 0.f);
+        const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ex2(ml.x - m_use);
+        l = l * old + warp_sum(ml.y * f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] *= old;
+        m = m_new;
+        const int n = min(32, parts - s0);
+#pragma unroll 4
+        for (int s = 0; s < n; ++s) {
+            const float fs = __shfl_sync(0xffffffffu, f, s);
+            if (fs == 0.f) continue;   // a part without keys wrote no output
+            const float* src = a.part_o + ((s0 + s) * n_rows + row) * D + lane * V;
+            if constexpr (V == 2) {
+                const float2 x = *reinterpret_cast<const float2*>(src);
+                o[0] += x.x * fs; o[1] += x.y * fs;
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(src + j);
+                    o[j] += x.x * fs; o[j + 1] += x.y * fs; o[j + 2] += x.z * fs; o[j + 3] += x.w * fs;
+                }
+            }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + token * a.ldo + (row - (int64_t)token * a.q_heads) * D + lane * V;
+#pragma unroll
+    for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t*>(out + j) = Pair<T>::pack(o[j] * inv, o[j + 1] * inv);
+}
+
+template <typename T, int D, int NT>
+void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
+    auto* kernel = lane_keys_kernel<T, D, NT>;
+    const size_t smem = LaneSmem<D>::bytes(NT);
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    kernel<<<dim3((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles), kWarps * 32, smem, s>>>(tk, tv, a, 0, p.chunk, p.shares, p.parts > 0 ? 0 : -1);
+    MK_LAUNCH_CHECK();
+}
+
+template <typename T, int D>
+void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t s) {
+    const uint64_t rows = (uint64_t)(a.pool_pages - 1) * (uint64_t)a.page_rows + (uint64_t)a.kv_heads * (uint64_t)a.block_tokens;
+    alignas(64) CUtensorMap tk, tv;
+    encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, kTile, true);
+    encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, kTile, true);
+    switch (p.items) {
+        case 8: launch_lanes<T, D, 1>(a, p, tk, tv, s); break;
+        case 16: launch_lanes<T, D, 2>(a, p, tk, tv, s); break;
+        default:
+            if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, tk, tv, s);
+    }
+    if (p.parts > 0) {
+        join_parts_kernel<T, D><<<(unsigned)(((int64_t)a.total * a.q_heads + 7) / 8), 256, 0, s>>>(a, (int)p.parts);
+        MK_LAUNCH_CHECK();
+    }
+}
+
+}  // namespace
+
+SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared) {
+    SharedAttnPlan p;
+    const int64_t items = (int64_t)rows * (q_heads / kv_heads);
+    if (items <= 0 || lanes <= 0 || total <= 0) return p;
+    p.items = (int)std::min<int64_t>((items + 7) / 8 * 8, d == 256 ? 16 : 24);
+    p.item_tiles = (int)((items + p.items - 1) / p.items);
+    const int64_t keys = (int64_t)width * block_tokens;
+    p.chunk = 512;
+    p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
+    p.parts = p.shares > 1 ? p.shares : 0;
+    return p;
+}
+
+void launch_shared_attention(SharedAttnArgs a, const SharedAttnPlan& p, cudaStream_t s) {
+    if (a.lanes <= 0 || a.total <= 0 || a.rows <= 0) return;
+    for (a.bt_shift = 0; (1 << a.bt_shift) < a.block_tokens; ++a.bt_shift) {}
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + p.parts * a.total * a.q_heads * a.d);
+    switch (a.d) {
+        case 64: a.bf16 ? launch_typed<__nv_bfloat16, 64>(a, p, s) : launch_typed<__half, 64>(a, p, s); break;
+        case 128: a.bf16 ? launch_typed<__nv_bfloat16, 128>(a, p, s) : launch_typed<__half, 128>(a, p, s); break;
+        case 256: a.bf16 ? launch_typed<__nv_bfloat16, 256>(a, p, s) : launch_typed<__half, 256>(a, p, s); break;
+        default: throw std::runtime_error("launch_shared_attention: unsupported head size");
+    }
+}
+
+}  // namespace mk
