@@ -668,7 +668,7 @@ int32_t mk_k_q4k_matmul_tc_noalloc_dev(const void* w_q4k_dev, int64_t rows, int6
 /* Attention of a batch whose lanes share their first pages.  Lane i has lengths[i] tokens in the pages tables[i][..] (the new ones
  * written already) and rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of q, at most `rows`, which are its last positions; cu_seqlens NULL:
  * `rows` each, total = lanes * rows.  A row at position p attends to max(0, p - window + 1) .. p (window 0: from the first);
- * scores are scale * q.k, with softcap > 0 then softcap * tanh(score / softcap).  A row that sees nothing becomes zeros; rows of q
+ * scores are scale * q.k (scale > 0), with softcap > 0 then softcap * tanh(score / softcap).  A row that sees nothing becomes zeros; rows of q
  * that belong to no lane are left as they were in out.  The first shared_len tokens (whole pages; 0 is allowed) are the same
  * pages in every lane's table, and are read once for all lanes, through lane 0's: the result is what attention lane by lane
  * gives.  They must hold finite values.  Values behind a lane's length may be anything.

@@ -6,6 +6,7 @@
 #include "shared_attention.h"
 #include "verify_drafts.h"
 #include <climits>
+#include <cmath>
 
 using namespace mk;
 
@@ -58,7 +59,8 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
         need(pool_pages > 0 && page_stride % head_dim == 0 && page_stride >= (int64_t)kv_heads * block_tokens * head_dim, "mk_k_shared_attention_dev: pages overlap, or do not begin at a row");
         need(pool_pages <= INT32_MAX && page_stride / head_dim <= INT32_MAX && pool_pages * (page_stride / head_dim) <= INT32_MAX,
              "mk_k_shared_attention_dev: a pool has at most 2^31 - 1 rows of a head");
-        need(softcap >= 0.f && window >= 0, "mk_k_shared_attention_dev: softcap and window are not negative");
+        need(scale > 0.f && std::isfinite(scale), "mk_k_shared_attention_dev: scale is positive");
+        need(softcap >= 0.f && std::isfinite(softcap) && window >= 0, "mk_k_shared_attention_dev: softcap and window are not negative");
         const int64_t bytes = p.bytes(total, q_heads, head_dim);
         need(bytes == 0 || (workspace_dev != nullptr && workspace_bytes >= bytes && aligned(workspace_dev, 16)), "mk_k_shared_attention_dev: the workspace is missing, too small or not aligned to 16 bytes");
         require_device();

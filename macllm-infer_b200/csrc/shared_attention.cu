@@ -12,6 +12,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace mk {
 
@@ -20,6 +21,7 @@ namespace {
 using namespace umma;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSms = 148;   // calls are cut without a device, for a B200
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -96,6 +98,50 @@ __device__ __forceinline__ LaneRange lane_range(const SharedAttnArgs& a, int lan
     return r;
 }
 
+// The parts [first, first + parts) of a row's results, added to a warp's (m, l, o), V values of o per thread.
+template <int D>
+__device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, int parts, float& m, float& l, float (&o)[D / 32]) {
+    constexpr int V = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int64_t n_rows = (int64_t)a.total * a.q_heads;
+    for (int s0 = 0; s0 < parts; s0 += 32) {
+        const float2 ml = s0 + lane < parts ? a.part_ml[(s0 + lane) * n_rows + row] : make_float2(-INFINITY, 0.f);
+        const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ex2(ml.x - m_use);
+        l = l * old + warp_sum(ml.y * f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] *= old;
+        m = m_new;
+        const int n = min(32, parts - s0);
+#pragma unroll 4
+        for (int s = 0; s < n; ++s) {
+            const float fs = __shfl_sync(0xffffffffu, f, s);
+            if (fs == 0.f) continue;   // a part without keys wrote no output
+            const float* src = a.part_o + ((s0 + s) * n_rows + row) * D + lane * V;
+            if constexpr (V == 2) {
+                const float2 x = *reinterpret_cast<const float2*>(src);
+                o[0] += x.x * fs; o[1] += x.y * fs;
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(src + j);
+                    o[j] += x.x * fs; o[j + 1] += x.y * fs; o[j + 2] += x.z * fs; o[j + 3] += x.w * fs;
+                }
+            }
+        }
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* out, const float (&o)[V], float l) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;   // a row that sees nothing: zeros
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int j = 0; j < V; j += 2) w[j / 2] = Pair<T>::pack(o[j] * inv, o[j + 1] * inv);
+    if constexpr (V == 2) *reinterpret_cast<uint32_t*>(out) = w[0];
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // ---- a lane's keys -----------------------------------------------------------------------------------------------
 //
 // A CTA takes a share of one lane's keys for NT * 8 (row, head) items of one KV head.  Each of its four warps walks tiles of 16 keys, which TMA brings
@@ -113,7 +159,7 @@ struct LaneSmem {
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
-                                                               int first_key, int chunk, int shares, int first_part) {
+                                                               int chunk, int shares, int shared_parts, int join) {
     using L = LaneSmem<D>;
     using P = Pair<T>;
     constexpr int ITEMS = NT * 8, RING = (L::STAGES * L::STAGE > ITEMS * (L::OP + 2) * 4 ? L::STAGES * L::STAGE : ITEMS * (L::OP + 2) * 4);
@@ -126,6 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_con
     const LaneRange at = lane_range(a, lane_id);
     const int item0 = blockIdx.z * ITEMS, n_items = min(ITEMS, at.n * g - item0);
     if (n_items <= 0) return;
+    const int first_key = a.shared;
     if (tid == 0) {
         for (int i = 0; i < kWarps * L::STAGES; ++i) bar_init(&bars[i], 1);
         bar_init_fence();
@@ -301,11 +348,14 @@ __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_con
             }
         }
     __syncthreads();
-    constexpr int STEP = RING / 4;
+    constexpr int STEP = RING / 4, V = D / 32;
     const float* first = reinterpret_cast<const float*>(rings);
-    for (int i = tid; i < n_items * (D / 4); i += kWarps * 32) {
-        const int item = i / (D / 4), c = (i - item * (D / 4)) * 4, r = (item0 + item) / g, hq = item0 + item - r * g;
-        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    pdl_wait();   // the shared keys' parts; and who comes after this kernel may rely on them too
+    for (int item = warp; item < n_items; item += kWarps) {
+        const int r = (item0 + item) / g, hq = item0 + item - r * g;
+        float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float mw = first[w * STEP + ITEMS * L::OP + item * 2];
@@ -315,18 +365,22 @@ __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_con
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float f = ex2(first[w * STEP + ITEMS * L::OP + item * 2] - m_use);
-            const float4 x = *reinterpret_cast<const float4*>(first + w * STEP + item * L::OP + c);
+            const float* x = first + w * STEP + item * L::OP + lane * V;
             l += first[w * STEP + ITEMS * L::OP + item * 2 + 1] * f;
-            o[0] += x.x * f; o[1] += x.y * f; o[2] += x.z * f; o[3] += x.w * f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] += x[j] * f;
         }
-        const int64_t row = at.first + r;
-        if (first_part < 0) {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
-            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * a.ldo + (kvh * g + hq) * D + c) = make_uint2(P::pack(o[0] * inv, o[1] * inv), P::pack(o[2] * inv, o[3] * inv));
+        const int64_t row = at.first + r, head = kvh * g + hq;
+        if (join) {
+            add_parts<D>(a, row * a.q_heads + head, shared_parts, m, l, o);
+            store_row<T, V>(static_cast<T*>(a.out) + row * a.ldo + head * D + lane * V, o, l);
         } else {
-            const int64_t slot = ((int64_t)(first_part + share) * a.total + row) * a.q_heads + kvh * g + hq;
-            if (l != 0.f) *reinterpret_cast<float4*>(a.part_o + slot * D + c) = make_float4(o[0], o[1], o[2], o[3]);
-            if (c == 0) a.part_ml[slot] = make_float2(m, l);
+            const int64_t slot = ((int64_t)(shared_parts + share) * a.total + row) * a.q_heads + head;
+            if (l != 0.f) {
+#pragma unroll
+                for (int j = 0; j < V; j += 2) *reinterpret_cast<float2*>(a.part_o + slot * D + lane * V + j) = make_float2(o[j], o[j + 1]);
+            }
+            if (lane == 0) a.part_ml[slot] = make_float2(m, l);
         }
     }
 }
@@ -336,44 +390,322 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ SharedAttnArgs a, int parts) {
     constexpr int V = D / 32;   // values of a thread
     pdl_wait();
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), n_rows = (int64_t)a.total * a.q_heads;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (row >= n_rows) return;
+    if (row >= (int64_t)a.total * a.q_heads) return;
     const int token = (int)(row / a.q_heads);
     if (a.cu != nullptr && (token < a.cu[0] || token >= a.cu[a.lanes])) return;
     float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = 0.f;
-    for (int s0 = 0; s0 < parts; s0 += 32) {
-        const float2 ml = s0 + lane < parts ? a.part_ml[(s0 + lane) * n_rows + row] : make_float2(-INFINITY, 0.f);
-        const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ex2(ml.x - m_use);
-        l = l * old + warp_sum(ml.y * f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] *= old;
-        m = m_new;
-        const int n = min(32, parts - s0);
-#pragma unroll 4
-        for (int s = 0; s < n; ++s) {
-            const float fs = __shfl_sync(0xffffffffu, f, s);
-            if (fs == 0.f) continue;   // a part without keys wrote no output
-            const float* src = a.part_o + ((s0 + s) * n_rows + row) * D + lane * V;
-            if constexpr (V == 2) {
-                const float2 x = *reinterpret_cast<const float2*>(src);
-                o[0] += x.x * fs; o[1] += x.y * fs;
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + j);
-                    o[j] += x.x * fs; o[j + 1] += x.y * fs; o[j + 2] += x.z * fs; o[j + 3] += x.w * fs;
+    add_parts<D>(a, row, parts, m, l, o);
+    store_row<T, V>(static_cast<T*>(a.out) + token * a.ldo + (row - (int64_t)token * a.q_heads) * D + lane * V, o, l);
+}
+
+// ---- the shared keys ---------------------------------------------------------------------------------------------
+//
+// All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA,
+// over a share of the keys in tiles of KEYS.  One warp brings keys and values by TMA, one issues the tcgen05 products, four per tile of items do the
+// softmax, a thread per item.  Products go round in units (tile of keys, tile of items): scores of unit u into one of two areas of tensor memory, u & 1; its
+// weights go back over its scores, as the A operand of O += P V; and the area is free for the scores of unit u + 2 as soon as that product is issued, since
+// products of one thread run in their order.  With two tiles of items the one's softmax runs under the other's products and a key is
+// fetched once for both.  The running maximum follows only when a tile exceeds it by kSlack (weights stay below 2^kSlack).
+constexpr float kSlack = 8.f;
+constexpr int kItems = 128;
+
+template <int D, int NQ>
+struct SharedSmem {
+    static constexpr int KEYS = D == 256 ? 64 : 128, PANELS = D / 64, PANEL = KEYS * 128, QPANEL = kItems * 128, BYTES = PANELS * PANEL;
+    static constexpr int STAGES = D == 64 ? 4 : 2, THREADS = NQ * 128 + 64;
+    static constexpr size_t SMEM = 1024 + (size_t)NQ * PANELS * QPANEL + (size_t)STAGES * 2 * BYTES;
+};
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(SharedSmem<D, NQ>::THREADS, 1)
+shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a, int box, int splits) {
+    using L = SharedSmem<D, NQ>;
+    constexpr int ST = L::STAGES, KEYS = L::KEYS, S_AT = NQ * D;   // columns of tensor memory: outputs, then the two areas
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[4 * ST + 7];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int4 sees[NQ * 4];
+    uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST, *s_full = bars + 4 * ST, *p_full = s_full + 2, *o_done = s_full + 4, *q_full = s_full + 6;
+    uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* ks = qs + NQ * L::PANELS * L::QPANEL;
+    uint8_t* vs = ks + ST * L::BYTES;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = a.q_heads / a.kv_heads;
+    const int split = blockIdx.x % splits, kvh = blockIdx.x / splits % a.kv_heads, tile = blockIdx.x / splits / a.kv_heads;
+    pdl_trigger();
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            bar_init(&k_full[i], 1);
+            bar_init(&k_empty[i], 1);
+            bar_init(&v_full[i], 1);
+            bar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&s_full[i], 1);
+            bar_init(&p_full[i], kItems);
+            bar_init(&o_done[i], 1);
+        }
+        bar_init(q_full, NQ * kItems);
+        bar_init_fence();
+    }
+    // what this thread's item is, and what it sees
+    const int64_t item = (int64_t)tile * (NQ * kItems) + tid;
+    int token = -1, head = 0, see_lo = 0, see_hi = 0;
+    if (warp < NQ * 4) {
+        const int64_t at_token = item / g;
+        if (at_token < a.total) {
+            int l = 0;
+            if (a.cu == nullptr) {
+                l = (int)at_token / a.rows;
+            } else {   // the last lane that begins at or before this row
+                int lo = 0, hi = a.lanes;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (a.cu[mid] <= at_token) lo = mid;
+                    else hi = mid;
                 }
+                l = lo;
+            }
+            const LaneRange at = lane_range(a, l);
+            if (at_token >= at.first && at_token < at.first + at.n) {
+                token = (int)at_token;
+                head = kvh * g + (int)(item - at_token * g);
+                const int p = at.position + token - at.first;
+                see_lo = attention_first_key(max(p, 0), a.window, 0);
+                see_hi = min(a.shared, p + 1);
+            }
+        }
+        const bool live = token >= 0 && see_hi > see_lo;
+        const int4 s = make_int4(__reduce_min_sync(0xffffffffu, live ? see_lo : INT_MAX), __reduce_max_sync(0xffffffffu, token >= 0 ? see_lo : 0),
+                                 __reduce_min_sync(0xffffffffu, token >= 0 ? see_hi : INT_MAX), __reduce_max_sync(0xffffffffu, live ? see_hi : 0));
+        if (lane == 0) sees[warp] = s;
+    }
+    if (warp == NQ * 4 + 1) tmem_alloc(&tmem_slot, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
+#pragma unroll
+    for (int w = 0; w < NQ * 4; ++w) {
+        lo_min = min(lo_min, sees[w].x);
+        lo_max = max(lo_max, sees[w].y);
+        hi_min = min(hi_min, sees[w].z);
+        hi_max = max(hi_max, sees[w].w);
+    }
+    const int all_tiles = (a.shared + KEYS - 1) / KEYS;
+    const int t_begin = max((int)((int64_t)all_tiles * split / splits), lo_min / KEYS);
+    const int t_end = min((int)((int64_t)all_tiles * (split + 1) / splits), (hi_max + KEYS - 1) / KEYS);
+    const int n_tiles = max(0, t_end - t_begin), units = n_tiles * NQ;
+
+    if (warp == NQ * 4) {
+        // ---- loader
+        const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most KEYS / 16 boxes of each of the panels: 16
+        const bool mine = panel < L::PANELS;
+        auto page_row = [&](int t) {
+            int pos = (t_begin + t) * KEYS + of * box;
+            if (pos >= a.shared) pos = a.shared - box;   // keys behind the last one are not seen; they are read from where there is something
+            int32_t page = mine && t < n_tiles ? a.tables[pos >> a.bt_shift] : 0;
+            if ((uint32_t)page >= (uint64_t)a.pool_pages) {
+                tell(a.status, kDevBadPage);
+                page = 0;
+            }
+            return (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
+        };
+        if (lane == 0) {
+            prefetch_tensormap(&tm_k);
+            prefetch_tensormap(&tm_v);
+        }
+        bool ok = true;
+        int t = 0, row = page_row(0);
+        for (; t < n_tiles; ++t) {
+            const int next = page_row(t + 1), st = t % ST;
+            const uint32_t ph = (uint32_t)(t / ST & 1) ^ 1;
+            ok = __all_sync(0xffffffffu, bar_wait(&k_empty[st], ph));
+            if (!ok) break;
+            if (lane == 0) bar_expect_tx(&k_full[st], L::BYTES);
+            __syncwarp();
+            if (mine) tma_load_2d(smem_u32(ks) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_k, panel * 64, row, &k_full[st]);
+            ok = __all_sync(0xffffffffu, bar_wait(&v_empty[st], ph));
+            if (!ok) break;
+            if (lane == 0) bar_expect_tx(&v_full[st], L::BYTES);
+            __syncwarp();
+            if (mine) tma_load_2d(smem_u32(vs) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_v, panel * 64, row, &v_full[st]);
+            row = next;
+        }
+        if (!ok) {
+            if (lane == 0) tell(a.status, kDevWait);
+            for (int u = max(0, t - ST); u <= t && u < n_tiles; ++u) {   // copies in flight land before the CTA ends
+                bar_wait(&k_full[u % ST], u / ST & 1);
+                if (u < t) bar_wait(&v_full[u % ST], u / ST & 1);
+            }
+        }
+    } else if (warp == NQ * 4 + 1) {
+        // ---- products
+        if (lane == 0 && units > 0) {
+            constexpr uint32_t kind = std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u;
+            constexpr uint32_t i_scores = f16_idesc(kItems, KEYS, false) | kind, i_out = f16_idesc(kItems, D, true) | kind;
+            const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
+            auto scores = [&](int u) {
+                const int t = u / NQ, q = u % NQ, st = t % ST;
+                if (q == 0) {
+                    if (!bar_wait(&k_full[st], t / ST & 1)) return false;
+                    fence_after();
+                }
+                const uint64_t qd = sw128_desc(q_addr + q * L::PANELS * L::QPANEL), kd = sw128_desc(k_addr + st * L::BYTES);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    mma(tmem + S_AT + (u & 1) * KEYS, qd + (i >> 2) * (L::QPANEL / 16) + (i & 3) * 2, kd + (i >> 2) * (L::PANEL / 16) + (i & 3) * 2, i_scores, i > 0);
+                if (q == NQ - 1) commit(&k_empty[st]);
+                commit(&s_full[u & 1]);
+                return true;
+            };
+            bool ok = bar_wait(q_full, 0);
+            fence_after();
+            ok = ok && scores(0) && (units < 2 || scores(1));
+            for (int u = 0; u < units && ok; ++u) {
+                const int t = u / NQ, q = u % NQ, st = t % ST;
+                ok = (q > 0 || bar_wait(&v_full[st], t / ST & 1)) && bar_wait(&p_full[u & 1], u >> 1 & 1);
+                if (!ok) break;
+                fence_after();
+                const uint32_t p = tmem + S_AT + (u & 1) * KEYS;
+                const uint64_t v = sw128_desc(v_addr + st * L::BYTES, L::PANEL);
+#pragma unroll
+                for (int i = 0; i < KEYS / 16; ++i) mma_tmem_a(tmem + q * D, p + i * 8, v + i * 128, i_out, t > 0 || i > 0);
+                if (q == NQ - 1) commit(&v_empty[st]);
+                commit(&o_done[u & 1]);
+                if (u + 2 < units) ok = scores(u + 2);
+            }
+            if (!ok) tell(a.status, kDevWait);
+        }
+    } else {
+        // ---- one item per thread
+        for (int i = tid; i < NQ * kItems * (D / 8); i += NQ * kItems) {
+            const int it = i / (D / 8), c = (i - it * (D / 8)) * 8;
+            const int64_t index = (int64_t)tile * (NQ * kItems) + it, tok = index / g;
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (tok < a.total) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.ldq + (kvh * g + (index - tok * g)) * D + c);
+            const int q = it / kItems, r = it % kItems;
+            *reinterpret_cast<uint4*>(qs + (q * L::PANELS + (c >> 6)) * L::QPANEL + r * 128 + (((c & 63) * 2) ^ ((r & 7) << 4))) = x;
+        }
+        fence_async_smem();
+        bar_arrive(q_full);
+
+        const int q = warp >> 2;
+        const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = my + q * D;
+        const float two_over_cap = a.softcap != 0.f ? 2.0f / a.softcap : 0.f, unit = a.softcap != 0.f ? kLog2e : a.scale * kLog2e;
+        float m_run = -INFINITY, sum = 0.f;   // the maximum as a base-2 logarithm
+        bool ok = true;
+        for (int u = NQ == 2 ? q : 0; u < units; u += NQ) {
+            const int t = u / NQ;
+            ok = __all_sync(0xffffffffu, bar_wait(&s_full[u & 1], u >> 1 & 1));
+            if (!ok) break;
+            fence_after();
+            const uint32_t s_at = my + S_AT + (u & 1) * KEYS;
+            float s[KEYS];
+#pragma unroll
+            for (int j = 0; j < KEYS; j += 32) tmem_ld32(s_at + j, reinterpret_cast<uint32_t*>(s) + j);
+            tmem_wait_ld();
+            const int pos0 = (t_begin + t) * KEYS;
+            if (a.softcap != 0.f) {
+#pragma unroll
+                for (int j = 0; j < KEYS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
+            }
+            if (pos0 + KEYS > hi_min || pos0 < lo_max) {   // uniform: some item does not see the whole tile
+#pragma unroll
+                for (int j = 0; j < KEYS; ++j) s[j] = pos0 + j >= see_lo && pos0 + j < see_hi ? s[j] : -INFINITY;
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int j = 4; j < KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
+            const bool grow = m_tile > m_run + kSlack;   // also when there was none yet
+            if (__any_sync(0xffffffffu, grow)) {
+                const float m_new = grow ? m_tile : m_run;
+                const float alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_new);
+                if (t > 0) {
+                    // the item's product before: with two tiles of items these scores were issued behind it
+                    if (NQ == 1) ok = __all_sync(0xffffffffu, bar_wait(&o_done[(u - 1) & 1], (u - 1) >> 1 & 1));
+                    if (!ok) break;
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                        tmem_st32(o_at + c, o);
+                    }
+                }
+                sum *= alpha;
+                m_run = m_new;
+            }
+            const float m_use = m_run == -INFINITY ? 0.f : m_run;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j0 = 0; j0 < KEYS; j0 += 64) {
+                uint32_t w[32];
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) {
+                    const float x = ex2(fmaf(s[j0 + j], unit, -m_use)), y = ex2(fmaf(s[j0 + j + 1], unit, -m_use));
+                    part[j & 3] += x;
+                    part[(j & 3) + 1] += y;
+                    w[j / 2] = Pair<T>::pack(x, y);
+                }
+                tmem_st32(s_at + j0 / 2, w);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            tmem_wait_st();
+            fence_before();
+            bar_arrive(&p_full[u & 1]);
+        }
+        if (ok && units > 0) {
+            const int last = units - NQ + (NQ == 2 ? q : 0);
+            ok = __all_sync(0xffffffffu, bar_wait(&o_done[last & 1], last >> 1 & 1));
+        }
+        if (!ok) {
+            if (lane == 0) tell(a.status, kDevWait);
+            sum = m_run = __int_as_float(0x7fffffff);   // the result says so
+        }
+        fence_after();
+        const int64_t slot = ((int64_t)split * a.total + token) * a.q_heads + head;
+        if (token >= 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
+        if (units > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_at + c, o);
+                tmem_wait_ld();
+                if (token < 0) continue;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    *reinterpret_cast<uint4*>(a.part_o + slot * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    T* out = static_cast<T*>(a.out) + token * a.ldo + (row - (int64_t)token * a.q_heads) * D + lane * V;
-#pragma unroll
-    for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t*>(out + j) = Pair<T>::pack(o[j] * inv, o[j + 1] * inv);
+    fence_before();
+    __syncthreads();
+    if (warp == NQ * 4 + 1) {
+        fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int D, int NQ>
+void launch_shared_part(const SharedAttnArgs& a, const SharedAttnPlan& p, uint64_t rows, cudaStream_t s) {
+    using L = SharedSmem<D, NQ>;
+    const int box = std::min(a.block_tokens, L::KEYS);
+    alignas(64) CUtensorMap tk, tv;
+    encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, (uint32_t)box, true);
+    encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, (uint32_t)box, true);
+    auto* kernel = shared_keys_kernel<T, D, NQ>;
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::SMEM);
+    kernel<<<(unsigned)(p.row_tiles * a.kv_heads * p.shared_parts), L::THREADS, L::SMEM, s>>>(tk, tv, a, box, p.shared_parts);
+    MK_LAUNCH_CHECK();
 }
 
 template <typename T, int D, int NT>
@@ -381,13 +713,24 @@ void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtens
     auto* kernel = lane_keys_kernel<T, D, NT>;
     const size_t smem = LaneSmem<D>::bytes(NT);
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-    kernel<<<dim3((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles), kWarps * 32, smem, s>>>(tk, tv, a, 0, p.chunk, p.shares, p.parts > 0 ? 0 : -1);
+    const dim3 grid((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles);
+    // behind the shared keys' kernel it starts early: what both read was there before that one
+    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(kWarps * 32), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
+    else kernel<<<grid, kWarps * 32, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
     MK_LAUNCH_CHECK();
 }
 
 template <typename T, int D>
 void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t s) {
     const uint64_t rows = (uint64_t)(a.pool_pages - 1) * (uint64_t)a.page_rows + (uint64_t)a.kv_heads * (uint64_t)a.block_tokens;
+    if (p.shared_parts > 0) {
+        if constexpr (D <= 128) {
+            if (p.item_rows == 2) launch_shared_part<T, D, 2>(a, p, rows, s);
+            else launch_shared_part<T, D, 1>(a, p, rows, s);
+        } else {
+            launch_shared_part<T, D, 1>(a, p, rows, s);
+        }
+    }
     alignas(64) CUtensorMap tk, tv;
     encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, kTile, true);
     encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, kTile, true);
@@ -397,24 +740,40 @@ void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t
         default:
             if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, tk, tv, s);
     }
-    if (p.parts > 0) {
-        join_parts_kernel<T, D><<<(unsigned)(((int64_t)a.total * a.q_heads + 7) / 8), 256, 0, s>>>(a, (int)p.parts);
-        MK_LAUNCH_CHECK();
-    }
+    if (p.shares > 1)
+        launch_pdl(join_parts_kernel<T, D>, dim3((unsigned)(((int64_t)a.total * a.q_heads + 7) / 8)), dim3(256), 0, s, a, (int)p.parts);
 }
 
 }  // namespace
 
 SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared) {
     SharedAttnPlan p;
-    const int64_t items = (int64_t)rows * (q_heads / kv_heads);
+    const int g = q_heads / kv_heads;
+    const int64_t items = (int64_t)rows * g;
     if (items <= 0 || lanes <= 0 || total <= 0) return p;
     p.items = (int)std::min<int64_t>((items + 7) / 8 * 8, d == 256 ? 16 : 24);
     p.item_tiles = (int)((items + p.items - 1) / p.items);
-    const int64_t keys = (int64_t)width * block_tokens;
-    p.chunk = 512;
+    // A lane's own keys: whole where the lanes fill the device, else in shares of at least 256 keys; never more than 1024, since lanes differ in length.
+    const int64_t keys = (int64_t)width * block_tokens - shared, ctas = (int64_t)lanes * kv_heads * p.item_tiles;
+    const int64_t wanted = std::max<int64_t>(1, (4 * kSms + ctas - 1) / ctas);
+    p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), 1024) / 16 * 16;
     p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
-    p.parts = p.shares > 1 ? p.shares : 0;
+    if (shared > 0) {
+        // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.5 us per
+        // tile of items, its start and end 4 us, and a share's results are written and read once.
+        const int64_t all = (int64_t)total * g;
+        p.item_rows = d <= 128 && all > kItems ? 2 : 1;
+        p.row_tiles = (int)((all + kItems * p.item_rows - 1) / (kItems * p.item_rows));
+        const int tiles = (shared + (d == 256 ? 63 : 127)) / (d == 256 ? 64 : 128);
+        const double results_us = (double)total * q_heads * d * 8 / 8e6;
+        double best = 0;
+        for (int n = 1; n <= std::min(tiles, 148); ++n) {
+            const int64_t waves = ((int64_t)p.row_tiles * kv_heads * n + kSms - 1) / kSms;
+            const double us = waves * ((tiles + n - 1) / n * 0.5 * p.item_rows + 4.0) + n * results_us;
+            if (n == 1 || us < best) best = us, p.shared_parts = n;
+        }
+    }
+    p.parts = p.shared_parts + (p.shares > 1 ? p.shares : 0);
     return p;
 }
 

@@ -38,6 +38,7 @@ struct SharedAttnPlan {
     int item_tiles = 0;      // blocks of (row, head) items of a lane and KV head
     int items = 0;           // items of such a block, a multiple of 8
     int chunk = 0, shares = 0;   // keys of a lane's share, and shares
+    int item_rows = 0, row_tiles = 0, shared_parts = 0;   // shared keys: tiles of items to a CTA, CTAs along the items, shares of the keys
     int64_t parts = 0;       // partial results of a row; 0: none are written
     int64_t bytes(int total, int q_heads, int d) const { return parts * total * q_heads * ((int64_t)d * 4 + 8); }
 };

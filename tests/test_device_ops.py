@@ -53,6 +53,8 @@ ATTENTION = dict(type=1, q=A, q_stride=1024, k_pool=A, v_pool=A, pool_pages=100,
     (dict(tables=None), "null pointer"),
     (dict(softcap=-1.0), "not negative"),
     (dict(window=-1), "not negative"),
+    (dict(scale=0.0), "positive"),
+    (dict(scale=float("nan")), "positive"),
     (dict(workspace=None), "workspace"),
     (dict(workspace_bytes=16), "workspace"),
     (dict(workspace=A + 4), "workspace"),
