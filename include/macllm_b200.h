@@ -684,7 +684,7 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
                                   float softcap, int32_t window, void* out_dev, int64_t out_stride, void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev,
                                   void* cuda_stream);
 
-/* Verification of drafted tokens.  logits [lanes][drafts + 1] rows of vocab values (logits_stride apart): row i of a lane is the
+/* Verification of drafted tokens.  logits [lanes][drafts + 1] rows of vocab values, at most 416000 (logits_stride apart): row i of a lane is the
  * target's answer behind its first i drafts.  Its distribution p_i is the sampler's (mk_k_sample): logits / temperature over the
  * top_k best tokens (lower token first among equals; top_k 0: all), of those the head that adds up to top_p (below 1 only with
  * top_k >= 1; top_k at most 1024); temperature 0: the best token.  drafts [lanes][drafts], a negative one ends a lane's;

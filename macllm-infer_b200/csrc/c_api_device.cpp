@@ -90,7 +90,9 @@ int32_t mk_k_verify_drafts_dev(int32_t type, const void* logits_dev, int64_t log
         need(type == MK_TYPE_F32 || type == MK_TYPE_F16 || type == MK_TYPE_BF16, "mk_k_verify_drafts_dev: logits are f32, f16 or bf16");
         need(lanes >= 0 && drafts >= 0 && vocab > 0 && logits_stride >= vocab, "mk_k_verify_drafts_dev: negative sizes, or rows overlap");
         need((int64_t)lanes * (drafts + 1) <= INT32_MAX / 16, "mk_k_verify_drafts_dev: too many rows");
+        need(vocab <= kVerifyMaxVocab, "mk_k_verify_drafts_dev: a vocabulary has at most 416000 tokens");
         if (lanes == 0) return;
+        need(aligned(logits_dev, type == MK_TYPE_F32 ? 4 : 2), "mk_k_verify_drafts_dev: logits are not aligned to their type");
         need(logits_dev != nullptr && (drafts_dev != nullptr || drafts == 0) && u_dev != nullptr && temperature_dev != nullptr && top_k_dev != nullptr && top_p_dev != nullptr &&
                  tokens_dev != nullptr && accepted_dev != nullptr,
              "mk_k_verify_drafts_dev: null pointer");

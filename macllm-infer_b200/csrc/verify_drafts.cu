@@ -6,17 +6,29 @@
 // p.  The tokens are then distributed as if drawn from the target one by one: q min(1, p / q) + (1 - sum q min(1, p / q)) max(p - q, 0) / sum max(p - q, 0) = p.
 // A draw takes the first token, in the order of tokens, whose cumulative weight exceeds u_n times the whole.
 //
-// Every row is judged by itself, and a second kernel takes a lane's first row that ends it.  Sums and weights of candidates are 64-bit.
+// Every row is judged by itself, by a cluster of eight CTAs that hold it in their shared memory: it is fetched once, with bulk copies, and what needs more than
+// one look at it (maximum, sum, candidates, draw) looks there.  A second kernel takes a lane's first row that ends it.
+//
+// Candidates of a top_k: each of the cluster's 4096 threads has the best of its own tokens, and the k-th best of those is a bound that at least k tokens reach and, since
+// tokens are dealt out evenly, few more do; those are sorted.  Where too many reach it (thousands of equal logits) bisection over (value, token) finds one that
+// fewer do.  Weights and sums of candidates are 64-bit.  Over the whole vocabulary a weight is a 32-bit number (ex2 of a product kept to twice 32 bits: 2^-22, and
+// with no trend, so that sums over many are better), a sum of four is added up in 64 bits.
 #include "verify_drafts.h"
 #include "sampling_math.h"
 #include "shared_attention.h"
+#include "umma.cuh"
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <algorithm>
 
 namespace mk {
 
 namespace {
 
-constexpr int kThreads = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kCtas = 8, kThreads = 512, kWarps = kThreads / 32, kPieces = 4;
+constexpr int kCandidates = 2048;   // sorted at once; at least twice the largest top_k
 
 __device__ __forceinline__ void tell(int32_t* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);
@@ -24,6 +36,28 @@ __device__ __forceinline__ void tell(int32_t* status, int bit) {
 __device__ __forceinline__ float value_of(float x) { return x; }
 __device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void set_low(float* x) { *x = -INFINITY; }
+__device__ __forceinline__ void set_low(__half* x) { *x = __ushort_as_half(0xFC00); }
+__device__ __forceinline__ void set_low(__nv_bfloat16* x) { *x = __ushort_as_bfloat16(0xFF80); }
+// The values of 16 bytes.
+__device__ __forceinline__ void unpack(const uint4& r, float (&v)[4], const float*) {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], const __half*) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], const __nv_bfloat16*) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
 // Larger first, the lower token first among equals; -0 counts as 0.
 __device__ __forceinline__ uint64_t key_of(float x, int i) { return rank_key(x + 0.0f, (uint32_t)i); }
 __device__ __forceinline__ float value_of_key(uint64_t k) {
@@ -31,18 +65,23 @@ __device__ __forceinline__ float value_of_key(uint64_t k) {
     return bits_f32((b & 0x80000000u) ? b & 0x7FFFFFFFu : ~b);
 }
 
-// Inclusive sums over the block's threads; *total: of all.
-__device__ double block_scan(double v, double* red, double* total) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+__device__ __forceinline__ double warp_scan(double v, int lane) {
     for (int o = 1; o < 32; o <<= 1) {
         const double t = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += t;
     }
+    return v;
+}
+// Inclusive sums over the block's threads; *total: of all.
+__device__ double block_scan(double v, double* red, double* total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    v = warp_scan(v, lane);
     __syncthreads();
     if (lane == 31) red[w] = v;
     __syncthreads();
     double before = 0.0, all = 0.0;
-    for (int i = 0; i < nw; ++i) {
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
         if (i < w) before += red[i];
         all += red[i];
     }
@@ -50,194 +89,444 @@ __device__ double block_scan(double v, double* red, double* total) {
     return before + v;
 }
 
-__device__ void sort_desc(uint64_t* a) {
-    for (int size = 2; size <= kThreads; size <<= 1)
+// n, a power of two, keys by the block.
+__device__ void sort_desc(uint64_t* a, int n) {
+    for (int size = 2; size <= n; size <<= 1)
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
             __syncthreads();
-            const int tid = threadIdx.x, partner = tid ^ stride;
-            if (partner > tid) {
-                const uint64_t x = a[tid], y = a[partner];
-                if ((x < y) == ((tid & size) == 0)) a[tid] = y, a[partner] = x;
+            for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+                const int at = (i / stride) * 2 * stride + i % stride;
+                const uint64_t x = a[at], y = a[at + stride];
+                if ((x < y) == ((at & size) == 0)) a[at] = y, a[at + stride] = x;
             }
         }
     __syncthreads();
 }
+__device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+
+// exp((x - top) / temperature) with 1 / (temperature ln 2) as the sum of two 32-bit numbers.
+struct Exponential {
+    float top, hi, lo;
+    __device__ __forceinline__ float operator()(float x) const {
+        const float y = x - top, t = y * hi, rest = fmaf(y, lo, fmaf(y, hi, -t));
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+        return t > -126.f ? fmaf(e, rest * 0.69314718f, e) : 0.f;   // -inf among what is not
+    }
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const __grid_constant__ VerifyArgs a) {
-    __shared__ uint64_t keys[kThreads];
-    __shared__ double weight[kThreads], red[32];
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t s_prefix, s_need, s_count;
-    __shared__ int s_pick, s_last;
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify_rows_kernel(const __grid_constant__ VerifyArgs a, int chunk) {
+    constexpr int EPV = 16 / (int)sizeof(T);   // values of 16 bytes
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint64_t bars[kPieces], best_of[kCtas], warp_best[kWarps];
+    __shared__ double sum_of[3][kCtas], red[kWarps], region[kWarps];
+    __shared__ int bad_of[kCtas], count_of[2][kCtas], warp_count[kWarps];
+    __shared__ uint32_t thread_best[kThreads], warp_low[kWarps];
+    __shared__ int s_count, s_pick, s_last, s_span;
     __shared__ double s_pd;
-    const int tid = threadIdx.x, lane = blockIdx.x / (a.n_drafts + 1), i = blockIdx.x - lane * (a.n_drafts + 1), vocab = a.vocab;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), index = blockIdx.x / kCtas;
+    const int lane = index / (a.n_drafts + 1), i = index - lane * (a.n_drafts + 1), vocab = a.vocab;
+    pdl_trigger();
     const int32_t* drafts = a.drafts + (int64_t)lane * a.n_drafts;
-    for (int j = 0; j < i; ++j)
-        if (drafts[j] < 0 || drafts[j] >= vocab) return;   // nothing gets here
+    bool gone = false;
+    for (int j = wl; j < i; j += 32) gone |= drafts[j] < 0 || drafts[j] >= vocab;
+    if (__any_sync(0xffffffffu, gone)) return;   // nothing gets here
     int d = i < a.n_drafts ? drafts[i] : -1;
     if (d >= vocab) {
         if (tid == 0) tell(a.status, kDevBadRange);
         d = -1;
     }
-    const T* x = static_cast<const T*>(a.logits) + blockIdx.x * a.ld;
+    const T* x = static_cast<const T*>(a.logits) + index * a.ld;
+    int2* out = a.rows + index;
     const float temperature = a.temperature[lane];
-    int2* out = a.rows + blockIdx.x;
 
+    // ---- this CTA's run of tokens, in 16-byte pieces of its row; places of the first and last piece that are not its hold -inf
+    const int n0 = min(vocab, rank * chunk), n = min(chunk, vocab - n0);
+    const uintptr_t src = reinterpret_cast<uintptr_t>(x + n0);
+    const int shift = (int)(src & 15), bytes = n * (int)sizeof(T), vecs = n > 0 ? (shift + bytes + 15) / 16 : 0;
+    const int v_lo = shift > 0 ? 1 : 0, v_hi = max(v_lo, (shift + bytes) / 16), per_piece = (v_hi - v_lo + kPieces - 1) / kPieces;
+    const int token0 = n0 - shift / (int)sizeof(T);   // of the first place
+    uint4* buf = reinterpret_cast<uint4*>(smem);
+    uint16_t* list = reinterpret_cast<uint16_t*>(smem + a.list_at);
+    if (tid == 0) {
+        for (int p = 0; p < kPieces; ++p) umma::bar_init(&bars[p], 1);
+        umma::bar_init_fence();
+        s_count = 0;
+        s_pick = INT_MAX;
+        s_last = -1;
+        s_span = 0;
+        s_pd = 0.0;
+    }
+    __syncthreads();
+    if (tid == 0)
+        for (int p = 0; p < kPieces; ++p) {
+            const int lo = v_lo + p * per_piece, hi = min(v_hi, lo + per_piece);
+            if (hi <= lo) continue;
+            umma::bar_expect_tx(&bars[p], (uint32_t)(hi - lo) * 16);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(umma::smem_u32(buf + lo)), "l"(src - shift + (uintptr_t)lo * 16),
+                         "r"((uint32_t)(hi - lo) * 16), "r"(umma::smem_u32(&bars[p]))
+                         : "memory");
+        }
+    auto edge = [&](int v) {
+        for (int j = tid; j < EPV; j += kThreads) {
+            const int t = token0 + v * EPV + j;
+            T* to = reinterpret_cast<T*>(buf + v) + j;
+            if (t >= n0 && t < n0 + n) *to = x[t];
+            else set_low(to);
+        }
+    };
+    if (vecs > 0 && v_lo == 1) edge(0);
+    if (vecs > v_hi && (v_hi > 0 || v_lo == 0)) edge(v_hi);
+    __syncthreads();
+
+    float mine = -INFINITY;
+    bool bad = false, ok = true;
     uint64_t best = 0;
-    bool bad = false;
-    for (int j = tid; j < vocab; j += kThreads) {
-        const float v = value_of(x[j]);
-        bad |= !(v < INFINITY);
-        const uint64_t k = key_of(v, j);
-        best = k > best ? k : best;
+    auto look = [&](int v) {
+        float f[EPV];
+        unpack(buf[v], f, static_cast<const T*>(nullptr));
+        float m = f[0];
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) {
+            bad |= !(f[j] < INFINITY);
+            m = fmaxf(m, f[j]);
+        }
+        if (m > mine || best == 0) {
+            mine = m;
+#pragma unroll
+            for (int j = EPV - 1; j >= 0; --j)
+                if (f[j] == m) best = key_of(m, token0 + v * EPV + j);
+        }
+    };
+    if (tid == 0 && vecs > 0 && v_lo == 1) look(0);
+    for (int p = 0; p < kPieces; ++p) {
+        const int lo = v_lo + p * per_piece, hi = min(v_hi, lo + per_piece);
+        if (hi <= lo) continue;
+        ok = umma::bar_wait(&bars[p], 0) && ok;
+        for (int v = lo + tid; v < hi; v += kThreads) look(v);
     }
-    bad = __syncthreads_or(bad);
-    keys[tid] = best;
-    __syncthreads();
-    for (int s = kThreads / 2; s > 0; s >>= 1) {
-        if (tid < s && keys[tid + s] > keys[tid]) keys[tid] = keys[tid + s];
-        __syncthreads();
+    if (tid == kThreads - 1 && vecs > v_hi && (v_hi > 0 || v_lo == 0)) look(v_hi);
+    if (best == 0) best = key_of(-INFINITY, vocab);
+    thread_best[tid] = (uint32_t)(best >> 32);
+    if (!ok) tell(a.status, kDevWait);
+    bad = __syncthreads_or(bad || !ok);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+        best = other > best ? other : best;
     }
-    best = keys[0];
+    if (wl == 0) warp_best[warp] = best;
     __syncthreads();
+    if (tid < kCtas) {
+        for (int w = 0; w < kWarps; ++w) best = warp_best[w] > best ? warp_best[w] : best;
+        *cluster.map_shared_rank(&best_of[rank], tid) = best;
+        *cluster.map_shared_rank(&bad_of[rank], tid) = bad;
+    }
+    cluster.sync();
+    best = best_of[0];
+    bad = bad_of[0];
+#pragma unroll
+    for (int c = 1; c < kCtas; ++c) {
+        best = best_of[c] > best ? best_of[c] : best;
+        bad |= bad_of[c] != 0;
+    }
     const float top = value_of_key(best);
     if (bad || top == -INFINITY) {
-        if (tid == 0) {
+        if (rank == 0 && tid == 0) {
             tell(a.status, kDevBadRow);
             *out = make_int2(0, -1);
         }
         return;
     }
     if (!(temperature > 0.f)) {
-        if (tid == 0) *out = make_int2(d == (int)rank_key_index(best), (int)rank_key_index(best));
+        if (rank == 0 && tid == 0) *out = make_int2(d == (int)rank_key_index(best), (int)rank_key_index(best));
         return;
     }
     int k = a.top_k[lane];
-    float top_p = a.top_p[lane];
+    const float top_p = a.top_p[lane];
     if (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f)) {
-        if (tid == 0) tell(a.status, kDevBadRange);
+        if (rank == 0 && tid == 0) tell(a.status, kDevBadRange);
         k = min(k, kVerifyMaxTopK);
     }
     k = min(k, vocab);
     const double per_t = 1.0 / (double)temperature;
     const float* q = a.draft_probs == nullptr || d < 0 ? nullptr : a.draft_probs + ((int64_t)lane * a.n_drafts + i) * vocab;
-    const double u_keep = d >= 0 ? (double)a.u[(int64_t)lane * (a.n_drafts + 1) + i] : 0.0, u_draw = (double)a.u[(int64_t)lane * (a.n_drafts + 1) + a.n_drafts];
-    const double qd = q != nullptr ? (double)q[d] : 1.0;
-    if (tid == 0) s_pick = INT_MAX, s_last = -1, s_pd = 0.0;
-    __syncthreads();
-    auto q_at = [&](int t) { return d < 0 ? 0.0 : (q != nullptr ? (double)q[t] : (t == d ? 1.0 : 0.0)); };
+    const float* u = a.u + (int64_t)lane * (a.n_drafts + 1);
+    const double u_draw = (double)u[a.n_drafts], kept_below = d >= 0 ? (double)u[i] * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
 
     if (k <= 0) {
-        // the whole vocabulary, a run of tokens per thread
-        const int per = (vocab + kThreads - 1) / kThreads, lo = min(vocab, tid * per), hi = min(vocab, lo + per);
-        auto weight_of = [&](int t) { return exp(((double)value_of(x[t]) - (double)top) * per_t); };
-        double mine = 0.0, z, total;
-        for (int t = lo; t < hi; ++t) mine += weight_of(t);
-        block_scan(mine, red, &z);
-        const double pd = d >= 0 ? weight_of(d) / z : 0.0;
-        if (d >= 0 && u_keep * qd < pd) {
-            if (tid == 0) *out = make_int2(1, -1);
+        // ---- the whole vocabulary
+        const double unit = per_t * 1.4426950408889634074;
+        Exponential weight;
+        weight.top = top;
+        weight.hi = (float)unit;
+        weight.lo = (float)(unit - (double)weight.hi);
+        auto block_sum_to = [&](double v, double* slot) {   // of this CTA, to the whole cluster
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            if (wl == 0) region[warp] = v;
+            __syncthreads();
+            if (tid < kCtas) {
+                double s = 0.0;
+                for (int w = 0; w < kWarps; ++w) s += region[w];
+                *cluster.map_shared_rank(slot + rank, tid) = s;
+            }
+            cluster.sync();
+        };
+        double part = 0.0;
+        for (int v = tid; v < vecs; v += kThreads) {
+            float f[EPV], s[EPV / 4];
+            unpack(buf[v], f, static_cast<const T*>(nullptr));
+#pragma unroll
+            for (int j = 0; j < EPV; j += 4) s[j / 4] = (weight(f[j]) + weight(f[j + 1])) + (weight(f[j + 2]) + weight(f[j + 3]));
+#pragma unroll
+            for (int j = 0; j < EPV / 4; ++j) part += (double)s[j];
+        }
+        block_sum_to(part, sum_of[0]);
+        double z = 0.0;
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) z += sum_of[0][c];
+        if (d >= 0 && kept_below < exp(((double)value_of(x[d]) - (double)top) * per_t) / z) {
+            if (rank == 0 && tid == 0) *out = make_int2(1, -1);
             return;
         }
+        const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
+        // The draw: every warp adds up a run of its own, one of them walks through the run where the target lies.
+        const int run = (vecs + kWarps - 1) / kWarps, r_lo = min(vecs, warp * run), r_hi = min(vecs, r_lo + run);
         bool rest = d >= 0;
-        auto share_of = [&](int t) {
-            const double p = weight_of(t) / z;
-            return rest ? fmax(p - q_at(t), 0.0) : p;
+        auto shares_of = [&](int v, float (&r)[EPV]) {
+            unpack(buf[v], r, static_cast<const T*>(nullptr));
+            const int t0 = token0 + v * EPV;
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) {
+                const float w = weight(r[j]);
+                if (rest) {
+                    const float qt = q != nullptr ? (t0 + j >= n0 && t0 + j < n0 + n ? q[t0 + j] : 0.f) : (t0 + j == d ? 1.f : 0.f);
+                    r[j] = fmaxf(fmaf(w, per_z, -qt) + w * per_z_rest, 0.f);
+                } else {
+                    r[j] = w;
+                }
+            }
         };
-        mine = 0.0;
-        for (int t = lo; t < hi; ++t) mine += share_of(t);
-        double upto = block_scan(mine, red, &total);
-        if (!(total > 0.0)) {   // the draft's distribution covers the target's
-            rest = false;
-            mine = 0.0;
-            for (int t = lo; t < hi; ++t) mine += share_of(t);
-            upto = block_scan(mine, red, &total);
+        double total = 0.0, *sums = sum_of[1];
+        for (;;) {
+            part = 0.0;
+            for (int v = r_lo + wl; v < r_hi; v += 32) {
+                float r[EPV];
+                shares_of(v, r);
+#pragma unroll
+                for (int j = 0; j < EPV; j += 4) part += (double)((r[j] + r[j + 1]) + (r[j + 2] + r[j + 3]));
+            }
+            block_sum_to(part, sums);
+            total = 0.0;
+#pragma unroll
+            for (int c = 0; c < kCtas; ++c) total += sums[c];
+            if (total > 0.0 || !rest) break;
+            rest = false;   // the draft's distribution covers the target's
+            sums = sum_of[2];
         }
         const double target = u_draw * total;
-        double c = upto - mine;
-        int last = -1;
-        for (int t = lo; t < hi; ++t) {
-            const double r = share_of(t);
-            c += r;
-            if (r > 0.0) last = t;
-            if (r > 0.0 && c > target) {
-                atomicMin(&s_pick, t);
-                break;
+        double before = 0.0;
+        int at = -1;
+        for (int c = 0; c < kCtas; ++c) {
+            if (sums[c] > 0.0) at = c;
+            if (before + sums[c] > target) break;
+            before += sums[c];
+        }
+        if (at != rank) return;
+        if (!(before + sums[at] > target)) before -= sums[at];   // rounding left none: the last with a share
+        int w_at = -1;
+        double w_before = before;
+        for (int w = 0; w < kWarps; ++w) {
+            if (region[w] > 0.0) w_at = w;
+            if (w_before + region[w] > target) break;
+            w_before += region[w];
+        }
+        if (w_at != warp) return;
+        if (!(w_before + region[w_at] > target)) w_before -= region[w_at];
+        int last = -1, pick = -1;
+        for (int v0 = r_lo; v0 < r_hi && pick < 0; v0 += 32) {
+            float r[EPV];
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) r[j] = 0.f;
+            if (v0 + wl < r_hi) shares_of(v0 + wl, r);
+            double s = 0.0;
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) {
+                s += (double)r[j];
+                if (r[j] > 0.f) last = token0 + (v0 + wl) * EPV + j;
+            }
+            double c = w_before + warp_scan(s, wl);
+            const unsigned over = __ballot_sync(0xffffffffu, s > 0.0 && c > target);
+            w_before = __shfl_sync(0xffffffffu, c, 31);
+            if (over != 0) {
+                const int first = __ffs(over) - 1;
+                if (wl == first) {
+                    c -= s;
+#pragma unroll
+                    for (int j = 0; j < EPV; ++j) {
+                        c += (double)r[j];
+                        if (pick < 0 && r[j] > 0.f && (c > target)) pick = token0 + (v0 + wl) * EPV + j;
+                    }
+                    if (pick < 0) pick = last;
+                }
+                pick = __shfl_sync(0xffffffffu, pick, first);
             }
         }
-        atomicMax(&s_last, last);
-        __syncthreads();
-        if (tid == 0) *out = make_int2(0, s_pick < INT_MAX ? s_pick : s_last);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (wl == 0) *out = make_int2(0, pick >= 0 ? pick : last);
         return;
     }
-    // the value of the k-th best token, eight bits at a time
-    uint32_t prefix = 0, mask = 0, need = (uint32_t)k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+
+    // ---- the k best
+    uint32_t others[kCtas];
+#pragma unroll
+    for (int c = 0; c < kCtas; ++c) others[c] = *cluster.map_shared_rank(&thread_best[tid], c);
+    auto block_count = [&](int v) {
+        v = __reduce_add_sync(0xffffffffu, v);
         __syncthreads();
-        for (int j = tid; j < vocab; j += kThreads) {
-            const uint32_t key = (uint32_t)(key_of(value_of(x[j]), j) >> 32);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+        if (wl == 0) warp_count[warp] = v;
+        __syncthreads();
+        int s = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s += warp_count[w];
+        return s;
+    };
+    uint32_t low = others[0];
+#pragma unroll
+    for (int c = 1; c < kCtas; ++c) low = min(low, others[c]);
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (wl == 0) warp_low[warp] = low;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) low = min(low, warp_low[w]);
+    uint32_t high = (uint32_t)(best >> 32);
+    // low: at least k threads' best reach it (at first: all)
+    for (int step = 0; step < 16 && high - low > 0; ++step) {
+        const uint32_t mid = low + (high - low) / 2 + 1;
+        int c = 0;
+#pragma unroll
+        for (int o = 0; o < kCtas; ++o) c += others[o] >= mid;
+        if (block_count(c) >= k) low = mid;
+        else high = mid - 1;
+    }
+    // tokens that reach a bound, listed by their places; at least k reach `enough`, fewer reach `few`
+    uint64_t enough = (uint64_t)low << 32, few = best + 1, bound = enough;
+    int n_all, turn = 0;
+    for (;; ++turn) {
+        const uint32_t bound_value = (uint32_t)(bound >> 32);
+        for (int v = tid; v < vecs; v += kThreads) {
+            float f[EPV];
+            unpack(buf[v], f, static_cast<const T*>(nullptr));
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) {
+                if (f32_order_key(f[j] + 0.0f) < bound_value) continue;
+                const int t = token0 + v * EPV + j;
+                if (key_of(f[j], t) < bound || t < n0 || t >= n0 + n) continue;
+                const int at = atomicAdd(&s_count, 1);
+                if (at < kCandidates) list[at] = (uint16_t)(v * EPV + j);
+            }
         }
         __syncthreads();
-        if (tid == 0) {
-            uint32_t acc = 0;
-            int b = 255;
-            for (; b > 0 && acc + hist[b] < need; --b) acc += hist[b];
-            s_prefix = prefix | (uint32_t)b << shift;
-            s_need = need - acc;
+        if (tid < kCtas) *cluster.map_shared_rank(&count_of[turn & 1][rank], tid) = s_count;
+        cluster.sync();
+        n_all = 0;
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) n_all += count_of[turn & 1][c];
+        if (n_all >= k && n_all <= kCandidates) break;
+        if (n_all >= k) enough = bound;
+        else few = bound;
+        bound = enough + (few - enough) / 2;   // keys differ, and kCandidates > k: it ends
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+    }
+    static_assert(kCandidates > kVerifyMaxTopK && kCandidates % kThreads == 0, "more can be sorted than are wanted");
+    // they meet where the first CTA had its tokens
+    const int mine_n = count_of[turn & 1][rank];
+    int first = 0;
+    for (int c = 0; c < rank; ++c) first += count_of[turn & 1][c];
+    uint64_t found[kCandidates / kThreads];
+#pragma unroll
+    for (int c = 0; c < kCandidates / kThreads; ++c)
+        if (tid + c * kThreads < mine_n) {
+            const int at = list[tid + c * kThreads];
+            found[c] = key_of(value_of(reinterpret_cast<const T*>(smem)[at]), token0 + at);
         }
-        __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
-        mask |= 255u << shift;
-        __syncthreads();
+    cluster.sync();
+    uint64_t* keys = reinterpret_cast<uint64_t*>(smem);
+    uint64_t* there = cluster.map_shared_rank(keys, 0);
+#pragma unroll
+    for (int c = 0; c < kCandidates / kThreads; ++c)
+        if (tid + c * kThreads < mine_n) there[first + tid + c * kThreads] = found[c];
+    cluster.sync();
+    if (rank != 0) return;
+    int size = power_of_two(n_all);
+    for (int j = n_all + tid; j < size; j += kThreads) keys[j] = 0;
+    sort_desc(keys, size);
+    // two candidates a thread: the head that adds up to top_p
+    double* weights = reinterpret_cast<double*>(keys + kVerifyMaxTopK);
+    const int j0 = 2 * tid;
+    int token[2];
+    double e[2], z, kept;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        token[j] = j0 + j < k ? (int)rank_key_index(keys[j0 + j]) : -1;
+        e[j] = j0 + j < k ? exp(((double)value_of_key(keys[j0 + j]) - (double)top) * per_t) : 0.0;
     }
-    if (tid == 0) s_count = 0;
-    keys[tid] = 0;
+    const double upto_e = block_scan(e[0] + e[1], red, &z);
+    bool in[2] = {j0 < k, j0 + 1 < k};
+    if (top_p < 1.f) {
+        in[0] = in[0] && (j0 == 0 || (upto_e - e[1] - e[0]) / z < (double)top_p);
+        in[1] = in[1] && (upto_e - e[1]) / z < (double)top_p;
+    }
+    // behind the last that is kept (a scan's sums may be out of order by a rounding)
+    if (in[0] || in[1]) atomicMax(&s_span, in[1] ? j0 + 2 : j0 + 1);
+    block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), red, &kept);
+    const int n_kept = block_count((int)in[0] + (int)in[1]);
+    size = power_of_two(s_span);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {   // in the order of tokens from here on
+        if (in[j] && token[j] == d) s_pd = e[j] / kept;
+        if (j0 + j < kVerifyMaxTopK) weights[j0 + j] = e[j] / kept;
+        if (j0 + j < size) keys[j0 + j] = in[j] ? (uint64_t)(0xFFFFFFFFu - (uint32_t)token[j]) << 32 | (uint32_t)(j0 + j) : 0;
+    }
     __syncthreads();
-    const int per = (vocab + kThreads - 1) / kThreads, lo = min(vocab, tid * per), hi = min(vocab, lo + per);
-    int equals = 0;
-    for (int j = lo; j < hi; ++j) {
-        const uint64_t key = key_of(value_of(x[j]), j);
-        if ((uint32_t)(key >> 32) > prefix) keys[atomicAdd(&s_count, 1u)] = key;
-        else if ((uint32_t)(key >> 32) == prefix) ++equals;
-    }
-    double all;
-    int rank = (int)block_scan((double)equals, red, &all) - equals;
-    for (int j = lo; j < hi && equals > 0 && rank < (int)need; ++j) {
-        const uint64_t key = key_of(value_of(x[j]), j);
-        if ((uint32_t)(key >> 32) == prefix) keys[k - (int)need + rank++] = key;
-    }
-    sort_desc(keys);
-    // the head that adds up to top_p
-    double e = tid < k ? exp(((double)value_of_key(keys[tid]) - (double)top) * per_t) : 0.0, z, kept;
-    const double upto_e = block_scan(e, red, &z);
-    if (tid > 0 && !((upto_e - e) / z < (double)top_p) && top_p < 1.f) e = 0.0;
-    block_scan(e, red, &kept);
-    const int token = tid < k ? (int)rank_key_index(keys[tid]) : -1;
-    if (tid < k && token == d) s_pd = e / kept;
-    weight[tid] = e / kept;
-    __syncthreads();
-    if (d >= 0 && u_keep * qd < s_pd) {
+    if (d >= 0 && kept_below < s_pd) {
         if (tid == 0) *out = make_int2(1, -1);
         return;
     }
-    // the draw, in the order of tokens
-    keys[tid] = tid < k ? (uint64_t)(0xFFFFFFFFu - (uint32_t)token) << 32 | (uint32_t)tid : 0;
-    sort_desc(keys);
-    const int t = tid < k ? (int)(0xFFFFFFFFu - (uint32_t)(keys[tid] >> 32)) : -1;
-    const double p = tid < k ? weight[(uint32_t)keys[tid]] : 0.0;
-    double r = d >= 0 && p > 0.0 ? fmax(p - q_at(t), 0.0) : p, total;
-    double upto = block_scan(r, red, &total);
-    if (!(total > 0.0)) {
-        r = p;
-        upto = block_scan(r, red, &total);
+    sort_desc(keys, size);
+    double p[2], r[2], total;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        token[j] = -1;
+        p[j] = r[j] = 0.0;
+        if (j0 + j < n_kept) {
+            const uint64_t key = keys[j0 + j];
+            token[j] = (int)(0xFFFFFFFFu - (uint32_t)(key >> 32));
+            p[j] = r[j] = weights[(uint32_t)key];
+            if (d >= 0) r[j] = fmax(p[j] - (q != nullptr ? (double)q[token[j]] : (token[j] == d ? 1.0 : 0.0)), 0.0);
+        }
     }
-    if (r > 0.0) {
-        if (upto > u_draw * total) atomicMin(&s_pick, t);
-        atomicMax(&s_last, t);
+    double upto = block_scan(r[0] + r[1], red, &total);
+    if (!(total > 0.0)) {   // the draft's distribution covers the target's
+        r[0] = p[0];
+        r[1] = p[1];
+        upto = block_scan(r[0] + r[1], red, &total);
+    }
+    const double target = u_draw * total;
+    if (r[0] > 0.0) {
+        if (upto - r[1] > target) atomicMin(&s_pick, token[0]);
+        atomicMax(&s_last, token[0]);
+    }
+    if (r[1] > 0.0) {
+        if (upto > target) atomicMin(&s_pick, token[1]);
+        atomicMax(&s_last, token[1]);
     }
     __syncthreads();
     if (tid == 0) *out = make_int2(0, s_pick < INT_MAX ? s_pick : s_last);
@@ -245,6 +534,7 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const __grid_cons
 
 __global__ void __launch_bounds__(128) verify_lanes_kernel(const __grid_constant__ VerifyArgs a) {
     const int lane = blockIdx.x * 4 + (threadIdx.x >> 5), t = threadIdx.x & 31, n = a.n_drafts;
+    pdl_wait();
     if (lane >= a.lanes) return;
     const int32_t* drafts = a.drafts + (int64_t)lane * n;
     const int2* rows = a.rows + (int64_t)lane * (n + 1);
@@ -258,13 +548,16 @@ __global__ void __launch_bounds__(128) verify_lanes_kernel(const __grid_constant
 
 }  // namespace
 
-void launch_verify_drafts(const VerifyArgs& a, cudaStream_t s) {
+void launch_verify_drafts(VerifyArgs a, cudaStream_t s) {
     if (a.lanes <= 0) return;
+    const int size = a.type == 0 ? 4 : 2, chunk = ((a.vocab + kCtas - 1) / kCtas + 7) / 8 * 8;
+    a.list_at = std::max(chunk * size + 32, kCandidates * 8);
+    const size_t smem = (size_t)a.list_at + kCandidates * 2;
     auto* kernel = a.type == 0 ? verify_rows_kernel<float> : (a.type == 1 ? verify_rows_kernel<__half> : verify_rows_kernel<__nv_bfloat16>);
-    kernel<<<(unsigned)(a.lanes * (a.n_drafts + 1)), kThreads, 0, s>>>(a);
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    kernel<<<(unsigned)(a.lanes * (a.n_drafts + 1) * kCtas), kThreads, smem, s>>>(a, chunk);
     MK_LAUNCH_CHECK();
-    verify_lanes_kernel<<<(unsigned)((a.lanes + 3) / 4), 128, 0, s>>>(a);
-    MK_LAUNCH_CHECK();
+    launch_pdl(verify_lanes_kernel, dim3((unsigned)((a.lanes + 3) / 4)), dim3(128), 0, s, a);
 }
 
 }  // namespace mk

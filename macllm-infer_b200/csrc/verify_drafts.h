@@ -6,6 +6,7 @@ namespace mk {
 
 constexpr int kDevBadRow = 8;     // a row of logits without a distribution (NaN, +inf or nothing above -inf); bits 1 to 4 in shared_attention.h
 constexpr int kVerifyMaxTopK = 1024;
+constexpr int kVerifyMaxVocab = 8 * 52000;   // eight CTAs' shared memory at 32 bits a value
 
 struct VerifyArgs {
     const void* logits = nullptr;      // [lanes][drafts + 1] rows of vocab values, ld values apart
@@ -22,8 +23,9 @@ struct VerifyArgs {
     int32_t* accepted = nullptr;       // [lanes]
     int2* rows = nullptr;              // scratch [lanes][n_drafts + 1]: (draft accepted, token drawn in its place)
     int32_t* status = nullptr;
+    int list_at = 0;                   // filled in by the launcher: where a CTA's list of candidates begins in its shared memory
 };
 inline int64_t verify_scratch_bytes(int lanes, int n_drafts) { return (int64_t)lanes * (n_drafts + 1) * 8; }
-void launch_verify_drafts(const VerifyArgs& a, cudaStream_t s);
+void launch_verify_drafts(VerifyArgs a, cudaStream_t s);
 
 }  // namespace mk

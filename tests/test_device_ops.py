@@ -96,6 +96,8 @@ VERIFY = dict(type=0, logits=A, stride=1000, lanes=3, drafts=4, vocab=1000, draf
     (dict(stride=999), "rows overlap"),
     (dict(lanes=-1), "negative sizes"),
     (dict(lanes=1 << 26), "too many rows"),
+    (dict(vocab=416001, stride=416001), "at most 416000"),
+    (dict(logits=A + 2), "aligned"),
     (dict(drafts_=None), "null pointer"),
     (dict(u=None), "null pointer"),
     (dict(accepted=None), "null pointer"),
