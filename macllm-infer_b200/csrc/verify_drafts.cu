@@ -89,20 +89,50 @@ __device__ double block_scan(double v, double* red, double* total) {
     return before + v;
 }
 
-// n, a power of two, keys by the block.
-__device__ void sort_desc(uint64_t* a, int n) {
-    for (int size = 2; size <= n; size <<= 1)
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-                const int at = (i / stride) * 2 * stride + i % stride;
-                const uint64_t x = a[at], y = a[at + stride];
-                if ((x < y) == ((at & size) == 0)) a[at] = y, a[at + stride] = x;
+// 512 E keys, the larger first: a thread has E neighbours, so that most exchanges of the bitonic network are inside a thread or a warp.
+template <int E>
+__device__ void sort_desc(uint64_t* keys) {
+    const int tid = threadIdx.x;
+    uint64_t a[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) a[e] = keys[tid * E + e];
+    for (int size = 2; size <= kThreads * E; size <<= 1) {
+        auto exchange = [&](int stride, auto&& partner) {
+            uint64_t y[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = partner(e);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int at = tid * E + e;
+                const bool larger = ((at & stride) == 0) == ((at & size) == 0);
+                a[e] = (y[e] > a[e]) == larger ? y[e] : a[e];
             }
+        };
+        for (int stride = size >> 1; stride >= 32 * E; stride >>= 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e) keys[tid * E + e] = a[e];
+            __syncthreads();
+            exchange(stride, [&](int e) { return keys[(tid * E + e) ^ stride]; });
         }
+        for (int stride = min(size >> 1, 16 * E); stride >= E; stride >>= 1) exchange(stride, [&](int e) { return __shfl_xor_sync(0xffffffffu, a[e], stride / E); });
+#pragma unroll
+        for (int stride = E / 2; stride > 0; stride >>= 1)
+            if (stride < size) exchange(stride, [&](int e) { return a[e ^ stride]; });
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) keys[tid * E + e] = a[e];
     __syncthreads();
 }
-__device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+__device__ void sort_desc(uint64_t* keys, int n) {   // keys behind n are there to be filled up
+    const int size = n <= kThreads ? kThreads : (n <= 2 * kThreads ? 2 * kThreads : 4 * kThreads);
+    for (int j = n + (int)threadIdx.x; j < size; j += kThreads) keys[j] = 0;
+    __syncthreads();
+    if (size == kThreads) sort_desc<1>(keys);
+    else if (size == 2 * kThreads) sort_desc<2>(keys);
+    else sort_desc<4>(keys);
+}
 
 // exp((x - top) / temperature) with 1 / (temperature ln 2) as the sum of two 32-bit numbers.
 struct Exponential {
@@ -121,26 +151,28 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint64_t bars[kPieces], best_of[kCtas], warp_best[kWarps];
     __shared__ double sum_of[3][kCtas], red[kWarps], region[kWarps];
-    __shared__ int bad_of[kCtas], count_of[2][kCtas], warp_count[kWarps];
+    __shared__ int bad_of[kCtas], count_of[2][kCtas];
     __shared__ uint32_t thread_best[kThreads], warp_low[kWarps];
-    __shared__ int s_count, s_pick, s_last, s_span;
+    __shared__ int s_count, s_pick, s_last, hist[256];
+    __shared__ int2 s_step;
     __shared__ double s_pd;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), index = blockIdx.x / kCtas;
     const int lane = index / (a.n_drafts + 1), i = index - lane * (a.n_drafts + 1), vocab = a.vocab;
     pdl_trigger();
     const int32_t* drafts = a.drafts + (int64_t)lane * a.n_drafts;
+    const float* u = a.u + (int64_t)lane * (a.n_drafts + 1);
+    const float temperature = a.temperature[lane], top_p = a.top_p[lane], u_last = u[a.n_drafts], u_mine = u[i];
+    int k = a.top_k[lane], d = i < a.n_drafts ? drafts[i] : -1;
     bool gone = false;
     for (int j = wl; j < i; j += 32) gone |= drafts[j] < 0 || drafts[j] >= vocab;
     if (__any_sync(0xffffffffu, gone)) return;   // nothing gets here
-    int d = i < a.n_drafts ? drafts[i] : -1;
     if (d >= vocab) {
         if (tid == 0) tell(a.status, kDevBadRange);
         d = -1;
     }
     const T* x = static_cast<const T*>(a.logits) + index * a.ld;
     int2* out = a.rows + index;
-    const float temperature = a.temperature[lane];
 
     // ---- this CTA's run of tokens, in 16-byte pieces of its row; places of the first and last piece that are not its hold -inf
     const int n0 = min(vocab, rank * chunk), n = min(chunk, vocab - n0);
@@ -156,7 +188,6 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         s_count = 0;
         s_pick = INT_MAX;
         s_last = -1;
-        s_span = 0;
         s_pd = 0.0;
     }
     __syncthreads();
@@ -219,10 +250,17 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
     }
     if (wl == 0) warp_best[warp] = best;
     __syncthreads();
-    if (tid < kCtas) {
-        for (int w = 0; w < kWarps; ++w) best = warp_best[w] > best ? warp_best[w] : best;
-        *cluster.map_shared_rank(&best_of[rank], tid) = best;
-        *cluster.map_shared_rank(&bad_of[rank], tid) = bad;
+    if (warp == 0) {
+        best = warp_best[wl % kWarps];
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) {
+            const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+            best = other > best ? other : best;
+        }
+        if (wl < kCtas) {
+            *cluster.map_shared_rank(&best_of[rank], wl) = best;
+            *cluster.map_shared_rank(&bad_of[rank], wl) = bad;
+        }
     }
     cluster.sync();
     best = best_of[0];
@@ -244,8 +282,6 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         if (rank == 0 && tid == 0) *out = make_int2(d == (int)rank_key_index(best), (int)rank_key_index(best));
         return;
     }
-    int k = a.top_k[lane];
-    const float top_p = a.top_p[lane];
     if (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f)) {
         if (rank == 0 && tid == 0) tell(a.status, kDevBadRange);
         k = min(k, kVerifyMaxTopK);
@@ -253,8 +289,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
     k = min(k, vocab);
     const double per_t = 1.0 / (double)temperature;
     const float* q = a.draft_probs == nullptr || d < 0 ? nullptr : a.draft_probs + ((int64_t)lane * a.n_drafts + i) * vocab;
-    const float* u = a.u + (int64_t)lane * (a.n_drafts + 1);
-    const double u_draw = (double)u[a.n_drafts], kept_below = d >= 0 ? (double)u[i] * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
+    const double u_draw = (double)u_last, kept_below = d >= 0 ? (double)u_mine * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
 
     if (k <= 0) {
         // ---- the whole vocabulary
@@ -271,10 +306,11 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
             v += __shfl_xor_sync(0xffffffffu, v, 1);
             if (wl == 0) region[warp] = v;
             __syncthreads();
-            if (tid < kCtas) {
-                double s = 0.0;
-                for (int w = 0; w < kWarps; ++w) s += region[w];
-                *cluster.map_shared_rank(slot + rank, tid) = s;
+            if (warp == 0) {
+                double s = region[wl % kWarps];
+#pragma unroll
+                for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (wl < kCtas) *cluster.map_shared_rank(slot + rank, wl) = s;
             }
             cluster.sync();
         };
@@ -299,28 +335,37 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         // The draw: every warp adds up a run of its own, one of them walks through the run where the target lies.
         const int run = (vecs + kWarps - 1) / kWarps, r_lo = min(vecs, warp * run), r_hi = min(vecs, r_lo + run);
         bool rest = d >= 0;
-        auto shares_of = [&](int v, float (&r)[EPV]) {
-            unpack(buf[v], r, static_cast<const T*>(nullptr));
+        auto load_q = [&](int v, float (&r)[EPV]) {   // what the draft's distribution has there, 0 where the row ends
             const int t0 = token0 + v * EPV;
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) r[j] = q != nullptr ? (t0 + j >= n0 && t0 + j < n0 + n && v < vecs ? q[t0 + j] : 0.f) : (t0 + j == d ? 1.f : 0.f);
+        };
+        auto shares_of = [&](int v, const float (&qv)[EPV], float (&r)[EPV]) {
+            unpack(buf[v], r, static_cast<const T*>(nullptr));
 #pragma unroll
             for (int j = 0; j < EPV; ++j) {
                 const float w = weight(r[j]);
-                if (rest) {
-                    const float qt = q != nullptr ? (t0 + j >= n0 && t0 + j < n0 + n ? q[t0 + j] : 0.f) : (t0 + j == d ? 1.f : 0.f);
-                    r[j] = fmaxf(fmaf(w, per_z, -qt) + w * per_z_rest, 0.f);
-                } else {
-                    r[j] = w;
-                }
+                r[j] = rest ? fmaxf(fmaf(w, per_z, -qv[j]) + w * per_z_rest, 0.f) : w;
             }
         };
         double total = 0.0, *sums = sum_of[1];
         for (;;) {
             part = 0.0;
-            for (int v = r_lo + wl; v < r_hi; v += 32) {
-                float r[EPV];
-                shares_of(v, r);
+            constexpr int AHEAD = 16 / EPV;   // the draft's values of several pieces are on their way together
+            for (int v0 = r_lo + wl; v0 < r_hi; v0 += 32 * AHEAD) {
+                float qv[AHEAD][EPV];
+                if (rest) {
 #pragma unroll
-                for (int j = 0; j < EPV; j += 4) part += (double)((r[j] + r[j + 1]) + (r[j + 2] + r[j + 3]));
+                    for (int c = 0; c < AHEAD; ++c) load_q(v0 + 32 * c, qv[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < AHEAD; ++c) {
+                    if (v0 + 32 * c >= r_hi) break;
+                    float r[EPV];
+                    shares_of(v0 + 32 * c, qv[c], r);
+#pragma unroll
+                    for (int j = 0; j < EPV; j += 4) part += (double)((r[j] + r[j + 1]) + (r[j + 2] + r[j + 3]));
+                }
             }
             block_sum_to(part, sums);
             total = 0.0;
@@ -333,53 +378,55 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         const double target = u_draw * total;
         double before = 0.0;
         int at = -1;
+#pragma unroll
         for (int c = 0; c < kCtas; ++c) {
-            if (sums[c] > 0.0) at = c;
-            if (before + sums[c] > target) break;
-            before += sums[c];
+            if (sums[c] > 0.0 && !(at >= 0 && before > target)) at = c;
+            if (!(before > target)) before += sums[c];
         }
         if (at != rank) return;
-        if (!(before + sums[at] > target)) before -= sums[at];   // rounding left none: the last with a share
+        // at: the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
+        before = 0.0;
+        for (int c = 0; c < rank; ++c) before += sums[c];
         int w_at = -1;
-        double w_before = before;
+        double w_before = before, upto_run = before;
         for (int w = 0; w < kWarps; ++w) {
-            if (region[w] > 0.0) w_at = w;
-            if (w_before + region[w] > target) break;
-            w_before += region[w];
-        }
-        if (w_at != warp) return;
-        if (!(w_before + region[w_at] > target)) w_before -= region[w_at];
-        int last = -1, pick = -1;
-        for (int v0 = r_lo; v0 < r_hi && pick < 0; v0 += 32) {
-            float r[EPV];
-#pragma unroll
-            for (int j = 0; j < EPV; ++j) r[j] = 0.f;
-            if (v0 + wl < r_hi) shares_of(v0 + wl, r);
-            double s = 0.0;
-#pragma unroll
-            for (int j = 0; j < EPV; ++j) {
-                s += (double)r[j];
-                if (r[j] > 0.f) last = token0 + (v0 + wl) * EPV + j;
+            if (region[w] > 0.0) {
+                w_at = w;
+                w_before = upto_run;
             }
-            double c = w_before + warp_scan(s, wl);
-            const unsigned over = __ballot_sync(0xffffffffu, s > 0.0 && c > target);
-            w_before = __shfl_sync(0xffffffffu, c, 31);
-            if (over != 0) {
-                const int first = __ffs(over) - 1;
-                if (wl == first) {
-                    c -= s;
+            upto_run += region[w];
+            if (upto_run > target) break;
+        }
+        // the whole CTA looks through that run
+        const int at_lo = min(vecs, w_at * run), at_hi = min(vecs, at_lo + run);
+        for (int v0 = at_lo; v0 < at_hi; v0 += kThreads) {
+            const int v = v0 + tid;
+            float qv[EPV], r[EPV];
+            double s = 0.0, all;
+            if (v < at_hi) {
+                load_q(v, qv);
+                shares_of(v, qv, r);
 #pragma unroll
-                    for (int j = 0; j < EPV; ++j) {
-                        c += (double)r[j];
-                        if (pick < 0 && r[j] > 0.f && (c > target)) pick = token0 + (v0 + wl) * EPV + j;
-                    }
-                    if (pick < 0) pick = last;
+                for (int j = 0; j < EPV; ++j) {
+                    s += (double)r[j];
+                    if (r[j] > 0.f) atomicMax(&s_last, token0 + v * EPV + j);
                 }
-                pick = __shfl_sync(0xffffffffu, pick, first);
             }
+            double c = w_before + block_scan(s, red, &all) - s;
+            if (v < at_hi && s > 0.0 && c + s > target) {
+                int pick = -1;
+#pragma unroll
+                for (int j = 0; j < EPV; ++j) {
+                    c += (double)r[j];
+                    if (r[j] > 0.f && (pick < 0 || !(c - (double)r[j] > target))) pick = token0 + v * EPV + j;
+                }
+                atomicMin(&s_pick, pick);
+            }
+            w_before += all;
+            __syncthreads();
+            if (s_pick < INT_MAX) break;
         }
-        last = __reduce_max_sync(0xffffffffu, last);
-        if (wl == 0) *out = make_int2(0, pick >= 0 ? pick : last);
+        if (tid == 0) *out = make_int2(0, s_pick < INT_MAX ? s_pick : s_last);
         return;
     }
 
@@ -387,16 +434,6 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
     uint32_t others[kCtas];
 #pragma unroll
     for (int c = 0; c < kCtas; ++c) others[c] = *cluster.map_shared_rank(&thread_best[tid], c);
-    auto block_count = [&](int v) {
-        v = __reduce_add_sync(0xffffffffu, v);
-        __syncthreads();
-        if (wl == 0) warp_count[warp] = v;
-        __syncthreads();
-        int s = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += warp_count[w];
-        return s;
-    };
     uint32_t low = others[0];
 #pragma unroll
     for (int c = 1; c < kCtas; ++c) low = min(low, others[c]);
@@ -405,15 +442,46 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) low = min(low, warp_low[w]);
+    // low: at least k threads' best reach it (at first: all); twice, 256 steps between it and the next bound
     uint32_t high = (uint32_t)(best >> 32);
-    // low: at least k threads' best reach it (at first: all)
-    for (int step = 0; step < 16 && high - low > 0; ++step) {
-        const uint32_t mid = low + (high - low) / 2 + 1;
-        int c = 0;
+    int wanted = k;
+    for (int round = 0; round < 2; ++round) {
+        const int bits = max(0, 24 - __clz(high - low));   // the range is less than 256 steps of 2^bits
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
 #pragma unroll
-        for (int o = 0; o < kCtas; ++o) c += others[o] >= mid;
-        if (block_count(c) >= k) low = mid;
-        else high = mid - 1;
+        for (int c = 0; c < kCtas; ++c)
+            if (others[c] >= low && others[c] <= high) atomicAdd(&hist[(others[c] - low) >> bits], 1);
+        __syncthreads();
+        if (warp == 0) {   // a lane has eight steps, the first lane the highest
+            int c[8], sum = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += c[j] = hist[255 - wl * 8 - j];
+            int incl = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, incl, o);
+                if (wl >= o) incl += other;
+            }
+            int over = incl - sum;   // threads above the lane's steps
+            if (over < wanted && incl >= wanted) {
+                int at = 255 - wl * 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (over + c[j] >= wanted) break;
+                    over += c[j];
+                    --at;
+                }
+                s_step = make_int2(at, over);
+            }
+        }
+        __syncthreads();
+        const int2 step = s_step;
+        wanted -= step.y;
+        low += (uint32_t)step.x << bits;
+        high = min(high, low + ((1u << bits) - 1u));
+        if (bits == 0) break;
+        __syncthreads();
     }
     // tokens that reach a bound, listed by their places; at least k reach `enough`, fewer reach `few`
     uint64_t enough = (uint64_t)low << 32, few = best + 1, bound = enough;
@@ -465,53 +533,119 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         if (tid + c * kThreads < mine_n) there[first + tid + c * kThreads] = found[c];
     cluster.sync();
     if (rank != 0) return;
-    int size = power_of_two(n_all);
-    for (int j = n_all + tid; j < size; j += kThreads) keys[j] = 0;
-    sort_desc(keys, size);
-    // two candidates a thread: the head that adds up to top_p
-    double* weights = reinterpret_cast<double*>(keys + kVerifyMaxTopK);
+    const double* shares;   // of the kept candidates in the order of tokens, and those
+    const int* tokens;
+    double* values = reinterpret_cast<double*>(keys + kCandidates);
+    int* ids = reinterpret_cast<int*>(values + kThreads);
+    int n_last;
+    if (n_all <= kThreads) {
+        // A candidate a thread, which counts those before it in either order.
+        const uint64_t key = tid < n_all ? keys[tid] : 0;
+        int rank_by_value = 0, rank_by_token = 0;
+        if (warp * 32 < n_all) {
+            if (tid < 2) keys[n_all + tid] = 0;
+        }
+        __syncthreads();
+        if (warp * 32 < n_all)
+            for (int j = 0; j < n_all; j += 2) {
+                const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(keys + j);
+                rank_by_value += (int)(other.x > key) + (int)(other.y > key);
+                rank_by_token += (int)((uint32_t)other.x > (uint32_t)key) + (int)((uint32_t)other.y > (uint32_t)key);
+            }
+        const bool among = tid < n_all && rank_by_value < k;
+        const double e = among ? exp(((double)value_of_key(key) - (double)top) * per_t) : 0.0;
+        bool in = among;
+        double kept;
+        if (top_p < 1.f) {
+            values[tid] = 0.0;
+            __syncthreads();
+            if (among) values[rank_by_value] = e;
+            __syncthreads();
+            const double mine_e = values[tid];
+            double z;
+            const double upto = block_scan(mine_e, red, &z);
+            values[tid] = upto - mine_e;
+            __syncthreads();
+            in = among && (rank_by_value == 0 || values[rank_by_value] / z < (double)top_p);
+            __syncthreads();
+        }
+        const double e_in = in ? e : 0.0;
+        block_scan(e_in, red, &kept);
+        const int token = (int)rank_key_index(key);
+        if (in && token == d) s_pd = e / kept;
+        values[tid] = 0.0;
+        __syncthreads();
+        if (d >= 0 && kept_below < s_pd) {
+            if (tid == 0) *out = make_int2(1, -1);
+            return;
+        }
+        if (tid < n_all) {
+            values[rank_by_token] = e_in / kept;
+            ids[rank_by_token] = token;
+        }
+        __syncthreads();
+        shares = values;
+        tokens = ids;
+        n_last = n_all;
+    } else {
+        // two candidates a thread: the head that adds up to top_p
+        sort_desc(keys, n_all);
+        const int j0 = 2 * tid;
+        int token[2];
+        double e[2], z, kept;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            token[j] = j0 + j < k ? (int)rank_key_index(keys[j0 + j]) : -1;
+            e[j] = j0 + j < k ? exp(((double)value_of_key(keys[j0 + j]) - (double)top) * per_t) : 0.0;
+        }
+        const double upto_e = block_scan(e[0] + e[1], red, &z);
+        bool in[2] = {j0 < k, j0 + 1 < k};
+        if (top_p < 1.f) {
+            in[0] = in[0] && (j0 == 0 || (upto_e - e[1] - e[0]) / z < (double)top_p);
+            in[1] = in[1] && (upto_e - e[1]) / z < (double)top_p;
+        }
+        block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), red, &kept);
+        double* weights = reinterpret_cast<double*>(keys + kVerifyMaxTopK);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (in[j] && token[j] == d) s_pd = e[j] / kept;
+            weights[j0 + j] = in[j] ? e[j] / kept : 0.0;
+            keys[j0 + j] = j0 + j < k ? (uint64_t)(0xFFFFFFFFu - (uint32_t)token[j]) << 32 | (uint32_t)(j0 + j) : 0;
+        }
+        __syncthreads();
+        if (d >= 0 && kept_below < s_pd) {
+            if (tid == 0) *out = make_int2(1, -1);
+            return;
+        }
+        sort_desc(keys, k);   // by token; at most kVerifyMaxTopK, the weights lie behind
+        double w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint64_t key = j0 + j < k ? keys[j0 + j] : 0;
+            token[j] = (int)(0xFFFFFFFFu - (uint32_t)(key >> 32));
+            w[j] = j0 + j < k ? weights[(uint32_t)key] : 0.0;
+        }
+        __syncthreads();
+        ids = reinterpret_cast<int*>(keys);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            weights[j0 + j] = w[j];
+            ids[j0 + j] = token[j];
+        }
+        __syncthreads();
+        shares = weights;
+        tokens = ids;
+        n_last = k;
+    }
+    // the draw, two tokens a thread
     const int j0 = 2 * tid;
     int token[2];
-    double e[2], z, kept;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        token[j] = j0 + j < k ? (int)rank_key_index(keys[j0 + j]) : -1;
-        e[j] = j0 + j < k ? exp(((double)value_of_key(keys[j0 + j]) - (double)top) * per_t) : 0.0;
-    }
-    const double upto_e = block_scan(e[0] + e[1], red, &z);
-    bool in[2] = {j0 < k, j0 + 1 < k};
-    if (top_p < 1.f) {
-        in[0] = in[0] && (j0 == 0 || (upto_e - e[1] - e[0]) / z < (double)top_p);
-        in[1] = in[1] && (upto_e - e[1]) / z < (double)top_p;
-    }
-    // behind the last that is kept (a scan's sums may be out of order by a rounding)
-    if (in[0] || in[1]) atomicMax(&s_span, in[1] ? j0 + 2 : j0 + 1);
-    block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), red, &kept);
-    const int n_kept = block_count((int)in[0] + (int)in[1]);
-    size = power_of_two(s_span);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {   // in the order of tokens from here on
-        if (in[j] && token[j] == d) s_pd = e[j] / kept;
-        if (j0 + j < kVerifyMaxTopK) weights[j0 + j] = e[j] / kept;
-        if (j0 + j < size) keys[j0 + j] = in[j] ? (uint64_t)(0xFFFFFFFFu - (uint32_t)token[j]) << 32 | (uint32_t)(j0 + j) : 0;
-    }
-    __syncthreads();
-    if (d >= 0 && kept_below < s_pd) {
-        if (tid == 0) *out = make_int2(1, -1);
-        return;
-    }
-    sort_desc(keys, size);
     double p[2], r[2], total;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        token[j] = -1;
-        p[j] = r[j] = 0.0;
-        if (j0 + j < n_kept) {
-            const uint64_t key = keys[j0 + j];
-            token[j] = (int)(0xFFFFFFFFu - (uint32_t)(key >> 32));
-            p[j] = r[j] = weights[(uint32_t)key];
-            if (d >= 0) r[j] = fmax(p[j] - (q != nullptr ? (double)q[token[j]] : (token[j] == d ? 1.0 : 0.0)), 0.0);
-        }
+        token[j] = j0 + j < n_last ? tokens[j0 + j] : -1;
+        p[j] = r[j] = j0 + j < n_last ? shares[j0 + j] : 0.0;
+        if (d >= 0 && p[j] > 0.0) r[j] = fmax(p[j] - (q != nullptr ? (double)q[token[j]] : (token[j] == d ? 1.0 : 0.0)), 0.0);
     }
     double upto = block_scan(r[0] + r[1], red, &total);
     if (!(total > 0.0)) {   // the draft's distribution covers the target's
@@ -551,7 +685,7 @@ __global__ void __launch_bounds__(128) verify_lanes_kernel(const __grid_constant
 void launch_verify_drafts(VerifyArgs a, cudaStream_t s) {
     if (a.lanes <= 0) return;
     const int size = a.type == 0 ? 4 : 2, chunk = ((a.vocab + kCtas - 1) / kCtas + 7) / 8 * 8;
-    a.list_at = std::max(chunk * size + 32, kCandidates * 8);
+    a.list_at = std::max(chunk * size + 32, kCandidates * 8 + kThreads * 12);   // where candidates meet
     const size_t smem = (size_t)a.list_at + kCandidates * 2;
     auto* kernel = a.type == 0 ? verify_rows_kernel<float> : (a.type == 1 ? verify_rows_kernel<__half> : verify_rows_kernel<__nv_bfloat16>);
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
