@@ -693,7 +693,7 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
  * replaced by a token of max(p_i - q_i, 0), and behind the last one a token of p is added, both drawn by u_drafts: the first token, in
  * their order, whose cumulative weight exceeds u times the whole.  tokens [lanes][drafts + 1]: the kept drafts, that token, -1 behind;
  * accepted [lanes]: how many were kept.  A row that is no distribution ends the lane with token -1 and MK_DEV_BAD_ROW. */
-int32_t mk_k_verify_drafts_workspace(int32_t lanes, int32_t drafts, int64_t* bytes);
+int32_t mk_k_verify_drafts_workspace(int32_t type, int32_t lanes, int32_t drafts, int32_t vocab, int64_t* bytes);
 int32_t mk_k_verify_drafts_dev(int32_t type, const void* logits_dev, int64_t logits_stride, int32_t lanes, int32_t drafts, int32_t vocab, const int32_t* drafts_dev,
                                const float* draft_probs_dev, const float* u_dev, const float* temperature_dev, const int32_t* top_k_dev, const float* top_p_dev,
                                int32_t* tokens_dev, int32_t* accepted_dev, void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev, void* cuda_stream);

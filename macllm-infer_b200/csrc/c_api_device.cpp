@@ -32,6 +32,15 @@ SharedAttnPlan checked_plan(int q_heads, int kv_heads, int d, int block_tokens, 
     return p;
 }
 
+int logits_kind(int type) { return type == MK_TYPE_F32 ? 0 : (type == MK_TYPE_F16 ? 1 : 2); }
+VerifyPlan checked_verify_plan(int type, int lanes, int drafts, int vocab) {
+    need(type == MK_TYPE_F32 || type == MK_TYPE_F16 || type == MK_TYPE_BF16, "mk_k_verify_drafts: logits are f32, f16 or bf16");
+    need(lanes >= 0 && drafts >= 0 && vocab > 0, "mk_k_verify_drafts: negative sizes");
+    need(vocab <= kVerifyMaxVocab, "mk_k_verify_drafts: a vocabulary has at most 416000 tokens");
+    need((int64_t)lanes * ((int64_t)drafts + 1) <= 1 << 22, "mk_k_verify_drafts: too many rows");
+    return verify_plan(logits_kind(type), lanes, drafts, vocab);
+}
+
 }  // namespace
 
 extern "C" {
@@ -76,35 +85,30 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
     });
 }
 
-int32_t mk_k_verify_drafts_workspace(int32_t lanes, int32_t drafts, int64_t* bytes) {
-    return guarded([&] {
-        need(lanes >= 0 && drafts >= 0, "mk_k_verify_drafts: negative lanes or drafts");
-        *bytes = verify_scratch_bytes(lanes, drafts);
-    });
+int32_t mk_k_verify_drafts_workspace(int32_t type, int32_t lanes, int32_t drafts, int32_t vocab, int64_t* bytes) {
+    return guarded([&] { *bytes = checked_verify_plan(type, lanes, drafts, vocab).bytes; });
 }
 
 int32_t mk_k_verify_drafts_dev(int32_t type, const void* logits_dev, int64_t logits_stride, int32_t lanes, int32_t drafts, int32_t vocab, const int32_t* drafts_dev,
                                const float* draft_probs_dev, const float* u_dev, const float* temperature_dev, const int32_t* top_k_dev, const float* top_p_dev,
                                int32_t* tokens_dev, int32_t* accepted_dev, void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev, void* cuda_stream) {
     return guarded([&] {
-        need(type == MK_TYPE_F32 || type == MK_TYPE_F16 || type == MK_TYPE_BF16, "mk_k_verify_drafts_dev: logits are f32, f16 or bf16");
-        need(lanes >= 0 && drafts >= 0 && vocab > 0 && logits_stride >= vocab, "mk_k_verify_drafts_dev: negative sizes, or rows overlap");
-        need((int64_t)lanes * (drafts + 1) <= INT32_MAX / 16, "mk_k_verify_drafts_dev: too many rows");
-        need(vocab <= kVerifyMaxVocab, "mk_k_verify_drafts_dev: a vocabulary has at most 416000 tokens");
+        const VerifyPlan p = checked_verify_plan(type, lanes, drafts, vocab);
+        need(logits_stride >= vocab, "mk_k_verify_drafts_dev: rows overlap");
         if (lanes == 0) return;
         need(aligned(logits_dev, type == MK_TYPE_F32 ? 4 : 2), "mk_k_verify_drafts_dev: logits are not aligned to their type");
         need(logits_dev != nullptr && (drafts_dev != nullptr || drafts == 0) && u_dev != nullptr && temperature_dev != nullptr && top_k_dev != nullptr && top_p_dev != nullptr &&
                  tokens_dev != nullptr && accepted_dev != nullptr,
              "mk_k_verify_drafts_dev: null pointer");
-        need(workspace_dev != nullptr && workspace_bytes >= verify_scratch_bytes(lanes, drafts) && aligned(workspace_dev, 16),
+        need(workspace_dev != nullptr && workspace_bytes >= p.bytes && aligned(workspace_dev, 16),
              "mk_k_verify_drafts_dev: the workspace is missing, too small or not aligned to 16 bytes");
         require_device();
         VerifyArgs a;
-        a.logits = logits_dev; a.ld = logits_stride; a.type = type == MK_TYPE_F32 ? 0 : (type == MK_TYPE_F16 ? 1 : 2);
+        a.logits = logits_dev; a.ld = logits_stride; a.type = logits_kind(type);
         a.lanes = lanes; a.n_drafts = drafts; a.vocab = vocab; a.drafts = drafts_dev; a.draft_probs = draft_probs_dev; a.u = u_dev;
         a.temperature = temperature_dev; a.top_k = top_k_dev; a.top_p = top_p_dev; a.tokens = tokens_dev; a.accepted = accepted_dev;
-        a.rows = static_cast<int2*>(workspace_dev); a.status = status_dev;
-        launch_verify_drafts(a, static_cast<cudaStream_t>(cuda_stream));
+        a.status = status_dev;
+        launch_verify_drafts(a, p, static_cast<uint8_t*>(workspace_dev), static_cast<cudaStream_t>(cuda_stream));
     });
 }
 

@@ -6,17 +6,18 @@
 // p.  The tokens are then distributed as if drawn from the target one by one: q min(1, p / q) + (1 - sum q min(1, p / q)) max(p - q, 0) / sum max(p - q, 0) = p.
 // A draw takes the first token, in the order of tokens, whose cumulative weight exceeds u_n times the whole.
 //
-// Every row is judged by itself, by a cluster of eight CTAs that hold it in their shared memory: it is fetched once, with bulk copies, and what needs more than
-// one look at it (maximum, sum, candidates, draw) looks there.  A second kernel takes a lane's first row that ends it.
+// Two kernels.  The first streams every row that can be reached once, a run of tokens to a CTA and at most 32 of them to a thread, and leaves what a run amounts
+// to: its best token, whether it holds what is no logit, the sum of its weights (whole vocabulary), and the best value of each thread's tokens (top_k).  What bounds it is HBM.
+// The second finishes rows, eight CTAs in a cluster to each.  Over the whole vocabulary a row's sum follows from its runs', so each cluster judges the rows in front
+// of its own too, and only the one whose row ends the lane goes through its row again, for the draw.  With a top_k the first CTA takes
+// candidates: the k-th best of the threads' best values is a bound that at least k tokens reach and few more do, and only the tokens of threads that reach it are read again;
+// where too many reach it (thousands of equal logits) bisection over (value, token) finds one that fewer do.  The CTA that ends last among a lane's rows puts the lane together.
 //
-// Candidates of a top_k: each of the cluster's 4096 threads has the best of its own tokens, and the k-th best of those is a bound that at least k tokens reach and, since
-// tokens are dealt out evenly, few more do; those are sorted.  Where too many reach it (thousands of equal logits) bisection over (value, token) finds one that
-// fewer do.  Weights and sums of candidates are 64-bit.  Over the whole vocabulary a weight is a 32-bit number (ex2 of a product kept to twice 32 bits: 2^-22, and
-// with no trend, so that sums over many are better), a sum of four is added up in 64 bits.
+// Weights and sums of candidates are 64-bit.  Over the whole vocabulary a weight is a 32-bit number (ex2 of a product kept to twice 32 bits: 2^-22, and with no trend, so that
+// sums over many are better) and sums are 64-bit.
 #include "verify_drafts.h"
 #include "sampling_math.h"
 #include "shared_attention.h"
-#include "umma.cuh"
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <algorithm>
@@ -27,8 +28,15 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kCtas = 8, kThreads = 512, kWarps = kThreads / 32, kPieces = 4;
-constexpr int kCandidates = 2048;   // sorted at once; at least twice the largest top_k
+constexpr int kCtas = 8, kThreads = 512, kWarps = kThreads / 32;
+constexpr int kScan = 256;          // threads of the first kernel's CTAs
+constexpr int kCandidates = 2048;   // sorted at once
+
+struct Run {
+    uint64_t best;   // key of its best token
+    double sum;      // of the weights against that one, where the whole vocabulary counts
+    int bad, pad_;
+};
 
 __device__ __forceinline__ void tell(int32_t* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);
@@ -36,9 +44,6 @@ __device__ __forceinline__ void tell(int32_t* status, int bit) {
 __device__ __forceinline__ float value_of(float x) { return x; }
 __device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void set_low(float* x) { *x = -INFINITY; }
-__device__ __forceinline__ void set_low(__half* x) { *x = __ushort_as_half(0xFC00); }
-__device__ __forceinline__ void set_low(__nv_bfloat16* x) { *x = __ushort_as_bfloat16(0xFF80); }
 // The values of 16 bytes.
 __device__ __forceinline__ void unpack(const uint4& r, float (&v)[4], const float*) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
@@ -137,6 +142,11 @@ __device__ void sort_desc(uint64_t* keys, int n) {   // keys behind n are there 
 // exp((x - top) / temperature) with 1 / (temperature ln 2) as the sum of two 32-bit numbers.
 struct Exponential {
     float top, hi, lo;
+    __device__ __forceinline__ Exponential(float best, float temperature) : top(best) {
+        const double unit = 1.4426950408889634074 / (double)temperature;
+        hi = (float)unit;
+        lo = (float)(unit - (double)hi);
+    }
     __device__ __forceinline__ float operator()(float x) const {
         const float y = x - top, t = y * hi, rest = fmaf(y, lo, fmaf(y, hi, -t));
         float e;
@@ -145,104 +155,65 @@ struct Exponential {
     }
 };
 
+// Piece v of a row, 16 bytes counted from the last boundary at or before its first value; places outside the row hold -inf.
 template <typename T>
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify_rows_kernel(const __grid_constant__ VerifyArgs a, int chunk) {
-    constexpr int EPV = 16 / (int)sizeof(T);   // values of 16 bytes
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint64_t bars[kPieces], best_of[kCtas], warp_best[kWarps];
-    __shared__ double sum_of[3][kCtas], red[kWarps], region[kWarps];
-    __shared__ int bad_of[kCtas], count_of[2][kCtas];
-    __shared__ uint32_t thread_best[kThreads], warp_low[kWarps];
-    __shared__ int s_count, s_pick, s_last, hist[256];
-    __shared__ int2 s_step;
-    __shared__ double s_pd;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), index = blockIdx.x / kCtas;
+struct Row {
+    static constexpr int EPV = 16 / (int)sizeof(T);
+    const T* x;
+    int vocab, shift;   // shift: values of the first piece that are in front of the row
+    __device__ __forceinline__ Row(const T* row, int n) : x(row), vocab(n), shift((int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))) {}
+    __device__ __forceinline__ int token(int v) const { return v * EPV - shift; }
+    __device__ __forceinline__ void load(int v, float (&f)[EPV]) const {
+        const int t0 = token(v);
+        if (t0 >= 0 && t0 + EPV <= vocab) {
+            unpack(*reinterpret_cast<const uint4*>(x + t0), f, static_cast<const T*>(nullptr));
+        } else {
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) f[j] = t0 + j >= 0 && t0 + j < vocab ? value_of(x[t0 + j]) : -INFINITY;
+        }
+    }
+};
+
+__device__ __forceinline__ bool is_draft(int d, int vocab) { return d >= 0 && d < vocab; }
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant__ VerifyArgs a) {
+    constexpr int EPV = 16 / (int)sizeof(T);
+    __shared__ uint64_t warp_best[kScan / 32];
+    __shared__ double warp_sum_of[kScan / 32];
+    const int tid = threadIdx.x, wl = tid & 31, warp = tid >> 5, index = blockIdx.x / a.runs, run = blockIdx.x - index * a.runs;
     const int lane = index / (a.n_drafts + 1), i = index - lane * (a.n_drafts + 1), vocab = a.vocab;
     pdl_trigger();
     const int32_t* drafts = a.drafts + (int64_t)lane * a.n_drafts;
-    const float* u = a.u + (int64_t)lane * (a.n_drafts + 1);
-    const float temperature = a.temperature[lane], top_p = a.top_p[lane], u_last = u[a.n_drafts], u_mine = u[i];
-    int k = a.top_k[lane], d = i < a.n_drafts ? drafts[i] : -1;
+    const float temperature = a.temperature[lane];
+    const int k = a.top_k[lane];
     bool gone = false;
-    for (int j = wl; j < i; j += 32) gone |= drafts[j] < 0 || drafts[j] >= vocab;
+    for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
+    if (i == 0 && run == 0 && tid == 0) a.counters[lane] = 0;
     if (__any_sync(0xffffffffu, gone)) return;   // nothing gets here
-    if (d >= vocab) {
-        if (tid == 0) tell(a.status, kDevBadRange);
-        d = -1;
-    }
-    const T* x = static_cast<const T*>(a.logits) + index * a.ld;
-    int2* out = a.rows + index;
-
-    // ---- this CTA's run of tokens, in 16-byte pieces of its row; places of the first and last piece that are not its hold -inf
-    const int n0 = min(vocab, rank * chunk), n = min(chunk, vocab - n0);
-    const uintptr_t src = reinterpret_cast<uintptr_t>(x + n0);
-    const int shift = (int)(src & 15), bytes = n * (int)sizeof(T), vecs = n > 0 ? (shift + bytes + 15) / 16 : 0;
-    const int v_lo = shift > 0 ? 1 : 0, v_hi = max(v_lo, (shift + bytes) / 16), per_piece = (v_hi - v_lo + kPieces - 1) / kPieces;
-    const int token0 = n0 - shift / (int)sizeof(T);   // of the first place
-    uint4* buf = reinterpret_cast<uint4*>(smem);
-    uint16_t* list = reinterpret_cast<uint16_t*>(smem + a.list_at);
-    if (tid == 0) {
-        for (int p = 0; p < kPieces; ++p) umma::bar_init(&bars[p], 1);
-        umma::bar_init_fence();
-        s_count = 0;
-        s_pick = INT_MAX;
-        s_last = -1;
-        s_pd = 0.0;
-    }
-    __syncthreads();
-    if (tid == 0)
-        for (int p = 0; p < kPieces; ++p) {
-            const int lo = v_lo + p * per_piece, hi = min(v_hi, lo + per_piece);
-            if (hi <= lo) continue;
-            umma::bar_expect_tx(&bars[p], (uint32_t)(hi - lo) * 16);
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(umma::smem_u32(buf + lo)), "l"(src - shift + (uintptr_t)lo * 16),
-                         "r"((uint32_t)(hi - lo) * 16), "r"(umma::smem_u32(&bars[p]))
-                         : "memory");
-        }
-    auto edge = [&](int v) {
-        for (int j = tid; j < EPV; j += kThreads) {
-            const int t = token0 + v * EPV + j;
-            T* to = reinterpret_cast<T*>(buf + v) + j;
-            if (t >= n0 && t < n0 + n) *to = x[t];
-            else set_low(to);
-        }
-    };
-    if (vecs > 0 && v_lo == 1) edge(0);
-    if (vecs > v_hi && (v_hi > 0 || v_lo == 0)) edge(v_hi);
-    __syncthreads();
-
-    float mine = -INFINITY;
-    bool bad = false, ok = true;
-    uint64_t best = 0;
-    auto look = [&](int v) {
-        float f[EPV];
-        unpack(buf[v], f, static_cast<const T*>(nullptr));
-        float m = f[0];
+    const Row<T> row(static_cast<const T*>(a.logits) + index * a.ld, vocab);
+    float f[VPT][EPV];
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) row.load((run * VPT + c) * kScan + tid, f[c]);
+    bool bad = false;
+    float top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < VPT; ++c)
 #pragma unroll
         for (int j = 0; j < EPV; ++j) {
-            bad |= !(f[j] < INFINITY);
-            m = fmaxf(m, f[j]);
+            bad |= !(f[c][j] < INFINITY);
+            top = fmaxf(top, f[c][j]);
         }
-        if (m > mine || best == 0) {
-            mine = m;
+    int at = vocab;
 #pragma unroll
-            for (int j = EPV - 1; j >= 0; --j)
-                if (f[j] == m) best = key_of(m, token0 + v * EPV + j);
-        }
-    };
-    if (tid == 0 && vecs > 0 && v_lo == 1) look(0);
-    for (int p = 0; p < kPieces; ++p) {
-        const int lo = v_lo + p * per_piece, hi = min(v_hi, lo + per_piece);
-        if (hi <= lo) continue;
-        ok = umma::bar_wait(&bars[p], 0) && ok;
-        for (int v = lo + tid; v < hi; v += kThreads) look(v);
-    }
-    if (tid == kThreads - 1 && vecs > v_hi && (v_hi > 0 || v_lo == 0)) look(v_hi);
-    if (best == 0) best = key_of(-INFINITY, vocab);
-    thread_best[tid] = (uint32_t)(best >> 32);
-    if (!ok) tell(a.status, kDevWait);
-    bad = __syncthreads_or(bad || !ok);
+    for (int c = VPT - 1; c >= 0; --c)
+#pragma unroll
+        for (int j = EPV - 1; j >= 0; --j)
+            if (f[c][j] == top) at = row.token((run * VPT + c) * kScan + tid) + j;
+    if (top == -INFINITY) at = vocab;
+    uint64_t best = key_of(top, at);
+    if (temperature > 0.f && k > 0) a.group_best[((int64_t)index * a.runs + run) * kScan + tid] = (uint32_t)(best >> 32);
+    bad = __syncthreads_or(bad);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -250,208 +221,288 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
     }
     if (wl == 0) warp_best[warp] = best;
     __syncthreads();
-    if (warp == 0) {
-        best = warp_best[wl % kWarps];
 #pragma unroll
-        for (int o = kWarps / 2; o > 0; o >>= 1) {
-            const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-            best = other > best ? other : best;
-        }
-        if (wl < kCtas) {
-            *cluster.map_shared_rank(&best_of[rank], wl) = best;
-            *cluster.map_shared_rank(&bad_of[rank], wl) = bad;
-        }
-    }
-    cluster.sync();
-    best = best_of[0];
-    bad = bad_of[0];
+    for (int w = 0; w < kScan / 32; ++w) best = warp_best[w] > best ? warp_best[w] : best;
+    double sum = 0.0;
+    if (temperature > 0.f && k <= 0) {
+        const Exponential weight(value_of_key(best), temperature);
 #pragma unroll
-    for (int c = 1; c < kCtas; ++c) {
-        best = best_of[c] > best ? best_of[c] : best;
-        bad |= bad_of[c] != 0;
+        for (int c = 0; c < VPT; ++c)
+#pragma unroll
+            for (int j = 0; j < EPV; j += 4) sum += (double)((weight(f[c][j]) + weight(f[c][j + 1])) + (weight(f[c][j + 2]) + weight(f[c][j + 3])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (wl == 0) warp_sum_of[warp] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < kScan / 32; ++w) sum += warp_sum_of[w];
     }
-    const float top = value_of_key(best);
-    if (bad || top == -INFINITY) {
-        if (rank == 0 && tid == 0) {
-            tell(a.status, kDevBadRow);
-            *out = make_int2(0, -1);
-        }
-        return;
+    if (tid == 0) {
+        Run r;
+        r.best = best;
+        r.sum = sum;
+        r.bad = bad;
+        r.pad_ = 0;
+        static_cast<Run*>(a.run_results)[(int64_t)index * a.runs + run] = r;
     }
-    if (!(temperature > 0.f)) {
-        if (rank == 0 && tid == 0) *out = make_int2(d == (int)rank_key_index(best), (int)rank_key_index(best));
-        return;
-    }
-    if (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f)) {
-        if (rank == 0 && tid == 0) tell(a.status, kDevBadRange);
-        k = min(k, kVerifyMaxTopK);
-    }
-    k = min(k, vocab);
-    const double per_t = 1.0 / (double)temperature;
-    const float* q = a.draft_probs == nullptr || d < 0 ? nullptr : a.draft_probs + ((int64_t)lane * a.n_drafts + i) * vocab;
-    const double u_draw = (double)u_last, kept_below = d >= 0 ? (double)u_mine * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
+}
 
-    if (k <= 0) {
-        // ---- the whole vocabulary
-        const double unit = per_t * 1.4426950408889634074;
-        Exponential weight;
-        weight.top = top;
-        weight.hi = (float)unit;
-        weight.lo = (float)(unit - (double)weight.hi);
-        auto block_sum_to = [&](double v, double* slot) {   // of this CTA, to the whole cluster
-            v += __shfl_xor_sync(0xffffffffu, v, 16);
-            v += __shfl_xor_sync(0xffffffffu, v, 8);
-            v += __shfl_xor_sync(0xffffffffu, v, 4);
-            v += __shfl_xor_sync(0xffffffffu, v, 2);
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            if (wl == 0) region[warp] = v;
+// What a warp knows of a row from its runs.
+struct RowSum {
+    uint64_t best;
+    double z;
+    bool bad;
+};
+__device__ __forceinline__ RowSum sum_runs(const Run* runs, int n, double unit, bool whole) {
+    const int wl = threadIdx.x & 31;
+    RowSum s{0, 0.0, false};
+    for (int c = wl; c < n; c += 32) {
+        s.best = runs[c].best > s.best ? runs[c].best : s.best;
+        s.bad |= runs[c].bad != 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, s.best, o);
+        s.best = other > s.best ? other : s.best;
+    }
+    const float top = value_of_key(s.best);
+    s.bad = __any_sync(0xffffffffu, s.bad) || top == -INFINITY;
+    if (whole && !s.bad) {
+        for (int c = wl; c < n; c += 32) {
+            const float own = value_of_key(runs[c].best);
+            if (own > -INFINITY) s.z += runs[c].sum * exp(((double)own - (double)top) * unit);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+    }
+    return s;
+}
+
+__device__ __forceinline__ void put_lane(const VerifyArgs& a, int lane, int end, int token) {   // a warp
+    for (int j = threadIdx.x & 31; j <= a.n_drafts; j += 32)
+        a.tokens[(int64_t)lane * (a.n_drafts + 1) + j] = j < end ? a.drafts[(int64_t)lane * a.n_drafts + j] : (j == end ? token : -1);
+    if ((threadIdx.x & 31) == 0) a.accepted[lane] = end;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish_rows_kernel(const __grid_constant__ VerifyArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ double sum_of[2][kCtas], red[kWarps], region[kWarps], s_pd, s_z;
+    __shared__ uint64_t s_best;
+    __shared__ uint32_t warp_low[kWarps];
+    __shared__ int s_count, s_groups, s_pick, s_last, s_reached, s_bad, s_kept, hist[256];
+    __shared__ int4 s_step;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), index = blockIdx.x / kCtas;
+    const int n_drafts = a.n_drafts, lane = index / (n_drafts + 1), i = index - lane * (n_drafts + 1), vocab = a.vocab;
+    const int32_t* drafts = a.drafts + (int64_t)lane * n_drafts;
+    const float* u = a.u + (int64_t)lane * (n_drafts + 1);
+    const float temperature = a.temperature[lane], top_p = a.top_p[lane];
+    int k = a.top_k[lane];
+    const bool whole = temperature > 0.f && k <= 0;
+    if (rank != 0 && !whole) return;
+    bool gone = false;
+    for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
+    if (__any_sync(0xffffffffu, gone)) return;
+    int d = i < n_drafts ? drafts[i] : -1;
+    const double u_draw = (double)u[n_drafts], per_t = temperature > 0.f ? 1.0 / (double)temperature : 0.0;
+    const T* x = static_cast<const T*>(a.logits) + index * a.ld;
+    if (rank == 0 && tid == 0 && (d >= vocab || (temperature > 0.f && (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f))))) tell(a.status, kDevBadRange);
+    if (!is_draft(d, vocab)) d = -1;
+    k = min(min(k, kVerifyMaxTopK), vocab);
+    const float* probs = a.draft_probs == nullptr ? nullptr : a.draft_probs + (int64_t)lane * n_drafts * vocab;
+    const float* q = probs == nullptr || d < 0 ? nullptr : probs + (int64_t)i * vocab;
+    if (tid == 0) {
+        s_count = s_groups = 0;
+        s_pick = INT_MAX;
+        s_last = -1;
+        s_reached = 1;
+        s_pd = 0.0;
+    }
+    __syncthreads();
+    pdl_wait();
+    const Run* runs = static_cast<const Run*>(a.run_results) + (int64_t)(index - i) * a.runs;   // of the lane
+
+    if (!(temperature > 0.f) || whole) {
+        // ---- rows that their runs tell all of: this one and those in front of it
+        for (int j = warp; j <= i; j += kWarps) {
+            const RowSum s = sum_runs(runs + (int64_t)j * a.runs, a.runs, per_t, whole);
+            const int dj = j < i ? drafts[j] : d;
+            bool kept = false;
+            if (dj >= 0 && !s.bad) {
+                if (whole) {
+                    const double qd = probs != nullptr ? (double)probs[(int64_t)j * vocab + dj] : 1.0;
+                    const double xd = (double)value_of(x[(int64_t)(j - i) * a.ld + dj]);
+                    kept = (double)u[j] * qd < exp((xd - (double)value_of_key(s.best)) * per_t) / s.z;
+                } else {
+                    kept = dj == (int)rank_key_index(s.best);
+                }
+            }
+            if (j < i && !kept) s_reached = 0;
+            if (j == i && wl == 0) {
+                s_best = s.best;
+                s_z = s.z;
+                s_bad = s.bad;
+                s_kept = kept;
+            }
+        }
+        __syncthreads();
+        if (!s_reached || s_kept) return;
+        if (s_bad || !whole) {
+            if (rank != 0 || warp != 0) return;
+            if (s_bad && wl == 0) tell(a.status, kDevBadRow);
+            put_lane(a, lane, i, s_bad ? -1 : (int)rank_key_index(s_best));
+            return;
+        }
+        // ---- the draw: every warp adds up a run of its own, and a CTA looks through the one where the target lies
+        const double z = s_z;
+        const Exponential weight(value_of_key(s_best), temperature);
+        const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
+        const int chunk = (vocab + kCtas - 1) / kCtas, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
+        const int run = (n1 - n0 + kWarps - 1) / kWarps, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
+        bool rest = d >= 0;
+        auto share = [&](float logit, float qt) {
+            const float w = weight(logit);
+            return rest ? fmaxf(fmaf(w, per_z, -qt) + w * per_z_rest, 0.f) : w;
+        };
+        auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
+        double total = 0.0, *sums = sum_of[0];
+        for (;;) {
+            constexpr int AHEAD = 8;
+            double part = 0.0;
+            for (int t0 = r_lo + wl; t0 < r_hi; t0 += 32 * AHEAD) {
+                float l[AHEAD], qv[AHEAD], s = 0.f;
+#pragma unroll
+                for (int c = 0; c < AHEAD; ++c) {
+                    const int t = t0 + 32 * c;
+                    l[c] = t < r_hi ? value_of(x[t]) : -INFINITY;
+                    qv[c] = t < r_hi ? q_at(t) : 0.f;
+                }
+#pragma unroll
+                for (int c = 0; c < AHEAD; ++c) s += share(l[c], qv[c]);
+                part += (double)s;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+            if (wl == 0) region[warp] = part;
             __syncthreads();
             if (warp == 0) {
                 double s = region[wl % kWarps];
 #pragma unroll
                 for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (wl < kCtas) *cluster.map_shared_rank(slot + rank, wl) = s;
+                if (wl < kCtas) *cluster.map_shared_rank(sums + rank, wl) = s;
             }
             cluster.sync();
-        };
-        double part = 0.0;
-        for (int v = tid; v < vecs; v += kThreads) {
-            float f[EPV], s[EPV / 4];
-            unpack(buf[v], f, static_cast<const T*>(nullptr));
-#pragma unroll
-            for (int j = 0; j < EPV; j += 4) s[j / 4] = (weight(f[j]) + weight(f[j + 1])) + (weight(f[j + 2]) + weight(f[j + 3]));
-#pragma unroll
-            for (int j = 0; j < EPV / 4; ++j) part += (double)s[j];
-        }
-        block_sum_to(part, sum_of[0]);
-        double z = 0.0;
-#pragma unroll
-        for (int c = 0; c < kCtas; ++c) z += sum_of[0][c];
-        if (d >= 0 && kept_below < exp(((double)value_of(x[d]) - (double)top) * per_t) / z) {
-            if (rank == 0 && tid == 0) *out = make_int2(1, -1);
-            return;
-        }
-        const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
-        // The draw: every warp adds up a run of its own, one of them walks through the run where the target lies.
-        const int run = (vecs + kWarps - 1) / kWarps, r_lo = min(vecs, warp * run), r_hi = min(vecs, r_lo + run);
-        bool rest = d >= 0;
-        auto load_q = [&](int v, float (&r)[EPV]) {   // what the draft's distribution has there, 0 where the row ends
-            const int t0 = token0 + v * EPV;
-#pragma unroll
-            for (int j = 0; j < EPV; ++j) r[j] = q != nullptr ? (t0 + j >= n0 && t0 + j < n0 + n && v < vecs ? q[t0 + j] : 0.f) : (t0 + j == d ? 1.f : 0.f);
-        };
-        auto shares_of = [&](int v, const float (&qv)[EPV], float (&r)[EPV]) {
-            unpack(buf[v], r, static_cast<const T*>(nullptr));
-#pragma unroll
-            for (int j = 0; j < EPV; ++j) {
-                const float w = weight(r[j]);
-                r[j] = rest ? fmaxf(fmaf(w, per_z, -qv[j]) + w * per_z_rest, 0.f) : w;
-            }
-        };
-        double total = 0.0, *sums = sum_of[1];
-        for (;;) {
-            part = 0.0;
-            constexpr int AHEAD = 16 / EPV;   // the draft's values of several pieces are on their way together
-            for (int v0 = r_lo + wl; v0 < r_hi; v0 += 32 * AHEAD) {
-                float qv[AHEAD][EPV];
-                if (rest) {
-#pragma unroll
-                    for (int c = 0; c < AHEAD; ++c) load_q(v0 + 32 * c, qv[c]);
-                }
-#pragma unroll
-                for (int c = 0; c < AHEAD; ++c) {
-                    if (v0 + 32 * c >= r_hi) break;
-                    float r[EPV];
-                    shares_of(v0 + 32 * c, qv[c], r);
-#pragma unroll
-                    for (int j = 0; j < EPV; j += 4) part += (double)((r[j] + r[j + 1]) + (r[j + 2] + r[j + 3]));
-                }
-            }
-            block_sum_to(part, sums);
             total = 0.0;
 #pragma unroll
             for (int c = 0; c < kCtas; ++c) total += sums[c];
             if (total > 0.0 || !rest) break;
             rest = false;   // the draft's distribution covers the target's
-            sums = sum_of[2];
+            sums = sum_of[1];
         }
         const double target = u_draw * total;
-        double before = 0.0;
+        // the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
+        double upto = 0.0;
         int at = -1;
 #pragma unroll
         for (int c = 0; c < kCtas; ++c) {
-            if (sums[c] > 0.0 && !(at >= 0 && before > target)) at = c;
-            if (!(before > target)) before += sums[c];
+            if (upto > target) break;
+            if (sums[c] > 0.0) at = c;
+            upto += sums[c];
         }
         if (at != rank) return;
-        // at: the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
-        before = 0.0;
-        for (int c = 0; c < rank; ++c) before += sums[c];
-        int w_at = -1;
-        double w_before = before, upto_run = before;
+        upto = 0.0;
+        for (int c = 0; c < rank; ++c) upto += sums[c];
+        int w_at = 0;
+        double before = upto;
         for (int w = 0; w < kWarps; ++w) {
             if (region[w] > 0.0) {
                 w_at = w;
-                w_before = upto_run;
+                before = upto;
             }
-            upto_run += region[w];
-            if (upto_run > target) break;
+            upto += region[w];
+            if (upto > target) break;
         }
-        // the whole CTA looks through that run
-        const int at_lo = min(vecs, w_at * run), at_hi = min(vecs, at_lo + run);
-        for (int v0 = at_lo; v0 < at_hi; v0 += kThreads) {
-            const int v = v0 + tid;
-            float qv[EPV], r[EPV];
-            double s = 0.0, all;
-            if (v < at_hi) {
-                load_q(v, qv);
-                shares_of(v, qv, r);
-#pragma unroll
-                for (int j = 0; j < EPV; ++j) {
-                    s += (double)r[j];
-                    if (r[j] > 0.f) atomicMax(&s_last, token0 + v * EPV + j);
-                }
+        const int at_lo = min(n1, n0 + w_at * run), at_hi = min(n1, at_lo + run);
+        for (int t0 = at_lo; t0 < at_hi; t0 += kThreads) {
+            const int t = t0 + tid;
+            const double r = t < at_hi ? (double)share(value_of(x[t]), q_at(t)) : 0.0;
+            double all;
+            const double c = before + block_scan(r, red, &all);
+            if (r > 0.0) {
+                atomicMax(&s_last, t);
+                if (c > target) atomicMin(&s_pick, t);
             }
-            double c = w_before + block_scan(s, red, &all) - s;
-            if (v < at_hi && s > 0.0 && c + s > target) {
-                int pick = -1;
-#pragma unroll
-                for (int j = 0; j < EPV; ++j) {
-                    c += (double)r[j];
-                    if (r[j] > 0.f && (pick < 0 || !(c - (double)r[j] > target))) pick = token0 + v * EPV + j;
-                }
-                atomicMin(&s_pick, pick);
-            }
-            w_before += all;
+            before += all;
             __syncthreads();
             if (s_pick < INT_MAX) break;
         }
-        if (tid == 0) *out = make_int2(0, s_pick < INT_MAX ? s_pick : s_last);
+        __syncthreads();
+        if (warp == 0) put_lane(a, lane, i, s_pick < INT_MAX ? s_pick : s_last);
         return;
     }
 
-    // ---- the k best
-    uint32_t others[kCtas];
-#pragma unroll
-    for (int c = 0; c < kCtas; ++c) others[c] = *cluster.map_shared_rank(&thread_best[tid], c);
-    uint32_t low = others[0];
-#pragma unroll
-    for (int c = 1; c < kCtas; ++c) low = min(low, others[c]);
+    // ---- the k best, by the cluster's first CTA
+    auto done = [&](int kept, int token) {   // the lane's last CTA puts it together
+        if (warp != 0) return;
+        int last = 0;
+        if (wl == 0) {
+            a.rows[index] = make_int2(kept, token);
+            __threadfence();
+            int reached = 1;
+            while (reached <= n_drafts && is_draft(drafts[reached - 1], vocab)) ++reached;
+            last = atomicAdd(a.counters + lane, 1) == reached - 1;
+            __threadfence();
+        }
+        if (!__shfl_sync(0xffffffffu, last, 0)) return;
+        const int2* results = a.rows + (index - i);
+        int end = 0;
+        int2 r = __ldcg(results);
+        while (end < n_drafts && r.x != 0) r = __ldcg(results + ++end);   // a row behind the last draft keeps nothing
+        put_lane(a, lane, end, r.y);
+    };
+    const int n_groups = a.runs * kScan, vpt = a.vpt;
+    uint32_t* group_best = reinterpret_cast<uint32_t*>(smem);
+    uint16_t* group_list = reinterpret_cast<uint16_t*>(smem + a.list_at);
+    uint64_t* keys = reinterpret_cast<uint64_t*>(smem + a.keys_at);
+    if (warp == 0) {
+        const RowSum s = sum_runs(runs + (int64_t)i * a.runs, a.runs, per_t, false);
+        if (wl == 0) {
+            s_best = s.best;
+            s_bad = s.bad;
+        }
+    }
+    uint32_t low = 0xFFFFFFFFu;
+    for (int j = tid; j < n_groups; j += kThreads) {
+        const uint32_t b = a.group_best[(int64_t)index * n_groups + j];
+        group_best[j] = b;
+        low = min(low, b);
+    }
     low = __reduce_min_sync(0xffffffffu, low);
     if (wl == 0) warp_low[warp] = low;
     __syncthreads();
+    if (s_bad) {
+        if (tid == 0) tell(a.status, kDevBadRow);
+        done(0, -1);
+        return;
+    }
+    const uint64_t best = s_best;
+    const float top = value_of_key(best);
+    const double kept_below = d >= 0 ? (double)u[i] * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) low = min(low, warp_low[w]);
-    // low: at least k threads' best reach it (at first: all); twice, 256 steps between it and the next bound
+    // low: at least k groups' best reach it (where there are fewer groups: all); twice, 256 steps between it and the next bound
     uint32_t high = (uint32_t)(best >> 32);
-    int wanted = k;
+    int wanted = min(k, n_groups);
     for (int round = 0; round < 2; ++round) {
         const int bits = max(0, 24 - __clz(high - low));   // the range is less than 256 steps of 2^bits
         if (tid < 256) hist[tid] = 0;
         __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kCtas; ++c)
-            if (others[c] >= low && others[c] <= high) atomicAdd(&hist[(others[c] - low) >> bits], 1);
+        for (int j = tid; j < n_groups; j += kThreads) {
+            const uint32_t b = group_best[j];
+            if (b >= low && b <= high) atomicAdd(&hist[(b - low) >> bits], 1);
+        }
         __syncthreads();
         if (warp == 0) {   // a lane has eight steps, the first lane the highest
             int c[8], sum = 0;
@@ -463,76 +514,63 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
                 const int other = __shfl_up_sync(0xffffffffu, incl, o);
                 if (wl >= o) incl += other;
             }
-            int over = incl - sum;   // threads above the lane's steps
+            int over = incl - sum;   // groups above the lane's steps
             if (over < wanted && incl >= wanted) {
-                int at = 255 - wl * 8;
+                int step = 255 - wl * 8, in = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (over + c[j] >= wanted) break;
-                    over += c[j];
-                    --at;
+                    in = c[j];
+                    if (over + in >= wanted) break;
+                    over += in;
+                    --step;
                 }
-                s_step = make_int2(at, over);
+                s_step = make_int4(step, over, in, 0);
             }
         }
         __syncthreads();
-        const int2 step = s_step;
+        const int4 step = s_step;
         wanted -= step.y;
         low += (uint32_t)step.x << bits;
         high = min(high, low + ((1u << bits) - 1u));
-        if (bits == 0) break;
+        if (bits == 0 || step.z - wanted < 64) break;   // few more than wanted reach it
         __syncthreads();
     }
-    // tokens that reach a bound, listed by their places; at least k reach `enough`, fewer reach `few`
+    if (k > n_groups) low = 0;
+    // tokens that reach a bound; at least k reach `enough`, fewer reach `few`
+    const Row<T> row(x, vocab);
+    constexpr int EPV = Row<T>::EPV;
     uint64_t enough = (uint64_t)low << 32, few = best + 1, bound = enough;
-    int n_all, turn = 0;
-    for (;; ++turn) {
+    int n_all;
+    for (;;) {
         const uint32_t bound_value = (uint32_t)(bound >> 32);
-        for (int v = tid; v < vecs; v += kThreads) {
+        for (int j = tid; j < n_groups; j += kThreads)
+            if (group_best[j] >= bound_value) group_list[atomicAdd(&s_groups, 1)] = (uint16_t)j;
+        __syncthreads();
+        const int pieces = s_groups * vpt;
+        for (int w = tid; w < pieces; w += kThreads) {
+            const int g = group_list[w / vpt], v = (g / kScan * vpt + w % vpt) * kScan + g % kScan, t0 = row.token(v);
             float f[EPV];
-            unpack(buf[v], f, static_cast<const T*>(nullptr));
+            row.load(v, f);
 #pragma unroll
             for (int j = 0; j < EPV; ++j) {
-                if (f32_order_key(f[j] + 0.0f) < bound_value) continue;
-                const int t = token0 + v * EPV + j;
-                if (key_of(f[j], t) < bound || t < n0 || t >= n0 + n) continue;
+                if (f32_order_key(f[j] + 0.0f) < bound_value || t0 + j < 0 || t0 + j >= vocab) continue;
+                const uint64_t key = key_of(f[j], t0 + j);
+                if (key < bound) continue;
                 const int at = atomicAdd(&s_count, 1);
-                if (at < kCandidates) list[at] = (uint16_t)(v * EPV + j);
+                if (at < kCandidates) keys[at] = key;
             }
         }
         __syncthreads();
-        if (tid < kCtas) *cluster.map_shared_rank(&count_of[turn & 1][rank], tid) = s_count;
-        cluster.sync();
-        n_all = 0;
-#pragma unroll
-        for (int c = 0; c < kCtas; ++c) n_all += count_of[turn & 1][c];
+        n_all = s_count;
         if (n_all >= k && n_all <= kCandidates) break;
         if (n_all >= k) enough = bound;
         else few = bound;
         bound = enough + (few - enough) / 2;   // keys differ, and kCandidates > k: it ends
-        if (tid == 0) s_count = 0;
+        __syncthreads();
+        if (tid == 0) s_count = s_groups = 0;
         __syncthreads();
     }
-    static_assert(kCandidates > kVerifyMaxTopK && kCandidates % kThreads == 0, "more can be sorted than are wanted");
-    // they meet where the first CTA had its tokens
-    const int mine_n = count_of[turn & 1][rank];
-    int first = 0;
-    for (int c = 0; c < rank; ++c) first += count_of[turn & 1][c];
-    uint64_t found[kCandidates / kThreads];
-#pragma unroll
-    for (int c = 0; c < kCandidates / kThreads; ++c)
-        if (tid + c * kThreads < mine_n) {
-            const int at = list[tid + c * kThreads];
-            found[c] = key_of(value_of(reinterpret_cast<const T*>(smem)[at]), token0 + at);
-        }
-    cluster.sync();
-    uint64_t* keys = reinterpret_cast<uint64_t*>(smem);
-    uint64_t* there = cluster.map_shared_rank(keys, 0);
-#pragma unroll
-    for (int c = 0; c < kCandidates / kThreads; ++c)
-        if (tid + c * kThreads < mine_n) there[first + tid + c * kThreads] = found[c];
-    cluster.sync();
-    if (rank != 0) return;
+    static_assert(kCandidates > kVerifyMaxTopK, "more can be sorted than are wanted");
     const double* shares;   // of the kept candidates in the order of tokens, and those
     const int* tokens;
     double* values = reinterpret_cast<double*>(keys + kCandidates);
@@ -576,7 +614,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         values[tid] = 0.0;
         __syncthreads();
         if (d >= 0 && kept_below < s_pd) {
-            if (tid == 0) *out = make_int2(1, -1);
+            done(1, -1);
             return;
         }
         if (tid < n_all) {
@@ -614,7 +652,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         }
         __syncthreads();
         if (d >= 0 && kept_below < s_pd) {
-            if (tid == 0) *out = make_int2(1, -1);
+            done(1, -1);
             return;
         }
         sort_desc(keys, k);   // by token; at most kVerifyMaxTopK, the weights lie behind
@@ -663,35 +701,70 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         atomicMax(&s_last, token[1]);
     }
     __syncthreads();
-    if (tid == 0) *out = make_int2(0, s_pick < INT_MAX ? s_pick : s_last);
-}
-
-__global__ void __launch_bounds__(128) verify_lanes_kernel(const __grid_constant__ VerifyArgs a) {
-    const int lane = blockIdx.x * 4 + (threadIdx.x >> 5), t = threadIdx.x & 31, n = a.n_drafts;
-    pdl_wait();
-    if (lane >= a.lanes) return;
-    const int32_t* drafts = a.drafts + (int64_t)lane * n;
-    const int2* rows = a.rows + (int64_t)lane * (n + 1);
-    int32_t* tokens = a.tokens + (int64_t)lane * (n + 1);
-    int end = 0;   // the lane's first row that ends it
-    for (;; ++end)
-        if (end == n || drafts[end] < 0 || drafts[end] >= a.vocab || rows[end].x == 0) break;
-    for (int i = t; i <= n; i += 32) tokens[i] = i < end ? drafts[i] : (i == end ? rows[end].y : -1);
-    if (t == 0) a.accepted[lane] = end;
+    done(0, s_pick < INT_MAX ? s_pick : s_last);
 }
 
 }  // namespace
 
-void launch_verify_drafts(VerifyArgs a, cudaStream_t s) {
+VerifyPlan verify_plan(int type, int lanes, int n_drafts, int vocab) {
+    // Threads' runs short enough that a row has about four times as many as candidates are ever wanted, and not longer than 32 tokens (registers).
+    VerifyPlan p;
+    const int per_piece = type == 0 ? 4 : 8, most = 32 / per_piece;
+    const int64_t pieces = ((int64_t)vocab + per_piece - 1 + per_piece - 1) / per_piece;   // with a first one that is shared with what is in front of the row
+    while (p.vpt < most && pieces > (int64_t)p.vpt * 4096) p.vpt *= 2;
+    p.runs = (int)((pieces + kScan * p.vpt - 1) / (kScan * p.vpt));
+    const int64_t rows = (int64_t)lanes * (n_drafts + 1);
+    p.results_at = (rows * p.runs * kScan * 4 + 255) / 256 * 256;
+    p.rows_at = p.results_at + rows * p.runs * (int64_t)sizeof(Run);
+    p.counters_at = p.rows_at + rows * 8;
+    p.bytes = p.counters_at + (int64_t)lanes * 4;
+    return p;
+}
+
+void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace, cudaStream_t s) {
     if (a.lanes <= 0) return;
-    const int size = a.type == 0 ? 4 : 2, chunk = ((a.vocab + kCtas - 1) / kCtas + 7) / 8 * 8;
-    a.list_at = std::max(chunk * size + 32, kCandidates * 8 + kThreads * 12);   // where candidates meet
-    const size_t smem = (size_t)a.list_at + kCandidates * 2;
-    auto* kernel = a.type == 0 ? verify_rows_kernel<float> : (a.type == 1 ? verify_rows_kernel<__half> : verify_rows_kernel<__nv_bfloat16>);
-    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-    kernel<<<(unsigned)(a.lanes * (a.n_drafts + 1) * kCtas), kThreads, smem, s>>>(a, chunk);
-    MK_LAUNCH_CHECK();
-    launch_pdl(verify_lanes_kernel, dim3((unsigned)((a.lanes + 3) / 4)), dim3(128), 0, s, a);
+    a.vpt = p.vpt;
+    a.runs = p.runs;
+    a.group_best = reinterpret_cast<uint32_t*>(workspace);
+    a.run_results = workspace + p.results_at;
+    a.rows = reinterpret_cast<int2*>(workspace + p.rows_at);
+    a.counters = reinterpret_cast<int32_t*>(workspace + p.counters_at);
+    const unsigned rows = (unsigned)(a.lanes * (a.n_drafts + 1));
+    auto scan = [&](auto* kernel) {
+        kernel<<<rows * (unsigned)p.runs, kScan, 0, s>>>(a);
+        MK_LAUNCH_CHECK();
+    };
+    auto finish = [&](auto* kernel) {
+        const int groups = p.runs * kScan;
+        a.list_at = groups * 4;
+        a.keys_at = (a.list_at + groups * 2 + 15) / 16 * 16;
+        const size_t smem = (size_t)a.keys_at + kCandidates * 8 + kThreads * 12;
+        ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+        launch_pdl(kernel, dim3(rows * kCtas), dim3(kThreads), smem, s, a);
+    };
+    if (a.type == 0) {
+        switch (p.vpt) {
+            case 1: scan(scan_rows_kernel<float, 1>); break;
+            case 2: scan(scan_rows_kernel<float, 2>); break;
+            case 4: scan(scan_rows_kernel<float, 4>); break;
+            default: scan(scan_rows_kernel<float, 8>);
+        }
+        finish(finish_rows_kernel<float>);
+    } else if (a.type == 1) {
+        switch (p.vpt) {
+            case 1: scan(scan_rows_kernel<__half, 1>); break;
+            case 2: scan(scan_rows_kernel<__half, 2>); break;
+            default: scan(scan_rows_kernel<__half, 4>);
+        }
+        finish(finish_rows_kernel<__half>);
+    } else {
+        switch (p.vpt) {
+            case 1: scan(scan_rows_kernel<__nv_bfloat16, 1>); break;
+            case 2: scan(scan_rows_kernel<__nv_bfloat16, 2>); break;
+            default: scan(scan_rows_kernel<__nv_bfloat16, 4>);
+        }
+        finish(finish_rows_kernel<__nv_bfloat16>);
+    }
 }
 
 }  // namespace mk

@@ -6,7 +6,7 @@ namespace mk {
 
 constexpr int kDevBadRow = 8;     // a row of logits without a distribution (NaN, +inf or nothing above -inf); bits 1 to 4 in shared_attention.h
 constexpr int kVerifyMaxTopK = 1024;
-constexpr int kVerifyMaxVocab = 8 * 52000;   // eight CTAs' shared memory at 32 bits a value
+constexpr int kVerifyMaxVocab = 416000;   // the best values of a row's threads fit shared memory, 32 tokens a thread
 
 struct VerifyArgs {
     const void* logits = nullptr;      // [lanes][drafts + 1] rows of vocab values, ld values apart
@@ -21,11 +21,21 @@ struct VerifyArgs {
     const float* top_p = nullptr;      // [lanes]
     int32_t* tokens = nullptr;         // [lanes][n_drafts + 1]
     int32_t* accepted = nullptr;       // [lanes]
-    int2* rows = nullptr;              // scratch [lanes][n_drafts + 1]: (draft accepted, token drawn in its place)
     int32_t* status = nullptr;
-    int list_at = 0;                   // filled in by the launcher: where a CTA's list of candidates begins in its shared memory
+    // filled in by the launcher
+    uint32_t* group_best = nullptr;    // [rows][runs][256] best value of each thread's tokens, as an order key
+    void* run_results = nullptr;       // [rows][runs]
+    int2* rows = nullptr;              // (draft kept, token drawn in its place)
+    int32_t* counters = nullptr;       // [lanes]
+    int vpt = 0, runs = 0, list_at = 0, keys_at = 0;
 };
-inline int64_t verify_scratch_bytes(int lanes, int n_drafts) { return (int64_t)lanes * (n_drafts + 1) * 8; }
-void launch_verify_drafts(VerifyArgs a, cudaStream_t s);
+
+// How a call is cut, and its workspace.
+struct VerifyPlan {
+    int vpt = 1, runs = 0;             // pieces of 16 bytes to a thread; runs of tokens, a CTA each, to a row
+    int64_t results_at = 0, rows_at = 0, counters_at = 0, bytes = 0;
+};
+VerifyPlan verify_plan(int type, int lanes, int n_drafts, int vocab);
+void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace, cudaStream_t s);
 
 }  // namespace mk

@@ -126,9 +126,14 @@ def verify_drafts(logits, drafts, u, *, temperature, top_k, top_p, draft_probs=N
         tokens = torch.empty((lanes, n + 1), dtype=torch.int32, device=device)
     if accepted is None:
         accepted = torch.empty((lanes,), dtype=torch.int32, device=device)
-    size = 8 * lanes * (n + 1)
+    need = C.c_int64()
+    lib = capi.lib()
+    code = lib.mk_k_verify_drafts_workspace(_TYPES[logits.dtype], lanes, n, vocab, C.byref(need))
+    if code:
+        capi.check(code)
+    size = need.value
     space = torch.empty(size, dtype=torch.uint8, device=device)
-    _call(device, capi.lib().mk_k_verify_drafts_dev, _TYPES[logits.dtype], logits.data_ptr(), ld, lanes, n, vocab, _dense(drafts, torch.int32, (lanes, n), device, "drafts"),
+    _call(device, lib.mk_k_verify_drafts_dev, _TYPES[logits.dtype], logits.data_ptr(), ld, lanes, n, vocab, _dense(drafts, torch.int32, (lanes, n), device, "drafts"),
           None if draft_probs is None else _dense(draft_probs, torch.float32, (lanes, n, vocab), device, "draft_probs"), _dense(u, torch.float32, (lanes, n + 1), device, "u"),
           _dense(temperature, torch.float32, (lanes,), device, "temperature"), _dense(top_k, torch.int32, (lanes,), device, "top_k"),
           _dense(top_p, torch.float32, (lanes,), device, "top_p"), _dense(tokens, torch.int32, (lanes, n + 1), device, "tokens"),

@@ -87,7 +87,7 @@ def test_the_workspace_covers_every_size(capi):
 
 
 VERIFY = dict(type=0, logits=A, stride=1000, lanes=3, drafts=4, vocab=1000, drafts_=A, probs=None, u=A, temperature=A, top_k=A, top_p=A, tokens=A, accepted=A, workspace=A,
-              workspace_bytes=1 << 20, status=None, stream=None)
+              workspace_bytes=1 << 24, status=None, stream=None)
 
 
 @pytest.mark.parametrize("change, message", [
@@ -96,6 +96,7 @@ VERIFY = dict(type=0, logits=A, stride=1000, lanes=3, drafts=4, vocab=1000, draf
     (dict(stride=999), "rows overlap"),
     (dict(lanes=-1), "negative sizes"),
     (dict(lanes=1 << 26), "too many rows"),
+    (dict(drafts=2 ** 31 - 1), "too many rows"),
     (dict(vocab=416001, stride=416001), "at most 416000"),
     (dict(logits=A + 2), "aligned"),
     (dict(drafts_=None), "null pointer"),
