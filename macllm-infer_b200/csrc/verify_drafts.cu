@@ -8,10 +8,10 @@
 //
 // Two kernels.  The first streams every row that can be reached once, a run of tokens to a CTA and at most 32 of them to a thread, and leaves what a run amounts
 // to: its best token, whether it holds what is no logit, the sum of its weights (whole vocabulary), and the best value of each thread's tokens (top_k).  What bounds it is HBM.
-// The second finishes rows, eight CTAs in a cluster to each.  Over the whole vocabulary a row's sum follows from its runs', so each cluster judges the rows in front
-// of its own too, and only the one whose row ends the lane goes through its row again, for the draw.  With a top_k the first CTA takes
-// candidates: the k-th best of the threads' best values is a bound that at least k tokens reach and few more do, and only the tokens of threads that reach it are read again;
-// where too many reach it (thousands of equal logits) bisection over (value, token) finds one that fewer do.  The CTA that ends last among a lane's rows puts the lane together.
+// The second finishes lanes, eight CTAs in a cluster to each.  Over the whole vocabulary a row's sum follows from its runs', which tells where the lane ends, and
+// the cluster goes through that one row again, for the draw.  With a top_k each CTA takes every eighth row: the k-th best of the threads' best values is a bound that at
+// least k tokens reach and few more do, and only the tokens of threads that reach it are read again; where too many reach it (thousands of equal
+// logits) bisection over (value, token) finds one that fewer do.
 //
 // Weights and sums of candidates are 64-bit.  Over the whole vocabulary a weight is a 32-bit number (ex2 of a product kept to twice 32 bits: 2^-22, and with no trend, so that
 // sums over many are better) and sums are 64-bit.
@@ -189,7 +189,6 @@ __global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant_
     const int k = a.top_k[lane];
     bool gone = false;
     for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
-    if (i == 0 && run == 0 && tid == 0) a.counters[lane] = 0;
     if (__any_sync(0xffffffffu, gone)) return;   // nothing gets here
     const Row<T> row(static_cast<const T*>(a.logits) + index * a.ld, vocab);
     float f[VPT][EPV];
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant_
             if (f[c][j] == top) at = row.token((run * VPT + c) * kScan + tid) + j;
     if (top == -INFINITY) at = vocab;
     uint64_t best = key_of(top, at);
-    if (temperature > 0.f && k > 0) a.group_best[((int64_t)index * a.runs + run) * kScan + tid] = (uint32_t)(best >> 32);
+    if (temperature > 0.f && k > 0) a.group_best[((int64_t)index * a.runs + run) * kScan + tid] = top;
     bad = __syncthreads_or(bad);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -285,347 +284,222 @@ __device__ __forceinline__ void put_lane(const VerifyArgs& a, int lane, int end,
     if ((threadIdx.x & 31) == 0) a.accepted[lane] = end;
 }
 
-template <typename T>
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish_rows_kernel(const __grid_constant__ VerifyArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ double sum_of[2][kCtas], red[kWarps], region[kWarps], s_pd, s_z;
-    __shared__ uint64_t s_best;
-    __shared__ uint32_t warp_low[kWarps];
-    __shared__ int s_count, s_groups, s_pick, s_last, s_reached, s_bad, s_kept, hist[256];
-    __shared__ int4 s_step;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), index = blockIdx.x / kCtas;
-    const int n_drafts = a.n_drafts, lane = index / (n_drafts + 1), i = index - lane * (n_drafts + 1), vocab = a.vocab;
-    const int32_t* drafts = a.drafts + (int64_t)lane * n_drafts;
-    const float* u = a.u + (int64_t)lane * (n_drafts + 1);
-    const float temperature = a.temperature[lane], top_p = a.top_p[lane];
-    int k = a.top_k[lane];
-    const bool whole = temperature > 0.f && k <= 0;
-    if (rank != 0 && !whole) return;
-    bool gone = false;
-    for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
-    if (__any_sync(0xffffffffu, gone)) return;
-    int d = i < n_drafts ? drafts[i] : -1;
-    const double u_draw = (double)u[n_drafts], per_t = temperature > 0.f ? 1.0 / (double)temperature : 0.0;
-    const T* x = static_cast<const T*>(a.logits) + index * a.ld;
-    if (rank == 0 && tid == 0 && (d >= vocab || (temperature > 0.f && (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f))))) tell(a.status, kDevBadRange);
-    if (!is_draft(d, vocab)) d = -1;
-    k = min(min(k, kVerifyMaxTopK), vocab);
-    const float* probs = a.draft_probs == nullptr ? nullptr : a.draft_probs + (int64_t)lane * n_drafts * vocab;
-    const float* q = probs == nullptr || d < 0 ? nullptr : probs + (int64_t)i * vocab;
-    if (tid == 0) {
-        s_count = s_groups = 0;
-        s_pick = INT_MAX;
-        s_last = -1;
-        s_reached = 1;
-        s_pd = 0.0;
-    }
+// A place in a list for each thread of a warp that wants one.
+__device__ __forceinline__ int list_place(int* count, bool wants) {
+    const unsigned who = __ballot_sync(0xffffffffu, wants);
+    if (who == 0) return 0;
+    const int wl = threadIdx.x & 31, first = __ffs(who) - 1;
+    int at = 0;
+    if (wl == first) at = atomicAdd(count, __popc(who));
+    return __shfl_sync(0xffffffffu, at, first) + __popc(who & ((1u << wl) - 1u));
+}
+// Sum over the block, the same in every thread.
+__device__ unsigned long long block_sum(unsigned long long v, unsigned long long* red) {
+    const int wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
-    pdl_wait();
-    const Run* runs = static_cast<const Run*>(a.run_results) + (int64_t)(index - i) * a.runs;   // of the lane
+    if (wl == 0) red[warp] = v;
+    __syncthreads();
+    v = red[wl % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
-    if (!(temperature > 0.f) || whole) {
-        // ---- rows that their runs tell all of: this one and those in front of it
-        for (int j = warp; j <= i; j += kWarps) {
-            const RowSum s = sum_runs(runs + (int64_t)j * a.runs, a.runs, per_t, whole);
-            const int dj = j < i ? drafts[j] : d;
-            bool kept = false;
-            if (dj >= 0 && !s.bad) {
-                if (whole) {
-                    const double qd = probs != nullptr ? (double)probs[(int64_t)j * vocab + dj] : 1.0;
-                    const double xd = (double)value_of(x[(int64_t)(j - i) * a.ld + dj]);
-                    kept = (double)u[j] * qd < exp((xd - (double)value_of_key(s.best)) * per_t) / s.z;
-                } else {
-                    kept = dj == (int)rank_key_index(s.best);
-                }
-            }
-            if (j < i && !kept) s_reached = 0;
-            if (j == i && wl == 0) {
-                s_best = s.best;
-                s_z = s.z;
-                s_bad = s.bad;
-                s_kept = kept;
-            }
-        }
-        __syncthreads();
-        if (!s_reached || s_kept) return;
-        if (s_bad || !whole) {
-            if (rank != 0 || warp != 0) return;
-            if (s_bad && wl == 0) tell(a.status, kDevBadRow);
-            put_lane(a, lane, i, s_bad ? -1 : (int)rank_key_index(s_best));
-            return;
-        }
-        // ---- the draw: every warp adds up a run of its own, and a CTA looks through the one where the target lies
-        const double z = s_z;
-        const Exponential weight(value_of_key(s_best), temperature);
-        const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
-        const int chunk = (vocab + kCtas - 1) / kCtas, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
-        const int run = (n1 - n0 + kWarps - 1) / kWarps, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
-        bool rest = d >= 0;
-        auto share = [&](float logit, float qt) {
-            const float w = weight(logit);
-            return rest ? fmaxf(fmaf(w, per_z, -qt) + w * per_z_rest, 0.f) : w;
-        };
-        auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
-        double total = 0.0, *sums = sum_of[0];
-        for (;;) {
-            constexpr int AHEAD = 8;
-            double part = 0.0;
-            for (int t0 = r_lo + wl; t0 < r_hi; t0 += 32 * AHEAD) {
-                float l[AHEAD], qv[AHEAD], s = 0.f;
-#pragma unroll
-                for (int c = 0; c < AHEAD; ++c) {
-                    const int t = t0 + 32 * c;
-                    l[c] = t < r_hi ? value_of(x[t]) : -INFINITY;
-                    qv[c] = t < r_hi ? q_at(t) : 0.f;
-                }
-#pragma unroll
-                for (int c = 0; c < AHEAD; ++c) s += share(l[c], qv[c]);
-                part += (double)s;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-            if (wl == 0) region[warp] = part;
-            __syncthreads();
-            if (warp == 0) {
-                double s = region[wl % kWarps];
-#pragma unroll
-                for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (wl < kCtas) *cluster.map_shared_rank(sums + rank, wl) = s;
-            }
-            cluster.sync();
-            total = 0.0;
-#pragma unroll
-            for (int c = 0; c < kCtas; ++c) total += sums[c];
-            if (total > 0.0 || !rest) break;
-            rest = false;   // the draft's distribution covers the target's
-            sums = sum_of[1];
-        }
-        const double target = u_draw * total;
-        // the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
-        double upto = 0.0;
-        int at = -1;
-#pragma unroll
-        for (int c = 0; c < kCtas; ++c) {
-            if (upto > target) break;
-            if (sums[c] > 0.0) at = c;
-            upto += sums[c];
-        }
-        if (at != rank) return;
-        upto = 0.0;
-        for (int c = 0; c < rank; ++c) upto += sums[c];
-        int w_at = 0;
-        double before = upto;
-        for (int w = 0; w < kWarps; ++w) {
-            if (region[w] > 0.0) {
-                w_at = w;
-                before = upto;
-            }
-            upto += region[w];
-            if (upto > target) break;
-        }
-        const int at_lo = min(n1, n0 + w_at * run), at_hi = min(n1, at_lo + run);
-        for (int t0 = at_lo; t0 < at_hi; t0 += kThreads) {
-            const int t = t0 + tid;
-            const double r = t < at_hi ? (double)share(value_of(x[t]), q_at(t)) : 0.0;
-            double all;
-            const double c = before + block_scan(r, red, &all);
-            if (r > 0.0) {
-                atomicMax(&s_last, t);
-                if (c > target) atomicMin(&s_pick, t);
-            }
-            before += all;
-            __syncthreads();
-            if (s_pick < INT_MAX) break;
-        }
-        __syncthreads();
-        if (warp == 0) put_lane(a, lane, i, s_pick < INT_MAX ? s_pick : s_last);
-        return;
-    }
+struct TopShared {
+    double red[kWarps], pd;
+    uint64_t best;
+    float warp_low[kWarps];
+    int warp_live[kWarps];
+    int count, groups, pick, last, bad, hist[256];
+    int2 step;
+};
 
-    // ---- the k best, by the cluster's first CTA
-    auto done = [&](int kept, int token) {   // the lane's last CTA puts it together
-        if (warp != 0) return;
-        int last = 0;
-        if (wl == 0) {
-            a.rows[index] = make_int2(kept, token);
-            __threadfence();
-            int reached = 1;
-            while (reached <= n_drafts && is_draft(drafts[reached - 1], vocab)) ++reached;
-            last = atomicAdd(a.counters + lane, 1) == reached - 1;
-            __threadfence();
-        }
-        if (!__shfl_sync(0xffffffffu, last, 0)) return;
-        const int2* results = a.rows + (index - i);
-        int end = 0;
-        int2 r = __ldcg(results);
-        while (end < n_drafts && r.x != 0) r = __ldcg(results + ++end);   // a row behind the last draft keeps nothing
-        put_lane(a, lane, end, r.y);
-    };
-    const int n_groups = a.runs * kScan, vpt = a.vpt;
-    uint32_t* group_best = reinterpret_cast<uint32_t*>(smem);
+// One row with a top_k, by a CTA: (draft kept, token drawn in its place).
+template <typename T>
+__device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem, int lane, int i, int d, int k, float temperature, float top_p, double u_keep, double u_draw) {
+    constexpr int EPV = Row<T>::EPV;
+    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, vocab = a.vocab, index = lane * (a.n_drafts + 1) + i, n_groups = a.runs * kScan, vpt = a.vpt;
+    const double per_t = 1.0 / (double)temperature;
+    const Row<T> row(static_cast<const T*>(a.logits) + index * a.ld, vocab);
+    const float* q = a.draft_probs == nullptr || d < 0 ? nullptr : a.draft_probs + ((int64_t)lane * a.n_drafts + i) * vocab;
+    const double kept_below = d >= 0 ? u_keep * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
+    float* group_best = reinterpret_cast<float*>(smem);
     uint16_t* group_list = reinterpret_cast<uint16_t*>(smem + a.list_at);
     uint64_t* keys = reinterpret_cast<uint64_t*>(smem + a.keys_at);
+    __syncthreads();   // the row before is done with
+    if (tid == 0) {
+        s.count = s.groups = 0;
+        s.pick = INT_MAX;
+        s.last = -1;
+        s.pd = 0.0;
+    }
+    if (tid < 256) s.hist[tid] = 0;
     if (warp == 0) {
-        const RowSum s = sum_runs(runs + (int64_t)i * a.runs, a.runs, per_t, false);
+        const RowSum r = sum_runs(static_cast<const Run*>(a.run_results) + (int64_t)index * a.runs, a.runs, per_t, false);
         if (wl == 0) {
-            s_best = s.best;
-            s_bad = s.bad;
+            s.best = r.best;
+            s.bad = r.bad;
+            s.step = make_int2(-1, 0);
         }
     }
-    uint32_t low = 0xFFFFFFFFu;
+    float low = INFINITY;
     for (int j = tid; j < n_groups; j += kThreads) {
-        const uint32_t b = a.group_best[(int64_t)index * n_groups + j];
+        const float b = a.group_best[(int64_t)index * n_groups + j];
         group_best[j] = b;
-        low = min(low, b);
+        if (b > -INFINITY) low = fminf(low, b);
     }
-    low = __reduce_min_sync(0xffffffffu, low);
-    if (wl == 0) warp_low[warp] = low;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    if (wl == 0) s.warp_low[warp] = low;
     __syncthreads();
-    if (s_bad) {
+    if (s.bad) {
         if (tid == 0) tell(a.status, kDevBadRow);
-        done(0, -1);
-        return;
+        return make_int2(0, -1);
     }
-    const uint64_t best = s_best;
+    const uint64_t best = s.best;
     const float top = value_of_key(best);
-    const double kept_below = d >= 0 ? (double)u[i] * (q != nullptr ? (double)q[d] : 1.0) : 0.0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) low = min(low, warp_low[w]);
-    // low: at least k groups' best reach it (where there are fewer groups: all); twice, 256 steps between it and the next bound
-    uint32_t high = (uint32_t)(best >> 32);
-    int wanted = min(k, n_groups);
-    for (int round = 0; round < 2; ++round) {
-        const int bits = max(0, 24 - __clz(high - low));   // the range is less than 256 steps of 2^bits
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < n_groups; j += kThreads) {
-            const uint32_t b = group_best[j];
-            if (b >= low && b <= high) atomicAdd(&hist[(b - low) >> bits], 1);
-        }
-        __syncthreads();
-        if (warp == 0) {   // a lane has eight steps, the first lane the highest
-            int c[8], sum = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += c[j] = hist[255 - wl * 8 - j];
-            int incl = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, incl, o);
-                if (wl >= o) incl += other;
-            }
-            int over = incl - sum;   // groups above the lane's steps
-            if (over < wanted && incl >= wanted) {
-                int step = 255 - wl * 8, in = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    in = c[j];
-                    if (over + in >= wanted) break;
-                    over += in;
-                    --step;
-                }
-                s_step = make_int4(step, over, in, 0);
-            }
-        }
-        __syncthreads();
-        const int4 step = s_step;
-        wanted -= step.y;
-        low += (uint32_t)step.x << bits;
-        high = min(high, low + ((1u << bits) - 1u));
-        if (bits == 0 || step.z - wanted < 64) break;   // few more than wanted reach it
-        __syncthreads();
+    for (int w = 0; w < kWarps; ++w) low = fminf(low, s.warp_low[w]);
+    // 256 steps of value between the groups' lowest and highest; the highest step with which at least k groups' best are counted.  Its lower end, moved down by more than
+    // the roundings on the way, is a bound that at least k tokens reach.
+    const float range = top - low, per_step = range > 0.f && range < INFINITY ? 256.f / range : 0.f;
+    for (int j = tid; j < n_groups; j += kThreads) {
+        const float b = group_best[j];
+        if (b > -INFINITY) atomicAdd(&s.hist[min(255, (int)((b - low) * per_step))], 1);
     }
-    if (k > n_groups) low = 0;
+    __syncthreads();
+    if (warp == 0) {   // a lane has eight steps, the first lane the highest
+        int c[8], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += c[j] = s.hist[255 - wl * 8 - j];
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, incl, o);
+            if (wl >= o) incl += other;
+        }
+        int over = incl - sum;   // groups above the lane's steps
+        if (over < k && incl >= k) {
+            int step = 255 - wl * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                over += c[j];
+                if (over >= k) break;
+                --step;
+            }
+            s.step = make_int2(step, over);
+        }
+    }
+    __syncthreads();
     // tokens that reach a bound; at least k reach `enough`, fewer reach `few`
-    const Row<T> row(x, vocab);
-    constexpr int EPV = Row<T>::EPV;
-    uint64_t enough = (uint64_t)low << 32, few = best + 1, bound = enough;
+    const float bound_low = s.step.x < 0 || per_step == 0.f ? (s.step.x < 0 ? -INFINITY : low) : low + (float)s.step.x / per_step - range * 1e-5f;
+    uint64_t enough = (uint64_t)f32_order_key(bound_low + 0.0f) << 32, few = best + 1, bound = enough;
     int n_all;
     for (;;) {
-        const uint32_t bound_value = (uint32_t)(bound >> 32);
-        for (int j = tid; j < n_groups; j += kThreads)
-            if (group_best[j] >= bound_value) group_list[atomicAdd(&s_groups, 1)] = (uint16_t)j;
+        const float bound_value = value_of_key(bound);
+        for (int j0 = 0; j0 < n_groups; j0 += kThreads) {   // n_groups is a multiple of 256: whole warps
+            const int j = j0 + tid;
+            const bool reaches = j < n_groups && group_best[j] >= bound_value;
+            const int at = list_place(&s.groups, reaches);
+            if (reaches) group_list[at] = (uint16_t)j;
+        }
         __syncthreads();
-        const int pieces = s_groups * vpt;
-        for (int w = tid; w < pieces; w += kThreads) {
-            const int g = group_list[w / vpt], v = (g / kScan * vpt + w % vpt) * kScan + g % kScan, t0 = row.token(v);
+        const int pieces = s.groups * vpt;
+        for (int w0 = 0; w0 < pieces; w0 += kThreads) {
+            const int w = w0 + tid;
             float f[EPV];
-            row.load(v, f);
+            int t0 = 0;
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) f[j] = -INFINITY;
+            if (w < pieces) {
+                const int g = group_list[w / vpt], v = (g / kScan * vpt + w % vpt) * kScan + g % kScan;
+                t0 = row.token(v);
+                row.load(v, f);
+            }
+            float highest = f[0];
+#pragma unroll
+            for (int j = 1; j < EPV; ++j) highest = fmaxf(highest, f[j]);
+            if (!__any_sync(0xffffffffu, w < pieces && highest >= bound_value)) continue;
 #pragma unroll
             for (int j = 0; j < EPV; ++j) {
-                if (f32_order_key(f[j] + 0.0f) < bound_value || t0 + j < 0 || t0 + j >= vocab) continue;
                 const uint64_t key = key_of(f[j], t0 + j);
-                if (key < bound) continue;
-                const int at = atomicAdd(&s_count, 1);
-                if (at < kCandidates) keys[at] = key;
+                const bool reaches = w < pieces && t0 + j >= 0 && t0 + j < vocab && key >= bound;
+                const int at = list_place(&s.count, reaches);
+                if (reaches && at < kCandidates) keys[at] = key;
             }
         }
         __syncthreads();
-        n_all = s_count;
+        n_all = s.count;
         if (n_all >= k && n_all <= kCandidates) break;
         if (n_all >= k) enough = bound;
         else few = bound;
         bound = enough + (few - enough) / 2;   // keys differ, and kCandidates > k: it ends
         __syncthreads();
-        if (tid == 0) s_count = s_groups = 0;
+        if (tid == 0) s.count = s.groups = 0;
         __syncthreads();
     }
     static_assert(kCandidates > kVerifyMaxTopK, "more can be sorted than are wanted");
-    const double* shares;   // of the kept candidates in the order of tokens, and those
-    const int* tokens;
-    double* values = reinterpret_cast<double*>(keys + kCandidates);
-    int* ids = reinterpret_cast<int*>(values + kThreads);
-    int n_last;
     if (n_all <= kThreads) {
-        // A candidate a thread, which counts those before it in either order.
-        const uint64_t key = tid < n_all ? keys[tid] : 0;
-        int rank_by_value = 0, rank_by_token = 0;
-        if (warp * 32 < n_all) {
-            if (tid < 2) keys[n_all + tid] = 0;
-        }
+        // Up to four threads to a candidate, which compares it with every other one: who is better, and how much those weigh; later whose token is lower.  The list's order is not
+        // the same in every call, so sums are of whole numbers of 2^-52.
+        unsigned long long* values = reinterpret_cast<unsigned long long*>(keys + kCandidates);
+        constexpr double kUnits = 4503599627370496.0;
+        const int parts = n_all <= kThreads / 4 ? 4 : (n_all <= kThreads / 2 ? 2 : 1), c = tid / parts, part = tid % parts;
+        const uint64_t key = c < n_all ? keys[c] : 0;
+        const int token = c < n_all ? (int)rank_key_index(key) : -1;
+        const double e = c < n_all ? exp(((double)value_of_key(key) - (double)top) * per_t) : 0.0;
+        const double qt = d >= 0 && c < n_all ? (q != nullptr ? (double)q[token] : (token == d ? 1.0 : 0.0)) : 0.0;
+        const unsigned long long units = __double2ull_rn(e * kUnits);
+        if (part == 0) values[c] = units;
         __syncthreads();
-        if (warp * 32 < n_all)
-            for (int j = 0; j < n_all; j += 2) {
-                const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(keys + j);
-                rank_by_value += (int)(other.x > key) + (int)(other.y > key);
-                rank_by_token += (int)((uint32_t)other.x > (uint32_t)key) + (int)((uint32_t)other.y > (uint32_t)key);
+        int better = 0;
+        unsigned long long before = 0;
+        for (int j = part; j < n_all; j += parts)
+            if (keys[j] > key) {
+                ++better;
+                before += values[j];
             }
-        const bool among = tid < n_all && rank_by_value < k;
-        const double e = among ? exp(((double)value_of_key(key) - (double)top) * per_t) : 0.0;
-        bool in = among;
-        double kept;
+        for (int o = 1; o < parts; o <<= 1) {
+            better += __shfl_xor_sync(0xffffffffu, better, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        bool in = c < n_all && better < k;
+        unsigned long long kept = block_sum(in && part == 0 ? units : 0ull, reinterpret_cast<unsigned long long*>(s.red));
         if (top_p < 1.f) {
-            values[tid] = 0.0;
-            __syncthreads();
-            if (among) values[rank_by_value] = e;
-            __syncthreads();
-            const double mine_e = values[tid];
-            double z;
-            const double upto = block_scan(mine_e, red, &z);
-            values[tid] = upto - mine_e;
-            __syncthreads();
-            in = among && (rank_by_value == 0 || values[rank_by_value] / z < (double)top_p);
-            __syncthreads();
+            in = in && (better == 0 || (double)before < (double)top_p * (double)kept);
+            kept = block_sum(in && part == 0 ? units : 0ull, reinterpret_cast<unsigned long long*>(s.red));
         }
-        const double e_in = in ? e : 0.0;
-        block_scan(e_in, red, &kept);
-        const int token = (int)rank_key_index(key);
-        if (in && token == d) s_pd = e / kept;
-        values[tid] = 0.0;
+        const double p = in ? e * (kUnits / (double)kept) : 0.0;
+        if (in && token == d) s.pd = p;
+        unsigned long long r = __double2ull_rn((d >= 0 && in ? fmax(p - qt, 0.0) : p) * kUnits);
+        if (part == 0) values[c] = r;
         __syncthreads();
-        if (d >= 0 && kept_below < s_pd) {
-            done(1, -1);
-            return;
+        if (d >= 0 && kept_below < s.pd) return make_int2(1, -1);
+        unsigned long long total = block_sum(part == 0 ? r : 0ull, reinterpret_cast<unsigned long long*>(s.red));
+        if (total == 0) {   // the draft's distribution covers the target's
+            r = __double2ull_rn(p * kUnits);
+            if (part == 0) values[c] = r;
+            total = block_sum(part == 0 ? r : 0ull, reinterpret_cast<unsigned long long*>(s.red));
         }
-        if (tid < n_all) {
-            values[rank_by_token] = e_in / kept;
-            ids[rank_by_token] = token;
+        unsigned long long upto = 0;
+        for (int j = part; j < n_all; j += parts)
+            if ((uint32_t)keys[j] >= (uint32_t)key) upto += values[j];   // its token, or a lower one
+        for (int o = 1; o < parts; o <<= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
+        if (r > 0 && part == 0) {
+            if ((double)upto > u_draw * (double)total) atomicMin(&s.pick, token);
+            atomicMax(&s.last, token);
         }
         __syncthreads();
-        shares = values;
-        tokens = ids;
-        n_last = n_all;
-    } else {
+        return make_int2(0, s.pick < INT_MAX ? s.pick : s.last);
+    }
+    // More: sorted, two candidates a thread from then on.
+    const double* shares;
+    const int* tokens;
+    int n_last;
+    {
+        int* ids;
         // two candidates a thread: the head that adds up to top_p
         sort_desc(keys, n_all);
         const int j0 = 2 * tid;
@@ -636,24 +510,23 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
             token[j] = j0 + j < k ? (int)rank_key_index(keys[j0 + j]) : -1;
             e[j] = j0 + j < k ? exp(((double)value_of_key(keys[j0 + j]) - (double)top) * per_t) : 0.0;
         }
-        const double upto_e = block_scan(e[0] + e[1], red, &z);
+        const double upto_e = block_scan(e[0] + e[1], s.red, &z);
         bool in[2] = {j0 < k, j0 + 1 < k};
         if (top_p < 1.f) {
             in[0] = in[0] && (j0 == 0 || (upto_e - e[1] - e[0]) / z < (double)top_p);
             in[1] = in[1] && (upto_e - e[1]) / z < (double)top_p;
         }
-        block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), red, &kept);
+        block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), s.red, &kept);
         double* weights = reinterpret_cast<double*>(keys + kVerifyMaxTopK);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            if (in[j] && token[j] == d) s_pd = e[j] / kept;
+            if (in[j] && token[j] == d) s.pd = e[j] / kept;
             weights[j0 + j] = in[j] ? e[j] / kept : 0.0;
             keys[j0 + j] = j0 + j < k ? (uint64_t)(0xFFFFFFFFu - (uint32_t)token[j]) << 32 | (uint32_t)(j0 + j) : 0;
         }
         __syncthreads();
-        if (d >= 0 && kept_below < s_pd) {
-            done(1, -1);
-            return;
+        if (d >= 0 && kept_below < s.pd) {
+            return make_int2(1, -1);
         }
         sort_desc(keys, k);   // by token; at most kVerifyMaxTopK, the weights lie behind
         double w[2];
@@ -675,7 +548,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
         tokens = ids;
         n_last = k;
     }
-    // the draw, two tokens a thread
+    // the draw
     const int j0 = 2 * tid;
     int token[2];
     double p[2], r[2], total;
@@ -685,23 +558,200 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
         p[j] = r[j] = j0 + j < n_last ? shares[j0 + j] : 0.0;
         if (d >= 0 && p[j] > 0.0) r[j] = fmax(p[j] - (q != nullptr ? (double)q[token[j]] : (token[j] == d ? 1.0 : 0.0)), 0.0);
     }
-    double upto = block_scan(r[0] + r[1], red, &total);
+    double upto = block_scan(r[0] + r[1], s.red, &total);
     if (!(total > 0.0)) {   // the draft's distribution covers the target's
         r[0] = p[0];
         r[1] = p[1];
-        upto = block_scan(r[0] + r[1], red, &total);
+        upto = block_scan(r[0] + r[1], s.red, &total);
     }
     const double target = u_draw * total;
     if (r[0] > 0.0) {
-        if (upto - r[1] > target) atomicMin(&s_pick, token[0]);
-        atomicMax(&s_last, token[0]);
+        if (upto - r[1] > target) atomicMin(&s.pick, token[0]);
+        atomicMax(&s.last, token[0]);
     }
     if (r[1] > 0.0) {
-        if (upto > target) atomicMin(&s_pick, token[1]);
-        atomicMax(&s_last, token[1]);
+        if (upto > target) atomicMin(&s.pick, token[1]);
+        atomicMax(&s.last, token[1]);
     }
     __syncthreads();
-    done(0, s_pick < INT_MAX ? s_pick : s_last);
+    return make_int2(0, s.pick < INT_MAX ? s.pick : s.last);
+}
+
+template <typename T>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_constant__ VerifyArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ TopShared top_shared;
+    __shared__ double sum_of[2][kCtas], region[kWarps], s_z;
+    __shared__ uint64_t s_best;
+    __shared__ int s_end, s_bad, s_pick, s_last;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), lane = blockIdx.x / kCtas, n_drafts = a.n_drafts, vocab = a.vocab;
+    const int32_t* drafts = a.drafts + (int64_t)lane * n_drafts;
+    const float* u = a.u + (int64_t)lane * (n_drafts + 1);
+    const float temperature = a.temperature[lane], top_p = a.top_p[lane];
+    const double u_draw = (double)u[n_drafts];
+    int k = a.top_k[lane];
+    int n = 0;   // drafts in front of the first that is none
+    for (bool more = true; more && n < n_drafts;) {
+        const unsigned none = __ballot_sync(0xffffffffu, n + wl >= n_drafts || !is_draft(drafts[n + wl], vocab));
+        more = none == 0;
+        n = more ? n + 32 : n + __ffs(none) - 1;
+    }
+    const bool hot = temperature > 0.f, whole = hot && k <= 0;
+    if (rank == 0 && tid == 0 && ((n < n_drafts && drafts[n] >= vocab) || (hot && (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f))))) tell(a.status, kDevBadRange);
+    if (rank != 0 && !hot) return;
+    if (tid == 0) {
+        s_end = INT_MAX;
+        s_pick = INT_MAX;
+        s_last = -1;
+    }
+    __syncthreads();
+    pdl_wait();
+    if (hot && !whole) {
+        // ---- rows with a top_k, every eighth one
+        k = min(min(k, kVerifyMaxTopK), vocab);
+        int2* rows = a.rows + (int64_t)lane * (n_drafts + 1);
+        for (int i = rank; i <= n; i += kCtas) {
+            const int2 r = finish_top_row<T>(a, top_shared, smem, lane, i, i < n ? drafts[i] : -1, k, temperature, top_p, (double)u[i], u_draw);
+            if (tid == 0) rows[i] = r;
+        }
+        cluster.sync();
+        if (rank != 0 || warp != 0) return;
+        int end = 0, token = -1;
+        for (bool more = true; more; end += more ? 32 : 0) {
+            int2 r = make_int2(0, -1);
+            if (end + wl <= n) r = __ldcg(rows + end + wl);
+            const unsigned ends = __ballot_sync(0xffffffffu, r.x == 0);   // the row behind the last draft keeps nothing
+            more = ends == 0;
+            if (!more) {
+                token = __shfl_sync(0xffffffffu, r.y, __ffs(ends) - 1);
+                end += __ffs(ends) - 1;
+            }
+        }
+        put_lane(a, lane, end, token);
+        return;
+    }
+    // ---- rows that their runs tell all of
+    const Run* runs = static_cast<const Run*>(a.run_results) + (int64_t)lane * (n_drafts + 1) * a.runs;
+    const T* logits = static_cast<const T*>(a.logits) + (int64_t)lane * (n_drafts + 1) * a.ld;
+    const float* probs = a.draft_probs == nullptr ? nullptr : a.draft_probs + (int64_t)lane * n_drafts * vocab;
+    const double per_t = hot ? 1.0 / (double)temperature : 0.0;
+    RowSum mine{0, 0.0, false};
+    int ends = INT_MAX;
+    for (int j = warp; j <= n; j += kWarps) {
+        const int d = j < n ? drafts[j] : -1;
+        const double below = d >= 0 && whole ? (double)u[j] * (probs != nullptr ? (double)probs[(int64_t)j * vocab + d] : 1.0) : 0.0;
+        const double logit = d >= 0 && whole ? (double)value_of(logits[j * a.ld + d]) : 0.0;
+        mine = sum_runs(runs + (int64_t)j * a.runs, a.runs, per_t, whole);
+        const bool kept = d >= 0 && !mine.bad && (whole ? below < exp((logit - (double)value_of_key(mine.best)) * per_t) / mine.z : d == (int)rank_key_index(mine.best));
+        if (!kept) {
+            ends = j;
+            break;
+        }
+    }
+    if (wl == 0 && ends < INT_MAX) atomicMin(&s_end, ends);
+    __syncthreads();
+    const int end = s_end;
+    if (ends == end && wl == 0) {
+        s_best = mine.best;
+        s_z = mine.z;
+        s_bad = mine.bad;
+    }
+    __syncthreads();
+    if (s_bad || !whole) {
+        if (rank != 0 || warp != 0) return;
+        if (s_bad && wl == 0) tell(a.status, kDevBadRow);
+        put_lane(a, lane, end, s_bad ? -1 : (int)rank_key_index(s_best));
+        return;
+    }
+    // ---- the draw: every warp adds up a run of its own, and a CTA looks through the one where the target lies
+    const T* x = logits + end * a.ld;
+    const int d = end < n ? drafts[end] : -1;
+    const float* q = probs == nullptr || d < 0 ? nullptr : probs + (int64_t)end * vocab;
+    const double z = s_z;
+    const Exponential weight(value_of_key(s_best), temperature);
+    const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
+    const int chunk = (vocab + kCtas - 1) / kCtas, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
+    const int run = (n1 - n0 + kWarps - 1) / kWarps, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
+    bool rest = d >= 0;
+    auto share = [&](float logit, float qt) {
+        const float w = weight(logit);
+        return rest ? fmaxf(fmaf(w, per_z, -qt) + w * per_z_rest, 0.f) : w;
+    };
+    auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
+    double total = 0.0, *sums = sum_of[0];
+    for (;;) {
+        constexpr int AHEAD = 8;
+        double part = 0.0;
+        for (int t0 = r_lo + wl; t0 < r_hi; t0 += 32 * AHEAD) {
+            float l[AHEAD], qv[AHEAD], s = 0.f;
+#pragma unroll
+            for (int c = 0; c < AHEAD; ++c) {
+                const int t = t0 + 32 * c;
+                l[c] = t < r_hi ? value_of(x[t]) : -INFINITY;
+                qv[c] = t < r_hi ? q_at(t) : 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < AHEAD; ++c) s += share(l[c], qv[c]);
+            part += (double)s;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        if (wl == 0) region[warp] = part;
+        __syncthreads();
+        if (warp == 0) {
+            double s = region[wl % kWarps];
+#pragma unroll
+            for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (wl < kCtas) *cluster.map_shared_rank(sums + rank, wl) = s;
+        }
+        cluster.sync();
+        total = 0.0;
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) total += sums[c];
+        if (total > 0.0 || !rest) break;
+        rest = false;   // the draft's distribution covers the target's
+        sums = sum_of[1];
+    }
+    const double target = u_draw * total;
+    // the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
+    double upto = 0.0;
+    int at = -1;
+#pragma unroll
+    for (int c = 0; c < kCtas; ++c) {
+        if (upto > target) break;
+        if (sums[c] > 0.0) at = c;
+        upto += sums[c];
+    }
+    if (at != rank) return;
+    upto = 0.0;
+    for (int c = 0; c < rank; ++c) upto += sums[c];
+    int w_at = 0;
+    double before = upto;
+    for (int w = 0; w < kWarps; ++w) {
+        if (region[w] > 0.0) {
+            w_at = w;
+            before = upto;
+        }
+        upto += region[w];
+        if (upto > target) break;
+    }
+    const int at_lo = min(n1, n0 + w_at * run), at_hi = min(n1, at_lo + run);
+    for (int t0 = at_lo; t0 < at_hi; t0 += kThreads) {
+        const int t = t0 + tid;
+        const double r = t < at_hi ? (double)share(value_of(x[t]), q_at(t)) : 0.0;
+        double all;
+        const double c = before + block_scan(r, top_shared.red, &all);
+        if (r > 0.0) {
+            atomicMax(&s_last, t);
+            if (c > target) atomicMin(&s_pick, t);
+        }
+        before += all;
+        __syncthreads();
+        if (s_pick < INT_MAX) break;
+    }
+    __syncthreads();
+    if (warp == 0) put_lane(a, lane, end, s_pick < INT_MAX ? s_pick : s_last);
 }
 
 }  // namespace
@@ -716,8 +766,7 @@ VerifyPlan verify_plan(int type, int lanes, int n_drafts, int vocab) {
     const int64_t rows = (int64_t)lanes * (n_drafts + 1);
     p.results_at = (rows * p.runs * kScan * 4 + 255) / 256 * 256;
     p.rows_at = p.results_at + rows * p.runs * (int64_t)sizeof(Run);
-    p.counters_at = p.rows_at + rows * 8;
-    p.bytes = p.counters_at + (int64_t)lanes * 4;
+    p.bytes = p.rows_at + rows * 8;
     return p;
 }
 
@@ -725,10 +774,9 @@ void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace,
     if (a.lanes <= 0) return;
     a.vpt = p.vpt;
     a.runs = p.runs;
-    a.group_best = reinterpret_cast<uint32_t*>(workspace);
+    a.group_best = reinterpret_cast<float*>(workspace);
     a.run_results = workspace + p.results_at;
     a.rows = reinterpret_cast<int2*>(workspace + p.rows_at);
-    a.counters = reinterpret_cast<int32_t*>(workspace + p.counters_at);
     const unsigned rows = (unsigned)(a.lanes * (a.n_drafts + 1));
     auto scan = [&](auto* kernel) {
         kernel<<<rows * (unsigned)p.runs, kScan, 0, s>>>(a);
@@ -738,9 +786,9 @@ void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace,
         const int groups = p.runs * kScan;
         a.list_at = groups * 4;
         a.keys_at = (a.list_at + groups * 2 + 15) / 16 * 16;
-        const size_t smem = (size_t)a.keys_at + kCandidates * 8 + kThreads * 12;
+        const size_t smem = (size_t)a.keys_at + kCandidates * 8 + kThreads * 8;
         ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-        launch_pdl(kernel, dim3(rows * kCtas), dim3(kThreads), smem, s, a);
+        launch_pdl(kernel, dim3((unsigned)(a.lanes * kCtas)), dim3(kThreads), smem, s, a);
     };
     if (a.type == 0) {
         switch (p.vpt) {
@@ -749,21 +797,21 @@ void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace,
             case 4: scan(scan_rows_kernel<float, 4>); break;
             default: scan(scan_rows_kernel<float, 8>);
         }
-        finish(finish_rows_kernel<float>);
+        finish(finish_lanes_kernel<float>);
     } else if (a.type == 1) {
         switch (p.vpt) {
             case 1: scan(scan_rows_kernel<__half, 1>); break;
             case 2: scan(scan_rows_kernel<__half, 2>); break;
             default: scan(scan_rows_kernel<__half, 4>);
         }
-        finish(finish_rows_kernel<__half>);
+        finish(finish_lanes_kernel<__half>);
     } else {
         switch (p.vpt) {
             case 1: scan(scan_rows_kernel<__nv_bfloat16, 1>); break;
             case 2: scan(scan_rows_kernel<__nv_bfloat16, 2>); break;
             default: scan(scan_rows_kernel<__nv_bfloat16, 4>);
         }
-        finish(finish_rows_kernel<__nv_bfloat16>);
+        finish(finish_lanes_kernel<__nv_bfloat16>);
     }
 }
 

@@ -23,17 +23,16 @@ struct VerifyArgs {
     int32_t* accepted = nullptr;       // [lanes]
     int32_t* status = nullptr;
     // filled in by the launcher
-    uint32_t* group_best = nullptr;    // [rows][runs][256] best value of each thread's tokens, as an order key
+    float* group_best = nullptr;       // [rows][runs][256] best value of each thread's tokens
     void* run_results = nullptr;       // [rows][runs]
     int2* rows = nullptr;              // (draft kept, token drawn in its place)
-    int32_t* counters = nullptr;       // [lanes]
     int vpt = 0, runs = 0, list_at = 0, keys_at = 0;
 };
 
 // How a call is cut, and its workspace.
 struct VerifyPlan {
     int vpt = 1, runs = 0;             // pieces of 16 bytes to a thread; runs of tokens, a CTA each, to a row
-    int64_t results_at = 0, rows_at = 0, counters_at = 0, bytes = 0;
+    int64_t results_at = 0, rows_at = 0, bytes = 0;
 };
 VerifyPlan verify_plan(int type, int lanes, int n_drafts, int vocab);
 void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace, cudaStream_t s);
