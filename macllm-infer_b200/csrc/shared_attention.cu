@@ -8,6 +8,7 @@
 #include "shared_attention.h"
 #include "hgemm_tc.h"
 #include "kernels.h"
+#include "tile_phases.h"
 #include "umma.cuh"
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -73,6 +74,29 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     return r;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {   // zeros where there is nothing
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Two warps meet at a named barrier; pair_any tells whether any of their threads says yes.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool yes) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"((uint32_t)yes), "r"(id) : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void tell(int32_t* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);
 }
@@ -105,7 +129,7 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
     const int lane = threadIdx.x & 31;
     const int64_t n_rows = (int64_t)a.total * a.q_heads;
     for (int s0 = 0; s0 < parts; s0 += 32) {
-        const float2 ml = s0 + lane < parts ? a.part_ml[(s0 + lane) * n_rows + row] : make_float2(-INFINITY, 0.f);
+        const float2 ml = s0 + lane < parts ? __ldcg(a.part_ml + (s0 + lane) * n_rows + row) : make_float2(-INFINITY, 0.f);
         const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
         const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ex2(ml.x - m_use);
         l = l * old + warp_sum(ml.y * f);
@@ -113,21 +137,27 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
         for (int j = 0; j < V; ++j) o[j] *= old;
         m = m_new;
         const int n = min(32, parts - s0);
-#pragma unroll 4
-        for (int s = 0; s < n; ++s) {
-            const float fs = __shfl_sync(0xffffffffu, f, s);
-            if (fs == 0.f) continue;   // a part without keys wrote no output
-            const float* src = a.part_o + ((s0 + s) * n_rows + row) * D + lane * V;
-            if constexpr (V == 2) {
-                const float2 x = *reinterpret_cast<const float2*>(src);
-                o[0] += x.x * fs; o[1] += x.y * fs;
-            } else {
+        constexpr int AHEAD = 32 / V;   // parts on their way together; one without keys wrote no output
+        for (int b = 0; b < n; b += AHEAD) {
+            float x[AHEAD][V], w[AHEAD];
 #pragma unroll
-                for (int j = 0; j < V; j += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + j);
-                    o[j] += x.x * fs; o[j + 1] += x.y * fs; o[j + 2] += x.z * fs; o[j + 3] += x.w * fs;
+            for (int s = 0; s < AHEAD; ++s) {
+                w[s] = b + s < 32 ? __shfl_sync(0xffffffffu, f, b + s) : 0.f;
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[s][j] = 0.f;
+                if (w[s] == 0.f) continue;
+                const float* src = a.part_o + ((s0 + b + s) * n_rows + row) * D + lane * V;
+                if constexpr (V == 2) {
+                    *reinterpret_cast<float2*>(x[s]) = __ldcg(reinterpret_cast<const float2*>(src));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(x[s] + j) = __ldcg(reinterpret_cast<const float4*>(src + j));
                 }
             }
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] += x[s][j] * w[s];
         }
     }
 }
@@ -404,19 +434,18 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
 
 // ---- the shared keys ---------------------------------------------------------------------------------------------
 //
-// All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA,
-// over a share of the keys in tiles of KEYS.  One warp brings keys and values by TMA, one issues the tcgen05 products, four per tile of items do the
-// softmax, a thread per item.  Products go round in units (tile of keys, tile of items): scores of unit u into one of two areas of tensor memory, u & 1; its
-// weights go back over its scores, as the A operand of O += P V; and the area is free for the scores of unit u + 2 as soon as that product is issued, since
-// products of one thread run in their order.  With two tiles of items the one's softmax runs under the other's products and a key is
-// fetched once for both.  The running maximum follows only when a tile exceeds it by kSlack (weights stay below 2^kSlack).
+// All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA, over a share of
+// the keys in tiles of 64.  One warp brings keys and values by TMA, one per tile of items issues the tcgen05 products, and eight do its softmax: two threads per item, half of
+// the keys each.  Scores of a tile of keys go to one of two areas of tensor memory that a tile of items has; its weights go back over its scores, as the A operand of
+// O += P V; the scores of the next tile are made meanwhile, so that the softmax, which the exponentials bound (16 per clock and SM), does not wait for products.  With two
+// tiles of items a key is fetched once for both.  The running maximum follows only when a tile exceeds it by kSlack (weights stay below 2^kSlack).
 constexpr float kSlack = 8.f;
-constexpr int kItems = 128;
+constexpr int kItems = 128, kKeys = 64;
 
 template <int D, int NQ>
 struct SharedSmem {
-    static constexpr int KEYS = D == 256 ? 64 : 128, PANELS = D / 64, PANEL = KEYS * 128, QPANEL = kItems * 128, BYTES = PANELS * PANEL;
-    static constexpr int STAGES = D == 64 ? 4 : 2, THREADS = NQ * 128 + 64;
+    static constexpr int PANELS = D / 64, PANEL = kKeys * 128, QPANEL = kItems * 128, BYTES = PANELS * PANEL;
+    static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? 4 : 6), WARPS = NQ * 8, THREADS = WARPS * 32 + 32 + NQ * 32;   // WARPS: of the softmax
     static constexpr size_t SMEM = 1024 + (size_t)NQ * PANELS * QPANEL + (size_t)STAGES * 2 * BYTES;
 };
 
@@ -424,12 +453,14 @@ template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(SharedSmem<D, NQ>::THREADS, 1)
 shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a, int box, int splits) {
     using L = SharedSmem<D, NQ>;
-    constexpr int ST = L::STAGES, KEYS = L::KEYS, S_AT = NQ * D;   // columns of tensor memory: outputs, then the two areas
+    constexpr int ST = L::STAGES, KEYS = kKeys, S_AT = NQ * D, AREAS = 2 * NQ;   // columns of tensor memory: outputs, then the areas
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[4 * ST + 7];
+    __shared__ uint64_t bars[4 * ST + 3 * AREAS + 1];
     __shared__ uint32_t tmem_slot;
-    __shared__ int4 sees[NQ * 4];
-    uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST, *s_full = bars + 4 * ST, *p_full = s_full + 2, *o_done = s_full + 4, *q_full = s_full + 6;
+    __shared__ int4 sees[L::WARPS];
+    __shared__ float row_max[L::WARPS][32];   // exchanged between an item's two threads; in the end the sums
+    uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST, *s_full = bars + 4 * ST, *p_full = s_full + AREAS, *o_done = p_full + AREAS,
+             *q_full = o_done + AREAS;
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ks = qs + NQ * L::PANELS * L::QPANEL;
     uint8_t* vs = ks + ST * L::BYTES;
@@ -439,27 +470,27 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             bar_init(&k_full[i], 1);
-            bar_init(&k_empty[i], 1);
+            bar_init(&k_empty[i], NQ);
             bar_init(&v_full[i], 1);
-            bar_init(&v_empty[i], 1);
+            bar_init(&v_empty[i], NQ);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < AREAS; ++i) {
             bar_init(&s_full[i], 1);
-            bar_init(&p_full[i], kItems);
+            bar_init(&p_full[i], 8);
             bar_init(&o_done[i], 1);
         }
-        bar_init(q_full, NQ * kItems);
+        bar_init(q_full, L::WARPS);
         bar_init_fence();
     }
     // what this thread's item is, and what it sees
-    const int64_t item = (int64_t)tile * (NQ * kItems) + tid;
+    const int q = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane, item = (tile * NQ + q) * kItems + row;
     int token = -1, head = 0, see_lo = 0, see_hi = 0;
-    if (warp < NQ * 4) {
-        const int64_t at_token = item / g;
+    if (warp < L::WARPS) {
+        const int at_token = item / g;
         if (at_token < a.total) {
             int l = 0;
             if (a.cu == nullptr) {
-                l = (int)at_token / a.rows;
+                l = at_token / a.rows;
             } else {   // the last lane that begins at or before this row
                 int lo = 0, hi = a.lanes;
                 while (hi - lo > 1) {
@@ -471,8 +502,8 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
             const LaneRange at = lane_range(a, l);
             if (at_token >= at.first && at_token < at.first + at.n) {
-                token = (int)at_token;
-                head = kvh * g + (int)(item - at_token * g);
+                token = at_token;
+                head = kvh * g + item - at_token * g;
                 const int p = at.position + token - at.first;
                 see_lo = attention_first_key(max(p, 0), a.window, 0);
                 see_hi = min(a.shared, p + 1);
@@ -483,14 +514,15 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                                  __reduce_min_sync(0xffffffffu, token >= 0 ? see_hi : INT_MAX), __reduce_max_sync(0xffffffffu, live ? see_hi : 0));
         if (lane == 0) sees[warp] = s;
     }
-    if (warp == NQ * 4 + 1) tmem_alloc(&tmem_slot, 512);
+    if (warp == L::WARPS + 1) tmem_alloc(&tmem_slot, 512);
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
 #pragma unroll
-    for (int w = 0; w < NQ * 4; ++w) {
+    for (int w = 0; w < L::WARPS; ++w) {
+        if ((w >> 2 & 1) != 0) continue;   // the same items
         lo_min = min(lo_min, sees[w].x);
         lo_max = max(lo_max, sees[w].y);
         hi_min = min(hi_min, sees[w].z);
@@ -499,11 +531,11 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int all_tiles = (a.shared + KEYS - 1) / KEYS;
     const int t_begin = max((int)((int64_t)all_tiles * split / splits), lo_min / KEYS);
     const int t_end = min((int)((int64_t)all_tiles * (split + 1) / splits), (hi_max + KEYS - 1) / KEYS);
-    const int n_tiles = max(0, t_end - t_begin), units = n_tiles * NQ;
+    const int n_tiles = max(0, t_end - t_begin);
 
-    if (warp == NQ * 4) {
+    if (warp == L::WARPS) {
         // ---- loader
-        const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most KEYS / 16 boxes of each of the panels: 16
+        const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most four boxes of each of the panels: 16
         const bool mine = panel < L::PANELS;
         auto page_row = [&](int t) {
             int pos = (t_begin + t) * KEYS + of * box;
@@ -543,96 +575,111 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 if (u < t) bar_wait(&v_full[u % ST], u / ST & 1);
             }
         }
-    } else if (warp == NQ * 4 + 1) {
-        // ---- products
-        if (lane == 0 && units > 0) {
+    } else if (warp > L::WARPS) {
+        // ---- products, a warp per tile of items: the one's waits pass under the other's products.  The whole warp walks along, so that descriptors and addresses are the same for
+        // all of it, and one elected thread issues (a lane of its own: 2500 clocks a tile of keys, 100 a product)
+        if (n_tiles > 0) {
             constexpr uint32_t kind = std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u;
             constexpr uint32_t i_scores = f16_idesc(kItems, KEYS, false) | kind, i_out = f16_idesc(kItems, D, true) | kind;
-            const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
-            auto scores = [&](int u) {
-                const int t = u / NQ, q = u % NQ, st = t % ST;
-                if (q == 0) {
-                    if (!bar_wait(&k_full[st], t / ST & 1)) return false;
-                    fence_after();
-                }
-                const uint64_t qd = sw128_desc(q_addr + q * L::PANELS * L::QPANEL), kd = sw128_desc(k_addr + st * L::BYTES);
+            const int q = NQ == 1 ? 0 : __shfl_sync(0xffffffffu, warp, 0) - L::WARPS - 1;
+            const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), s_base = base + S_AT + q * 2 * KEYS, o_base = base + q * D;
+            const uint64_t q_desc = sw128_desc(smem_u32(qs) + q * L::PANELS * L::QPANEL), k_desc = sw128_desc(smem_u32(ks)), v_desc = sw128_desc(smem_u32(vs), L::PANEL);
+            const bool issues = elect_one();
+            auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)) != 0; };
+            auto scores = [&](int t) {
+                const int st = t % ST, at = tile_phase(t).at;
+                if (!wait(&k_full[st], t / ST & 1)) return false;
+                fence_after();
+                if (issues) {
+                    const uint64_t kd = k_desc + st * (L::BYTES / 16);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma(tmem + S_AT + (u & 1) * KEYS, qd + (i >> 2) * (L::QPANEL / 16) + (i & 3) * 2, kd + (i >> 2) * (L::PANEL / 16) + (i & 3) * 2, i_scores, i > 0);
-                if (q == NQ - 1) commit(&k_empty[st]);
-                commit(&s_full[u & 1]);
+                    for (int i = 0; i < D / 16; ++i)
+                        mma(s_base + at * KEYS, q_desc + (i >> 2) * (L::QPANEL / 16) + (i & 3) * 2, kd + (i >> 2) * (L::PANEL / 16) + (i & 3) * 2, i_scores, i > 0);
+                    commit(&k_empty[st]);
+                    commit(&s_full[q * 2 + at]);
+                }
+                __syncwarp();
                 return true;
             };
-            bool ok = bar_wait(q_full, 0);
+            bool ok = wait(q_full, 0);
             fence_after();
-            ok = ok && scores(0) && (units < 2 || scores(1));
-            for (int u = 0; u < units && ok; ++u) {
-                const int t = u / NQ, q = u % NQ, st = t % ST;
-                ok = (q > 0 || bar_wait(&v_full[st], t / ST & 1)) && bar_wait(&p_full[u & 1], u >> 1 & 1);
+            ok = ok && scores(0);
+            for (int t = 0; t < n_tiles && ok; ++t) {
+                const int st = t % ST;
+                const TilePhase ph = tile_phase(t);
+                // the scores of tile t + 1 go where the weights of tile t - 1 were: their product was issued before, and products of one thread run in their order
+                if (t + 1 < n_tiles) ok = scores(t + 1);
+                ok = ok && wait(&v_full[st], t / ST & 1) && wait(&p_full[q * 2 + ph.at], ph.parity);
                 if (!ok) break;
                 fence_after();
-                const uint32_t p = tmem + S_AT + (u & 1) * KEYS;
-                const uint64_t v = sw128_desc(v_addr + st * L::BYTES, L::PANEL);
+                if (issues) {
+                    const uint64_t vd = v_desc + st * (L::BYTES / 16);
 #pragma unroll
-                for (int i = 0; i < KEYS / 16; ++i) mma_tmem_a(tmem + q * D, p + i * 8, v + i * 128, i_out, t > 0 || i > 0);
-                if (q == NQ - 1) commit(&v_empty[st]);
-                commit(&o_done[u & 1]);
-                if (u + 2 < units) ok = scores(u + 2);
+                    for (int i = 0; i < KEYS / 16; ++i) mma_tmem_a(o_base, s_base + ph.at * KEYS + i * 8, vd + i * 128, i_out, t > 0 || i > 0);
+                    commit(&v_empty[st]);
+                    commit(&o_done[q * 2 + ph.at]);
+                }
+                __syncwarp();
             }
-            if (!ok) tell(a.status, kDevWait);
+            if (!ok && lane == 0) tell(a.status, kDevWait);
         }
     } else {
-        // ---- one item per thread
-        for (int i = tid; i < NQ * kItems * (D / 8); i += NQ * kItems) {
-            const int it = i / (D / 8), c = (i - it * (D / 8)) * 8;
-            const int64_t index = (int64_t)tile * (NQ * kItems) + it, tok = index / g;
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (tok < a.total) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.ldq + (kvh * g + (index - tok * g)) * D + c);
-            const int q = it / kItems, r = it % kItems;
-            *reinterpret_cast<uint4*>(qs + (q * L::PANELS + (c >> 6)) * L::QPANEL + r * 128 + (((c & 63) * 2) ^ ((r & 7) << 4))) = x;
+        // ---- softmax: half an item per thread.  The queries' pieces first, all on their way together: one after the other they took 0.6 us each, 10 us at heads of 128
+#pragma unroll 4
+        for (int i = tid; i < NQ * kItems * (D / 8); i += L::WARPS * 32) {
+            const int it = i / (D / 8), c = (i - it * (D / 8)) * 8, r = it % kItems;
+            const int index = tile * (NQ * kItems) + it, tok = index / g;   // total * q_heads is far below 2^31
+            const bool there = tok < a.total;
+            const T* src = static_cast<const T*>(a.q) + (there ? tok * a.ldq + (kvh * g + (index - tok * g)) * D + c : 0);
+            cp_async16(smem_u32(qs) + (it / kItems * L::PANELS + (c >> 6)) * L::QPANEL + r * 128 + (((c & 63) * 2) ^ ((r & 7) << 4)), src, there);
         }
+        cp_async_wait_all();
         fence_async_smem();
-        bar_arrive(q_full);
+        __syncwarp();
+        if (lane == 0) bar_arrive(q_full);
 
-        const int q = warp >> 2;
-        const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = my + q * D;
+        constexpr int COLS = KEYS / 2;
+        const int pair = 1 + q * 4 + (warp & 3), other = warp ^ 4;   // the named barrier of the two warps
+        const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = my + q * D + half * (D / 2);
         const float two_over_cap = a.softcap != 0.f ? 2.0f / a.softcap : 0.f, unit = a.softcap != 0.f ? kLog2e : a.scale * kLog2e;
         float m_run = -INFINITY, sum = 0.f;   // the maximum as a base-2 logarithm
-        bool ok = true;
-        for (int u = NQ == 2 ? q : 0; u < units; u += NQ) {
-            const int t = u / NQ;
-            ok = __all_sync(0xffffffffu, bar_wait(&s_full[u & 1], u >> 1 & 1));
-            if (!ok) break;
+        bool ok = true;   // once a wait gave up nothing is waited for any more, but every step is taken: the other warp counts on it
+        for (int t = 0; t < n_tiles; ++t) {
+            const TilePhase ph = tile_phase(t);
+            ok = ok && bar_wait(&s_full[q * 2 + ph.at], ph.parity);
+            __syncwarp();
             fence_after();
-            const uint32_t s_at = my + S_AT + (u & 1) * KEYS;
-            float s[KEYS];
-#pragma unroll
-            for (int j = 0; j < KEYS; j += 32) tmem_ld32(s_at + j, reinterpret_cast<uint32_t*>(s) + j);
+            const uint32_t s_at = my + S_AT + (q * 2 + ph.at) * KEYS;
+            float s[COLS];
+            tmem_ld32(s_at + half * COLS, reinterpret_cast<uint32_t*>(s));
             tmem_wait_ld();
-            const int pos0 = (t_begin + t) * KEYS;
+            const int pos0 = (t_begin + t) * KEYS + half * COLS;
             if (a.softcap != 0.f) {
 #pragma unroll
-                for (int j = 0; j < KEYS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
+                for (int j = 0; j < COLS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
             }
-            if (pos0 + KEYS > hi_min || pos0 < lo_max) {   // uniform: some item does not see the whole tile
+            if (pos0 + COLS > hi_min || pos0 < lo_max) {   // uniform: some item does not see all of them
 #pragma unroll
-                for (int j = 0; j < KEYS; ++j) s[j] = pos0 + j >= see_lo && pos0 + j < see_hi ? s[j] : -INFINITY;
+                for (int j = 0; j < COLS; ++j) s[j] = pos0 + j >= see_lo && pos0 + j < see_hi ? s[j] : -INFINITY;
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int j = 4; j < KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
-            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
-            const bool grow = m_tile > m_run + kSlack;   // also when there was none yet
-            if (__any_sync(0xffffffffu, grow)) {
-                const float m_new = grow ? m_tile : m_run;
+            for (int j = 4; j < COLS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+            float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
+            // also when there was none yet.  Behind this barrier both warps have read their scores, so weights may go over them.
+            if (pair_any(pair, m_tile > m_run + kSlack)) {
+                row_max[warp][lane] = m_tile;
+                pair_sync(pair);
+                m_tile = fmaxf(m_tile, row_max[other][lane]);
+                const float m_new = m_tile > m_run + kSlack ? m_tile : m_run;
                 const float alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_new);
                 if (t > 0) {
-                    // the item's product before: with two tiles of items these scores were issued behind it
-                    if (NQ == 1) ok = __all_sync(0xffffffffu, bar_wait(&o_done[(u - 1) & 1], (u - 1) >> 1 & 1));
-                    if (!ok) break;
+                    const TilePhase before = tile_phase(t - 1);
+                    ok = ok && bar_wait(&o_done[q * 2 + before.at], before.parity);
+                    __syncwarp();
                     fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
+                    for (int c = 0; c < D / 2; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_at + c, o);
                         tmem_wait_ld();
@@ -646,50 +693,53 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             float part[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t w[COLS / 2];
 #pragma unroll
-            for (int j0 = 0; j0 < KEYS; j0 += 64) {
-                uint32_t w[32];
-#pragma unroll
-                for (int j = 0; j < 64; j += 2) {
-                    const float x = ex2(fmaf(s[j0 + j], unit, -m_use)), y = ex2(fmaf(s[j0 + j + 1], unit, -m_use));
-                    part[j & 3] += x;
-                    part[(j & 3) + 1] += y;
-                    w[j / 2] = Pair<T>::pack(x, y);
-                }
-                tmem_st32(s_at + j0 / 2, w);
+            for (int j = 0; j < COLS; j += 2) {
+                const float x = ex2(fmaf(s[j], unit, -m_use)), y = ex2(fmaf(s[j + 1], unit, -m_use));
+                part[j & 3] += x;
+                part[(j & 3) + 1] += y;
+                w[j / 2] = Pair<T>::pack(x, y);
             }
+            tmem_st16(s_at + half * (COLS / 2), w);
             sum += (part[0] + part[1]) + (part[2] + part[3]);
             tmem_wait_st();
             fence_before();
-            bar_arrive(&p_full[u & 1]);
+            __syncwarp();
+            if (lane == 0) bar_arrive(&p_full[q * 2 + ph.at]);
         }
-        if (ok && units > 0) {
-            const int last = units - NQ + (NQ == 2 ? q : 0);
-            ok = __all_sync(0xffffffffu, bar_wait(&o_done[last & 1], last >> 1 & 1));
+        if (n_tiles > 0) {
+            const TilePhase last = tile_phase(n_tiles - 1);
+            ok = ok && bar_wait(&o_done[q * 2 + last.at], last.parity);
         }
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
             if (lane == 0) tell(a.status, kDevWait);
-            sum = m_run = __int_as_float(0x7fffffff);   // the result says so
+            sum = __int_as_float(0x7fffffff);   // the result says so
         }
+        pair_sync(pair);
+        row_max[warp][lane] = sum;
+        pair_sync(pair);
+        sum += row_max[other][lane];
         fence_after();
         const int64_t slot = ((int64_t)split * a.total + token) * a.q_heads + head;
-        if (token >= 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
-        if (units > 0) {
+        if (token >= 0 && half == 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
+        if (n_tiles > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = 0; c < D / 2; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_at + c, o);
                 tmem_wait_ld();
                 if (token < 0) continue;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<uint4*>(a.part_o + slot * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    *reinterpret_cast<uint4*>(a.part_o + slot * D + half * (D / 2) + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
         }
     }
     fence_before();
     __syncthreads();
-    if (warp == NQ * 4 + 1) {
+    if (warp == L::WARPS + 1) {
         fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -698,7 +748,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 template <typename T, int D, int NQ>
 void launch_shared_part(const SharedAttnArgs& a, const SharedAttnPlan& p, uint64_t rows, cudaStream_t s) {
     using L = SharedSmem<D, NQ>;
-    const int box = std::min(a.block_tokens, L::KEYS);
+    const int box = std::min(a.block_tokens, kKeys);
     alignas(64) CUtensorMap tk, tv;
     encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, (uint32_t)box, true);
     encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, (uint32_t)box, true);
@@ -759,17 +809,17 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
     p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), 1024) / 16 * 16;
     p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
     if (shared > 0) {
-        // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.5 us per
+        // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.35 us per
         // tile of items, its start and end 4 us, and a share's results are written and read once.
         const int64_t all = (int64_t)total * g;
         p.item_rows = d <= 128 && all > kItems ? 2 : 1;
         p.row_tiles = (int)((all + kItems * p.item_rows - 1) / (kItems * p.item_rows));
-        const int tiles = (shared + (d == 256 ? 63 : 127)) / (d == 256 ? 64 : 128);
+        const int tiles = (shared + kKeys - 1) / kKeys;
         const double results_us = (double)total * q_heads * d * 8 / 8e6;
         double best = 0;
         for (int n = 1; n <= std::min(tiles, 148); ++n) {
             const int64_t waves = ((int64_t)p.row_tiles * kv_heads * n + kSms - 1) / kSms;
-            const double us = waves * ((tiles + n - 1) / n * 0.5 * p.item_rows + 4.0) + n * results_us;
+            const double us = waves * ((tiles + n - 1) / n * 0.35 * p.item_rows + 4.0) + n * results_us;
             if (n == 1 || us < best) best = us, p.shared_parts = n;
         }
     }
