@@ -79,18 +79,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Two warps meet at a named barrier; pair_any tells whether any of their threads says yes.
+// Two warps at a named barrier, one of which waits for the other.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool pair_any(int id, bool yes) {
-    uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"((uint32_t)yes), "r"(id) : "memory");
-    return any != 0;
-}
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
-                 "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
+__device__ __forceinline__ void pair_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -435,22 +426,24 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
 // ---- the shared keys ---------------------------------------------------------------------------------------------
 //
 // All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA, over a share of
-// the keys in tiles of 64.  One warp brings keys and values by TMA, one per tile of items issues the tcgen05 products, and eight do its softmax: two threads per item, half of
-// the keys each.  Scores of a tile of keys go to one of two areas of tensor memory that a tile of items has; its weights go back over its scores, as the A operand of
-// O += P V; the scores of the next tile are made meanwhile, so that the softmax, which the exponentials bound (16 per clock and SM), does not wait for products.  With two
-// tiles of items a key is fetched once for both.  The running maximum follows only when a tile exceeds it by kSlack (weights stay below 2^kSlack).
+// the keys in tiles of 64.  One warp brings keys and values by TMA, one per tile of items issues the tcgen05 products, four do its softmax, a thread per item.  Scores of a tile
+// of keys go to one of two areas of tensor memory that a tile of items has; its weights go back over its scores, as the A operand of O += P V; the scores of the next tile are
+// made meanwhile.  What bounds the softmax are the exponentials (16 per clock and SM).  With two tiles of items a key is fetched once for both, and the two warps that share a
+// quarter of the SM take turns at the exponentials: left alone they fall into step, and the unit idles while both do the rest (1850 clocks a tile of keys instead of
+// TURNS).  One tile of items to a CTA: two CTAs on an SM do the same for one another.  The running maximum follows only when a tile exceeds it by kSlack (weights stay below 2^kSlack).
 constexpr float kSlack = 8.f;
 constexpr int kItems = 128, kKeys = 64;
 
 template <int D, int NQ>
 struct SharedSmem {
     static constexpr int PANELS = D / 64, PANEL = kKeys * 128, QPANEL = kItems * 128, BYTES = PANELS * PANEL;
-    static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? 4 : 6), WARPS = NQ * 8, THREADS = WARPS * 32 + 32 + NQ * 32;   // WARPS: of the softmax
+    static constexpr int STAGES = D == 256 || (D == 128 && NQ == 1) ? 2 : (D == 128 ? 4 : (NQ == 1 ? 5 : 6)), WARPS = NQ * 4, THREADS = WARPS * 32 + 32 + NQ * 32;   // WARPS: of the softmax
+    static constexpr int CTAS = NQ == 1 && D <= 128 ? 2 : 1, TMEM = NQ * (D + 2 * kKeys) <= 256 ? 256 : 512;
     static constexpr size_t SMEM = 1024 + (size_t)NQ * PANELS * QPANEL + (size_t)STAGES * 2 * BYTES;
 };
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(SharedSmem<D, NQ>::THREADS, 1)
+__global__ void __launch_bounds__(SharedSmem<D, NQ>::THREADS, SharedSmem<D, NQ>::CTAS)
 shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a, int box, int splits) {
     using L = SharedSmem<D, NQ>;
     constexpr int ST = L::STAGES, KEYS = kKeys, S_AT = NQ * D, AREAS = 2 * NQ;   // columns of tensor memory: outputs, then the areas
@@ -458,7 +451,6 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     __shared__ uint64_t bars[4 * ST + 3 * AREAS + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int4 sees[L::WARPS];
-    __shared__ float row_max[L::WARPS][32];   // exchanged between an item's two threads; in the end the sums
     uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST, *s_full = bars + 4 * ST, *p_full = s_full + AREAS, *o_done = p_full + AREAS,
              *q_full = o_done + AREAS;
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -476,14 +468,14 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
         for (int i = 0; i < AREAS; ++i) {
             bar_init(&s_full[i], 1);
-            bar_init(&p_full[i], 8);
+            bar_init(&p_full[i], 4);
             bar_init(&o_done[i], 1);
         }
         bar_init(q_full, L::WARPS);
         bar_init_fence();
     }
     // what this thread's item is, and what it sees
-    const int q = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane, item = (tile * NQ + q) * kItems + row;
+    const int q = warp >> 2, item = tile * (NQ * kItems) + tid;
     int token = -1, head = 0, see_lo = 0, see_hi = 0;
     if (warp < L::WARPS) {
         const int at_token = item / g;
@@ -514,7 +506,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                                  __reduce_min_sync(0xffffffffu, token >= 0 ? see_hi : INT_MAX), __reduce_max_sync(0xffffffffu, live ? see_hi : 0));
         if (lane == 0) sees[warp] = s;
     }
-    if (warp == L::WARPS + 1) tmem_alloc(&tmem_slot, 512);
+    if (warp == L::WARPS + 1) tmem_alloc(&tmem_slot, L::TMEM);
     fence_before();
     __syncthreads();
     fence_after();
@@ -522,7 +514,6 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
 #pragma unroll
     for (int w = 0; w < L::WARPS; ++w) {
-        if ((w >> 2 & 1) != 0) continue;   // the same items
         lo_min = min(lo_min, sees[w].x);
         lo_max = max(lo_max, sees[w].y);
         hi_min = min(hi_min, sees[w].z);
@@ -624,7 +615,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (!ok && lane == 0) tell(a.status, kDevWait);
         }
     } else {
-        // ---- softmax: half an item per thread.  The queries' pieces first, all on their way together: one after the other they took 0.6 us each, 10 us at heads of 128
+        // ---- softmax, an item per thread.  The queries' pieces first, all on their way together: one after the other they took 0.6 us each, 10 us at heads of 128
 #pragma unroll 4
         for (int i = tid; i < NQ * kItems * (D / 8); i += L::WARPS * 32) {
             const int it = i / (D / 8), c = (i - it * (D / 8)) * 8, r = it % kItems;
@@ -638,40 +629,38 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         __syncwarp();
         if (lane == 0) bar_arrive(q_full);
 
-        constexpr int COLS = KEYS / 2;
-        const int pair = 1 + q * 4 + (warp & 3), other = warp ^ 4;   // the named barrier of the two warps
-        const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = my + q * D + half * (D / 2);
+        const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = my + q * D;
         const float two_over_cap = a.softcap != 0.f ? 2.0f / a.softcap : 0.f, unit = a.softcap != 0.f ? kLog2e : a.scale * kLog2e;
+        const int turn = 1 + (warp & 3) * 2;   // named barriers of the two warps, one for either's turn
         float m_run = -INFINITY, sum = 0.f;   // the maximum as a base-2 logarithm
         bool ok = true;   // once a wait gave up nothing is waited for any more, but every step is taken: the other warp counts on it
+        if (NQ == 2 && q == 1 && n_tiles > 0) pair_arrive(turn);
         for (int t = 0; t < n_tiles; ++t) {
             const TilePhase ph = tile_phase(t);
             ok = ok && bar_wait(&s_full[q * 2 + ph.at], ph.parity);
             __syncwarp();
             fence_after();
             const uint32_t s_at = my + S_AT + (q * 2 + ph.at) * KEYS;
-            float s[COLS];
-            tmem_ld32(s_at + half * COLS, reinterpret_cast<uint32_t*>(s));
+            float s[KEYS];
+            tmem_ld32(s_at, reinterpret_cast<uint32_t*>(s));
+            tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s) + 32);
             tmem_wait_ld();
-            const int pos0 = (t_begin + t) * KEYS + half * COLS;
+            const int pos0 = (t_begin + t) * KEYS;
             if (a.softcap != 0.f) {
 #pragma unroll
-                for (int j = 0; j < COLS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
+                for (int j = 0; j < KEYS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
             }
-            if (pos0 + COLS > hi_min || pos0 < lo_max) {   // uniform: some item does not see all of them
+            if (pos0 + KEYS > hi_min || pos0 < lo_max) {   // uniform: some item does not see the whole tile
 #pragma unroll
-                for (int j = 0; j < COLS; ++j) s[j] = pos0 + j >= see_lo && pos0 + j < see_hi ? s[j] : -INFINITY;
+                for (int j = 0; j < KEYS; ++j) s[j] = pos0 + j >= see_lo && pos0 + j < see_hi ? s[j] : -INFINITY;
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int j = 4; j < COLS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
-            float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
-            // also when there was none yet.  Behind this barrier both warps have read their scores, so weights may go over them.
-            if (pair_any(pair, m_tile > m_run + kSlack)) {
-                row_max[warp][lane] = m_tile;
-                pair_sync(pair);
-                m_tile = fmaxf(m_tile, row_max[other][lane]);
-                const float m_new = m_tile > m_run + kSlack ? m_tile : m_run;
+            for (int j = 4; j < KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
+            const bool grow = m_tile > m_run + kSlack;   // also when there was none yet
+            if (__any_sync(0xffffffffu, grow)) {
+                const float m_new = grow ? m_tile : m_run;
                 const float alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_new);
                 if (t > 0) {
                     const TilePhase before = tile_phase(t - 1);
@@ -679,7 +668,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                     __syncwarp();
                     fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 2; c += 32) {
+                    for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_at + c, o);
                         tmem_wait_ld();
@@ -693,15 +682,17 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             float part[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t w[COLS / 2];
+            uint32_t w[KEYS / 2];
+            if (NQ == 2) pair_sync(turn + q);
 #pragma unroll
-            for (int j = 0; j < COLS; j += 2) {
+            for (int j = 0; j < KEYS; j += 2) {
                 const float x = ex2(fmaf(s[j], unit, -m_use)), y = ex2(fmaf(s[j + 1], unit, -m_use));
                 part[j & 3] += x;
                 part[(j & 3) + 1] += y;
                 w[j / 2] = Pair<T>::pack(x, y);
             }
-            tmem_st16(s_at + half * (COLS / 2), w);
+            if (NQ == 2 && (q == 0 || t + 1 < n_tiles)) pair_arrive(turn + 1 - q);
+            tmem_st32(s_at, w);
             sum += (part[0] + part[1]) + (part[2] + part[3]);
             tmem_wait_st();
             fence_before();
@@ -715,25 +706,21 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
             if (lane == 0) tell(a.status, kDevWait);
-            sum = __int_as_float(0x7fffffff);   // the result says so
+            sum = m_run = __int_as_float(0x7fffffff);   // the result says so
         }
-        pair_sync(pair);
-        row_max[warp][lane] = sum;
-        pair_sync(pair);
-        sum += row_max[other][lane];
         fence_after();
         const int64_t slot = ((int64_t)split * a.total + token) * a.q_heads + head;
-        if (token >= 0 && half == 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
+        if (token >= 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
         if (n_tiles > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 32) {
+            for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_at + c, o);
                 tmem_wait_ld();
                 if (token < 0) continue;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<uint4*>(a.part_o + slot * D + half * (D / 2) + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    *reinterpret_cast<uint4*>(a.part_o + slot * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
         }
     }
@@ -741,7 +728,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     __syncthreads();
     if (warp == L::WARPS + 1) {
         fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, L::TMEM);
     }
 }
 
@@ -818,7 +805,7 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
         const double results_us = (double)total * q_heads * d * 8 / 8e6;
         double best = 0;
         for (int n = 1; n <= std::min(tiles, 148); ++n) {
-            const int64_t waves = ((int64_t)p.row_tiles * kv_heads * n + kSms - 1) / kSms;
+            const int64_t slots = d <= 128 && p.item_rows == 1 ? 2 * kSms : kSms, waves = ((int64_t)p.row_tiles * kv_heads * n + slots - 1) / slots;
             const double us = waves * ((tiles + n - 1) / n * 0.35 * p.item_rows + 4.0) + n * results_us;
             if (n == 1 || us < best) best = us, p.shared_parts = n;
         }
