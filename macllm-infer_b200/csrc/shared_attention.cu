@@ -165,25 +165,27 @@ __device__ __forceinline__ void store_row(T* out, const float (&o)[V], float l) 
 
 // ---- a lane's keys -----------------------------------------------------------------------------------------------
 //
-// A CTA takes a share of one lane's keys for NT * 8 (row, head) items of one KV head.  Each of its four warps walks tiles of 16 keys, which TMA brings
-// into a ring of its own; the items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.
-constexpr int kWarps = 4;
+// A CTA takes a share of one lane's keys for NT * 8 (row, head) items of one KV head.  Each of its warps walks tiles of 16 keys, which TMA brings into a ring of its own; the
+// items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.  What bounds it is HBM where lanes have much of their own, else the chain of dependent fetches at a CTA's two
+// ends: so a warp asks for its first tiles before anything else, and rings are short enough for three CTAs on an SM.
 constexpr int kTile = 16;
 
 template <int D>
 struct LaneSmem {
+    static constexpr int WARPS = D == 256 ? 2 : 4, THREADS = WARPS * 32;
     static constexpr int PANELS = D / 64, K_BYTES = kTile * D * 2, STAGE = 2 * K_BYTES;
-    static constexpr int STAGES = D == 256 ? 2 : (D == 128 ? 3 : 4);
+    static constexpr int STAGES = D == 64 ? 4 : 2;
     static constexpr int QP = D + 8, OP = D + 4;
-    static constexpr size_t bytes(int nt) { return 1024 + (size_t)kWarps * std::max(STAGES * STAGE, nt * 8 * (OP + 2) * 4) + (size_t)nt * 8 * QP * 2; }
+    __host__ __device__ static constexpr int ring(int nt) { return ((STAGES * STAGE > nt * 8 * (OP + 2) * 4 ? STAGES * STAGE : nt * 8 * (OP + 2) * 4) + 1023) / 1024 * 1024; }
+    static constexpr size_t bytes(int nt) { return 1024 + (size_t)WARPS * ring(nt) + (size_t)nt * 8 * QP * 2; }
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
+__global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
                                                                int chunk, int shares, int shared_parts, int join) {
     using L = LaneSmem<D>;
     using P = Pair<T>;
-    constexpr int ITEMS = NT * 8, RING = (L::STAGES * L::STAGE > ITEMS * (L::OP + 2) * 4 ? L::STAGES * L::STAGE : ITEMS * (L::OP + 2) * 4);
+    constexpr int ITEMS = NT * 8, RING = L::ring(NT), kWarps = L::WARPS;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[kWarps * L::STAGES];
     uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -194,37 +196,24 @@ __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_con
     const int item0 = blockIdx.z * ITEMS, n_items = min(ITEMS, at.n * g - item0);
     if (n_items <= 0) return;
     const int first_key = a.shared;
-    if (tid == 0) {
-        for (int i = 0; i < kWarps * L::STAGES; ++i) bar_init(&bars[i], 1);
-        bar_init_fence();
-    }
     const int p0 = at.position + item0 / g, p1 = at.position + (item0 + n_items - 1) / g;
     const int lo = max(first_key + share * chunk, attention_first_key(max(p0, 0), a.window, 0)), hi = min(min(p1 + 1, at.keys), shares > 1 ? first_key + (share + 1) * chunk : INT_MAX);
     const int begin = lo / kTile * kTile, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0;
     const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
 
-    for (int i = tid; i < ITEMS * (D / 8); i += kWarps * 32) {
-        const int item = i / (D / 8), c = (i - item * (D / 8)) * 8;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (item < n_items) {
-            const int r = (item0 + item) / g, hq = (item0 + item) - r * g;
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(at.first + r) * a.ldq + (kvh * g + hq) * D + c);
-        }
-        *reinterpret_cast<uint4*>(qs + item * L::QP + c) = v;
-    }
-    __syncthreads();
-
     uint8_t* ring = rings + warp * RING;
     uint64_t* full = bars + warp * L::STAGES;
     const int32_t* table = a.tables + lane_id * a.ld_table;
-    auto load_tile = [&](int i) {   // one lane
+    auto page_row = [&](int i) {
         const int pos = begin + (warp + kWarps * i) * kTile;
         int32_t page = table[pos >> a.bt_shift];
         if ((uint32_t)page >= (uint64_t)a.pool_pages) {
             tell(a.status, kDevBadPage);
             page = 0;
         }
-        const int row = (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
+        return (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
+    };
+    auto load_tile = [&](int i, int row) {   // one lane
         const int st = i % L::STAGES;
         const uint32_t dst = smem_u32(ring) + st * L::STAGE;
         bar_expect_tx(&full[st], L::STAGE);
@@ -234,8 +223,28 @@ __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_con
             tma_load_2d(dst + L::K_BYTES + p * (kTile * 128), &tm_v, p * 64, row, &full[st]);
         }
     };
-    if (lane == 0)
-        for (int i = 0; i < L::STAGES && i < my_tiles; ++i) load_tile(i);
+    int next_row = 0;   // of the tile that the ring takes next
+    if (lane == 0 && my_tiles > 0) {
+        int rows[L::STAGES + 1];
+#pragma unroll
+        for (int i = 0; i <= L::STAGES; ++i) rows[i] = i < my_tiles ? page_row(i) : 0;
+        for (int i = 0; i < L::STAGES; ++i) bar_init(&full[i], 1);
+        bar_init_fence();
+#pragma unroll
+        for (int i = 0; i < L::STAGES; ++i)
+            if (i < my_tiles) load_tile(i, rows[i]);
+        next_row = rows[L::STAGES];
+    }
+    for (int i = tid; i < ITEMS * (D / 8); i += L::THREADS) {
+        const int item = i / (D / 8), c = (i - item * (D / 8)) * 8;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (item < n_items) {
+            const int r = (item0 + item) / g, hq = (item0 + item) - r * g;
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(at.first + r) * a.ldq + (kvh * g + hq) * D + c);
+        }
+        *reinterpret_cast<uint4*>(qs + item * L::QP + c) = v;
+    }
+    __syncthreads();
 
     float o_acc[NT][D / 16][4], m_run[NT][2], l_run[NT][2];
     int see_lo[NT][2], see_hi[NT][2];   // keys that the lane's two items of a group of eight see
@@ -337,7 +346,10 @@ __global__ void __launch_bounds__(kWarps * 32) lane_keys_kernel(const __grid_con
             for (int n = 0; n < NT; ++n) P::mma(o_acc[n][j], af, b0[n], b1[n]);
         }
         __syncwarp();
-        if (lane == 0 && i + L::STAGES < my_tiles) load_tile(i + L::STAGES);
+        if (lane == 0 && i + L::STAGES < my_tiles) {
+            load_tile(i + L::STAGES, next_row);
+            if (i + L::STAGES + 1 < my_tiles) next_row = page_row(i + L::STAGES + 1);
+        }
     }
     if (!ok) {   // what this warp still has under way lands before the CTA ends; the result says so
         for (int i = 0; i < L::STAGES; ++i)
@@ -750,10 +762,11 @@ void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtens
     auto* kernel = lane_keys_kernel<T, D, NT>;
     const size_t smem = LaneSmem<D>::bytes(NT);
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    constexpr int threads = LaneSmem<D>::THREADS;
     const dim3 grid((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles);
     // behind the shared keys' kernel it starts early: what both read was there before that one
-    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(kWarps * 32), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
-    else kernel<<<grid, kWarps * 32, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
+    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(threads), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
+    else kernel<<<grid, threads, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
     MK_LAUNCH_CHECK();
 }
 
