@@ -114,7 +114,7 @@ __device__ __forceinline__ LaneRange lane_range(const SharedAttnArgs& a, int lan
 }
 
 // The parts [first, first + parts) of a row's results, added to a warp's (m, l, o), V values of o per thread.
-template <int D>
+template <int D, int AHEAD>
 __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, int parts, float& m, float& l, float (&o)[D / 32]) {
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
         for (int j = 0; j < V; ++j) o[j] *= old;
         m = m_new;
         const int n = min(32, parts - s0);
-        constexpr int AHEAD = 32 / V;   // parts on their way together; one without keys wrote no output
+        // AHEAD parts on their way together; one without keys wrote no output
         for (int b = 0; b < n; b += AHEAD) {
             float x[AHEAD][V], w[AHEAD];
 #pragma unroll
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
         }
         const int64_t row = at.first + r, head = kvh * g + hq;
         if (join) {
-            add_parts<D>(a, row * a.q_heads + head, shared_parts, m, l, o);
+            add_parts<D, 256 / D * 4>(a, row * a.q_heads + head, shared_parts, m, l, o);
             store_row<T, V>(static_cast<T*>(a.out) + row * a.ldo + head * D + lane * V, o, l);
         } else {
             const int64_t slot = ((int64_t)(shared_parts + share) * a.total + row) * a.q_heads + head;
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
     float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = 0.f;
-    add_parts<D>(a, row, parts, m, l, o);
+    add_parts<D, 32 / (D / 64)>(a, row, parts, m, l, o);
     store_row<T, V>(static_cast<T*>(a.out) + token * a.ldo + (row - (int64_t)token * a.q_heads) * D + lane * V, o, l);
 }
 
@@ -471,7 +471,8 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = a.q_heads / a.kv_heads;
     const int split = blockIdx.x % splits, kvh = blockIdx.x / splits % a.kv_heads, tile = blockIdx.x / splits / a.kv_heads;
     pdl_trigger();
-    if (tid == 0) {
+    const int all_tiles = (a.shared + KEYS - 1) / KEYS, first_tile = (int)((int64_t)all_tiles * split / splits), last_tile = (int)((int64_t)all_tiles * (split + 1) / splits);
+    if (warp == L::WARPS && lane == 0) {
         for (int i = 0; i < ST; ++i) {
             bar_init(&k_full[i], 1);
             bar_init(&k_empty[i], NQ);
@@ -485,6 +486,54 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
         bar_init(q_full, L::WARPS);
         bar_init_fence();
+    }
+    // The queries' pieces and the first tiles of keys and values are on their way before anything else is looked at (one after the other the queries took 0.6 us a piece, 10 us at
+    // heads of 128).
+    const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most four boxes of each of the panels: 16
+    const bool brings = warp == L::WARPS && panel < L::PANELS;
+    auto page_row = [&](int t) {
+        int pos = t * KEYS + of * box;
+        if (pos >= a.shared) pos = a.shared - box;   // keys behind the last one are not seen; they are read from where there is something
+        int32_t page = brings && t < last_tile ? a.tables[pos >> a.bt_shift] : 0;
+        if ((uint32_t)page >= (uint64_t)a.pool_pages) {
+            tell(a.status, kDevBadPage);
+            page = 0;
+        }
+        return (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
+    };
+    auto bring_k = [&](int st, int row) {
+        if (lane == 0) bar_expect_tx(&k_full[st], L::BYTES);
+        __syncwarp();
+        if (brings) tma_load_2d(smem_u32(ks) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_k, panel * 64, row, &k_full[st]);
+    };
+    auto bring_v = [&](int st, int row) {
+        if (lane == 0) bar_expect_tx(&v_full[st], L::BYTES);
+        __syncwarp();
+        if (brings) tma_load_2d(smem_u32(vs) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_v, panel * 64, row, &v_full[st]);
+    };
+    int early = 0;   // tiles asked for here; where there is a window, what is seen has to be known first
+    if (warp == L::WARPS && a.window == 0) {
+        __syncwarp();
+        early = min(ST, last_tile - first_tile);
+        int rows[ST];
+#pragma unroll
+        for (int i = 0; i < ST; ++i) rows[i] = page_row(first_tile + i);
+#pragma unroll
+        for (int i = 0; i < ST; ++i)
+            if (i < early) {
+                bring_k(i, rows[i]);
+                bring_v(i, rows[i]);
+            }
+    }
+    if (warp < L::WARPS) {
+#pragma unroll 4
+        for (int i = tid; i < NQ * kItems * (D / 8); i += L::WARPS * 32) {
+            const int it = i / (D / 8), c = (i - it * (D / 8)) * 8, r = it % kItems;
+            const int index = tile * (NQ * kItems) + it, tok = index / g;   // total * q_heads is far below 2^31
+            const bool there = tok < a.total;
+            const T* src = static_cast<const T*>(a.q) + (there ? tok * a.ldq + (kvh * g + (index - tok * g)) * D + c : 0);
+            cp_async16(smem_u32(qs) + (it / kItems * L::PANELS + (c >> 6)) * L::QPANEL + r * 128 + (((c & 63) * 2) ^ ((r & 7) << 4)), src, there);
+        }
     }
     // what this thread's item is, and what it sees
     const int q = warp >> 2, item = tile * (NQ * kItems) + tid;
@@ -531,44 +580,22 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         hi_min = min(hi_min, sees[w].z);
         hi_max = max(hi_max, sees[w].w);
     }
-    const int all_tiles = (a.shared + KEYS - 1) / KEYS;
-    const int t_begin = max((int)((int64_t)all_tiles * split / splits), lo_min / KEYS);
-    const int t_end = min((int)((int64_t)all_tiles * (split + 1) / splits), (hi_max + KEYS - 1) / KEYS);
+    const int t_begin = a.window == 0 ? first_tile : max(first_tile, lo_min / KEYS), t_end = a.window == 0 ? last_tile : min(last_tile, (hi_max + KEYS - 1) / KEYS);
     const int n_tiles = max(0, t_end - t_begin);
 
     if (warp == L::WARPS) {
         // ---- loader
-        const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most four boxes of each of the panels: 16
-        const bool mine = panel < L::PANELS;
-        auto page_row = [&](int t) {
-            int pos = (t_begin + t) * KEYS + of * box;
-            if (pos >= a.shared) pos = a.shared - box;   // keys behind the last one are not seen; they are read from where there is something
-            int32_t page = mine && t < n_tiles ? a.tables[pos >> a.bt_shift] : 0;
-            if ((uint32_t)page >= (uint64_t)a.pool_pages) {
-                tell(a.status, kDevBadPage);
-                page = 0;
-            }
-            return (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
-        };
-        if (lane == 0) {
-            prefetch_tensormap(&tm_k);
-            prefetch_tensormap(&tm_v);
-        }
         bool ok = true;
-        int t = 0, row = page_row(0);
+        int t = early, row = page_row(t_begin + t);
         for (; t < n_tiles; ++t) {
-            const int next = page_row(t + 1), st = t % ST;
+            const int next = page_row(t_begin + t + 1), st = t % ST;
             const uint32_t ph = (uint32_t)(t / ST & 1) ^ 1;
             ok = __all_sync(0xffffffffu, bar_wait(&k_empty[st], ph));
             if (!ok) break;
-            if (lane == 0) bar_expect_tx(&k_full[st], L::BYTES);
-            __syncwarp();
-            if (mine) tma_load_2d(smem_u32(ks) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_k, panel * 64, row, &k_full[st]);
+            bring_k(st, row);
             ok = __all_sync(0xffffffffu, bar_wait(&v_empty[st], ph));
             if (!ok) break;
-            if (lane == 0) bar_expect_tx(&v_full[st], L::BYTES);
-            __syncwarp();
-            if (mine) tma_load_2d(smem_u32(vs) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_v, panel * 64, row, &v_full[st]);
+            bring_v(st, row);
             row = next;
         }
         if (!ok) {
@@ -627,15 +654,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (!ok && lane == 0) tell(a.status, kDevWait);
         }
     } else {
-        // ---- softmax, an item per thread.  The queries' pieces first, all on their way together: one after the other they took 0.6 us each, 10 us at heads of 128
-#pragma unroll 4
-        for (int i = tid; i < NQ * kItems * (D / 8); i += L::WARPS * 32) {
-            const int it = i / (D / 8), c = (i - it * (D / 8)) * 8, r = it % kItems;
-            const int index = tile * (NQ * kItems) + it, tok = index / g;   // total * q_heads is far below 2^31
-            const bool there = tok < a.total;
-            const T* src = static_cast<const T*>(a.q) + (there ? tok * a.ldq + (kvh * g + (index - tok * g)) * D + c : 0);
-            cp_async16(smem_u32(qs) + (it / kItems * L::PANELS + (c >> 6)) * L::QPANEL + r * 128 + (((c & 63) * 2) ^ ((r & 7) << 4)), src, there);
-        }
+        // ---- softmax, an item per thread
         cp_async_wait_all();
         fence_async_smem();
         __syncwarp();
@@ -805,7 +824,7 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
     p.item_tiles = (int)((items + p.items - 1) / p.items);
     // A lane's own keys: whole where the lanes fill the device, else in shares of at least 256 keys; never more than 1024, since lanes differ in length.
     const int64_t keys = (int64_t)width * block_tokens - shared, ctas = (int64_t)lanes * kv_heads * p.item_tiles;
-    const int64_t wanted = std::max<int64_t>(1, (4 * kSms + ctas - 1) / ctas);
+    const int64_t wanted = std::max<int64_t>(1, (3 * kSms / 2 + ctas - 1) / ctas);
     p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), 1024) / 16 * 16;
     p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
     if (shared > 0) {
