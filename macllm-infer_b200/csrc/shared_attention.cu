@@ -479,13 +479,20 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             bar_init(&v_full[i], 1);
             bar_init(&v_empty[i], NQ);
         }
-        for (int i = 0; i < AREAS; ++i) {
-            bar_init(&s_full[i], 1);
-            bar_init(&p_full[i], 4);
-            bar_init(&o_done[i], 1);
-        }
-        bar_init(q_full, L::WARPS);
         bar_init_fence();
+    }
+    if (warp == L::WARPS + 1) {
+        if (lane == 0) {
+            for (int i = 0; i < 2 * NQ; ++i) {
+                bar_init(&s_full[i], 1);
+                bar_init(&p_full[i], 4);
+                bar_init(&o_done[i], 1);
+            }
+            bar_init(q_full, L::WARPS);
+            bar_init_fence();
+        }
+        __syncwarp();
+        tmem_alloc(&tmem_slot, L::TMEM);
     }
     // The queries' pieces and the first tiles of keys and values are on their way before anything else is looked at (one after the other the queries took 0.6 us a piece, 10 us at
     // heads of 128).
@@ -514,6 +521,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     int early = 0;   // tiles asked for here; where there is a window, what is seen has to be known first
     if (warp == L::WARPS && a.window == 0) {
         __syncwarp();
+        asm volatile("bar.arrive 15, %0;" ::"n"(L::THREADS) : "memory");
         early = min(ST, last_tile - first_tile);
         int rows[ST];
 #pragma unroll
@@ -525,21 +533,23 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 bring_v(i, rows[i]);
             }
     }
+    const int q = warp >> 2, item = tile * (NQ * kItems) + tid, at_token = item / g;   // total * q_heads is far below 2^31
     if (warp < L::WARPS) {
-#pragma unroll 4
-        for (int i = tid; i < NQ * kItems * (D / 8); i += L::WARPS * 32) {
-            const int it = i / (D / 8), c = (i - it * (D / 8)) * 8, r = it % kItems;
-            const int index = tile * (NQ * kItems) + it, tok = index / g;   // total * q_heads is far below 2^31
-            const bool there = tok < a.total;
-            const T* src = static_cast<const T*>(a.q) + (there ? tok * a.ldq + (kvh * g + (index - tok * g)) * D + c : 0);
-            cp_async16(smem_u32(qs) + (it / kItems * L::PANELS + (c >> 6)) * L::QPANEL + r * 128 + (((c & 63) * 2) ^ ((r & 7) << 4)), src, there);
+        // eight threads to a piece of 128 bytes; where a row is comes from the thread whose item it is
+        const int64_t mine = at_token < a.total ? at_token * a.ldq + (kvh * g + item - at_token * g) * D : -1;
+        const uint32_t to = smem_u32(qs) + q * L::PANELS * L::QPANEL + (warp & 3) * 32 * 128;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int r = k * 4 + lane / 8, c = lane % 8;
+            const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+#pragma unroll
+            for (int p = 0; p < L::PANELS; ++p)
+                cp_async16(to + p * L::QPANEL + r * 128 + ((c ^ (r & 7)) << 4), static_cast<const T*>(a.q) + (at < 0 ? 0 : at + p * 64 + c * 8), at >= 0);
         }
     }
     // what this thread's item is, and what it sees
-    const int q = warp >> 2, item = tile * (NQ * kItems) + tid;
     int token = -1, head = 0, see_lo = 0, see_hi = 0;
     if (warp < L::WARPS) {
-        const int at_token = item / g;
         if (at_token < a.total) {
             int l = 0;
             if (a.cu == nullptr) {
@@ -567,9 +577,9 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                                  __reduce_min_sync(0xffffffffu, token >= 0 ? see_hi : INT_MAX), __reduce_max_sync(0xffffffffu, live ? see_hi : 0));
         if (lane == 0) sees[warp] = s;
     }
-    if (warp == L::WARPS + 1) tmem_alloc(&tmem_slot, L::TMEM);
     fence_before();
-    __syncthreads();
+    // nobody waits for the loader's first requests, and it needs nothing of the others where there is no window
+    if (warp != L::WARPS || a.window != 0) asm volatile("bar.sync 15, %0;" ::"n"(L::THREADS) : "memory");
     fence_after();
     const uint32_t tmem = tmem_slot;
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
@@ -742,16 +752,29 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         fence_after();
         const int64_t slot = ((int64_t)split * a.total + token) * a.q_heads + head;
         if (token >= 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
-        if (n_tiles > 0) {
+        if (n_tiles > 0 && __any_sync(0xffffffffu, token >= 0)) {
+            // Rows go out through where the queries were, half a row at a time, so that a warp writes whole rows (a thread a row: 2.6 us for heads of 128).
+            constexpr int HALF = D / 2, PIECES = HALF / 4;   // values and 16-byte pieces of half a row
+            float4* stage = reinterpret_cast<float4*>(qs + q * L::PANELS * L::QPANEL) + (warp & 3) * 32 * PIECES;
+            const int64_t mine = token < 0 ? -1 : slot * D;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(o_at + c, o);
-                tmem_wait_ld();
-                if (token < 0) continue;
+            for (int half = 0; half < 2; ++half) {
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<uint4*>(a.part_o + slot * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                for (int c = 0; c < HALF; c += 32) {
+                    float o[32];
+                    tmem_ld32(o_at + half * HALF + c, reinterpret_cast<uint32_t*>(o));
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) stage[lane * PIECES + ((c / 4 + j) ^ (lane & 7))] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = lane; i < 32 * PIECES; i += 32) {
+                    const int r = i / PIECES, c = i % PIECES;
+                    const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+                    if (at >= 0) *reinterpret_cast<float4*>(a.part_o + at + half * HALF + c * 4) = stage[r * PIECES + (c ^ (r & 7))];
+                }
             }
         }
     }
@@ -828,17 +851,16 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
     p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), 1024) / 16 * 16;
     p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
     if (shared > 0) {
-        // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.35 us per
-        // tile of items, its start and end 4 us, and a share's results are written and read once.
+        // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.7 us, or 1 us for two tiles of items, its start and end 4 us, and a share's results are written and read once (2.5 TB/s, and 0.1 us).
         const int64_t all = (int64_t)total * g;
         p.item_rows = d <= 128 && all > kItems ? 2 : 1;
         p.row_tiles = (int)((all + kItems * p.item_rows - 1) / (kItems * p.item_rows));
         const int tiles = (shared + kKeys - 1) / kKeys;
-        const double results_us = (double)total * q_heads * d * 8 / 8e6;
+        const double results_us = 0.1 + (double)total * q_heads * d * 8 / 2.5e6;
         double best = 0;
         for (int n = 1; n <= std::min(tiles, 148); ++n) {
             const int64_t slots = d <= 128 && p.item_rows == 1 ? 2 * kSms : kSms, waves = ((int64_t)p.row_tiles * kv_heads * n + slots - 1) / slots;
-            const double us = waves * ((tiles + n - 1) / n * 0.35 * p.item_rows + 4.0) + n * results_us;
+            const double us = waves * ((tiles + n - 1) / n * (p.item_rows == 2 ? 1.0 : 0.7) + 4.0) + n * results_us;
             if (n == 1 || us < best) best = us, p.shared_parts = n;
         }
     }
