@@ -807,8 +807,8 @@ void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtens
     constexpr int threads = LaneSmem<D>::THREADS;
     const dim3 grid((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles);
     // behind the shared keys' kernel it starts early: what both read was there before that one
-    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(threads), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
-    else kernel<<<grid, threads, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.shares == 1 ? 1 : 0);
+    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(threads), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1);
+    else kernel<<<grid, threads, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1);
     MK_LAUNCH_CHECK();
 }
 
@@ -832,7 +832,7 @@ void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t
         default:
             if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, tk, tv, s);
     }
-    if (p.shares > 1)
+    if (p.joined)
         launch_pdl(join_parts_kernel<T, D>, dim3((unsigned)(((int64_t)a.total * a.q_heads + 7) / 8)), dim3(256), 0, s, a, (int)p.parts);
 }
 
@@ -864,7 +864,10 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
             if (n == 1 || us < best) best = us, p.shared_parts = n;
         }
     }
-    p.parts = p.shared_parts + (p.shares > 1 ? p.shares : 0);
+    // A lane's CTA joins the parts itself where its warps have at most two rows each to join, one after the other (1 lane, 5 rows of 2 heads of 256 each behind 768 shared tokens:
+    // 20 us so, JOINED with a kernel of its own).
+    p.joined = p.shares > 1 || (p.shared_parts > 0 && items > (d == 256 ? 4 : 8));
+    p.parts = p.shared_parts + (p.joined ? p.shares : 0);
     return p;
 }
 

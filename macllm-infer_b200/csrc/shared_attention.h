@@ -39,6 +39,7 @@ struct SharedAttnPlan {
     int items = 0;           // items of such a block, a multiple of 8
     int chunk = 0, shares = 0;   // keys of a lane's share, and shares
     int item_rows = 0, row_tiles = 0, shared_parts = 0;   // shared keys: tiles of items to a CTA, CTAs along the items, shares of the keys
+    bool joined = false;     // by a kernel of its own
     int64_t parts = 0;       // partial results of a row; 0: none are written
     int64_t bytes(int total, int q_heads, int d) const { return parts * total * q_heads * ((int64_t)d * 4 + 8); }
 };
