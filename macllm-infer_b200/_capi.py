@@ -282,7 +282,7 @@ SIGNATURES = {
     "mk_state_slots_query": (_i32, [P, C.POINTER(_i32), C.POINTER(_i32)]),
     "mk_k_router_logits": (_i32, [P, _i32, _i32, P, _i32, P]),
     "mk_k_moe_route": (_i32, [P, _i32, _i32, _i32, P, P]),
-    "mk_k_shared_attention_workspace": (_i32, [_i32] * 9 + [C.POINTER(_i64)]),
+    "mk_k_shared_attention_workspace": (_i32, [_i32] * 10 + [C.POINTER(_i64)]),
     "mk_k_shared_attention_dev": (_i32, [_i32, P, _i64, P, P, _i64, _i64, _i32, _i32, _i32, _i32, P, _i64, _i32, P, P, _i32, _i32, _i32, _i32, _f32, _f32, _i32, P, _i64, P, _i64,
                                          P, P]),
     "mk_k_verify_drafts_workspace": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(_i64)]),

@@ -5,6 +5,7 @@
 #include "kv_rows.h"
 #include "shared_attention.h"
 #include "verify_drafts.h"
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -17,7 +18,8 @@ void need(bool ok, const char* what) {
 }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-SharedAttnPlan checked_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared) {
+SharedAttnPlan checked_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared, int window) {
+    need(window >= 0, "mk_k_shared_attention: window is not negative");
     need(d == 64 || d == 128 || d == 256, "mk_k_shared_attention: head_dim is 64, 128 or 256");
     need(kv_heads > 0 && q_heads > 0 && q_heads % kv_heads == 0, "mk_k_shared_attention: q_heads is a multiple of kv_heads");
     need(q_heads / kv_heads <= 128 && kv_heads <= 65535, "mk_k_shared_attention: at most 128 query heads share a KV head, and there are at most 65535 of those");
@@ -27,8 +29,8 @@ SharedAttnPlan checked_plan(int q_heads, int kv_heads, int d, int block_tokens, 
     need((int64_t)rows * (q_heads / kv_heads) <= 65535, "mk_k_shared_attention: rows of a lane times query heads of a KV head go up to 65535");
     need((int64_t)total * q_heads <= INT32_MAX / 4, "mk_k_shared_attention: too many rows");
     need(shared >= 0 && shared % block_tokens == 0 && shared / block_tokens <= width, "mk_k_shared_attention: shared_len is whole pages of the tables");
-    const SharedAttnPlan p = shared_attention_plan(q_heads, kv_heads, d, block_tokens, width, lanes, rows, total, shared);
-    need((int64_t)lanes * p.shares <= INT32_MAX, "mk_k_shared_attention: too many lanes");
+    const SharedAttnPlan p = shared_attention_plan(q_heads, kv_heads, d, block_tokens, width, lanes, rows, total, shared, window);
+    need((int64_t)lanes * p.shares * std::max(1, p.item_tiles) * kv_heads <= INT32_MAX, "mk_k_shared_attention: too many lanes");
     return p;
 }
 
@@ -46,8 +48,8 @@ VerifyPlan checked_verify_plan(int type, int lanes, int drafts, int vocab) {
 extern "C" {
 
 int32_t mk_k_shared_attention_workspace(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_tokens, int32_t table_width, int32_t lanes, int32_t rows,
-                                        int32_t total, int32_t shared_len, int64_t* bytes) {
-    return guarded([&] { *bytes = checked_plan(q_heads, kv_heads, head_dim, block_tokens, table_width, lanes, rows, total, shared_len).bytes(total, q_heads, head_dim); });
+                                        int32_t total, int32_t shared_len, int32_t window, int64_t* bytes) {
+    return guarded([&] { *bytes = checked_plan(q_heads, kv_heads, head_dim, block_tokens, table_width, lanes, rows, total, shared_len, window).bytes(total, q_heads, head_dim); });
 }
 
 int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_stride, const void* k_pool_dev, const void* v_pool_dev, int64_t pool_pages, int64_t page_stride,
@@ -57,7 +59,7 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
                                   void* cuda_stream) {
     return guarded([&] {
         need(type == MK_TYPE_F16 || type == MK_TYPE_BF16, "mk_k_shared_attention_dev: queries, pools and results are f16 or bf16, all of one type");
-        const SharedAttnPlan p = checked_plan(q_heads, kv_heads, head_dim, block_tokens, table_width, lanes, rows, total, shared_len);
+        const SharedAttnPlan p = checked_plan(q_heads, kv_heads, head_dim, block_tokens, table_width, lanes, rows, total, shared_len, window);
         if (lanes == 0 || total == 0 || rows == 0) return;
         need(q_dev != nullptr && k_pool_dev != nullptr && v_pool_dev != nullptr && lengths_dev != nullptr && out_dev != nullptr && (tables_dev != nullptr || table_width == 0),
              "mk_k_shared_attention_dev: null pointer");
@@ -69,7 +71,7 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
         need(pool_pages <= INT32_MAX && page_stride / head_dim <= INT32_MAX && pool_pages * (page_stride / head_dim) <= INT32_MAX,
              "mk_k_shared_attention_dev: a pool has at most 2^31 - 1 rows of a head");
         need(scale > 0.f && std::isfinite(scale), "mk_k_shared_attention_dev: scale is positive");
-        need(softcap >= 0.f && std::isfinite(softcap) && window >= 0, "mk_k_shared_attention_dev: softcap and window are not negative");
+        need(softcap >= 0.f && std::isfinite(softcap), "mk_k_shared_attention_dev: softcap is not negative");
         const int64_t bytes = p.bytes(total, q_heads, head_dim);
         need(bytes == 0 || (workspace_dev != nullptr && workspace_bytes >= bytes && aligned(workspace_dev, 16)), "mk_k_shared_attention_dev: the workspace is missing, too small or not aligned to 16 bytes");
         require_device();

@@ -454,9 +454,11 @@ struct SharedSmem {
     static constexpr size_t SMEM = 1024 + (size_t)NQ * PANELS * QPANEL + (size_t)STAGES * 2 * BYTES;
 };
 
-template <typename T, int D, int NQ>
+// OWN: the same for one lane's rows and its own keys, where a lane has so many (row, head) items that the small products of lane_keys_kernel would be made over and over.
+template <typename T, int D, int NQ, bool OWN>
 __global__ void __launch_bounds__(SharedSmem<D, NQ>::THREADS, SharedSmem<D, NQ>::CTAS)
-shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a, int box, int splits) {
+shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a, int box, int splits, int chunk,
+                   int lane_tiles, int first_part) {
     using L = SharedSmem<D, NQ>;
     constexpr int ST = L::STAGES, KEYS = kKeys, S_AT = NQ * D, AREAS = 2 * NQ;   // columns of tensor memory: outputs, then the areas
     extern __shared__ uint8_t smem_raw[];
@@ -469,9 +471,16 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     uint8_t* ks = qs + NQ * L::PANELS * L::QPANEL;
     uint8_t* vs = ks + ST * L::BYTES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = a.q_heads / a.kv_heads;
-    const int split = blockIdx.x % splits, kvh = blockIdx.x / splits % a.kv_heads, tile = blockIdx.x / splits / a.kv_heads;
+    const int split = blockIdx.x % splits, kvh = blockIdx.x / splits % a.kv_heads, block = blockIdx.x / splits / a.kv_heads, lane_id = OWN ? block / lane_tiles : 0,
+              tile = OWN ? block - lane_id * lane_tiles : block;
     pdl_trigger();
-    const int all_tiles = (a.shared + KEYS - 1) / KEYS, first_tile = (int)((int64_t)all_tiles * split / splits), last_tile = (int)((int64_t)all_tiles * (split + 1) / splits);
+    const LaneRange mine_range = OWN ? lane_range(a, lane_id) : LaneRange{0, a.total, 0, 0};
+    if (OWN && tile * (NQ * kItems) >= mine_range.n * g) return;
+    const int base_key = OWN ? a.shared : 0, keys_end = OWN ? min(mine_range.keys, a.shared + (split + 1) * chunk) : a.shared;   // positions of tiles are counted from the first
+    const int32_t* table = a.tables + lane_id * a.ld_table;
+    constexpr bool kEarly = !OWN;
+    const int all_tiles = (a.shared + KEYS - 1) / KEYS, first_tile = OWN ? split * chunk / KEYS : (int)((int64_t)all_tiles * split / splits),
+              last_tile = OWN ? max(first_tile, (keys_end - base_key + KEYS - 1) / KEYS) : (int)((int64_t)all_tiles * (split + 1) / splits);
     if (warp == L::WARPS && lane == 0) {
         for (int i = 0; i < ST; ++i) {
             bar_init(&k_full[i], 1);
@@ -498,10 +507,11 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // heads of 128).
     const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most four boxes of each of the panels: 16
     const bool brings = warp == L::WARPS && panel < L::PANELS;
+    const int most_tiles = a.window != 0 && !OWN ? all_tiles : last_tile;
     auto page_row = [&](int t) {
-        int pos = t * KEYS + of * box;
-        if (pos >= a.shared) pos = a.shared - box;   // keys behind the last one are not seen; they are read from where there is something
-        int32_t page = brings && t < last_tile ? a.tables[pos >> a.bt_shift] : 0;
+        int pos = base_key + t * KEYS + of * box;
+        if (pos >= keys_end) pos = (keys_end - 1) / box * box;   // keys behind the last one are not seen; they are read from where there is something
+        int32_t page = brings && t < most_tiles ? table[pos >> a.bt_shift] : 0;
         if ((uint32_t)page >= (uint64_t)a.pool_pages) {
             tell(a.status, kDevBadPage);
             page = 0;
@@ -519,7 +529,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         if (brings) tma_load_2d(smem_u32(vs) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_v, panel * 64, row, &v_full[st]);
     };
     int early = 0;   // tiles asked for here; where there is a window, what is seen has to be known first
-    if (warp == L::WARPS && a.window == 0) {
+    if (kEarly && warp == L::WARPS && a.window == 0) {
         __syncwarp();
         asm volatile("bar.arrive 15, %0;" ::"n"(L::THREADS) : "memory");
         early = min(ST, last_tile - first_tile);
@@ -533,10 +543,11 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 bring_v(i, rows[i]);
             }
     }
-    const int q = warp >> 2, item = tile * (NQ * kItems) + tid, at_token = item / g;   // total * q_heads is far below 2^31
+    const int q = warp >> 2, item = tile * (NQ * kItems) + tid, at_row = item / g, at_token = mine_range.first + at_row;   // total * q_heads is far below 2^31
+    const bool exists = at_row < mine_range.n;   // of the batch, or of the lane
     if (warp < L::WARPS) {
         // eight threads to a piece of 128 bytes; where a row is comes from the thread whose item it is
-        const int64_t mine = at_token < a.total ? at_token * a.ldq + (kvh * g + item - at_token * g) * D : -1;
+        const int64_t mine = exists ? at_token * a.ldq + (kvh * g + item - at_row * g) * D : -1;
         const uint32_t to = smem_u32(qs) + q * L::PANELS * L::QPANEL + (warp & 3) * 32 * 128;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -550,26 +561,28 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // what this thread's item is, and what it sees
     int token = -1, head = 0, see_lo = 0, see_hi = 0;
     if (warp < L::WARPS) {
-        if (at_token < a.total) {
-            int l = 0;
-            if (a.cu == nullptr) {
-                l = at_token / a.rows;
-            } else {   // the last lane that begins at or before this row
-                int lo = 0, hi = a.lanes;
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) / 2;
-                    if (a.cu[mid] <= at_token) lo = mid;
-                    else hi = mid;
+        if (exists) {
+            LaneRange at = mine_range;
+            if (!OWN) {
+                int l = 0;
+                if (a.cu == nullptr) {
+                    l = at_token / a.rows;
+                } else {   // the last lane that begins at or before this row
+                    int hi = a.lanes;
+                    while (hi - l > 1) {
+                        const int mid = (l + hi) / 2;
+                        if (a.cu[mid] <= at_token) l = mid;
+                        else hi = mid;
+                    }
                 }
-                l = lo;
+                at = lane_range(a, l);
             }
-            const LaneRange at = lane_range(a, l);
             if (at_token >= at.first && at_token < at.first + at.n) {
                 token = at_token;
-                head = kvh * g + item - at_token * g;
+                head = kvh * g + item - at_row * g;
                 const int p = at.position + token - at.first;
-                see_lo = attention_first_key(max(p, 0), a.window, 0);
-                see_hi = min(a.shared, p + 1);
+                see_lo = max(base_key, attention_first_key(max(p, 0), a.window, 0));
+                see_hi = min(keys_end, p + 1);
             }
         }
         const bool live = token >= 0 && see_hi > see_lo;
@@ -579,7 +592,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     fence_before();
     // nobody waits for the loader's first requests, and it needs nothing of the others where there is no window
-    if (warp != L::WARPS || a.window != 0) asm volatile("bar.sync 15, %0;" ::"n"(L::THREADS) : "memory");
+    if (!kEarly || warp != L::WARPS || a.window != 0) asm volatile("bar.sync 15, %0;" ::"n"(L::THREADS) : "memory");
     fence_after();
     const uint32_t tmem = tmem_slot;
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
@@ -590,7 +603,12 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         hi_min = min(hi_min, sees[w].z);
         hi_max = max(hi_max, sees[w].w);
     }
-    const int t_begin = a.window == 0 ? first_tile : max(first_tile, lo_min / KEYS), t_end = a.window == 0 ? last_tile : min(last_tile, (hi_max + KEYS - 1) / KEYS);
+    int t_begin = first_tile, t_end = last_tile;
+    if (a.window != 0) {   // only what some item sees, shared out anew where all CTAs of the same items see it alike
+        const int low = (min(lo_min, INT_MAX / 2) - base_key) / KEYS, high = (hi_max - base_key + KEYS - 1) / KEYS;
+        t_begin = OWN ? max(first_tile, low) : low + (int)((int64_t)max(0, high - low) * split / splits);
+        t_end = OWN ? min(last_tile, high) : low + (int)((int64_t)max(0, high - low) * (split + 1) / splits);
+    }
     const int n_tiles = max(0, t_end - t_begin);
 
     if (warp == L::WARPS) {
@@ -686,7 +704,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             tmem_ld32(s_at, reinterpret_cast<uint32_t*>(s));
             tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s) + 32);
             tmem_wait_ld();
-            const int pos0 = (t_begin + t) * KEYS;
+            const int pos0 = base_key + (t_begin + t) * KEYS;
             if (a.softcap != 0.f) {
 #pragma unroll
                 for (int j = 0; j < KEYS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
@@ -735,6 +753,14 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (NQ == 2 && (q == 0 || t + 1 < n_tiles)) pair_arrive(turn + 1 - q);
             tmem_st32(s_at, w);
             sum += (part[0] + part[1]) + (part[2] + part[3]);
+            if (OWN && pos0 + KEYS > keys_end) {
+                // behind the lane's last key a page holds whatever it held: weights of 0 need finite values there
+                ok = ok && bar_wait(&v_full[t % ST], t / ST & 1);
+                const int first = max(0, keys_end - pos0), pieces = (KEYS - first) * 8;
+                for (int i = tid & 127; i < pieces * L::PANELS; i += 128)
+                    *reinterpret_cast<uint4*>(vs + (t % ST) * L::BYTES + i / pieces * L::PANEL + first * 128 + i % pieces * 16) = make_uint4(0u, 0u, 0u, 0u);
+                fence_async_smem();
+            }
             tmem_wait_st();
             fence_before();
             __syncwarp();
@@ -750,7 +776,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             sum = m_run = __int_as_float(0x7fffffff);   // the result says so
         }
         fence_after();
-        const int64_t slot = ((int64_t)split * a.total + token) * a.q_heads + head;
+        const int64_t slot = ((int64_t)(first_part + split) * a.total + token) * a.q_heads + head;
         if (token >= 0) a.part_ml[slot] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_run, sum);
         if (n_tiles > 0 && __any_sync(0xffffffffu, token >= 0)) {
             // Rows go out through where the queries were, half a row at a time, so that a warp writes whole rows (a thread a row: 2.6 us for heads of 128).
@@ -778,6 +804,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
         }
     }
+    if (OWN) pdl_wait();   // who comes after this kernel relies on the one before it too
     fence_before();
     __syncthreads();
     if (warp == L::WARPS + 1) {
@@ -786,16 +813,23 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
 }
 
-template <typename T, int D, int NQ>
-void launch_shared_part(const SharedAttnArgs& a, const SharedAttnPlan& p, uint64_t rows, cudaStream_t s) {
+template <typename T, int D, int NQ, bool OWN>
+void launch_tall(const SharedAttnArgs& a, const SharedAttnPlan& p, uint64_t rows, cudaStream_t s) {
     using L = SharedSmem<D, NQ>;
     const int box = std::min(a.block_tokens, kKeys);
     alignas(64) CUtensorMap tk, tv;
     encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, (uint32_t)box, true);
     encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, (uint32_t)box, true);
-    auto* kernel = shared_keys_kernel<T, D, NQ>;
+    auto* kernel = shared_keys_kernel<T, D, NQ, OWN>;
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::SMEM);
-    kernel<<<(unsigned)(p.row_tiles * a.kv_heads * p.shared_parts), L::THREADS, L::SMEM, s>>>(tk, tv, a, box, p.shared_parts);
+    if (!OWN) {
+        kernel<<<(unsigned)(p.row_tiles * a.kv_heads * p.shared_parts), L::THREADS, L::SMEM, s>>>(tk, tv, a, box, p.shared_parts, 0, 0, 0);
+        MK_LAUNCH_CHECK();
+        return;
+    }
+    const unsigned grid = (unsigned)(a.lanes * p.item_tiles * a.kv_heads * p.shares);
+    if (p.shared_parts > 0) launch_pdl(kernel, dim3(grid), dim3(L::THREADS), L::SMEM, s, tk, tv, a, box, p.shares, p.chunk, p.item_tiles, p.shared_parts);
+    else kernel<<<grid, L::THREADS, L::SMEM, s>>>(tk, tv, a, box, p.shares, p.chunk, p.item_tiles, 0);
     MK_LAUNCH_CHECK();
 }
 
@@ -817,20 +851,29 @@ void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t
     const uint64_t rows = (uint64_t)(a.pool_pages - 1) * (uint64_t)a.page_rows + (uint64_t)a.kv_heads * (uint64_t)a.block_tokens;
     if (p.shared_parts > 0) {
         if constexpr (D <= 128) {
-            if (p.item_rows == 2) launch_shared_part<T, D, 2>(a, p, rows, s);
-            else launch_shared_part<T, D, 1>(a, p, rows, s);
+            if (p.item_rows == 2) launch_tall<T, D, 2, false>(a, p, rows, s);
+            else launch_tall<T, D, 1, false>(a, p, rows, s);
         } else {
-            launch_shared_part<T, D, 1>(a, p, rows, s);
+            launch_tall<T, D, 1, false>(a, p, rows, s);
         }
     }
-    alignas(64) CUtensorMap tk, tv;
-    encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, kTile, true);
-    encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, kTile, true);
-    switch (p.items) {
-        case 8: launch_lanes<T, D, 1>(a, p, tk, tv, s); break;
-        case 16: launch_lanes<T, D, 2>(a, p, tk, tv, s); break;
-        default:
-            if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, tk, tv, s);
+    if (p.items >= kItems) {
+        if constexpr (D <= 128) {
+            if (p.items > kItems) launch_tall<T, D, 2, true>(a, p, rows, s);
+            else launch_tall<T, D, 1, true>(a, p, rows, s);
+        } else {
+            launch_tall<T, D, 1, true>(a, p, rows, s);
+        }
+    } else {
+        alignas(64) CUtensorMap tk, tv;
+        encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, kTile, true);
+        encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, kTile, true);
+        switch (p.items) {
+            case 8: launch_lanes<T, D, 1>(a, p, tk, tv, s); break;
+            case 16: launch_lanes<T, D, 2>(a, p, tk, tv, s); break;
+            default:
+                if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, tk, tv, s);
+        }
     }
     if (p.joined)
         launch_pdl(join_parts_kernel<T, D>, dim3((unsigned)(((int64_t)a.total * a.q_heads + 7) / 8)), dim3(256), 0, s, a, (int)p.parts);
@@ -838,24 +881,33 @@ void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t
 
 }  // namespace
 
-SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared) {
+SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared, int window) {
     SharedAttnPlan p;
     const int g = q_heads / kv_heads;
     const int64_t items = (int64_t)rows * g;
     if (items <= 0 || lanes <= 0 || total <= 0) return p;
-    p.items = (int)std::min<int64_t>((items + 7) / 8 * 8, d == 256 ? 16 : 24);
-    p.item_tiles = (int)((items + p.items - 1) / p.items);
-    // A lane's own keys: whole where the lanes fill the device, else in shares of at least 256 keys; never more than 1024, since lanes differ in length.
-    const int64_t keys = (int64_t)width * block_tokens - shared, ctas = (int64_t)lanes * kv_heads * p.item_tiles;
-    const int64_t wanted = std::max<int64_t>(1, (3 * kSms / 2 + ctas - 1) / ctas);
-    p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), 1024) / 16 * 16;
+    const int64_t keys = (int64_t)width * block_tokens - shared;
+    if (items > 24 || (items > 16 && (d == 256 || lanes * (int64_t)kv_heads >= kSms))) {
+        // Lanes of more items than the small products take at once (17 to 24: where lanes fill the device; 31 lanes of 20 items 39 us so, 47 with the others, 24 lanes 54 and 50): tiles of 128 or 256 of them, and their keys in shares until about two CTAs are there for each place on an SM
+        p.items = d <= 128 && items > kItems ? 2 * kItems : kItems;
+        p.item_tiles = (int)((items + p.items - 1) / p.items);
+        const int64_t ctas = (int64_t)lanes * kv_heads * p.item_tiles, wanted = std::max<int64_t>(1, (2 * (p.items == kItems && d <= 128 ? 2 : 1) * kSms + ctas - 1) / ctas);
+        p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + kKeys - 1), 4096) / kKeys * kKeys;
+    } else {
+        p.items = (int)((items + 7) / 8 * 8);
+        p.item_tiles = 1;
+        // A lane's own keys: whole where the lanes fill the device, else in shares of at least 256 keys; never more than 1024 (512 at heads of 256),
+        // which take a CTA about 12 us: lanes differ in length.
+        const int64_t ctas = (int64_t)lanes * kv_heads, wanted = std::max<int64_t>(1, (3 * kSms / 2 + ctas - 1) / ctas);
+        p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), d == 256 ? 512 : 1024) / 16 * 16;
+    }
     p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
     if (shared > 0) {
         // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.7 us, or 1 us for two tiles of items, its start and end 4 us, and a share's results are written and read once (2.5 TB/s, and 0.1 us).
         const int64_t all = (int64_t)total * g;
         p.item_rows = d <= 128 && all > kItems ? 2 : 1;
         p.row_tiles = (int)((all + kItems * p.item_rows - 1) / (kItems * p.item_rows));
-        const int tiles = (shared + kKeys - 1) / kKeys;
+        const int tiles = (int)(std::min<int64_t>(shared, window > 0 ? (int64_t)window + rows : INT_MAX) + kKeys - 1) / kKeys;
         const double results_us = 0.1 + (double)total * q_heads * d * 8 / 2.5e6;
         double best = 0;
         for (int n = 1; n <= std::min(tiles, 148); ++n) {
@@ -866,7 +918,7 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
     }
     // A lane's CTA joins the parts itself where its warps have at most two rows each to join, one after the other (1 lane, 5 rows of 2 heads of 256 each behind 768 shared tokens:
     // 20 us so, JOINED with a kernel of its own).
-    p.joined = p.shares > 1 || (p.shared_parts > 0 && items > (d == 256 ? 4 : 8));
+    p.joined = p.shares > 1 || p.items >= kItems || (p.shared_parts > 0 && items > (d == 256 ? 4 : 8));
     p.parts = p.shared_parts + (p.joined ? p.shares : 0);
     return p;
 }

@@ -43,7 +43,7 @@ struct SharedAttnPlan {
     int64_t parts = 0;       // partial results of a row; 0: none are written
     int64_t bytes(int total, int q_heads, int d) const { return parts * total * q_heads * ((int64_t)d * 4 + 8); }
 };
-SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared);
+SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared, int window);
 
 void launch_shared_attention(SharedAttnArgs a, const SharedAttnPlan& p, cudaStream_t s);
 

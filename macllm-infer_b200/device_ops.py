@@ -114,7 +114,7 @@ def shared_attention(q, k_pool, v_pool, tables, lengths, shared_len: int, *, sca
         if out.shape != shape or out.dtype is not dtype or out.get_device() != device or (total and out_strides[1:] != (dim, 1)):
             raise ValueError("out is like q, the heads of a row dense")
         out_stride = out_strides[0] if total > 1 else heads * dim
-    need = _attention_workspace(heads, kv_heads, dim, page, width, lanes, rows, total, shared_len)
+    need = _attention_workspace(heads, kv_heads, dim, page, width, lanes, rows, total, shared_len, window)
     space = q.new_empty(need // 2) if need else None
     _run(device, capi.lib().mk_k_shared_attention_dev, _TYPES[dtype], q.data_ptr(), q_strides[0] if total > 1 else heads * dim, k_pool.data_ptr(), v_pool.data_ptr(), pages,
          strides[0] if pages > 1 else kv_heads * page * dim, heads, kv_heads, dim, page, table, table_stride, width, _dense(lengths, _I32, (lanes,), device, "lengths"), cu, lanes, rows,

@@ -81,7 +81,7 @@ def test_the_workspace_covers_every_size(capi):
         for page, width in ((16, 0), (16, 1), (16, 700), (64, 600), (16, 8192)):
             for lanes, rows in ((1, 1), (3, 7), (64, 1), (128, 5), (500, 16)):
                 for pages in {0, width // 2, width}:
-                    capi.check(capi.lib().mk_k_shared_attention_workspace(heads, kv, dim, page, width, lanes, rows, lanes * rows, pages * page, C.byref(need)))
+                    capi.check(capi.lib().mk_k_shared_attention_workspace(heads, kv, dim, page, width, lanes, rows, lanes * rows, pages * page, 0, C.byref(need)))
                     parts, rest = divmod(need.value, lanes * rows * heads * (dim * 4 + 8))
                     assert rest == 0 and 0 <= parts <= 2 + width * page // 64
 
