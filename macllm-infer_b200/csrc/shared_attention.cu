@@ -139,10 +139,14 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
                 if (w[s] == 0.f) continue;
                 const float* src = a.part_o + ((s0 + b + s) * n_rows + row) * D + lane * V;
                 if constexpr (V == 2) {
-                    *reinterpret_cast<float2*>(x[s]) = __ldcg(reinterpret_cast<const float2*>(src));
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+                    x[s][0] = y.x; x[s][1] = y.y;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(x[s] + j) = __ldcg(reinterpret_cast<const float4*>(src + j));
+                    for (int j = 0; j < V; j += 4) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(src + j));
+                        x[s][j] = y.x; x[s][j + 1] = y.y; x[s][j + 2] = y.z; x[s][j + 3] = y.w;
+                    }
                 }
             }
 #pragma unroll

@@ -44,6 +44,19 @@ __device__ __forceinline__ void tell(int32_t* status, int bit) {
 __device__ __forceinline__ float value_of(float x) { return x; }
 __device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void load4(const float* x, float (&v)[4]) {
+    const float4 r = *reinterpret_cast<const float4*>(x);
+    v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+}
+__device__ __forceinline__ void load4(const __half* x, float (&v)[4]) {
+    const uint2 r = *reinterpret_cast<const uint2*>(x);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* x, float (&v)[4]) {
+    const uint2 r = *reinterpret_cast<const uint2*>(x);
+    v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xFFFF0000u); v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xFFFF0000u);
+}
 // The values of 16 bytes.
 __device__ __forceinline__ void unpack(const uint4& r, float (&v)[4], const float*) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
@@ -174,79 +187,6 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ bool is_draft(int d, int vocab) { return d >= 0 && d < vocab; }
-
-template <typename T, int VPT>
-__global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant__ VerifyArgs a) {
-    constexpr int EPV = 16 / (int)sizeof(T);
-    __shared__ uint64_t warp_best[kScan / 32];
-    __shared__ double warp_sum_of[kScan / 32];
-    const int tid = threadIdx.x, wl = tid & 31, warp = tid >> 5, index = blockIdx.x / a.runs, run = blockIdx.x - index * a.runs;
-    const int lane = index / (a.n_drafts + 1), i = index - lane * (a.n_drafts + 1), vocab = a.vocab;
-    pdl_trigger();
-    const int32_t* drafts = a.drafts + (int64_t)lane * a.n_drafts;
-    const float temperature = a.temperature[lane];
-    const int k = a.top_k[lane];
-    bool gone = false;
-    for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
-    if (__any_sync(0xffffffffu, gone)) return;   // nothing gets here
-    const Row<T> row(static_cast<const T*>(a.logits) + index * a.ld, vocab);
-    float f[VPT][EPV];
-#pragma unroll
-    for (int c = 0; c < VPT; ++c) row.load((run * VPT + c) * kScan + tid, f[c]);
-    bool bad = false;
-    float top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < VPT; ++c)
-#pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-            bad |= !(f[c][j] < INFINITY);
-            top = fmaxf(top, f[c][j]);
-        }
-    int at = vocab;
-#pragma unroll
-    for (int c = VPT - 1; c >= 0; --c)
-#pragma unroll
-        for (int j = EPV - 1; j >= 0; --j)
-            if (f[c][j] == top) at = row.token((run * VPT + c) * kScan + tid) + j;
-    if (top == -INFINITY) at = vocab;
-    uint64_t best = key_of(top, at);
-    if (temperature > 0.f && k > 0) a.group_best[((int64_t)index * a.runs + run) * kScan + tid] = top;
-    bad = __syncthreads_or(bad);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-        best = other > best ? other : best;
-    }
-    if (wl == 0) warp_best[warp] = best;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kScan / 32; ++w) best = warp_best[w] > best ? warp_best[w] : best;
-    double sum = 0.0;
-    if (temperature > 0.f && k <= 0) {
-        const Exponential weight(value_of_key(best), temperature);
-#pragma unroll
-        for (int c = 0; c < VPT; ++c)
-#pragma unroll
-            for (int j = 0; j < EPV; j += 4) sum += (double)((weight(f[c][j]) + weight(f[c][j + 1])) + (weight(f[c][j + 2]) + weight(f[c][j + 3])));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (wl == 0) warp_sum_of[warp] = sum;
-        __syncthreads();
-        sum = 0.0;
-#pragma unroll
-        for (int w = 0; w < kScan / 32; ++w) sum += warp_sum_of[w];
-    }
-    if (tid == 0) {
-        Run r;
-        r.best = best;
-        r.sum = sum;
-        r.bad = bad;
-        r.pad_ = 0;
-        static_cast<Run*>(a.run_results)[(int64_t)index * a.runs + run] = r;
-    }
-}
-
 // What a warp knows of a row from its runs.
 struct RowSum {
     uint64_t best;
@@ -276,6 +216,75 @@ __device__ __forceinline__ RowSum sum_runs(const Run* runs, int n, double unit, 
         for (int o = 16; o > 0; o >>= 1) s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
     }
     return s;
+}
+
+__device__ __forceinline__ bool is_draft(int d, int vocab) { return d >= 0 && d < vocab; }
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant__ VerifyArgs a) {
+    constexpr int EPV = 16 / (int)sizeof(T);
+    __shared__ Run warp_runs[kScan / 32];
+    const int tid = threadIdx.x, wl = tid & 31, warp = tid >> 5, index = blockIdx.x / a.runs, run = blockIdx.x - index * a.runs;
+    const int lane = index / (a.n_drafts + 1), i = index - lane * (a.n_drafts + 1), vocab = a.vocab;
+    pdl_trigger();
+    const int32_t* drafts = a.drafts + (int64_t)lane * a.n_drafts;
+    const float temperature = a.temperature[lane];
+    const int k = a.top_k[lane];
+    bool gone = false;
+    for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
+    if (__any_sync(0xffffffffu, gone)) return;   // nothing gets here
+    const Row<T> row(static_cast<const T*>(a.logits) + index * a.ld, vocab);
+    float f[VPT][EPV];
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) row.load((run * VPT + c) * kScan + tid, f[c]);
+    bool bad = false;
+    float top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < VPT; ++c)
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) {
+            bad |= !(f[c][j] < INFINITY);
+            top = fmaxf(top, f[c][j]);
+        }
+    if (temperature > 0.f && k > 0) a.group_best[((int64_t)index * a.runs + run) * kScan + tid] = top;
+    // warps by themselves, then the block's by one of them
+    const uint32_t value = f32_order_key(top + 0.0f), warp_value = __reduce_max_sync(0xffffffffu, value);
+    int at = vocab;
+    if (value == warp_value && top > -INFINITY) {
+#pragma unroll
+        for (int c = VPT - 1; c >= 0; --c)
+#pragma unroll
+            for (int j = EPV - 1; j >= 0; --j)
+                if (f[c][j] == top) at = row.token((run * VPT + c) * kScan + tid) + j;
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+    bad = __any_sync(0xffffffffu, bad);
+    Run r;
+    r.best = (uint64_t)warp_value << 32 | (0xFFFFFFFFu - (uint32_t)at);
+    r.sum = 0.0;
+    const bool whole = temperature > 0.f && k <= 0;
+    if (whole) {
+        const Exponential weight(value_of_key(r.best), temperature);
+#pragma unroll
+        for (int c = 0; c < VPT; ++c)
+#pragma unroll
+            for (int j = 0; j < EPV; j += 4) r.sum += (double)((weight(f[c][j]) + weight(f[c][j + 1])) + (weight(f[c][j + 2]) + weight(f[c][j + 3])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+    }
+    r.bad = bad;
+    r.pad_ = 0;
+    if (wl == 0) warp_runs[warp] = r;
+    __syncthreads();
+    if (warp != 0) return;
+    const RowSum s = sum_runs(warp_runs, kScan / 32, whole ? 1.0 / (double)temperature : 0.0, whole);
+    if (wl == 0) {
+        r.best = s.best;
+        r.sum = s.z;
+        r.bad = s.bad && value_of_key(s.best) > -INFINITY;   // a run of nothing is no fault of the row's
+        for (int w = 0; w < kScan / 32; ++w) r.bad |= warp_runs[w].bad;
+        static_cast<Run*>(a.run_results)[(int64_t)index * a.runs + run] = r;
+    }
 }
 
 __device__ __forceinline__ void put_lane(const VerifyArgs& a, int lane, int end, int token) {   // a warp
@@ -671,8 +680,9 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     const double z = s_z;
     const Exponential weight(value_of_key(s_best), temperature);
     const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
-    const int chunk = (vocab + kCtas - 1) / kCtas, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
-    const int run = (n1 - n0 + kWarps - 1) / kWarps, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
+    const int chunk = (vocab + 4 * kCtas - 1) / (4 * kCtas) * 4, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
+    const int run = (n1 - n0 + 4 * kWarps - 1) / (4 * kWarps) * 4, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
+    const bool fours = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;   // rows begin where four values can be read at once
     bool rest = d >= 0;
     auto share = [&](float logit, float qt) {
         const float w = weight(logit);
@@ -681,19 +691,29 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
     double total = 0.0, *sums = sum_of[0];
     for (;;) {
-        constexpr int AHEAD = 8;
+        constexpr int AHEAD = 4;   // fours of tokens a thread has on their way together
         double part = 0.0;
-        for (int t0 = r_lo + wl; t0 < r_hi; t0 += 32 * AHEAD) {
-            float l[AHEAD], qv[AHEAD], s = 0.f;
+        for (int t0 = r_lo + wl * 4; t0 < r_hi; t0 += 128 * AHEAD) {
+            float l[AHEAD][4], qv[AHEAD][4];
 #pragma unroll
             for (int c = 0; c < AHEAD; ++c) {
-                const int t = t0 + 32 * c;
-                l[c] = t < r_hi ? value_of(x[t]) : -INFINITY;
-                qv[c] = t < r_hi ? q_at(t) : 0.f;
+                const int t = t0 + 128 * c;
+                if (fours && t + 4 <= r_hi) {
+                    load4(x + t, l[c]);
+                    if (rest && q != nullptr) load4(q + t, qv[c]);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) qv[c][j] = q_at(t + j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        l[c][j] = t + j < r_hi ? value_of(x[t + j]) : -INFINITY;
+                        qv[c][j] = t + j < r_hi ? q_at(t + j) : 0.f;
+                    }
+                }
             }
 #pragma unroll
-            for (int c = 0; c < AHEAD; ++c) s += share(l[c], qv[c]);
-            part += (double)s;
+            for (int c = 0; c < AHEAD; ++c) part += (double)((share(l[c][0], qv[c][0]) + share(l[c][1], qv[c][1])) + (share(l[c][2], qv[c][2]) + share(l[c][3], qv[c][3])));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
