@@ -152,19 +152,53 @@ __device__ void sort_desc(uint64_t* keys, int n) {   // keys behind n are there 
     else sort_desc<4>(keys);
 }
 
-// exp((x - top) / temperature) with 1 / (temperature ln 2) as the sum of two 32-bit numbers.
+// Two 32-bit numbers in one instruction.
+struct Two {
+    unsigned long long v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void apart(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+// The larger, or NaN where there is one.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// exp((x - top) / temperature) with 1 / (temperature ln 2) as the sum of two 32-bit numbers: t = y hi rounded, what it lost and y lo come behind as a factor.  What is below 2^-126 of the
+// best counts as that much, -inf too.
 struct Exponential {
-    float top, hi, lo;
+    float top, hi, lo, least;
     __device__ __forceinline__ Exponential(float best, float temperature) : top(best) {
         const double unit = 1.4426950408889634074 / (double)temperature;
         hi = (float)unit;
         lo = (float)(unit - (double)hi);
+        least = -125.f / hi;
     }
-    __device__ __forceinline__ float operator()(float x) const {
-        const float y = x - top, t = y * hi, rest = fmaf(y, lo, fmaf(y, hi, -t));
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        return t > -126.f ? fmaf(e, rest * 0.69314718f, e) : 0.f;   // -inf among what is not
+    __device__ __forceinline__ void operator()(float& a, float& b) const {
+        a = fmaxf(a - top, least);
+        b = fmaxf(b - top, least);
+        const Two y = two(a, b), h = two(hi, hi), t = mul2(y, h), lost = fma2(y, two(lo, lo), fma2(y, h, mul2(t, two(-1.f, -1.f))));
+        float u, v;
+        apart(t, u, v);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(u));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(v));
+        const Two e = two(u, v);
+        apart(fma2(e, mul2(lost, two(0.69314718f, 0.69314718f)), e), a, b);
     }
 };
 
@@ -237,28 +271,29 @@ __global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant_
     float f[VPT][EPV];
 #pragma unroll
     for (int c = 0; c < VPT; ++c) row.load((run * VPT + c) * kScan + tid, f[c]);
-    bool bad = false;
-    float top = -INFINITY;
+    float best_of[VPT];
 #pragma unroll
-    for (int c = 0; c < VPT; ++c)
+    for (int c = 0; c < VPT; ++c) {
+        best_of[c] = f[c][0];
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-            bad |= !(f[c][j] < INFINITY);
-            top = fmaxf(top, f[c][j]);
-        }
+        for (int j = 1; j < EPV; ++j) best_of[c] = max_or_nan(best_of[c], f[c][j]);
+    }
+    float top = best_of[0];
+#pragma unroll
+    for (int c = 1; c < VPT; ++c) top = max_or_nan(top, best_of[c]);
+    const bool bad = __any_sync(0xffffffffu, !(top < INFINITY));
     if (temperature > 0.f && k > 0) a.group_best[((int64_t)index * a.runs + run) * kScan + tid] = top;
     // warps by themselves, then the block's by one of them
     const uint32_t value = f32_order_key(top + 0.0f), warp_value = __reduce_max_sync(0xffffffffu, value);
-    int at = vocab;
-    if (value == warp_value && top > -INFINITY) {
+    int at = vocab;   // which token it is: for greedy lanes
+    if (!(temperature > 0.f) && value == warp_value && top > -INFINITY) {
 #pragma unroll
         for (int c = VPT - 1; c >= 0; --c)
 #pragma unroll
             for (int j = EPV - 1; j >= 0; --j)
                 if (f[c][j] == top) at = row.token((run * VPT + c) * kScan + tid) + j;
     }
-    at = __reduce_min_sync(0xffffffffu, at);
-    bad = __any_sync(0xffffffffu, bad);
+    if (!(temperature > 0.f)) at = __reduce_min_sync(0xffffffffu, at);
     Run r;
     r.best = (uint64_t)warp_value << 32 | (0xFFFFFFFFu - (uint32_t)at);
     r.sum = 0.0;
@@ -268,7 +303,11 @@ __global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant_
 #pragma unroll
         for (int c = 0; c < VPT; ++c)
 #pragma unroll
-            for (int j = 0; j < EPV; j += 4) r.sum += (double)((weight(f[c][j]) + weight(f[c][j + 1])) + (weight(f[c][j + 2]) + weight(f[c][j + 3])));
+            for (int j = 0; j < EPV; j += 4) {
+                weight(f[c][j], f[c][j + 1]);
+                weight(f[c][j + 2], f[c][j + 3]);
+                r.sum += (double)((f[c][j] + f[c][j + 1]) + (f[c][j + 2] + f[c][j + 3]));
+            }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
     }
@@ -404,7 +443,7 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
     __syncthreads();
     // tokens that reach a bound; at least k reach `enough`, fewer reach `few`
     const float bound_low = s.step.x < 0 || per_step == 0.f ? (s.step.x < 0 ? -INFINITY : low) : low + (float)s.step.x / per_step - range * 1e-5f;
-    uint64_t enough = (uint64_t)f32_order_key(bound_low + 0.0f) << 32, few = best + 1, bound = enough;
+    uint64_t enough = (uint64_t)f32_order_key(bound_low + 0.0f) << 32, few = (best | 0xFFFFFFFFu) + 1, bound = enough;
     int n_all;
     for (;;) {
         const float bound_value = value_of_key(bound);
@@ -684,9 +723,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     const int run = (n1 - n0 + 4 * kWarps - 1) / (4 * kWarps) * 4, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
     const bool fours = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;   // rows begin where four values can be read at once
     bool rest = d >= 0;
-    auto share = [&](float logit, float qt) {
-        const float w = weight(logit);
-        return rest ? fmaxf(fmaf(w, per_z, -qt) + w * per_z_rest, 0.f) : w;
+    auto shares2 = [&](float& a, float& b, float qa, float qb) {   // of two tokens
+        weight(a, b);
+        if (rest) {
+            a = fmaxf(fmaf(a, per_z, -qa) + a * per_z_rest, 0.f);
+            b = fmaxf(fmaf(b, per_z, -qb) + b * per_z_rest, 0.f);
+        }
     };
     auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
     double total = 0.0, *sums = sum_of[0];
@@ -713,7 +755,13 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
                 }
             }
 #pragma unroll
-            for (int c = 0; c < AHEAD; ++c) part += (double)((share(l[c][0], qv[c][0]) + share(l[c][1], qv[c][1])) + (share(l[c][2], qv[c][2]) + share(l[c][3], qv[c][3])));
+            for (int c = 0; c < AHEAD; ++c) {
+                const int there = r_hi - (t0 + 128 * c);
+                if (there <= 0) break;
+                shares2(l[c][0], l[c][1], qv[c][0], qv[c][1]);
+                shares2(l[c][2], l[c][3], qv[c][2], qv[c][3]);
+                part += (double)((l[c][0] + (there > 1 ? l[c][1] : 0.f)) + ((there > 2 ? l[c][2] : 0.f) + (there > 3 ? l[c][3] : 0.f)));
+            }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -759,7 +807,10 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     const int at_lo = min(n1, n0 + w_at * run), at_hi = min(n1, at_lo + run);
     for (int t0 = at_lo; t0 < at_hi; t0 += kThreads) {
         const int t = t0 + tid;
-        const double r = t < at_hi ? (double)share(value_of(x[t]), q_at(t)) : 0.0;
+        float r_mine = t < at_hi ? value_of(x[t]) : -INFINITY, none = -INFINITY;
+        const bool masked = r_mine == -INFINITY;
+        shares2(r_mine, none, t < at_hi ? q_at(t) : 0.f, 0.f);
+        const double r = masked ? 0.0 : (double)r_mine;
         double all;
         const double c = before + block_scan(r, top_shared.red, &all);
         if (r > 0.0) {
