@@ -647,7 +647,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     }
     const bool hot = temperature > 0.f, whole = hot && k <= 0;
     if (rank == 0 && tid == 0 && ((n < n_drafts && drafts[n] >= vocab) || (hot && (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f))))) tell(a.status, kDevBadRange);
-    if (rank != 0 && !hot) return;
+    if (rank != 0 && (!hot || (!whole && rank > n))) return;   // no row for this CTA: whom the cluster's barrier then does not wait for
     if (tid == 0) {
         s_end = INT_MAX;
         s_pick = INT_MAX;
