@@ -671,7 +671,8 @@ int32_t mk_k_q4k_matmul_tc_noalloc_dev(const void* w_q4k_dev, int64_t rows, int6
  * scores are scale * q.k (scale > 0), with softcap > 0 then softcap * tanh(score / softcap).  A row that sees nothing becomes zeros; rows of q
  * that belong to no lane are left as they were in out.  The first shared_len tokens (whole pages; 0 is allowed) are the same
  * pages in every lane's table, and are read once for all lanes, through lane 0's: the result is what attention lane by lane
- * gives.  They must hold finite values.  Values behind a lane's length may be anything.
+ * gives.  Keys and values of a lane's tokens are finite, those of the first shared_len tokens also where a lane is shorter; what lies
+ * behind a lane's length may be anything.
  * q, out [total] rows of q_heads x head_dim values, q_stride / out_stride values apart; pools of one layer, pages [kv_heads]
  * [block_tokens][head_dim] page_stride values apart (a layer of the model's arena: kv_heads * block_tokens * head_dim); all
  * f16 or all bf16 (type).  Rows, strides and pools are 16-byte aligned.  head_dim 64, 128 or 256; any group size up to 128.  Scores, softmax
@@ -687,7 +688,7 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
 /* Verification of drafted tokens.  logits [lanes][drafts + 1] rows of vocab values, at most 416000 (logits_stride apart): row i of a lane is the
  * target's answer behind its first i drafts.  Its distribution p_i is the sampler's (mk_k_sample): logits / temperature over the
  * top_k best tokens (lower token first among equals; top_k 0: all), of those the head that adds up to top_p (below 1 only with
- * top_k >= 1; top_k at most 1024); temperature 0: the best token.  drafts [lanes][drafts], a negative one ends a lane's;
+ * top_k >= 1; top_k at most 1024); temperature 0 (or below 1e-30): the best token.  drafts [lanes][drafts], a negative one ends a lane's;
  * draft_probs [lanes][drafts][vocab] f32: the distributions q_i that they were drawn from, NULL: drafts without one (looked up), q_i = 1
  * on the draft.  u [lanes][drafts + 1] uniform in [0, 1).  Draft i is kept while u_i q_i(d_i) < p_i(d_i); the first that is not is
  * replaced by a token of max(p_i - q_i, 0), and behind the last one a token of p is added, both drawn by u_drafts: the first token, in

@@ -171,7 +171,8 @@ __device__ __forceinline__ void store_row(T* out, const float (&o)[V], float l) 
 //
 // A CTA takes a share of one lane's keys for NT * 8 (row, head) items of one KV head.  Each of its warps walks tiles of 16 keys, which TMA brings into a ring of its own; the
 // items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.  What bounds it is HBM where lanes have much of their own, else the chain of dependent fetches at a CTA's two
-// ends: so a warp asks for its first tiles before anything else, and rings are short enough for three CTAs on an SM.
+// ends: so a warp asks for its first tiles before anything else, and rings are short enough for three CTAs on an SM.  40 lanes of 16 heads of 256 over 8 with 300 to 4000 keys of
+// their own: 80 us, 5.4 TB/s; 128 lanes of 32 heads of 128 over 8 with 20 to 700: 35 us, 2.9 TB/s.
 constexpr int kTile = 16;
 
 template <int D>
@@ -444,9 +445,13 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
 // All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA, over a share of
 // the keys in tiles of 64.  One warp brings keys and values by TMA, one per tile of items issues the tcgen05 products, four do its softmax, a thread per item.  Scores of a tile
 // of keys go to one of two areas of tensor memory that a tile of items has; its weights go back over its scores, as the A operand of O += P V; the scores of the next tile are
-// made meanwhile.  What bounds the softmax are the exponentials (16 per clock and SM).  With two tiles of items a key is fetched once for both, and the two warps that share a
-// quarter of the SM take turns at the exponentials: left alone they fall into step, and the unit idles while both do the rest (1850 clocks a tile of keys instead of
-// TURNS).  One tile of items to a CTA: two CTAs on an SM do the same for one another.  The running maximum follows only when a tile exceeds it by kSlack (weights stay below 2^kSlack).
+// made meanwhile.  With two tiles of items a key is fetched once for both; with one, two CTAs share an SM.  The running maximum follows only when a tile exceeds it by kSlack
+// (weights stay below 2^kSlack).
+//
+// What bounds it, for two tiles of items and a tile of keys: the exponentials, 16 per clock and SM, take 1024 clocks; at heads of 128 the products take 1280 (measured alone: 48 clocks for
+// 16 dimensions of 128 x 64 scores, whose operands shared memory delivers in that time, 65 for 16 keys of 128 x 128 outputs); at heads of 64 half of that.  Left alone, the warps that
+// share a quarter of the SM fall into step and the exponential unit idles while both do the rest, so they take turns (heads of 64: 1850 clocks a tile, 1470 so; heads of 128: 2000 and 1850).
+// 128 lanes of 32 heads of 128 over 8 behind 32768 shared tokens: 78 us, 880 TFLOP/s; 32 lanes behind 2048: 7 us.
 constexpr float kSlack = 8.f;
 constexpr int kItems = 128, kKeys = 64;
 
@@ -921,7 +926,7 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
         }
     }
     // A lane's CTA joins the parts itself where its warps have at most two rows each to join, one after the other (1 lane, 5 rows of 2 heads of 256 each behind 768 shared tokens:
-    // 20 us so, JOINED with a kernel of its own).
+    // 20 us so, 15 with a kernel of its own).
     p.joined = p.shares > 1 || p.items >= kItems || (p.shared_parts > 0 && items > (d == 256 ? 4 : 8));
     p.parts = p.shared_parts + (p.joined ? p.shares : 0);
     return p;

@@ -253,6 +253,11 @@ __device__ __forceinline__ RowSum sum_runs(const Run* runs, int n, double unit, 
 }
 
 __device__ __forceinline__ bool is_draft(int d, int vocab) { return d >= 0 && d < vocab; }
+// A lane's temperature: 0 where it is none or so low that only the best token is left, and not beyond what 32 bits turn into a factor.
+__device__ __forceinline__ float temperature_of(const VerifyArgs& a, int lane) {
+    const float t = a.temperature[lane];
+    return t > 1e-30f ? fminf(t, 1e30f) : 0.f;
+}
 
 template <typename T, int VPT>
 __global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant__ VerifyArgs a) {
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kScan) scan_rows_kernel(const __grid_constant_
     const int lane = index / (a.n_drafts + 1), i = index - lane * (a.n_drafts + 1), vocab = a.vocab;
     pdl_trigger();
     const int32_t* drafts = a.drafts + (int64_t)lane * a.n_drafts;
-    const float temperature = a.temperature[lane];
+    const float temperature = temperature_of(a, lane);
     const int k = a.top_k[lane];
     bool gone = false;
     for (int j = wl; j < i; j += 32) gone |= !is_draft(drafts[j], vocab);
@@ -636,7 +641,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), lane = blockIdx.x / kCtas, n_drafts = a.n_drafts, vocab = a.vocab;
     const int32_t* drafts = a.drafts + (int64_t)lane * n_drafts;
     const float* u = a.u + (int64_t)lane * (n_drafts + 1);
-    const float temperature = a.temperature[lane], top_p = a.top_p[lane];
+    const float temperature = temperature_of(a, lane), top_p = a.top_p[lane];
     const double u_draw = (double)u[n_drafts];
     int k = a.top_k[lane];
     int n = 0;   // drafts in front of the first that is none

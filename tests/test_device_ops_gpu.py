@@ -424,6 +424,23 @@ def test_rows_without_a_distribution_and_settings_out_of_range(dops):
             dops.check_status(status)
 
 
+@pytest.mark.parametrize("top_k", [0, 30])
+def test_temperatures_without_measure(dops, top_k):
+    """The lowest leave the best token, the highest make all alike; nothing between overflows."""
+    logits, drafts, u, _ = verify_case(13, 4, 2, 1000)
+    logits[:, :, 5] = -math.inf
+    k = torch.full((4,), top_k, dtype=torch.int32, device="cuda")
+    one = torch.ones(4, device="cuda")
+    args = [logits.cuda(), torch.from_numpy(drafts).cuda(), torch.from_numpy(u).cuda()]
+    greedy = dops.verify_drafts(*args, temperature=0 * one, top_k=k, top_p=one)
+    for t in (1e-45, 1e-38, 1e-31, 1e-28, 1e-20):
+        assert all(torch.equal(a, b) for a, b in zip(greedy, dops.verify_drafts(*args, temperature=t * one, top_k=k, top_p=one))), t
+    hot = [dops.verify_drafts(*args, temperature=t * one, top_k=k, top_p=one) for t in (1e25, 1e35, math.inf)]
+    assert all(torch.equal(a, b) for other in hot[1:] for a, b in zip(hot[0], other))
+    drawn = hot[0][0][torch.arange(4), hot[0][1].long()]
+    assert ((drawn >= 0) & (drawn != 5)).all()
+
+
 def test_padded_rows_of_logits(dops):
     logits, drafts, u, _ = verify_case(10, 5, 3, 1001)
     wide = torch.full((5, 4, 1030), math.nan, device="cuda")
