@@ -29,6 +29,18 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// x * a + b and x + y for two numbers at once.
+__device__ __forceinline__ void scale2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\tfma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
 // cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)).
 __device__ __forceinline__ float capped(float v, float cap, float two_over_cap) {
     return cap - __fdividef(2.0f * cap, 1.0f + __expf(fminf(v * two_over_cap, 80.0f)));
@@ -443,7 +455,8 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
 // ---- the shared keys ---------------------------------------------------------------------------------------------
 //
 // All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA, over a share of
-// the keys in tiles of 64.  One warp brings keys and values by TMA, one per tile of items issues the tcgen05 products, four do its softmax, a thread per item.  Scores of a tile
+// the keys in tiles of 64.  One warp brings keys and values by TMA (two with two tiles of items: a page of 16 tokens is 2 KB a box,
+// and one warp's requests, sixteen a tile of keys, bounded the kernel at 2000 clocks), one per tile of items issues the tcgen05 products, four do its softmax, a thread per item.  Scores of a tile
 // of keys go to one of two areas of tensor memory that a tile of items has; its weights go back over its scores, as the A operand of O += P V; the scores of the next tile are
 // made meanwhile.  With two tiles of items a key is fetched once for both; with one, two CTAs share an SM.  The running maximum follows only when a tile exceeds it by kSlack
 // (weights stay below 2^kSlack).
@@ -458,7 +471,7 @@ constexpr int kItems = 128, kKeys = 64;
 template <int D, int NQ>
 struct SharedSmem {
     static constexpr int PANELS = D / 64, PANEL = kKeys * 128, QPANEL = kItems * 128, BYTES = PANELS * PANEL;
-    static constexpr int STAGES = D == 256 || (D == 128 && NQ == 1) ? 2 : (D == 128 ? 4 : (NQ == 1 ? 5 : 6)), WARPS = NQ * 4, THREADS = WARPS * 32 + 32 + NQ * 32;   // WARPS: of the softmax
+    static constexpr int STAGES = D == 256 || (D == 128 && NQ == 1) ? 2 : (D == 128 ? 4 : (NQ == 1 ? 5 : 6)), WARPS = NQ * 4, LOADERS = NQ, THREADS = (WARPS + LOADERS + NQ) * 32;   // WARPS: of the softmax
     static constexpr int CTAS = NQ == 1 && D <= 128 ? 2 : 1, TMEM = NQ * (D + 2 * kKeys) <= 256 ? 256 : 512;
     static constexpr size_t SMEM = 1024 + (size_t)NQ * PANELS * QPANEL + (size_t)STAGES * 2 * BYTES;
 };
@@ -490,16 +503,22 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     constexpr bool kEarly = !OWN;
     const int all_tiles = (a.shared + KEYS - 1) / KEYS, first_tile = OWN ? split * chunk / KEYS : (int)((int64_t)all_tiles * split / splits),
               last_tile = OWN ? max(first_tile, (keys_end - base_key + KEYS - 1) / KEYS) : (int)((int64_t)all_tiles * (split + 1) / splits);
-    if (warp == L::WARPS && lane == 0) {
+    // two loaders, one for keys and one for values, or one for both
+    const bool loads = warp >= L::WARPS && warp < L::WARPS + L::LOADERS, loads_k = warp == L::WARPS, loads_v = warp == L::WARPS + L::LOADERS - 1;
+    if (loads && lane == 0) {
         for (int i = 0; i < ST; ++i) {
-            bar_init(&k_full[i], 1);
-            bar_init(&k_empty[i], NQ);
-            bar_init(&v_full[i], 1);
-            bar_init(&v_empty[i], NQ);
+            if (loads_k) {
+                bar_init(&k_full[i], 1);
+                bar_init(&k_empty[i], NQ);
+            }
+            if (loads_v) {
+                bar_init(&v_full[i], 1);
+                bar_init(&v_empty[i], NQ);
+            }
         }
         bar_init_fence();
     }
-    if (warp == L::WARPS + 1) {
+    if (warp == L::WARPS + L::LOADERS) {
         if (lane == 0) {
             for (int i = 0; i < 2 * NQ; ++i) {
                 bar_init(&s_full[i], 1);
@@ -515,7 +534,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // The queries' pieces and the first tiles of keys and values are on their way before anything else is looked at (one after the other the queries took 0.6 us a piece, 10 us at
     // heads of 128).
     const int boxes = KEYS / box, of = lane % boxes, panel = lane / boxes;   // at most four boxes of each of the panels: 16
-    const bool brings = warp == L::WARPS && panel < L::PANELS;
+    const bool brings = loads && panel < L::PANELS;
     const int most_tiles = a.window != 0 && !OWN ? all_tiles : last_tile;
     auto page_row = [&](int t) {
         int pos = base_key + t * KEYS + of * box;
@@ -538,7 +557,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         if (brings) tma_load_2d(smem_u32(vs) + st * L::BYTES + panel * L::PANEL + of * box * 128, &tm_v, panel * 64, row, &v_full[st]);
     };
     int early = 0;   // tiles asked for here; where there is a window, what is seen has to be known first
-    if (kEarly && warp == L::WARPS && a.window == 0) {
+    if (kEarly && loads && a.window == 0) {
         __syncwarp();
         asm volatile("bar.arrive 15, %0;" ::"n"(L::THREADS) : "memory");
         early = min(ST, last_tile - first_tile);
@@ -548,8 +567,8 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
         for (int i = 0; i < ST; ++i)
             if (i < early) {
-                bring_k(i, rows[i]);
-                bring_v(i, rows[i]);
+                if (loads_k) bring_k(i, rows[i]);
+                if (loads_v) bring_v(i, rows[i]);
             }
     }
     const int q = warp >> 2, item = tile * (NQ * kItems) + tid, at_row = item / g, at_token = mine_range.first + at_row;   // total * q_heads is far below 2^31
@@ -601,7 +620,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     fence_before();
     // nobody waits for the loader's first requests, and it needs nothing of the others where there is no window
-    if (!kEarly || warp != L::WARPS || a.window != 0) asm volatile("bar.sync 15, %0;" ::"n"(L::THREADS) : "memory");
+    if (!kEarly || !loads || a.window != 0) asm volatile("bar.sync 15, %0;" ::"n"(L::THREADS) : "memory");
     fence_after();
     const uint32_t tmem = tmem_slot;
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
@@ -620,35 +639,39 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     const int n_tiles = max(0, t_end - t_begin);
 
-    if (warp == L::WARPS) {
+    if (loads) {
         // ---- loader
         bool ok = true;
         int t = early, row = page_row(t_begin + t);
         for (; t < n_tiles; ++t) {
             const int next = page_row(t_begin + t + 1), st = t % ST;
             const uint32_t ph = (uint32_t)(t / ST & 1) ^ 1;
-            ok = __all_sync(0xffffffffu, bar_wait(&k_empty[st], ph));
-            if (!ok) break;
-            bring_k(st, row);
-            ok = __all_sync(0xffffffffu, bar_wait(&v_empty[st], ph));
-            if (!ok) break;
-            bring_v(st, row);
+            if (loads_k) {
+                ok = __all_sync(0xffffffffu, bar_wait(&k_empty[st], ph));
+                if (!ok) break;
+                bring_k(st, row);
+            }
+            if (loads_v) {
+                ok = __all_sync(0xffffffffu, bar_wait(&v_empty[st], ph));
+                if (!ok) break;
+                bring_v(st, row);
+            }
             row = next;
         }
         if (!ok) {
             if (lane == 0) tell(a.status, kDevWait);
             for (int u = max(0, t - ST); u <= t && u < n_tiles; ++u) {   // copies in flight land before the CTA ends
-                bar_wait(&k_full[u % ST], u / ST & 1);
-                if (u < t) bar_wait(&v_full[u % ST], u / ST & 1);
+                if (loads_k && (u < t || loads_v)) bar_wait(&k_full[u % ST], u / ST & 1);
+                if (loads_v && u < t) bar_wait(&v_full[u % ST], u / ST & 1);
             }
         }
-    } else if (warp > L::WARPS) {
+    } else if (warp >= L::WARPS + L::LOADERS) {
         // ---- products, a warp per tile of items: the one's waits pass under the other's products.  The whole warp walks along, so that descriptors and addresses are the same for
         // all of it, and one elected thread issues (a lane of its own: 2500 clocks a tile of keys, 100 a product)
         if (n_tiles > 0) {
             constexpr uint32_t kind = std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u;
             constexpr uint32_t i_scores = f16_idesc(kItems, KEYS, false) | kind, i_out = f16_idesc(kItems, D, true) | kind;
-            const int q = NQ == 1 ? 0 : __shfl_sync(0xffffffffu, warp, 0) - L::WARPS - 1;
+            const int q = NQ == 1 ? 0 : __shfl_sync(0xffffffffu, warp, 0) - L::WARPS - L::LOADERS;
             const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), s_base = base + S_AT + q * 2 * KEYS, o_base = base + q * D;
             const uint64_t q_desc = sw128_desc(smem_u32(qs) + q * L::PANELS * L::QPANEL), k_desc = sw128_desc(smem_u32(ks)), v_desc = sw128_desc(smem_u32(vs), L::PANEL);
             const bool issues = elect_one();
@@ -724,7 +747,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int j = 4; j < KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+            for (int j = 4; j + 1 < KEYS; j += 2) top[j / 2 & 3] = max3(top[j / 2 & 3], s[j], s[j + 1]);
             const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
             const bool grow = m_tile > m_run + kSlack;   // also when there was none yet
             if (__any_sync(0xffffffffu, grow)) {
@@ -754,9 +777,9 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (NQ == 2) pair_sync(turn + q);
 #pragma unroll
             for (int j = 0; j < KEYS; j += 2) {
-                const float x = ex2(fmaf(s[j], unit, -m_use)), y = ex2(fmaf(s[j + 1], unit, -m_use));
-                part[j & 3] += x;
-                part[(j & 3) + 1] += y;
+                scale2(s[j], s[j + 1], unit, -m_use);
+                const float x = ex2(s[j]), y = ex2(s[j + 1]);
+                add2(part[j & 2], part[(j & 2) + 1], x, y);
                 w[j / 2] = Pair<T>::pack(x, y);
             }
             if (NQ == 2 && (q == 0 || t + 1 < n_tiles)) pair_arrive(turn + 1 - q);
@@ -816,7 +839,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     if (OWN) pdl_wait();   // who comes after this kernel relies on the one before it too
     fence_before();
     __syncthreads();
-    if (warp == L::WARPS + 1) {
+    if (warp == L::WARPS + L::LOADERS) {
         fence_after();
         tmem_dealloc(tmem, L::TMEM);
     }
