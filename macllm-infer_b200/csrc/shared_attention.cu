@@ -34,13 +34,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// x * a + b and x + y for two numbers at once.
-__device__ __forceinline__ void scale2(float& x, float& y, float a, float b) {
-    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\tfma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
-    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
-}
 // cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)).
 __device__ __forceinline__ float capped(float v, float cap, float two_over_cap) {
     return cap - __fdividef(2.0f * cap, 1.0f + __expf(fminf(v * two_over_cap, 80.0f)));
@@ -777,9 +770,9 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (NQ == 2) pair_sync(turn + q);
 #pragma unroll
             for (int j = 0; j < KEYS; j += 2) {
-                scale2(s[j], s[j + 1], unit, -m_use);
-                const float x = ex2(s[j]), y = ex2(s[j + 1]);
-                add2(part[j & 2], part[(j & 2) + 1], x, y);
+                const float x = ex2(fmaf(s[j], unit, -m_use)), y = ex2(fmaf(s[j + 1], unit, -m_use));
+                part[j & 3] += x;
+                part[(j & 3) + 1] += y;
                 w[j / 2] = Pair<T>::pack(x, y);
             }
             if (NQ == 2 && (q == 0 || t + 1 < n_tiles)) pair_arrive(turn + 1 - q);
