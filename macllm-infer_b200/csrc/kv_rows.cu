@@ -34,14 +34,16 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
     }
 }
 
-// A CTA per (lane, head, K or V) and run of layers walks the kept tokens in their order.  Where 1024 of them come from and go to is looked up once for all its layers (per
-// 64 tokens and layer: 325 us for 9600 tokens of 36 layers of 4 heads of 128, 274 so).  A chunk is read whole before it is written, and the one behind it is on its way by
-// then: since keep ascends and keep[j] >= first + j, what a chunk writes is in front of what a later one reads, so in place is the same as apart.
-constexpr int kGatherThreads = 256, kGatherTokens = 1024;
+// A CTA per (lane, head, K or V) and run of layers walks the kept tokens in their order.  Where 1024 of them come from and go to is looked up once for all its layers.  A chunk
+// is read whole before it is written, and the one behind it is on its way by then: since keep ascends and keep[j] >= first + j, what a chunk writes is in front of what a later
+// one reads, so in place is the same as apart.  9600 tokens of 36 layers of 4 heads of 128 (1.4 GB read and written): 241 us, 5.9 TB/s; with the rows looked up per 64 tokens and
+// layer 325 us; 274 us with 256 threads of four pieces, which wait longer at the barrier between reading and writing; 324 us with a warp for each column, which has too few
+// pieces on their way.
+constexpr int kGatherThreads = 128, kGatherTokens = 1024;
 
 template <typename PIECE>
 __global__ void __launch_bounds__(kGatherThreads) gather_tokens_kernel(const __grid_constant__ KvRowsArgs a) {
-    constexpr int PER = 4;
+    constexpr int PER = 2;
     __shared__ longlong2 rows[kGatherTokens];   // (from, to) in rows of a layer; from < 0: left out
     const int tid = threadIdx.x, row_pieces = a.row_bytes / (int)sizeof(PIECE), lane = blockIdx.x / a.kv_heads, head = blockIdx.x - lane * a.kv_heads;
     const int count = a.counts[lane], first = a.first[lane];
@@ -127,8 +129,9 @@ void launch_copy_pages(const KvRowsArgs& a, cudaStream_t s) {
 
 void launch_gather_tokens(const KvRowsArgs& a, cudaStream_t s) {
     if (a.lanes <= 0 || a.layers <= 0 || a.keep_width <= 0) return;
-    // as many layers to a CTA as leave eight CTAs for each SM
-    const int64_t columns = (int64_t)a.lanes * a.kv_heads * 2, runs = std::min<int64_t>({a.layers, std::max<int64_t>(1, (8 * 148 + columns - 1) / columns), 65535});
+    // as many layers to a CTA as leave 32 CTAs for each SM (16: 246 us where these take 241), split evenly
+    const int64_t columns = (int64_t)a.lanes * a.kv_heads * 2, most = std::min<int64_t>({a.layers, std::max<int64_t>(1, (32 * 148 + columns - 1) / columns), 65535});
+    const int64_t each = (a.layers + most - 1) / most, runs = (a.layers + each - 1) / each;
     with_piece(a, [&](auto piece) { gather_tokens_kernel<decltype(piece)><<<dim3((unsigned)(a.lanes * a.kv_heads), (unsigned)runs, 2), kGatherThreads, 0, s>>>(a); });
     MK_LAUNCH_CHECK();
 }
