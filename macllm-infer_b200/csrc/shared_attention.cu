@@ -175,31 +175,32 @@ __device__ __forceinline__ void store_row(T* out, const float (&o)[V], float l) 
 // ---- a lane's keys -----------------------------------------------------------------------------------------------
 //
 // A CTA takes a share of one lane's keys for NT * 8 (row, head) items of one KV head.  Each of its warps walks tiles of 16 keys, which TMA brings into a ring of its own; the
-// items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.  What bounds it is HBM where lanes have much of their own, else the chain of dependent fetches at a CTA's two
-// ends: so a warp asks for its first tiles before anything else, and rings are short enough for three CTAs on an SM.  40 lanes of 16 heads of 256 over 8 with 300 to 4000 keys of
-// their own: 80 us, 5.4 TB/s; 128 lanes of 32 heads of 128 over 8 with 20 to 700: 35 us, 2.9 TB/s.
+// items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.  What bounds it is HBM where lanes have much of their own, else the chain of dependent fetches at a
+// CTA's two ends: so a warp asks for its first tiles before anything else, rings are short enough for three CTAs on an SM, and warps with one tile on its way each do better than
+// half as many with two (heads of 256: 92 us where those take 104; heads of 64, 4 lanes of 1 to 60 keys: 8 warps 8.3 us, 4 warps 10.1, but 18 where 8 take 22 with two groups of items).
 constexpr int kTile = 16;
 
-template <int D>
+template <int D, int NT>
 struct LaneSmem {
-    static constexpr int WARPS = D == 256 ? 2 : 4, THREADS = WARPS * 32;
+    static constexpr int WARPS = D == 64 && NT == 1 ? 8 : 4, THREADS = WARPS * 32;
     static constexpr int PANELS = D / 64, K_BYTES = kTile * D * 2, STAGE = 2 * K_BYTES;
-    static constexpr int STAGES = D == 64 ? 4 : 2;
+    static constexpr int STAGES = 65536 / (WARPS * STAGE);   // at most
     static constexpr int QP = D + 8, OP = D + 4;
-    __host__ __device__ static constexpr int ring(int nt) { return ((STAGES * STAGE > nt * 8 * (OP + 2) * 4 ? STAGES * STAGE : nt * 8 * (OP + 2) * 4) + 1023) / 1024 * 1024; }
-    static constexpr size_t bytes(int nt) { return 1024 + (size_t)WARPS * ring(nt) + (size_t)nt * 8 * QP * 2; }
+    __host__ __device__ static int ring(int stages) { return (max(stages * STAGE, NT * 8 * (OP + 2) * 4) + 1023) / 1024 * 1024; }
+    static size_t bytes(int stages) { return 1024 + (size_t)WARPS * ring(stages) + (size_t)NT * 8 * QP * 2; }
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
-                                                               int chunk, int shares, int shared_parts, int join) {
-    using L = LaneSmem<D>;
+__global__ void __launch_bounds__(LaneSmem<D, NT>::THREADS) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
+                                                                                   int chunk, int shares, int shared_parts, int join, int stage_bits) {
+    using L = LaneSmem<D, NT>;
     using P = Pair<T>;
-    constexpr int ITEMS = NT * 8, RING = L::ring(NT), kWarps = L::WARPS;
+    constexpr int ITEMS = NT * 8, kWarps = L::WARPS;
+    const int stages = 1 << stage_bits, ring_bytes = L::ring(stages);
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[kWarps * L::STAGES];
     uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    T* qs = reinterpret_cast<T*>(rings + kWarps * RING);
+    T* qs = reinterpret_cast<T*>(rings + kWarps * ring_bytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
     const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y, g = a.q_heads / a.kv_heads;
     const LaneRange at = lane_range(a, lane_id);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
     const int begin = lo / kTile * kTile, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0;
     const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
 
-    uint8_t* ring = rings + warp * RING;
+    uint8_t* ring = rings + warp * ring_bytes;
     uint64_t* full = bars + warp * L::STAGES;
     const int32_t* table = a.tables + lane_id * a.ld_table;
     auto page_row = [&](int i) {
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
         return (int)(page * a.page_rows) + kvh * a.block_tokens + (pos & (a.block_tokens - 1));
     };
     auto load_tile = [&](int i, int row) {   // one lane
-        const int st = i % L::STAGES;
+        const int st = i & (stages - 1);
         const uint32_t dst = smem_u32(ring) + st * L::STAGE;
         bar_expect_tx(&full[st], L::STAGE);
 #pragma unroll
@@ -235,15 +236,16 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
     };
     int next_row = 0;   // of the tile that the ring takes next
     if (lane == 0 && my_tiles > 0) {
-        int rows[L::STAGES + 1];
+        const int ahead = min(stages, my_tiles);
+        int rows[L::STAGES];
 #pragma unroll
-        for (int i = 0; i <= L::STAGES; ++i) rows[i] = i < my_tiles ? page_row(i) : 0;
-        for (int i = 0; i < L::STAGES; ++i) bar_init(&full[i], 1);
+        for (int i = 0; i < L::STAGES; ++i) rows[i] = i < ahead ? page_row(i) : 0;
+        next_row = stages < my_tiles ? page_row(stages) : 0;
+        for (int i = 0; i < stages; ++i) bar_init(&full[i], 1);
         bar_init_fence();
 #pragma unroll
         for (int i = 0; i < L::STAGES; ++i)
-            if (i < my_tiles) load_tile(i, rows[i]);
-        next_row = rows[L::STAGES];
+            if (i < ahead) load_tile(i, rows[i]);
     }
     for (int i = tid; i < ITEMS * (D / 8); i += L::THREADS) {
         const int item = i / (D / 8), c = (i - item * (D / 8)) * 8;
@@ -276,8 +278,8 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
     const uint32_t q_at = smem_u32(qs) + (uint32_t)((lane & 7) * L::QP + (lane >> 3) * 8) * 2;
     bool ok = true;
     for (int i = 0; i < my_tiles; ++i) {
-        const int st = i % L::STAGES;
-        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i / L::STAGES & 1));
+        const int st = i & (stages - 1);
+        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i >> stage_bits & 1));
         if (!ok) {
             if (lane == 0) tell(a.status, kDevWait);
             break;
@@ -356,13 +358,13 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
             for (int n = 0; n < NT; ++n) P::mma(o_acc[n][j], af, b0[n], b1[n]);
         }
         __syncwarp();
-        if (lane == 0 && i + L::STAGES < my_tiles) {
-            load_tile(i + L::STAGES, next_row);
-            if (i + L::STAGES + 1 < my_tiles) next_row = page_row(i + L::STAGES + 1);
+        if (lane == 0 && i + stages < my_tiles) {
+            load_tile(i + stages, next_row);
+            if (i + stages + 1 < my_tiles) next_row = page_row(i + stages + 1);
         }
     }
     if (!ok) {   // what this warp still has under way lands before the CTA ends; the result says so
-        for (int i = 0; i < L::STAGES; ++i)
+        for (int i = 0; i < stages; ++i)
             if (i < my_tiles) bar_wait(&full[i], 0), bar_wait(&full[i], 1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) l_run[n][0] = l_run[n][1] = m_run[n][0] = m_run[n][1] = __int_as_float(0x7fffffff);
@@ -391,7 +393,8 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
             }
         }
     __syncthreads();
-    constexpr int STEP = RING / 4, V = D / 32;
+    constexpr int V = D / 32;
+    const int step = ring_bytes / 4;
     const float* first = reinterpret_cast<const float*>(rings);
     pdl_wait();   // the shared keys' parts; and who comes after this kernel may rely on them too
     for (int item = warp; item < n_items; item += kWarps) {
@@ -401,15 +404,15 @@ __global__ void __launch_bounds__(LaneSmem<D>::THREADS) lane_keys_kernel(const _
         for (int j = 0; j < V; ++j) o[j] = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float mw = first[w * STEP + ITEMS * L::OP + item * 2];
+            const float mw = first[w * step + ITEMS * L::OP + item * 2];
             m = mw > m || mw != mw ? mw : m;
         }
         const float m_use = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = ex2(first[w * STEP + ITEMS * L::OP + item * 2] - m_use);
-            const float* x = first + w * STEP + item * L::OP + lane * V;
-            l += first[w * STEP + ITEMS * L::OP + item * 2 + 1] * f;
+            const float f = ex2(first[w * step + ITEMS * L::OP + item * 2] - m_use);
+            const float* x = first + w * step + item * L::OP + lane * V;
+            l += first[w * step + ITEMS * L::OP + item * 2 + 1] * f;
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] += x[j] * f;
         }
@@ -860,14 +863,20 @@ void launch_tall(const SharedAttnArgs& a, const SharedAttnPlan& p, uint64_t rows
 
 template <typename T, int D, int NT>
 void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
+    using L = LaneSmem<D, NT>;
     auto* kernel = lane_keys_kernel<T, D, NT>;
-    const size_t smem = LaneSmem<D>::bytes(NT);
-    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-    constexpr int threads = LaneSmem<D>::THREADS;
+    // Half the ring (32 KB) where there are more than two CTAs for each SM: more of them run at once, also beside a CTA of the shared keys, and what one waits for another uses (128
+    // lanes of 8 heads with 1 to 60 keys 24.1 us and 20.3; 117 of 4 with one 16.6 and 12.7).  Fewer CTAs need more of their own on its way (32 lanes of 8 heads with 17 to 500 keys
+    // 14.7 us with the whole ring, 15.9 with half; 8 with 3000 23.0 and 26.8).
+    int stage_bits = 0;
+    while ((2 << stage_bits) <= L::STAGES) ++stage_bits;
+    if (stage_bits > 0 && (int64_t)a.lanes * p.shares * a.kv_heads > 2 * kSms) --stage_bits;
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::bytes(L::STAGES));
+    const size_t smem = L::bytes(1 << stage_bits);
     const dim3 grid((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles);
     // behind the shared keys' kernel it starts early: what both read was there before that one
-    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(threads), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1);
-    else kernel<<<grid, threads, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1);
+    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(L::THREADS), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1, stage_bits);
+    else kernel<<<grid, L::THREADS, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1, stage_bits);
     MK_LAUNCH_CHECK();
 }
 
