@@ -841,28 +841,40 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
 }
 
+// The pools as tensor maps with boxes of so many tokens; made anew only where a call's kernels differ in it (a map takes the host 0.6 us).
+struct Maps {
+    alignas(64) CUtensorMap k, v;
+    int box = 0;
+    void need(const SharedAttnArgs& a, int tokens) {
+        if (box == tokens) return;
+        const uint64_t rows = (uint64_t)(a.pool_pages - 1) * (uint64_t)a.page_rows + (uint64_t)a.kv_heads * (uint64_t)a.block_tokens;
+        encode_tma_2d(&k, false, a.k_pool, (uint64_t)a.d, rows, (uint64_t)a.d * 2, 64, (uint32_t)tokens, true);
+        encode_tma_2d(&v, false, a.v_pool, (uint64_t)a.d, rows, (uint64_t)a.d * 2, 64, (uint32_t)tokens, true);
+        box = tokens;
+    }
+};
+
 template <typename T, int D, int NQ, bool OWN>
-void launch_tall(const SharedAttnArgs& a, const SharedAttnPlan& p, uint64_t rows, cudaStream_t s) {
+void launch_tall(const SharedAttnArgs& a, const SharedAttnPlan& p, Maps& maps, cudaStream_t s) {
     using L = SharedSmem<D, NQ>;
     const int box = std::min(a.block_tokens, kKeys);
-    alignas(64) CUtensorMap tk, tv;
-    encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, (uint32_t)box, true);
-    encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, (uint32_t)box, true);
+    maps.need(a, box);
     auto* kernel = shared_keys_kernel<T, D, NQ, OWN>;
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::SMEM);
     if (!OWN) {
-        kernel<<<(unsigned)(p.row_tiles * a.kv_heads * p.shared_parts), L::THREADS, L::SMEM, s>>>(tk, tv, a, box, p.shared_parts, 0, 0, 0);
+        kernel<<<(unsigned)(p.row_tiles * a.kv_heads * p.shared_parts), L::THREADS, L::SMEM, s>>>(maps.k, maps.v, a, box, p.shared_parts, 0, 0, 0);
         MK_LAUNCH_CHECK();
         return;
     }
     const unsigned grid = (unsigned)(a.lanes * p.item_tiles * a.kv_heads * p.shares);
-    if (p.shared_parts > 0) launch_pdl(kernel, dim3(grid), dim3(L::THREADS), L::SMEM, s, tk, tv, a, box, p.shares, p.chunk, p.item_tiles, p.shared_parts);
-    else kernel<<<grid, L::THREADS, L::SMEM, s>>>(tk, tv, a, box, p.shares, p.chunk, p.item_tiles, 0);
+    if (p.shared_parts > 0) launch_pdl(kernel, dim3(grid), dim3(L::THREADS), L::SMEM, s, maps.k, maps.v, a, box, p.shares, p.chunk, p.item_tiles, p.shared_parts);
+    else kernel<<<grid, L::THREADS, L::SMEM, s>>>(maps.k, maps.v, a, box, p.shares, p.chunk, p.item_tiles, 0);
     MK_LAUNCH_CHECK();
 }
 
 template <typename T, int D, int NT>
-void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
+void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, Maps& maps, cudaStream_t s) {
+    maps.need(a, kTile);
     using L = LaneSmem<D, NT>;
     auto* kernel = lane_keys_kernel<T, D, NT>;
     // Half the ring (32 KB) where there are more than two CTAs for each SM: more of them run at once, also beside a CTA of the shared keys, and what one waits for another uses (128
@@ -875,38 +887,35 @@ void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, const CUtens
     const size_t smem = L::bytes(1 << stage_bits);
     const dim3 grid((unsigned)(a.lanes * p.shares), (unsigned)a.kv_heads, (unsigned)p.item_tiles);
     // behind the shared keys' kernel it starts early: what both read was there before that one
-    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(L::THREADS), smem, s, tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1, stage_bits);
-    else kernel<<<grid, L::THREADS, smem, s>>>(tk, tv, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1, stage_bits);
+    if (p.shared_parts > 0) launch_pdl(kernel, grid, dim3(L::THREADS), smem, s, maps.k, maps.v, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1, stage_bits);
+    else kernel<<<grid, L::THREADS, smem, s>>>(maps.k, maps.v, a, p.chunk, p.shares, p.shared_parts, p.joined ? 0 : 1, stage_bits);
     MK_LAUNCH_CHECK();
 }
 
 template <typename T, int D>
 void launch_typed(const SharedAttnArgs& a, const SharedAttnPlan& p, cudaStream_t s) {
-    const uint64_t rows = (uint64_t)(a.pool_pages - 1) * (uint64_t)a.page_rows + (uint64_t)a.kv_heads * (uint64_t)a.block_tokens;
+    Maps maps;
     if (p.shared_parts > 0) {
         if constexpr (D <= 128) {
-            if (p.item_rows == 2) launch_tall<T, D, 2, false>(a, p, rows, s);
-            else launch_tall<T, D, 1, false>(a, p, rows, s);
+            if (p.item_rows == 2) launch_tall<T, D, 2, false>(a, p, maps, s);
+            else launch_tall<T, D, 1, false>(a, p, maps, s);
         } else {
-            launch_tall<T, D, 1, false>(a, p, rows, s);
+            launch_tall<T, D, 1, false>(a, p, maps, s);
         }
     }
     if (p.items >= kItems) {
         if constexpr (D <= 128) {
-            if (p.items > kItems) launch_tall<T, D, 2, true>(a, p, rows, s);
-            else launch_tall<T, D, 1, true>(a, p, rows, s);
+            if (p.items > kItems) launch_tall<T, D, 2, true>(a, p, maps, s);
+            else launch_tall<T, D, 1, true>(a, p, maps, s);
         } else {
-            launch_tall<T, D, 1, true>(a, p, rows, s);
+            launch_tall<T, D, 1, true>(a, p, maps, s);
         }
     } else {
-        alignas(64) CUtensorMap tk, tv;
-        encode_tma_2d(&tk, false, a.k_pool, D, rows, D * 2, 64, kTile, true);
-        encode_tma_2d(&tv, false, a.v_pool, D, rows, D * 2, 64, kTile, true);
         switch (p.items) {
-            case 8: launch_lanes<T, D, 1>(a, p, tk, tv, s); break;
-            case 16: launch_lanes<T, D, 2>(a, p, tk, tv, s); break;
+            case 8: launch_lanes<T, D, 1>(a, p, maps, s); break;
+            case 16: launch_lanes<T, D, 2>(a, p, maps, s); break;
             default:
-                if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, tk, tv, s);
+                if constexpr (D <= 128) launch_lanes<T, D, 3>(a, p, maps, s);
         }
     }
     if (p.joined)
