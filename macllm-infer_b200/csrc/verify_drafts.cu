@@ -31,6 +31,9 @@ namespace cg = cooperative_groups;
 constexpr int kCtas = 8, kThreads = 512, kWarps = kThreads / 32;
 constexpr int kScan = 256;          // threads of the first kernel's CTAs
 constexpr int kCandidates = 2048;   // sorted at once
+// Candidates that are compared with one another, by four threads each; more are sorted (4 lanes with 4 drafts of 128256 in f16: 15.1 us and 21.2 sorted at top_k 40, 17.6 and 21.9 at
+// 100; two threads each, for up to 256: 20.1 and 22.4 at 128, 23.5 and 23.0 at 200, and slower below).
+constexpr int kCounted = 128;
 
 struct Run {
     uint64_t best;   // key of its best token
@@ -108,15 +111,15 @@ __device__ double block_scan(double v, double* red, double* total) {
 }
 
 // 512 E keys, the larger first: a thread has E neighbours, so that most exchanges of the bitonic network are inside a thread or a warp.
-template <int E>
-__device__ void sort_desc(uint64_t* keys) {
+template <int E, typename K>
+__device__ void sort_desc(K* keys) {
     const int tid = threadIdx.x;
-    uint64_t a[E];
+    K a[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) a[e] = keys[tid * E + e];
     for (int size = 2; size <= kThreads * E; size <<= 1) {
         auto exchange = [&](int stride, auto&& partner) {
-            uint64_t y[E];
+            K y[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) y[e] = partner(e);
 #pragma unroll
@@ -143,7 +146,8 @@ __device__ void sort_desc(uint64_t* keys) {
     for (int e = 0; e < E; ++e) keys[tid * E + e] = a[e];
     __syncthreads();
 }
-__device__ void sort_desc(uint64_t* keys, int n) {   // keys behind n are there to be filled up
+template <typename K>
+__device__ void sort_desc(K* keys, int n) {   // keys behind n are there to be filled up
     const int size = n <= kThreads ? kThreads : (n <= 2 * kThreads ? 2 * kThreads : 4 * kThreads);
     for (int j = n + (int)threadIdx.x; j < size; j += kThreads) keys[j] = 0;
     __syncthreads();
@@ -337,14 +341,17 @@ __device__ __forceinline__ void put_lane(const VerifyArgs& a, int lane, int end,
     if ((threadIdx.x & 31) == 0) a.accepted[lane] = end;
 }
 
-// A place in a list for each thread of a warp that wants one.
-__device__ __forceinline__ int list_place(int* count, bool wants) {
-    const unsigned who = __ballot_sync(0xffffffffu, wants);
-    if (who == 0) return 0;
-    const int wl = threadIdx.x & 31, first = __ffs(who) - 1;
-    int at = 0;
-    if (wl == first) at = atomicAdd(count, __popc(who));
-    return __shfl_sync(0xffffffffu, at, first) + __popc(who & ((1u << wl) - 1u));
+// Places in a list, n of them one after the other for each thread of a warp.
+__device__ __forceinline__ int list_places(int* count, int n) {
+    const int wl = threadIdx.x & 31;
+    int upto = n, at = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (wl >= o) upto += other;
+    }
+    if (wl == 31 && upto > 0) at = atomicAdd(count, upto);
+    return __shfl_sync(0xffffffffu, at, 31) + upto - n;
 }
 // Sum over the block, the same in every thread.
 __device__ unsigned long long block_sum(unsigned long long v, unsigned long long* red) {
@@ -452,36 +459,46 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
     int n_all;
     for (;;) {
         const float bound_value = value_of_key(bound);
-        for (int j0 = 0; j0 < n_groups; j0 += kThreads) {   // n_groups is a multiple of 256: whole warps
-            const int j = j0 + tid;
-            const bool reaches = j < n_groups && group_best[j] >= bound_value;
-            const int at = list_place(&s.groups, reaches);
-            if (reaches) group_list[at] = (uint16_t)j;
+        for (int j0 = tid; j0 - tid < n_groups; j0 += 32 * kThreads) {
+            unsigned mine = 0;
+            for (int b = 0; b < 32 && j0 + b * kThreads < n_groups; ++b)
+                if (group_best[j0 + b * kThreads] >= bound_value) mine |= 1u << b;
+            int at = list_places(&s.groups, __popc(mine));
+            for (; mine != 0; mine &= mine - 1) group_list[at++] = (uint16_t)(j0 + (__ffs(mine) - 1) * kThreads);
         }
         __syncthreads();
+        // their tokens, two pieces on their way to a thread (a place for each token by itself: twice the time)
         const int pieces = s.groups * vpt;
-        for (int w0 = 0; w0 < pieces; w0 += kThreads) {
-            const int w = w0 + tid;
-            float f[EPV];
-            int t0 = 0;
+        for (int w0 = 0; w0 < pieces; w0 += 2 * kThreads) {
+            float f[2][EPV];
+            int t0[2] = {INT_MIN / 2, INT_MIN / 2};
 #pragma unroll
-            for (int j = 0; j < EPV; ++j) f[j] = -INFINITY;
-            if (w < pieces) {
-                const int g = group_list[w / vpt], v = (g / kScan * vpt + w % vpt) * kScan + g % kScan;
-                t0 = row.token(v);
-                row.load(v, f);
+            for (int h = 0; h < 2; ++h) {
+                const int w = w0 + h * kThreads + tid;
+#pragma unroll
+                for (int j = 0; j < EPV; ++j) f[h][j] = -INFINITY;
+                if (w < pieces) {
+                    const int g = group_list[w / vpt], v = (g / kScan * vpt + w % vpt) * kScan + g % kScan;
+                    t0[h] = row.token(v);
+                    row.load(v, f[h]);
+                }
             }
-            float highest = f[0];
+            unsigned mine = 0;
 #pragma unroll
-            for (int j = 1; j < EPV; ++j) highest = fmaxf(highest, f[j]);
-            if (!__any_sync(0xffffffffu, w < pieces && highest >= bound_value)) continue;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < EPV; ++j) {
-                const uint64_t key = key_of(f[j], t0 + j);
-                const bool reaches = w < pieces && t0 + j >= 0 && t0 + j < vocab && key >= bound;
-                const int at = list_place(&s.count, reaches);
-                if (reaches && at < kCandidates) keys[at] = key;
-            }
+                for (int j = 0; j < EPV; ++j)
+                    if (t0[h] + j >= 0 && t0[h] + j < vocab && key_of(f[h][j], t0[h] + j) >= bound) mine |= 1u << (h * EPV + j);
+            if (!__any_sync(0xffffffffu, mine != 0)) continue;
+            int at = list_places(&s.count, __popc(mine));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < EPV; ++j)
+                    if (mine >> (h * EPV + j) & 1) {
+                        if (at < kCandidates) keys[at] = key_of(f[h][j], t0[h] + j);
+                        ++at;
+                    }
         }
         __syncthreads();
         n_all = s.count;
@@ -494,12 +511,13 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
         __syncthreads();
     }
     static_assert(kCandidates > kVerifyMaxTopK, "more can be sorted than are wanted");
-    if (n_all <= kThreads) {
-        // Up to four threads to a candidate, which compares it with every other one: who is better, and how much those weigh; later whose token is lower.  The list's order is not
+    if (n_all <= kCounted) {
+        // Four threads to a candidate, which compare it with every other one: who is better, and how much those weigh; later whose token is lower.  The list's order is not
         // the same in every call, so sums are of whole numbers of 2^-52.
         unsigned long long* values = reinterpret_cast<unsigned long long*>(keys + kCandidates);
         constexpr double kUnits = 4503599627370496.0;
-        const int parts = n_all <= kThreads / 4 ? 4 : (n_all <= kThreads / 2 ? 2 : 1), c = tid / parts, part = tid % parts;
+        constexpr int parts = kThreads / kCounted;
+        const int c = tid / parts, part = tid % parts;
         const uint64_t key = c < n_all ? keys[c] : 0;
         const int token = c < n_all ? (int)rank_key_index(key) : -1;
         const double e = c < n_all ? exp(((double)value_of_key(key) - (double)top) * per_t) : 0.0;
@@ -571,23 +589,26 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
         }
         block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), s.red, &kept);
         double* weights = reinterpret_cast<double*>(keys + kVerifyMaxTopK);
+        uint32_t* by_token = reinterpret_cast<uint32_t*>(keys);   // a token and where it was, in 32 bits
+        constexpr uint32_t kLastToken = (1u << 22) - 1;
+        static_assert(kVerifyMaxVocab <= kLastToken && kVerifyMaxTopK <= 1 << 10, "a token and a place fit 32 bits");
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (in[j] && token[j] == d) s.pd = e[j] / kept;
             weights[j0 + j] = in[j] ? e[j] / kept : 0.0;
-            keys[j0 + j] = j0 + j < k ? (uint64_t)(0xFFFFFFFFu - (uint32_t)token[j]) << 32 | (uint32_t)(j0 + j) : 0;
+            by_token[j0 + j] = j0 + j < k ? (kLastToken - (uint32_t)token[j]) << 10 | (uint32_t)(j0 + j) : 0;
         }
         __syncthreads();
         if (d >= 0 && kept_below < s.pd) {
             return make_int2(1, -1);
         }
-        sort_desc(keys, k);   // by token; at most kVerifyMaxTopK, the weights lie behind
+        sort_desc(by_token, k);   // the weights lie behind
         double w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint64_t key = j0 + j < k ? keys[j0 + j] : 0;
-            token[j] = (int)(0xFFFFFFFFu - (uint32_t)(key >> 32));
-            w[j] = j0 + j < k ? weights[(uint32_t)key] : 0.0;
+            const uint32_t key = j0 + j < k ? by_token[j0 + j] : 0;
+            token[j] = (int)(kLastToken - (key >> 10));
+            w[j] = j0 + j < k ? weights[key & 1023] : 0.0;
         }
         __syncthreads();
         ids = reinterpret_cast<int*>(keys);
@@ -862,7 +883,7 @@ void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace,
         const int groups = p.runs * kScan;
         a.list_at = groups * 4;
         a.keys_at = (a.list_at + groups * 2 + 15) / 16 * 16;
-        const size_t smem = (size_t)a.keys_at + kCandidates * 8 + kThreads * 8;
+        const size_t smem = (size_t)a.keys_at + kCandidates * 8 + kCounted * 8;
         ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
         launch_pdl(kernel, dim3((unsigned)(a.lanes * kCtas)), dim3(kThreads), smem, s, a);
     };
