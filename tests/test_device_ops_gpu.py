@@ -331,6 +331,13 @@ def test_numbers_of_drafts(dops, lanes, n):
     verify_check(dops, *verify_case(3, lanes, n, 900), 0.8, 20, 0.9)
 
 
+@pytest.mark.parametrize("top_k", [16, 126, 127, 128, 129, 200, 511, 512, 513, 700, 1023, 1024])
+@pytest.mark.parametrize("vocab", [3001, 70000])
+def test_numbers_of_candidates(dops, top_k, vocab):
+    """Around what is compared with one another, and sorted by one, two and four to a thread."""
+    verify_check(dops, *verify_case(13, 4, 3, vocab, F16, given=top_k % 2 == 0), [0.8, 1.5] * 2, top_k, [0.99, 1.0] * 2)
+
+
 def test_greedy_ragged_and_mixed_lanes(dops):
     verify_check(dops, *verify_case(4, 24, 5, 3000, ragged=True), [0.0, 0.8, 1.0] * 8, [0, 7, 0, 100] * 6, [1.0, 0.6, 1.0, 0.9] * 6)
     verify_check(dops, *verify_case(5, 24, 5, 3000, given=True, ragged=True), [0.0, 0.8, 1.0] * 8, [3, 0, 50, 0] * 6, [0.5, 1.0, 0.9, 1.0] * 6)
