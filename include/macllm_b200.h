@@ -671,8 +671,8 @@ int32_t mk_k_q4k_matmul_tc_noalloc_dev(const void* w_q4k_dev, int64_t rows, int6
  * scores are scale * q.k (scale > 0), with softcap > 0 then softcap * tanh(score / softcap).  A row that sees nothing becomes zeros; rows of q
  * that belong to no lane are left as they were in out.  The first shared_len tokens (whole pages; 0 is allowed) are the same
  * pages in every lane's table, and are read once for all lanes, through lane 0's: the result is what attention lane by lane
- * gives.  Keys and values of a lane's tokens are finite, those of the first shared_len tokens also where a lane is shorter; what lies
- * behind a lane's length may be anything.
+ * gives.  Keys and values of a lane's tokens are finite and their pages in the table, also where a window hides them, those of the first
+ * shared_len tokens also where a lane is shorter; what lies behind a lane's length may be anything.
  * q, out [total] rows of q_heads x head_dim values, q_stride / out_stride values apart; pools of one layer, pages [kv_heads]
  * [block_tokens][head_dim] page_stride values apart (a layer of the model's arena: kv_heads * block_tokens * head_dim); all
  * f16 or all bf16 (type).  Rows, strides and pools are 16-byte aligned.  head_dim 64, 128 or 256; any group size up to 128.  Scores, softmax
@@ -707,7 +707,7 @@ int32_t mk_k_copy_pages_dev(void* k_pool_dev, void* v_pool_dev, int64_t layers, 
 
 /* Kept tokens of lanes moved together: token keep[i][j] of the pages from_tables[i] becomes token first[i] + j of the pages
  * to_tables[i], for j < counts[i], in every layer and head, K and V.  keep ascends.  The two tables may name the same pages (then
- * first[i] <= keep[i][0], and what has been kept stays where it is read until it has moved); otherwise no page of one lane's
+ * first[i] <= keep[i][0], no token is kept twice, and what has been kept stays where it is read until it has moved); otherwise no page of one lane's
  * destination is read or written by another copy.  Accepted branches of drafted trees, and contexts thinned out. */
 int32_t mk_k_gather_tokens_dev(void* k_pool_dev, void* v_pool_dev, int64_t layers, int64_t pages, int32_t kv_heads, int32_t block_tokens, int32_t row_bytes,
                                const int32_t* from_tables_dev, int64_t from_stride, int32_t from_width, const int32_t* keep_dev, int64_t keep_stride, int32_t keep_width,

@@ -205,7 +205,10 @@ __global__ void __launch_bounds__(LaneSmem<D, NT>::THREADS) lane_keys_kernel(con
     const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y, g = a.q_heads / a.kv_heads;
     const LaneRange at = lane_range(a, lane_id);
     const int item0 = blockIdx.z * ITEMS, n_items = min(ITEMS, at.n * g - item0);
-    if (n_items <= 0) return;
+    if (n_items <= 0) {
+        pdl_wait();   // also where no lane has rows, nobody behind this kernel overtakes the one before it
+        return;
+    }
     const int first_key = a.shared;
     const int p0 = at.position + item0 / g, p1 = at.position + (item0 + n_items - 1) / g;
     const int lo = max(first_key + share * chunk, attention_first_key(max(p0, 0), a.window, 0)), hi = min(min(p1 + 1, at.keys), shares > 1 ? first_key + (share + 1) * chunk : INT_MAX);
@@ -493,7 +496,10 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               tile = OWN ? block - lane_id * lane_tiles : block;
     pdl_trigger();
     const LaneRange mine_range = OWN ? lane_range(a, lane_id) : LaneRange{0, a.total, 0, 0};
-    if (OWN && tile * (NQ * kItems) >= mine_range.n * g) return;
+    if (OWN && tile * (NQ * kItems) >= mine_range.n * g) {
+        pdl_wait();
+        return;
+    }
     const int base_key = OWN ? a.shared : 0, keys_end = OWN ? min(mine_range.keys, a.shared + (split + 1) * chunk) : a.shared;   // positions of tiles are counted from the first
     const int32_t* table = a.tables + lane_id * a.ld_table;
     constexpr bool kEarly = !OWN;

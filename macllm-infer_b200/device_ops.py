@@ -173,7 +173,7 @@ def copy_pages(k_pool, v_pool, copies, *, status=None) -> None:
 
 def gather_tokens(k_pool, v_pool, from_tables, keep, counts, to_tables, first, *, status=None) -> None:
     """Moves kept tokens of lanes together, in every layer: token keep[i, j] of the pages from_tables[i] becomes token first[i] + j of the pages to_tables[i], for
-    j < counts[i].  keep ascends; the tables name the same pages, or pages that nothing else here reads or writes."""
+    j < counts[i].  keep ascends; the tables name the same pages (then first[i] <= keep[i, 0] and no token is kept twice), or pages that nothing else here reads or writes."""
     if keep.dim() != 2:
         raise ValueError("keep is [lanes, kept tokens]")
     device, lanes = k_pool.get_device(), keep.shape[0]
