@@ -8,8 +8,8 @@
 //
 // Two kernels.  The first streams every row that can be reached once, a run of tokens to a CTA and at most 32 of them to a thread, and leaves what a run amounts
 // to: its best token, whether it holds what is no logit, the sum of its weights (whole vocabulary), and the best value of each thread's tokens (top_k).  What bounds it is HBM.
-// The second finishes lanes, eight CTAs in a cluster to each.  Over the whole vocabulary a row's sum follows from its runs', which tells where the lane ends, and
-// the cluster goes through that one row again, for the draw.  With a top_k each CTA takes every eighth row: the k-th best of the threads' best values is a bound that at
+// The second finishes lanes, a cluster of eight CTAs to each, or fewer where there are many lanes.  Over the whole vocabulary a row's sum follows from its runs', which tells where the lane ends, and
+// the cluster goes through that one row again, for the draw.  With a top_k they share out the rows: the k-th best of the threads' best values is a bound that at
 // least k tokens reach and few more do, and only the tokens of threads that reach it are read again; where too many reach it (thousands of equal
 // logits) bisection over (value, token) finds one that fewer do.
 //
@@ -28,7 +28,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kCtas = 8, kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMostCtas = 8, kThreads = 512, kWarps = kThreads / 32;
 constexpr int kScan = 256;          // threads of the first kernel's CTAs
 constexpr int kCandidates = 2048;   // sorted at once
 // Candidates that are compared with one another, by four threads each; more are sorted (4 lanes with 4 drafts of 128256 in f16: 15.1 us and 21.2 sorted at top_k 40, 17.6 and 21.9 at
@@ -652,14 +652,14 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
 }
 
 template <typename T>
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_constant__ VerifyArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ TopShared top_shared;
-    __shared__ double sum_of[2][kCtas], region[kWarps], s_z;
+    __shared__ double sum_of[2][kMostCtas], region[kWarps], s_z;
     __shared__ uint64_t s_best;
     __shared__ int s_end, s_bad, s_pick, s_last;
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, rank = (int)cluster.block_rank(), lane = blockIdx.x / kCtas, n_drafts = a.n_drafts, vocab = a.vocab;
+    const int tid = threadIdx.x, warp = tid >> 5, wl = tid & 31, ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = blockIdx.x / ctas, n_drafts = a.n_drafts, vocab = a.vocab;
     const int32_t* drafts = a.drafts + (int64_t)lane * n_drafts;
     const float* u = a.u + (int64_t)lane * (n_drafts + 1);
     const float temperature = temperature_of(a, lane), top_p = a.top_p[lane];
@@ -682,10 +682,10 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     __syncthreads();
     pdl_wait();
     if (hot && !whole) {
-        // ---- rows with a top_k, every eighth one
+        // ---- rows with a top_k, shared out over the CTAs
         k = min(min(k, kVerifyMaxTopK), vocab);
         int2* rows = a.rows + (int64_t)lane * (n_drafts + 1);
-        for (int i = rank; i <= n; i += kCtas) {
+        for (int i = rank; i <= n; i += ctas) {
             const int2 r = finish_top_row<T>(a, top_shared, smem, lane, i, i < n ? drafts[i] : -1, k, temperature, top_p, (double)u[i], u_draw);
             if (tid == 0) rows[i] = r;
         }
@@ -739,13 +739,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
         return;
     }
     // ---- the draw: every warp adds up a run of its own, and a CTA looks through the one where the target lies
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");   // every CTA is there before one writes to another's memory
     const T* x = logits + end * a.ld;
     const int d = end < n ? drafts[end] : -1;
     const float* q = probs == nullptr || d < 0 ? nullptr : probs + (int64_t)end * vocab;
     const double z = s_z;
     const Exponential weight(value_of_key(s_best), temperature);
     const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
-    const int chunk = (vocab + 4 * kCtas - 1) / (4 * kCtas) * 4, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
+    const int chunk = (vocab + 4 * ctas - 1) / (4 * ctas) * 4, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
     const int run = (n1 - n0 + 4 * kWarps - 1) / (4 * kWarps) * 4, r_lo = min(n1, n0 + warp * run), r_hi = min(n1, r_lo + run);
     const bool fours = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;   // rows begin where four values can be read at once
     bool rest = d >= 0;
@@ -792,17 +793,17 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
         if (wl == 0) region[warp] = part;
+        if (sums == sum_of[0]) asm volatile("barrier.cluster.wait;" ::: "memory");
         __syncthreads();
         if (warp == 0) {
             double s = region[wl % kWarps];
 #pragma unroll
             for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (wl < kCtas) *cluster.map_shared_rank(sums + rank, wl) = s;
+            if (wl < ctas) *cluster.map_shared_rank(sums + rank, wl) = s;
         }
         cluster.sync();
         total = 0.0;
-#pragma unroll
-        for (int c = 0; c < kCtas; ++c) total += sums[c];
+        for (int c = 0; c < ctas; ++c) total += sums[c];
         if (total > 0.0 || !rest) break;
         rest = false;   // the draft's distribution covers the target's
         sums = sum_of[1];
@@ -811,8 +812,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) finish
     // the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
     double upto = 0.0;
     int at = -1;
-#pragma unroll
-    for (int c = 0; c < kCtas; ++c) {
+    for (int c = 0; c < ctas; ++c) {
         if (upto > target) break;
         if (sums[c] > 0.0) at = c;
         upto += sums[c];
@@ -885,7 +885,11 @@ void launch_verify_drafts(VerifyArgs a, const VerifyPlan& p, uint8_t* workspace,
         a.keys_at = (a.list_at + groups * 2 + 15) / 16 * 16;
         const size_t smem = (size_t)a.keys_at + kCandidates * 8 + kCounted * 8;
         ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-        launch_pdl(kernel, dim3((unsigned)(a.lanes * kCtas)), dim3(kThreads), smem, s, a);
+        // An SM holds two of these CTAs: with many lanes fewer to each (64 lanes with 4 drafts of 151936, whole vocabulary: 78 us with eight, 67 with four, 78 with two; 128 with 4 of
+        // 128256: 131, 116, 114), but not where all but a few fit (40 with 6 drafts of 128256, top_k 64: 30 us with eight, 39 with four).
+        int ctas = kMostCtas;
+        while (ctas > 2 && (int64_t)a.lanes * ctas > 384) ctas /= 2;
+        launch_pdl_cluster(kernel, ctas, dim3((unsigned)(a.lanes * ctas)), dim3(kThreads), smem, s, a);
     };
     if (a.type == 0) {
         switch (p.vpt) {

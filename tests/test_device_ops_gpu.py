@@ -338,6 +338,14 @@ def test_numbers_of_candidates(dops, top_k, vocab):
     verify_check(dops, *verify_case(13, 4, 3, vocab, F16, given=top_k % 2 == 0), [0.8, 1.5] * 2, top_k, [0.99, 1.0] * 2)
 
 
+@pytest.mark.parametrize("lanes", [47, 49, 97, 300])
+@pytest.mark.parametrize("given", [False, True])
+def test_numbers_of_lanes(dops, lanes, given):
+    """Eight, four and two CTAs to a lane, all kinds of lanes beside one another."""
+    t, k, p = (np.resize(v, lanes) for v in ([0.9, 0.9, 0.0, 1.2, 0.7], [0, 20, 0, 200, 0], [1.0, 0.9, 1.0, 1.0, 1.0]))
+    verify_check(dops, *verify_case(14, lanes, 4, 901, given=given, ragged=True), t, k, p)
+
+
 def test_greedy_ragged_and_mixed_lanes(dops):
     verify_check(dops, *verify_case(4, 24, 5, 3000, ragged=True), [0.0, 0.8, 1.0] * 8, [0, 7, 0, 100] * 6, [1.0, 0.6, 1.0, 0.9] * 6)
     verify_check(dops, *verify_case(5, 24, 5, 3000, given=True, ragged=True), [0.0, 0.8, 1.0] * 8, [3, 0, 50, 0] * 6, [0.5, 1.0, 0.9, 1.0] * 6)
