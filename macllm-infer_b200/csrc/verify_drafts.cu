@@ -176,6 +176,11 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
 // The larger, or NaN where there is one.
 __device__ __forceinline__ float max_or_nan(float a, float b) {
     float r;
@@ -194,13 +199,12 @@ struct Exponential {
         least = -125.f / hi;
     }
     __device__ __forceinline__ void operator()(float& a, float& b) const {
-        a = fmaxf(a - top, least);
-        b = fmaxf(b - top, least);
-        const Two y = two(a, b), h = two(hi, hi), t = mul2(y, h), lost = fma2(y, two(lo, lo), fma2(y, h, mul2(t, two(-1.f, -1.f))));
         float u, v;
-        apart(t, u, v);
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(u));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(v));
+        apart(add2(two(a, b), two(-top, -top)), u, v);
+        const Two y = two(fmaxf(u, least), fmaxf(v, least)), minus_t = mul2(y, two(-hi, -hi)), lost = fma2(y, two(lo, lo), fma2(y, two(hi, hi), minus_t));
+        apart(minus_t, u, v);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(-u));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(-v));
         const Two e = two(u, v);
         apart(fma2(e, mul2(lost, two(0.69314718f, 0.69314718f)), e), a, b);
     }
