@@ -178,6 +178,7 @@ __device__ __forceinline__ void store_row(T* out, const float (&o)[V], float l) 
 // items are the short side of both products: S^T = K Q^T, O^T = V^T P^T.  What bounds it is HBM where lanes have much of their own, else the chain of dependent fetches at a
 // CTA's two ends: so a warp asks for its first tiles before anything else, rings are short enough for three CTAs on an SM, and warps with one tile on its way each do better than
 // half as many with two (heads of 256: 92 us where those take 104; heads of 64, 4 lanes of 1 to 60 keys: 8 warps 8.3 us, 4 warps 10.1, but 18 where 8 take 22 with two groups of items).
+// 40 lanes of 16 heads of 256 over 8 with 300 to 4000 keys of their own: 79 us, 6.0 TB/s; 128 lanes of 32 heads of 128 over 8 with 20 to 700: 34 us, 3.0 TB/s.
 constexpr int kTile = 16;
 
 template <int D, int NT>
@@ -455,15 +456,16 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
 //
 // All rows of the batch see the same keys, so they are the rows of one tall product: the (row, head) items of a KV head in tiles of 128, NQ tiles to a CTA, over a share of
 // the keys in tiles of 64.  One warp brings keys and values by TMA (two with two tiles of items: a page of 16 tokens is 2 KB a box,
-// and one warp's requests, sixteen a tile of keys, bounded the kernel at 2000 clocks), one per tile of items issues the tcgen05 products, four do its softmax, a thread per item.  Scores of a tile
+// and one warp's requests, sixteen a tile of keys, bounded the kernel at 2000 clocks for two tiles of items), one per tile of items issues the tcgen05 products, four do its softmax, a thread per item.  Scores of a tile
 // of keys go to one of two areas of tensor memory that a tile of items has; its weights go back over its scores, as the A operand of O += P V; the scores of the next tile are
 // made meanwhile.  With two tiles of items a key is fetched once for both; with one, two CTAs share an SM.  The running maximum follows only when a tile exceeds it by kSlack
 // (weights stay below 2^kSlack).
 //
 // What bounds it, for two tiles of items and a tile of keys: the exponentials, 16 per clock and SM, take 1024 clocks; at heads of 128 the products take 1280 (measured alone: 48 clocks for
 // 16 dimensions of 128 x 64 scores, whose operands shared memory delivers in that time, 65 for 16 keys of 128 x 128 outputs); at heads of 64 half of that.  Left alone, the warps that
-// share a quarter of the SM fall into step and the exponential unit idles while both do the rest, so they take turns (heads of 64: 1850 clocks a tile, 1470 so; heads of 128: 2000 and 1850).
-// 128 lanes of 32 heads of 128 over 8 behind 32768 shared tokens: 78 us, 880 TFLOP/s; 32 lanes behind 2048: 7 us.
+// share a quarter of the SM fall into step and the exponential unit idles while both do the rest, so they take turns (a tile of keys, when that was built: heads of 64 1850 clocks, 1470 so; heads of 128 2000 and 1850).
+// 128 lanes of 32 heads of 128 over 8 behind 32768 shared tokens: 73 us, 940 TFLOP/s, the tensor pipe 54 % and the exponential unit 55 % busy; 24 lanes of 16 heads over 4 with up to
+// five rows behind 16384: 27 us.
 constexpr float kSlack = 8.f;
 constexpr int kItems = 128, kKeys = 64;
 
