@@ -108,7 +108,7 @@ def shared_attention(q, k_pool, v_pool, tables, lengths, shared_len: int, *, sca
     if total and q_strides[1:] != (dim, 1):
         raise ValueError("the heads of a row are dense")
     if out is None:
-        out, out_stride = q.new_empty(shape), heads * dim
+        out, out_stride = torch.empty_like(q), heads * dim   # dense, since the heads of a row are
     else:
         out_strides = out.stride()
         if out.shape != shape or out.dtype is not dtype or out.get_device() != device or (total and out_strides[1:] != (dim, 1)):
@@ -142,9 +142,9 @@ def verify_drafts(logits, drafts, u, *, temperature, top_k, top_p, draft_probs=N
     n -= 1
     given = _dense(drafts, _I32, (lanes, n), device, "drafts")
     if tokens is None:
-        tokens = u.new_empty(of_row, dtype=_I32)
+        tokens = torch.empty_like(u, dtype=_I32)
     if accepted is None:
-        accepted = u.new_empty(of_lane, dtype=_I32)
+        accepted = torch.empty_like(top_k)
     space = logits.new_empty(need // logits.element_size() + 1)
     _run(device, capi.lib().mk_k_verify_drafts_dev, _TYPES[dtype], logits.data_ptr(), ld, lanes, n, vocab, given,
          None if draft_probs is None else _dense(draft_probs, _F32, (lanes, n, vocab), device, "draft_probs"), _dense(u, _F32, of_row, device, "u"),
