@@ -670,8 +670,8 @@ int32_t mk_k_q4k_matmul_tc_noalloc_dev(const void* w_q4k_dev, int64_t rows, int6
  * `rows` each, total = lanes * rows.  A row at position p attends to max(0, p - window + 1) .. p (window 0: from the first);
  * scores are scale * q.k (scale > 0), with softcap > 0 then softcap * tanh(score / softcap).  A row that sees nothing becomes zeros; rows of q
  * that belong to no lane are left as they were in out.  The first shared_len tokens (whole pages; 0 is allowed) are the same
- * pages in every lane's table, and are read once for all lanes, through lane 0's: the result is what attention lane by lane
- * gives.  Keys and values of a lane's tokens are finite and their pages in the table, also where a window hides them, those of the first
+ * pages in every lane's table, and are read once for all lanes, through lane 0's (where they are few, by each lane through its own):
+ * the result is what attention lane by lane gives.  Keys and values of a lane's tokens are finite and their pages in the table, also where a window hides them, those of the first
  * shared_len tokens also where a lane is shorter; what lies behind a lane's length may be anything.
  * q, out [total] rows of q_heads x head_dim values, q_stride / out_stride values apart; pools of one layer, pages [kv_heads]
  * [block_tokens][head_dim] page_stride values apart (a layer of the model's arena: kv_heads * block_tokens * head_dim); all

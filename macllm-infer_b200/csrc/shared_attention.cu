@@ -937,8 +937,14 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
     const int g = q_heads / kv_heads;
     const int64_t items = (int64_t)rows * g;
     if (items <= 0 || lanes <= 0 || total <= 0) return p;
+    const bool small = items <= 16 || (items <= 24 && d != 256 && lanes * (int64_t)kv_heads < kSms);
+    // Few keys: every lane reads the shared ones too, in one launch without parts (4 lanes of 4 KV heads of 64: 4.1 us and 8.0 with the shared keys' kernel behind 64 shared tokens, 7.7 and 8.4
+    // behind 512, 11.3 and 8.9 behind 1024; of 8 heads of 128: 5.0 and 9.0, 11.5 and 9.6 behind 512; 32 lanes: 5.7 and 9.5, 8.7 and 10.2 behind 256), as long as two CTAs an SM do for them.
+    const int64_t all_keys = std::min((int64_t)width * block_tokens, window > 0 ? (int64_t)window + rows : INT64_MAX);
+    p.alone = shared > 0 && small && lanes * (int64_t)kv_heads <= 2 * kSms && all_keys <= (d == 64 ? 640 : 384);
+    if (p.alone) shared = 0;
     const int64_t keys = (int64_t)width * block_tokens - shared;
-    if (items > 24 || (items > 16 && (d == 256 || lanes * (int64_t)kv_heads >= kSms))) {
+    if (!small) {
         // Lanes of more items than the small products take at once (17 to 24: where lanes fill the device; 31 lanes of 20 items 39 us so, 47 with the others, 24 lanes 54 and 50): tiles of 128 or 256 of them, and their keys in shares until about two CTAs are there for each place on an SM
         p.items = d <= 128 && items > kItems ? 2 * kItems : kItems;
         p.item_tiles = (int)((items + p.items - 1) / p.items);
@@ -952,6 +958,7 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
         const int64_t ctas = (int64_t)lanes * kv_heads, wanted = std::max<int64_t>(1, (3 * kSms / 2 + ctas - 1) / ctas);
         p.chunk = (int)std::min<int64_t>(std::max<int64_t>(256, (keys + wanted - 1) / wanted + 15), d == 256 ? 512 : 1024) / 16 * 16;
     }
+    if (p.alone) p.chunk = (int)((keys + 15) / 16 * 16);
     p.shares = (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk);
     if (shared > 0) {
         // Tiles of items two at a time where there are more than one.  Shares of the shared keys: a CTA has an SM to itself; a tile of keys takes it about 0.7 us, or 1 us for two tiles of items, its start and end 4 us, and a share's results are written and read once (2.5 TB/s, and 0.1 us).
@@ -976,6 +983,7 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
 
 void launch_shared_attention(SharedAttnArgs a, const SharedAttnPlan& p, cudaStream_t s) {
     if (a.lanes <= 0 || a.total <= 0 || a.rows <= 0) return;
+    if (p.alone) a.shared = 0;
     for (a.bt_shift = 0; (1 << a.bt_shift) < a.block_tokens; ++a.bt_shift) {}
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.parts * a.total * a.q_heads * a.d);
     switch (a.d) {

@@ -35,6 +35,7 @@ struct SharedAttnArgs {
 
 // How a call is cut, from sizes alone.
 struct SharedAttnPlan {
+    bool alone = false;      // each lane reads the shared keys as its own
     int item_tiles = 0;      // blocks of (row, head) items of a lane and KV head
     int items = 0;           // items of such a block, a multiple of 8
     int chunk = 0, shares = 0;   // keys of a lane's share, and shares
