@@ -134,6 +134,18 @@ def test_rows_at_and_before_the_first_key(dops):
     assert (got[0] == 0).all()
 
 
+@pytest.mark.parametrize("dim, kv_heads", [(64, 4), (128, 8), (256, 2)])
+@pytest.mark.parametrize("shared", [16, 320, 368, 576, 640])
+@pytest.mark.parametrize("lanes", [1, 5, 40])
+def test_few_keys(dops, dim, kv_heads, shared, lanes):
+    """Around the numbers of keys and lanes from which the shared ones are read once; lanes shorter than them and without rows among them."""
+    own = [16, 3, -7, 0, 15][:lanes] * max(1, lanes // 5)
+    rows = [2, 1, 2, 0, 4][:lanes] * max(1, lanes // 5)
+    b = Batch(BF16, 2 * kv_heads, kv_heads, dim, 16, shared, own, rows, seed=30)
+    for window, softcap in ((0, 0.0), (100, 30.0)):
+        b.check(b.run(dops, window=window, softcap=softcap), window, softcap)
+
+
 @pytest.mark.parametrize("window", [1, 5, 64, 300, 2000])
 @pytest.mark.parametrize("softcap", [0.0, 20.0])
 @pytest.mark.parametrize("dim", [128, 256])
