@@ -189,14 +189,14 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
 }
 
 // exp((x - top) / temperature) with 1 / (temperature ln 2) as the sum of two 32-bit numbers: t = y hi rounded, what it lost and y lo come behind as a factor.  What is below 2^-126 of the
-// best counts as that much, -inf too.
+// best counts as 0 (ex2 flushes what is no normal number), -inf too: y is not followed beyond 2^-160.
 struct Exponential {
     float top, hi, lo, least;
     __device__ __forceinline__ Exponential(float best, float temperature) : top(best) {
         const double unit = 1.4426950408889634074 / (double)temperature;
         hi = (float)unit;
         lo = (float)(unit - (double)hi);
-        least = -125.f / hi;
+        least = -160.f / hi;
     }
     __device__ __forceinline__ void operator()(float& a, float& b) const {
         float u, v;
@@ -657,6 +657,12 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
     return make_int2(0, s.pick < INT_MAX ? s.pick : s.last);
 }
 
+// A token's share of a draw in 64 bits.  Not inlined: it is needed once in 2^24 draws, and its registers are everyone's.
+__device__ __noinline__ double wide_share(float x, float top, float temperature, bool rest, double z, float q) {
+    const double w = exp(((double)x - (double)top) / (double)temperature);
+    return rest ? fmax(w / z - (double)q, 0.0) : w;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_constant__ VerifyArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -764,11 +770,17 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
         }
     };
     auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
+    auto share64 = [&](int t) { return wide_share(value_of(x[t]), value_of_key(s_best), temperature, rest, s_z, q_at(t)); };
+    // All the weights that 32 bits leave out are together below 2^-100 of the whole.  Where the target is so small that they may decide (u = 0, or a remainder of nothing else), shares are
+    // 64-bit: one draw in 2^24, or where the draft's distribution all but covers the target's.
+    constexpr double kLeastTarget = 0x1p-60;
+    bool wide = false, first = true;
     double total = 0.0, *sums = sum_of[0];
-    for (;;) {
+    for (;; first = false) {
         constexpr int AHEAD = 4;   // fours of tokens a thread has on their way together
         double part = 0.0;
-        for (int t0 = r_lo + wl * 4; t0 < r_hi; t0 += 128 * AHEAD) {
+        for (int t = r_lo + wl; wide && t < r_hi; t += 32) part += share64(t);
+        for (int t0 = r_lo + wl * 4; !wide && t0 < r_hi; t0 += 128 * AHEAD) {
             float l[AHEAD][4], qv[AHEAD][4];
 #pragma unroll
             for (int c = 0; c < AHEAD; ++c) {
@@ -789,17 +801,16 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
             }
 #pragma unroll
             for (int c = 0; c < AHEAD; ++c) {
-                const int there = r_hi - (t0 + 128 * c);
-                if (there <= 0) break;
+                if (t0 + 128 * c >= r_hi) break;
                 shares2(l[c][0], l[c][1], qv[c][0], qv[c][1]);
                 shares2(l[c][2], l[c][3], qv[c][2], qv[c][3]);
-                part += (double)((l[c][0] + (there > 1 ? l[c][1] : 0.f)) + ((there > 2 ? l[c][2] : 0.f) + (there > 3 ? l[c][3] : 0.f)));
+                part += (double)((l[c][0] + l[c][1]) + (l[c][2] + l[c][3]));
             }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
         if (wl == 0) region[warp] = part;
-        if (sums == sum_of[0]) asm volatile("barrier.cluster.wait;" ::: "memory");
+        if (first) asm volatile("barrier.cluster.wait;" ::: "memory");
         __syncthreads();
         if (warp == 0) {
             double s = region[wl % kWarps];
@@ -810,9 +821,10 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
         cluster.sync();
         total = 0.0;
         for (int c = 0; c < ctas; ++c) total += sums[c];
-        if (total > 0.0 || !rest) break;
-        rest = false;   // the draft's distribution covers the target's
-        sums = sum_of[1];
+        if (!wide && !(u_draw * total >= kLeastTarget)) wide = true;
+        else if (rest && !(total > 0.0)) rest = false;   // the draft's distribution covers the target's
+        else break;
+        sums = sums == sum_of[0] ? sum_of[1] : sum_of[0];   // nobody is still at the one before the last
     }
     const double target = u_draw * total;
     // the first CTA up to whose end the sum exceeds the target, or, where rounding left none, the last with a share; the same for its warps' runs
@@ -839,11 +851,14 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
     const int at_lo = min(n1, n0 + w_at * run), at_hi = min(n1, at_lo + run);
     for (int t0 = at_lo; t0 < at_hi; t0 += kThreads) {
         const int t = t0 + tid;
-        float r_mine = t < at_hi ? value_of(x[t]) : -INFINITY, none = -INFINITY;
-        const bool masked = r_mine == -INFINITY;
-        shares2(r_mine, none, t < at_hi ? q_at(t) : 0.f, 0.f);
-        const double r = masked ? 0.0 : (double)r_mine;
-        double all;
+        double r = 0.0, all;
+        if (wide) {
+            if (t < at_hi) r = share64(t);
+        } else {
+            float r_mine = t < at_hi ? value_of(x[t]) : -INFINITY, none = -INFINITY;
+            shares2(r_mine, none, t < at_hi ? q_at(t) : 0.f, 0.f);
+            r = (double)r_mine;
+        }
         const double c = before + block_scan(r, top_shared.red, &all);
         if (r > 0.0) {
             atomicMax(&s_last, t);

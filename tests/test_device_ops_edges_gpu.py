@@ -1,0 +1,65 @@
+"""Operators over device buffers at the edges of what their calls allow: draws at the ends of the unit interval, settings and rows that end a lane, large caps, and the
+forms of the attention that few sizes reach."""
+import importlib
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_device_ops_gpu import BF16, F16, F32, Batch, dops, pools, verify_case, verify_check, verify_plain  # noqa: E402,F401 (dops is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def verify(dops, logits, drafts, u, probs, temperature, top_k, top_p=1.0, status=None):
+    lanes = len(u)
+    settings = [torch.from_numpy(np.broadcast_to(np.asarray(v, dtype=d), (lanes,)).copy()) for v, d in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32))]
+    tokens, accepted = dops.verify_drafts(logits.cuda(), torch.from_numpy(drafts).cuda(), torch.from_numpy(u).cuda(), temperature=settings[0].cuda(), top_k=settings[1].cuda(),
+                                          top_p=settings[2].cuda(), draft_probs=None if probs is None else torch.from_numpy(probs).cuda(), status=status)
+    return tokens.cpu().numpy(), accepted.cpu().numpy(), [x.numpy() for x in settings]
+
+
+def masked_case(mask, kind, lanes, dtype, seed=40, vocab=9000, live=60):
+    """Rows in which `live` tokens in the middle count and all others are masked: no draft, a looked-up one or one of a distribution, both on a masked token, and a
+    distribution that covers the target's."""
+    rng = np.random.default_rng(seed)
+    logits = torch.full((lanes, 2, vocab), mask, dtype=F32)
+    at = 5003 + 7 * np.arange(live)
+    logits[:, :, at] = torch.tensor(rng.standard_normal((lanes, 2, live)), dtype=F32)
+    if kind == "covers":
+        logits[:, :, at[1:]] = mask
+    if dtype != F32:
+        logits = logits.clamp_min(torch.finfo(dtype).min if math.isfinite(mask) else -math.inf).to(dtype)
+    drafts, probs = np.full((lanes, 1), -1 if kind == "none" else 3, np.int32), None
+    if kind == "given":
+        z = np.exp(rng.standard_normal((lanes, 1, vocab)))
+        probs = (z / z.sum(-1, keepdims=True)).astype(np.float32)
+    elif kind == "covers":
+        probs = np.zeros((lanes, 1, vocab), np.float32)
+        probs[:, :, at[0]] = 1.0
+        probs[:, :, 3] = 1e-9
+    return logits, drafts, probs
+
+
+@pytest.mark.parametrize("mask", [-math.inf, -1e9, -3.0e38, -100.0])
+@pytest.mark.parametrize("kind", ["none", "looked up", "given", "covers"])
+@pytest.mark.parametrize("lanes, dtype", [(1, F32), (60, F32), (100, F32), (3, F16), (3, BF16)])
+def test_whole_vocabulary_draws_at_the_ends_of_the_unit_interval(dops, mask, kind, lanes, dtype):
+    """Masked tokens in front and behind: u = 0 draws the first token that has a weight in 64 bits (a mask of -100 leaves one), the highest u the last that counts."""
+    logits, drafts, probs = masked_case(mask, kind, lanes, dtype)
+    for end in (0.0, 1e-30, 2.0 ** -24, 1.0 - 2.0 ** -24):
+        u = np.full((lanes, 2), 0.5, np.float32)
+        u[:, 1] = end
+        tokens, accepted, (t, k, p) = verify(dops, logits, drafts, u, probs, 0.9, 0)
+        want, count, _ = verify_plain(logits.float().numpy(), drafts, u, t, k, p, probs)
+        assert np.array_equal(accepted, count) and np.array_equal(tokens, want), (end, tokens[:3].tolist(), want[:3].tolist())
+
+
+@pytest.mark.parametrize("kind", ["none", "looked up", "given", "covers"])
+@pytest.mark.parametrize("vocab", [32000, 128256])
+def test_a_draw_of_zero_behind_a_long_mask(dops, kind, vocab):
+    logits, drafts, probs = masked_case(-math.inf, kind, 2, F32, vocab=vocab)
+    u = np.zeros((2, 2), np.float32)
+    tokens, _, _ = verify(dops, logits, drafts, u, probs, 1.0, 0)
+    assert (tokens[:, 0] == 5003).all()
