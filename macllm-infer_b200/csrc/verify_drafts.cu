@@ -519,9 +519,10 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
     static_assert(kCandidates > kVerifyMaxTopK, "more can be sorted than are wanted");
     if (n_all <= kCounted) {
         // Four threads to a candidate, which compare it with every other one: who is better, and how much those weigh; later whose token is lower.  The list's order is not
-        // the same in every call, so sums are of whole numbers of 2^-52.
+        // the same in every call, so sums are of whole numbers of 2^-52.  Where the target is less than 2^-40 (u = 0, or a remainder of next to nothing) what is below a unit may decide:
+        // then candidates are sorted, and their shares are 64-bit numbers.
         unsigned long long* values = reinterpret_cast<unsigned long long*>(keys + kCandidates);
-        constexpr double kUnits = 4503599627370496.0;
+        constexpr double kUnits = 0x1p52, kLeastUnits = 0x1p12;
         constexpr int parts = kThreads / kCounted;
         const int c = tid / parts, part = tid % parts;
         const uint64_t key = c < n_all ? keys[c] : 0;
@@ -550,28 +551,25 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
         }
         const double p = in ? e * (kUnits / (double)kept) : 0.0;
         if (in && token == d) s.pd = p;
-        unsigned long long r = __double2ull_rn((d >= 0 && in ? fmax(p - qt, 0.0) : p) * kUnits);
+        const unsigned long long r = __double2ull_rn((d >= 0 && in ? fmax(p - qt, 0.0) : p) * kUnits);
         if (part == 0) values[c] = r;
         __syncthreads();
         if (d >= 0 && kept_below < s.pd) return make_int2(1, -1);
-        unsigned long long total = block_sum(part == 0 ? r : 0ull, reinterpret_cast<unsigned long long*>(s.red));
-        if (total == 0) {   // the draft's distribution covers the target's
-            r = __double2ull_rn(p * kUnits);
-            if (part == 0) values[c] = r;
-            total = block_sum(part == 0 ? r : 0ull, reinterpret_cast<unsigned long long*>(s.red));
+        const unsigned long long total = block_sum(part == 0 ? r : 0ull, reinterpret_cast<unsigned long long*>(s.red));
+        if (u_draw * (double)total >= kLeastUnits) {
+            unsigned long long upto = 0;
+            for (int j = part; j < n_all; j += parts)
+                if ((uint32_t)keys[j] >= (uint32_t)key) upto += values[j];   // its token, or a lower one
+            for (int o = 1; o < parts; o <<= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
+            if (r > 0 && part == 0) {
+                if ((double)upto > u_draw * (double)total) atomicMin(&s.pick, token);
+                atomicMax(&s.last, token);
+            }
+            __syncthreads();
+            return make_int2(0, s.pick < INT_MAX ? s.pick : s.last);
         }
-        unsigned long long upto = 0;
-        for (int j = part; j < n_all; j += parts)
-            if ((uint32_t)keys[j] >= (uint32_t)key) upto += values[j];   // its token, or a lower one
-        for (int o = 1; o < parts; o <<= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
-        if (r > 0 && part == 0) {
-            if ((double)upto > u_draw * (double)total) atomicMin(&s.pick, token);
-            atomicMax(&s.last, token);
-        }
-        __syncthreads();
-        return make_int2(0, s.pick < INT_MAX ? s.pick : s.last);
     }
-    // More: sorted, two candidates a thread from then on.
+    // More, or a draw that such units are too coarse for: sorted, two candidates a thread from then on.
     const double* shares;
     const int* tokens;
     int n_last;

@@ -63,3 +63,19 @@ def test_a_draw_of_zero_behind_a_long_mask(dops, kind, vocab):
     u = np.zeros((2, 2), np.float32)
     tokens, _, _ = verify(dops, logits, drafts, u, probs, 1.0, 0)
     assert (tokens[:, 0] == 5003).all()
+
+
+@pytest.mark.parametrize("mask", [-math.inf, -1e9, -100.0, -45.0])
+@pytest.mark.parametrize("kind", ["none", "looked up", "given", "covers"])
+@pytest.mark.parametrize("top_k", [50, 70, 128, 129, 1000])
+def test_draws_among_candidates_at_the_ends_of_the_unit_interval(dops, mask, kind, top_k):
+    """A top_k beyond the tokens that count takes masked ones in: where they have a weight in 64 bits, they have their share of the draw."""
+    logits, drafts, probs = masked_case(mask, kind, 5, F32, seed=41)
+    if mask > -1e6 and top_k != 129:   # no two alike
+        logits -= (logits == mask) * 5 * torch.rand(logits.shape, generator=torch.Generator().manual_seed(42))
+    for end in (0.0, 1e-30, 2.0 ** -24, 1.0 - 2.0 ** -24):
+        u = np.full((5, 2), 0.5, np.float32)
+        u[:, 1] = end
+        tokens, accepted, (t, k, p) = verify(dops, logits, drafts, u, probs, 0.9, top_k)
+        want, count, _ = verify_plain(logits.numpy(), drafts, u, t, k, p, probs)
+        assert np.array_equal(accepted, count) and np.array_equal(tokens, want), (end, tokens.tolist(), want.tolist())
