@@ -382,7 +382,7 @@ struct TopShared {
     int2 step;
 };
 
-// One row with a top_k, by a CTA: (draft kept, token drawn in its place).
+// One row with a top_k, by a CTA: (draft kept, token drawn in its place; -1 where the row is no distribution).
 template <typename T>
 __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem, int lane, int i, int d, int k, float temperature, float top_p, double u_keep, double u_draw) {
     constexpr int EPV = Row<T>::EPV;
@@ -420,10 +420,7 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
     for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
     if (wl == 0) s.warp_low[warp] = low;
     __syncthreads();
-    if (s.bad) {
-        if (tid == 0) tell(a.status, kDevBadRow);
-        return make_int2(0, -1);
-    }
+    if (s.bad) return make_int2(0, -1);   // told of where the lane gets here
     const uint64_t best = s.best;
     const float top = value_of_key(best);
 #pragma unroll
@@ -712,6 +709,7 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
                 end += __ffs(ends) - 1;
             }
         }
+        if (token < 0 && wl == 0) tell(a.status, kDevBadRow);
         put_lane(a, lane, end, token);
         return;
     }

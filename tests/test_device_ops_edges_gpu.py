@@ -79,3 +79,16 @@ def test_draws_among_candidates_at_the_ends_of_the_unit_interval(dops, mask, kin
         tokens, accepted, (t, k, p) = verify(dops, logits, drafts, u, probs, 0.9, top_k)
         want, count, _ = verify_plain(logits.numpy(), drafts, u, t, k, p, probs)
         assert np.array_equal(accepted, count) and np.array_equal(tokens, want), (end, tokens.tolist(), want.tolist())
+
+
+@pytest.mark.parametrize("temperature, top_k", [(1.0, 0), (1.0, 9), (1.0, 200), (0.0, 0)])
+def test_rows_that_a_lane_does_not_reach_are_not_told_of(dops, temperature, top_k):
+    logits, drafts, u, _ = verify_case(42, 4, 3, 700)
+    drafts[:] = logits[:, :3].argmax(-1).numpy()
+    u[:, :3] = 0.0
+    logits[1, 0, drafts[1, 0]] = -math.inf   # refused at once
+    logits[1, 2, 30], logits[1, 3] = math.nan, -math.inf
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _, accepted, _ = verify(dops, logits, drafts, u, None, temperature, top_k, status=status)
+    assert accepted.tolist() == [3, 0, 3, 3]
+    dops.check_status(status)
