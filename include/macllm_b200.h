@@ -687,8 +687,9 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
 
 /* Verification of drafted tokens.  logits [lanes][drafts + 1] rows of vocab values, at most 416000 (logits_stride apart): row i of a lane is the
  * target's answer behind its first i drafts.  Its distribution p_i is the sampler's (mk_k_sample): logits / temperature over the
- * top_k best tokens (lower token first among equals; top_k 0: all), of those the head that adds up to top_p (below 1 only with
- * top_k >= 1; top_k at most 1024); temperature 0 (or below 1e-30): the best token.  drafts [lanes][drafts], a negative one ends a lane's;
+ * top_k best tokens (lower token first among equals; top_k 0: all), of those the head that adds up to top_p; temperature 0 (or below
+ * 1e-30): the best token.  As for that sampler top_k is at most 1024 and top_p below 1 only with a top_k: a lane with another setting
+ * keeps nothing and ends with token -1 and MK_DEV_BAD_RANGE.  A draft beyond the vocabulary ends the lane's drafts with the same bit.  drafts [lanes][drafts], a negative one ends a lane's;
  * draft_probs [lanes][drafts][vocab] f32: the distributions q_i that they were drawn from, NULL: drafts without one (looked up), q_i = 1
  * on the draft.  u [lanes][drafts + 1] uniform in [0, 1).  Draft i is kept while u_i q_i(d_i) < p_i(d_i); the first that is not is
  * replaced by a token of max(p_i - q_i, 0), and behind the last one a token of p is added, both drawn by u_drafts: the first token, in

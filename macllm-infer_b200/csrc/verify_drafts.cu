@@ -678,9 +678,9 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
         more = none == 0;
         n = more ? n + 32 : n + __ffs(none) - 1;
     }
-    const bool hot = temperature > 0.f, whole = hot && k <= 0;
-    if (rank == 0 && tid == 0 && ((n < n_drafts && drafts[n] >= vocab) || (hot && (k > kVerifyMaxTopK || (k <= 0 && top_p < 1.f))))) tell(a.status, kDevBadRange);
-    if (rank != 0 && (!hot || (!whole && rank > n))) return;   // no row for this CTA: whom the cluster's barrier then does not wait for
+    const bool hot = temperature > 0.f, whole = hot && k <= 0, unknown = hot && (k > kVerifyMaxTopK || (whole && top_p < 1.f));
+    if (rank == 0 && tid == 0 && ((n < n_drafts && drafts[n] >= vocab) || unknown)) tell(a.status, kDevBadRange);
+    if (rank != 0 && (!hot || unknown || (!whole && rank > n))) return;   // no row for this CTA: whom the cluster's barrier then does not wait for
     if (tid == 0) {
         s_end = INT_MAX;
         s_pick = INT_MAX;
@@ -688,9 +688,13 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
     }
     __syncthreads();
     pdl_wait();
+    if (unknown) {   // no draw from a distribution that nobody asked for
+        if (warp == 0) put_lane(a, lane, 0, -1);
+        return;
+    }
     if (hot && !whole) {
         // ---- rows with a top_k, shared out over the CTAs
-        k = min(min(k, kVerifyMaxTopK), vocab);
+        k = min(k, vocab);
         int2* rows = a.rows + (int64_t)lane * (n_drafts + 1);
         for (int i = rank; i <= n; i += ctas) {
             const int2 r = finish_top_row<T>(a, top_shared, smem, lane, i, i < n ? drafts[i] : -1, k, temperature, top_p, (double)u[i], u_draw);

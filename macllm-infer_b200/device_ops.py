@@ -128,7 +128,8 @@ def verify_drafts(logits, drafts, u, *, temperature, top_k, top_p, draft_probs=N
 
     logits [lanes, drafts + 1, vocab] f32, f16 or bf16 (rows may be further apart); drafts [lanes, drafts], a negative one ends a lane's; u [lanes, drafts + 1] f32 in
     [0, 1); temperature, top_k, top_p [lanes] as of the sampler (temperature 0: greedy, top_k 0: the whole vocabulary); draft_probs [lanes, drafts, vocab] f32, or None for
-    drafts that were looked up.  Returns (tokens [lanes, drafts + 1]: kept drafts, the token behind them, -1 behind that; accepted [lanes])."""
+    drafts that were looked up.  As of the sampler too, top_k goes up to 1024 and top_p below 1 needs a top_k: a lane with another setting gets token -1, no drafts and
+    BAD_RANGE, and one that reaches a row that is no distribution token -1 and BAD_ROW.  Returns (tokens [lanes, drafts + 1]: kept drafts, the token behind them, -1 behind that; accepted [lanes])."""
     dtype, device, shape = logits.dtype, logits.get_device(), logits.shape
     if len(shape) != 3 or dtype not in _TYPES or shape[1] < 1 or shape[2] < 1:
         raise ValueError("logits is a float32, float16 or bfloat16 tensor [lanes, drafts + 1, vocabulary]")

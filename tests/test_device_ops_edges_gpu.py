@@ -92,3 +92,19 @@ def test_rows_that_a_lane_does_not_reach_are_not_told_of(dops, temperature, top_
     _, accepted, _ = verify(dops, logits, drafts, u, None, temperature, top_k, status=status)
     assert accepted.tolist() == [3, 0, 3, 3]
     dops.check_status(status)
+
+
+@pytest.mark.parametrize("top_k, top_p", [(0, 0.9), (-1, 0.5), (1025, 1.0), (5000, 0.9)])
+def test_a_setting_that_the_call_does_not_have_ends_its_lane(dops, top_k, top_p):
+    """No token is drawn from another distribution than the one asked for; greedy lanes have no use for either setting, and the other lanes get what they get alone."""
+    capi = importlib.import_module("macllm_infer_b200._capi")
+    logits, drafts, u, _ = verify_case(43, 6, 2, 3000)
+    t, k, p = [0.8, 0.8, 0.0, 0.8, 1.1, 0.0], np.array([20, top_k, top_k, 0, 5, 0]), np.array([0.9, top_p, top_p, 1.0, 1.0, 1.0])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    tokens, accepted, settings = verify(dops, logits, drafts, u, None, t, k, p, status=status)
+    with pytest.raises(capi.MkError, match="range"):
+        dops.check_status(status)
+    assert accepted[1] == 0 and tokens[1].tolist() == [-1, -1, -1]
+    rest = [0, 2, 3, 4, 5]
+    want, count, margin = verify_plain(logits[rest].numpy(), drafts[rest], u[rest], *(x[rest] for x in settings), None)
+    assert margin > 1e-7 and np.array_equal(tokens[rest], want) and np.array_equal(accepted[rest], count)
