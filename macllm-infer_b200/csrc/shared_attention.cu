@@ -496,7 +496,6 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = a.q_heads / a.kv_heads;
     const int split = blockIdx.x % splits, kvh = blockIdx.x / splits % a.kv_heads, block = blockIdx.x / splits / a.kv_heads, lane_id = OWN ? block / lane_tiles : 0,
               tile = OWN ? block - lane_id * lane_tiles : block;
-    pdl_trigger();
     const LaneRange mine_range = OWN ? lane_range(a, lane_id) : LaneRange{0, a.total, 0, 0};
     if (OWN && tile * (NQ * kItems) >= mine_range.n * g) {
         pdl_wait();
@@ -534,6 +533,8 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
         __syncwarp();
         tmem_alloc(&tmem_slot, L::TMEM);
+        // Not before: a kernel behind this one (the own-keys form) holds tensor memory while it waits for this grid's end, which must not wait for that memory.
+        pdl_trigger();
     }
     // The queries' pieces and the first tiles of keys and values are on their way before anything else is looked at (one after the other the queries took 0.6 us a piece, 10 us at
     // heads of 128).
