@@ -485,11 +485,11 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     using L = SharedSmem<D, NQ>;
     constexpr int ST = L::STAGES, KEYS = kKeys, S_AT = NQ * D, AREAS = 2 * NQ;   // columns of tensor memory: outputs, then the areas
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[4 * ST + 3 * AREAS + 1];
+    __shared__ uint64_t bars[4 * ST + 3 * AREAS + 1 + NQ];
     __shared__ uint32_t tmem_slot;
     __shared__ int4 sees[L::WARPS];
     uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST, *s_full = bars + 4 * ST, *p_full = s_full + AREAS, *o_done = p_full + AREAS,
-             *q_full = o_done + AREAS;
+             *q_full = o_done + AREAS, *drained = q_full + 1;
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ks = qs + NQ * L::PANELS * L::QPANEL;
     uint8_t* vs = ks + ST * L::BYTES;
@@ -529,6 +529,7 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 bar_init(&o_done[i], 1);
             }
             bar_init(q_full, L::WARPS);
+            for (int i = 0; i < NQ; ++i) bar_init(&drained[i], 1);
             bar_init_fence();
         }
         __syncwarp();
@@ -663,12 +664,10 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
             row = next;
         }
-        if (!ok) {
-            if (lane == 0) tell(a.status, kDevWait);
-            for (int u = max(0, t - ST); u <= t && u < n_tiles; ++u) {   // copies in flight land before the CTA ends
-                if (loads_k && (u < t || loads_v)) bar_wait(&k_full[u % ST], u / ST & 1);
-                if (loads_v && u < t) bar_wait(&v_full[u % ST], u / ST & 1);
-            }
+        if (!ok && lane == 0) tell(a.status, kDevWait);
+        for (int u = max(0, t - ST); u <= t && u < n_tiles; ++u) {   // copies in flight land before the CTA ends, also where the others gave up
+            if (loads_k && (u < t || loads_v)) bar_wait(&k_full[u % ST], u / ST & 1);
+            if (loads_v && u < t) bar_wait(&v_full[u % ST], u / ST & 1);
         }
     } else if (warp >= L::WARPS + L::LOADERS) {
         // ---- products, a warp per tile of items: the one's waits pass under the other's products.  The whole warp walks along, so that descriptors and addresses are the same for
@@ -716,7 +715,11 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 }
                 __syncwarp();
             }
-            if (!ok && lane == 0) tell(a.status, kDevWait);
+            if (!ok) {   // products under way end before their operands' memory is given back
+                if (lane == 0) tell(a.status, kDevWait);
+                if (issues) commit(&drained[q]);
+                wait(&drained[q], 0);
+            }
         }
     } else {
         // ---- softmax, an item per thread

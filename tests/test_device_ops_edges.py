@@ -16,3 +16,19 @@ def test_kernels_have_their_tensor_memory_before_the_next_may_start():
             seen.add(name)
             assert takes[-1] < body.index("pdl_trigger()"), (file, name)
     assert {"shared_keys_kernel", "attn_umma_kernel", "hgemm_tc_kernel", "latent_umma_kernel"} <= seen
+
+
+def test_a_loader_outlasts_its_last_copies():
+    """Behind its loop the loader of shared_keys_kernel waits for the copies of the last tiles that it asked for, stage u % ST in parity u / ST & 1.  A wait in a parity is over when the
+    barrier's present phase has the other one, and a tile is asked for only when the stage's copy before has landed: so no wait is over ahead of its copy, and none lasts beyond it."""
+    body = next(b for _, name, _, b in kernels() if name == "shared_keys_kernel")
+    loader = body[body.index("bar_wait(&v_empty[st], ph)"):body.index("f16_idesc(kItems, KEYS, false)")]
+    assert re.search(r"for \(int u = max\(0, t - ST\); u <= t && u < n_tiles; \+\+u\)", loader) and loader.count("bar_wait(&k_full[u % ST], u / ST & 1)") == 1
+    assert not re.search(r"if \(!ok\)\s*\{", loader)   # also where only the others gave up
+    for stages in range(2, 7):
+        for asked in range(1, 20):
+            for under_way in range(0, min(stages, asked) + 1):   # of the last copies
+                landed = [sum(1 for u in range(asked - under_way) if u % stages == st) for st in range(stages)]
+                for u in range(max(0, asked - stages), asked):
+                    over = (landed[u % stages] & 1) != (u // stages & 1)
+                    assert over == (u < asked - under_way)
