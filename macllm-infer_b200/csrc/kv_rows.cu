@@ -19,8 +19,9 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
     const int64_t page_pieces = (int64_t)a.kv_heads * a.block_tokens * row_pieces;
     const int32_t* c = a.copies + (int64_t)blockIdx.x * 3;
     const int from = c[0], to = c[1], rows = c[2];
-    if (from < 0 || from >= a.pages || to < 0 || to >= a.pages || rows < 0 || rows > a.block_tokens) {
-        if (threadIdx.x == 0) tell(a.status, kDevBadPage);
+    const int wrong = (from < 0 || from >= a.pages || to < 0 || to >= a.pages ? kDevBadPage : 0) | (rows < 0 || rows > a.block_tokens ? kDevBadRange : 0);
+    if (wrong != 0) {
+        if (threadIdx.x == 0) tell(a.status, wrong);
         return;
     }
     if (from == to) return;

@@ -108,3 +108,15 @@ def test_a_setting_that_the_call_does_not_have_ends_its_lane(dops, top_k, top_p)
     rest = [0, 2, 3, 4, 5]
     want, count, margin = verify_plain(logits[rest].numpy(), drafts[rest], u[rest], *(x[rest] for x in settings), None)
     assert margin > 1e-7 and np.array_equal(tokens[rest], want) and np.array_equal(accepted[rest], count)
+
+
+@pytest.mark.parametrize("rows", [17, -1])
+def test_a_number_of_rows_that_a_page_has_not_is_out_of_range(dops, rows):
+    capi = importlib.import_module("macllm_infer_b200._capi")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v = pools(2, 10, 2, 16, 64, F16)
+    before = k.clone()
+    dops.copy_pages(k, v, torch.tensor([[2, 3, rows]], dtype=torch.int32, device="cuda"), status=status)
+    assert torch.equal(k, before) and int(status) == dops.BAD_RANGE
+    with pytest.raises(capi.MkError, match="length, count"):
+        dops.check_status(status)
