@@ -34,9 +34,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)).
+// cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)), which rounds in parts of the cap: 2^-14 and less up to kCapOfDifference.
+constexpr float kCapOfDifference = 256.f;
 __device__ __forceinline__ float capped(float v, float cap, float two_over_cap) {
     return cap - __fdividef(2.0f * cap, 1.0f + __expf(fminf(v * two_over_cap, 80.0f)));
+}
+// For caps above, by kernels of their own (beside the other in one kernel it cost calls without any cap 1.5 %): with x = v / cap below 1/4 as v (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315), whose next term is 3.4e-7 of v; from there on the roundings above are less than 2^-20 of v.
+__device__ __forceinline__ float capped_wide(float v, float cap, float two_over_cap) {
+    const float x = 0.5f * v * two_over_cap, y = x * x;
+    return y < 0.0625f ? v * fmaf(y, fmaf(y, fmaf(y, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f) : capped(v, cap, two_over_cap);
 }
 
 template <typename T>
@@ -191,7 +197,7 @@ struct LaneSmem {
     static size_t bytes(int stages) { return 1024 + (size_t)WARPS * ring(stages) + (size_t)NT * 8 * QP * 2; }
 };
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool WIDE>
 __global__ void __launch_bounds__(LaneSmem<D, NT>::THREADS) lane_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a,
                                                                                    int chunk, int shares, int shared_parts, int join, int stage_bits) {
     using L = LaneSmem<D, NT>;
@@ -324,7 +330,8 @@ __global__ void __launch_bounds__(LaneSmem<D, NT>::THREADS) lane_keys_kernel(con
             for (int e = 0; e < 4; ++e) {
                 const int pos = pos0 + gid + 8 * (e >> 1);
                 float v = sc[n][e] * unit;
-                if (a.softcap != 0.f) v = capped(v, a.softcap, two_over_cap) * kLog2e;
+                if (WIDE) v = capped_wide(v, a.softcap, two_over_cap) * kLog2e;
+                else if (a.softcap != 0.f) v = capped(v, a.softcap, two_over_cap) * kLog2e;
                 sc[n][e] = whole || (pos >= see_lo[n][e & 1] && pos < see_hi[n][e & 1]) ? v : -INFINITY;
             }
             float alpha[2], m_use[2];
@@ -478,7 +485,7 @@ struct SharedSmem {
 };
 
 // OWN: the same for one lane's rows and its own keys, where a lane has so many (row, head) items that the small products of lane_keys_kernel would be made over and over.
-template <typename T, int D, int NQ, bool OWN>
+template <typename T, int D, int NQ, bool OWN, bool WIDE>
 __global__ void __launch_bounds__(SharedSmem<D, NQ>::THREADS, SharedSmem<D, NQ>::CTAS)
 shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedAttnArgs a, int box, int splits, int chunk,
                    int lane_tiles, int first_part) {
@@ -745,7 +752,10 @@ shared_keys_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s) + 32);
             tmem_wait_ld();
             const int pos0 = base_key + (t_begin + t) * KEYS;
-            if (a.softcap != 0.f) {
+            if (WIDE) {
+#pragma unroll
+                for (int j = 0; j < KEYS; ++j) s[j] = capped_wide(s[j] * a.scale, a.softcap, two_over_cap);
+            } else if (a.softcap != 0.f) {
 #pragma unroll
                 for (int j = 0; j < KEYS; ++j) s[j] = capped(s[j] * a.scale, a.softcap, two_over_cap);
             }
@@ -871,7 +881,7 @@ void launch_tall(const SharedAttnArgs& a, const SharedAttnPlan& p, Maps& maps, c
     using L = SharedSmem<D, NQ>;
     const int box = std::min(a.block_tokens, kKeys);
     maps.need(a, box);
-    auto* kernel = shared_keys_kernel<T, D, NQ, OWN>;
+    auto* kernel = a.softcap > kCapOfDifference ? shared_keys_kernel<T, D, NQ, OWN, true> : shared_keys_kernel<T, D, NQ, OWN, false>;
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::SMEM);
     if (!OWN) {
         kernel<<<(unsigned)(p.row_tiles * a.kv_heads * p.shared_parts), L::THREADS, L::SMEM, s>>>(maps.k, maps.v, a, box, p.shared_parts, 0, 0, 0);
@@ -888,7 +898,7 @@ template <typename T, int D, int NT>
 void launch_lanes(const SharedAttnArgs& a, const SharedAttnPlan& p, Maps& maps, cudaStream_t s) {
     maps.need(a, kTile);
     using L = LaneSmem<D, NT>;
-    auto* kernel = lane_keys_kernel<T, D, NT>;
+    auto* kernel = a.softcap > kCapOfDifference ? lane_keys_kernel<T, D, NT, true> : lane_keys_kernel<T, D, NT, false>;
     // Half the ring (32 KB) where there are more than two CTAs for each SM: more of them run at once, also beside a CTA of the shared keys, and what one waits for another uses (128
     // lanes of 8 heads with 1 to 60 keys 24.1 us and 20.3; 117 of 4 with one 16.6 and 12.7).  Fewer CTAs need more of their own on its way (32 lanes of 8 heads with 17 to 500 keys
     // 14.7 us with the whole ring, 15.9 with half; 8 with 3000 23.0 and 26.8).

@@ -120,3 +120,12 @@ def test_a_number_of_rows_that_a_page_has_not_is_out_of_range(dops, rows):
     assert torch.equal(k, before) and int(status) == dops.BAD_RANGE
     with pytest.raises(capi.MkError, match="length, count"):
         dops.check_status(status)
+
+
+@pytest.mark.parametrize("cap", [3e4, 1e9, 3e38])
+@pytest.mark.parametrize("dim, shared, rows", [(128, 160, 1), (64, 1600, 2), (256, 1600, 2), (128, 1600, 2), (128, 1600, 40)])
+def test_caps_far_above_the_scores(dops, cap, dim, shared, rows):
+    """cap tanh(x / cap) = x - x^3 / (3 cap^2) + ..: scores stay below 60 here, so a cap of 3e4 moves them by less than 60^3 / (3 * 9e8) = 8e-5, which is less than what the bound below
+    has for a score's 32-bit sums: (dim + 8) 2^-24 of the largest sum of |scale q k|, above 20 here, is 8e-5 at heads of 64 and more at wider ones."""
+    b = Batch(F16, 8, 2, dim, 16, shared, [rows, 40 + rows, 300], rows, seed=45, spread=4.0)
+    b.check(b.run(dops, softcap=cap))
