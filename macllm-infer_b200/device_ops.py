@@ -167,6 +167,8 @@ def _pools(k_pool, v_pool):
 def copy_pages(k_pool, v_pool, copies, *, status=None) -> None:
     """Copies the first ``rows`` tokens of pages to other pages, in every layer: copies [n, 3] of (from page, to page, rows).  No page is written twice, or
     written by one copy and read by another."""
+    if copies.dim() != 2:
+        raise ValueError("copies is [n, 3]")
     device, n = k_pool.get_device(), copies.shape[0]
     _run(device, capi.lib().mk_k_copy_pages_dev, *_pools(k_pool, v_pool), _dense(copies, _I32, (n, 3), device, "copies"), n,
          None if status is None else _dense(status, _I32, (1,), device, "status"))

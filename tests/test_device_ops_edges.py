@@ -1,7 +1,17 @@
 """Operators over device buffers at the edges of what their calls allow, without a device."""
+import importlib
 import re
 
+import pytest
+
 from test_dependent_launches import kernels
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def dops(mk):
+    return importlib.import_module("macllm_infer_b200.device_ops")
 
 # more than 860 threads and 180 KB of shared memory: no CTA that wants tensor memory fits beside one of these
 ALONE_ON_AN_SM = {"qstream_tc_kernel"}
@@ -32,3 +42,10 @@ def test_a_loader_outlasts_its_last_copies():
                 for u in range(max(0, asked - stages), asked):
                     over = (landed[u % stages] & 1) != (u // stages & 1)
                     assert over == (u < asked - under_way)
+
+
+def test_copies_of_any_shape_but_a_table_are_refused(dops):
+    pool = torch.zeros(2, 10, 2, 16, 64)
+    for copies in (torch.tensor(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 3, 1, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="copies"):
+            dops.copy_pages(pool, pool, copies)
