@@ -4,7 +4,7 @@ Unlike the wrappers of ``ops``, which move host arrays to the device and back, t
 the current stream of the tensors' device and return without waiting; they may be captured into a CUDA graph (sizes, pointers, Python
 numbers and strides are fixed then, contents are not).  Index tensors are int32.  ``status`` is an optional int32 tensor of one element into
 which the kernels OR what they met (``BAD_PAGE``, ``WAIT_GAVE_UP``, ``BAD_RANGE``, ``BAD_ROW``); ``check_status`` reads it.  Arguments that can be judged by shape, type and
-stride are refused with ValueError before anything is launched.
+stride are refused with ValueError before anything is launched, what the entry points themselves refuse (a head size, a length, an alignment, rows that overlap) with MkError, also before.
 """
 from __future__ import annotations
 
@@ -84,15 +84,15 @@ def shared_attention(q, k_pool, v_pool, tables, lengths, shared_len: int, *, sca
     they are long); tables [lanes, width] page numbers; lengths [lanes] tokens of each lane, its rows of q being the last of them.  Without cu_seqlens
     [lanes + 1] every lane has total / lanes rows; with it, ``max_rows`` is the most that a lane has.  Returns [total, q_heads, head_dim]; rows outside
     cu_seqlens are left as ``out`` had them."""
-    dtype, device, shape, pool, strides = q.dtype, q.get_device(), q.shape, k_pool.shape, k_pool.stride()
+    dtype, device, shape, pool, strides, v_strides = q.dtype, q.get_device(), q.shape, k_pool.shape, k_pool.stride(), v_pool.stride()
     if len(shape) != 3 or (dtype is not torch.float16 and dtype is not torch.bfloat16):
         raise ValueError("q is a float16 or bfloat16 tensor [rows, heads, head size]")
     total, heads, dim = shape
-    if (len(pool) != 4 or pool[3] != dim or v_pool.shape != pool or v_pool.stride() != strides or k_pool.dtype is not dtype or v_pool.dtype is not dtype
+    if (len(pool) != 4 or pool[3] != dim or v_pool.shape != pool or (v_strides != strides and any(x != y and n != 1 for n, x, y in zip(pool, strides, v_strides))) or k_pool.dtype is not dtype or v_pool.dtype is not dtype
             or k_pool.get_device() != device or v_pool.get_device() != device):
         raise ValueError("k_pool and v_pool are [pages, kv heads, tokens of a page, head size] of q's type and head size, strided alike, on its device")
     pages, kv_heads, page, _ = pool
-    if strides[1:] != (page * dim, dim, 1):
+    if strides[1:] != (page * dim, dim, 1) and (kv_heads != 1 or strides[2:] != (dim, 1)):
         raise ValueError("pages are dense")
     lanes = tables.shape[0] if tables.dim() == 2 else -1
     table, table_stride, width = _rows(tables, lanes, device, "tables")
@@ -105,13 +105,14 @@ def shared_attention(q, k_pool, v_pool, tables, lengths, shared_len: int, *, sca
         if max_rows <= 0 and total:
             raise ValueError("with cu_seqlens, max_rows says how many rows a lane has at most")
     q_strides = q.stride()
-    if total and q_strides[1:] != (dim, 1):
+    if total and q_strides[1:] != (dim, 1) and (heads != 1 or q_strides[2] != 1):
         raise ValueError("the heads of a row are dense")
     if out is None:
         out, out_stride = torch.empty_like(q), heads * dim   # dense, since the heads of a row are
     else:
         out_strides = out.stride()
-        if out.shape != shape or out.dtype is not dtype or out.get_device() != device or (total and out_strides[1:] != (dim, 1)):
+        if (out.shape != shape or out.dtype is not dtype or out.get_device() != device
+                or (total and out_strides[1:] != (dim, 1) and (heads != 1 or out_strides[2] != 1))):
             raise ValueError("out is like q, the heads of a row dense")
         out_stride = out_strides[0] if total > 1 else heads * dim
     need = _attention_workspace(heads, kv_heads, dim, page, width, lanes, rows, total, shared_len, window)

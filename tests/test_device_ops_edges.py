@@ -49,3 +49,18 @@ def test_copies_of_any_shape_but_a_table_are_refused(dops):
     for copies in (torch.tensor(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 3, 1, dtype=torch.int32)):
         with pytest.raises(ValueError, match="copies"):
             dops.copy_pages(pool, pool, copies)
+
+
+def test_strides_of_one_head_or_one_page_do_not_matter(dops):
+    """Dense tensors whose dimensions of one element have any stride pass every check but that for a device."""
+    q, pool = torch.zeros(4, 1, 64, dtype=torch.float16), torch.zeros(10, 1, 16, 64, dtype=torch.float16)
+    tables, lengths = torch.zeros(4, 4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    odd_q, odd_pool = q.as_strided((4, 1, 64), (64, 7, 1)), pool.as_strided((10, 1, 16, 64), (1024, 5, 64, 1))
+    one_page = [pool[:1], pool.as_strided((1, 1, 16, 64), (3, 5, 64, 1))]
+    for args, out in (((odd_q, pool, pool), None), ((q, odd_pool, odd_pool), None), ((q, pool, odd_pool), None), ((q, *one_page), None), ((q, pool, pool), odd_q)):
+        with pytest.raises(ValueError, match="CUDA device"):
+            dops.shared_attention(*args, tables, lengths, 0, scale=1.0, out=out)
+    for args, message in (((q, pool, pool.as_strided((5, 1, 16, 64), (2048, 1024, 64, 1))), "strided alike"), ((q, pool[:5], pool.as_strided((5, 1, 16, 64), (2048, 1024, 64, 1))), "strided alike"),
+                          ((q.as_strided((2, 1, 64), (64, 64, 2)), pool, pool), "dense"), ((torch.zeros(4, 2, 64, dtype=torch.float16).as_strided((4, 2, 64), (64, 7, 1)), pool, pool), "dense")):
+        with pytest.raises(ValueError, match=message):
+            dops.shared_attention(*args, tables[:args[0].shape[0]], lengths[:args[0].shape[0]], 0, scale=1.0)

@@ -129,3 +129,18 @@ def test_caps_far_above_the_scores(dops, cap, dim, shared, rows):
     has for a score's 32-bit sums: (dim + 8) 2^-24 of the largest sum of |scale q k|, above 20 here, is 8e-5 at heads of 64 and more at wider ones."""
     b = Batch(F16, 8, 2, dim, 16, shared, [rows, 40 + rows, 300], rows, seed=45, spread=4.0)
     b.check(b.run(dops, softcap=cap))
+
+
+@pytest.mark.parametrize("shared, rows", [(160, 1), (1600, 2), (1600, 140)])
+def test_one_head_with_any_stride(dops, shared, rows):
+    """A dimension of one element has any stride: queries, pools and results say so, and what is written is where the rows are."""
+    b = Batch(F16, 1, 1, 128, 16, shared, [rows, 40 + rows, 300], rows, seed=46, q_gap=128)
+    n, pages = b.q.shape[0], b.pools[0].shape[0]
+    b.q = b.q.as_strided((n, 1, 128), (256, 9, 1))
+    b.pools = [b.pools[0], b.pools[1].as_strided((pages, 1, 16, 128), (2048, 3, 128, 1), b.pools[1].storage_offset())]
+    b.check(b.run(dops))
+    wide = torch.full((n, 384), 7.0, dtype=F16, device="cuda")
+    out = wide.as_strided((n, 1, 128), (384, 5, 1))
+    b.run(dops, out=out)
+    b.check(out)
+    assert (wide[:, 128:] == 7).all()
