@@ -17,6 +17,9 @@ void need(bool ok, const char* what) {
     if (!ok) throw std::runtime_error(what);
 }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+// Arrays of 32-bit numbers, and the status word; null ones are aligned.
+template <typename... P>
+bool words(const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) == 0; }
 
 SharedAttnPlan checked_plan(int q_heads, int kv_heads, int d, int block_tokens, int width, int lanes, int rows, int total, int shared, int window) {
     need(window >= 0, "mk_k_shared_attention: window is not negative");
@@ -49,7 +52,10 @@ extern "C" {
 
 int32_t mk_k_shared_attention_workspace(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_tokens, int32_t table_width, int32_t lanes, int32_t rows,
                                         int32_t total, int32_t shared_len, int32_t window, int64_t* bytes) {
-    return guarded([&] { *bytes = checked_plan(q_heads, kv_heads, head_dim, block_tokens, table_width, lanes, rows, total, shared_len, window).bytes(total, q_heads, head_dim); });
+    return guarded([&] {
+        need(bytes != nullptr, "mk_k_shared_attention_workspace: null pointer");
+        *bytes = checked_plan(q_heads, kv_heads, head_dim, block_tokens, table_width, lanes, rows, total, shared_len, window).bytes(total, q_heads, head_dim);
+    });
 }
 
 int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_stride, const void* k_pool_dev, const void* v_pool_dev, int64_t pool_pages, int64_t page_stride,
@@ -66,6 +72,7 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
         need(cu_seqlens_dev != nullptr || (int64_t)lanes * rows == total, "mk_k_shared_attention_dev: without cu_seqlens every lane has the same number of rows");
         need(aligned(q_dev, 16) && aligned(k_pool_dev, 16) && aligned(v_pool_dev, 16) && aligned(out_dev, 16) && q_stride % 8 == 0 && out_stride % 8 == 0,
              "mk_k_shared_attention_dev: rows and pools begin at multiples of 16 bytes");
+        need(words(tables_dev, lengths_dev, cu_seqlens_dev, status_dev), "mk_k_shared_attention_dev: tables, lengths, rows and status are words aligned to 4 bytes");
         need(q_stride >= (int64_t)q_heads * head_dim && out_stride >= (int64_t)q_heads * head_dim && table_stride >= table_width, "mk_k_shared_attention_dev: rows overlap");
         need(pool_pages > 0 && page_stride % head_dim == 0 && page_stride >= (int64_t)kv_heads * block_tokens * head_dim, "mk_k_shared_attention_dev: pages overlap, or do not begin at a row");
         need(pool_pages <= INT32_MAX && page_stride / head_dim <= INT32_MAX && pool_pages * (page_stride / head_dim) <= INT32_MAX,
@@ -88,7 +95,10 @@ int32_t mk_k_shared_attention_dev(int32_t type, const void* q_dev, int64_t q_str
 }
 
 int32_t mk_k_verify_drafts_workspace(int32_t type, int32_t lanes, int32_t drafts, int32_t vocab, int64_t* bytes) {
-    return guarded([&] { *bytes = checked_verify_plan(type, lanes, drafts, vocab).bytes; });
+    return guarded([&] {
+        need(bytes != nullptr, "mk_k_verify_drafts_workspace: null pointer");
+        *bytes = checked_verify_plan(type, lanes, drafts, vocab).bytes;
+    });
 }
 
 int32_t mk_k_verify_drafts_dev(int32_t type, const void* logits_dev, int64_t logits_stride, int32_t lanes, int32_t drafts, int32_t vocab, const int32_t* drafts_dev,
@@ -102,6 +112,7 @@ int32_t mk_k_verify_drafts_dev(int32_t type, const void* logits_dev, int64_t log
         need(logits_dev != nullptr && (drafts_dev != nullptr || drafts == 0) && u_dev != nullptr && temperature_dev != nullptr && top_k_dev != nullptr && top_p_dev != nullptr &&
                  tokens_dev != nullptr && accepted_dev != nullptr,
              "mk_k_verify_drafts_dev: null pointer");
+        need(words(drafts_dev, draft_probs_dev, u_dev, temperature_dev, top_k_dev, top_p_dev, tokens_dev, accepted_dev, status_dev), "mk_k_verify_drafts_dev: arrays are not aligned to 4 bytes");
         need(workspace_dev != nullptr && workspace_bytes >= p.bytes && aligned(workspace_dev, 16),
              "mk_k_verify_drafts_dev: the workspace is missing, too small or not aligned to 16 bytes");
         require_device();
@@ -123,6 +134,7 @@ int32_t mk_k_copy_pages_dev(void* k_pool_dev, void* v_pool_dev, int64_t layers, 
         if (n == 0 || layers == 0) return;
         need(k_pool_dev != nullptr && v_pool_dev != nullptr && copies_dev != nullptr, "mk_k_copy_pages_dev: null pointer");
         need(aligned(k_pool_dev, 2) && aligned(v_pool_dev, 2), "mk_k_copy_pages_dev: pools begin at even addresses");
+        need(words(copies_dev, status_dev), "mk_k_copy_pages_dev: arrays are not aligned to 4 bytes");
         require_device();
         KvRowsArgs a;
         a.k_pool = k_pool_dev; a.v_pool = v_pool_dev; a.layers = layers; a.pages = pages; a.kv_heads = kv_heads; a.block_tokens = block_tokens; a.row_bytes = row_bytes;
@@ -145,6 +157,7 @@ int32_t mk_k_gather_tokens_dev(void* k_pool_dev, void* v_pool_dev, int64_t layer
         need(k_pool_dev != nullptr && v_pool_dev != nullptr && from_tables_dev != nullptr && to_tables_dev != nullptr && keep_dev != nullptr && counts_dev != nullptr && first_dev != nullptr,
              "mk_k_gather_tokens_dev: null pointer");
         need(aligned(k_pool_dev, 2) && aligned(v_pool_dev, 2), "mk_k_gather_tokens_dev: pools begin at even addresses");
+        need(words(from_tables_dev, keep_dev, counts_dev, to_tables_dev, first_dev, status_dev), "mk_k_gather_tokens_dev: arrays are not aligned to 4 bytes");
         require_device();
         KvRowsArgs a;
         a.k_pool = k_pool_dev; a.v_pool = v_pool_dev; a.layers = layers; a.pages = pages; a.kv_heads = kv_heads; a.block_tokens = block_tokens; a.row_bytes = row_bytes;

@@ -5,6 +5,7 @@ import re
 import pytest
 
 from test_dependent_launches import kernels
+from test_device_ops import ATTENTION, COPY, GATHER, VERIFY, A, capi  # noqa: F401 (capi is a fixture)
 
 torch = pytest.importorskip("torch")
 
@@ -64,3 +65,19 @@ def test_strides_of_one_head_or_one_page_do_not_matter(dops):
                           ((q.as_strided((2, 1, 64), (64, 64, 2)), pool, pool), "dense"), ((torch.zeros(4, 2, 64, dtype=torch.float16).as_strided((4, 2, 64), (64, 7, 1)), pool, pool), "dense")):
         with pytest.raises(ValueError, match=message):
             dops.shared_attention(*args, tables[:args[0].shape[0]], lengths[:args[0].shape[0]], 0, scale=1.0)
+
+
+def test_arrays_that_are_no_words_and_sizes_without_a_place_are_refused(capi):  # noqa: F811
+    lib = capi.lib()
+    for call, good, names, message in ((lib.mk_k_shared_attention_dev, ATTENTION, ("tables", "lengths", "cu", "status"), "aligned to 4"),
+                                       (lib.mk_k_verify_drafts_dev, VERIFY, ("drafts_", "probs", "u", "temperature", "top_k", "top_p", "tokens", "accepted", "status"), "aligned to 4"),
+                                       (lib.mk_k_copy_pages_dev, COPY, ("copies", "status"), "aligned to 4"),
+                                       (lib.mk_k_gather_tokens_dev, GATHER, ("frm", "keep", "counts", "to", "first", "status"), "aligned to 4")):
+        for name in names:
+            assert name in good
+            with pytest.raises(capi.MkError, match=message):
+                capi.check(call(*{**good, name: A + 2}.values()))
+    with pytest.raises(capi.MkError, match="null pointer"):
+        capi.check(lib.mk_k_shared_attention_workspace(8, 2, 128, 16, 100, 3, 1, 3, 32, 0, None))
+    with pytest.raises(capi.MkError, match="null pointer"):
+        capi.check(lib.mk_k_verify_drafts_workspace(0, 3, 4, 1000, None))
