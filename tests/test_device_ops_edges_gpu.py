@@ -1,5 +1,6 @@
 """Operators over device buffers at the edges of what their calls allow: draws at the ends of the unit interval, settings and rows that end a lane, large caps, and the
 forms of the attention that few sizes reach."""
+import ctypes
 import importlib
 import math
 
@@ -144,3 +145,133 @@ def test_one_head_with_any_stride(dops, shared, rows):
     b.run(dops, out=out)
     b.check(out)
     assert (wide[:, 128:] == 7).all()
+
+
+# ---- forms of the attention -----------------------------------------------------------------------------------------------------
+#
+# With few keys altogether every lane reads the shared ones itself, in one launch without parts; else the shared keys' kernel is there, and a lane's own go through the small
+# products (up to 24 items; joined by the lane's CTA or by a kernel of its own) or the tall ones.  Which of them a call takes shows in its workspace, so that the sizes below stay what
+# they are for.
+FORMS = {
+    "one launch": dict(heads=(8, 2, 128), shared=160, own=[40, 3], rows=1),
+    "joined by lanes": dict(heads=(8, 2, 128), shared=1024, own=[40, 3], rows=2),
+    "two groups, joined": dict(heads=(8, 2, 128), shared=1024, own=[40, 13], rows=4),
+    "three groups, joined": dict(heads=(8, 2, 64), shared=1024, own=[40, 13], rows=6),
+    "two groups, wide heads": dict(heads=(8, 2, 256), shared=1024, own=[40, 13], rows=4),
+    "shares of own keys": dict(heads=(8, 2, 128), shared=1024, own=[1900, 13], rows=1),
+    "tall, 128 items": dict(heads=(8, 2, 128), shared=1024, own=[400, 23], rows=10),
+    "tall, 256 items": dict(heads=(8, 2, 64), shared=1024, own=[900, 83], rows=40),
+    "tall, wide heads": dict(heads=(8, 2, 256), shared=1024, own=[700, 43], rows=20),
+    "tall alone": dict(heads=(8, 2, 128), shared=0, own=[1500, 43], rows=20),
+}
+
+
+def form(name, dtype=F16, seed=50, **more):
+    """A batch of that form; its workspace says that it is one."""
+    f = FORMS[name]
+    capi = importlib.import_module("macllm_infer_b200._capi")
+    heads, kv_heads, dim = f["heads"]
+    b = Batch(dtype, heads, kv_heads, dim, 16, f["shared"], f["own"], f["rows"], seed=seed, **more)
+    lanes, rows, width = len(f["own"]), f["rows"], b.tables.shape[1]
+
+    def parts(width, shared):
+        need = ctypes.c_int64()
+        capi.check(capi.lib().mk_k_shared_attention_workspace(heads, kv_heads, dim, 16, width, lanes, rows, lanes * rows, shared, 0, ctypes.byref(need)))
+        return need.value // (lanes * rows * heads * (dim * 4 + 8))
+
+    own = parts(width - f["shared"] // 16, 0)
+    assert (own > 0) == (name.startswith("tall") or name == "shares of own keys")
+    assert (parts(width, f["shared"]) > own) == (name not in ("one launch", "tall alone"))
+    return b
+
+
+@pytest.mark.parametrize("name", FORMS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("window, softcap", [(0, 0.0), (1, 0.0), (5, 20.0), (64, 0.0), (300, 300.0), (1000, 0.0), (1200, 200.0), (5000, 0.0)])
+def test_windows_and_caps_in_every_form(dops, name, dtype, window, softcap):
+    b = form(name, dtype, spread=2.0)
+    b.check(b.run(dops, window=window, softcap=softcap), window, softcap)
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_lanes_of_different_rows_in_every_form(dops, name):
+    """Rows that no lane has, lanes without rows and ones that are shorter than the shared part or than their rows."""
+    f = FORMS[name]
+    heads, kv_heads, dim = f["heads"]
+    rows = [f["rows"], 0, 1, max(1, f["rows"] - 1), f["rows"]]
+    own = [f["own"][0], 7, -f["shared"] // 2, f["own"][1], -f["shared"] + f["rows"] // 2]
+    b = Batch(BF16, heads, kv_heads, dim, 16, f["shared"], own, rows, seed=51)
+    q = torch.cat([b.q, b.q[:3]])
+    for window in (0, 40):
+        out = torch.full_like(q, 5.0)
+        dops.shared_attention(q, *b.pools, b.tables, b.lengths, b.shared, scale=b.scale, cu_seqlens=b.cu, max_rows=f["rows"], out=out, window=window)
+        b.check(out[:-3], window)
+        assert (out[-3:] == 5).all()
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_strides_in_every_form(dops, name):
+    b = form(name, seed=52, page_gap=256 * 24, q_gap=64)
+    n, heads, dim = b.q.shape
+    wide = torch.full((n + 2, heads * dim + 24), 7.0, dtype=F16, device="cuda")
+    out = wide[1:n + 1, :heads * dim].view(n, heads, dim)
+    assert b.run(dops, out=out) is out
+    b.check(out)
+    assert (wide[0] == 7).all() and (wide[n + 1] == 7).all() and (wide[:, heads * dim:] == 7).all()
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_bad_pages_lengths_and_rows_are_told_in_every_form(dops, name):
+    """Whatever the index arrays hold is told of and read nowhere; the call after that is as if nothing had been."""
+    capi = importlib.import_module("macllm_infer_b200._capi")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    b = form(name, seed=53)
+    first = b.run(dops, status=status)
+    b.check(first)
+    dops.check_status(status)
+    tables, lengths, rows = b.tables.clone(), b.lengths.clone(), FORMS[name]["rows"]
+    places = [(0, b.shared // 16, -1), (1, b.shared // 16, 1 << 30), (1, int(lengths[1] - 1) // 16, -(1 << 31))]
+    for lane, column, value in places + ([(0, 0, -5), (0, b.shared // 16 - 1, 10 ** 6)] if b.shared else []):
+        b.tables[lane, column] = value
+        b.run(dops, status=status)
+        with pytest.raises(capi.MkError, match="page number"):
+            dops.check_status(status)
+        b.tables.copy_(tables)
+    for length in (-3, -(1 << 31), b.tables.shape[1] * 16 + 1, 2 ** 31 - 1):
+        b.lengths[1] = length
+        b.run(dops, status=status)
+        with pytest.raises(capi.MkError, match="length"):
+            dops.check_status(status)
+        b.lengths.copy_(lengths)
+    n = 2 * rows
+    for cu in ([0, n + 1, n], [-1, rows, n], [0, rows, n + 3], [n + 1, n + 2, n + 3], [0, 0, 2 ** 31 - 1], [0, -(1 << 31), n], [rows, rows + 1, 0]):
+        dops.shared_attention(b.q, *b.pools, b.tables, b.lengths, b.shared, scale=b.scale, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), max_rows=rows, status=status)
+        with pytest.raises(capi.MkError, match="range"):
+            dops.check_status(status)
+    assert torch.equal(b.run(dops, status=status), first)
+    dops.check_status(status)
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_every_form_in_two_graphs_and_on_two_streams(dops, name):
+    """Replayed beside one another on streams of their own, and again: workspaces are each call's, and nothing is kept."""
+    batches = [form(name, seed=54 + i) for i in range(2)]
+    want = [b.run(dops) for b in batches]
+    for b, x in zip(batches, want):
+        b.check(x)
+    streams, graphs, outs = [torch.cuda.Stream() for _ in batches], [], []
+    torch.cuda.synchronize()
+    for b, s in zip(batches, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            outs.append(b.run(dops))
+        graphs.append(graph)
+    for _ in range(3):
+        for x in outs:
+            x.fill_(3.0)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
