@@ -275,3 +275,28 @@ def test_every_form_in_two_graphs_and_on_two_streams(dops, name):
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+# ---- large vocabularies ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("vocab", [256000, 416000])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("top_k", [0, 64, 1024])
+def test_the_largest_vocabularies_from_odd_addresses(dops, vocab, dtype, top_k):
+    """The most runs and the most shared memory that the kernels are cut for; rows begin off 16 bytes."""
+    logits, drafts, u, _ = verify_case(47, 1, 2, vocab, dtype)
+    want, count, margin = verify_plain(logits.float().numpy(), drafts, u, np.full(1, 0.9, np.float32), np.full(1, top_k, np.int32), np.ones(1, np.float32), None)
+    assert margin > 1e-7
+    wide = torch.full((1, 3, vocab + 13), math.nan, dtype=dtype, device="cuda")
+    wide[:, :, 5:vocab + 5] = logits.cuda()
+    one = torch.ones(1, device="cuda")
+    tokens, accepted = dops.verify_drafts(wide[:, :, 5:vocab + 5], torch.from_numpy(drafts).cuda(), torch.from_numpy(u).cuda(), temperature=0.9 * one, top_k=(top_k * one).int(), top_p=one)
+    assert np.array_equal(tokens.cpu().numpy(), want) and np.array_equal(accepted.cpu().numpy(), count)
+
+
+def test_a_vocabulary_beyond_the_largest_is_refused(dops):
+    capi = importlib.import_module("macllm_infer_b200._capi")
+    one = torch.ones(1, device="cuda")
+    with pytest.raises(capi.MkError, match="at most 416000"):
+        dops.verify_drafts(torch.zeros(1, 1, 416001, device="cuda"), torch.zeros(1, 0, dtype=torch.int32, device="cuda"), one[:, None], temperature=one, top_k=one.int(), top_p=one)
