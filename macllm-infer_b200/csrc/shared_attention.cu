@@ -139,7 +139,8 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
         for (int j = 0; j < V; ++j) o[j] *= old;
         m = m_new;
         const int n = min(32, parts - s0);
-        // AHEAD parts on their way together; one without keys wrote no output
+        // AHEAD parts at a time, none of which waits for another's values where the compiler keeps their loads together (heads of 64 and 256: 100 registers; at heads of 128 it takes 48 and
+        // the loads come one after the other); one without keys wrote no output
         for (int b = 0; b < n; b += AHEAD) {
             float x[AHEAD][V], w[AHEAD];
 #pragma unroll
@@ -952,8 +953,12 @@ SharedAttnPlan shared_attention_plan(int q_heads, int kv_heads, int d, int block
     const int64_t items = (int64_t)rows * g;
     if (items <= 0 || lanes <= 0 || total <= 0) return p;
     const bool small = items <= 16 || (items <= 24 && d != 256 && lanes * (int64_t)kv_heads < kSms);
-    // Few keys: every lane reads the shared ones too, in one launch without parts (4 lanes of 4 KV heads of 64: 4.1 us and 8.0 with the shared keys' kernel behind 64 shared tokens, 7.7 and 8.4
-    // behind 512, 11.3 and 8.9 behind 1024; of 8 heads of 128: 5.0 and 9.0, 11.5 and 9.6 behind 512; 32 lanes: 5.7 and 9.5, 8.7 and 10.2 behind 256), as long as two CTAs an SM do for them.
+    // Few keys: every lane reads the shared ones too, in one launch without parts, as long as two CTAs an SM do for them.  Us so, and with the shared keys' kernel, by keys of a lane (48 of
+    // them its own):
+    //   4 lanes of 4 KV heads of 64    256: 4.9, 7.9   512: 6.8, 8.4    640: 7.7, 8.5    768: 8.5, 8.7    1024: 10.5, 9.0
+    //   4 lanes of 8 KV heads of 128   256: 6.7, 8.8   384: 8.5, 8.9    448: 9.5, 9.0    512: 10.3, 9.0
+    //   4 lanes of 8 KV heads of 256   256: 8.0, 11.2  384: 10.5, 12.0  448: 11.9, 12.2  512: 13.1, 12.2
+    //   32 lanes of 8 KV heads         of 64 640: 8.8, 9.7   of 128 384: 9.8, 10.5   of 256 320: 11.7, 12.3, and 384: 13.2, 12.4
     const int64_t all_keys = std::min((int64_t)width * block_tokens, window > 0 ? (int64_t)window + rows : INT64_MAX);
     p.alone = shared > 0 && small && lanes * (int64_t)kv_heads <= 2 * kSms && all_keys <= (d == 64 ? 640 : 384);
     if (p.alone) shared = 0;

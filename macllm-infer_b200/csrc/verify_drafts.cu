@@ -14,7 +14,7 @@
 // logits) bisection over (value, token) finds one that fewer do.
 //
 // Weights and sums of candidates are 64-bit.  Over the whole vocabulary a weight is a 32-bit number (ex2 of a product kept to twice 32 bits: 2^-22, and with no trend, so that
-// sums over many are better) and sums are 64-bit.
+// sums over many are better) and sums are 64-bit; where a draw's target is so small that what 32 bits leave out may decide, its weights are 64-bit too.
 #include "verify_drafts.h"
 #include "sampling_math.h"
 #include "shared_attention.h"
