@@ -93,10 +93,11 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
     }
     return v;
 }
-// Inclusive sums over the block's threads; *total: of all.
-__device__ double block_scan(double v, double* red, double* total) {
+// What the block's threads before this one add up to, which no larger number is taken from again; *total: of all.
+__device__ double block_before(double v, double* red, double* total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     v = warp_scan(v, lane);
+    const double others = __shfl_up_sync(0xffffffffu, v, 1);
     __syncthreads();
     if (lane == 31) red[w] = v;
     __syncthreads();
@@ -107,7 +108,7 @@ __device__ double block_scan(double v, double* red, double* total) {
         all += red[i];
     }
     *total = all;
-    return before + v;
+    return lane > 0 ? before + others : before;
 }
 
 // 512 E keys, the larger first: a thread has E neighbours, so that most exchanges of the bitonic network are inside a thread or a warp.
@@ -582,13 +583,13 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
             token[j] = j0 + j < k ? (int)rank_key_index(keys[j0 + j]) : -1;
             e[j] = j0 + j < k ? exp(((double)value_of_key(keys[j0 + j]) - (double)top) * per_t) : 0.0;
         }
-        const double upto_e = block_scan(e[0] + e[1], s.red, &z);
+        const double before_e = block_before(e[0] + e[1], s.red, &z);
         bool in[2] = {j0 < k, j0 + 1 < k};
         if (top_p < 1.f) {
-            in[0] = in[0] && (j0 == 0 || (upto_e - e[1] - e[0]) / z < (double)top_p);
-            in[1] = in[1] && (upto_e - e[1]) / z < (double)top_p;
+            in[0] = in[0] && (j0 == 0 || before_e / z < (double)top_p);
+            in[1] = in[1] && (before_e + e[0]) / z < (double)top_p;
         }
-        block_scan((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), s.red, &kept);
+        block_before((in[0] ? e[0] : 0.0) + (in[1] ? e[1] : 0.0), s.red, &kept);
         double* weights = reinterpret_cast<double*>(keys + kVerifyMaxTopK);
         uint32_t* by_token = reinterpret_cast<uint32_t*>(keys);   // a token and where it was, in 32 bits
         constexpr uint32_t kLastToken = (1u << 22) - 1;
@@ -633,19 +634,19 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
         p[j] = r[j] = j0 + j < n_last ? shares[j0 + j] : 0.0;
         if (d >= 0 && p[j] > 0.0) r[j] = fmax(p[j] - (q != nullptr ? (double)q[token[j]] : (token[j] == d ? 1.0 : 0.0)), 0.0);
     }
-    double upto = block_scan(r[0] + r[1], s.red, &total);
+    double before = block_before(r[0] + r[1], s.red, &total);
     if (!(total > 0.0)) {   // the draft's distribution covers the target's
         r[0] = p[0];
         r[1] = p[1];
-        upto = block_scan(r[0] + r[1], s.red, &total);
+        before = block_before(r[0] + r[1], s.red, &total);
     }
     const double target = u_draw * total;
     if (r[0] > 0.0) {
-        if (upto - r[1] > target) atomicMin(&s.pick, token[0]);
+        if (before + r[0] > target) atomicMin(&s.pick, token[0]);
         atomicMax(&s.last, token[0]);
     }
     if (r[1] > 0.0) {
-        if (upto > target) atomicMin(&s.pick, token[1]);
+        if (before + (r[0] + r[1]) > target) atomicMin(&s.pick, token[1]);
         atomicMax(&s.last, token[1]);
     }
     __syncthreads();
@@ -859,7 +860,7 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
             shares2(r_mine, none, t < at_hi ? q_at(t) : 0.f, 0.f);
             r = (double)r_mine;
         }
-        const double c = before + block_scan(r, top_shared.red, &all);
+        const double c = before + (block_before(r, top_shared.red, &all) + r);
         if (r > 0.0) {
             atomicMax(&s_last, t);
             if (c > target) atomicMin(&s_pick, t);

@@ -82,6 +82,20 @@ def test_draws_among_candidates_at_the_ends_of_the_unit_interval(dops, mask, kin
         assert np.array_equal(accepted, count) and np.array_equal(tokens, want), (end, tokens.tolist(), want.tolist())
 
 
+@pytest.mark.parametrize("vocab, top_k", [(2, 2), (3, 3), (17, 17), (257, 129), (700, 700)])
+@pytest.mark.parametrize("t, low", [(1.0, -60.0), (0.3, -20.0), (50.0, -30000.0), (1.0, -40.0)])
+def test_a_light_token_beside_a_heavy_one_has_its_share(dops, vocab, top_k, t, low):
+    """Sums of a thread's two candidates are not taken apart again, where the lighter one would be lost in the other."""
+    logits = torch.full((3, 1, vocab), low)
+    logits[0, 0, 1], logits[1, 0, vocab - 1], logits[2, 0, vocab // 2] = 1.0, 1.0, 1.0
+    logits[:, :, ::2] -= torch.arange((vocab + 1) // 2) * t / 16   # no two alike
+    drafts = np.empty((3, 0), np.int32)
+    for u in (0.0, 1e-45, 1e-30, 0.5, 1.0 - 2.0 ** -24):
+        tokens, accepted, settings = verify(dops, logits, drafts, np.full((3, 1), u, np.float32), None, t, top_k)
+        want, _, _ = verify_plain(logits.numpy(), drafts, np.full((3, 1), u, np.float32), *settings, None)
+        assert np.array_equal(tokens, want), (u, tokens.tolist(), want.tolist())
+
+
 @pytest.mark.parametrize("temperature, top_k", [(1.0, 0), (1.0, 9), (1.0, 200), (0.0, 0)])
 def test_rows_that_a_lane_does_not_reach_are_not_told_of(dops, temperature, top_k):
     logits, drafts, u, _ = verify_case(42, 4, 3, 700)
