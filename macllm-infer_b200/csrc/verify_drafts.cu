@@ -660,7 +660,7 @@ __device__ __noinline__ double wide_share(float x, float top, float temperature,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) finish_lanes_kernel(const __grid_constant__ VerifyArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ TopShared top_shared;
     __shared__ double sum_of[2][kMostCtas], region[kWarps], s_z;
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
     const T* x = logits + end * a.ld;
     const int d = end < n ? drafts[end] : -1;
     const float* q = probs == nullptr || d < 0 ? nullptr : probs + (int64_t)end * vocab;
-    const double z = s_z;
+    double z = s_z;
     const Exponential weight(value_of_key(s_best), temperature);
     const float per_z = (float)(1.0 / z), per_z_rest = (float)(1.0 / z - (double)per_z);
     const int chunk = (vocab + 4 * ctas - 1) / (4 * ctas) * 4, n0 = min(vocab, rank * chunk), n1 = min(vocab, n0 + chunk);
@@ -771,11 +771,12 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
         }
     };
     auto q_at = [&](int t) { return !rest ? 0.f : (q != nullptr ? q[t] : (t == d ? 1.f : 0.f)); };
-    auto share64 = [&](int t) { return wide_share(value_of(x[t]), value_of_key(s_best), temperature, rest, s_z, q_at(t)); };
-    // All the weights that 32 bits leave out are together below 2^-100 of the whole.  Where the target is so small that they may decide (u = 0, or a remainder of nothing else), shares are
-    // 64-bit: one draw in 2^24, or where the draft's distribution all but covers the target's.
-    constexpr double kLeastTarget = 0x1p-60;
-    bool wide = false, first = true;
+    // All the weights that 32 bits leave out are together below 2^-100 of the whole, and what they round is 2^-22 of a share of p.  Where the target is so small that the former may decide (u = 0),
+    // or the remainder so small that the latter do (draft and target all but agree), weights, their sum and shares are 64-bit: one draw in 2^24, and one in 1024 that end at such a remainder, since
+    // its size is how often that happens.
+    constexpr double kLeastTarget = 0x1p-60, kLeastRest = 0x1p-10;
+    bool wide = false, weigh = false, first = true;   // weigh: for the sum of the weights
+    auto share64 = [&](int t) { return wide_share(value_of(x[t]), value_of_key(s_best), temperature, rest && !weigh, z, q_at(t)); };
     double total = 0.0, *sums = sum_of[0];
     for (;; first = false) {
         constexpr int AHEAD = 4;   // fours of tokens a thread has on their way together
@@ -822,8 +823,13 @@ __global__ void __launch_bounds__(kThreads) finish_lanes_kernel(const __grid_con
         cluster.sync();
         total = 0.0;
         for (int c = 0; c < ctas; ++c) total += sums[c];
-        if (!wide && !(u_draw * total >= kLeastTarget)) wide = true;
-        else if (rest && !(total > 0.0)) rest = false;   // the draft's distribution covers the target's
+        if (!wide && (!(u_draw * total >= kLeastTarget) || (rest && total < kLeastRest))) {
+            wide = true;
+            weigh = rest;
+        } else if (weigh) {
+            z = total;
+            weigh = false;
+        } else if (rest && !(total > 0.0)) rest = false;   // the draft's distribution covers the target's
         else break;
         sums = sums == sum_of[0] ? sum_of[1] : sum_of[0];   // nobody is still at the one before the last
     }
