@@ -14,7 +14,7 @@
 // logits) bisection over (value, token) finds one that fewer do.
 //
 // Weights and sums of candidates are 64-bit.  Over the whole vocabulary a weight is a 32-bit number (ex2 of a product kept to twice 32 bits: 2^-22, and with no trend, so that
-// sums over many are better) and sums are 64-bit; where a draw's target is so small that what 32 bits leave out may decide, its weights are 64-bit too.
+// sums over many are better) and sums are 64-bit; where a draw's target or remainder is so small that what 32 bits leave out may decide, its weights are 64-bit too.
 #include "verify_drafts.h"
 #include "sampling_math.h"
 #include "shared_attention.h"
@@ -653,7 +653,7 @@ __device__ int2 finish_top_row(const VerifyArgs& a, TopShared& s, uint8_t* smem,
     return make_int2(0, s.pick < INT_MAX ? s.pick : s.last);
 }
 
-// A token's share of a draw in 64 bits.  Not inlined: it is needed once in 2^24 draws, and its registers are everyone's.
+// A token's share of a draw in 64 bits.  Not inlined: it is hardly ever needed, and its registers are everyone's.
 __device__ __noinline__ double wide_share(float x, float top, float temperature, bool rest, double z, float q) {
     const double w = exp(((double)x - (double)top) / (double)temperature);
     return rest ? fmax(w / z - (double)q, 0.0) : w;
