@@ -715,6 +715,50 @@ int32_t mk_k_gather_tokens_dev(void* k_pool_dev, void* v_pool_dev, int64_t layer
                                const int32_t* counts_dev, const int32_t* to_tables_dev, int64_t to_stride, int32_t to_width, const int32_t* first_dev, int32_t lanes,
                                int32_t* status_dev, void* cuda_stream);
 
+/* Paged caches of keys and values in 4 or 8 bits.  Pools of one layer: codes, pages [kv_heads][block_tokens] of rows of head_dim * bits / 8 bytes
+ * (value i of a row in bits i * bits % 8 .. of byte i * bits / 8), codes_stride bytes apart; and scales, pages [kv_heads][block_tokens][head_dim / 64] of
+ * pairs (step, lowest value), scales_stride values apart, f16 or bf16 (type) as the rows that are written, read and attended with.  A group of 64 neighbouring values of
+ * a head's row holds its lowest value and a step, (highest - lowest) / (2^bits - 1) rounded to `type`; code c stands for lowest + step * c, and
+ * codes are the nearest ones (halves to even).  A group with a value that is not finite, or whose range is not, reads as NaN.
+ * Pools and pages begin at multiples of 16 bytes.  head_dim 64, 128 or 256; block_tokens a power of two from 16.
+ *
+ * Rows of keys and values [total][kv_heads][head_dim] (strides between rows and heads in values, multiples of 8) into the pages, and what the pages hold
+ * back into rows, rounded to `type`, at most its largest value.  Lanes, tables and cu_seqlens are as of mk_k_shared_attention_dev: lane i has lengths[i] tokens
+ * in the pages tables[i][..], and its rows are the last of them; cu_seqlens NULL: total / lanes rows each.  Rows in front of a lane's first token are
+ * not written anywhere, and come back as zeros, as do rows whose page or length is out of range; rows that belong to no lane are left as they were.  No token is
+ * written by two rows of a call. */
+int32_t mk_k_quantize_rows_dev(const void* k_dev, int64_t k_row_stride, int64_t k_head_stride, const void* v_dev, int64_t v_row_stride, int64_t v_head_stride,
+                               int32_t type, int32_t bits, void* k_codes_dev, void* v_codes_dev, void* k_scales_dev, void* v_scales_dev,
+                               int64_t pool_pages, int64_t codes_stride, int64_t scales_stride, int32_t kv_heads, int32_t head_dim, int32_t block_tokens,
+                               const int32_t* tables_dev, int64_t table_stride, int32_t table_width, const int32_t* lengths_dev, const int32_t* cu_seqlens_dev, int32_t lanes,
+                               int32_t total, int32_t* status_dev, void* cuda_stream);
+int32_t mk_k_dequantize_rows_dev(int32_t type, int32_t bits, const void* k_codes_dev, const void* v_codes_dev, const void* k_scales_dev, const void* v_scales_dev,
+                                 int64_t pool_pages, int64_t codes_stride, int64_t scales_stride, int32_t kv_heads, int32_t head_dim, int32_t block_tokens,
+                                 const int32_t* tables_dev, int64_t table_stride, int32_t table_width, const int32_t* lengths_dev, const int32_t* cu_seqlens_dev, int32_t lanes,
+                                 int32_t total, void* k_dev, int64_t k_row_stride, int64_t k_head_stride, void* v_dev, int64_t v_row_stride, int64_t v_head_stride,
+                                 int32_t* status_dev, void* cuda_stream);
+
+/* Attention over such pools.  Lanes, rows, window, scale and softcap are as of mk_k_shared_attention_dev; q, out [total] rows of q_heads x head_dim values of the
+ * pools' type.  Keys and values are what their codes stand for.  What a row does not see, behind it, in front of its window or behind the
+ * lane's length, may hold anything.  The pages of a lane's tokens are in the table, also where a window hides them. */
+int32_t mk_k_quantized_attention_workspace(int32_t bits, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_tokens, int32_t table_width, int32_t lanes,
+                                           int32_t rows, int32_t total, int32_t window, int64_t* bytes);
+int32_t mk_k_quantized_attention_dev(const void* q_dev, int64_t q_stride, int32_t q_heads,
+                                     int32_t type, int32_t bits, const void* k_codes_dev, const void* v_codes_dev, const void* k_scales_dev, const void* v_scales_dev,
+                                     int64_t pool_pages, int64_t codes_stride, int64_t scales_stride, int32_t kv_heads, int32_t head_dim, int32_t block_tokens,
+                                     const int32_t* tables_dev, int64_t table_stride, int32_t table_width, const int32_t* lengths_dev, const int32_t* cu_seqlens_dev, int32_t lanes,
+                                     int32_t rows, int32_t total, float scale, float softcap, int32_t window, void* out_dev, int64_t out_stride, void* workspace_dev,
+                                     int64_t workspace_bytes, int32_t* status_dev, void* cuda_stream);
+
+/* Log probabilities of given tokens.  For each of `rows` rows of vocab logits (logits_stride apart; f32, f16 or bf16; -inf is a token that cannot be): the natural
+ * logarithm of tokens[row]'s probability, the entropy of the row's distribution (natural logarithms too), the token's rank (1 is the likeliest; among equals the
+ * lower token comes first) and the `top` likeliest tokens, at most 64, in that order, with their log probabilities ([rows][top]).  A negative
+ * token asks for none: log probability 0, rank 0; one beyond the vocabulary gets NaN, rank 0 and MK_DEV_BAD_RANGE.  A row that is no distribution (NaN, +inf, or nothing above
+ * -inf) gets NaN, rank 0, tokens -1 and MK_DEV_BAD_ROW. */
+int32_t mk_k_token_logprobs_dev(int32_t type, const void* logits_dev, int64_t logits_stride, int32_t rows, int32_t vocab, const int32_t* tokens_dev, int32_t top,
+                                float* logprobs_dev, float* entropy_dev, int32_t* ranks_dev, int32_t* top_tokens_dev, float* top_logprobs_dev, int32_t* status_dev,
+                                void* cuda_stream);
+
 /* TokenEmbedding::forward_validated (src/model_weights.rs:489-502). */
 int32_t mk_k_embed(int32_t type, const void* w, int64_t rows, int64_t cols, const uint32_t* ids, int32_t T, float scale, float* out);
 

@@ -155,6 +155,10 @@ class AttnForms(C.Structure):
 # Every symbol include/macllm_b200.h declares, with its ctypes signature (restype is int32 unless noted).
 P = C.c_void_p
 _i32, _i64, _u32, _u64, _f32 = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float
+# a paged cache in 4 or 8 bits: type, bits, codes, scales, pages and their strides, layout; and tables of pages
+_QUANTIZED_POOLS = [_i32, _i32, P, P, P, P, _i64, _i64, _i64, _i32, _i32, _i32]
+_TABLES = [P, _i64, _i32]
+
 SIGNATURES = {
     "mk_last_error": (C.c_char_p, []),
     "mk_version": (C.c_char_p, []),
@@ -289,6 +293,11 @@ SIGNATURES = {
     "mk_k_verify_drafts_dev": (_i32, [_i32, P, _i64, _i32, _i32, _i32, P, P, P, P, P, P, P, P, P, _i64, P, P]),
     "mk_k_copy_pages_dev": (_i32, [P, P, _i64, _i64, _i32, _i32, _i32, P, _i32, P, P]),
     "mk_k_gather_tokens_dev": (_i32, [P, P, _i64, _i64, _i32, _i32, _i32, P, _i64, _i32, P, _i64, _i32, P, P, _i64, _i32, P, _i32, P, P]),
+    "mk_k_quantize_rows_dev": (_i32, [P, _i64, _i64, P, _i64, _i64, *_QUANTIZED_POOLS, *_TABLES, P, P, _i32, _i32, P, P]),
+    "mk_k_dequantize_rows_dev": (_i32, [*_QUANTIZED_POOLS, *_TABLES, P, P, _i32, _i32, P, _i64, _i64, P, _i64, _i64, P, P]),
+    "mk_k_quantized_attention_workspace": (_i32, [_i32] * 10 + [C.POINTER(_i64)]),
+    "mk_k_quantized_attention_dev": (_i32, [P, _i64, _i32, *_QUANTIZED_POOLS, *_TABLES, P, P, _i32, _i32, _i32, _f32, _f32, _i32, P, _i64, P, _i64, P, P]),
+    "mk_k_token_logprobs_dev": (_i32, [_i32, P, _i64, _i32, _i32, P, _i32, P, P, P, P, P, P, P]),
 }
 
 # entry points that only the full library carries

@@ -1,0 +1,25 @@
+// Attention over paged caches in 4 or 8 bits (see quantized_attention.cu).
+#pragma once
+#include "quantized_kv.h"
+
+namespace mk {
+
+struct QuantAttnArgs {
+    QuantPools pools;
+    QuantLanes lanes;             // lanes.rows: the most rows that a lane has
+    const void* q = nullptr;      // [total] rows of q_heads * d values, row stride ldq
+    void* out = nullptr;          // the same, row stride ldo
+    int64_t ldq = 0, ldo = 0;
+    int q_heads = 0;
+    float scale = 1.f, softcap = 0.f;
+    int window = 0;
+};
+
+// How a call is cut, from sizes alone.
+struct QuantAttnPlan {
+    int64_t bytes = 0;
+};
+QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window);
+void launch_quantized_attention(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s);
+
+}  // namespace mk

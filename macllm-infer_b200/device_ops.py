@@ -1,4 +1,5 @@
-"""Operators over tensors in device memory (the mk_k_*_dev entry points), for serving many continuations of one prompt.
+"""Operators over tensors in device memory (the mk_k_*_dev entry points), for serving many continuations of one prompt, for caches of keys and values
+in 4 or 8 bits, and for scoring given tokens.
 
 Unlike the wrappers of ``ops``, which move host arrays to the device and back, these take CUDA tensors as they are, enqueue their kernels on
 the current stream of the tensors' device and return without waiting; they may be captured into a CUDA graph (sizes, pointers, Python
@@ -10,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -158,9 +160,9 @@ def verify_drafts(logits, drafts, u, *, temperature, top_k, top_p, draft_probs=N
 
 def _pools(k_pool, v_pool):
     shape, dtype = k_pool.shape, k_pool.dtype
-    if (len(shape) != 5 or v_pool.shape != shape or v_pool.dtype is not dtype or dtype not in _TYPES or v_pool.get_device() != k_pool.get_device()
+    if (len(shape) != 5 or v_pool.shape != shape or v_pool.dtype is not dtype or (dtype not in _TYPES and dtype is not torch.uint8) or v_pool.get_device() != k_pool.get_device()
             or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
-        raise ValueError("k_pool and v_pool are contiguous [layers, pages, kv heads, tokens of a page, head size] of one shape and type (float32, float16 or bfloat16), on one device")
+        raise ValueError("k_pool and v_pool are contiguous [layers, pages, kv heads, tokens of a page, head size] of one shape and type (float32, float16, bfloat16, or uint8 for codes), on one device")
     layers, pages, heads, page, dim = shape
     return k_pool.data_ptr(), v_pool.data_ptr(), layers, pages, heads, page, dim * dtype.itemsize
 
@@ -184,3 +186,176 @@ def gather_tokens(k_pool, v_pool, from_tables, keep, counts, to_tables, first, *
     _run(device, capi.lib().mk_k_gather_tokens_dev, *_pools(k_pool, v_pool), *_rows(from_tables, lanes, device, "from_tables"), *_rows(keep, lanes, device, "keep"),
          _dense(counts, _I32, (lanes,), device, "counts"), *_rows(to_tables, lanes, device, "to_tables"), _dense(first, _I32, (lanes,), device, "first"), lanes,
          None if status is None else _dense(status, _I32, (1,), device, "status"))
+
+
+# ---- caches in 4 or 8 bits -----------------------------------------------------------------------------------------------------------------------------------------
+
+_GROUP = 64
+
+
+class QuantizedPools(NamedTuple):
+    """One layer's keys and values in 4 or 8 bits: codes [pages, kv_heads, block_tokens, head_dim * bits / 8] uint8 (the lower four bits of a byte come first), and for each
+    group of 64 neighbouring values of a row a pair (step, lowest value) [pages, kv_heads, block_tokens, head_dim / 64, 2] of the rows' type; code c stands for
+    lowest + step * c.  Where a call takes pools, any tuple of four such tensors will do; pages may be further apart than they are long, all at the same distances."""
+    k_codes: torch.Tensor
+    v_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def quantized_pools(pages: int, kv_heads: int, block_tokens: int, head_dim: int, *, bits: int = 4, dtype=torch.float16, device="cuda") -> QuantizedPools:
+    """Empty pools for one layer, of 4.5 or 8.5 bits a value."""
+    if bits not in (4, 8) or head_dim not in (64, 128, 256) or dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("a cache has 4 or 8 bits, heads of 64, 128 or 256 values and float16 or bfloat16 rows")
+    codes = [torch.zeros(pages, kv_heads, block_tokens, head_dim * bits // 8, dtype=torch.uint8, device=device) for _ in range(2)]
+    scales = [torch.zeros(pages, kv_heads, block_tokens, head_dim // _GROUP, 2, dtype=dtype, device=device) for _ in range(2)]
+    return QuantizedPools(*codes, *scales)
+
+
+def _quantized(pools, device):
+    """The pools' arguments of an entry point; head size and type beside them."""
+    k_codes, v_codes, k_scales, v_scales = pools
+    shape, of_scales, dtype = k_codes.shape, k_scales.shape, k_scales.dtype
+    if len(shape) != 4 or len(of_scales) != 5 or of_scales[:3] != shape[:3] or of_scales[4] != 2 or (dtype is not torch.float16 and dtype is not torch.bfloat16):
+        raise ValueError("pools are codes [pages, kv heads, tokens of a page, bytes] and scales [pages, kv heads, tokens of a page, groups, 2], float16 or bfloat16")
+    pages, heads, page, row = shape
+    groups = of_scales[3]
+    dim = groups * _GROUP
+    bits = row * 8 // dim if dim else 0
+    strides, of_strides = k_codes.stride(), k_scales.stride()
+    if (bits * dim != row * 8 or bits not in (4, 8) or k_codes.dtype is not torch.uint8 or v_codes.dtype is not torch.uint8 or v_scales.dtype is not dtype or v_codes.shape != shape
+            or v_scales.shape != of_scales or not k_codes.get_device() == v_codes.get_device() == k_scales.get_device() == v_scales.get_device() == device):
+        raise ValueError("codes are uint8, half a byte or a byte for each value of 64 to a scale, keys and values alike, on the device of the others")
+    if pages > 1 and (v_codes.stride(0) != strides[0] or v_scales.stride(0) != of_strides[0]):
+        raise ValueError("pages of keys and of values are equally far apart")
+    if pages and not (k_codes[0].is_contiguous() and v_codes[0].is_contiguous() and k_scales[0].is_contiguous() and v_scales[0].is_contiguous()):
+        raise ValueError("pages are dense")
+    return dim, dtype, (_TYPES[dtype], bits, k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, strides[0] if pages > 1 else heads * page * row,
+                        of_strides[0] if pages > 1 else heads * page * groups * 2, heads, dim, page)
+
+
+def _lanes(tables, lengths, cu_seqlens, device):
+    lanes = tables.shape[0] if tables.dim() == 2 else -1
+    return lanes, (*_rows(tables, lanes, device, "tables"), _dense(lengths, _I32, (lanes,), device, "lengths"),
+                   None if cu_seqlens is None else _dense(cu_seqlens, _I32, (lanes + 1,), device, "cu_seqlens"), lanes)
+
+
+def _head_rows(t, shape, dtype, device, what: str):
+    """Address and strides of rows [total, kv heads, head size] whose heads are dense."""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (t.numel() and t.stride(2) != 1):
+        raise ValueError(f"{what} is a {dtype} tensor of shape {tuple(shape)} with dense heads on the device of the others: got {t.dtype} {tuple(t.shape)} on {t.device}")
+    row, head, _ = t.stride()
+    return t.data_ptr(), row if shape[0] > 1 else shape[1] * shape[2], head if shape[1] > 1 else shape[2]
+
+
+def _word(status, device):
+    return None if status is None else _dense(status, _I32, (1,), device, "status")
+
+
+def quantize_rows(k, v, pools, tables, lengths, *, cu_seqlens=None, status=None) -> None:
+    """Writes rows of keys and values [total, kv_heads, head_dim] into the pages of ``pools``, as codes and scales.
+
+    tables [lanes, width] page numbers; lengths [lanes] tokens of each lane, the last of which are its rows (cu_seqlens [lanes + 1], or total / lanes rows each): rows and
+    heads may be strided.  Rows in front of a lane's first token are left out.  A group with a value that is not finite reads as NaN."""
+    device = k.get_device()
+    dim, dtype, cache = _quantized(pools, device)
+    lanes, where = _lanes(tables, lengths, cu_seqlens, device)
+    shape = torch.Size((k.shape[0] if k.dim() else 0, pools[0].shape[1], dim))
+    _run(device, capi.lib().mk_k_quantize_rows_dev, *_head_rows(k, shape, dtype, device, "k"), *_head_rows(v, shape, dtype, device, "v"), *cache, *where, shape[0],
+         _word(status, device))
+
+
+def dequantize_rows(pools, tables, lengths, total: int, *, cu_seqlens=None, k=None, v=None, status=None):
+    """Reads the tokens that ``quantize_rows`` with the same tables, lengths and cu_seqlens writes back into rows.
+
+    Returns (k, v) [total, kv_heads, head_dim] of the scales' type.  Rows in front of a lane's first token are zeros, and rows outside cu_seqlens left as ``k`` and ``v`` had them."""
+    device = pools[0].get_device()
+    dim, dtype, cache = _quantized(pools, device)
+    lanes, where = _lanes(tables, lengths, cu_seqlens, device)
+    shape = torch.Size((total, pools[0].shape[1], dim))
+    if k is None:
+        k = torch.empty(shape, dtype=dtype, device=pools[0].device)
+    if v is None:
+        v = torch.empty(shape, dtype=dtype, device=pools[0].device)
+    _run(device, capi.lib().mk_k_dequantize_rows_dev, *cache, *where, total, *_head_rows(k, shape, dtype, device, "k"), *_head_rows(v, shape, dtype, device, "v"),
+         _word(status, device))
+    return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _quantized_workspace(*sizes) -> int:
+    need = C.c_int64()
+    capi.check(capi.lib().mk_k_quantized_attention_workspace(*sizes, C.byref(need)))
+    return need.value
+
+
+def quantized_attention(q, pools, tables, lengths, *, scale: float, cu_seqlens=None, max_rows: int = 0, softcap: float = 0.0, window: int = 0, out=None, status=None):
+    """Attention of a ragged batch over a cache in 4 or 8 bits, read as it is.
+
+    q [total, q_heads, head_dim] of the scales' type; tables, lengths, cu_seqlens and ``max_rows`` as of ``shared_attention``: a lane's rows are the last of its tokens, whose
+    keys and values are in the pages already.  Returns [total, q_heads, head_dim]; a row that sees nothing becomes zeros, rows outside cu_seqlens are left as ``out`` had them."""
+    device, shape = q.get_device(), q.shape
+    dim, dtype, cache = _quantized(pools, device)
+    if len(shape) != 3 or q.dtype is not dtype or shape[2] != dim:
+        raise ValueError(f"q is a {dtype} tensor [rows, heads, {dim}], as the pools are")
+    total, heads, _ = shape
+    lanes, where = _lanes(tables, lengths, cu_seqlens, device)
+    if cu_seqlens is None:
+        rows = total // lanes if lanes else 0
+        if rows * lanes != total:
+            raise ValueError("without cu_seqlens every lane has the same number of rows")
+    else:
+        rows = max_rows
+        if max_rows <= 0 and total:
+            raise ValueError("with cu_seqlens, max_rows says how many rows a lane has at most")
+    q_strides = q.stride()
+    if total and q_strides[1:] != (dim, 1) and (heads != 1 or q_strides[2] != 1):
+        raise ValueError("the heads of a row are dense")
+    if out is None:
+        out, out_stride = torch.empty_like(q), heads * dim   # dense, since the heads of a row are
+    else:
+        out_strides = out.stride()
+        if (out.shape != shape or out.dtype is not dtype or out.get_device() != device
+                or (total and out_strides[1:] != (dim, 1) and (heads != 1 or out_strides[2] != 1))):
+            raise ValueError("out is like q, the heads of a row dense")
+        out_stride = out_strides[0] if total > 1 else heads * dim
+    need = _quantized_workspace(cache[1], heads, *cache[9:], where[2], lanes, rows, total, window)
+    space = q.new_empty(need // 2) if need else None
+    _run(device, capi.lib().mk_k_quantized_attention_dev, q.data_ptr(), q_strides[0] if total > 1 else heads * dim, heads, *cache, *where, rows, total, scale, softcap, window,
+         out.data_ptr(), out_stride, space.data_ptr() if need else None, need, _word(status, device))
+    return out
+
+
+# ---- scoring -------------------------------------------------------------------------------------------------------------------------------------------------------
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor       # [rows] f32
+    entropy: torch.Tensor        # [rows] f32
+    ranks: torch.Tensor          # [rows] int32, 1 is the likeliest
+    top_tokens: torch.Tensor     # [rows, top] int32
+    top_logprobs: torch.Tensor   # [rows, top] f32
+
+
+def token_logprobs(logits, tokens, *, top: int = 0, status=None) -> TokenLogprobs:
+    """Log probabilities (natural) of given tokens, with the entropy of their distributions, their ranks and the ``top`` likeliest tokens, at most 64.
+
+    logits [rows, vocab] f32, f16 or bf16 (rows may be further apart; -inf is a token that cannot be); tokens [rows] int32.  Equal logits are ranked by rising token.  A
+    negative token asks for none (log probability 0, rank 0), one beyond the vocabulary gets NaN and BAD_RANGE; a row that is no distribution NaN, rank 0, tokens -1 and BAD_ROW."""
+    dtype, device, shape = logits.dtype, logits.get_device(), logits.shape
+    if len(shape) != 2 or dtype not in _TYPES or shape[1] < 1:
+        raise ValueError("logits is a float32, float16 or bfloat16 tensor [rows, vocabulary]")
+    rows, vocab = shape
+    strides = logits.stride()
+    if rows and vocab > 1 and strides[1] != 1:
+        raise ValueError("rows of logits are dense")
+    given = _dense(tokens, _I32, (rows,), device, "tokens")
+    if not 0 <= top <= min(64, vocab):
+        raise ValueError("top is at most 64 and at most the vocabulary")
+    # one allocation: what a row has, then its likeliest tokens
+    words = torch.empty(rows * (3 + 2 * top), dtype=_F32, device=logits.device)
+    logprobs, entropy, ranks, top_tokens, top_logprobs = words.split((rows, rows, rows, rows * top, rows * top))
+    out = TokenLogprobs(logprobs, entropy, ranks.view(_I32), top_tokens.view(_I32).view(rows, top), top_logprobs.view(rows, top))
+    _run(device, capi.lib().mk_k_token_logprobs_dev, _TYPES[dtype], logits.data_ptr(), strides[0] if rows > 1 else vocab, rows, vocab, given, top, logprobs.data_ptr(),
+         entropy.data_ptr(), ranks.data_ptr(), top_tokens.data_ptr(), top_logprobs.data_ptr(), _word(status, device))
+    return out
