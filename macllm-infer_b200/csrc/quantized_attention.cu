@@ -2,13 +2,20 @@
 //
 // Row t of lane i has position p = length_i - n_i + t and sees the keys max(0, p - window + 1) .. p of the lane's pages:
 //   o = sum_j w_j v_j / sum_j w_j,   w_j = exp(cap(scale q . k_j) - m),
-// with k_j and v_j what their codes stand for, low + step c, not rounded to 16 bits.  Scores, weights, maxima and sums are 32-bit.
+// with k_j and v_j what their codes stand for, low + step c for each group of 64 values.
 #include "quantized_attention.h"
+#include "attention_math.cuh"
 #include "kernels.h"
+#include "umma.cuh"
+#include <algorithm>
 
 namespace mk {
 
 namespace {
+
+using namespace umma;
+
+constexpr int kSms = 148;   // calls are cut without a device, for a B200
 
 __device__ __forceinline__ void tell(int32_t* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);
@@ -19,75 +26,615 @@ __device__ __forceinline__ float2 wide_pair(uint32_t w) {
     if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&w));
     else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-
-// A warp to a (row, query head): D / 32 values to a thread, one key after the other.
-template <typename T, int D, int BITS>
-__global__ void __launch_bounds__(32) quantized_attention_kernel(const __grid_constant__ QuantAttnArgs a) {
-    constexpr int V = D / 32, G = D / kQuantGroup;
-    const QuantPools& p = a.pools;
-    const int lane_id = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, kvh = head / (a.q_heads / p.kv_heads);
-    int first = a.lanes.cu != nullptr ? a.lanes.cu[lane_id] : lane_id * a.lanes.rows, n = a.lanes.cu != nullptr ? a.lanes.cu[lane_id + 1] - first : a.lanes.rows;
-    const int length = a.lanes.lengths[lane_id];
-    const int keys = (int)min((int64_t)max(length, 0), (int64_t)a.lanes.width << p.bt_shift);
-    if (first < 0 || first > a.lanes.total || n < 0 || n > a.lanes.rows || n > a.lanes.total - first || keys != length) {
-        if (lane == 0) tell(a.lanes.status, kDevBadRange);
-        if (first < 0 || first > a.lanes.total) first = 0, n = 0;
-        n = min(max(n, 0), min(a.lanes.rows, a.lanes.total - first));
-    }
-    for (int r = blockIdx.z; r < n; r += gridDim.z) {
-        const int position = keys - n + r;
-        const T* q = static_cast<const T*>(a.q) + (int64_t)(first + r) * a.ldq + head * D + lane * V;
-        float qv[V], o[V], m = -INFINITY, l = 0.f;
-        for (int j = 0; j < V; ++j) qv[j] = (float)q[j], o[j] = 0.f;
-        auto value = [&](const uint8_t* codes, const uint32_t* scales, int64_t row, float (&x)[V]) {
-            const float2 sl = wide_pair<T>(scales[row * G + lane * V / kQuantGroup]);
-            for (int j = 0; j < V; ++j) {
-                const int i = lane * V + j;
-                const uint32_t c = BITS == 8 ? codes[row * D + i] : codes[row * (D / 2) + i / 2] >> (i % 2 * 4) & 15;
-                x[j] = fmaf(sl.x, (float)c, sl.y);
-            }
-        };
-        for (int key = attention_first_key(max(position, 0), a.window, 0); key <= position; ++key) {
-            int page = a.lanes.tables[lane_id * a.lanes.ld_table + (key >> p.bt_shift)];
-            if (page < 0 || page >= p.pages) {
-                if (lane == 0) tell(a.lanes.status, kDevBadPage);
-                page = 0;
-            }
-            const int64_t row = (int64_t)kvh * p.block_tokens + (key & (p.block_tokens - 1));
-            float x[V], s = 0.f;
-            value(p.k_codes + page * p.codes_stride, p.k_scales + page * p.scales_stride, row, x);
-            for (int j = 0; j < V; ++j) s = fmaf(qv[j], x[j], s);
-            s = warp_sum(s) * a.scale;
-            if (a.softcap != 0.f) s = a.softcap * tanhf(s / a.softcap);
-            const float m_new = fmaxf(m, s), m_use = m_new == -INFINITY ? 0.f : m_new, alpha = expf(m - m_use), w = expf(s - m_use);
-            m = m_new;
-            l = fmaf(l, alpha, w);
-            value(p.v_codes + page * p.codes_stride, p.v_scales + page * p.scales_stride, row, x);
-            for (int j = 0; j < V; ++j) o[j] = fmaf(o[j], alpha, w * x[j]);
-        }
-        T* out = static_cast<T*>(a.out) + (int64_t)(first + r) * a.ldo + head * D + lane * V;
-        for (int j = 0; j < V; ++j) out[j] = (T)(l == 0.f ? 0.f : o[j] / l);
+template <typename T>
+__device__ __forceinline__ uint32_t narrow_pair(float x, float y) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
 
-template <typename T, int BITS>
-void launch(const QuantAttnArgs& a, cudaStream_t s) {
-    const dim3 grid(a.lanes.lanes, a.q_heads, std::min(a.lanes.rows, 64));
-    switch (a.pools.d) {
-        case 64: quantized_attention_kernel<T, 64, BITS><<<grid, 32, 0, s>>>(a); break;
-        case 128: quantized_attention_kernel<T, 128, BITS><<<grid, 32, 0, s>>>(a); break;
-        default: quantized_attention_kernel<T, 256, BITS><<<grid, 32, 0, s>>>(a); break;
+// Where a lane's rows and keys are; whatever the arrays hold, rows stay inside [0, total) and keys inside the table.
+struct LaneRange {
+    int first, n;       // rows
+    int position;       // of its first row
+    int keys;           // length, at most what the table holds
+};
+__device__ __forceinline__ LaneRange lane_range(const QuantAttnArgs& a, int lane) {
+    const QuantLanes& l = a.lanes;
+    LaneRange r;
+    r.first = l.cu != nullptr ? l.cu[lane] : lane * l.rows;
+    r.n = l.cu != nullptr ? l.cu[lane + 1] - r.first : l.rows;
+    const int length = l.lengths[lane];
+    r.keys = min(max(length, 0), l.width << a.pools.bt_shift);
+    if (r.first < 0 || r.first > l.total || r.n < 0 || r.n > l.rows || r.n > l.total - r.first || r.keys != length) {
+        tell(l.status, kDevBadRange);
+        if (r.first < 0 || r.first > l.total) r.first = 0, r.n = 0;
+        r.n = min(max(r.n, 0), min(l.rows, l.total - r.first));
     }
+    r.position = r.keys - r.n;
+    return r;
+}
+
+// The keys of a block of items, and how they are shared out: `chunk` of them from `begin` on to each share, the last of which ends at `hi`.
+struct Shares {
+    int lo, hi, begin, chunk;
+    __device__ __forceinline__ int used() const { return hi > lo ? (hi - begin + chunk - 1) / chunk : 0; }
+};
+__device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRange& at, int item0, int n_items, int g, int chunk_min, int shares) {
+    const int p0 = at.position + item0 / g, p1 = at.position + (item0 + n_items - 1) / g;
+    Shares s;
+    s.lo = attention_first_key(max(p0, 0), a.window, 0);
+    s.hi = min(p1 + 1, at.keys);
+    s.begin = s.lo / 16 * 16;
+    const int each = s.hi > s.begin ? (s.hi - s.begin + shares - 1) / shares : 0;
+    s.chunk = max(chunk_min, (each + 15) / 16 * 16);
+    return s;
+}
+
+// ---- few items -----------------------------------------------------------------------------------------------------
+//
+// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks tiles of 16 keys, whose codes and scales bulk copies
+// bring into a ring of its own.  Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
+// are the f16 number c 2^-24 (a subnormal, which the tensor cores take in full), so that it costs a mask and half a shift.  With steps and lowest values of the groups
+//   q . k = sum_g step_g (q_g . c_g) + low_g sum(q_g),   o = sum_j (w_j step_jg) c_j + sum_j w_j low_jg,
+// steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
+// Queries are brought to f16 by a power of two per item, weights by one for the largest step met so far; either is exact.  The running maximum follows only
+// when a score exceeds it by more than 2^kSlack, which a vote of the warp tells.
+constexpr int kTile = 16;
+constexpr int kWarps = 4;
+constexpr float kSlack = 8.f;            // base-2 logarithm
+constexpr float kWeightScale = 128.f;    // weights up to 2^kSlack, times this, times a step over the largest: below f16's largest
+
+template <int D, int BITS, int NT>
+struct Few {
+    static constexpr int G = D / kQuantGroup, ITEMS = NT * 8;
+    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, STAGE = 2 * (CODES + SCALES);
+    static constexpr int STAGES = STAGE <= 2400 ? 8 : 4;
+    static constexpr int OP = D + 4;                                     // pitch of a warp's results, in floats
+    static constexpr int RING = ((STAGES * STAGE > ITEMS * OP * 4 ? STAGES * STAGE : ITEMS * OP * 4) + 127) / 128 * 128;
+    static constexpr int QP = D + 8;
+    static constexpr size_t SMEM = 128 + (size_t)kWarps * RING + (size_t)ITEMS * QP * 2;
+    static constexpr bool Q_IN_REGISTERS = NT * D <= 256;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A copy of a multiple of 16 bytes, both addresses multiples of 16.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+template <typename V>
+__device__ __forceinline__ V lds(uint32_t at) {
+    V v;
+    if constexpr (sizeof(V) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+    else if constexpr (sizeof(V) == 8) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+// The key of a tile that row r of a product stands for: with neighbours swapped in every other pair, the rows that a load takes at once lie on both halves of the banks.
+__device__ __forceinline__ int key_of(int r) { return r ^ (r >> 1 & 1); }
+
+template <typename T, int D, int BITS, int NT, int CAP>
+__global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_constant__ QuantAttnArgs a, int chunk_min, int shares, float* part_o, float2* part_ml) {
+    using L = Few<D, BITS, NT>;
+    constexpr int G = L::G;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[kWarps * L::STAGES];
+    __shared__ float item_factor[L::ITEMS], item_sums[L::ITEMS][G];
+    __shared__ float2 warp_ml[kWarps][L::ITEMS];
+    uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
+    __half* qs = reinterpret_cast<__half*>(rings + kWarps * L::RING);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
+    const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y;
+    const QuantPools& p = a.pools;
+    const int g = a.q_heads / p.kv_heads;
+    pdl_trigger();
+    const LaneRange at = lane_range(a, lane_id);
+    const int item0 = blockIdx.z * L::ITEMS, n_items = min(L::ITEMS, at.n * g - item0);
+    if (n_items <= 0) return;
+    const Shares sh = shares_of(a, at, item0, n_items, g, chunk_min, shares);
+    if (share > 0 && share >= sh.used()) return;
+    const int lo = max(sh.lo, sh.begin + share * sh.chunk), hi = min(sh.hi, sh.begin + (share + 1) * sh.chunk);
+    const int begin = sh.begin + share * sh.chunk, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0;
+    const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
+
+    const uint32_t ring = smem_u32(rings + warp * L::RING);
+    uint64_t* full = bars + warp * L::STAGES;
+    const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
+    // the page numbers of 32 tiles sit in the warp's threads, those of the next 32 on their way
+    auto page_of = [&](int i) {
+        if (i >= my_tiles) return 0;
+        const int32_t page = table[(begin + (warp + kWarps * i) * kTile) >> p.bt_shift];
+        if ((uint32_t)page < (uint64_t)p.pages) return page;
+        tell(a.lanes.status, kDevBadPage);
+        return 0;
+    };
+    int page_now = page_of(lane), page_next = my_tiles > 32 ? page_of(32 + lane) : 0;
+    auto load_tile = [&](int i) {   // the whole warp; one copy to each of four threads
+        if ((i & 31) == 0 && i > 0) {
+            page_now = page_next;
+            page_next = page_of(i + 32 + lane);
+        }
+        const int64_t page = __shfl_sync(0xffffffffu, page_now, i & 31);
+        const int st = i & (L::STAGES - 1);
+        const int64_t row = (int64_t)kvh * p.block_tokens + ((begin + (warp + kWarps * i) * kTile) & (p.block_tokens - 1));
+        if (lane == 0) bar_expect_tx(&full[st], L::STAGE);
+        __syncwarp();
+        if (lane < 4) {   // codes of keys, of values, scales of keys, of values
+            const bool codes = lane < 2, keys = (lane & 1) == 0;
+            const uint8_t* from = codes ? (keys ? p.k_codes : p.v_codes) + page * p.codes_stride + row * L::ROW
+                                        : reinterpret_cast<const uint8_t*>((keys ? p.k_scales : p.v_scales) + page * p.scales_stride + row * G);
+            bulk_load(ring + st * L::STAGE + (codes ? lane * L::CODES : 2 * L::CODES + (lane - 2) * L::SCALES), from, codes ? L::CODES : L::SCALES, &full[st]);
+        }
+    };
+    if (lane == 0) {
+        for (int i = 0; i < L::STAGES; ++i) bar_init(&full[i], 1);
+        bar_init_fence();
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < min(L::STAGES, my_tiles); ++i) load_tile(i);
+
+    // queries: a warp has an item, V neighbouring values to a thread
+    constexpr int V = D / 32;
+    const float unit = CAP ? a.scale : a.scale * kLog2e;
+    for (int item = warp; item < L::ITEMS; item += kWarps) {
+        float x[V], sum = 0.f, top = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = 0.f;
+        if (item < n_items) {
+            const int r = (item0 + item) / g, hq = (item0 + item) - r * g;
+            const T* q = static_cast<const T*>(a.q) + (int64_t)(at.first + r) * a.ldq + (kvh * g + hq) * D + lane * V;
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const float2 y = wide_pair<T>(*reinterpret_cast<const uint32_t*>(q + j));
+                x[j] = y.x;
+                x[j + 1] = y.y;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            sum += x[j];
+            top = fmaxf(top, fabsf(x[j]));
+        }
+        // the largest becomes 2^14 and a bit; powers of two that neither the factor here nor the one of the scores overflows
+        top = warp_max(top);
+        const int e = top > 0.f ? min(max(14 - (int)((__float_as_uint(top) >> 23) - 127), -86), 100) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t*>(qs + item * L::QP + lane * V + j) = narrow_pair<__half>(x[j] * up, x[j + 1] * up);
+        // sums of the groups, each of which 64 / V threads hold
+#pragma unroll
+        for (int o = 1; o < kQuantGroup / V; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane % (kQuantGroup / V) == 0) item_sums[item][lane * V / kQuantGroup] = sum * up * 0x1p-24f;
+        if (lane == 0) item_factor[item] = unit * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
+    }
+    __syncthreads();
+
+    float o_acc[NT][G][4][4], low_acc[NT][G][2], m_run[NT][2], l_run[NT][2], factor[NT][2], sums[NT][G][2];
+    int see_lo[NT][2], see_hi[NT][2];   // keys that the thread's two items of a group of eight see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o_acc[n][j][u][0] = o_acc[n][j][u][1] = o_acc[n][j][u][2] = o_acc[n][j][u][3] = 0.f;
+            low_acc[n][j][0] = low_acc[n][j][1] = 0.f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int item = n * 8 + 2 * tq + h, pos = at.position + (item0 + item) / g;
+            m_run[n][h] = -INFINITY;
+            l_run[n][h] = 0.f;
+            factor[n][h] = item_factor[item];
+#pragma unroll
+            for (int j = 0; j < G; ++j) sums[n][j][h] = item_sums[item][j];
+            see_lo[n][h] = max(lo, attention_first_key(max(pos, 0), a.window, 0));
+            see_hi[n][h] = min(hi, pos + 1);
+        }
+    }
+    const int p0 = at.position + item0 / g, p1 = at.position + (item0 + n_items - 1) / g;
+    const int all_lo = max(lo, attention_first_key(max(p1, 0), a.window, 0)), all_hi = min(hi, p0 + 1);   // keys that every item sees
+    const float two_over_cap = CAP ? 2.0f / a.softcap : 0.f;
+    const bool wide_cap = CAP && a.softcap > kCapOfDifference;
+    // queries as the B operand of step s of group j: the values that stand in the codes' order of the thread's words
+    auto query = [&](int n, int j, int s, uint32_t& b0, uint32_t& b1) {
+        const __half* q = qs + (n * 8 + gid) * L::QP + j * kQuantGroup + tq * 16;
+        if constexpr (BITS == 4) {
+            const __half* w = q + (s >> 1) * 8 + (s & 1) * 2;
+            const __half2 x = __halves2half2(w[0], w[4]), y = __hmul2(__halves2half2(w[1], w[5]), __float2half2_rn(0.0625f));   // codes of the second pair are 16 times theirs
+            b0 = *reinterpret_cast<const uint32_t*>(&x);
+            b1 = *reinterpret_cast<const uint32_t*>(&y);
+        } else {
+            const __half* w = q + s * 4;
+            const __half2 x = __halves2half2(w[0], w[2]), y = __halves2half2(w[1], w[3]);
+            b0 = *reinterpret_cast<const uint32_t*>(&x);
+            b1 = *reinterpret_cast<const uint32_t*>(&y);
+        }
+    };
+    uint32_t q_reg[L::Q_IN_REGISTERS ? NT : 1][G][4][2];
+    if constexpr (L::Q_IN_REGISTERS) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) query(n, j, s, q_reg[n][j][s][0], q_reg[n][j][s][1]);
+    }
+    float cap_step = 0.f, to_step = 0.f;   // a power of two no step so far exceeds; kWeightScale over it
+    const int key0 = key_of(gid), key1 = key0 + 8;
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < my_tiles; ++i) {
+        const int st = i & (L::STAGES - 1);
+        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i / L::STAGES & 1));
+        if (!ok) {
+            if (lane == 0) tell(a.lanes.status, kDevWait);
+            break;
+        }
+        const uint32_t kt = ring + st * L::STAGE, vt = kt + L::CODES, kst = vt + L::CODES, vst = kst + L::SCALES;
+        const int pos0 = begin + (warp + kWarps * i) * kTile;
+        // ---- scores
+        float sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            uint32_t w0[4], w1[4];   // words of the thread's two keys
+            if constexpr (BITS == 4) {
+                const uint2 x = lds<uint2>(kt + key0 * L::ROW + j * 32 + tq * 8), y = lds<uint2>(kt + key1 * L::ROW + j * 32 + tq * 8);
+                w0[0] = x.x, w0[1] = x.y, w1[0] = y.x, w1[1] = y.y;
+            } else {
+                const uint4 x = lds<uint4>(kt + key0 * L::ROW + j * 64 + tq * 16), y = lds<uint4>(kt + key1 * L::ROW + j * 64 + tq * 16);
+                w0[0] = x.x, w0[1] = x.y, w0[2] = x.z, w0[3] = x.w, w1[0] = y.x, w1[1] = y.y, w1[2] = y.z, w1[3] = y.w;
+            }
+            float acc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                uint32_t a0, a1, a2, a3;
+                if constexpr (BITS == 4) {
+                    const uint32_t x = s & 1 ? w0[s >> 1] >> 8 : w0[s >> 1], y = s & 1 ? w1[s >> 1] >> 8 : w1[s >> 1];
+                    a0 = x & 0x000f000fu, a2 = x & 0x00f000f0u, a1 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                } else {
+                    a0 = w0[s] & 0x00ff00ffu, a2 = w0[s] >> 8 & 0x00ff00ffu, a1 = w1[s] & 0x00ff00ffu, a3 = w1[s] >> 8 & 0x00ff00ffu;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t b0, b1;
+                    if constexpr (L::Q_IN_REGISTERS) b0 = q_reg[n][j][s][0], b1 = q_reg[n][j][s][1];
+                    else query(n, j, s, b0, b1);
+                    mma_f16(acc[n], a0, a1, a2, a3, b0, b1);
+                }
+            }
+            const float2 sl0 = wide_pair<T>(lds<uint32_t>(kst + (key0 * G + j) * 4)), sl1 = wide_pair<T>(lds<uint32_t>(kst + (key1 * G + j) * 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                sc[n][0] = fmaf(sl0.x, acc[n][0], fmaf(sl0.y, sums[n][j][0], sc[n][0]));
+                sc[n][1] = fmaf(sl0.x, acc[n][1], fmaf(sl0.y, sums[n][j][1], sc[n][1]));
+                sc[n][2] = fmaf(sl1.x, acc[n][2], fmaf(sl1.y, sums[n][j][0], sc[n][2]));
+                sc[n][3] = fmaf(sl1.x, acc[n][3], fmaf(sl1.y, sums[n][j][1], sc[n][3]));
+            }
+        }
+        float2 v0[G], v1[G];   // (step, lowest) of the thread's two keys' values
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            v0[j] = wide_pair<T>(lds<uint32_t>(vst + (key0 * G + j) * 4));
+            v1[j] = wide_pair<T>(lds<uint32_t>(vst + (key1 * G + j) * 4));
+        }
+        const bool whole = pos0 >= all_lo && pos0 + kTile <= all_hi;
+        if (!whole) {   // keys that no item of the block sees may have any scales: those of values count as 0
+            if (pos0 + key0 < lo || pos0 + key0 >= hi) {
+#pragma unroll
+                for (int j = 0; j < G; ++j) v0[j] = make_float2(0.f, 0.f);
+            }
+            if (pos0 + key1 < lo || pos0 + key1 >= hi) {
+#pragma unroll
+                for (int j = 0; j < G; ++j) v1[j] = make_float2(0.f, 0.f);
+            }
+        }
+        bool up = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v = sc[n][e] * factor[n][e & 1];
+                if (CAP) v = (wide_cap ? capped_wide(v, a.softcap, two_over_cap) : capped(v, a.softcap, two_over_cap)) * kLog2e;
+                if (!whole) {
+                    const int pos = pos0 + (e < 2 ? key0 : key1);
+                    v = pos >= see_lo[n][e & 1] && pos < see_hi[n][e & 1] ? v : -INFINITY;
+                }
+                sc[n][e] = v;
+                up |= v > m_run[n][e & 1] + kSlack;   // also when there was none yet
+            }
+        }
+        float top_step = 0.f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) top_step = fmaxf(top_step, fmaxf(v0[j].x, v1[j].x));
+        top_step = top_step < INFINITY ? top_step : 0.f;
+        up |= top_step > cap_step;
+        if (__any_sync(0xffffffffu, up)) {
+            const float largest = fmaxf(warp_max(top_step), cap_step);
+            // the next power of two, between those whose inverse is one too
+            const float cap_new = largest > 0.f ? __uint_as_float(min(max((__float_as_uint(largest) + 0x007fffffu) & 0x7f800000u, 8u << 23), 252u << 23)) : 0.f;
+            const float shrink = cap_new > 0.f ? cap_step / cap_new : 1.f;
+            cap_step = cap_new;
+            to_step = cap_new > 0.f ? kWeightScale / cap_new : 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float alpha[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float top = fmaxf(sc[n][h], sc[n][2 + h]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float m_new = fmaxf(m_run[n][h], top);
+                    alpha[h] = m_new == -INFINITY ? 1.f : ex2(m_run[n][h] - m_new);
+                    m_run[n][h] = m_new;
+                    l_run[n][h] *= alpha[h];
+#pragma unroll
+                    for (int j = 0; j < G; ++j) low_acc[n][j][h] *= alpha[h];
+                    alpha[h] *= shrink;
+                }
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        o_acc[n][j][u][0] *= alpha[0];
+                        o_acc[n][j][u][1] *= alpha[1];
+                        o_acc[n][j][u][2] *= alpha[0];
+                        o_acc[n][j][u][3] *= alpha[1];
+                    }
+            }
+        }
+        // ---- weights
+        uint32_t hi_b[NT][G][2], lo_b[NT][G][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float m = m_run[n][e & 1];
+                w[e] = ex2(sc[n][e] - (m == -INFINITY ? 0.f : m));
+            }
+            l_run[n][0] += w[0] + w[2];
+            l_run[n][1] += w[1] + w[3];
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                float x[4];
+                if (whole) {
+                    low_acc[n][j][0] = fmaf(w[0], v0[j].y, fmaf(w[2], v1[j].y, low_acc[n][j][0]));
+                    low_acc[n][j][1] = fmaf(w[1], v0[j].y, fmaf(w[3], v1[j].y, low_acc[n][j][1]));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = w[e] * ((e < 2 ? v0[j].x : v1[j].x) * to_step);
+                } else {   // what an item does not see does not count, also where it is not finite
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v = e < 2 ? v0[j] : v1[j];
+                        const bool seen = sc[n][e] != -INFINITY;
+                        low_acc[n][j][e & 1] += seen ? w[e] * v.y : 0.f;
+                        x[e] = seen ? w[e] * (v.x * to_step) : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t high = narrow_pair<__half>(x[2 * h], x[2 * h + 1]);
+                    const float2 r = wide_pair<__half>(high);
+                    hi_b[n][j][h] = transpose_8x8(high);
+                    lo_b[n][j][h] = transpose_8x8(narrow_pair<__half>(x[2 * h] - r.x, x[2 * h + 1] - r.y));
+                }
+            }
+        }
+        // ---- output
+        const int va = key_of(2 * tq), vb = key_of(2 * tq + 1);   // the thread's keys: these and eight further on
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            constexpr int WORDS = BITS / 4;
+            uint32_t w[4][WORDS];   // eight values of each of four keys
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t from = vt + ((k & 1 ? vb : va) + (k >> 1) * 8) * L::ROW + j * (kQuantGroup * BITS / 8) + gid * BITS;
+                if constexpr (BITS == 4) {
+                    w[k][0] = lds<uint32_t>(from);
+                } else {
+                    const uint2 x = lds<uint2>(from);
+                    w[k][0] = x.x, w[k][1] = x.y;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {   // values 2 u and 2 u + 1 of the eight
+                uint32_t a0, a1, a2, a3;
+                if constexpr (BITS == 4) {
+                    uint32_t x = __byte_perm(w[0][0], w[1][0], u < 2 ? 0x5410 : 0x7632), y = __byte_perm(w[2][0], w[3][0], u < 2 ? 0x5410 : 0x7632);
+                    if (u & 1) x >>= 8, y >>= 8;
+                    a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                } else {
+                    const uint32_t x = __byte_perm(w[0][u >> 1], w[1][u >> 1], u & 1 ? 0x7632 : 0x5410), y = __byte_perm(w[2][u >> 1], w[3][u >> 1], u & 1 ? 0x7632 : 0x5410);
+                    a0 = x & 0x00ff00ffu, a1 = x >> 8 & 0x00ff00ffu, a2 = y & 0x00ff00ffu, a3 = y >> 8 & 0x00ff00ffu;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma_f16(o_acc[n][j][u], a0, a1, a2, a3, hi_b[n][j][0], hi_b[n][j][1]);
+                    mma_f16(o_acc[n][j][u], a0, a1, a2, a3, lo_b[n][j][0], lo_b[n][j][1]);
+                }
+            }
+        }
+        __syncwarp();
+        if (i + L::STAGES < my_tiles) load_tile(i + L::STAGES);
+    }
+    if (!ok) {   // copies in flight land before the CTA ends
+        for (int st = 0; st < L::STAGES; ++st) bar_wait(&full[st], 0), bar_wait(&full[st], 1);
+    }
+
+    // ---- a warp's results, over its own sum: [item][D] and (maximum, sum)
+    float* mine = reinterpret_cast<float*>(rings + warp * L::RING);
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float l = l_run[n][h];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            const int item = n * 8 + 2 * tq + h;
+            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], ok ? l : NAN);
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                float low = low_acc[n][j][h];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) low += __shfl_xor_sync(0xffffffffu, low, o);
+                low *= inv;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    // codes were c 2^-24, those of the second value 16 times that
+                    const float x = o_acc[n][j][u][h] * inv * (0x1p24f / kWeightScale), y = o_acc[n][j][u][2 + h] * inv * (BITS == 4 ? 0x1p20f / kWeightScale : 0x1p24f / kWeightScale);
+                    *reinterpret_cast<float2*>(mine + item * L::OP + j * kQuantGroup + gid * 8 + 2 * u) = make_float2(fmaf(x, cap_step, low), fmaf(y, cap_step, low));
+                }
+            }
+        }
+    }
+    __syncthreads();
+    // ---- the warps' results together
+    const bool last = shares == 1;
+    const int64_t n_rows = (int64_t)a.lanes.total * a.q_heads;
+    for (int i = tid; i < n_items * (D / 4); i += kWarps * 32) {
+        const int item = i / (D / 4), c = (i - item * (D / 4)) * 4;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_ml[w][item].x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = warp_ml[w][item];
+            if (ml.y == 0.f) continue;
+            const float f = ml.y * ex2(ml.x - (m == -INFINITY ? 0.f : m));
+            const float4 x = *reinterpret_cast<const float4*>(rings + w * L::RING + (item * L::OP + c) * 4);
+            l += f;
+            o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;   // a row that sees nothing: zeros
+        o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+        const int r = (item0 + item) / g, hq = (item0 + item) - r * g;
+        if (last) {
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(at.first + r) * a.ldo + (kvh * g + hq) * D + c) = make_uint2(narrow_pair<T>(o.x, o.y), narrow_pair<T>(o.z, o.w));
+        } else {
+            const int64_t row = share * n_rows + (int64_t)(at.first + r) * a.q_heads + kvh * g + hq;
+            *reinterpret_cast<float4*>(part_o + row * D + c) = o;
+            if (c == 0) part_ml[row] = make_float2(m, l);
+        }
+    }
+}
+
+// ---- shares joined: a warp to a (row, query head) ----------------------------------------------------------------------
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ QuantAttnArgs a, int items_of_block, int chunk_min, int shares, const float* part_o, const float2* part_ml) {
+    constexpr int V = D / 32;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.q_heads / a.pools.kv_heads;
+    const int lane_id = blockIdx.x, i = blockIdx.y * 4 + warp;
+    const LaneRange at = lane_range(a, lane_id);
+    const int64_t n_rows = (int64_t)a.lanes.total * a.q_heads;
+    for (int64_t at_row = i; at_row < (int64_t)at.n * a.q_heads; at_row += (int64_t)gridDim.y * 4) {
+        const int r = (int)(at_row / a.q_heads), head = (int)(at_row - (int64_t)r * a.q_heads), item = r * g + head % g, item0 = item / items_of_block * items_of_block;
+        const int used = max(1, shares_of(a, at, item0, min(items_of_block, at.n * g - item0), g, chunk_min, shares).used());
+        const int64_t row = (int64_t)(at.first + r) * a.q_heads + head;
+        float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = 0.f;
+        for (int s0 = 0; s0 < used; s0 += 32) {
+            const float2 ml = s0 + lane < used ? __ldcg(part_ml + (s0 + lane) * n_rows + row) : make_float2(-INFINITY, 0.f);
+            const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ml.y * ex2(ml.x - m_use);
+            l = l * old + warp_sum(f);
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] *= old;
+            m = m_new;
+            for (int s = 0; s < min(32, used - s0); ++s) {
+                const float w = __shfl_sync(0xffffffffu, f, s);
+                if (w == 0.f) continue;
+                const float* src = part_o + ((s0 + s) * n_rows + row) * D + lane * V;
+#pragma unroll
+                for (int j = 0; j < V; j += 2) {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src + j));
+                    o[j] = fmaf(w, y.x, o[j]);
+                    o[j + 1] = fmaf(w, y.y, o[j + 1]);
+                }
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        T* out = static_cast<T*>(a.out) + (int64_t)(at.first + r) * a.ldo + head * D + lane * V;
+#pragma unroll
+        for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t*>(out + j) = narrow_pair<T>(o[j] * inv, o[j + 1] * inv);
+    }
+}
+
+template <typename T, int D, int BITS, int NT, int CAP>
+void launch_few(const QuantAttnArgs& a, const QuantAttnPlan& p, float* part_o, float2* part_ml, cudaStream_t s) {
+    auto* kernel = few_items_kernel<T, D, BITS, NT, CAP>;
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Few<D, BITS, NT>::SMEM);
+    kernel<<<dim3((unsigned)(a.lanes.lanes * p.shares), (unsigned)a.pools.kv_heads, (unsigned)p.blocks), kWarps * 32, Few<D, BITS, NT>::SMEM, s>>>(a, p.chunk, p.shares, part_o, part_ml);
     MK_LAUNCH_CHECK();
+}
+
+template <typename T, int D>
+void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s) {
+    float* part_o = static_cast<float*>(workspace);
+    float2* part_ml = reinterpret_cast<float2*>(part_o + (p.shares > 1 ? p.shares * (int64_t)a.lanes.total * a.q_heads * D : 0));
+    auto run = [&](auto bits, auto nt) {
+        constexpr int B = decltype(bits)::value, N = decltype(nt)::value;
+        a.softcap != 0.f ? launch_few<T, D, B, N, 1>(a, p, part_o, part_ml, s) : launch_few<T, D, B, N, 0>(a, p, part_o, part_ml, s);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Four = std::integral_constant<int, 4>;
+    using Eight = std::integral_constant<int, 8>;
+    if (a.pools.bits == 4) p.items == 8 ? run(Four{}, One{}) : run(Four{}, Two{});
+    else p.items == 8 ? run(Eight{}, One{}) : run(Eight{}, Two{});
+    if (p.shares > 1) {
+        const int64_t rows = (int64_t)a.lanes.rows * a.q_heads;
+        launch_pdl(join_kernel<T, D>, dim3((unsigned)a.lanes.lanes, (unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(128), 0, s, a, p.items, p.chunk, p.shares,
+                   (const float*)part_o, (const float2*)part_ml);
+        MK_LAUNCH_CHECK();
+    }
 }
 
 }  // namespace
 
-QuantAttnPlan quantized_attention_plan(int, int, int, int, int, int, int, int, int, int) { return QuantAttnPlan{}; }
+QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window) {
+    QuantAttnPlan p;
+    const int64_t items = (int64_t)rows * (q_heads / kv_heads);
+    p.items = items <= 8 ? 8 : 16;
+    p.blocks = (int)std::max<int64_t>(1, (items + p.items - 1) / p.items);
+    const int64_t most = window > 0 ? std::min<int64_t>((int64_t)width * block_tokens, (int64_t)window + rows + 15) : (int64_t)width * block_tokens;
+    p.chunk = 256;
+    const int64_t columns = std::max<int64_t>(1, (int64_t)lanes * kv_heads * p.blocks);
+    // as many shares as make six waves of three CTAs on each SM, of 256 keys at least
+    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>((most + p.chunk - 1) / p.chunk, (6 * 3 * kSms + columns - 1) / columns));
+    if (p.shares > 1) p.bytes = (int64_t)p.shares * total * q_heads * ((int64_t)d * 4 + 8);
+    return p;
+}
 
-void launch_quantized_attention(const QuantAttnArgs& a, const QuantAttnPlan&, void*, cudaStream_t s) {
-    if (a.pools.bf16) a.pools.bits == 4 ? launch<__nv_bfloat16, 4>(a, s) : launch<__nv_bfloat16, 8>(a, s);
-    else a.pools.bits == 4 ? launch<__half, 4>(a, s) : launch<__half, 8>(a, s);
+void launch_quantized_attention(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s) {
+    auto with_type = [&](auto type) {
+        using T = decltype(type);
+        switch (a.pools.d) {
+            case 64: launch<T, 64>(a, p, workspace, s); break;
+            case 128: launch<T, 128>(a, p, workspace, s); break;
+            default: launch<T, 256>(a, p, workspace, s); break;
+        }
+    };
+    a.pools.bf16 ? with_type(__nv_bfloat16{}) : with_type(__half{});
 }
 
 }  // namespace mk

@@ -17,7 +17,9 @@ struct QuantAttnArgs {
 
 // How a call is cut, from sizes alone.
 struct QuantAttnPlan {
-    int64_t bytes = 0;
+    int items = 0, blocks = 0;   // (row, query head) items of a lane and KV head to a CTA, and such blocks
+    int shares = 1, chunk = 0;   // shares of a lane's keys, and the fewest keys of one
+    int64_t bytes = 0;           // workspace
 };
 QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window);
 void launch_quantized_attention(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s);

@@ -6,6 +6,7 @@
 // l_b e^(m_b - m), o likewise.  Maxima, sums and outputs of parts are 32-bit; weights are rounded to the pools' type for the product with V, as the
 // result itself is at the end.
 #include "shared_attention.h"
+#include "attention_math.cuh"
 #include "hgemm_tc.h"
 #include "kernels.h"
 #include "tile_phases.h"
@@ -21,30 +22,13 @@ namespace {
 
 using namespace umma;
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSms = 148;   // calls are cut without a device, for a B200
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)), which rounds in parts of the cap: 2^-14 and less up to kCapOfDifference.
-constexpr float kCapOfDifference = 256.f;
-__device__ __forceinline__ float capped(float v, float cap, float two_over_cap) {
-    return cap - __fdividef(2.0f * cap, 1.0f + __expf(fminf(v * two_over_cap, 80.0f)));
-}
-// For caps above, by kernels of their own (beside the other in one kernel it cost calls without any cap 1.5 %): with x = v / cap below 1/4 as v (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315), whose next term is 3.4e-7 of v; from there on the roundings above are less than 2^-20 of v.
-__device__ __forceinline__ float capped_wide(float v, float cap, float two_over_cap) {
-    const float x = 0.5f * v * two_over_cap, y = x * x;
-    return y < 0.0625f ? v * fmaf(y, fmaf(y, fmaf(y, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f) : capped(v, cap, two_over_cap);
-}
-
 template <typename T>
 struct Pair;
 template <>
@@ -77,12 +61,6 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
 }
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
-}
-// The 8 x 8 tile of 16-bit numbers that a warp holds as (row lane / 4, columns 2 (lane % 4), + 1), transposed.
-__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {   // zeros where there is nothing
