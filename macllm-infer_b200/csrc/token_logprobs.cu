@@ -2,103 +2,482 @@
 //
 // For a row x of logits with maximum m and Z = sum e^(x_i - m):  log p_i = x_i - m - ln Z,  entropy = -sum p_i log p_i = ln Z - sum e^(x_i - m) (x_i - m) / Z.  The rank of
 // a token is its place among all, by falling logit and, among equals, rising token; the likeliest tokens come in that order.
+//
+// One kernel, in which a row is read once from memory: by one CTA, or by a cluster of up to eight where rows are few, a run of the row to each.  A thread takes vectors of 16 bytes, eight of
+// them at a time, and keeps its maximum, both sums under it, and how many values stand before the given token's; maxima and sums of threads, warps and CTAs join
+// exactly but for roundings.  Differences x - m are taken before anything is scaled, so that they carry one rounding, and sums are 32-bit: a few hundred terms to a thread, then a tree.
+// The likeliest `top` of a run: the top-th best of the threads' maxima is a bound that at least `top` values reach and few more do, only the vectors of threads that reach it are
+// looked at again (in L2), and the candidates are ranked by counting.  Where too many reach it - thousands of equal logits, or most of them masked - a radix select over (value, token) finds the
+// top-th key exactly, in up to seven more passes.  The leader of a cluster merges the sorted lists by binary search.
 #include "token_logprobs.h"
 #include <cuda_bf16.h>
+#include <cooperative_groups.h>
+#include <algorithm>
 
 namespace mk {
 
 namespace {
 
-constexpr int kThreads = 256;
+namespace cg = cooperative_groups;
 
-template <typename T>
-__device__ __forceinline__ float wide(T x) { return (float)x; }
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kBatch = 8;             // vectors of a thread on their way together
+constexpr int kCandidates = 512;
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tell(int32_t* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);
 }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 
-// The best (value, token) of the block's threads, falling value first, then rising token.
-__device__ __forceinline__ void block_best(float& v, int& i, float* red_v, int* red_i) {
-    auto better = [](float v0, int i0, float v1, int i1) { return v0 > v1 || (v0 == v1 && i0 < i1); };
-    for (int o = 16; o > 0; o >>= 1) {
-        const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, i, o);
-        if (better(ov, oi, v, i)) v = ov, i = oi;
+// Numbers as unsigned ones of the same order (no NaN; both zeros are one).
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_ordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+// (value, token) of the same order as the likeliest come in: the larger key first.
+__device__ __forceinline__ uint64_t key_of(float x, int token) { return (uint64_t)ordered(x) << 24 | (uint32_t)(0xffffff - token); }
+__device__ __forceinline__ int token_of(uint64_t key) { return 0xffffff - (int)(key & 0xffffff); }
+__device__ __forceinline__ float value_of(uint64_t key) { return of_ordered((uint32_t)(key >> 24)); }
+
+// Vectors of 16 bytes: their values, maximum, and how many reach a bound.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ float value(const uint4& v, int i) { return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
+    static __device__ __forceinline__ float top(const uint4& v) { return max_nan(max_nan(value(v, 0), value(v, 1)), max_nan(value(v, 2), value(v, 3))); }
+    static __device__ __forceinline__ int reach(const uint4& v, float bound) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += value(v, i) >= bound ? 1 : 0;
+        return n;
+    }
+    static __device__ __forceinline__ float after(float x) {   // the next number up
+        const uint32_t b = __float_as_uint(x + 0.f);
+        return __uint_as_float(b & 0x80000000u ? b - 1 : b + 1);
+    }
+};
+template <typename P>
+__device__ __forceinline__ P as_pair(uint32_t w) { return *reinterpret_cast<const P*>(&w); }
+template <>
+struct Vec<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+    static __device__ __forceinline__ float value(const uint4& v, int i) {
+        const float2 f = __half22float2(as_pair<__half2>(word(v, i >> 1)));
+        return i & 1 ? f.y : f.x;
+    }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        const __half2 m = __hmax2_nan(__hmax2_nan(as_pair<__half2>(v.x), as_pair<__half2>(v.y)), __hmax2_nan(as_pair<__half2>(v.z), as_pair<__half2>(v.w)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ int reach(const uint4& v, float bound) {
+        const __half2 b = __float2half2_rn(bound);   // a number of the type
+        const __half2 n = __hadd2(__hadd2(__hge2(as_pair<__half2>(v.x), b), __hge2(as_pair<__half2>(v.y), b)), __hadd2(__hge2(as_pair<__half2>(v.z), b), __hge2(as_pair<__half2>(v.w), b)));
+        return (int)(__low2float(n) + __high2float(n));
+    }
+    static __device__ __forceinline__ float after(float x) {
+        const unsigned short b = __half_as_ushort(__float2half_rn(x + 0.f));
+        return __half2float(__ushort_as_half(b & 0x8000u ? b - 1 : b + 1));
+    }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ float value(const uint4& v, int i) {
+        const uint32_t w = Vec<__half>::word(v, i >> 1);
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        using P = __nv_bfloat162;
+        const P m = __hmax2_nan(__hmax2_nan(as_pair<P>(v.x), as_pair<P>(v.y)), __hmax2_nan(as_pair<P>(v.z), as_pair<P>(v.w)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ int reach(const uint4& v, float bound) {
+        using P = __nv_bfloat162;
+        const P b = __float2bfloat162_rn(bound);
+        const P n = __hadd2(__hadd2(__hge2(as_pair<P>(v.x), b), __hge2(as_pair<P>(v.y), b)), __hadd2(__hge2(as_pair<P>(v.z), b), __hge2(as_pair<P>(v.w), b)));
+        return (int)(__low2float(n) + __high2float(n));
+    }
+    static __device__ __forceinline__ float after(float x) {
+        const uint32_t b = __float_as_uint(x + 0.f) >> 16;
+        return __uint_as_float((b & 0x8000u ? b - 1 : b + 1) << 16);
+    }
+};
+
+// The values of a CTA's run of a row: `vectors` of 16 bytes from token `first` on, and, in single ones, those of the row in front of the first vector and behind the last.
+template <typename T>
+struct Run {
+    const T* row;
+    int first, vectors;
+    int head, tail_at, tail;   // tokens [0, head) and [tail_at, tail_at + tail)
+    __device__ __forceinline__ uint4 vector(int i) const { return __ldg(reinterpret_cast<const uint4*>(row + first) + i); }
+    // f(value, token), `there` false where a thread of the warp has none; the warp's threads come together
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        constexpr int N = Vec<T>::N;
+        for (int i0 = 0; i0 < vectors; i0 += kThreads) {
+            const int i = i0 + (int)threadIdx.x;
+            const bool there = i < vectors;
+            const uint4 v = there ? vector(i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int j = 0; j < N; ++j) f(Vec<T>::value(v, j), first + i * N + j, there);
+        }
+        const int e = edge();
+        f(e >= 0 ? (float)row[e] : 0.f, e, e >= 0);
+    }
+    __device__ __forceinline__ int edge() const {   // the thread's single token, or -1
+        const int i = (int)threadIdx.x;
+        return i < head ? i : (i < head + tail ? tail_at + i - head : -1);
+    }
+};
+
+struct Sums {   // of a part of a row: maximum, sum of e^(x - m), sum of e^(x - m) (x - m), values in front of the given token's
+    float m, z, zx;
+    int before;
+};
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+    Sums r;
+    r.m = max_nan(a.m, b.m);
+    r.before = a.before + b.before;
+    if (!(r.m > -INFINITY)) {   // nothing, or NaN
+        r.z = a.z + b.z;
+        r.zx = a.zx + b.zx;
+        return r;
+    }
+    // a difference that overflows belongs to a sum that vanishes
+    const float da = fmaxf(a.m - r.m, -3e38f), db = fmaxf(b.m - r.m, -3e38f), fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
+    r.z = a.z * fa + b.z * fb;
+    r.zx = (fa > 0.f ? fa * fmaf(a.z, da, a.zx) : 0.f) + (fb > 0.f ? fb * fmaf(b.z, db, b.zx) : 0.f);
+    return r;
+}
+
+struct Shared {
+    Sums warp_sums[kWarps], sums;
+    uint32_t tops[kThreads];
+    uint64_t candidates[kCandidates];
+    uint64_t best[kLogprobMaxTop];          // of the run, in order
+    uint64_t lists[kMaxCluster][kLogprobMaxTop];
+    uint32_t histogram[256];
+    uint64_t prefix;
+    uint32_t bound;
+    int n_candidates, n_best, left;
+    int list_n[kMaxCluster];
+};
+
+// The `top` best keys of the run into s.best, in order; s.n_best of them.
+template <typename T>
+__device__ __forceinline__ void best_of_run(const Run<T>& run, float my_top, int top, Shared& s) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    s.tops[tid] = ordered(my_top);
+    if (tid == 0) s.n_candidates = 0;
+    __syncthreads();
+    if (warp == 0) {   // a bound that `top` threads' maxima reach, and hardly twice as many
+        uint32_t k[kThreads / 32], lo = UINT32_MAX, hi = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) {
+            k[i] = s.tops[i * 32 + lane];
+            lo = min(lo, k[i]);
+            hi = max(hi, k[i]);
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);   // all reach it
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kThreads / 32; ++i) n += k[i] >= mid ? 1 : 0;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (n >= top) lo = mid;
+            else hi = mid - 1;
+            if (n >= top && n <= top + top / 2) break;
+        }
+        if (lane == 0) s.bound = lo;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red_v[threadIdx.x >> 5] = v, red_i[threadIdx.x >> 5] = i;
+    const uint32_t bound = s.bound;
+    if (ordered(my_top) >= bound) {
+        constexpr int N = Vec<T>::N;
+        auto offer = [&](float x, int token) {
+            if (ordered(x) < bound) return;
+            const int at = atomicAdd(&s.n_candidates, 1);
+            if (at < kCandidates) s.candidates[at] = key_of(x, token);
+        };
+        const float least = of_ordered(bound);
+        for (int i0 = tid; i0 < run.vectors; i0 += kThreads * 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = i0 + k * kThreads < run.vectors ? run.vector(i0 + k * kThreads) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * kThreads;
+                if (i >= run.vectors || Vec<T>::top(v[k]) < least) continue;
+#pragma unroll
+                for (int j = 0; j < N; ++j) offer(Vec<T>::value(v[k], j), run.first + i * N + j);
+            }
+        }
+        const int e = run.edge();
+        if (e >= 0) offer((float)run.row[e], e);
+    }
     __syncthreads();
-    v = red_v[0], i = red_i[0];
-    for (int w = 1; w < kThreads / 32; ++w)
-        if (better(red_v[w], red_i[w], v, i)) v = red_v[w], i = red_i[w];
+    if (s.n_candidates > kCandidates) {   // digit by digit from the top: the key that `top` keys reach
+        if (tid == 0) s.prefix = 0, s.left = top;   // more than kCandidates values are there
+        for (int shift = 48; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += kThreads) s.histogram[i] = 0;
+            __syncthreads();
+            const uint64_t prefix = s.prefix;
+            run.each([&](float x, int token, bool there) {
+                const uint64_t key = key_of(x, token);
+                const bool in = there && key >> 8 >> shift == prefix;
+                const int digit = (int)(key >> shift & 255);
+                const uint32_t of = __ballot_sync(0xffffffffu, in);
+                if (of == 0) return;
+                // equal digits are counted at once: thousands of equal logits would queue at one counter
+                const int first_digit = __shfl_sync(0xffffffffu, digit, __ffs(of) - 1);   // every thread of the warp comes here
+                if (__all_sync(0xffffffffu, !in || digit == first_digit)) {
+                    if (lane == __ffs(of) - 1) atomicAdd(&s.histogram[digit], __popc(of));
+                } else if (in) {
+                    atomicAdd(&s.histogram[digit], 1);
+                }
+            });
+            __syncthreads();
+            if (warp == 0) {   // the digit in which the top-th key lies: eight counters to a thread, from the top
+                uint32_t mine = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mine += s.histogram[255 - 8 * lane - i];
+                uint32_t upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t before = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += before;
+                }
+                const uint32_t left = (uint32_t)s.left;
+                __syncwarp();
+                if (upto >= left && upto - mine < left) {
+                    uint32_t rest = left - (upto - mine);
+                    int d = 255 - 8 * lane;
+                    while (s.histogram[d] < rest) rest -= s.histogram[d--];
+                    s.prefix = prefix << 8 | (uint64_t)d;
+                    s.left = (int)rest;
+                    s.n_candidates = 0;
+                }
+            }
+            __syncthreads();
+        }
+        const uint64_t least = s.prefix;
+        run.each([&](float x, int token, bool there) {
+            if (!there || key_of(x, token) < least) return;
+            const int at = atomicAdd(&s.n_candidates, 1);
+            if (at < kCandidates) s.candidates[at] = key_of(x, token);
+        });
+        __syncthreads();
+    }
+    const int n = min(s.n_candidates, kCandidates);
+    for (int i = tid; i < n; i += kThreads) {
+        const uint64_t mine = s.candidates[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += s.candidates[j] > mine ? 1 : 0;
+        if (rank < top) s.best[rank] = mine;
+    }
+    if (tid == 0) s.n_best = min(n, top);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    __shared__ float red[32];
-    __shared__ int red_i[32];
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
+    constexpr int N = Vec<T>::N;
+    __shared__ Shared s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t row = blockIdx.x / parts;
+    const int part = blockIdx.x - (int)row * parts;
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     const int token = a.tokens[row];
     const bool given = token >= 0 && token < a.vocab;
-    const float mine = given ? wide(x[token]) : 0.f;
-    float top = -INFINITY, odd = 0.f;
-    for (int i = tid; i < a.vocab; i += kThreads) {
-        const float v = wide(x[i]);
-        top = fmaxf(top, v);
-        if (!(v < INFINITY)) odd = 1.f;
+    const float mine = given ? (float)x[token] : INFINITY;
+
+    // the row's vectors, evenly shared out; its ends in single values go to the first CTA
+    Run<T> run;
+    {
+        const int off = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), head = min(off, a.vocab), vectors = (a.vocab - head) / N;
+        const int each = (vectors + parts - 1) / parts, from = min(part * each, vectors);
+        run.row = x;
+        run.first = head + from * N;
+        run.vectors = min(each, vectors - from);
+        run.head = part == 0 ? head : 0;
+        run.tail_at = head + vectors * N;
+        run.tail = part == 0 ? a.vocab - run.tail_at : 0;
     }
-    const float m = block_max(top, red);
-    const bool bad = block_max(odd, red) != 0.f || m == -INFINITY;
-    float z = 0.f, zx = 0.f, before = 0.f;
-    if (!bad) {
-        for (int i = tid; i < a.vocab; i += kThreads) {
-            const float v = wide(x[i]), e = expf(v - m);
-            z += e;
-            if (v > -INFINITY) zx += e * (v - m);
-            if (given && (v > mine || (v == mine && i < token))) before += 1.f;
+    // tokens in front of the given one count where they reach its logit, those behind it where they exceed it; its own vector's are looked at one by one
+    const float above = given ? Vec<T>::after(mine) : INFINITY;
+    const int own_vector = given && token >= run.first ? (token - run.first) / N : -1;
+
+    Sums my{-INFINITY, 0.f, 0.f, 0};
+    auto add = [&](float v, float m) {
+        const float d = v - m, e = ex2(d * kLog2e);
+        my.z += e;
+        my.zx = fmaf(e, fmaxf(d, -3e38f), my.zx);
+    };
+    auto raise = [&](float top) {   // the maximum to at least `top`; what to subtract
+        const float m = max_nan(my.m, top);
+        if (m > my.m) {
+            const float d = fmaxf(my.m - m, -3e38f), f = ex2(d * kLog2e);
+            my.zx = f > 0.f ? f * fmaf(my.z, d, my.zx) : 0.f;
+            my.z *= f;
+        }
+        my.m = m;
+        return m == -INFINITY ? 0.f : m;
+    };
+    for (int i0 = tid; i0 < run.vectors; i0 += kThreads * kBatch) {
+        uint4 v[kBatch];
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (i0 + k * kThreads < run.vectors) v[k] = run.vector(i0 + k * kThreads);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (i0 + k * kThreads < run.vectors) top = max_nan(top, Vec<T>::top(v[k]));
+        const float m = raise(top);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + k * kThreads;
+            if (i >= run.vectors) break;
+#pragma unroll
+            for (int j = 0; j < N; ++j) add(Vec<T>::value(v[k], j), m);
+            my.before += Vec<T>::reach(v[k], i < own_vector ? mine : (i == own_vector ? INFINITY : above));
         }
     }
-    z = block_sum(z, red);
-    zx = block_sum(zx, red);
-    before = block_sum(before, red);
-    const float log_z = logf(z);
+    {
+        const int e = run.edge();
+        if (e >= 0) {
+            const float v = (float)x[e];
+            add(v, raise(v));
+            if (given) my.before += e < token ? v >= mine : v >= above;
+        }
+        if (own_vector >= 0 && own_vector < run.vectors && tid < N) {
+            const int e = run.first + own_vector * N + tid;
+            if (e != token) my.before += (float)x[e] >= (e < token ? mine : above) ? 1 : 0;
+        }
+    }
+    const float my_top = my.m;
+    Sums all = my;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Sums other;
+        other.m = __shfl_xor_sync(0xffffffffu, all.m, o);
+        other.z = __shfl_xor_sync(0xffffffffu, all.z, o);
+        other.zx = __shfl_xor_sync(0xffffffffu, all.zx, o);
+        other.before = __shfl_xor_sync(0xffffffffu, all.before, o);
+        all = joined(all, other);
+    }
+    if (lane == 0) s.warp_sums[warp] = all;
+    __syncthreads();
+    if (tid == 0) {
+        all = s.warp_sums[0];
+        for (int w = 1; w < kWarps; ++w) all = joined(all, s.warp_sums[w]);
+        s.sums = all;
+        s.n_best = 0;
+    }
+    __syncthreads();
+    const bool finite = s.sums.m < INFINITY;   // of this run: no NaN, no +inf
+    if (a.top > 0 && finite) best_of_run(run, my_top, a.top, s);
+    if (parts > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (part == 0) {
+            if (tid < parts) s.list_n[tid] = cluster.map_shared_rank(&s, tid)->n_best;
+            for (int i = tid; i < parts * a.top; i += kThreads) s.lists[i / a.top][i % a.top] = cluster.map_shared_rank(&s, i / a.top)->best[i % a.top];
+            if (tid == 0) {
+                all = s.sums;
+                for (int c = 1; c < parts; ++c) all = joined(all, cluster.map_shared_rank(&s, c)->sums);
+                s.warp_sums[0] = all;
+            }
+        }
+        cluster.sync();
+        if (part != 0) return;
+        all = s.warp_sums[0];
+    } else {
+        __syncthreads();
+        all = s.sums;
+    }
+    const bool bad = !(all.m < INFINITY) || all.m == -INFINITY;
+    const float log_z = logf(all.z);
     if (tid == 0) {
         if (bad) tell(a.status, kDevBadRow);
         if (token >= a.vocab) tell(a.status, kDevBadRange);
-        a.logprobs[row] = token < 0 ? 0.f : (given && !bad ? mine - m - log_z : NAN);
-        a.entropy[row] = bad ? NAN : log_z - zx / z;
-        a.ranks[row] = given && !bad ? (int)before + 1 : 0;
+        a.logprobs[row] = token < 0 ? 0.f : (given && !bad ? mine - all.m - log_z : NAN);
+        a.entropy[row] = bad ? NAN : log_z - all.zx / all.z;
+        a.ranks[row] = given && !bad ? all.before + 1 : 0;
     }
-    float last_v = INFINITY;
-    int last_i = -1;
-    for (int k = 0; k < a.top; ++k) {
-        float v = -INFINITY;
-        int best = INT32_MAX;
-        if (!bad) {
-            for (int i = tid; i < a.vocab; i += kThreads) {
-                const float y = wide(x[i]);
-                if ((y < last_v || (y == last_v && i > last_i)) && (y > v || (y == v && i < best))) v = y, best = i;
+    if (a.top == 0) return;
+    auto put = [&](int rank, uint64_t key) {
+        a.top_tokens[row * a.top + rank] = token_of(key);
+        a.top_logprobs[row * a.top + rank] = value_of(key) - all.m - log_z;
+    };
+    if (bad) {
+        if (tid < a.top) {
+            a.top_tokens[row * a.top + tid] = -1;
+            a.top_logprobs[row * a.top + tid] = NAN;
+        }
+    } else if (parts == 1) {
+        if (tid < s.n_best) put(tid, s.best[tid]);
+    } else {
+        for (int i = tid; i < parts * a.top; i += kThreads) {
+            const int c = i / a.top, r = i - c * a.top;
+            if (r >= s.list_n[c]) continue;
+            const uint64_t key = s.lists[c][r];
+            int rank = r;
+            for (int o = 0; o < parts && rank < a.top; ++o) {
+                if (o == c) continue;
+                int lo = 0, hi = s.list_n[o];   // how many of the other's come first
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (s.lists[o][mid] > key) lo = mid + 1;
+                    else hi = mid;
+                }
+                rank += lo;
             }
+            if (rank < a.top) put(rank, key);
         }
-        block_best(v, best, red, red_i);
-        if (tid == 0) {
-            a.top_tokens[row * a.top + k] = bad ? -1 : best;
-            a.top_logprobs[row * a.top + k] = bad ? NAN : v - m - log_z;
-        }
-        last_v = v, last_i = best;
     }
+}
+
+template <typename T>
+void launch(const LogprobArgs& a, int parts, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.rows * parts));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    cuda_check(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, parts), "kernel launch", __FILE__, __LINE__);
 }
 
 }  // namespace
 
 void launch_token_logprobs(const LogprobArgs& a, cudaStream_t s) {
-    if (a.kind == 0) token_logprobs_kernel<float><<<a.rows, kThreads, 0, s>>>(a);
-    else if (a.kind == 1) token_logprobs_kernel<__half><<<a.rows, kThreads, 0, s>>>(a);
-    else token_logprobs_kernel<__nv_bfloat16><<<a.rows, kThreads, 0, s>>>(a);
-    MK_LAUNCH_CHECK();
+    // as many CTAs to a row as leave each SM two, and each thread a batch of vectors or two
+    const int64_t vectors = (int64_t)a.vocab * (a.kind == 0 ? 4 : 2) / 16;
+    int parts = 1;
+    while (parts < kMaxCluster && (int64_t)a.rows * parts < 2 * 148 && vectors > (int64_t)parts * kThreads * kBatch / 4) parts *= 2;
+    if (a.kind == 0) launch<float>(a, parts, s);
+    else if (a.kind == 1) launch<__half>(a, parts, s);
+    else launch<__nv_bfloat16>(a, parts, s);
 }
 
 }  // namespace mk
