@@ -535,6 +535,443 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
     }
 }
 
+// ---- many items ----------------------------------------------------------------------------------------------------
+//
+// A CTA takes SUBS tiles of 128 (row, query head) items of a lane and KV head and walks the keys they see, or a share of them, in tiles of 64, on the fifth-generation tensor
+// cores: scores Q K^T (128 x 64, f32) into one of two areas of tensor memory per tile of items, O += P V with P as the A operand in tensor memory, over its scores.  Four warps bring
+// 16 keys each: bulk copies of codes and scales into a ring, as f16 numbers into the swizzled rows that the products read.  One warp issues the products; the others hold
+// an item to a thread.  Two tiles of items share the numbers made from the codes (about 90 clocks of issue slots per tile of keys and of items, where exponentials and products take 512 each), and
+// one's softmax runs under the other's products.
+// A code becomes 1024 + c by its bits, c by a subtraction, and low + step c by one fused multiply-add in f16: rounded once, to 11 bits, as a 16-bit cache would hold it; weights are
+// rounded to 11 bits for the second product.  Scales come with a power of two of their own for every 16 keys (multiples of 2^8, so that neighbours share one): scores are multiplied by the
+// keys', weights by the values' over the largest so far where they differ, so that bf16 caches of any range fit f16.  Values of a chunk of eight lie in the order in which the
+// codes' masks give them; queries are laid out alike and results put back in order at the end.  Where a value's scales are not finite they count as zero, and the rows
+// that see the key get NaN for that group at the end: a weight of 0 does not hide NaN from a product.
+constexpr int kItemTile = 128, kKeyTile = 64, kCodeWarps = 4;
+
+template <int D, int BITS, int SUBS>
+struct Many {
+    static constexpr int G = D / kQuantGroup, PANELS = D / 64;
+    static constexpr int Q_PANEL = kItemTile * 128, PANEL = kKeyTile * 128;
+    static constexpr int Q_BYTES = PANELS * Q_PANEL, TILE_BYTES = PANELS * PANEL;
+    static constexpr int K_STAGES = 2, V_STAGES = D == 256 ? 1 : 2;
+    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, RAW = 2 * (CODES + SCALES);
+    static constexpr int FIXED = 1024 + SUBS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + kCodeWarps * 2 * SCALES;
+    static constexpr int MOST = (227 * 1024 - 2048 - FIXED) / (kCodeWarps * RAW), RAW_STAGES = MOST > 6 ? 6 : MOST;
+    static_assert(RAW_STAGES >= 1, "no room for codes");
+    static constexpr size_t SMEM = (size_t)FIXED + (size_t)kCodeWarps * RAW_STAGES * RAW;
+    static constexpr int ITEM_WARPS = 4 * SUBS, MMA_WARP = ITEM_WARPS + kCodeWarps, THREADS = (MMA_WARP + 1) * 32;
+    static constexpr int S_AT = SUBS * D;   // columns of tensor memory: outputs, then scores
+    static_assert(S_AT + SUBS * 2 * kKeyTile <= 512, "tensor memory");
+};
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// The place of value i of eight in their chunk: as the masks give them.
+template <int BITS>
+__host__ __device__ constexpr int place_of(int i) { return BITS == 4 ? (i % 4) * 2 + i / 4 : i / 4 * 4 + (i % 2) * 2 + i % 4 / 2; }
+
+template <typename T, int D, int BITS, int SUBS, int CAP>
+__global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_kernel(const __grid_constant__ QuantAttnArgs a, int chunk_min, int shares, float* part_o, float2* part_ml) {
+    using L = Many<D, BITS, SUBS>;
+    constexpr int G = L::G, RST = L::RAW_STAGES, KST = L::K_STAGES, VST = L::V_STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[kCodeWarps * RST + 2 * KST + 2 * VST + 6 * SUBS + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int4 tile_info[4];                       // of each 16 keys: exponents of keys (low 16 bits, signed) and of values; exponents are multiples of 8, bit 0 tells of scales that are not finite
+    __shared__ uint8_t odd_groups[4][kKeyTile];         // groups of a key's values whose scales are not finite, where the bit is set
+    uint64_t *raw_full = bars, *k_full = bars + kCodeWarps * RST, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
+             *o_done = p_full + 2 * SUBS, *q_full = o_done + 2 * SUBS;
+    uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* ks = qs + SUBS * L::Q_BYTES;
+    uint8_t* vs = ks + KST * L::TILE_BYTES;
+    uint8_t* raws = vs + VST * L::TILE_BYTES;
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(raws + kCodeWarps * RST * L::RAW);   // (step, lowest) as scaled f16 numbers [warp][keys, values][16][G]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const QuantPools& p = a.pools;
+    const int g = a.q_heads / p.kv_heads;
+    const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y;
+    pdl_trigger();
+    const LaneRange at = lane_range(a, lane_id);
+    // the last rows see the most keys: their blocks come first
+    const int item0 = (int)(gridDim.z - 1 - blockIdx.z) * (SUBS * kItemTile), n_items = min(SUBS * kItemTile, at.n * g - item0);
+    if (n_items <= 0) return;
+    const Shares sh = shares_of(a, at, item0, n_items, g, chunk_min, shares);
+    if (share > 0 && share >= sh.used()) return;
+    const int begin = sh.begin + share * sh.chunk, lo = max(sh.lo, begin), hi = min(sh.hi, begin + sh.chunk);
+    const int n_tiles = hi > lo ? (hi - begin + kKeyTile - 1) / kKeyTile : 0, subs = SUBS == 1 || n_items <= kItemTile ? 1 : 2;
+
+    if (tid == 0) {
+        for (int i = 0; i < kCodeWarps * RST; ++i) bar_init(&raw_full[i], 1);
+        for (int i = 0; i < KST; ++i) bar_init(&k_full[i], kCodeWarps), bar_init(&k_empty[i], 1);
+        for (int i = 0; i < VST; ++i) bar_init(&v_full[i], kCodeWarps), bar_init(&v_empty[i], 1);
+        for (int i = 0; i < 2 * SUBS; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kItemTile), bar_init(&o_done[i], 1);
+        bar_init(q_full, kItemTile * subs);
+        bar_init_fence();
+    }
+    if (warp == L::MMA_WARP) tmem_alloc(&tmem_slot, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp >= L::ITEM_WARPS && warp < L::MMA_WARP) {
+        // ---- codes to numbers: 16 keys of each tile
+        const int w = warp - L::ITEM_WARPS;
+        const uint32_t raw = smem_u32(raws + w * RST * L::RAW);
+        uint64_t* full = raw_full + w * RST;
+        uint32_t* pair = pairs + w * 2 * kTile * G;
+        const uint32_t pair_at = smem_u32(pair);
+        const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
+        auto there = [&](int t) { return begin + t * kKeyTile + w * kTile < hi; };
+        auto page_of = [&](int t) {
+            if (t >= n_tiles || !there(t)) return 0;
+            const int32_t page = table[(begin + t * kKeyTile + w * kTile) >> p.bt_shift];
+            if ((uint32_t)page < (uint64_t)p.pages) return page;
+            tell(a.lanes.status, kDevBadPage);
+            return 0;
+        };
+        int page_now = page_of(lane), page_next = n_tiles > 32 ? page_of(32 + lane) : 0;
+        auto load = [&](int t) {
+            if ((t & 31) == 0 && t > 0) {
+                page_now = page_next;
+                page_next = page_of(t + 32 + lane);
+            }
+            const int64_t page = __shfl_sync(0xffffffffu, page_now, t & 31);
+            if (!there(t)) return;
+            const int st = t % RST;
+            const int64_t row = (int64_t)kvh * p.block_tokens + ((begin + t * kKeyTile + w * kTile) & (p.block_tokens - 1));
+            if (lane == 0) bar_expect_tx(&full[st], L::RAW);
+            __syncwarp();
+            if (lane < 4) {   // codes of keys, of values, scales of keys, of values
+                const bool codes = lane < 2, keys = (lane & 1) == 0;
+                const uint8_t* from = codes ? (keys ? p.k_codes : p.v_codes) + page * p.codes_stride + row * L::ROW
+                                            : reinterpret_cast<const uint8_t*>((keys ? p.k_scales : p.v_scales) + page * p.scales_stride + row * G);
+                bulk_load(raw + st * L::RAW + (codes ? lane * L::CODES : 2 * L::CODES + (lane - 2) * L::SCALES), from, codes ? L::CODES : L::SCALES, &full[st]);
+            }
+        };
+#pragma unroll 1
+        for (int t = 0; t < min(RST, n_tiles); ++t) load(t);
+        // eight neighbouring values of a key to a thread
+        auto numbers = [&](uint32_t codes, uint32_t of_pairs, uint8_t* to) {
+            constexpr int CHUNKS = D / 8;
+#pragma unroll 4
+            for (int i = lane; i < kTile * CHUNKS; i += 32) {
+                const int key = i / CHUNKS, c = i - key * CHUNKS;
+                const uint32_t sl = lds<uint32_t>(of_pairs + (key * G + c / 8) * 4);
+                const __half2 both = *reinterpret_cast<const __half2*>(&sl), step = __low2half2(both), low = __high2half2(both), minus = __float2half2_rn(-1024.f);
+                auto number = [&](uint32_t bits, __half2 by) {
+                    bits |= 0x64006400u;
+                    const __half2 y = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&bits), minus), by, low);
+                    return *reinterpret_cast<const uint32_t*>(&y);
+                };
+                uint4 out;
+                if constexpr (BITS == 4) {
+                    const uint32_t x = lds<uint32_t>(codes + i * 4), y = x >> 8;
+                    const __half2 sixteenth = __hmul2(step, __float2half2_rn(0.0625f));   // codes in bits 4 .. 7 are 16 times theirs
+                    out = make_uint4(number(x & 0x000f000fu, step), number(x & 0x00f000f0u, sixteenth), number(y & 0x000f000fu, step), number(y & 0x00f000f0u, sixteenth));
+                } else {
+                    const uint2 x = lds<uint2>(codes + i * 8);
+                    out = make_uint4(number(x.x & 0x00ff00ffu, step), number(x.x >> 8 & 0x00ff00ffu, step), number(x.y & 0x00ff00ffu, step), number(x.y >> 8 & 0x00ff00ffu, step));
+                }
+                *reinterpret_cast<uint4*>(to + (c >> 3) * L::PANEL + (w * kTile + key) * 128 + (((c & 7) ^ (key & 7)) << 4)) = out;
+            }
+        };
+        bool ok = true;
+#pragma unroll 1
+        for (int t = 0; t < n_tiles; ++t) {
+            const int st = t % RST, pos0 = begin + t * kKeyTile + w * kTile;
+            const uint32_t from = raw + st * L::RAW;
+            if (there(t)) {
+                ok = __all_sync(0xffffffffu, bar_wait(&full[st], t / RST & 1));
+                if (!ok) break;
+            }
+            // scales: a key's to a thread, then a value's
+            {
+                const int key = lane & 15, kind = lane >> 4;
+                const bool seen = pos0 + key >= lo && pos0 + key < hi;
+                float2 sl[G];
+                float bound = 0.f;
+                uint32_t odd = 0;
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    sl[j] = seen ? wide_pair<T>(lds<uint32_t>(from + 2 * L::CODES + kind * L::SCALES + (key * G + j) * 4)) : make_float2(0.f, 0.f);
+                    const bool fine = fabsf(sl[j].x) < INFINITY && fabsf(sl[j].y) < INFINITY;
+                    if (fine) bound = fmaxf(bound, fmaxf(fabsf(sl[j].y), fabsf(fmaf(sl[j].x, (float)((1 << BITS) - 1), sl[j].y))));
+                    else odd |= 1u << j;
+                    if (!fine && kind == 1) sl[j] = make_float2(0.f, 0.f);
+                }
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+                // numbers below 2^15; 120 is beyond what f16 or bf16 pools need
+                const int e = bound > 0.f ? min(max((((int)(__float_as_uint(bound) >> 23) - 126 - 15 + 1024 + 7) / 8 - 128) * 8, -120), 120) : -120;
+                const float by = power_of_two(-e);
+#pragma unroll
+                for (int j = 0; j < G; ++j) pair[(kind * kTile + key) * G + j] = narrow_pair<__half>(sl[j].x * by, sl[j].y * by);
+                const bool any_odd = __any_sync(0xffffffffu, kind == 1 && odd != 0);
+                if (any_odd && kind == 1) odd_groups[t & 3][w * kTile + key] = (uint8_t)odd;
+                const int e_values = __shfl_sync(0xffffffffu, e, 16);
+                if (lane == 0) reinterpret_cast<int*>(&tile_info[t & 3])[w] = (e & 0xffff) | (int)((uint32_t)(e_values | (any_odd ? 1 : 0)) << 16);
+                __syncwarp();
+            }
+            ok = __all_sync(0xffffffffu, bar_wait(&k_empty[t % KST], (t / KST & 1) ^ 1));
+            if (!ok) break;
+            numbers(from, pair_at, ks + (t % KST) * L::TILE_BYTES);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&k_full[t % KST]);
+            ok = __all_sync(0xffffffffu, bar_wait(&v_empty[t % VST], (t / VST & 1) ^ 1));
+            if (!ok) break;
+            numbers(from + L::CODES, pair_at + kTile * G * 4, vs + (t % VST) * L::TILE_BYTES);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&v_full[t % VST]);
+            if (t + RST < n_tiles) load(t + RST);
+        }
+        if (!ok) {
+            if (lane == 0) tell(a.lanes.status, kDevWait);
+            for (int st = 0; st < RST; ++st) bar_wait(&full[st], 0), bar_wait(&full[st], 1);   // copies in flight land before the CTA ends
+        }
+    } else if (warp == L::MMA_WARP) {
+        // ---- products
+        if (lane == 0 && n_tiles > 0) {
+            constexpr uint32_t i_scores = f16_idesc(kItemTile, kKeyTile, false), i_out = f16_idesc(kItemTile, D, true);
+            const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
+            auto scores = [&](int t) {
+                if (!bar_wait(&k_full[t % KST], t / KST & 1)) return false;
+                fence_after();
+                const uint64_t k = sw128_desc(k_addr + (t % KST) * L::TILE_BYTES);
+                for (int s = 0; s < subs; ++s) {
+                    const uint64_t q = sw128_desc(q_addr + s * L::Q_BYTES);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                        mma(tmem + L::S_AT + (s * 2 + (t & 1)) * kKeyTile, q + (i >> 2) * (L::Q_PANEL / 16) + (i & 3) * 2, k + (i >> 2) * (L::PANEL / 16) + (i & 3) * 2, i_scores, i > 0);
+                    commit(&s_full[s * 2 + (t & 1)]);
+                }
+                commit(&k_empty[t % KST]);
+                return true;
+            };
+            bool ok = bar_wait(q_full, 0);
+            fence_after();
+            ok = ok && scores(0);
+            for (int t = 0; t < n_tiles && ok; ++t) {
+                // scores of tile t + 1 go to the area that P of tile t - 1 occupied: its product was issued before, and products of one thread run in the order of their issue
+                if (t + 1 < n_tiles) ok = scores(t + 1);
+                ok = ok && bar_wait(&v_full[t % VST], t / VST & 1);
+                const uint64_t v = sw128_desc(v_addr + (t % VST) * L::TILE_BYTES, L::PANEL);
+                for (int s = 0; s < subs && ok; ++s) {
+                    ok = bar_wait(&p_full[s * 2 + (t & 1)], t >> 1 & 1);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t pt = tmem + L::S_AT + (s * 2 + (t & 1)) * kKeyTile;
+#pragma unroll
+                    for (int i = 0; i < kKeyTile / 16; ++i) mma_tmem_a(tmem + s * D, pt + i * 8, v + i * 128, i_out, t > 0 || i > 0);
+                    commit(&o_done[s * 2 + (t & 1)]);
+                }
+                if (ok) commit(&v_empty[t % VST]);
+            }
+            if (!ok) tell(a.lanes.status, kDevWait);
+        }
+    } else if (warp < 4 * subs) {
+        // ---- an item to a thread
+        const int sub = warp >> 2, item = tid, row = item0 + item < at.n * g ? (item0 + item) / g : 0, head = item0 + item - row * g;
+        const bool mine = item < n_items;
+        const float unit = CAP ? a.scale : a.scale * kLog2e;
+        float factor;   // of scores that come from scaled queries
+        {
+            const T* q = static_cast<const T*>(a.q) + (int64_t)(at.first + row) * a.ldq + (kvh * g + head) * D;
+            float top = 0.f;
+            if (mine) {
+#pragma unroll 4
+                for (int c = 0; c < D; c += 8) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(q + c);
+                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 y = wide_pair<T>(u[j]);
+                        top = max3(top, fabsf(y.x), fabsf(y.y));
+                    }
+                }
+            }
+            // the largest becomes 2^14 and a bit, exactly
+            const int e = top > 0.f ? min(max(14 - (int)((__float_as_uint(top) >> 23) - 127), -100), 100) : 0;
+            const float up = power_of_two(e);
+            factor = unit * power_of_two(-e);
+            uint8_t* to = qs + sub * L::Q_BYTES + (item & 127) * 128;
+#pragma unroll 4
+            for (int c = 0; c < D; c += 8) {
+                uint32_t out[4] = {0u, 0u, 0u, 0u};
+                if (mine) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(q + c);
+                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 z = wide_pair<T>(u[j]);
+                        y[place_of<BITS>(2 * j)] = z.x * up;
+                        y[place_of<BITS>(2 * j + 1)] = z.y * up;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) out[j] = narrow_pair<__half>(y[2 * j], y[2 * j + 1]);
+                }
+                *reinterpret_cast<uint4*>(to + (c >> 6) * L::Q_PANEL + ((((c & 63) * 2) ^ ((item & 7) << 4)))) = make_uint4(out[0], out[1], out[2], out[3]);
+            }
+            fence_async_smem();
+            bar_arrive(q_full);
+        }
+        const int pos = at.position + row, see_lo = max(lo, attention_first_key(max(pos, 0), a.window, 0)), see_hi = mine ? min(hi, pos + 1) : 0;
+        // keys that all rows of the tile of items see
+        const int last = min(item0 + n_items, item0 + (sub + 1) * kItemTile) - 1, p0 = at.position + (item0 + sub * kItemTile) / g, p1 = at.position + last / g;
+        const int all_lo = max(lo, attention_first_key(max(p1, 0), a.window, 0)), all_hi = min(hi, p0 + 1);
+        const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), my_o = my + sub * D;
+        const float two_over_cap = CAP ? 2.0f / a.softcap : 0.f;
+        const bool wide_cap = CAP && a.softcap > kCapOfDifference;
+        float m_run = -INFINITY, sum = 0.f;
+        int e_run = -120;
+        uint32_t odd = 0;
+        bool ok = true;
+#pragma unroll 1
+        for (int t = 0; t < n_tiles; ++t) {
+            const int area = sub * 2 + (t & 1);
+            ok = __all_sync(0xffffffffu, bar_wait(&s_full[area], t >> 1 & 1));
+            if (!ok) break;
+            fence_after();
+            const uint32_t s_at = my + L::S_AT + area * kKeyTile;
+            float s[kKeyTile];
+            tmem_ld32(s_at, reinterpret_cast<uint32_t*>(s));
+            tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s) + 32);
+            const int4 info = tile_info[t & 3];
+            const int of[4] = {info.x, info.y, info.z, info.w};
+            const int pos0 = begin + t * kKeyTile;
+            tmem_wait_ld();
+            // neither 0 nor infinite: where it would be, scores are 0 or overflow whatever it is
+            auto unit_of = [&](int info_of) { return fminf(fmaxf(factor * power_of_two((int)(int16_t)info_of), 1e-37f), 3e38f); };
+            float u = unit_of(of[0]);
+            const bool even = (((of[0] ^ of[1]) | (of[0] ^ of[2]) | (of[0] ^ of[3])) & 0xffff) == 0;
+            if (CAP || !even) {   // scores one by one; then they are what is exponentiated
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float ub = unit_of(of[b]);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float v = s[b * 16 + j] * ub;
+                        if (CAP) v = (wide_cap ? capped_wide(v, a.softcap, two_over_cap) : capped(v, a.softcap, two_over_cap)) * kLog2e;
+                        s[b * 16 + j] = v;
+                    }
+                }
+                u = 1.f;
+            }
+            if (pos0 < all_lo || pos0 + kKeyTile > all_hi) {   // uniform: some row does not see the whole tile
+#pragma unroll
+                for (int j = 0; j < kKeyTile; ++j) s[j] = pos0 + j >= see_lo && pos0 + j < see_hi ? s[j] : -INFINITY;
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int j = 4; j < kKeyTile; j += 8) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top[k] = j + k + 4 < kKeyTile ? max3(top[k], s[j + k], s[j + k + 4]) : fmaxf(top[k], s[j + k]);
+            }
+            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * u;
+            // exponents of the values: one for all that came so far
+            const int e_tile = max(max(of[0] >> 19, of[1] >> 19), max(of[2] >> 19, of[3] >> 19)) * 8;
+            const bool e_grow = e_tile > e_run, grow = m_tile > m_run + kSlack;   // also when there was none yet
+            if (__any_sync(0xffffffffu, grow) || e_grow) {
+                const float m_new = grow ? m_tile : m_run;
+                float alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_new);
+                sum *= alpha;
+                m_run = m_new;
+                if (e_grow) {
+                    alpha *= e_run - e_tile < -126 ? 0.f : power_of_two(e_run - e_tile);
+                    e_run = e_tile;
+                }
+                if (t > 0) {
+                    ok = __all_sync(0xffffffffu, bar_wait(&o_done[sub * 2 + (t - 1 & 1)], t - 1 >> 1 & 1));
+                    if (!ok) break;
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(my_o + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                        tmem_st32(my_o + c, o);
+                    }
+                }
+            }
+            const float m_use = m_run == -INFINITY ? 0.f : m_run;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < kKeyTile; ++j) {
+                s[j] = ex2(fmaf(s[j], u, -m_use));
+                part[j & 3] += s[j];
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            if ((of[0] >> 19 << 3) != e_run || (of[1] >> 19 << 3) != e_run || (of[2] >> 19 << 3) != e_run || (of[3] >> 19 << 3) != e_run) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int d = (of[b] >> 19 << 3) - e_run;
+                    const float down = d < -126 ? 0.f : power_of_two(d);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[b * 16 + j] *= down;
+                }
+            }
+            uint32_t w[kKeyTile / 2];
+#pragma unroll
+            for (int j = 0; j < kKeyTile / 2; ++j) w[j] = narrow_pair<__half>(s[2 * j], s[2 * j + 1]);
+            tmem_st32(s_at, w);
+            if ((of[0] | of[1] | of[2] | of[3]) >> 16 & 1) {
+                for (int j = 0; j < kKeyTile; ++j)
+                    if (of[j >> 4] >> 16 & 1 && pos0 + j >= see_lo && pos0 + j < see_hi) odd |= odd_groups[t & 3][j];
+            }
+            tmem_wait_st();
+            fence_before();
+            bar_arrive(&p_full[area]);
+        }
+        if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[sub * 2 + (n_tiles - 1 & 1)], n_tiles - 1 >> 1 & 1));
+        if (!ok && lane == 0) tell(a.lanes.status, kDevWait);
+        fence_after();
+        const float inv = !ok ? NAN : (sum == 0.f ? 0.f : 1.0f / sum), back = power_of_two(e_run);
+        const int64_t out_row = (int64_t)(at.first + row), part_row = share * ((int64_t)a.lanes.total * a.q_heads) + out_row * a.q_heads + kvh * g + head;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            if (n_tiles > 0 && ok) {
+                tmem_ld32(my_o + c, o);
+                tmem_wait_ld();
+            }
+            if (!mine) continue;
+            float x[32];
+            const bool none = sum == 0.f && ok, not_a_number = odd >> (c / kQuantGroup) & 1;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float v = __uint_as_float(o[j / 8 * 8 + place_of<BITS>(j % 8)]);
+                x[j] = none ? 0.f : (not_a_number ? NAN : v * inv * back);
+            }
+            if (shares == 1) {
+                T* to = static_cast<T*>(a.out) + out_row * a.ldo + (kvh * g + head) * D + c;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                    *reinterpret_cast<uint4*>(to + j) = make_uint4(narrow_pair<T>(x[j], x[j + 1]), narrow_pair<T>(x[j + 2], x[j + 3]), narrow_pair<T>(x[j + 4], x[j + 5]), narrow_pair<T>(x[j + 6], x[j + 7]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(part_o + part_row * D + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            }
+        }
+        if (mine && shares > 1) part_ml[part_row] = make_float2(m_run, ok ? sum : NAN);
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == L::MMA_WARP) {
+        fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 // ---- shares joined: a warp to a (row, query head) ----------------------------------------------------------------------
 
 template <typename T, int D>
@@ -587,20 +1024,35 @@ void launch_few(const QuantAttnArgs& a, const QuantAttnPlan& p, float* part_o, f
     MK_LAUNCH_CHECK();
 }
 
+template <typename T, int D, int BITS, int CAP>
+void launch_many(const QuantAttnArgs& a, const QuantAttnPlan& p, float* part_o, float2* part_ml, cudaStream_t s) {
+    constexpr int SUBS = D == 256 ? 1 : 2;
+    using L = Many<D, BITS, SUBS>;
+    auto* kernel = many_items_kernel<T, D, BITS, SUBS, CAP>;
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::SMEM);
+    kernel<<<dim3((unsigned)(a.lanes.lanes * p.shares), (unsigned)a.pools.kv_heads, (unsigned)p.blocks), L::THREADS, L::SMEM, s>>>(a, p.chunk, p.shares, part_o, part_ml);
+    MK_LAUNCH_CHECK();
+}
+
 template <typename T, int D>
 void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s) {
     float* part_o = static_cast<float*>(workspace);
     float2* part_ml = reinterpret_cast<float2*>(part_o + (p.shares > 1 ? p.shares * (int64_t)a.lanes.total * a.q_heads * D : 0));
-    auto run = [&](auto bits, auto nt) {
-        constexpr int B = decltype(bits)::value, N = decltype(nt)::value;
-        a.softcap != 0.f ? launch_few<T, D, B, N, 1>(a, p, part_o, part_ml, s) : launch_few<T, D, B, N, 0>(a, p, part_o, part_ml, s);
-    };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
     using Four = std::integral_constant<int, 4>;
     using Eight = std::integral_constant<int, 8>;
-    if (a.pools.bits == 4) p.items == 8 ? run(Four{}, One{}) : run(Four{}, Two{});
-    else p.items == 8 ? run(Eight{}, One{}) : run(Eight{}, Two{});
+    auto few = [&](auto bits, auto nt) {
+        constexpr int B = decltype(bits)::value, N = decltype(nt)::value;
+        a.softcap != 0.f ? launch_few<T, D, B, N, 1>(a, p, part_o, part_ml, s) : launch_few<T, D, B, N, 0>(a, p, part_o, part_ml, s);
+    };
+    auto many = [&](auto bits) {
+        constexpr int B = decltype(bits)::value;
+        a.softcap != 0.f ? launch_many<T, D, B, 1>(a, p, part_o, part_ml, s) : launch_many<T, D, B, 0>(a, p, part_o, part_ml, s);
+    };
+    if (p.items > 16) a.pools.bits == 4 ? many(Four{}) : many(Eight{});
+    else if (a.pools.bits == 4) p.items == 8 ? few(Four{}, One{}) : few(Four{}, Two{});
+    else p.items == 8 ? few(Eight{}, One{}) : few(Eight{}, Two{});
     if (p.shares > 1) {
         const int64_t rows = (int64_t)a.lanes.rows * a.q_heads;
         launch_pdl(join_kernel<T, D>, dim3((unsigned)a.lanes.lanes, (unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(128), 0, s, a, p.items, p.chunk, p.shares,
@@ -614,13 +1066,13 @@ void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cud
 QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window) {
     QuantAttnPlan p;
     const int64_t items = (int64_t)rows * (q_heads / kv_heads);
-    p.items = items <= 8 ? 8 : 16;
+    p.items = items <= 8 ? 8 : (items <= 16 ? 16 : (d == 256 ? kItemTile : 2 * kItemTile));
     p.blocks = (int)std::max<int64_t>(1, (items + p.items - 1) / p.items);
     const int64_t most = window > 0 ? std::min<int64_t>((int64_t)width * block_tokens, (int64_t)window + rows + 15) : (int64_t)width * block_tokens;
-    p.chunk = 256;
     const int64_t columns = std::max<int64_t>(1, (int64_t)lanes * kv_heads * p.blocks);
-    // as many shares as make six waves of three CTAs on each SM, of 256 keys at least
-    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>((most + p.chunk - 1) / p.chunk, (6 * 3 * kSms + columns - 1) / columns));
+    // few items: as many shares as make six waves of three CTAs on each SM; many: one wave of one
+    p.chunk = 256;
+    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>((most + p.chunk - 1) / p.chunk, ((p.items <= 16 ? 6 * 3 * kSms : kSms) + columns - 1) / columns));
     if (p.shares > 1) p.bytes = (int64_t)p.shares * total * q_heads * ((int64_t)d * 4 + 8);
     return p;
 }
