@@ -122,7 +122,9 @@ QuantAttnPlan checked_quantized_plan(const QuantPools& p, int q_heads, int width
     need(q_heads > 0 && q_heads % p.kv_heads == 0, "mk_k_quantized_attention: q_heads is a multiple of kv_heads");
     need(q_heads / p.kv_heads <= 128, "mk_k_quantized_attention: at most 128 query heads share a KV head");
     need((int64_t)rows * (q_heads / p.kv_heads) <= 4 << 20 && (int64_t)total * q_heads <= INT32_MAX / 4, "mk_k_quantized_attention: too many rows");
-    return quantized_attention_plan(q_heads, p.kv_heads, p.d, p.bits, p.block_tokens, width, lanes, rows, total, window);
+    const QuantAttnPlan plan = quantized_attention_plan(q_heads, p.kv_heads, p.d, p.bits, p.block_tokens, width, lanes, rows, total, window);
+    need((int64_t)lanes * plan.shares <= INT32_MAX / p.kv_heads / plan.blocks, "mk_k_quantized_attention: too many lanes");
+    return plan;
 }
 
 }  // namespace

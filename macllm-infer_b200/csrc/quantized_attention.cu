@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
 // keys', weights by the values' over the largest so far where they differ, so that bf16 caches of any range fit f16.  Values of a chunk of eight lie in the order in which the
 // codes' masks give them; queries are laid out alike and results put back in order at the end.  Where a value's scales are not finite they count as zero, and the rows
 // that see the key get NaN for that group at the end: a weight of 0 does not hide NaN from a product.
-constexpr int kItemTile = 128, kKeyTile = 64, kCodeWarps = 4;
+constexpr int kItemTile = 128, kKeyTile = 64, kCodeWarps = 8;   // four for keys, four for values
 
 template <int D, int BITS, int SUBS>
 struct Many {
@@ -555,34 +555,63 @@ struct Many {
     static constexpr int Q_PANEL = kItemTile * 128, PANEL = kKeyTile * 128;
     static constexpr int Q_BYTES = PANELS * Q_PANEL, TILE_BYTES = PANELS * PANEL;
     static constexpr int K_STAGES = 2, V_STAGES = D == 256 ? 1 : 2;
-    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, RAW = 2 * (CODES + SCALES);
-    static constexpr int FIXED = 1024 + SUBS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + kCodeWarps * 2 * SCALES;
+    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, RAW = CODES + SCALES;
+    static constexpr int FIXED = 1024 + SUBS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + kCodeWarps * SCALES;
     static constexpr int MOST = (227 * 1024 - 2048 - FIXED) / (kCodeWarps * RAW), RAW_STAGES = MOST > 6 ? 6 : MOST;
     static_assert(RAW_STAGES >= 1, "no room for codes");
     static constexpr size_t SMEM = (size_t)FIXED + (size_t)kCodeWarps * RAW_STAGES * RAW;
-    static constexpr int ITEM_WARPS = 4 * SUBS, MMA_WARP = ITEM_WARPS + kCodeWarps, THREADS = (MMA_WARP + 1) * 32;
+    static constexpr int ITEM_WARPS = 4 * SUBS, MMA_WARP = ITEM_WARPS + kCodeWarps, THREADS = (MMA_WARP + 4) * 32;
+    // Twenty warps have 96 registers a thread at launch, 1920 of them a lane of all warps: eight warps of items then take 144, eight of codes keep 72, the last four 40 (1888).
+    static constexpr bool SPLIT_REGISTERS = SUBS == 2;
+    static constexpr int LAUNCH_REGISTERS = 96, ITEM_REGISTERS = 144, CODE_REGISTERS = 72, OTHER_REGISTERS = 40;
+    static_assert(!SPLIT_REGISTERS || ITEM_WARPS * ITEM_REGISTERS + kCodeWarps * CODE_REGISTERS + 4 * OTHER_REGISTERS <= THREADS / 32 * LAUNCH_REGISTERS, "more registers than the launch has");
     static constexpr int S_AT = SUBS * D;   // columns of tensor memory: outputs, then scores
     static_assert(S_AT + SUBS * 2 * kKeyTile <= 512, "tensor memory");
 };
 
+// The exponent under which numbers up to `bound` are below 2^15, a multiple of eight; the one before stays while it leaves them above 2^-9, so that neighbours share one.
+__device__ __forceinline__ int exponent_of(float bound, int before) {
+    const int above = (int)(__float_as_uint(bound) >> 23) - 126;   // bound < 2^above
+    const int e = bound > 0.f ? min(max(((above - 15 + 1024 + 7) / 8 - 128) * 8, -120), 120) : -120;
+    return e <= before && (e >= before - 16 || bound == 0.f) ? before : e;
+}
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
+// The lane with the rank-th most tokens, the first of equals first, among up to kRanked lanes; more lanes keep their order.  All threads of the CTA.
+constexpr int kRanked = 256;
+__device__ __forceinline__ int lane_of_rank(const QuantLanes& l, int rank) {
+    if (l.lanes == 1 || l.lanes > kRanked) return rank;
+    __shared__ int lengths[kRanked], found;
+    const int tid = threadIdx.x;
+    if (tid < l.lanes) lengths[tid] = l.lengths[tid];
+    if (tid == 0) found = rank;
+    __syncthreads();
+    if (tid < l.lanes) {
+        const int mine = lengths[tid];
+        int before = 0;
+        for (int i = 0; i < l.lanes; ++i) before += lengths[i] > mine || (lengths[i] == mine && i < tid) ? 1 : 0;
+        if (before == rank) found = tid;
+    }
+    __syncthreads();
+    return found;
+}
+
 // The place of value i of eight in their chunk: as the masks give them.
 template <int BITS>
 __host__ __device__ constexpr int place_of(int i) { return BITS == 4 ? (i % 4) * 2 + i / 4 : i / 4 * 4 + (i % 2) * 2 + i % 4 / 2; }
 
 template <typename T, int D, int BITS, int SUBS, int CAP>
-__global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_kernel(const __grid_constant__ QuantAttnArgs a, int chunk_min, int shares, float* part_o, float2* part_ml) {
+__global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_kernel(const __grid_constant__ QuantAttnArgs a, int blocks, int chunk_min, int shares, float* part_o, float2* part_ml) {
     using L = Many<D, BITS, SUBS>;
     constexpr int G = L::G, RST = L::RAW_STAGES, KST = L::K_STAGES, VST = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[kCodeWarps * RST + 2 * KST + 2 * VST + 6 * SUBS + 1];
     __shared__ uint32_t tmem_slot;
-    __shared__ int4 tile_info[4];                       // of each 16 keys: exponents of keys (low 16 bits, signed) and of values; exponents are multiples of 8, bit 0 tells of scales that are not finite
+    __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 2; bit 0 tells of values' scales that are not finite
     __shared__ uint8_t odd_groups[4][kKeyTile];         // groups of a key's values whose scales are not finite, where the bit is set
     uint64_t *raw_full = bars, *k_full = bars + kCodeWarps * RST, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
              *o_done = p_full + 2 * SUBS, *q_full = o_done + 2 * SUBS;
@@ -594,11 +623,13 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const QuantPools& p = a.pools;
     const int g = a.q_heads / p.kv_heads;
-    const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y;
+    // the longest lanes come first, and of each the last rows, which see the most keys: what is left at the end is short
+    const int of_lane = p.kv_heads * blocks * shares, rank = blockIdx.x / of_lane, rest = blockIdx.x - rank * of_lane, block = blocks - 1 - rest / (p.kv_heads * shares), kvh = rest / shares % p.kv_heads,
+              share = rest % shares;
     pdl_trigger();
+    const int lane_id = lane_of_rank(a.lanes, rank);
     const LaneRange at = lane_range(a, lane_id);
-    // the last rows see the most keys: their blocks come first
-    const int item0 = (int)(gridDim.z - 1 - blockIdx.z) * (SUBS * kItemTile), n_items = min(SUBS * kItemTile, at.n * g - item0);
+    const int item0 = block * (SUBS * kItemTile), n_items = min(SUBS * kItemTile, at.n * g - item0);
     if (n_items <= 0) return;
     const Shares sh = shares_of(a, at, item0, n_items, g, chunk_min, shares);
     if (share > 0 && share >= sh.used()) return;
@@ -607,8 +638,8 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
 
     if (tid == 0) {
         for (int i = 0; i < kCodeWarps * RST; ++i) bar_init(&raw_full[i], 1);
-        for (int i = 0; i < KST; ++i) bar_init(&k_full[i], kCodeWarps), bar_init(&k_empty[i], 1);
-        for (int i = 0; i < VST; ++i) bar_init(&v_full[i], kCodeWarps), bar_init(&v_empty[i], 1);
+        for (int i = 0; i < KST; ++i) bar_init(&k_full[i], 4), bar_init(&k_empty[i], 1);
+        for (int i = 0; i < VST; ++i) bar_init(&v_full[i], 4), bar_init(&v_empty[i], 1);
         for (int i = 0; i < 2 * SUBS; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kItemTile), bar_init(&o_done[i], 1);
         bar_init(q_full, kItemTile * subs);
         bar_init_fence();
@@ -620,13 +651,16 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     const uint32_t tmem = tmem_slot;
 
     if (warp >= L::ITEM_WARPS && warp < L::MMA_WARP) {
-        // ---- codes to numbers: 16 keys of each tile
-        const int w = warp - L::ITEM_WARPS;
-        const uint32_t raw = smem_u32(raws + w * RST * L::RAW);
-        uint64_t* full = raw_full + w * RST;
-        uint32_t* pair = pairs + w * 2 * kTile * G;
-        const uint32_t pair_at = smem_u32(pair);
+        // ---- codes to numbers: 16 keys, or their values, of each tile
+        if constexpr (L::SPLIT_REGISTERS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::CODE_REGISTERS));
+        const int w = warp & 3, of = warp - L::ITEM_WARPS;
+        const bool keys = of < 4;
+        const uint32_t raw = smem_u32(raws + of * RST * L::RAW);
+        uint64_t* full = raw_full + of * RST;
+        uint32_t* pair = pairs + of * kTile * G;
         const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
+        const uint8_t* codes_of = (keys ? p.k_codes : p.v_codes) + (int64_t)kvh * p.block_tokens * L::ROW;
+        const uint32_t* scales_of = (keys ? p.k_scales : p.v_scales) + (int64_t)kvh * p.block_tokens * G;
         auto there = [&](int t) { return begin + t * kKeyTile + w * kTile < hi; };
         auto page_of = [&](int t) {
             if (t >= n_tiles || !there(t)) return 0;
@@ -642,103 +676,97 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 page_next = page_of(t + 32 + lane);
             }
             const int64_t page = __shfl_sync(0xffffffffu, page_now, t & 31);
-            if (!there(t)) return;
-            const int st = t % RST;
-            const int64_t row = (int64_t)kvh * p.block_tokens + ((begin + t * kKeyTile + w * kTile) & (p.block_tokens - 1));
-            if (lane == 0) bar_expect_tx(&full[st], L::RAW);
-            __syncwarp();
-            if (lane < 4) {   // codes of keys, of values, scales of keys, of values
-                const bool codes = lane < 2, keys = (lane & 1) == 0;
-                const uint8_t* from = codes ? (keys ? p.k_codes : p.v_codes) + page * p.codes_stride + row * L::ROW
-                                            : reinterpret_cast<const uint8_t*>((keys ? p.k_scales : p.v_scales) + page * p.scales_stride + row * G);
-                bulk_load(raw + st * L::RAW + (codes ? lane * L::CODES : 2 * L::CODES + (lane - 2) * L::SCALES), from, codes ? L::CODES : L::SCALES, &full[st]);
-            }
+            if (lane != 0 || !there(t)) return;
+            const int st = t % RST, row = (begin + t * kKeyTile + w * kTile) & (p.block_tokens - 1);
+            bar_expect_tx(&full[st], L::RAW);
+            bulk_load(raw + st * L::RAW, codes_of + page * p.codes_stride + row * L::ROW, L::CODES, &full[st]);
+            bulk_load(raw + st * L::RAW + L::CODES, scales_of + page * p.scales_stride + row * G, L::SCALES, &full[st]);
         };
 #pragma unroll 1
         for (int t = 0; t < min(RST, n_tiles); ++t) load(t);
-        // eight neighbouring values of a key to a thread
-        auto numbers = [&](uint32_t codes, uint32_t of_pairs, uint8_t* to) {
-            constexpr int CHUNKS = D / 8;
-#pragma unroll 4
-            for (int i = lane; i < kTile * CHUNKS; i += 32) {
-                const int key = i / CHUNKS, c = i - key * CHUNKS;
-                const uint32_t sl = lds<uint32_t>(of_pairs + (key * G + c / 8) * 4);
-                const __half2 both = *reinterpret_cast<const __half2*>(&sl), step = __low2half2(both), low = __high2half2(both), minus = __float2half2_rn(-1024.f);
-                auto number = [&](uint32_t bits, __half2 by) {
+        uint64_t *mine_full = keys ? k_full : v_full, *mine_empty = keys ? k_empty : v_empty;
+        const int stages = keys ? KST : VST;
+        uint8_t* tiles = (keys ? ks : vs) + w * kTile * 128;
+        bool ok = true;
+        int st = 0, stage = 0, e = -120;
+        uint32_t full_parity = 0, empty_parity = 1;
+#pragma unroll 1
+        for (int t = 0; t < n_tiles; ++t) {
+            const int pos0 = begin + t * kKeyTile + w * kTile;
+            const uint32_t from = raw + st * L::RAW;
+            if (there(t)) {
+                ok = __all_sync(0xffffffffu, bar_wait(&full[st], full_parity));
+                if (!ok) break;
+            }
+            // scales: a key to a thread, every other group
+            const int key = lane & 15;
+            const bool seen = pos0 + key >= lo && pos0 + key < hi;
+            float2 sl[(G + 1) / 2];
+            float bound = 0.f;
+            uint32_t odd = 0;
+#pragma unroll
+            for (int k = 0; k < (G + 1) / 2; ++k) {
+                const int j = 2 * k + (lane >> 4);
+                sl[k] = seen && j < G ? wide_pair<T>(lds<uint32_t>(from + L::CODES + (key * G + j) * 4)) : make_float2(0.f, 0.f);
+                const bool fine = fabsf(sl[k].x) < INFINITY && fabsf(sl[k].y) < INFINITY;
+                if (fine) bound = fmaxf(bound, fmaxf(fabsf(sl[k].y), fabsf(fmaf(sl[k].x, (float)((1 << BITS) - 1), sl[k].y))));
+                else odd |= 1u << j;
+                if (!fine && !keys) sl[k] = make_float2(0.f, 0.f);
+            }
+            bound = warp_max(bound);
+            e = exponent_of(bound, e);
+            const float by = power_of_two(-e);
+#pragma unroll
+            for (int k = 0; k < (G + 1) / 2; ++k)
+                if (2 * k + (lane >> 4) < G) pair[key * G + 2 * k + (lane >> 4)] = narrow_pair<__half>(sl[k].x * by, sl[k].y * by);
+            const bool any_odd = __any_sync(0xffffffffu, !keys && odd != 0);
+            ok = __all_sync(0xffffffffu, bar_wait(&mine_empty[stage], empty_parity));
+            if (!ok) break;
+            if (any_odd) {
+                odd |= __shfl_xor_sync(0xffffffffu, odd, 16);
+                if (lane < 16) odd_groups[t & 3][w * kTile + key] = (uint8_t)odd;
+            }
+            if (lane == 0) reinterpret_cast<int*>(keys ? &k_info[t & 3] : &v_info[t & 3])[w] = e * 2 | (any_odd ? 1 : 0);
+            __syncwarp();
+            // eight neighbouring values of a key to a thread
+            constexpr int CHUNKS = D / 8, EACH = kTile * CHUNKS / 32;
+            uint8_t* to = tiles + stage * L::TILE_BYTES;
+#pragma unroll 8
+            for (int k = 0; k < EACH; ++k) {
+                const int i = lane + k * 32, row = i / CHUNKS, c = i - row * CHUNKS;
+                const uint32_t both = pair[row * G + c / 8];
+                const __half2 step = __low2half2(*reinterpret_cast<const __half2*>(&both)), low = __high2half2(*reinterpret_cast<const __half2*>(&both));
+                auto number = [&](uint32_t bits, __half2 by_step) {   // 1024 + c, c, low + step c
                     bits |= 0x64006400u;
-                    const __half2 y = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&bits), minus), by, low);
+                    const __half2 y = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(-1024.f)), by_step, low);
                     return *reinterpret_cast<const uint32_t*>(&y);
                 };
                 uint4 out;
                 if constexpr (BITS == 4) {
-                    const uint32_t x = lds<uint32_t>(codes + i * 4), y = x >> 8;
+                    const uint32_t x = lds<uint32_t>(from + i * 4), y = x >> 8;
                     const __half2 sixteenth = __hmul2(step, __float2half2_rn(0.0625f));   // codes in bits 4 .. 7 are 16 times theirs
                     out = make_uint4(number(x & 0x000f000fu, step), number(x & 0x00f000f0u, sixteenth), number(y & 0x000f000fu, step), number(y & 0x00f000f0u, sixteenth));
                 } else {
-                    const uint2 x = lds<uint2>(codes + i * 8);
+                    const uint2 x = lds<uint2>(from + i * 8);
                     out = make_uint4(number(x.x & 0x00ff00ffu, step), number(x.x >> 8 & 0x00ff00ffu, step), number(x.y & 0x00ff00ffu, step), number(x.y >> 8 & 0x00ff00ffu, step));
                 }
-                *reinterpret_cast<uint4*>(to + (c >> 3) * L::PANEL + (w * kTile + key) * 128 + (((c & 7) ^ (key & 7)) << 4)) = out;
+                *reinterpret_cast<uint4*>(to + (c >> 3) * L::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = out;
             }
-        };
-        bool ok = true;
-#pragma unroll 1
-        for (int t = 0; t < n_tiles; ++t) {
-            const int st = t % RST, pos0 = begin + t * kKeyTile + w * kTile;
-            const uint32_t from = raw + st * L::RAW;
-            if (there(t)) {
-                ok = __all_sync(0xffffffffu, bar_wait(&full[st], t / RST & 1));
-                if (!ok) break;
-            }
-            // scales: a key's to a thread, then a value's
-            {
-                const int key = lane & 15, kind = lane >> 4;
-                const bool seen = pos0 + key >= lo && pos0 + key < hi;
-                float2 sl[G];
-                float bound = 0.f;
-                uint32_t odd = 0;
-#pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    sl[j] = seen ? wide_pair<T>(lds<uint32_t>(from + 2 * L::CODES + kind * L::SCALES + (key * G + j) * 4)) : make_float2(0.f, 0.f);
-                    const bool fine = fabsf(sl[j].x) < INFINITY && fabsf(sl[j].y) < INFINITY;
-                    if (fine) bound = fmaxf(bound, fmaxf(fabsf(sl[j].y), fabsf(fmaf(sl[j].x, (float)((1 << BITS) - 1), sl[j].y))));
-                    else odd |= 1u << j;
-                    if (!fine && kind == 1) sl[j] = make_float2(0.f, 0.f);
-                }
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
-                // numbers below 2^15; 120 is beyond what f16 or bf16 pools need
-                const int e = bound > 0.f ? min(max((((int)(__float_as_uint(bound) >> 23) - 126 - 15 + 1024 + 7) / 8 - 128) * 8, -120), 120) : -120;
-                const float by = power_of_two(-e);
-#pragma unroll
-                for (int j = 0; j < G; ++j) pair[(kind * kTile + key) * G + j] = narrow_pair<__half>(sl[j].x * by, sl[j].y * by);
-                const bool any_odd = __any_sync(0xffffffffu, kind == 1 && odd != 0);
-                if (any_odd && kind == 1) odd_groups[t & 3][w * kTile + key] = (uint8_t)odd;
-                const int e_values = __shfl_sync(0xffffffffu, e, 16);
-                if (lane == 0) reinterpret_cast<int*>(&tile_info[t & 3])[w] = (e & 0xffff) | (int)((uint32_t)(e_values | (any_odd ? 1 : 0)) << 16);
-                __syncwarp();
-            }
-            ok = __all_sync(0xffffffffu, bar_wait(&k_empty[t % KST], (t / KST & 1) ^ 1));
-            if (!ok) break;
-            numbers(from, pair_at, ks + (t % KST) * L::TILE_BYTES);
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) bar_arrive(&k_full[t % KST]);
-            ok = __all_sync(0xffffffffu, bar_wait(&v_empty[t % VST], (t / VST & 1) ^ 1));
-            if (!ok) break;
-            numbers(from + L::CODES, pair_at + kTile * G * 4, vs + (t % VST) * L::TILE_BYTES);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) bar_arrive(&v_full[t % VST]);
+            if (lane == 0) bar_arrive(&mine_full[stage]);
             if (t + RST < n_tiles) load(t + RST);
+            if (++st == RST) st = 0, full_parity ^= 1;
+            if (++stage == stages) stage = 0, empty_parity ^= 1;
         }
         if (!ok) {
             if (lane == 0) tell(a.lanes.status, kDevWait);
-            for (int st = 0; st < RST; ++st) bar_wait(&full[st], 0), bar_wait(&full[st], 1);   // copies in flight land before the CTA ends
+            for (int i = 0; i < RST; ++i) bar_wait(&full[i], 0), bar_wait(&full[i], 1);   // copies in flight land before the CTA ends
         }
-    } else if (warp == L::MMA_WARP) {
+    } else if (warp >= L::MMA_WARP) {
         // ---- products
-        if (lane == 0 && n_tiles > 0) {
+        if constexpr (L::SPLIT_REGISTERS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::OTHER_REGISTERS));
+        if (warp == L::MMA_WARP && lane == 0 && n_tiles > 0) {
             constexpr uint32_t i_scores = f16_idesc(kItemTile, kKeyTile, false), i_out = f16_idesc(kItemTile, D, true);
             const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
             auto scores = [&](int t) {
@@ -778,6 +806,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         }
     } else if (warp < 4 * subs) {
         // ---- an item to a thread
+        if constexpr (L::SPLIT_REGISTERS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::ITEM_REGISTERS));
         const int sub = warp >> 2, item = tid, row = item0 + item < at.n * g ? (item0 + item) / g : 0, head = item0 + item - row * g;
         const bool mine = item < n_items;
         const float unit = CAP ? a.scale : a.scale * kLog2e;
@@ -844,14 +873,14 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
             float s[kKeyTile];
             tmem_ld32(s_at, reinterpret_cast<uint32_t*>(s));
             tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s) + 32);
-            const int4 info = tile_info[t & 3];
-            const int of[4] = {info.x, info.y, info.z, info.w};
+            const int4 ki = k_info[t & 3];
+            const int of[4] = {ki.x, ki.y, ki.z, ki.w};
             const int pos0 = begin + t * kKeyTile;
             tmem_wait_ld();
             // neither 0 nor infinite: where it would be, scores are 0 or overflow whatever it is
-            auto unit_of = [&](int info_of) { return fminf(fmaxf(factor * power_of_two((int)(int16_t)info_of), 1e-37f), 3e38f); };
+            auto unit_of = [&](int info_of) { return fminf(fmaxf(factor * power_of_two(info_of >> 1), 1e-37f), 3e38f); };
             float u = unit_of(of[0]);
-            const bool even = (((of[0] ^ of[1]) | (of[0] ^ of[2]) | (of[0] ^ of[3])) & 0xffff) == 0;
+            const bool even = of[0] == of[1] && of[0] == of[2] && of[0] == of[3];
             if (CAP || !even) {   // scores one by one; then they are what is exponentiated
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
@@ -877,31 +906,11 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
             }
             const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * u;
             // exponents of the values: one for all that came so far
-            const int e_tile = max(max(of[0] >> 19, of[1] >> 19), max(of[2] >> 19, of[3] >> 19)) * 8;
-            const bool e_grow = e_tile > e_run, grow = m_tile > m_run + kSlack;   // also when there was none yet
-            if (__any_sync(0xffffffffu, grow) || e_grow) {
-                const float m_new = grow ? m_tile : m_run;
-                float alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_new);
+            float alpha = 1.f;
+            if (m_tile > m_run + kSlack) {   // also when there was none yet
+                alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_tile);
                 sum *= alpha;
-                m_run = m_new;
-                if (e_grow) {
-                    alpha *= e_run - e_tile < -126 ? 0.f : power_of_two(e_run - e_tile);
-                    e_run = e_tile;
-                }
-                if (t > 0) {
-                    ok = __all_sync(0xffffffffu, bar_wait(&o_done[sub * 2 + (t - 1 & 1)], t - 1 >> 1 & 1));
-                    if (!ok) break;
-                    fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(my_o + c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                        tmem_st32(my_o + c, o);
-                    }
-                }
+                m_run = m_tile;
             }
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             float part[4] = {0.f, 0.f, 0.f, 0.f};
@@ -911,10 +920,33 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 part[j & 3] += s[j];
             }
             sum += (part[0] + part[1]) + (part[2] + part[3]);
-            if ((of[0] >> 19 << 3) != e_run || (of[1] >> 19 << 3) != e_run || (of[2] >> 19 << 3) != e_run || (of[3] >> 19 << 3) != e_run) {
+            // exponents of the values: the largest so far for all
+            ok = __all_sync(0xffffffffu, bar_wait(&v_full[t % VST], t / VST & 1));
+            if (!ok) break;
+            const int4 vi = v_info[t & 3];
+            const int ev[4] = {vi.x, vi.y, vi.z, vi.w}, e_tile = max(max(ev[0] >> 1, ev[1] >> 1), max(ev[2] >> 1, ev[3] >> 1));
+            if (e_tile > e_run) {
+                alpha *= e_run - e_tile < -126 ? 0.f : power_of_two(e_run - e_tile);
+                e_run = e_tile;
+            }
+            if (t > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                ok = __all_sync(0xffffffffu, bar_wait(&o_done[sub * 2 + (t - 1 & 1)], t - 1 >> 1 & 1));
+                if (!ok) break;
+                fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(my_o + c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                    tmem_st32(my_o + c, o);
+                }
+            }
+            if (ev[0] >> 1 != e_run || ev[1] >> 1 != e_run || ev[2] >> 1 != e_run || ev[3] >> 1 != e_run) {
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const int d = (of[b] >> 19 << 3) - e_run;
+                    const int d = (ev[b] >> 1) - e_run;
                     const float down = d < -126 ? 0.f : power_of_two(d);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) s[b * 16 + j] *= down;
@@ -924,9 +956,9 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
 #pragma unroll
             for (int j = 0; j < kKeyTile / 2; ++j) w[j] = narrow_pair<__half>(s[2 * j], s[2 * j + 1]);
             tmem_st32(s_at, w);
-            if ((of[0] | of[1] | of[2] | of[3]) >> 16 & 1) {
+            if ((ev[0] | ev[1] | ev[2] | ev[3]) & 1) {
                 for (int j = 0; j < kKeyTile; ++j)
-                    if (of[j >> 4] >> 16 & 1 && pos0 + j >= see_lo && pos0 + j < see_hi) odd |= odd_groups[t & 3][j];
+                    if (ev[j >> 4] & 1 && pos0 + j >= see_lo && pos0 + j < see_hi) odd |= odd_groups[t & 3][j];
             }
             tmem_wait_st();
             fence_before();
@@ -1030,7 +1062,15 @@ void launch_many(const QuantAttnArgs& a, const QuantAttnPlan& p, float* part_o, 
     using L = Many<D, BITS, SUBS>;
     auto* kernel = many_items_kernel<T, D, BITS, SUBS, CAP>;
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::SMEM);
-    kernel<<<dim3((unsigned)(a.lanes.lanes * p.shares), (unsigned)a.pools.kv_heads, (unsigned)p.blocks), L::THREADS, L::SMEM, s>>>(a, p.chunk, p.shares, part_o, part_ml);
+    if constexpr (L::SPLIT_REGISTERS) {   // warps that ask for more registers than the launch has would wait for good
+        static const int registers = [&] {
+            cudaFuncAttributes at{};
+            cuda_check(cudaFuncGetAttributes(&at, kernel), "function attributes", __FILE__, __LINE__);
+            return at.numRegs;
+        }();
+        if (registers < L::LAUNCH_REGISTERS) throw std::runtime_error("quantized attention: the kernel was built with fewer registers than its warps share out");
+    }
+    kernel<<<(unsigned)(a.lanes.lanes * p.shares * a.pools.kv_heads * p.blocks), L::THREADS, L::SMEM, s>>>(a, p.blocks, p.chunk, p.shares, part_o, part_ml);
     MK_LAUNCH_CHECK();
 }
 
