@@ -118,6 +118,11 @@ __device__ __forceinline__ V lds(uint32_t at) {
     else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
     return v;
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // The key of a tile that row r of a product stands for: with neighbours swapped in every other pair, the rows that a load takes at once lie on both halves of the banks.
 __device__ __forceinline__ int key_of(int r) { return r ^ (r >> 1 & 1); }
 
@@ -556,7 +561,7 @@ struct Many {
     static constexpr int Q_BYTES = PANELS * Q_PANEL, TILE_BYTES = PANELS * PANEL;
     static constexpr int K_STAGES = 2, V_STAGES = D == 256 ? 1 : 2;
     static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, RAW = CODES + SCALES;
-    static constexpr int FIXED = 1024 + SUBS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + kCodeWarps * SCALES;
+    static constexpr int FIXED = 1024 + SUBS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + kCodeWarps * kTile * G * 16;
     static constexpr int MOST = (227 * 1024 - 2048 - FIXED) / (kCodeWarps * RAW), RAW_STAGES = MOST > 6 ? 6 : MOST;
     static_assert(RAW_STAGES >= 1, "no room for codes");
     static constexpr size_t SMEM = (size_t)FIXED + (size_t)kCodeWarps * RAW_STAGES * RAW;
@@ -575,12 +580,8 @@ __device__ __forceinline__ int exponent_of(float bound, int before) {
     const int e = bound > 0.f ? min(max(((above - 15 + 1024 + 7) / 8 - 128) * 8, -120), 120) : -120;
     return e <= before && (e >= before - 16 || bound == 0.f) ? before : e;
 }
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
 // The lane with the rank-th most tokens, the first of equals first, among up to kRanked lanes; more lanes keep their order.  All threads of the CTA.
 constexpr int kRanked = 256;
 __device__ __forceinline__ int lane_of_rank(const QuantLanes& l, int rank) {
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     using L = Many<D, BITS, SUBS>;
     constexpr int G = L::G, RST = L::RAW_STAGES, KST = L::K_STAGES, VST = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[kCodeWarps * RST + 2 * KST + 2 * VST + 6 * SUBS + 1];
+    __shared__ uint64_t bars[kCodeWarps * RST + 2 * KST + 2 * VST + 7 * SUBS];
     __shared__ uint32_t tmem_slot;
     __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 2; bit 0 tells of values' scales that are not finite
     __shared__ uint8_t odd_groups[4][kKeyTile];         // groups of a key's values whose scales are not finite, where the bit is set
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     uint8_t* ks = qs + SUBS * L::Q_BYTES;
     uint8_t* vs = ks + KST * L::TILE_BYTES;
     uint8_t* raws = vs + VST * L::TILE_BYTES;
-    uint32_t* pairs = reinterpret_cast<uint32_t*>(raws + kCodeWarps * RST * L::RAW);   // (step, lowest) as scaled f16 numbers [warp][keys, values][16][G]
+    uint4* pairs = reinterpret_cast<uint4*>(raws + kCodeWarps * RST * L::RAW);   // steps and lowest values as scaled f16 numbers [warp][16][G]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const QuantPools& p = a.pools;
     const int g = a.q_heads / p.kv_heads;
@@ -638,10 +639,10 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
 
     if (tid == 0) {
         for (int i = 0; i < kCodeWarps * RST; ++i) bar_init(&raw_full[i], 1);
-        for (int i = 0; i < KST; ++i) bar_init(&k_full[i], 4), bar_init(&k_empty[i], 1);
-        for (int i = 0; i < VST; ++i) bar_init(&v_full[i], 4), bar_init(&v_empty[i], 1);
+        for (int i = 0; i < KST; ++i) bar_init(&k_full[i], 4), bar_init(&k_empty[i], subs);
+        for (int i = 0; i < VST; ++i) bar_init(&v_full[i], 4), bar_init(&v_empty[i], subs);
         for (int i = 0; i < 2 * SUBS; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kItemTile), bar_init(&o_done[i], 1);
-        bar_init(q_full, kItemTile * subs);
+        for (int i = 0; i < SUBS; ++i) bar_init(&q_full[i], kItemTile);
         bar_init_fence();
     }
     if (warp == L::MMA_WARP) tmem_alloc(&tmem_slot, 512);
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         const bool keys = of < 4;
         const uint32_t raw = smem_u32(raws + of * RST * L::RAW);
         uint64_t* full = raw_full + of * RST;
-        uint32_t* pair = pairs + of * kTile * G;
+        uint4* pair = pairs + of * kTile * G;
         const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
         const uint8_t* codes_of = (keys ? p.k_codes : p.v_codes) + (int64_t)kvh * p.block_tokens * L::ROW;
         const uint32_t* scales_of = (keys ? p.k_scales : p.v_scales) + (int64_t)kvh * p.block_tokens * G;
@@ -689,6 +690,8 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         uint8_t* tiles = (keys ? ks : vs) + w * kTile * 128;
         bool ok = true;
         int st = 0, stage = 0, e = -120;
+        float by = power_of_two(120);
+        uint32_t most = 0, least = 1;   // bounds for which the exponent stays
         uint32_t full_parity = 0, empty_parity = 1;
 #pragma unroll 1
         for (int t = 0; t < n_tiles; ++t) {
@@ -702,24 +705,41 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
             const int key = lane & 15;
             const bool seen = pos0 + key >= lo && pos0 + key < hi;
             float2 sl[(G + 1) / 2];
-            float bound = 0.f;
-            uint32_t odd = 0;
+            uint32_t bound = 0;   // of the numbers' absolute values, as bits: what is not finite is above all others
 #pragma unroll
             for (int k = 0; k < (G + 1) / 2; ++k) {
                 const int j = 2 * k + (lane >> 4);
                 sl[k] = seen && j < G ? wide_pair<T>(lds<uint32_t>(from + L::CODES + (key * G + j) * 4)) : make_float2(0.f, 0.f);
-                const bool fine = fabsf(sl[k].x) < INFINITY && fabsf(sl[k].y) < INFINITY;
-                if (fine) bound = fmaxf(bound, fmaxf(fabsf(sl[k].y), fabsf(fmaf(sl[k].x, (float)((1 << BITS) - 1), sl[k].y))));
-                else odd |= 1u << j;
-                if (!fine && !keys) sl[k] = make_float2(0.f, 0.f);
+                bound = max(bound, __float_as_uint(max_nan(fabsf(sl[k].y), fabsf(fmaf(sl[k].x, (float)((1 << BITS) - 1), sl[k].y)))));
             }
-            bound = warp_max(bound);
-            e = exponent_of(bound, e);
-            const float by = power_of_two(-e);
+            bound = __reduce_max_sync(0xffffffffu, bound);
+            uint32_t odd = 0;
+            if (bound > most || bound < least) {
+                if (bound >= 0x7f800000u) {   // the largest of the finite ones; values whose scales are not count as 0
+                    float fine_bound = 0.f;
 #pragma unroll
-            for (int k = 0; k < (G + 1) / 2; ++k)
-                if (2 * k + (lane >> 4) < G) pair[key * G + 2 * k + (lane >> 4)] = narrow_pair<__half>(sl[k].x * by, sl[k].y * by);
-            const bool any_odd = __any_sync(0xffffffffu, !keys && odd != 0);
+                    for (int k = 0; k < (G + 1) / 2; ++k) {
+                        const float b = max_nan(fabsf(sl[k].y), fabsf(fmaf(sl[k].x, (float)((1 << BITS) - 1), sl[k].y)));
+                        if (b < INFINITY) fine_bound = fmaxf(fine_bound, b);
+                        else odd |= 1u << (2 * k + (lane >> 4));
+                        if (!(b < INFINITY) && !keys) sl[k] = make_float2(0.f, 0.f);
+                    }
+                    bound = __reduce_max_sync(0xffffffffu, __float_as_uint(fine_bound));
+                }
+                e = exponent_of(__uint_as_float(bound), e);
+                by = power_of_two(-e);
+                most = min((uint32_t)(127 + 15 + e) << 23, 0x7f7fffffu);
+                least = (uint32_t)max(127 + 15 - 24 + e, 1) << 23;
+            }
+#pragma unroll
+            for (int k = 0; k < (G + 1) / 2; ++k) {
+                const int j = 2 * k + (lane >> 4);
+                if (j >= G) continue;
+                // step, a sixteenth of it (codes in bits 4 .. 7 are 16 times theirs) and lowest value, twice each
+                const __half2 step = __float2half2_rn(sl[k].x * by), part = __hmul2(step, __float2half2_rn(0.0625f)), low = __float2half2_rn(sl[k].y * by);
+                pair[key * G + j] = make_uint4(*reinterpret_cast<const uint32_t*>(&step), *reinterpret_cast<const uint32_t*>(&part), *reinterpret_cast<const uint32_t*>(&low), 0u);
+            }
+            const bool any_odd = !keys && __any_sync(0xffffffffu, odd != 0);
             ok = __all_sync(0xffffffffu, bar_wait(&mine_empty[stage], empty_parity));
             if (!ok) break;
             if (any_odd) {
@@ -734,17 +754,16 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
 #pragma unroll 8
             for (int k = 0; k < EACH; ++k) {
                 const int i = lane + k * 32, row = i / CHUNKS, c = i - row * CHUNKS;
-                const uint32_t both = pair[row * G + c / 8];
-                const __half2 step = __low2half2(*reinterpret_cast<const __half2*>(&both)), low = __high2half2(*reinterpret_cast<const __half2*>(&both));
+                const uint4 scale = pair[row * G + c / 8];
+                const __half2 step = as_half2(scale.x), sixteenth = as_half2(scale.y), low = as_half2(scale.z);
                 auto number = [&](uint32_t bits, __half2 by_step) {   // 1024 + c, c, low + step c
                     bits |= 0x64006400u;
-                    const __half2 y = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(-1024.f)), by_step, low);
+                    const __half2 y = __hfma2(__hadd2(as_half2(bits), __float2half2_rn(-1024.f)), by_step, low);
                     return *reinterpret_cast<const uint32_t*>(&y);
                 };
                 uint4 out;
                 if constexpr (BITS == 4) {
                     const uint32_t x = lds<uint32_t>(from + i * 4), y = x >> 8;
-                    const __half2 sixteenth = __hmul2(step, __float2half2_rn(0.0625f));   // codes in bits 4 .. 7 are 16 times theirs
                     out = make_uint4(number(x & 0x000f000fu, step), number(x & 0x00f000f0u, sixteenth), number(y & 0x000f000fu, step), number(y & 0x00f000f0u, sixteenth));
                 } else {
                     const uint2 x = lds<uint2>(from + i * 8);
@@ -766,43 +785,51 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     } else if (warp >= L::MMA_WARP) {
         // ---- products
         if constexpr (L::SPLIT_REGISTERS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::OTHER_REGISTERS));
-        if (warp == L::MMA_WARP && lane == 0 && n_tiles > 0) {
+        const int sub = warp - L::MMA_WARP;   // a warp for each tile of items: the whole of it waits, one thread issues
+        if (sub < subs && n_tiles > 0) {
             constexpr uint32_t i_scores = f16_idesc(kItemTile, kKeyTile, false), i_out = f16_idesc(kItemTile, D, true);
-            const uint32_t q_addr = smem_u32(qs), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
+            const bool issues = elect_one();
+            const uint64_t q = sw128_desc(smem_u32(qs) + sub * L::Q_BYTES), k0 = sw128_desc(smem_u32(ks)), v0 = sw128_desc(smem_u32(vs), L::PANEL);
+            const uint32_t s_base = tmem + L::S_AT + sub * 2 * kKeyTile, o_base = tmem + sub * D;
             auto scores = [&](int t) {
-                if (!bar_wait(&k_full[t % KST], t / KST & 1)) return false;
+                const int st = t % KST;
+                if (!__all_sync(0xffffffffu, bar_wait(&k_full[st], t / KST & 1))) return false;
                 fence_after();
-                const uint64_t k = sw128_desc(k_addr + (t % KST) * L::TILE_BYTES);
-                for (int s = 0; s < subs; ++s) {
-                    const uint64_t q = sw128_desc(q_addr + s * L::Q_BYTES);
+                if (issues) {
+                    const uint64_t k = k0 + st * (L::TILE_BYTES / 16);
+                    const uint32_t to = s_base + (t & 1) * kKeyTile;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        mma(tmem + L::S_AT + (s * 2 + (t & 1)) * kKeyTile, q + (i >> 2) * (L::Q_PANEL / 16) + (i & 3) * 2, k + (i >> 2) * (L::PANEL / 16) + (i & 3) * 2, i_scores, i > 0);
-                    commit(&s_full[s * 2 + (t & 1)]);
+                    for (int i = 0; i < D / 16; ++i) mma(to, q + (i >> 2) * (L::Q_PANEL / 16) + (i & 3) * 2, k + (i >> 2) * (L::PANEL / 16) + (i & 3) * 2, i_scores, i > 0);
+                    commit(&s_full[sub * 2 + (t & 1)]);
+                    commit(&k_empty[st]);
                 }
-                commit(&k_empty[t % KST]);
+                __syncwarp();
                 return true;
             };
-            bool ok = bar_wait(q_full, 0);
+            bool ok = __all_sync(0xffffffffu, bar_wait(&q_full[sub], 0));
             fence_after();
             ok = ok && scores(0);
             for (int t = 0; t < n_tiles && ok; ++t) {
                 // scores of tile t + 1 go to the area that P of tile t - 1 occupied: its product was issued before, and products of one thread run in the order of their issue
-                if (t + 1 < n_tiles) ok = scores(t + 1);
-                ok = ok && bar_wait(&v_full[t % VST], t / VST & 1);
-                const uint64_t v = sw128_desc(v_addr + (t % VST) * L::TILE_BYTES, L::PANEL);
-                for (int s = 0; s < subs && ok; ++s) {
-                    ok = bar_wait(&p_full[s * 2 + (t & 1)], t >> 1 & 1);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t pt = tmem + L::S_AT + (s * 2 + (t & 1)) * kKeyTile;
-#pragma unroll
-                    for (int i = 0; i < kKeyTile / 16; ++i) mma_tmem_a(tmem + s * D, pt + i * 8, v + i * 128, i_out, t > 0 || i > 0);
-                    commit(&o_done[s * 2 + (t & 1)]);
+                if (t + 1 < n_tiles && !scores(t + 1)) {
+                    ok = false;
+                    break;
                 }
-                if (ok) commit(&v_empty[t % VST]);
+                const int st = t % VST;
+                ok = __all_sync(0xffffffffu, bar_wait(&v_full[st], t / VST & 1) && bar_wait(&p_full[sub * 2 + (t & 1)], t >> 1 & 1));
+                if (!ok) break;
+                fence_after();
+                if (issues) {
+                    const uint64_t v = v0 + st * (L::TILE_BYTES / 16);
+                    const uint32_t from = s_base + (t & 1) * kKeyTile;
+#pragma unroll
+                    for (int i = 0; i < kKeyTile / 16; ++i) mma_tmem_a(o_base, from + i * 8, v + i * 128, i_out, t > 0 || i > 0);
+                    commit(&o_done[sub * 2 + (t & 1)]);
+                    commit(&v_empty[st]);
+                }
+                __syncwarp();
             }
-            if (!ok) tell(a.lanes.status, kDevWait);
+            if (!ok && lane == 0) tell(a.lanes.status, kDevWait);
         }
     } else if (warp < 4 * subs) {
         // ---- an item to a thread
@@ -850,7 +877,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 *reinterpret_cast<uint4*>(to + (c >> 6) * L::Q_PANEL + ((((c & 63) * 2) ^ ((item & 7) << 4)))) = make_uint4(out[0], out[1], out[2], out[3]);
             }
             fence_async_smem();
-            bar_arrive(q_full);
+            bar_arrive(&q_full[sub]);
         }
         const int pos = at.position + row, see_lo = max(lo, attention_first_key(max(pos, 0), a.window, 0)), see_hi = mine ? min(hi, pos + 1) : 0;
         // keys that all rows of the tile of items see

@@ -5,6 +5,7 @@
 // c_i stands for low + step c_i.  low is one of the values, so it needs no rounding; the step's is 2^-11 (f16) or 2^-8 (bf16) of it at most and moves no value by more than
 // L times that, and since the codes are made with the rounded step they are the nearest ones under it.  A group with a value, or a range, that is not finite reads as NaN throughout.
 #include "quantized_kv.h"
+#include "attention_math.cuh"
 #include <algorithm>
 
 namespace mk {
@@ -37,17 +38,6 @@ struct Two<__nv_bfloat16> {
     }
     static constexpr float largest = 3.3895313892515355e38f;
 };
-// Minimum and maximum that are NaN where either is.
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float y;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
 
 // The lane of row t, by a whole warp: the last one whose rows do not begin behind t, 32 of them looked at in each turn.  Whatever cu holds, the index is a lane's.
 __device__ __forceinline__ int lane_of_row(const QuantLanes& a, int t) {

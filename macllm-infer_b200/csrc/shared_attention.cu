@@ -24,11 +24,6 @@ using namespace umma;
 
 constexpr int kSms = 148;   // calls are cut without a device, for a B200
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
 template <typename T>
 struct Pair;
 template <>

@@ -10,6 +10,7 @@
 // looked at again (in L2), and the candidates are ranked by counting.  Where too many reach it - thousands of equal logits, or most of them masked - a radix select over (value, token) finds the
 // top-th key exactly, in up to seven more passes.  The leader of a cluster merges the sorted lists by binary search.
 #include "token_logprobs.h"
+#include "attention_math.cuh"
 #include <cuda_bf16.h>
 #include <cooperative_groups.h>
 #include <algorithm>
@@ -24,20 +25,9 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBatch = 8;             // vectors of a thread on their way together
 constexpr int kCandidates = 512;
 constexpr int kMaxCluster = 8;
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tell(int32_t* status, int bit) {
     if (status != nullptr) atomicOr(status, bit);
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
 }
 
 // Numbers as unsigned ones of the same order (no NaN; both zeros are one).
