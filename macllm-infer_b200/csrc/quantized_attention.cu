@@ -560,11 +560,9 @@ struct Many {
     static constexpr int Q_PANEL = kItemTile * 128, PANEL = kKeyTile * 128;
     static constexpr int Q_BYTES = PANELS * Q_PANEL, TILE_BYTES = PANELS * PANEL;
     static constexpr int K_STAGES = 2, V_STAGES = D == 256 ? 1 : 2;
-    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, RAW = CODES + SCALES;
-    static constexpr int FIXED = 1024 + SUBS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + kCodeWarps * kTile * G * 16;
-    static constexpr int MOST = (227 * 1024 - 2048 - FIXED) / (kCodeWarps * RAW), RAW_STAGES = MOST > 6 ? 6 : MOST;
-    static_assert(RAW_STAGES >= 1, "no room for codes");
-    static constexpr size_t SMEM = (size_t)FIXED + (size_t)kCodeWarps * RAW_STAGES * RAW;
+    static constexpr size_t SMEM = 1024 + (size_t)SUBS * Q_BYTES + (size_t)(K_STAGES + V_STAGES) * TILE_BYTES;
+    // a warp's codes of 16 keys in pieces of 16 bytes: PASSES to a thread, each CHUNKS times eight numbers
+    static constexpr int ROW = D * BITS / 8, PIECES = ROW / 16, PASSES = ROW / 32, CHUNKS = 16 / BITS;
     static constexpr int ITEM_WARPS = 4 * SUBS, MMA_WARP = ITEM_WARPS + kCodeWarps, THREADS = (MMA_WARP + 4) * 32;
     // Twenty warps have 96 registers a thread at launch, 1920 of them a lane of all warps: eight warps of items then take 144, eight of codes keep 72, the last four 40 (1888).
     static constexpr bool SPLIT_REGISTERS = SUBS == 2;
@@ -608,19 +606,17 @@ __host__ __device__ constexpr int place_of(int i) { return BITS == 4 ? (i % 4) *
 template <typename T, int D, int BITS, int SUBS, int CAP>
 __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_kernel(const __grid_constant__ QuantAttnArgs a, int blocks, int chunk_min, int shares, float* part_o, float2* part_ml) {
     using L = Many<D, BITS, SUBS>;
-    constexpr int G = L::G, RST = L::RAW_STAGES, KST = L::K_STAGES, VST = L::V_STAGES;
+    constexpr int G = L::G, KST = L::K_STAGES, VST = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[kCodeWarps * RST + 2 * KST + 2 * VST + 7 * SUBS];
+    __shared__ uint64_t bars[2 * KST + 2 * VST + 7 * SUBS];
     __shared__ uint32_t tmem_slot;
     __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 2; bit 0 tells of values' scales that are not finite
-    __shared__ uint8_t odd_groups[4][kKeyTile];         // groups of a key's values whose scales are not finite, where the bit is set
-    uint64_t *raw_full = bars, *k_full = bars + kCodeWarps * RST, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
+    __shared__ uint32_t odd_groups[4][kKeyTile];        // groups of a key's values whose scales are not finite, where the bit is set
+    uint64_t *k_full = bars, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
              *o_done = p_full + 2 * SUBS, *q_full = o_done + 2 * SUBS;
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ks = qs + SUBS * L::Q_BYTES;
     uint8_t* vs = ks + KST * L::TILE_BYTES;
-    uint8_t* raws = vs + VST * L::TILE_BYTES;
-    uint4* pairs = reinterpret_cast<uint4*>(raws + kCodeWarps * RST * L::RAW);   // steps and lowest values as scaled f16 numbers [warp][16][G]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const QuantPools& p = a.pools;
     const int g = a.q_heads / p.kv_heads;
@@ -638,7 +634,6 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     const int n_tiles = hi > lo ? (hi - begin + kKeyTile - 1) / kKeyTile : 0, subs = SUBS == 1 || n_items <= kItemTile ? 1 : 2;
 
     if (tid == 0) {
-        for (int i = 0; i < kCodeWarps * RST; ++i) bar_init(&raw_full[i], 1);
         for (int i = 0; i < KST; ++i) bar_init(&k_full[i], 4), bar_init(&k_empty[i], subs);
         for (int i = 0; i < VST; ++i) bar_init(&v_full[i], 4), bar_init(&v_empty[i], subs);
         for (int i = 0; i < 2 * SUBS; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kItemTile), bar_init(&o_done[i], 1);
@@ -654,75 +649,79 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     if (warp >= L::ITEM_WARPS && warp < L::MMA_WARP) {
         // ---- codes to numbers: 16 keys, or their values, of each tile
         if constexpr (L::SPLIT_REGISTERS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::CODE_REGISTERS));
-        const int w = warp & 3, of = warp - L::ITEM_WARPS;
-        const bool keys = of < 4;
-        const uint32_t raw = smem_u32(raws + of * RST * L::RAW);
-        uint64_t* full = raw_full + of * RST;
-        uint4* pair = pairs + of * kTile * G;
+        const int w = warp & 3;
+        const bool keys = warp - L::ITEM_WARPS < 4;
         const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
         const uint8_t* codes_of = (keys ? p.k_codes : p.v_codes) + (int64_t)kvh * p.block_tokens * L::ROW;
         const uint32_t* scales_of = (keys ? p.k_scales : p.v_scales) + (int64_t)kvh * p.block_tokens * G;
-        auto there = [&](int t) { return begin + t * kKeyTile + w * kTile < hi; };
+        auto there = [&](int t) { return t < n_tiles && begin + t * kKeyTile + w * kTile < hi; };
         auto page_of = [&](int t) {
-            if (t >= n_tiles || !there(t)) return 0;
+            if (!there(t)) return 0;
             const int32_t page = table[(begin + t * kKeyTile + w * kTile) >> p.bt_shift];
             if ((uint32_t)page < (uint64_t)p.pages) return page;
             tell(a.lanes.status, kDevBadPage);
             return 0;
         };
         int page_now = page_of(lane), page_next = n_tiles > 32 ? page_of(32 + lane) : 0;
-        auto load = [&](int t) {
+        // A thread's pieces: eight threads that store at once have two pieces, 64 bytes of numbers apart, of four keys, whose chunks lie on eight different groups of banks.
+        auto key_of_pass = [&](int i) { return (lane >> 1 & 3) + ((lane >> 3) + 4 * i) / (L::PIECES / 2) * 4; };
+        auto piece_of_pass = [&](int i) {
+            const int rest = ((lane >> 3) + 4 * i) % (L::PIECES / 2);
+            return BITS == 4 ? (lane & 1) + 2 * rest : (lane & 1) * 2 + (rest & 1) + 4 * (rest >> 1);
+        };
+        struct Raw {
+            uint4 codes[L::PASSES];
+            uint32_t scales[L::PASSES];
+        };
+        auto load = [&](int t, Raw& r) {
             if ((t & 31) == 0 && t > 0) {
                 page_now = page_next;
                 page_next = page_of(t + 32 + lane);
             }
             const int64_t page = __shfl_sync(0xffffffffu, page_now, t & 31);
-            if (lane != 0 || !there(t)) return;
-            const int st = t % RST, row = (begin + t * kKeyTile + w * kTile) & (p.block_tokens - 1);
-            bar_expect_tx(&full[st], L::RAW);
-            bulk_load(raw + st * L::RAW, codes_of + page * p.codes_stride + row * L::ROW, L::CODES, &full[st]);
-            bulk_load(raw + st * L::RAW + L::CODES, scales_of + page * p.scales_stride + row * G, L::SCALES, &full[st]);
+            if (!there(t)) {
+                r = Raw{};
+                return;
+            }
+            const int row = (begin + t * kKeyTile + w * kTile) & (p.block_tokens - 1);
+            const uint8_t* codes = codes_of + page * p.codes_stride + row * L::ROW;
+            const uint32_t* scales = scales_of + page * p.scales_stride + row * G;
+#pragma unroll
+            for (int i = 0; i < L::PASSES; ++i) {
+                const int key = key_of_pass(i), piece = piece_of_pass(i);
+                r.codes[i] = *reinterpret_cast<const uint4*>(codes + key * L::ROW + piece * 16);
+                r.scales[i] = scales[key * G + piece * 8 * L::CHUNKS / kQuantGroup];
+            }
         };
-#pragma unroll 1
-        for (int t = 0; t < min(RST, n_tiles); ++t) load(t);
         uint64_t *mine_full = keys ? k_full : v_full, *mine_empty = keys ? k_empty : v_empty;
         const int stages = keys ? KST : VST;
         uint8_t* tiles = (keys ? ks : vs) + w * kTile * 128;
-        bool ok = true;
-        int st = 0, stage = 0, e = -120;
+        int stage = 0, e = -120;
+        uint32_t empty_parity = 1;
         float by = power_of_two(120);
-        uint32_t most = 0, least = 1;   // bounds for which the exponent stays
-        uint32_t full_parity = 0, empty_parity = 1;
-#pragma unroll 1
-        for (int t = 0; t < n_tiles; ++t) {
+        uint32_t most = 0, least = 1;   // bounds, as bits, for which the exponent stays
+        auto make = [&](int t, const Raw& r) {
             const int pos0 = begin + t * kKeyTile + w * kTile;
-            const uint32_t from = raw + st * L::RAW;
-            if (there(t)) {
-                ok = __all_sync(0xffffffffu, bar_wait(&full[st], full_parity));
-                if (!ok) break;
-            }
-            // scales: a key to a thread, every other group
-            const int key = lane & 15;
-            const bool seen = pos0 + key >= lo && pos0 + key < hi;
-            float2 sl[(G + 1) / 2];
+            float2 sl[L::PASSES];
             uint32_t bound = 0;   // of the numbers' absolute values, as bits: what is not finite is above all others
+            auto bound_of = [](float2 v) { return max_nan(fabsf(v.y), fabsf(fmaf(v.x, (float)((1 << BITS) - 1), v.y))); };
 #pragma unroll
-            for (int k = 0; k < (G + 1) / 2; ++k) {
-                const int j = 2 * k + (lane >> 4);
-                sl[k] = seen && j < G ? wide_pair<T>(lds<uint32_t>(from + L::CODES + (key * G + j) * 4)) : make_float2(0.f, 0.f);
-                bound = max(bound, __float_as_uint(max_nan(fabsf(sl[k].y), fabsf(fmaf(sl[k].x, (float)((1 << BITS) - 1), sl[k].y)))));
+            for (int i = 0; i < L::PASSES; ++i) {
+                const int pos = pos0 + key_of_pass(i);
+                sl[i] = pos >= lo && pos < hi ? wide_pair<T>(r.scales[i]) : make_float2(0.f, 0.f);
+                bound = max(bound, __float_as_uint(bound_of(sl[i])));
             }
             bound = __reduce_max_sync(0xffffffffu, bound);
-            uint32_t odd = 0;
+            uint32_t odd = 0;   // passes
             if (bound > most || bound < least) {
                 if (bound >= 0x7f800000u) {   // the largest of the finite ones; values whose scales are not count as 0
                     float fine_bound = 0.f;
 #pragma unroll
-                    for (int k = 0; k < (G + 1) / 2; ++k) {
-                        const float b = max_nan(fabsf(sl[k].y), fabsf(fmaf(sl[k].x, (float)((1 << BITS) - 1), sl[k].y)));
+                    for (int i = 0; i < L::PASSES; ++i) {
+                        const float b = bound_of(sl[i]);
                         if (b < INFINITY) fine_bound = fmaxf(fine_bound, b);
-                        else odd |= 1u << (2 * k + (lane >> 4));
-                        if (!(b < INFINITY) && !keys) sl[k] = make_float2(0.f, 0.f);
+                        else odd |= 1u << i;
+                        if (!(b < INFINITY) && !keys) sl[i] = make_float2(0.f, 0.f);
                     }
                     bound = __reduce_max_sync(0xffffffffu, __float_as_uint(fine_bound));
                 }
@@ -731,57 +730,63 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 most = min((uint32_t)(127 + 15 + e) << 23, 0x7f7fffffu);
                 least = (uint32_t)max(127 + 15 - 24 + e, 1) << 23;
             }
-#pragma unroll
-            for (int k = 0; k < (G + 1) / 2; ++k) {
-                const int j = 2 * k + (lane >> 4);
-                if (j >= G) continue;
-                // step, a sixteenth of it (codes in bits 4 .. 7 are 16 times theirs) and lowest value, twice each
-                const __half2 step = __float2half2_rn(sl[k].x * by), part = __hmul2(step, __float2half2_rn(0.0625f)), low = __float2half2_rn(sl[k].y * by);
-                pair[key * G + j] = make_uint4(*reinterpret_cast<const uint32_t*>(&step), *reinterpret_cast<const uint32_t*>(&part), *reinterpret_cast<const uint32_t*>(&low), 0u);
-            }
             const bool any_odd = !keys && __any_sync(0xffffffffu, odd != 0);
-            ok = __all_sync(0xffffffffu, bar_wait(&mine_empty[stage], empty_parity));
-            if (!ok) break;
+            if (!__all_sync(0xffffffffu, bar_wait(&mine_empty[stage], empty_parity))) return false;
             if (any_odd) {
-                odd |= __shfl_xor_sync(0xffffffffu, odd, 16);
-                if (lane < 16) odd_groups[t & 3][w * kTile + key] = (uint8_t)odd;
+                if (lane < kTile) odd_groups[t & 3][w * kTile + lane] = 0;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < L::PASSES; ++i)
+                    if (odd >> i & 1) atomicOr(&odd_groups[t & 3][w * kTile + key_of_pass(i)], 1u << (piece_of_pass(i) * 8 * L::CHUNKS / kQuantGroup));
             }
             if (lane == 0) reinterpret_cast<int*>(keys ? &k_info[t & 3] : &v_info[t & 3])[w] = e * 2 | (any_odd ? 1 : 0);
-            __syncwarp();
-            // eight neighbouring values of a key to a thread
-            constexpr int CHUNKS = D / 8, EACH = kTile * CHUNKS / 32;
             uint8_t* to = tiles + stage * L::TILE_BYTES;
-#pragma unroll 8
-            for (int k = 0; k < EACH; ++k) {
-                const int i = lane + k * 32, row = i / CHUNKS, c = i - row * CHUNKS;
-                const uint4 scale = pair[row * G + c / 8];
-                const __half2 step = as_half2(scale.x), sixteenth = as_half2(scale.y), low = as_half2(scale.z);
+#pragma unroll
+            for (int i = 0; i < L::PASSES; ++i) {
+                const __half2 step = __float2half2_rn(sl[i].x * by), part = __hmul2(step, __float2half2_rn(0.0625f)), low = __float2half2_rn(sl[i].y * by);   // codes in bits 4 .. 7 are 16 times theirs
+                const uint32_t words[4] = {r.codes[i].x, r.codes[i].y, r.codes[i].z, r.codes[i].w};
                 auto number = [&](uint32_t bits, __half2 by_step) {   // 1024 + c, c, low + step c
                     bits |= 0x64006400u;
                     const __half2 y = __hfma2(__hadd2(as_half2(bits), __float2half2_rn(-1024.f)), by_step, low);
                     return *reinterpret_cast<const uint32_t*>(&y);
                 };
-                uint4 out;
-                if constexpr (BITS == 4) {
-                    const uint32_t x = lds<uint32_t>(from + i * 4), y = x >> 8;
-                    out = make_uint4(number(x & 0x000f000fu, step), number(x & 0x00f000f0u, sixteenth), number(y & 0x000f000fu, step), number(y & 0x00f000f0u, sixteenth));
-                } else {
-                    const uint2 x = lds<uint2>(from + i * 8);
-                    out = make_uint4(number(x.x & 0x00ff00ffu, step), number(x.x >> 8 & 0x00ff00ffu, step), number(x.y & 0x00ff00ffu, step), number(x.y >> 8 & 0x00ff00ffu, step));
+                const int key = key_of_pass(i), chunk0 = piece_of_pass(i) * L::CHUNKS;
+                uint8_t* row = to + (chunk0 >> 3) * L::PANEL + key * 128;
+#pragma unroll
+                for (int j = 0; j < L::CHUNKS; ++j) {
+                    uint4 out;
+                    if constexpr (BITS == 4) {
+                        const uint32_t x = words[j], y = x >> 8;
+                        out = make_uint4(number(x & 0x000f000fu, step), number(x & 0x00f000f0u, part), number(y & 0x000f000fu, step), number(y & 0x00f000f0u, part));
+                    } else {
+                        const uint32_t x = words[2 * j], y = words[2 * j + 1];
+                        out = make_uint4(number(x & 0x00ff00ffu, step), number(x >> 8 & 0x00ff00ffu, step), number(y & 0x00ff00ffu, step), number(y >> 8 & 0x00ff00ffu, step));
+                    }
+                    *reinterpret_cast<uint4*>(row + (((chunk0 + j & 7) ^ (key & 7)) << 4)) = out;
                 }
-                *reinterpret_cast<uint4*>(to + (c >> 3) * L::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = out;
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) bar_arrive(&mine_full[stage]);
-            if (t + RST < n_tiles) load(t + RST);
-            if (++st == RST) st = 0, full_parity ^= 1;
             if (++stage == stages) stage = 0, empty_parity ^= 1;
+            return true;
+        };
+        // two tiles on their way
+        Raw even, uneven;
+        load(0, even);
+        load(1, uneven);
+        bool ok = true;
+#pragma unroll 1
+        for (int t = 0; t < n_tiles; t += 2) {
+            ok = make(t, even);
+            if (!ok) break;
+            load(t + 2, even);
+            if (t + 1 == n_tiles) break;
+            ok = make(t + 1, uneven);
+            if (!ok) break;
+            load(t + 3, uneven);
         }
-        if (!ok) {
-            if (lane == 0) tell(a.lanes.status, kDevWait);
-            for (int i = 0; i < RST; ++i) bar_wait(&full[i], 0), bar_wait(&full[i], 1);   // copies in flight land before the CTA ends
-        }
+        if (!ok && lane == 0) tell(a.lanes.status, kDevWait);
     } else if (warp >= L::MMA_WARP) {
         // ---- products
         if constexpr (L::SPLIT_REGISTERS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::OTHER_REGISTERS));
