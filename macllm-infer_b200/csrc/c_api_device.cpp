@@ -123,7 +123,7 @@ QuantAttnPlan checked_quantized_plan(const QuantPools& p, int q_heads, int width
     need(q_heads / p.kv_heads <= 128, "mk_k_quantized_attention: at most 128 query heads share a KV head");
     need((int64_t)rows * (q_heads / p.kv_heads) <= 4 << 20 && (int64_t)total * q_heads <= INT32_MAX / 4, "mk_k_quantized_attention: too many rows");
     const QuantAttnPlan plan = quantized_attention_plan(q_heads, p.kv_heads, p.d, p.bits, p.block_tokens, width, lanes, rows, total, window);
-    need((int64_t)lanes * plan.shares <= INT32_MAX / p.kv_heads / plan.blocks, "mk_k_quantized_attention: too many lanes");
+    need(plan.slots <= INT32_MAX / p.kv_heads / plan.blocks, "mk_k_quantized_attention: too many lanes");
     return plan;
 }
 

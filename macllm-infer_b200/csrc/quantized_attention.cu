@@ -59,26 +59,66 @@ __device__ __forceinline__ LaneRange lane_range(const QuantAttnArgs& a, int lane
     return r;
 }
 
-// The keys of a block of items, and how they are shared out: `chunk` of them from `begin` on to each share, the last of which ends at `hi`.
+// How the lanes' keys are shared out among CTAs.  With `want` CTAs for each KV head and block of items, a lane of n keys gets n / max(least, total / want) shares, rounded up: as many as its
+// part of all keys asks for.  The lengths are the device's, so every CTA finds its lane and share by itself, from the number of its slot; a lane's slots follow one another.
+struct Piece {
+    int lane, share, shares, slot;   // the lane's first slot; lane < 0: none
+};
+// Of slot `slot`, or of the whole of lane `of_lane` where that is not negative; by a whole warp.
+__device__ __forceinline__ Piece piece_of(const QuantAttnArgs& a, const QuantAttnCut& c, int slot, int of_lane) {
+    const int n_lanes = a.lanes.lanes, lane = threadIdx.x & 31;
+    if (!c.split) return Piece{of_lane >= 0 ? of_lane : slot, 0, 1, 0};
+    auto keys_of = [&](int i) {
+        if (i >= n_lanes) return 0;
+        const int n = min(max(a.lanes.lengths[i], 0), a.lanes.width << a.pools.bt_shift);
+        return a.window > 0 ? min(n, c.window_keys) : n;
+    };
+    const int mine = keys_of(lane);
+    float total = (float)mine;
+    for (int i = 32 + lane; i < n_lanes; i += 32) total += (float)keys_of(i);
+    const float per_share = 1.0f / fmaxf((float)c.least, warp_sum(total) / c.want);
+    int before = 0;
+    for (int i0 = 0; i0 < n_lanes; i0 += 32) {
+        const int n = i0 == 0 ? mine : keys_of(i0 + lane), shares = i0 + lane < n_lanes ? max(1, (int)ceilf((float)n * per_share - 1e-3f)) : 0;   // roundings make no share
+        int upto = shares;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        upto += before;
+        const uint32_t hit = __ballot_sync(0xffffffffu, of_lane >= 0 ? i0 + lane == of_lane : slot < upto);
+        if (hit != 0) {
+            const int at = __ffs(hit) - 1, its = __shfl_sync(0xffffffffu, shares, at), first = __shfl_sync(0xffffffffu, upto, at) - its;
+            return Piece{i0 + at, of_lane >= 0 ? 0 : slot - first, its, first};
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return Piece{-1, 0, 1, 0};
+}
+
+// The keys of a block of items: `chunk` of them from `begin` on to each share, the last of which ends at `hi`.
 struct Shares {
     int lo, hi, begin, chunk;
     __device__ __forceinline__ int used() const { return hi > lo ? (hi - begin + chunk - 1) / chunk : 0; }
 };
-__device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRange& at, int item0, int n_items, int g, int chunk_min, int shares) {
+__device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRange& at, int item0, int n_items, int g, int shares) {
     const int p0 = at.position + item0 / g, p1 = at.position + (item0 + n_items - 1) / g;
     Shares s;
     s.lo = attention_first_key(max(p0, 0), a.window, 0);
     s.hi = min(p1 + 1, at.keys);
     s.begin = s.lo / 16 * 16;
-    const int each = s.hi > s.begin ? (s.hi - s.begin + shares - 1) / shares : 0;
-    s.chunk = max(chunk_min, (each + 15) / 16 * 16);
+    const int n = max(s.hi - s.begin, 0);
+    s.chunk = shares == 1 ? (n + 15) / 16 * 16 : ((n + shares - 1) / shares + 15) / 16 * 16;
+    s.chunk = max(s.chunk, 16);
     return s;
 }
 
 // ---- few items -----------------------------------------------------------------------------------------------------
 //
-// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks tiles of 16 keys, whose codes and scales bulk copies
-// bring into a ring of its own.  Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
+// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks tiles of 16 keys, whose codes and scales come from
+// memory into the registers of the threads that multiply them: those of the next tile's keys once this one's scores are there, its values' once this one's output is.
+// Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
 // are the f16 number c 2^-24 (a subnormal, which the tensor cores take in full), so that it costs a mask and half a shift.  With steps and lowest values of the groups
 //   q . k = sum_g step_g (q_g . c_g) + low_g sum(q_g),   o = sum_j (w_j step_jg) c_j + sum_j w_j low_jg,
 // steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
@@ -89,15 +129,18 @@ constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;            // base-2 logarithm
 constexpr float kWeightScale = 128.f;    // weights up to 2^kSlack, times this, times a step over the largest: below f16's largest
 
+// CTAs on an SM: what registers allow.
+__host__ __device__ constexpr int few_ctas(int d, int nt) { return d == 64 ? (nt == 1 ? 5 : 4) : (d == 128 && nt == 1 ? 4 : 2); }
+
 template <int D, int BITS, int NT>
 struct Few {
     static constexpr int G = D / kQuantGroup, ITEMS = NT * 8;
-    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, STAGE = 2 * (CODES + SCALES);
-    static constexpr int STAGES = STAGE <= 2400 ? 8 : 4;
+    static constexpr int ROW = D * BITS / 8;
     static constexpr int OP = D + 4;                                     // pitch of a warp's results, in floats
-    static constexpr int RING = ((STAGES * STAGE > ITEMS * OP * 4 ? STAGES * STAGE : ITEMS * OP * 4) + 127) / 128 * 128;
+    static constexpr int RESULTS = ITEMS * OP * 4;
     static constexpr int QP = D + 8;
-    static constexpr size_t SMEM = 128 + (size_t)kWarps * RING + (size_t)ITEMS * QP * 2;
+    static constexpr size_t SMEM = (size_t)kWarps * RESULTS + (size_t)ITEMS * QP * 2;
+    static constexpr int CTAS = few_ctas(D, NT);
     static constexpr bool Q_IN_REGISTERS = NT * D <= 256;
 };
 
@@ -106,52 +149,35 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// A copy of a multiple of 16 bytes, both addresses multiples of 16.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-template <typename V>
-__device__ __forceinline__ V lds(uint32_t at) {
-    V v;
-    if constexpr (sizeof(V) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
-    else if constexpr (sizeof(V) == 8) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-    else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
-}
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// The key of a tile that row r of a product stands for: with neighbours swapped in every other pair, the rows that a load takes at once lie on both halves of the banks.
-__device__ __forceinline__ int key_of(int r) { return r ^ (r >> 1 & 1); }
-
 template <typename T, int D, int BITS, int NT, int CAP>
-__global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_constant__ QuantAttnArgs a, int chunk_min, int shares, float* part_o, float2* part_ml) {
+__global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items_kernel(const __grid_constant__ QuantAttnArgs a, const __grid_constant__ QuantAttnCut cut, float* part_o, float2* part_ml) {
     using L = Few<D, BITS, NT>;
     constexpr int G = L::G;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[kWarps * L::STAGES];
+    extern __shared__ __align__(16) uint8_t results[];   // of the warps; queries behind them
     __shared__ float item_factor[L::ITEMS], item_sums[L::ITEMS][G];
     __shared__ float2 warp_ml[kWarps][L::ITEMS];
-    uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
-    __half* qs = reinterpret_cast<__half*>(rings + kWarps * L::RING);
+    __half* qs = reinterpret_cast<__half*>(results + kWarps * L::RESULTS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
-    const int lane_id = blockIdx.x / shares, share = blockIdx.x - lane_id * shares, kvh = blockIdx.y;
     const QuantPools& p = a.pools;
-    const int g = a.q_heads / p.kv_heads;
+    const int g = a.q_heads / p.kv_heads, slot = blockIdx.x, kvh = blockIdx.y;
     pdl_trigger();
+    const Piece piece = piece_of(a, cut, slot, -1);
+    if (piece.lane < 0) return;
+    const int lane_id = piece.lane, share = piece.share, shares = piece.shares;
     const LaneRange at = lane_range(a, lane_id);
     const int item0 = blockIdx.z * L::ITEMS, n_items = min(L::ITEMS, at.n * g - item0);
     if (n_items <= 0) return;
-    const Shares sh = shares_of(a, at, item0, n_items, g, chunk_min, shares);
+    const Shares sh = shares_of(a, at, item0, n_items, g, shares);
     if (share > 0 && share >= sh.used()) return;
     const int lo = max(sh.lo, sh.begin + share * sh.chunk), hi = min(sh.hi, sh.begin + (share + 1) * sh.chunk);
     const int begin = sh.begin + share * sh.chunk, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0;
     const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
 
-    const uint32_t ring = smem_u32(rings + warp * L::RING);
-    uint64_t* full = bars + warp * L::STAGES;
     const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
     // the page numbers of 32 tiles sit in the warp's threads, those of the next 32 on their way
     auto page_of = [&](int i) {
@@ -162,30 +188,54 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
         return 0;
     };
     int page_now = page_of(lane), page_next = my_tiles > 32 ? page_of(32 + lane) : 0;
-    auto load_tile = [&](int i) {   // the whole warp; one copy to each of four threads
+    // a thread's keys are rows gid and gid + 8 of a tile, its values those of keys 2 tq, 2 tq + 1 and the same eight further on
+    uint32_t kc[G][2][BITS / 2], vc[G][4][BITS / 4], kp[2][G], vp[2][G];   // codes, and pairs (step, lowest) of keys gid and gid + 8
+    auto load_words = [](auto& to, const void* from) {
+        constexpr int N = sizeof(to) / 4;
+        if constexpr (N == 1) {
+            to[0] = *static_cast<const uint32_t*>(from);
+        } else if constexpr (N == 2) {
+            const uint2 x = *static_cast<const uint2*>(from);
+            to[0] = x.x, to[1] = x.y;
+        } else {
+            const uint4 x = *static_cast<const uint4*>(from);
+            to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+        }
+    };
+    int64_t code_at = 0, pair_at = 0;   // of the tile that is loaded next
+    auto find = [&](int i) {            // the whole warp
         if ((i & 31) == 0 && i > 0) {
             page_now = page_next;
             page_next = page_of(i + 32 + lane);
         }
         const int64_t page = __shfl_sync(0xffffffffu, page_now, i & 31);
-        const int st = i & (L::STAGES - 1);
-        const int64_t row = (int64_t)kvh * p.block_tokens + ((begin + (warp + kWarps * i) * kTile) & (p.block_tokens - 1));
-        if (lane == 0) bar_expect_tx(&full[st], L::STAGE);
-        __syncwarp();
-        if (lane < 4) {   // codes of keys, of values, scales of keys, of values
-            const bool codes = lane < 2, keys = (lane & 1) == 0;
-            const uint8_t* from = codes ? (keys ? p.k_codes : p.v_codes) + page * p.codes_stride + row * L::ROW
-                                        : reinterpret_cast<const uint8_t*>((keys ? p.k_scales : p.v_scales) + page * p.scales_stride + row * G);
-            bulk_load(ring + st * L::STAGE + (codes ? lane * L::CODES : 2 * L::CODES + (lane - 2) * L::SCALES), from, codes ? L::CODES : L::SCALES, &full[st]);
+        const int row = kvh * p.block_tokens + ((begin + (warp + kWarps * i) * kTile) & (p.block_tokens - 1));
+        code_at = page * p.codes_stride + row * L::ROW;
+        pair_at = page * p.scales_stride + row * G;
+    };
+    auto load_keys = [&] {
+        const uint8_t* from = p.k_codes + code_at + gid * L::ROW + tq * (BITS * 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) load_words(kc[j][h], from + h * 8 * L::ROW + j * (kQuantGroup * BITS / 8));
+            load_words(kp[h], p.k_scales + pair_at + (gid + h * 8) * G);
         }
     };
-    if (lane == 0) {
-        for (int i = 0; i < L::STAGES; ++i) bar_init(&full[i], 1);
-        bar_init_fence();
+    auto load_values = [&] {
+        const uint8_t* from = p.v_codes + code_at + 2 * tq * L::ROW + gid * BITS;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < G; ++j) load_words(vc[j][k], from + ((k & 1) + (k >> 1) * 8) * L::ROW + j * (kQuantGroup * BITS / 8));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_words(vp[h], p.v_scales + pair_at + (gid + h * 8) * G);
+    };
+    if (my_tiles > 0) {
+        find(0);
+        load_keys();
+        load_values();
     }
-    __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < min(L::STAGES, my_tiles); ++i) load_tile(i);
 
     // queries: a warp has an item, V neighbouring values to a thread
     constexpr int V = D / 32;
@@ -274,17 +324,9 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
                 for (int s = 0; s < 4; ++s) query(n, j, s, q_reg[n][j][s][0], q_reg[n][j][s][1]);
     }
     float cap_step = 0.f, to_step = 0.f;   // a power of two no step so far exceeds; kWeightScale over it
-    const int key0 = key_of(gid), key1 = key0 + 8;
-    bool ok = true;
+    const int key0 = gid, key1 = gid + 8;
 #pragma unroll 1
     for (int i = 0; i < my_tiles; ++i) {
-        const int st = i & (L::STAGES - 1);
-        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i / L::STAGES & 1));
-        if (!ok) {
-            if (lane == 0) tell(a.lanes.status, kDevWait);
-            break;
-        }
-        const uint32_t kt = ring + st * L::STAGE, vt = kt + L::CODES, kst = vt + L::CODES, vst = kst + L::SCALES;
         const int pos0 = begin + (warp + kWarps * i) * kTile;
         // ---- scores
         float sc[NT][4];
@@ -292,14 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
         for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-            uint32_t w0[4], w1[4];   // words of the thread's two keys
-            if constexpr (BITS == 4) {
-                const uint2 x = lds<uint2>(kt + key0 * L::ROW + j * 32 + tq * 8), y = lds<uint2>(kt + key1 * L::ROW + j * 32 + tq * 8);
-                w0[0] = x.x, w0[1] = x.y, w1[0] = y.x, w1[1] = y.y;
-            } else {
-                const uint4 x = lds<uint4>(kt + key0 * L::ROW + j * 64 + tq * 16), y = lds<uint4>(kt + key1 * L::ROW + j * 64 + tq * 16);
-                w0[0] = x.x, w0[1] = x.y, w0[2] = x.z, w0[3] = x.w, w1[0] = y.x, w1[1] = y.y, w1[2] = y.z, w1[3] = y.w;
-            }
+            const auto &w0 = kc[j][0], &w1 = kc[j][1];   // words of the thread's two keys
             float acc[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
@@ -320,7 +355,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
                     mma_f16(acc[n], a0, a1, a2, a3, b0, b1);
                 }
             }
-            const float2 sl0 = wide_pair<T>(lds<uint32_t>(kst + (key0 * G + j) * 4)), sl1 = wide_pair<T>(lds<uint32_t>(kst + (key1 * G + j) * 4));
+            const float2 sl0 = wide_pair<T>(kp[0][j]), sl1 = wide_pair<T>(kp[1][j]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 sc[n][0] = fmaf(sl0.x, acc[n][0], fmaf(sl0.y, sums[n][j][0], sc[n][0]));
@@ -329,11 +364,15 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
                 sc[n][3] = fmaf(sl1.x, acc[n][3], fmaf(sl1.y, sums[n][j][1], sc[n][3]));
             }
         }
+        if (i + 1 < my_tiles) {
+            find(i + 1);
+            load_keys();
+        }
         float2 v0[G], v1[G];   // (step, lowest) of the thread's two keys' values
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-            v0[j] = wide_pair<T>(lds<uint32_t>(vst + (key0 * G + j) * 4));
-            v1[j] = wide_pair<T>(lds<uint32_t>(vst + (key1 * G + j) * 4));
+            v0[j] = wide_pair<T>(vp[0][j]);
+            v1[j] = wide_pair<T>(vp[1][j]);
         }
         const bool whole = pos0 >= all_lo && pos0 + kTile <= all_hi;
         if (!whole) {   // keys that no item of the block sees may have any scales: those of values count as 0
@@ -440,21 +479,9 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
             }
         }
         // ---- output
-        const int va = key_of(2 * tq), vb = key_of(2 * tq + 1);   // the thread's keys: these and eight further on
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-            constexpr int WORDS = BITS / 4;
-            uint32_t w[4][WORDS];   // eight values of each of four keys
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t from = vt + ((k & 1 ? vb : va) + (k >> 1) * 8) * L::ROW + j * (kQuantGroup * BITS / 8) + gid * BITS;
-                if constexpr (BITS == 4) {
-                    w[k][0] = lds<uint32_t>(from);
-                } else {
-                    const uint2 x = lds<uint2>(from);
-                    w[k][0] = x.x, w[k][1] = x.y;
-                }
-            }
+            const auto& w = vc[j];   // eight values of each of four keys
 #pragma unroll
             for (int u = 0; u < 4; ++u) {   // values 2 u and 2 u + 1 of the eight
                 uint32_t a0, a1, a2, a3;
@@ -473,16 +500,11 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
                 }
             }
         }
-        __syncwarp();
-        if (i + L::STAGES < my_tiles) load_tile(i + L::STAGES);
-    }
-    if (!ok) {   // copies in flight land before the CTA ends
-        for (int st = 0; st < L::STAGES; ++st) bar_wait(&full[st], 0), bar_wait(&full[st], 1);
+        if (i + 1 < my_tiles) load_values();
     }
 
     // ---- a warp's results, over its own sum: [item][D] and (maximum, sum)
-    float* mine = reinterpret_cast<float*>(rings + warp * L::RING);
-    __syncwarp();
+    float* mine = reinterpret_cast<float*>(results + warp * L::RESULTS);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -492,7 +514,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
             for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             const int item = n * 8 + 2 * tq + h;
-            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], ok ? l : NAN);
+            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], l);
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 float low = low_acc[n][j][h];
@@ -511,7 +533,6 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
     __syncthreads();
     // ---- the warps' results together
     const bool last = shares == 1;
-    const int64_t n_rows = (int64_t)a.lanes.total * a.q_heads;
     for (int i = tid; i < n_items * (D / 4); i += kWarps * 32) {
         const int item = i / (D / 4), c = (i - item * (D / 4)) * 4;
         float m = -INFINITY, l = 0.f;
@@ -523,7 +544,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
             const float2 ml = warp_ml[w][item];
             if (ml.y == 0.f) continue;
             const float f = ml.y * ex2(ml.x - (m == -INFINITY ? 0.f : m));
-            const float4 x = *reinterpret_cast<const float4*>(rings + w * L::RING + (item * L::OP + c) * 4);
+            const float4 x = *reinterpret_cast<const float4*>(results + w * L::RESULTS + (item * L::OP + c) * 4);
             l += f;
             o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
         }
@@ -533,7 +554,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_items_kernel(const __grid_con
         if (last) {
             *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(at.first + r) * a.ldo + (kvh * g + hq) * D + c) = make_uint2(narrow_pair<T>(o.x, o.y), narrow_pair<T>(o.z, o.w));
         } else {
-            const int64_t row = share * n_rows + (int64_t)(at.first + r) * a.q_heads + kvh * g + hq;
+            const int64_t row = ((int64_t)slot * a.lanes.rows + r) * a.q_heads + kvh * g + hq;
             *reinterpret_cast<float4*>(part_o + row * D + c) = o;
             if (c == 0) part_ml[row] = make_float2(m, l);
         }
@@ -604,7 +625,7 @@ template <int BITS>
 __host__ __device__ constexpr int place_of(int i) { return BITS == 4 ? (i % 4) * 2 + i / 4 : i / 4 * 4 + (i % 2) * 2 + i % 4 / 2; }
 
 template <typename T, int D, int BITS, int SUBS, int CAP>
-__global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_kernel(const __grid_constant__ QuantAttnArgs a, int blocks, int chunk_min, int shares, float* part_o, float2* part_ml) {
+__global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_kernel(const __grid_constant__ QuantAttnArgs a, const __grid_constant__ QuantAttnCut cut, int blocks, float* part_o, float2* part_ml) {
     using L = Many<D, BITS, SUBS>;
     constexpr int G = L::G, KST = L::K_STAGES, VST = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -621,14 +642,15 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     const QuantPools& p = a.pools;
     const int g = a.q_heads / p.kv_heads;
     // the longest lanes come first, and of each the last rows, which see the most keys: what is left at the end is short
-    const int of_lane = p.kv_heads * blocks * shares, rank = blockIdx.x / of_lane, rest = blockIdx.x - rank * of_lane, block = blocks - 1 - rest / (p.kv_heads * shares), kvh = rest / shares % p.kv_heads,
-              share = rest % shares;
+    const int of_slot = p.kv_heads * blocks, slot = blockIdx.x / of_slot, rest = blockIdx.x - slot * of_slot, block = blocks - 1 - rest / p.kv_heads, kvh = rest % p.kv_heads;
     pdl_trigger();
-    const int lane_id = lane_of_rank(a.lanes, rank);
+    const Piece piece = piece_of(a, cut, slot, -1);
+    if (piece.lane < 0) return;
+    const int lane_id = cut.split ? piece.lane : lane_of_rank(a.lanes, slot), share = piece.share, shares = piece.shares;
     const LaneRange at = lane_range(a, lane_id);
     const int item0 = block * (SUBS * kItemTile), n_items = min(SUBS * kItemTile, at.n * g - item0);
     if (n_items <= 0) return;
-    const Shares sh = shares_of(a, at, item0, n_items, g, chunk_min, shares);
+    const Shares sh = shares_of(a, at, item0, n_items, g, shares);
     if (share > 0 && share >= sh.used()) return;
     const int begin = sh.begin + share * sh.chunk, lo = max(sh.lo, begin), hi = min(sh.hi, begin + sh.chunk);
     const int n_tiles = hi > lo ? (hi - begin + kKeyTile - 1) / kKeyTile : 0, subs = SUBS == 1 || n_items <= kItemTile ? 1 : 2;
@@ -1000,7 +1022,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         if (!ok && lane == 0) tell(a.lanes.status, kDevWait);
         fence_after();
         const float inv = !ok ? NAN : (sum == 0.f ? 0.f : 1.0f / sum), back = power_of_two(e_run);
-        const int64_t out_row = (int64_t)(at.first + row), part_row = share * ((int64_t)a.lanes.total * a.q_heads) + out_row * a.q_heads + kvh * g + head;
+        const int64_t out_row = (int64_t)(at.first + row), part_row = ((int64_t)slot * a.lanes.rows + row) * a.q_heads + kvh * g + head;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
@@ -1039,17 +1061,19 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
 // ---- shares joined: a warp to a (row, query head) ----------------------------------------------------------------------
 
 template <typename T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ QuantAttnArgs a, int items_of_block, int chunk_min, int shares, const float* part_o, const float2* part_ml) {
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ QuantAttnArgs a, const __grid_constant__ QuantAttnCut cut, int items_of_block, const float* part_o, const float2* part_ml) {
     constexpr int V = D / 32;
-    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.q_heads / a.pools.kv_heads;
     const int lane_id = blockIdx.x, i = blockIdx.y * 4 + warp;
+    const Piece piece = piece_of(a, cut, 0, lane_id);
     const LaneRange at = lane_range(a, lane_id);
-    const int64_t n_rows = (int64_t)a.lanes.total * a.q_heads;
+    pdl_wait();
+    if (piece.shares == 1) return;   // written as it is
+    const int64_t n_rows = (int64_t)a.lanes.rows * a.q_heads;
     for (int64_t at_row = i; at_row < (int64_t)at.n * a.q_heads; at_row += (int64_t)gridDim.y * 4) {
         const int r = (int)(at_row / a.q_heads), head = (int)(at_row - (int64_t)r * a.q_heads), item = r * g + head % g, item0 = item / items_of_block * items_of_block;
-        const int used = max(1, shares_of(a, at, item0, min(items_of_block, at.n * g - item0), g, chunk_min, shares).used());
-        const int64_t row = (int64_t)(at.first + r) * a.q_heads + head;
+        const int used = max(1, shares_of(a, at, item0, min(items_of_block, at.n * g - item0), g, piece.shares).used());
+        const int64_t row = piece.slot * n_rows + at_row;
         float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = 0.f;
@@ -1084,7 +1108,7 @@ template <typename T, int D, int BITS, int NT, int CAP>
 void launch_few(const QuantAttnArgs& a, const QuantAttnPlan& p, float* part_o, float2* part_ml, cudaStream_t s) {
     auto* kernel = few_items_kernel<T, D, BITS, NT, CAP>;
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Few<D, BITS, NT>::SMEM);
-    kernel<<<dim3((unsigned)(a.lanes.lanes * p.shares), (unsigned)a.pools.kv_heads, (unsigned)p.blocks), kWarps * 32, Few<D, BITS, NT>::SMEM, s>>>(a, p.chunk, p.shares, part_o, part_ml);
+    kernel<<<dim3((unsigned)p.slots, (unsigned)a.pools.kv_heads, (unsigned)p.blocks), kWarps * 32, Few<D, BITS, NT>::SMEM, s>>>(a, p.cut, part_o, part_ml);
     MK_LAUNCH_CHECK();
 }
 
@@ -1102,14 +1126,14 @@ void launch_many(const QuantAttnArgs& a, const QuantAttnPlan& p, float* part_o, 
         }();
         if (registers < L::LAUNCH_REGISTERS) throw std::runtime_error("quantized attention: the kernel was built with fewer registers than its warps share out");
     }
-    kernel<<<(unsigned)(a.lanes.lanes * p.shares * a.pools.kv_heads * p.blocks), L::THREADS, L::SMEM, s>>>(a, p.blocks, p.chunk, p.shares, part_o, part_ml);
+    kernel<<<(unsigned)(p.slots * a.pools.kv_heads * p.blocks), L::THREADS, L::SMEM, s>>>(a, p.cut, p.blocks, part_o, part_ml);
     MK_LAUNCH_CHECK();
 }
 
 template <typename T, int D>
 void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s) {
     float* part_o = static_cast<float*>(workspace);
-    float2* part_ml = reinterpret_cast<float2*>(part_o + (p.shares > 1 ? p.shares * (int64_t)a.lanes.total * a.q_heads * D : 0));
+    float2* part_ml = reinterpret_cast<float2*>(part_o + (p.cut.split ? p.slots * (int64_t)a.lanes.rows * a.q_heads * D : 0));
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
     using Four = std::integral_constant<int, 4>;
@@ -1122,13 +1146,17 @@ void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cud
         constexpr int B = decltype(bits)::value;
         a.softcap != 0.f ? launch_many<T, D, B, 1>(a, p, part_o, part_ml, s) : launch_many<T, D, B, 0>(a, p, part_o, part_ml, s);
     };
-    if (p.items > 16) a.pools.bits == 4 ? many(Four{}) : many(Eight{});
-    else if (a.pools.bits == 4) p.items == 8 ? few(Four{}, One{}) : few(Four{}, Two{});
-    else p.items == 8 ? few(Eight{}, One{}) : few(Eight{}, Two{});
-    if (p.shares > 1) {
+    if (p.items > 16) {
+        a.pools.bits == 4 ? many(Four{}) : many(Eight{});
+    } else if (p.items == 8) {
+        a.pools.bits == 4 ? few(Four{}, One{}) : few(Eight{}, One{});
+    } else {
+        if constexpr (D != 256) a.pools.bits == 4 ? few(Four{}, Two{}) : few(Eight{}, Two{});   // heads of 256: 255 registers and more, so they take two blocks instead
+    }
+    if (p.cut.split) {
         const int64_t rows = (int64_t)a.lanes.rows * a.q_heads;
-        launch_pdl(join_kernel<T, D>, dim3((unsigned)a.lanes.lanes, (unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(128), 0, s, a, p.items, p.chunk, p.shares,
-                   (const float*)part_o, (const float2*)part_ml);
+        launch_pdl(join_kernel<T, D>, dim3((unsigned)a.lanes.lanes, (unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(128), 0, s, a, p.cut, p.items, (const float*)part_o,
+                   (const float2*)part_ml);
         MK_LAUNCH_CHECK();
     }
 }
@@ -1138,14 +1166,18 @@ void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cud
 QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window) {
     QuantAttnPlan p;
     const int64_t items = (int64_t)rows * (q_heads / kv_heads);
-    p.items = items <= 8 ? 8 : (items <= 16 ? 16 : (d == 256 ? kItemTile : 2 * kItemTile));
+    p.items = items <= 8 || (items <= 16 && d == 256) ? 8 : (items <= 16 ? 16 : (d == 256 ? kItemTile : 2 * kItemTile));
     p.blocks = (int)std::max<int64_t>(1, (items + p.items - 1) / p.items);
-    const int64_t most = window > 0 ? std::min<int64_t>((int64_t)width * block_tokens, (int64_t)window + rows + 15) : (int64_t)width * block_tokens;
-    const int64_t columns = std::max<int64_t>(1, (int64_t)lanes * kv_heads * p.blocks);
-    // few items: as many shares as make six waves of three CTAs on each SM; many: one wave of one
-    p.chunk = 256;
-    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>((most + p.chunk - 1) / p.chunk, ((p.items <= 16 ? 6 * 3 * kSms : kSms) + columns - 1) / columns));
-    if (p.shares > 1) p.bytes = (int64_t)p.shares * total * q_heads * ((int64_t)d * 4 + 8);
+    // one wave of CTAs
+    const int ctas = p.items > 16 ? 1 : few_ctas(d, p.items / 8);
+    const double want = (double)kSms * ctas / ((double)kv_heads * p.blocks);
+    const int64_t table = (int64_t)width * block_tokens, window_keys = (int64_t)window + rows + 16;
+    p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
+    p.cut.least = p.items > 16 ? 256 : 512;
+    p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < 4 * want;
+    p.cut.want = (float)std::max(want / 2, want - 0.5 * lanes);   // the shares' rounding adds half a share for each lane
+    p.slots = p.cut.split ? lanes + (int)std::min(want, (double)lanes * (double)table / p.cut.least) + 1 : lanes;   // a lane's last share is a part of one
+    if (p.cut.split) p.bytes = (int64_t)p.slots * rows * q_heads * ((int64_t)d * 4 + 8);
     return p;
 }
 

@@ -15,11 +15,19 @@ struct QuantAttnArgs {
     int window = 0;
 };
 
+// How the lanes' keys are shared out on the device (see quantized_attention.cu).
+struct QuantAttnCut {
+    bool split = false;     // otherwise every lane has one share
+    int least = 0;          // keys of a share, at least
+    float want = 1.f;       // shares in all
+    int window_keys = 0;    // keys of a lane that a window leaves, at most
+};
 // How a call is cut, from sizes alone.
 struct QuantAttnPlan {
     int items = 0, blocks = 0;   // (row, query head) items of a lane and KV head to a CTA, and such blocks
-    int shares = 1, chunk = 0;   // shares of a lane's keys, and the fewest keys of one
-    int64_t bytes = 0;           // workspace
+    int slots = 0;               // shares of all lanes, at most
+    QuantAttnCut cut;
+    int64_t bytes = 0;           // workspace: a partial result of each slot's rows
 };
 QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window);
 void launch_quantized_attention(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cudaStream_t s);
