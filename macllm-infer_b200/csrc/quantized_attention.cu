@@ -116,30 +116,30 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 
 // ---- few items -----------------------------------------------------------------------------------------------------
 //
-// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks tiles of 16 keys, whose codes and scales come from
-// memory into the registers of the threads that multiply them: those of the next tile's keys once this one's scores are there, its values' once this one's output is.
-// Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
+// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks steps of 32 keys, whose codes and scales bulk copies
+// bring into a ring of its own.  Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
 // are the f16 number c 2^-24 (a subnormal, which the tensor cores take in full), so that it costs a mask and half a shift.  With steps and lowest values of the groups
 //   q . k = sum_g step_g (q_g . c_g) + low_g sum(q_g),   o = sum_j (w_j step_jg) c_j + sum_j w_j low_jg,
 // steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
 // Queries are brought to f16 by a power of two per item, weights by one for the largest step met so far; either is exact.  The running maximum follows only
 // when a score exceeds it by more than 2^kSlack, which a vote of the warp tells.
-constexpr int kTile = 16;
+constexpr int kTile = 16, kHalves = 2, kStep = kHalves * kTile;
 constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;            // base-2 logarithm
 constexpr float kWeightScale = 128.f;    // weights up to 2^kSlack, times this, times a step over the largest: below f16's largest
 
 // CTAs on an SM: what registers allow.
-__host__ __device__ constexpr int few_ctas(int d, int nt) { return d == 64 ? (nt == 1 ? 5 : 4) : (d == 128 && nt == 1 ? 4 : 2); }
+__host__ __device__ constexpr int few_ctas(int d, int nt) { return d == 64 ? (nt == 1 ? 5 : 4) : (d == 128 ? (nt == 1 ? 3 : 2) : 2); }
 
 template <int D, int BITS, int NT>
 struct Few {
     static constexpr int G = D / kQuantGroup, ITEMS = NT * 8;
-    static constexpr int ROW = D * BITS / 8;
+    static constexpr int ROW = D * BITS / 8, CODES = kTile * ROW, SCALES = kTile * G * 4, HALF = 2 * (CODES + SCALES), STAGE = kHalves * HALF;
+    static constexpr int STAGES = STAGE <= 2400 ? 4 : 2;
     static constexpr int OP = D + 4;                                     // pitch of a warp's results, in floats
-    static constexpr int RESULTS = ITEMS * OP * 4;
+    static constexpr int RING = ((STAGES * STAGE > ITEMS * OP * 4 ? STAGES * STAGE : ITEMS * OP * 4) + 127) / 128 * 128;
     static constexpr int QP = D + 8;
-    static constexpr size_t SMEM = (size_t)kWarps * RESULTS + (size_t)ITEMS * QP * 2;
+    static constexpr size_t SMEM = 128 + (size_t)kWarps * RING + (size_t)ITEMS * QP * 2;
     static constexpr int CTAS = few_ctas(D, NT);
     static constexpr bool Q_IN_REGISTERS = NT * D <= 256;
 };
@@ -149,6 +149,20 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// A copy of a multiple of 16 bytes, both addresses multiples of 16.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// N words of shared memory.
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t at) {
+    if constexpr (N == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(at));
+    else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
+    else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
+}
+// The key of a tile that row r of a product stands for: with neighbours swapped in every other pair, the rows that a load takes at once lie on both halves of the banks.
+__device__ __forceinline__ int key_of(int r) { return r ^ (r >> 1 & 1); }
+
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -158,10 +172,12 @@ template <typename T, int D, int BITS, int NT, int CAP>
 __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items_kernel(const __grid_constant__ QuantAttnArgs a, const __grid_constant__ QuantAttnCut cut, float* part_o, float2* part_ml) {
     using L = Few<D, BITS, NT>;
     constexpr int G = L::G;
-    extern __shared__ __align__(16) uint8_t results[];   // of the warps; queries behind them
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[kWarps * L::STAGES];
     __shared__ float item_factor[L::ITEMS], item_sums[L::ITEMS][G];
     __shared__ float2 warp_ml[kWarps][L::ITEMS];
-    __half* qs = reinterpret_cast<__half*>(results + kWarps * L::RESULTS);
+    uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);   // a warp's results at the end
+    __half* qs = reinterpret_cast<__half*>(rings + kWarps * L::RING);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
     const QuantPools& p = a.pools;
     const int g = a.q_heads / p.kv_heads, slot = blockIdx.x, kvh = blockIdx.y;
@@ -175,67 +191,51 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
     const Shares sh = shares_of(a, at, item0, n_items, g, shares);
     if (share > 0 && share >= sh.used()) return;
     const int lo = max(sh.lo, sh.begin + share * sh.chunk), hi = min(sh.hi, sh.begin + (share + 1) * sh.chunk);
-    const int begin = sh.begin + share * sh.chunk, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0;
-    const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
+    const int begin = sh.begin + share * sh.chunk, n_tiles = hi > lo ? (hi - begin + kTile - 1) / kTile : 0, n_steps = (n_tiles + kHalves - 1) / kHalves;
+    const int my_steps = n_steps > warp ? (n_steps - warp + kWarps - 1) / kWarps : 0;
 
+    const uint32_t ring = smem_u32(rings + warp * L::RING);
+    uint64_t* full = bars + warp * L::STAGES;
     const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
-    // the page numbers of 32 tiles sit in the warp's threads, those of the next 32 on their way
+    auto tile_of = [&](int i) { return ((i >> 1) * kWarps + warp) * kHalves + (i & 1); };   // of the warp's half i
+    // the page numbers of 32 halves sit in the warp's threads, those of the next 32 on their way
     auto page_of = [&](int i) {
-        if (i >= my_tiles) return 0;
-        const int32_t page = table[(begin + (warp + kWarps * i) * kTile) >> p.bt_shift];
+        const int tile = tile_of(i);
+        if (tile >= n_tiles) return 0;
+        const int32_t page = table[(begin + tile * kTile) >> p.bt_shift];
         if ((uint32_t)page < (uint64_t)p.pages) return page;
         tell(a.lanes.status, kDevBadPage);
         return 0;
     };
-    int page_now = page_of(lane), page_next = my_tiles > 32 ? page_of(32 + lane) : 0;
-    // a thread's keys are rows gid and gid + 8 of a tile, its values those of keys 2 tq, 2 tq + 1 and the same eight further on
-    uint32_t kc[G][2][BITS / 2], vc[G][4][BITS / 4], kp[2][G], vp[2][G];   // codes, and pairs (step, lowest) of keys gid and gid + 8
-    auto load_words = [](auto& to, const void* from) {
-        constexpr int N = sizeof(to) / 4;
-        if constexpr (N == 1) {
-            to[0] = *static_cast<const uint32_t*>(from);
-        } else if constexpr (N == 2) {
-            const uint2 x = *static_cast<const uint2*>(from);
-            to[0] = x.x, to[1] = x.y;
-        } else {
-            const uint4 x = *static_cast<const uint4*>(from);
-            to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
-        }
-    };
-    int64_t code_at = 0, pair_at = 0;   // of the tile that is loaded next
-    auto find = [&](int i) {            // the whole warp
-        if ((i & 31) == 0 && i > 0) {
+    int page_now = page_of(lane), page_next = my_steps > 16 ? page_of(32 + lane) : 0;
+    // eight threads bring a step: four its first half's codes of keys, of values, scales of keys, of values, four its second's
+    const int part = lane & 3;
+    const uint8_t* part_from = part < 2 ? (part == 0 ? p.k_codes : p.v_codes) : reinterpret_cast<const uint8_t*>(part == 2 ? p.k_scales : p.v_scales);
+    const int64_t part_page = part < 2 ? p.codes_stride : p.scales_stride * 4;
+    const int part_row = part < 2 ? L::ROW : G * 4;
+    const uint32_t part_bytes = part < 2 ? L::CODES : L::SCALES, part_to = (part < 2 ? part * L::CODES : 2 * L::CODES + (part - 2) * L::SCALES) + (lane >> 2) * L::HALF;
+    auto load_step = [&](int i) {   // the whole warp
+        if ((i & 15) == 0 && i > 0) {
             page_now = page_next;
-            page_next = page_of(i + 32 + lane);
+            page_next = page_of(2 * i + 32 + lane);
         }
-        const int64_t page = __shfl_sync(0xffffffffu, page_now, i & 31);
-        const int row = kvh * p.block_tokens + ((begin + (warp + kWarps * i) * kTile) & (p.block_tokens - 1));
-        code_at = page * p.codes_stride + row * L::ROW;
-        pair_at = page * p.scales_stride + row * G;
-    };
-    auto load_keys = [&] {
-        const uint8_t* from = p.k_codes + code_at + gid * L::ROW + tq * (BITS * 2);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < G; ++j) load_words(kc[j][h], from + h * 8 * L::ROW + j * (kQuantGroup * BITS / 8));
-            load_words(kp[h], p.k_scales + pair_at + (gid + h * 8) * G);
+        const int half = lane >> 2 & 1;
+        const int64_t page = __shfl_sync(0xffffffffu, page_now, (2 * i & 31) + half);
+        const int tile = tile_of(2 * i + half), st = i & (L::STAGES - 1);
+        if (lane == 0) bar_expect_tx(&full[st], tile + 1 < n_tiles ? L::STAGE : L::HALF);
+        __syncwarp();
+        if (lane < 8 && tile < n_tiles) {
+            const int row = kvh * p.block_tokens + ((begin + tile * kTile) & (p.block_tokens - 1));
+            bulk_load(ring + st * L::STAGE + part_to, part_from + page * part_page + (int64_t)row * part_row, part_bytes, &full[st]);
         }
     };
-    auto load_values = [&] {
-        const uint8_t* from = p.v_codes + code_at + 2 * tq * L::ROW + gid * BITS;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int j = 0; j < G; ++j) load_words(vc[j][k], from + ((k & 1) + (k >> 1) * 8) * L::ROW + j * (kQuantGroup * BITS / 8));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) load_words(vp[h], p.v_scales + pair_at + (gid + h * 8) * G);
-    };
-    if (my_tiles > 0) {
-        find(0);
-        load_keys();
-        load_values();
+    if (lane == 0) {
+        for (int i = 0; i < L::STAGES; ++i) bar_init(&full[i], 1);
+        bar_init_fence();
     }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < min(L::STAGES, my_steps); ++i) load_step(i);
 
     // queries: a warp has an item, V neighbouring values to a thread
     constexpr int V = D / 32;
@@ -324,89 +324,101 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                 for (int s = 0; s < 4; ++s) query(n, j, s, q_reg[n][j][s][0], q_reg[n][j][s][1]);
     }
     float cap_step = 0.f, to_step = 0.f;   // a power of two no step so far exceeds; kWeightScale over it
-    const int key0 = gid, key1 = gid + 8;
+    const int key0 = key_of(gid), va = key_of(2 * tq), vb = key_of(2 * tq + 1);
+    bool ok = true;
 #pragma unroll 1
-    for (int i = 0; i < my_tiles; ++i) {
-        const int pos0 = begin + (warp + kWarps * i) * kTile;
+    for (int i = 0; i < my_steps; ++i) {
+        const int st = i & (L::STAGES - 1);
+        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i / L::STAGES & 1));
+        if (!ok) break;
+        const uint32_t stage = ring + st * L::STAGE;
+        const int pos0 = begin + tile_of(2 * i) * kTile;
+        const bool whole = pos0 >= all_lo && pos0 + kStep <= all_hi;
         // ---- scores
-        float sc[NT][4];
+        float sc[kHalves][NT][4];
+        float2 v0[kHalves][G], v1[kHalves][G];   // (step, lowest) of the values of the thread's keys
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        for (int h = 0; h < kHalves; ++h) {
+            const uint32_t kt = stage + h * L::HALF, scales = kt + 2 * L::CODES + key0 * (G * 4);
+            uint32_t kp[2][G], vp[2][G];
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const auto &w0 = kc[j][0], &w1 = kc[j][1];   // words of the thread's two keys
-            float acc[NT][4];
+            for (int r = 0; r < 2; ++r) {
+                lds(kp[r], scales + r * 8 * G * 4);
+                lds(vp[r], scales + L::SCALES + r * 8 * G * 4);
+            }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+            for (int n = 0; n < NT; ++n) sc[h][n][0] = sc[h][n][1] = sc[h][n][2] = sc[h][n][3] = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint32_t a0, a1, a2, a3;
-                if constexpr (BITS == 4) {
-                    const uint32_t x = s & 1 ? w0[s >> 1] >> 8 : w0[s >> 1], y = s & 1 ? w1[s >> 1] >> 8 : w1[s >> 1];
-                    a0 = x & 0x000f000fu, a2 = x & 0x00f000f0u, a1 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
-                } else {
-                    a0 = w0[s] & 0x00ff00ffu, a2 = w0[s] >> 8 & 0x00ff00ffu, a1 = w1[s] & 0x00ff00ffu, a3 = w1[s] >> 8 & 0x00ff00ffu;
+            for (int j = 0; j < G; ++j) {
+                uint32_t w0[BITS / 2], w1[BITS / 2];   // words of the thread's two keys
+                lds(w0, kt + key0 * L::ROW + j * (kQuantGroup * BITS / 8) + tq * (BITS * 2));
+                lds(w1, kt + (key0 + 8) * L::ROW + j * (kQuantGroup * BITS / 8) + tq * (BITS * 2));
+                float acc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t a0, a1, a2, a3;
+                    if constexpr (BITS == 4) {
+                        const uint32_t x = s & 1 ? w0[s >> 1] >> 8 : w0[s >> 1], y = s & 1 ? w1[s >> 1] >> 8 : w1[s >> 1];
+                        a0 = x & 0x000f000fu, a2 = x & 0x00f000f0u, a1 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                    } else {
+                        a0 = w0[s] & 0x00ff00ffu, a2 = w0[s] >> 8 & 0x00ff00ffu, a1 = w1[s] & 0x00ff00ffu, a3 = w1[s] >> 8 & 0x00ff00ffu;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        uint32_t b0, b1;
+                        if constexpr (L::Q_IN_REGISTERS) b0 = q_reg[n][j][s][0], b1 = q_reg[n][j][s][1];
+                        else query(n, j, s, b0, b1);
+                        mma_f16(acc[n], a0, a1, a2, a3, b0, b1);
+                    }
                 }
+                const float2 sl0 = wide_pair<T>(kp[0][j]), sl1 = wide_pair<T>(kp[1][j]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    uint32_t b0, b1;
-                    if constexpr (L::Q_IN_REGISTERS) b0 = q_reg[n][j][s][0], b1 = q_reg[n][j][s][1];
-                    else query(n, j, s, b0, b1);
-                    mma_f16(acc[n], a0, a1, a2, a3, b0, b1);
+                    sc[h][n][0] = fmaf(sl0.x, acc[n][0], fmaf(sl0.y, sums[n][j][0], sc[h][n][0]));
+                    sc[h][n][1] = fmaf(sl0.x, acc[n][1], fmaf(sl0.y, sums[n][j][1], sc[h][n][1]));
+                    sc[h][n][2] = fmaf(sl1.x, acc[n][2], fmaf(sl1.y, sums[n][j][0], sc[h][n][2]));
+                    sc[h][n][3] = fmaf(sl1.x, acc[n][3], fmaf(sl1.y, sums[n][j][1], sc[h][n][3]));
                 }
-            }
-            const float2 sl0 = wide_pair<T>(kp[0][j]), sl1 = wide_pair<T>(kp[1][j]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                sc[n][0] = fmaf(sl0.x, acc[n][0], fmaf(sl0.y, sums[n][j][0], sc[n][0]));
-                sc[n][1] = fmaf(sl0.x, acc[n][1], fmaf(sl0.y, sums[n][j][1], sc[n][1]));
-                sc[n][2] = fmaf(sl1.x, acc[n][2], fmaf(sl1.y, sums[n][j][0], sc[n][2]));
-                sc[n][3] = fmaf(sl1.x, acc[n][3], fmaf(sl1.y, sums[n][j][1], sc[n][3]));
+                v0[h][j] = wide_pair<T>(vp[0][j]);
+                v1[h][j] = wide_pair<T>(vp[1][j]);
             }
         }
-        if (i + 1 < my_tiles) {
-            find(i + 1);
-            load_keys();
-        }
-        float2 v0[G], v1[G];   // (step, lowest) of the thread's two keys' values
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-            v0[j] = wide_pair<T>(vp[0][j]);
-            v1[j] = wide_pair<T>(vp[1][j]);
-        }
-        const bool whole = pos0 >= all_lo && pos0 + kTile <= all_hi;
         if (!whole) {   // keys that no item of the block sees may have any scales: those of values count as 0
-            if (pos0 + key0 < lo || pos0 + key0 >= hi) {
 #pragma unroll
-                for (int j = 0; j < G; ++j) v0[j] = make_float2(0.f, 0.f);
-            }
-            if (pos0 + key1 < lo || pos0 + key1 >= hi) {
+            for (int h = 0; h < kHalves; ++h) {
+                const int pos = pos0 + h * kTile + key0;
 #pragma unroll
-                for (int j = 0; j < G; ++j) v1[j] = make_float2(0.f, 0.f);
+                for (int j = 0; j < G; ++j) {
+                    if (pos < lo || pos >= hi) v0[h][j] = make_float2(0.f, 0.f);
+                    if (pos + 8 < lo || pos + 8 >= hi) v1[h][j] = make_float2(0.f, 0.f);
+                }
             }
         }
         bool up = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = sc[n][e] * factor[n][e & 1];
-                if (CAP) v = (wide_cap ? capped_wide(v, a.softcap, two_over_cap) : capped(v, a.softcap, two_over_cap)) * kLog2e;
-                if (!whole) {
-                    const int pos = pos0 + (e < 2 ? key0 : key1);
-                    v = pos >= see_lo[n][e & 1] && pos < see_hi[n][e & 1] ? v : -INFINITY;
-                }
-                sc[n][e] = v;
-                up |= v > m_run[n][e & 1] + kSlack;   // also when there was none yet
-            }
-        }
         float top_step = 0.f;
 #pragma unroll
-        for (int j = 0; j < G; ++j) top_step = fmaxf(top_step, fmaxf(v0[j].x, v1[j].x));
-        top_step = top_step < INFINITY ? top_step : 0.f;
+        for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = sc[h][n][e] * factor[n][e & 1];
+                    if (CAP) v = (wide_cap ? capped_wide(v, a.softcap, two_over_cap) : capped(v, a.softcap, two_over_cap)) * kLog2e;
+                    if (!whole) {
+                        const int pos = pos0 + h * kTile + key0 + (e >> 1) * 8;
+                        v = pos >= see_lo[n][e & 1] && pos < see_hi[n][e & 1] ? v : -INFINITY;
+                    }
+                    sc[h][n][e] = v;
+                    up |= v > m_run[n][e & 1] + kSlack;   // also when there was none yet
+                }
+#pragma unroll
+            for (int j = 0; j < G; ++j) top_step = max3(top_step, v0[h][j].x, v1[h][j].x);
+        }
         up |= top_step > cap_step;
         if (__any_sync(0xffffffffu, up)) {
-            const float largest = fmaxf(warp_max(top_step), cap_step);
+            const float largest = fmaxf(warp_max(top_step < INFINITY ? top_step : 0.f), cap_step);
             // the next power of two, between those whose inverse is one too
             const float cap_new = largest > 0.f ? __uint_as_float(min(max((__float_as_uint(largest) + 0x007fffffu) & 0x7f800000u, 8u << 23), 252u << 23)) : 0.f;
             const float shrink = cap_new > 0.f ? cap_step / cap_new : 1.f;
@@ -416,18 +428,18 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             for (int n = 0; n < NT; ++n) {
                 float alpha[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float top = fmaxf(sc[n][h], sc[n][2 + h]);
+                for (int c = 0; c < 2; ++c) {
+                    float top = fmaxf(fmaxf(sc[0][n][c], sc[0][n][2 + c]), fmaxf(sc[1][n][c], sc[1][n][2 + c]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float m_new = fmaxf(m_run[n][h], top);
-                    alpha[h] = m_new == -INFINITY ? 1.f : ex2(m_run[n][h] - m_new);
-                    m_run[n][h] = m_new;
-                    l_run[n][h] *= alpha[h];
+                    const float m_new = fmaxf(m_run[n][c], top);
+                    alpha[c] = m_new == -INFINITY ? 1.f : ex2(m_run[n][c] - m_new);
+                    m_run[n][c] = m_new;
+                    l_run[n][c] *= alpha[c];
 #pragma unroll
-                    for (int j = 0; j < G; ++j) low_acc[n][j][h] *= alpha[h];
-                    alpha[h] *= shrink;
+                    for (int j = 0; j < G; ++j) low_acc[n][j][c] *= alpha[c];
+                    alpha[c] *= shrink;
                 }
 #pragma unroll
                 for (int j = 0; j < G; ++j)
@@ -440,71 +452,83 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                     }
             }
         }
-        // ---- weights
-        uint32_t hi_b[NT][G][2], lo_b[NT][G][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float w[4];
+        for (int h = 0; h < kHalves; ++h) {
+            // ---- weights
+            uint32_t hi_b[NT][G][2], lo_b[NT][G][2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float m = m_run[n][e & 1];
-                w[e] = ex2(sc[n][e] - (m == -INFINITY ? 0.f : m));
-            }
-            l_run[n][0] += w[0] + w[2];
-            l_run[n][1] += w[1] + w[3];
+            for (int n = 0; n < NT; ++n) {
+                float w[4];
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                float x[4];
-                if (whole) {
-                    low_acc[n][j][0] = fmaf(w[0], v0[j].y, fmaf(w[2], v1[j].y, low_acc[n][j][0]));
-                    low_acc[n][j][1] = fmaf(w[1], v0[j].y, fmaf(w[3], v1[j].y, low_acc[n][j][1]));
+                for (int e = 0; e < 4; ++e) {
+                    const float m = m_run[n][e & 1];
+                    w[e] = ex2(sc[h][n][e] - (m == -INFINITY ? 0.f : m));
+                }
+                l_run[n][0] += w[0] + w[2];
+                l_run[n][1] += w[1] + w[3];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = w[e] * ((e < 2 ? v0[j].x : v1[j].x) * to_step);
-                } else {   // what an item does not see does not count, also where it is not finite
+                for (int j = 0; j < G; ++j) {
+                    float x[4];
+                    const float step0 = v0[h][j].x * to_step, step1 = v1[h][j].x * to_step;
+                    if (whole) {
+                        low_acc[n][j][0] = fmaf(w[0], v0[h][j].y, fmaf(w[2], v1[h][j].y, low_acc[n][j][0]));
+                        low_acc[n][j][1] = fmaf(w[1], v0[h][j].y, fmaf(w[3], v1[h][j].y, low_acc[n][j][1]));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v = e < 2 ? v0[j] : v1[j];
-                        const bool seen = sc[n][e] != -INFINITY;
-                        low_acc[n][j][e & 1] += seen ? w[e] * v.y : 0.f;
-                        x[e] = seen ? w[e] * (v.x * to_step) : 0.f;
+                        for (int e = 0; e < 4; ++e) x[e] = w[e] * (e < 2 ? step0 : step1);
+                    } else {   // what an item does not see does not count, also where it is not finite
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool seen = sc[h][n][e] != -INFINITY;
+                            low_acc[n][j][e & 1] += seen ? w[e] * (e < 2 ? v0[h][j].y : v1[h][j].y) : 0.f;
+                            x[e] = seen ? w[e] * (e < 2 ? step0 : step1) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t high = narrow_pair<__half>(x[2 * r], x[2 * r + 1]);
+                        const float2 back = wide_pair<__half>(high);
+                        hi_b[n][j][r] = transpose_8x8(high);
+                        lo_b[n][j][r] = transpose_8x8(narrow_pair<__half>(x[2 * r] - back.x, x[2 * r + 1] - back.y));
                     }
                 }
+            }
+            // ---- output; the thread's values are those of keys va, vb and the same eight further on
+            const uint32_t vt = stage + h * L::HALF + L::CODES;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t high = narrow_pair<__half>(x[2 * h], x[2 * h + 1]);
-                    const float2 r = wide_pair<__half>(high);
-                    hi_b[n][j][h] = transpose_8x8(high);
-                    lo_b[n][j][h] = transpose_8x8(narrow_pair<__half>(x[2 * h] - r.x, x[2 * h + 1] - r.y));
+            for (int j = 0; j < G; ++j) {
+                uint32_t w[4][BITS / 4];   // eight values of each of four keys
+#pragma unroll
+                for (int k = 0; k < 4; ++k) lds(w[k], vt + ((k & 1 ? vb : va) + (k >> 1) * 8) * L::ROW + j * (kQuantGroup * BITS / 8) + gid * BITS);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {   // values 2 u and 2 u + 1 of the eight
+                    uint32_t a0, a1, a2, a3;
+                    if constexpr (BITS == 4) {
+                        uint32_t x = __byte_perm(w[0][0], w[1][0], u < 2 ? 0x5410 : 0x7632), y = __byte_perm(w[2][0], w[3][0], u < 2 ? 0x5410 : 0x7632);
+                        if (u & 1) x >>= 8, y >>= 8;
+                        a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                    } else {
+                        const uint32_t x = __byte_perm(w[0][u >> 1], w[1][u >> 1], u & 1 ? 0x7632 : 0x5410), y = __byte_perm(w[2][u >> 1], w[3][u >> 1], u & 1 ? 0x7632 : 0x5410);
+                        a0 = x & 0x00ff00ffu, a1 = x >> 8 & 0x00ff00ffu, a2 = y & 0x00ff00ffu, a3 = y >> 8 & 0x00ff00ffu;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_f16(o_acc[n][j][u], a0, a1, a2, a3, hi_b[n][j][0], hi_b[n][j][1]);
+                        mma_f16(o_acc[n][j][u], a0, a1, a2, a3, lo_b[n][j][0], lo_b[n][j][1]);
+                    }
                 }
             }
         }
-        // ---- output
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const auto& w = vc[j];   // eight values of each of four keys
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {   // values 2 u and 2 u + 1 of the eight
-                uint32_t a0, a1, a2, a3;
-                if constexpr (BITS == 4) {
-                    uint32_t x = __byte_perm(w[0][0], w[1][0], u < 2 ? 0x5410 : 0x7632), y = __byte_perm(w[2][0], w[3][0], u < 2 ? 0x5410 : 0x7632);
-                    if (u & 1) x >>= 8, y >>= 8;
-                    a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
-                } else {
-                    const uint32_t x = __byte_perm(w[0][u >> 1], w[1][u >> 1], u & 1 ? 0x7632 : 0x5410), y = __byte_perm(w[2][u >> 1], w[3][u >> 1], u & 1 ? 0x7632 : 0x5410);
-                    a0 = x & 0x00ff00ffu, a1 = x >> 8 & 0x00ff00ffu, a2 = y & 0x00ff00ffu, a3 = y >> 8 & 0x00ff00ffu;
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma_f16(o_acc[n][j][u], a0, a1, a2, a3, hi_b[n][j][0], hi_b[n][j][1]);
-                    mma_f16(o_acc[n][j][u], a0, a1, a2, a3, lo_b[n][j][0], lo_b[n][j][1]);
-                }
-            }
-        }
-        if (i + 1 < my_tiles) load_values();
+        __syncwarp();
+        if (i + L::STAGES < my_steps) load_step(i + L::STAGES);
+    }
+    if (!ok) {   // copies in flight land before the CTA ends
+        if (lane == 0) tell(a.lanes.status, kDevWait);
+        for (int st = 0; st < L::STAGES; ++st) bar_wait(&full[st], 0), bar_wait(&full[st], 1);
     }
 
     // ---- a warp's results, over its own sum: [item][D] and (maximum, sum)
-    float* mine = reinterpret_cast<float*>(results + warp * L::RESULTS);
+    float* mine = reinterpret_cast<float*>(rings + warp * L::RING);
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -514,7 +538,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             const int item = n * 8 + 2 * tq + h;
-            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], l);
+            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], ok ? l : NAN);
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 float low = low_acc[n][j][h];
@@ -544,7 +568,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             const float2 ml = warp_ml[w][item];
             if (ml.y == 0.f) continue;
             const float f = ml.y * ex2(ml.x - (m == -INFINITY ? 0.f : m));
-            const float4 x = *reinterpret_cast<const float4*>(results + w * L::RESULTS + (item * L::OP + c) * 4);
+            const float4 x = *reinterpret_cast<const float4*>(rings + w * L::RING + (item * L::OP + c) * 4);
             l += f;
             o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
         }
@@ -1174,8 +1198,8 @@ QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bit
     const int64_t table = (int64_t)width * block_tokens, window_keys = (int64_t)window + rows + 16;
     p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
     p.cut.least = p.items > 16 ? 256 : 512;
-    p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < 4 * want;
-    p.cut.want = (float)std::max(want / 2, want - 0.5 * lanes);   // the shares' rounding adds half a share for each lane
+    p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < (p.items > 16 ? 1 : 4) * want;
+    p.cut.want = (float)std::max(want / 2, want - lanes);   // a lane's last share is a part of one
     p.slots = p.cut.split ? lanes + (int)std::min(want, (double)lanes * (double)table / p.cut.least) + 1 : lanes;   // a lane's last share is a part of one
     if (p.cut.split) p.bytes = (int64_t)p.slots * rows * q_heads * ((int64_t)d * 4 + 8);
     return p;
