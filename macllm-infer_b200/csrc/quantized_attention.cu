@@ -116,8 +116,8 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 
 // ---- few items -----------------------------------------------------------------------------------------------------
 //
-// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks steps of 32 keys, whose codes and scales bulk copies
-// bring into a ring of its own.  Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
+// A CTA takes a share of one lane's keys for NT * 8 (row, query head) items of one KV head; each of its warps walks steps of 32 keys, whose codes and scales asynchronous
+// copies of 16 bytes bring into a ring of its own (bulk copies take their operands from the warp's uniform registers: eight threads with one each cost 80 instructions for 16 keys).  Items are the short side of both products, S^T = K Q^T and O^T = V^T P^T, which run over the codes themselves: a code's bits alone
 // are the f16 number c 2^-24 (a subnormal, which the tensor cores take in full), so that it costs a mask and half a shift.  With steps and lowest values of the groups
 //   q . k = sum_g step_g (q_g . c_g) + low_g sum(q_g),   o = sum_j (w_j step_jg) c_j + sum_j w_j low_jg,
 // steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
@@ -149,10 +149,10 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// A copy of a multiple of 16 bytes, both addresses multiples of 16.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }   // all but the last N groups are there
 // N words of shared memory.
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t at) {
@@ -160,8 +160,17 @@ __device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t at) {
     else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
     else asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
 }
-// The key of a tile that row r of a product stands for: with neighbours swapped in every other pair, the rows that a load takes at once lie on both halves of the banks.
-__device__ __forceinline__ int key_of(int r) { return r ^ (r >> 1 & 1); }
+// The key of a tile that row r of a product stands for.  A load of eight rows of K takes keys 0, 4, 1, 5 and 2, 6, 3, 7 at once, one of V keys 0 .. 3, or 4 .. 7, and so on.
+__device__ __forceinline__ int key_of(int r) { return (r & 8) | (r & 7) >> 1 | (r & 1) << 2; }
+// Where byte b of a key's codes lies in its tile: the 32 bytes that a load takes of each of four keys are on four different quarters of the banks (8-bit codes of heads of 64, whose loads of K
+// take 64 bytes of two keys: on two of four).
+template <int ROW>
+__device__ __forceinline__ uint32_t place_in_tile(int key, int b) {
+    const int turn = (key & 3) ^ (key >> 1 & 2);
+    if constexpr (ROW == 32) return (key ^ (key >> 1 & 2)) * 32 + b;
+    else if constexpr (ROW == 64) return key * 64 + (b ^ (turn & 2) << 4);
+    else return key * ROW + (b ^ turn << 5);
+}
 
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -173,7 +182,6 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
     using L = Few<D, BITS, NT>;
     constexpr int G = L::G;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[kWarps * L::STAGES];
     __shared__ float item_factor[L::ITEMS], item_sums[L::ITEMS][G];
     __shared__ float2 warp_ml[kWarps][L::ITEMS];
     uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);   // a warp's results at the end
@@ -195,7 +203,6 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
     const int my_steps = n_steps > warp ? (n_steps - warp + kWarps - 1) / kWarps : 0;
 
     const uint32_t ring = smem_u32(rings + warp * L::RING);
-    uint64_t* full = bars + warp * L::STAGES;
     const int32_t* table = a.lanes.tables + lane_id * a.lanes.ld_table;
     auto tile_of = [&](int i) { return ((i >> 1) * kWarps + warp) * kHalves + (i & 1); };   // of the warp's half i
     // the page numbers of 32 halves sit in the warp's threads, those of the next 32 on their way
@@ -208,34 +215,42 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
         return 0;
     };
     int page_now = page_of(lane), page_next = my_steps > 16 ? page_of(32 + lane) : 0;
-    // eight threads bring a step: four its first half's codes of keys, of values, scales of keys, of values, four its second's
-    const int part = lane & 3;
-    const uint8_t* part_from = part < 2 ? (part == 0 ? p.k_codes : p.v_codes) : reinterpret_cast<const uint8_t*>(part == 2 ? p.k_scales : p.v_scales);
-    const int64_t part_page = part < 2 ? p.codes_stride : p.scales_stride * 4;
-    const int part_row = part < 2 ? L::ROW : G * 4;
-    const uint32_t part_bytes = part < 2 ? L::CODES : L::SCALES, part_to = (part < 2 ? part * L::CODES : 2 * L::CODES + (part - 2) * L::SCALES) + (lane >> 2) * L::HALF;
-    auto load_step = [&](int i) {   // the whole warp
-        if ((i & 15) == 0 && i > 0) {
-            page_now = page_next;
-            page_next = page_of(2 * i + 32 + lane);
+    // 16 bytes to a thread and copy: codes in runs of 512, the scales of 16 keys by neighbouring threads
+    constexpr int RUNS = L::CODES / 512, SCALE_COPIES = L::SCALES / 16;   // 1 .. 8; 4, 8, 16
+    static_assert(L::CODES % 512 == 0, "whole runs");
+    uint32_t to[RUNS];
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) to[r] = ring + place_in_tile<L::ROW>((r * 512 + lane * 16) / L::ROW, (r * 512 + lane * 16) % L::ROW);
+    const bool scale_of_keys = lane < SCALE_COPIES;
+    const int scale_copy = scale_of_keys ? lane : lane - SCALE_COPIES;
+    const uint32_t scale_to = ring + 2 * L::CODES + (scale_of_keys ? 0 : L::SCALES) + scale_copy * 16;
+    const uint32_t* scales_from = (scale_of_keys ? p.k_scales : p.v_scales) + (int64_t)kvh * p.block_tokens * G + scale_copy * 4;
+    const uint8_t *keys_from = p.k_codes + (int64_t)kvh * p.block_tokens * L::ROW + lane * 16, *values_from = p.v_codes + (int64_t)kvh * p.block_tokens * L::ROW + lane * 16;
+    auto load_step = [&](int i) {   // the whole warp; a group of copies, an empty one behind the last step
+        if (i < my_steps) {
+            if ((i & 15) == 0 && i > 0) {
+                page_now = page_next;
+                page_next = page_of(2 * i + 32 + lane);
+            }
+            const uint32_t st = (i & (L::STAGES - 1)) * L::STAGE;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                const int64_t page = __shfl_sync(0xffffffffu, page_now, (2 * i + h) & 31);
+                const int tile = tile_of(2 * i + h), row = (begin + tile * kTile) & (p.block_tokens - 1);
+                if (tile >= n_tiles) break;
+                const int64_t at = page * p.codes_stride + row * L::ROW;
+#pragma unroll
+                for (int r = 0; r < RUNS; ++r) {
+                    copy16(to[r] + st + h * L::HALF, keys_from + at + r * 512);
+                    copy16(to[r] + st + h * L::HALF + L::CODES, values_from + at + r * 512);
+                }
+                if (lane < 2 * SCALE_COPIES) copy16(scale_to + st + h * L::HALF, scales_from + page * p.scales_stride + row * G);
+            }
         }
-        const int half = lane >> 2 & 1;
-        const int64_t page = __shfl_sync(0xffffffffu, page_now, (2 * i & 31) + half);
-        const int tile = tile_of(2 * i + half), st = i & (L::STAGES - 1);
-        if (lane == 0) bar_expect_tx(&full[st], tile + 1 < n_tiles ? L::STAGE : L::HALF);
-        __syncwarp();
-        if (lane < 8 && tile < n_tiles) {
-            const int row = kvh * p.block_tokens + ((begin + tile * kTile) & (p.block_tokens - 1));
-            bulk_load(ring + st * L::STAGE + part_to, part_from + page * part_page + (int64_t)row * part_row, part_bytes, &full[st]);
-        }
+        copies_end();
     };
-    if (lane == 0) {
-        for (int i = 0; i < L::STAGES; ++i) bar_init(&full[i], 1);
-        bar_init_fence();
-    }
-    __syncwarp();
 #pragma unroll 1
-    for (int i = 0; i < min(L::STAGES, my_steps); ++i) load_step(i);
+    for (int i = 0; i < L::STAGES; ++i) load_step(i);
 
     // queries: a warp has an item, V neighbouring values to a thread
     constexpr int V = D / 32;
@@ -325,13 +340,11 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
     }
     float cap_step = 0.f, to_step = 0.f;   // a power of two no step so far exceeds; kWeightScale over it
     const int key0 = key_of(gid), va = key_of(2 * tq), vb = key_of(2 * tq + 1);
-    bool ok = true;
 #pragma unroll 1
     for (int i = 0; i < my_steps; ++i) {
-        const int st = i & (L::STAGES - 1);
-        ok = __all_sync(0xffffffffu, bar_wait(&full[st], i / L::STAGES & 1));
-        if (!ok) break;
-        const uint32_t stage = ring + st * L::STAGE;
+        copies_wait<L::STAGES - 1>();
+        __syncwarp();   // the other threads' too
+        const uint32_t stage = ring + (i & (L::STAGES - 1)) * L::STAGE;
         const int pos0 = begin + tile_of(2 * i) * kTile;
         const bool whole = pos0 >= all_lo && pos0 + kStep <= all_hi;
         // ---- scores
@@ -351,8 +364,9 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 uint32_t w0[BITS / 2], w1[BITS / 2];   // words of the thread's two keys
-                lds(w0, kt + key0 * L::ROW + j * (kQuantGroup * BITS / 8) + tq * (BITS * 2));
-                lds(w1, kt + (key0 + 8) * L::ROW + j * (kQuantGroup * BITS / 8) + tq * (BITS * 2));
+                const uint32_t at_key = kt + place_in_tile<L::ROW>(key0, j * (kQuantGroup * BITS / 8) + tq * (BITS * 2));
+                lds(w0, at_key);
+                lds(w1, at_key + 8 * L::ROW);   // the same place of eight keys on
                 float acc[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             for (int j = 0; j < G; ++j) {
                 uint32_t w[4][BITS / 4];   // eight values of each of four keys
 #pragma unroll
-                for (int k = 0; k < 4; ++k) lds(w[k], vt + ((k & 1 ? vb : va) + (k >> 1) * 8) * L::ROW + j * (kQuantGroup * BITS / 8) + gid * BITS);
+                for (int k = 0; k < 4; ++k) lds(w[k], vt + place_in_tile<L::ROW>(k & 1 ? vb : va, j * (kQuantGroup * BITS / 8) + gid * BITS) + (k >> 1) * 8 * L::ROW);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {   // values 2 u and 2 u + 1 of the eight
                     uint32_t a0, a1, a2, a3;
@@ -519,13 +533,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             }
         }
         __syncwarp();
-        if (i + L::STAGES < my_steps) load_step(i + L::STAGES);
+        load_step(i + L::STAGES);
     }
-    if (!ok) {   // copies in flight land before the CTA ends
-        if (lane == 0) tell(a.lanes.status, kDevWait);
-        for (int st = 0; st < L::STAGES; ++st) bar_wait(&full[st], 0), bar_wait(&full[st], 1);
-    }
-
     // ---- a warp's results, over its own sum: [item][D] and (maximum, sum)
     float* mine = reinterpret_cast<float*>(rings + warp * L::RING);
     __syncwarp();
@@ -538,7 +547,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             const int item = n * 8 + 2 * tq + h;
-            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], ok ? l : NAN);
+            if (gid == 0) warp_ml[warp][item] = make_float2(m_run[n][h], l);
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 float low = low_acc[n][j][h];
@@ -1082,26 +1091,31 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     }
 }
 
-// ---- shares joined: a warp to a (row, query head) ----------------------------------------------------------------------
-
-template <typename T, int D>
+// ---- shares joined ---------------------------------------------------------------------------------------------------
+//
+// WARPS warps to a (row, query head), a part to each in turn, eight of them on their way; where parts are many and rows few, the chain of loads is what it takes (48 rows of 100 parts: 18 us with a warp each).
+template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ QuantAttnArgs a, const __grid_constant__ QuantAttnCut cut, int items_of_block, const float* part_o, const float2* part_ml) {
-    constexpr int V = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.q_heads / a.pools.kv_heads;
-    const int lane_id = blockIdx.x, i = blockIdx.y * 4 + warp;
+    constexpr int V = D / 32, ROWS = 4 / WARPS, AHEAD = 8;
+    __shared__ float sums[WARPS > 1 ? WARPS : 1][D];
+    __shared__ float2 warp_ml[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.q_heads / a.pools.kv_heads, mine = warp % WARPS;
+    const int lane_id = blockIdx.x;
     const Piece piece = piece_of(a, cut, 0, lane_id);
     const LaneRange at = lane_range(a, lane_id);
     pdl_wait();
     if (piece.shares == 1) return;   // written as it is
-    const int64_t n_rows = (int64_t)a.lanes.rows * a.q_heads;
-    for (int64_t at_row = i; at_row < (int64_t)at.n * a.q_heads; at_row += (int64_t)gridDim.y * 4) {
-        const int r = (int)(at_row / a.q_heads), head = (int)(at_row - (int64_t)r * a.q_heads), item = r * g + head % g, item0 = item / items_of_block * items_of_block;
-        const int used = max(1, shares_of(a, at, item0, min(items_of_block, at.n * g - item0), g, piece.shares).used());
+    const int64_t n_rows = (int64_t)a.lanes.rows * a.q_heads, n = (int64_t)at.n * a.q_heads;
+    for (int64_t row0 = (int64_t)blockIdx.y * ROWS; row0 < n; row0 += (int64_t)gridDim.y * ROWS) {
+        const int64_t at_row = row0 + warp / WARPS;
+        const bool there = at_row < n;
+        const int r = there ? (int)(at_row / a.q_heads) : 0, head = there ? (int)(at_row - (int64_t)r * a.q_heads) : 0, item = r * g + head % g, item0 = item / items_of_block * items_of_block;
+        const int used = there ? max(1, shares_of(a, at, item0, min(items_of_block, at.n * g - item0), g, piece.shares).used()) : 0;
         const int64_t row = piece.slot * n_rows + at_row;
         float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = 0.f;
-        for (int s0 = 0; s0 < used; s0 += 32) {
+        for (int s0 = mine * 32; s0 < used; s0 += WARPS * 32) {
             const float2 ml = s0 + lane < used ? __ldcg(part_ml + (s0 + lane) * n_rows + row) : make_float2(-INFINITY, 0.f);
             const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
             const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ml.y * ex2(ml.x - m_use);
@@ -1109,18 +1123,52 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Quant
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] *= old;
             m = m_new;
-            for (int s = 0; s < min(32, used - s0); ++s) {
-                const float w = __shfl_sync(0xffffffffu, f, s);
-                if (w == 0.f) continue;
-                const float* src = part_o + ((s0 + s) * n_rows + row) * D + lane * V;
+            const int parts = min(32, used - s0);
+            for (int b = 0; b < parts; b += AHEAD) {
+                float x[AHEAD][V], w[AHEAD];
 #pragma unroll
-                for (int j = 0; j < V; j += 2) {
-                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src + j));
-                    o[j] = fmaf(w, y.x, o[j]);
-                    o[j + 1] = fmaf(w, y.y, o[j + 1]);
+                for (int s = 0; s < AHEAD; ++s) {
+                    w[s] = b + s < 32 ? __shfl_sync(0xffffffffu, f, b + s) : 0.f;   // 0 behind the last part
+#pragma unroll
+                    for (int j = 0; j < V; ++j) x[s][j] = 0.f;
+                    if (w[s] == 0.f) continue;
+                    const float* src = part_o + ((s0 + b + s) * n_rows + row) * D + lane * V;
+#pragma unroll
+                    for (int j = 0; j < V; j += 2) {
+                        const float2 y = __ldcg(reinterpret_cast<const float2*>(src + j));
+                        x[s][j] = y.x;
+                        x[s][j + 1] = y.y;
+                    }
                 }
+#pragma unroll
+                for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] = fmaf(w[s], x[s][j], o[j]);
             }
         }
+        if constexpr (WARPS > 1) {
+            if (lane == 0) warp_ml[warp] = make_float2(m, l);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sums[mine][lane * V + j] = o[j];
+            __syncthreads();
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, warp_ml[w].x);
+            l = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float2 ml = warp_ml[w];
+                if (ml.y == 0.f) continue;
+                const float f = ex2(ml.x - (top == -INFINITY ? 0.f : top));
+                l = fmaf(ml.y, f, l);
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] = fmaf(f, sums[w][lane * V + j], o[j]);
+            }
+            __syncthreads();
+        }
+        if (!there || mine != 0) continue;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         T* out = static_cast<T*>(a.out) + (int64_t)(at.first + r) * a.ldo + head * D + lane * V;
 #pragma unroll
@@ -1179,8 +1227,10 @@ void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cud
     }
     if (p.cut.split) {
         const int64_t rows = (int64_t)a.lanes.rows * a.q_heads;
-        launch_pdl(join_kernel<T, D>, dim3((unsigned)a.lanes.lanes, (unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(128), 0, s, a, p.cut, p.items, (const float*)part_o,
-                   (const float2*)part_ml);
+        // rows that do not fill the SMs with a warp each get four
+        const bool few_rows = rows * a.lanes.lanes <= 4 * 16 * kSms;
+        launch_pdl(few_rows ? join_kernel<T, D, 4> : join_kernel<T, D, 1>, dim3((unsigned)a.lanes.lanes, (unsigned)std::min<int64_t>(few_rows ? rows : (rows + 3) / 4, 4096)), dim3(128), 0, s, a, p.cut,
+                   p.items, (const float*)part_o, (const float2*)part_ml);
         MK_LAUNCH_CHECK();
     }
 }
@@ -1199,7 +1249,8 @@ QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bit
     p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
     p.cut.least = p.items > 16 ? 256 : 512;
     p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < (p.items > 16 ? 1 : 4) * want;
-    p.cut.want = (float)std::max(want / 2, want - lanes);   // a lane's last share is a part of one
+    // a lane's last share is a part of one; CTAs of few items are many to an SM and may come in a second wave (48 lanes of 200 to 6000 tokens: 51 us where one wave of larger ones takes 56)
+    p.cut.want = (float)(p.items > 16 ? std::max(want / 2, want - lanes) : want);
     p.slots = p.cut.split ? lanes + (int)std::min(want, (double)lanes * (double)table / p.cut.least) + 1 : lanes;   // a lane's last share is a part of one
     if (p.cut.split) p.bytes = (int64_t)p.slots * rows * q_heads * ((int64_t)d * 4 + 8);
     return p;
