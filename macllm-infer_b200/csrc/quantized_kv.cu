@@ -52,35 +52,41 @@ __device__ __forceinline__ int lane_of_row(const QuantLanes& a, int t) {
     return lo;
 }
 
-// Where a row's token is: its page, or -1 where it has none (rows of no lane, rows in front of a lane's first token, what the arrays should not hold).
+// Where a row's token is; page: -1 where it has none (in front of a lane's first token, or what the arrays should not hold), -2 where the row belongs to no lane.
 struct Place {
     int page, in_page;
-    bool mine;   // the row belongs to a lane
 };
-__device__ __forceinline__ Place place_of_row(const QuantLanes& a, const QuantPools& p, int t) {
-    int lane, begin, end;
+// Of row first + the thread's number in its warp, where that is below `rows`; the whole warp.
+__device__ __forceinline__ Place place_of_row(const QuantLanes& a, const QuantPools& p, int first, int rows) {
+    const int t = first + (threadIdx.x & 31);
+    int lane = 0, begin, end;
     if (a.cu == nullptr) {
-        lane = t / a.rows;
+        lane = min(t, a.total - 1) / a.rows;
         begin = lane * a.rows;
         end = begin + a.rows;
     } else {
-        lane = lane_of_row(a, t);
+        lane = lane_of_row(a, first);
+        for (int hi = a.lanes; rows > 1 && hi - lane > 1;) {   // the thread's own row, behind the first one's lane
+            const int mid = (lane + hi) / 2;
+            if (a.cu[mid] <= t) lane = mid;
+            else hi = mid;
+        }
         begin = a.cu[lane];
         end = a.cu[lane + 1];
     }
-    Place r{-1, 0, t >= begin && t < end};
-    if (!r.mine) return r;
+    Place r{-2, 0};
+    if ((int)(threadIdx.x & 31) >= rows || t < begin || t >= end) return r;
+    r.page = -1;
     const int length = a.lengths[lane];
-    const bool first = (threadIdx.x & 31) == 0;
     if (length < 0 || length > (int64_t)a.width << p.bt_shift) {
-        if (first) tell(a.status, kDevBadRange);
+        tell(a.status, kDevBadRange);
         return r;
     }
     const int position = length - (end - t);
     if (position < 0) return r;
     const int page = a.tables[lane * a.ld_table + (position >> p.bt_shift)];
     if (page < 0 || page >= p.pages) {
-        if (first) tell(a.status, kDevBadPage);
+        tell(a.status, kDevBadPage);
         return r;
     }
     r.page = page;
@@ -88,119 +94,172 @@ __device__ __forceinline__ Place place_of_row(const QuantLanes& a, const QuantPo
     return r;
 }
 
-// A warp has one row of K or V: eight values to a thread, a group to eight threads.
-template <typename T, int BITS>
+// Codes of eight values x under (step, low); step is positive.  The quotient by a reciprocal is off by 2^-22 of it, 2^-14 at most, so that it decides wherever it is not that near to a half.
+template <int BITS>
+__device__ __forceinline__ void codes_of(const float (&x)[8], float low, float step, uint32_t (&word)[BITS / 4]) {
+    constexpr int L = (1 << BITS) - 1;
+    constexpr float kWhole = 12582912.f;   // 2^23 + 2^22: sums keep whole numbers, in their lowest bits
+    const float inv = 1.0f / step;
+    float off = inv < INFINITY ? 0.f : 1.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float q = (x[j] - low) * inv, c = fminf(q, (float)L) + kWhole;
+        off = fmaxf(off, fabsf(q - (c - kWhole)));
+        word[j * BITS / 32] = j * BITS % 32 == 0 ? __float_as_uint(c) & L : word[j * BITS / 32] | (__float_as_uint(c) & L) << (j * BITS % 32);
+    }
+    if (off < 0.4999f) return;
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) word[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) word[j * BITS / 32] |= min((uint32_t)L, (uint32_t)__float2int_rn(__fdiv_rn(x[j] - low, step))) << (j * BITS % 32);
+}
+
+// A warp has ROWS rows of K or V, and their places in as many threads; eight values to a thread, a group to eight threads, four of a thread's pieces on their way together.
+constexpr int kAhead = 4;
+
+template <typename T, int BITS, int ROWS>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_constant__ QuantRowsArgs a) {
     constexpr int L = (1 << BITS) - 1;
     const QuantPools& p = a.pools;
-    const int lane = threadIdx.x & 31, t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (t >= a.lanes.total) return;
-    const Place at = place_of_row(a.lanes, p, t);
-    if (at.page < 0) return;
+    const int lane = threadIdx.x & 31, first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * ROWS;
+    if (first >= a.lanes.total) return;
+    const Place place = place_of_row(a.lanes, p, first, ROWS);
     const bool keys = blockIdx.y == 0;
-    const T* rows = static_cast<const T*>(keys ? a.k : a.v) + t * (keys ? a.k_row : a.v_row);
-    const int64_t head_stride = keys ? a.k_head : a.v_head;
-    uint8_t* codes = (keys ? p.k_codes : p.v_codes) + at.page * p.codes_stride;
-    uint32_t* scales = (keys ? p.k_scales : p.v_scales) + at.page * p.scales_stride;
-    const int pieces = p.d / 8, groups = p.d / kQuantGroup;
-    for (int i0 = 0; i0 < p.kv_heads * pieces; i0 += 32) {
-        const int i = i0 + lane, head = i / pieces, piece = i - head * pieces;
-        if (i >= p.kv_heads * pieces) return;   // whole groups of eight threads
-        const uint32_t group_mask = 0xffu << (lane & 24);
-        const uint4 w = *reinterpret_cast<const uint4*>(rows + head * head_stride + piece * 8);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-        float x[8], low = INFINITY, high = -INFINITY;
+    const int64_t row_stride = keys ? a.k_row : a.v_row, head_stride = keys ? a.k_head : a.v_head;
+    const int pieces_shift = p.d == 64 ? 3 : (p.d == 128 ? 4 : 5), n = p.kv_heads << pieces_shift;
+#pragma unroll 1
+    for (int r = 0; r < ROWS; ++r) {
+        const int page = __shfl_sync(0xffffffffu, place.page, r), in_page = __shfl_sync(0xffffffffu, place.in_page, r);
+        if (page < 0) continue;
+        const T* row = static_cast<const T*>(keys ? a.k : a.v) + (first + r) * row_stride;
+        uint8_t* codes = (keys ? p.k_codes : p.v_codes) + page * p.codes_stride;
+        uint32_t* scales = (keys ? p.k_scales : p.v_scales) + page * p.scales_stride;
+        for (int i0 = lane; i0 - lane < n; i0 += 32 * kAhead) {
+            uint4 w[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 v = Two<T>::wide(u[j]);
-            x[2 * j] = v.x;
-            x[2 * j + 1] = v.y;
-            low = min_nan(low, min_nan(v.x, v.y));
-            high = max_nan(high, max_nan(v.x, v.y));
-        }
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
+                w[k] = i < n ? *reinterpret_cast<const uint4*>(row + head * head_stride + piece * 8) : make_uint4(0u, 0u, 0u, 0u);
+            }
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            low = min_nan(low, __shfl_xor_sync(group_mask, low, o));
-            high = max_nan(high, __shfl_xor_sync(group_mask, high, o));
-        }
-        const float range = high - low;
-        uint32_t pair = Two<T>::pack(__fdiv_rn(range, (float)L), low);
-        if (!isfinite(range)) pair = Two<T>::pack(NAN, NAN);
-        const float step = Two<T>::wide(pair).x;
-        uint32_t word[BITS / 4] = {};
-        if (step > 0.f) {
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
+                if (i - lane >= n) break;
+                const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                float x[8], low = INFINITY, high = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t c = min((uint32_t)L, (uint32_t)__float2int_rn(__fdiv_rn(x[j] - low, step)));
-                word[j * BITS / 32] |= c << (j * BITS % 32);
+                for (int j = 0; j < 4; ++j) {
+                    const float2 v = Two<T>::wide(u[j]);
+                    x[2 * j] = v.x;
+                    x[2 * j + 1] = v.y;
+                    low = min_nan(low, min_nan(v.x, v.y));
+                    high = max_nan(high, max_nan(v.x, v.y));
+                }
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) {
+                    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+                    high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
+                }
+                const float range = high - low;
+                uint32_t pair = Two<T>::pack(__fdiv_rn(range, (float)L), low);
+                if (!isfinite(range)) pair = Two<T>::pack(NAN, NAN);
+                const float step = Two<T>::wide(pair).x;
+                uint32_t word[BITS / 4] = {};
+                if (step > 0.f) codes_of<BITS>(x, low, step, word);
+                if (i >= n) break;
+                const int64_t at = ((int64_t)head * p.block_tokens + in_page) << pieces_shift;   // in pieces
+                uint8_t* to = codes + (at + piece) * BITS;
+                if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = word[0];
+                else *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[1]);
+                if ((lane & 7) == 0) scales[(at + piece) >> 3] = pair;
             }
         }
-        const int64_t row = (int64_t)head * p.block_tokens + at.in_page;
-        uint8_t* to = codes + row * (p.d * BITS / 8) + piece * BITS;
-        if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = word[0];
-        else *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[1]);
-        if ((lane & 7) == 0) scales[row * groups + piece / 8] = pair;
     }
 }
 
 // The same the other way; a row without a token becomes zeros, and a value beyond the type's largest that largest (a rounded step may lead there).
-template <typename T, int BITS>
+template <typename T, int BITS, int ROWS>
 __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const __grid_constant__ QuantRowsArgs a) {
     const QuantPools& p = a.pools;
-    const int lane = threadIdx.x & 31, t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (t >= a.lanes.total) return;
-    const Place at = place_of_row(a.lanes, p, t);
-    if (!at.mine) return;
+    const int lane = threadIdx.x & 31, first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * ROWS;
+    if (first >= a.lanes.total) return;
+    const Place place = place_of_row(a.lanes, p, first, ROWS);
     const bool keys = blockIdx.y == 0;
-    T* rows = static_cast<T*>(keys ? a.k : a.v) + t * (keys ? a.k_row : a.v_row);
-    const int64_t head_stride = keys ? a.k_head : a.v_head;
-    const int page = max(at.page, 0);
-    const uint8_t* codes = (keys ? p.k_codes : p.v_codes) + page * p.codes_stride;
-    const uint32_t* scales = (keys ? p.k_scales : p.v_scales) + page * p.scales_stride;
-    const int pieces = p.d / 8, groups = p.d / kQuantGroup;
-    for (int i = lane; i < p.kv_heads * pieces; i += 32) {
-        const int head = i / pieces, piece = i - head * pieces;
-        uint32_t w[4] = {};
-        if (at.page >= 0) {
-            const int64_t row = (int64_t)head * p.block_tokens + at.in_page;
-            const float2 sl = Two<T>::wide(scales[row * groups + piece / 8]);
-            const uint8_t* from = codes + row * (p.d * BITS / 8) + piece * BITS;
-            uint32_t c[2];
-            if constexpr (BITS == 4) c[0] = *reinterpret_cast<const uint32_t*>(from), c[1] = c[0] >> 16;
-            else c[0] = reinterpret_cast<const uint2*>(from)->x, c[1] = reinterpret_cast<const uint2*>(from)->y;
+    const int64_t row_stride = keys ? a.k_row : a.v_row, head_stride = keys ? a.k_head : a.v_head;
+    const int pieces_shift = p.d == 64 ? 3 : (p.d == 128 ? 4 : 5), n = p.kv_heads << pieces_shift;
+#pragma unroll 1
+    for (int r = 0; r < ROWS; ++r) {
+        const int page = __shfl_sync(0xffffffffu, place.page, r), in_page = __shfl_sync(0xffffffffu, place.in_page, r);
+        if (page < -1) continue;
+        T* row = static_cast<T*>(keys ? a.k : a.v) + (first + r) * row_stride;
+        const uint8_t* codes = (keys ? p.k_codes : p.v_codes) + page * p.codes_stride;
+        const uint32_t* scales = (keys ? p.k_scales : p.v_scales) + page * p.scales_stride;
+        for (int i0 = lane; i0 < n; i0 += 32 * kAhead) {
+            uint32_t pair[kAhead], c[kAhead][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float v[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int b = (j & 1) * 2 + h;
-                    const float y = fmaf(sl.x, (float)(c[j >> 1] >> (b * BITS) & ((1u << BITS) - 1)), sl.y);
-                    v[h] = y > Two<T>::largest ? Two<T>::largest : y;   // NaN stays
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
+                pair[k] = c[k][0] = c[k][1] = 0u;
+                if (i >= n || page < 0) continue;
+                const int64_t at = (((int64_t)head * p.block_tokens + in_page) << pieces_shift) + piece;
+                pair[k] = scales[at >> 3];
+                if constexpr (BITS == 4) {
+                    c[k][0] = *reinterpret_cast<const uint32_t*>(codes + at * 4);
+                    c[k][1] = c[k][0] >> 16;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(codes + at * 8);
+                    c[k][0] = x.x;
+                    c[k][1] = x.y;
                 }
-                w[j] = Two<T>::pack(v[0], v[1]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
+                if (i >= n) break;
+                const float2 sl = Two<T>::wide(pair[k]);
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float v[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        // 2^23 + c by its bits
+                        const float code = __uint_as_float((c[k][j >> 1] >> (((j & 1) * 2 + h) * BITS) & ((1u << BITS) - 1)) | 0x4b000000u) - 8388608.f;
+                        v[h] = min_nan(fmaf(sl.x, code, sl.y), Two<T>::largest);
+                    }
+                    w[j] = Two<T>::pack(v[0], v[1]);
+                }
+                *reinterpret_cast<uint4*>(row + head * head_stride + piece * 8) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        *reinterpret_cast<uint4*>(rows + head * head_stride + piece * 8) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
+// Rows of a warp: one where rows are few (a launch of 64 rows of 8 heads of 128 has 128 warps then), eight where there are many, so that looking up their places does not count.
 template <typename F>
-void with_types(const QuantPools& p, F&& f) {
-    if (p.bf16) p.bits == 4 ? f(__nv_bfloat16{}, std::integral_constant<int, 4>{}) : f(__nv_bfloat16{}, std::integral_constant<int, 8>{});
-    else p.bits == 4 ? f(__half{}, std::integral_constant<int, 4>{}) : f(__half{}, std::integral_constant<int, 8>{});
+void with_types(const QuantRowsArgs& a, F&& f) {
+    const bool many = a.lanes.total >= 8 * 148 * 8;
+    auto with_rows = [&](auto type, auto bits) {
+        constexpr int kFew = 1, kMany = 8;
+        const int rows = many ? kMany : kFew, warps = kThreads / 32;
+        const dim3 grid((unsigned)((a.lanes.total + warps * rows - 1) / (warps * rows)), 2);
+        many ? f(type, bits, std::integral_constant<int, kMany>{}, grid) : f(type, bits, std::integral_constant<int, kFew>{}, grid);
+    };
+    using Four = std::integral_constant<int, 4>;
+    using Eight = std::integral_constant<int, 8>;
+    if (a.pools.bf16) a.pools.bits == 4 ? with_rows(__nv_bfloat16{}, Four{}) : with_rows(__nv_bfloat16{}, Eight{});
+    else a.pools.bits == 4 ? with_rows(__half{}, Four{}) : with_rows(__half{}, Eight{});
 }
-
-dim3 row_grid(const QuantRowsArgs& a) { return dim3((unsigned)((a.lanes.total + kThreads / 32 - 1) / (kThreads / 32)), 2); }
 
 }  // namespace
 
 void launch_quantize_rows(const QuantRowsArgs& a, cudaStream_t s) {
-    with_types(a.pools, [&](auto type, auto bits) { quantize_rows_kernel<decltype(type), decltype(bits)::value><<<row_grid(a), kThreads, 0, s>>>(a); });
+    with_types(a, [&](auto type, auto bits, auto rows, dim3 grid) { quantize_rows_kernel<decltype(type), decltype(bits)::value, decltype(rows)::value><<<grid, kThreads, 0, s>>>(a); });
     MK_LAUNCH_CHECK();
 }
 
 void launch_dequantize_rows(const QuantRowsArgs& a, cudaStream_t s) {
-    with_types(a.pools, [&](auto type, auto bits) { dequantize_rows_kernel<decltype(type), decltype(bits)::value><<<row_grid(a), kThreads, 0, s>>>(a); });
+    with_types(a, [&](auto type, auto bits, auto rows, dim3 grid) { dequantize_rows_kernel<decltype(type), decltype(bits)::value, decltype(rows)::value><<<grid, kThreads, 0, s>>>(a); });
     MK_LAUNCH_CHECK();
 }
 

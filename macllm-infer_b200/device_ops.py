@@ -213,7 +213,7 @@ def quantized_pools(pages: int, kv_heads: int, block_tokens: int, head_dim: int,
 
 
 def _quantized(pools, device):
-    """The pools' arguments of an entry point; head size and type beside them."""
+    """The pools' arguments of an entry point; head size, type and KV heads beside them."""
     k_codes, v_codes, k_scales, v_scales = pools
     shape, of_scales, dtype = k_codes.shape, k_scales.shape, k_scales.dtype
     if len(shape) != 4 or len(of_scales) != 5 or of_scales[:3] != shape[:3] or of_scales[4] != 2 or (dtype is not torch.float16 and dtype is not torch.bfloat16):
@@ -221,17 +221,18 @@ def _quantized(pools, device):
     pages, heads, page, row = shape
     groups = of_scales[3]
     dim = groups * _GROUP
-    bits = row * 8 // dim if dim else 0
-    strides, of_strides = k_codes.stride(), k_scales.stride()
-    if (bits * dim != row * 8 or bits not in (4, 8) or k_codes.dtype is not torch.uint8 or v_codes.dtype is not torch.uint8 or v_scales.dtype is not dtype or v_codes.shape != shape
-            or v_scales.shape != of_scales or not k_codes.get_device() == v_codes.get_device() == k_scales.get_device() == v_scales.get_device() == device):
+    if (v_codes.shape != shape or v_scales.shape != of_scales or k_codes.dtype is not torch.uint8 or v_codes.dtype is not torch.uint8 or v_scales.dtype is not dtype
+            or (2 * row != dim and row != dim) or not k_codes.get_device() == v_codes.get_device() == k_scales.get_device() == v_scales.get_device() == device):
         raise ValueError("codes are uint8, half a byte or a byte for each value of 64 to a scale, keys and values alike, on the device of the others")
-    if pages > 1 and (v_codes.stride(0) != strides[0] or v_scales.stride(0) != of_strides[0]):
-        raise ValueError("pages of keys and of values are equally far apart")
-    if pages and not (k_codes[0].is_contiguous() and v_codes[0].is_contiguous() and k_scales[0].is_contiguous() and v_scales[0].is_contiguous()):
-        raise ValueError("pages are dense")
-    return dim, dtype, (_TYPES[dtype], bits, k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, strides[0] if pages > 1 else heads * page * row,
-                        of_strides[0] if pages > 1 else heads * page * groups * 2, heads, dim, page)
+    strides, of_strides = k_codes.stride(), k_scales.stride()
+    if v_codes.stride() != strides or v_scales.stride() != of_strides or strides[1:] != (page * row, row, 1) or of_strides[1:] != (page * groups * 2, groups * 2, 2, 1):
+        # a dimension of one element may have any stride
+        if pages > 1 and (v_codes.stride(0) != strides[0] or v_scales.stride(0) != of_strides[0]):
+            raise ValueError("pages of keys and of values are equally far apart")
+        if pages and not (k_codes[0].is_contiguous() and v_codes[0].is_contiguous() and k_scales[0].is_contiguous() and v_scales[0].is_contiguous()):
+            raise ValueError("pages are dense")
+    return dim, dtype, heads, (_TYPES[dtype], 8 * row // dim, k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages,
+                               strides[0] if pages > 1 else heads * page * row, of_strides[0] if pages > 1 else heads * page * groups * 2, heads, dim, page)
 
 
 def _lanes(tables, lengths, cu_seqlens, device):
@@ -242,7 +243,7 @@ def _lanes(tables, lengths, cu_seqlens, device):
 
 def _head_rows(t, shape, dtype, device, what: str):
     """Address and strides of rows [total, kv heads, head size] whose heads are dense."""
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (t.numel() and t.stride(2) != 1):
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (t.stride()[2] != 1 and shape[0]):
         raise ValueError(f"{what} is a {dtype} tensor of shape {tuple(shape)} with dense heads on the device of the others: got {t.dtype} {tuple(t.shape)} on {t.device}")
     row, head, _ = t.stride()
     return t.data_ptr(), row if shape[0] > 1 else shape[1] * shape[2], head if shape[1] > 1 else shape[2]
@@ -258,9 +259,9 @@ def quantize_rows(k, v, pools, tables, lengths, *, cu_seqlens=None, status=None)
     tables [lanes, width] page numbers; lengths [lanes] tokens of each lane, the last of which are its rows (cu_seqlens [lanes + 1], or total / lanes rows each): rows and
     heads may be strided.  Rows in front of a lane's first token are left out.  A group with a value that is not finite reads as NaN."""
     device = k.get_device()
-    dim, dtype, cache = _quantized(pools, device)
-    lanes, where = _lanes(tables, lengths, cu_seqlens, device)
-    shape = torch.Size((k.shape[0] if k.dim() else 0, pools[0].shape[1], dim))
+    dim, dtype, heads, cache = _quantized(pools, device)
+    _, where = _lanes(tables, lengths, cu_seqlens, device)
+    shape = (k.shape[0] if k.dim() else 0, heads, dim)
     _run(device, capi.lib().mk_k_quantize_rows_dev, *_head_rows(k, shape, dtype, device, "k"), *_head_rows(v, shape, dtype, device, "v"), *cache, *where, shape[0],
          _word(status, device))
 
@@ -270,13 +271,13 @@ def dequantize_rows(pools, tables, lengths, total: int, *, cu_seqlens=None, k=No
 
     Returns (k, v) [total, kv_heads, head_dim] of the scales' type.  Rows in front of a lane's first token are zeros, and rows outside cu_seqlens left as ``k`` and ``v`` had them."""
     device = pools[0].get_device()
-    dim, dtype, cache = _quantized(pools, device)
-    lanes, where = _lanes(tables, lengths, cu_seqlens, device)
-    shape = torch.Size((total, pools[0].shape[1], dim))
+    dim, dtype, heads, cache = _quantized(pools, device)
+    _, where = _lanes(tables, lengths, cu_seqlens, device)
+    shape = (total, heads, dim)
     if k is None:
-        k = torch.empty(shape, dtype=dtype, device=pools[0].device)
+        k = pools[2].new_empty(shape)
     if v is None:
-        v = torch.empty(shape, dtype=dtype, device=pools[0].device)
+        v = pools[2].new_empty(shape)
     _run(device, capi.lib().mk_k_dequantize_rows_dev, *cache, *where, total, *_head_rows(k, shape, dtype, device, "k"), *_head_rows(v, shape, dtype, device, "v"),
          _word(status, device))
     return k, v
@@ -295,7 +296,7 @@ def quantized_attention(q, pools, tables, lengths, *, scale: float, cu_seqlens=N
     q [total, q_heads, head_dim] of the scales' type; tables, lengths, cu_seqlens and ``max_rows`` as of ``shared_attention``: a lane's rows are the last of its tokens, whose
     keys and values are in the pages already.  Returns [total, q_heads, head_dim]; a row that sees nothing becomes zeros, rows outside cu_seqlens are left as ``out`` had them."""
     device, shape = q.get_device(), q.shape
-    dim, dtype, cache = _quantized(pools, device)
+    dim, dtype, _, cache = _quantized(pools, device)
     if len(shape) != 3 or q.dtype is not dtype or shape[2] != dim:
         raise ValueError(f"q is a {dtype} tensor [rows, heads, {dim}], as the pools are")
     total, heads, _ = shape
@@ -352,10 +353,9 @@ def token_logprobs(logits, tokens, *, top: int = 0, status=None) -> TokenLogprob
     given = _dense(tokens, _I32, (rows,), device, "tokens")
     if not 0 <= top <= min(64, vocab):
         raise ValueError("top is at most 64 and at most the vocabulary")
-    # one allocation: what a row has, then its likeliest tokens
-    words = torch.empty(rows * (3 + 2 * top), dtype=_F32, device=logits.device)
-    logprobs, entropy, ranks, top_tokens, top_logprobs = words.split((rows, rows, rows, rows * top, rows * top))
-    out = TokenLogprobs(logprobs, entropy, ranks.view(_I32), top_tokens.view(_I32).view(rows, top), top_logprobs.view(rows, top))
+    likeliest = (rows, top)
+    out = TokenLogprobs(torch.empty_like(tokens, dtype=_F32), torch.empty_like(tokens, dtype=_F32), torch.empty_like(tokens), tokens.new_empty(likeliest), tokens.new_empty(likeliest, dtype=_F32))
+    logprobs, entropy, ranks, top_tokens, top_logprobs = out
     _run(device, capi.lib().mk_k_token_logprobs_dev, _TYPES[dtype], logits.data_ptr(), strides[0] if rows > 1 else vocab, rows, vocab, given, top, logprobs.data_ptr(),
          entropy.data_ptr(), ranks.data_ptr(), top_tokens.data_ptr(), top_logprobs.data_ptr(), _word(status, device))
     return out
