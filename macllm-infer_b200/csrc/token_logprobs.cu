@@ -41,20 +41,55 @@ __device__ __forceinline__ uint64_t key_of(float x, int token) { return (uint64_
 __device__ __forceinline__ int token_of(uint64_t key) { return 0xffffff - (int)(key & 0xffffff); }
 __device__ __forceinline__ float value_of(uint64_t key) { return of_ordered((uint32_t)(key >> 24)); }
 
-// Vectors of 16 bytes: their values, maximum, and how many reach a bound.
+// Two 32-bit numbers at once.
+struct Two {
+    float x, y;
+    __device__ __forceinline__ uint64_t bits() const {
+        uint64_t b;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(x), "f"(y));
+        return b;
+    }
+    static __device__ __forceinline__ Two of(uint64_t b) {
+        Two t;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(t.x), "=f"(t.y) : "l"(b));
+        return t;
+    }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()));
+    return Two::of(r);
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()));
+    return Two::of(r);
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()), "l"(c.bits()));
+    return Two::of(r);
+}
+
+// Vectors of 16 bytes: N values, taken two at a time with none below `least`; their maximum; and counts of those that reach a bound, in a form of the type's own that holds a batch's.
 template <typename T>
 struct Vec;
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 template <>
 struct Vec<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ float value(const uint4& v, int i) { return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
+    using Count = int;
+    using Bound = float;
+    static __device__ __forceinline__ float value(const uint4& v, int i) { return __uint_as_float(word_of(v, i)); }
+    static constexpr float lowest = -3.4028234663852886e38f;
+    static __device__ __forceinline__ Bound bound(float x) { return x; }
+    static __device__ __forceinline__ Two two(const uint4& v, int i, Bound least) { return Two{fmaxf(value(v, 2 * i), least), fmaxf(value(v, 2 * i + 1), least)}; }
     static __device__ __forceinline__ float top(const uint4& v) { return max_nan(max_nan(value(v, 0), value(v, 1)), max_nan(value(v, 2), value(v, 3))); }
-    static __device__ __forceinline__ int reach(const uint4& v, float bound) {
-        int n = 0;
+    static __device__ __forceinline__ void reach(const uint4& v, Bound b, Count& n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += value(v, i) >= bound ? 1 : 0;
-        return n;
+        for (int i = 0; i < 4; ++i) n += value(v, i) >= b ? 1 : 0;
     }
+    static __device__ __forceinline__ int count(Count n) { return n; }
     static __device__ __forceinline__ float after(float x) {   // the next number up
         const uint32_t b = __float_as_uint(x + 0.f);
         return __uint_as_float(b & 0x80000000u ? b - 1 : b + 1);
@@ -62,22 +97,32 @@ struct Vec<float> {
 };
 template <typename P>
 __device__ __forceinline__ P as_pair(uint32_t w) { return *reinterpret_cast<const P*>(&w); }
-template <>
-struct Vec<__half> {
+template <typename P>
+struct HalfVec {   // of two 16-bit types
     static constexpr int N = 8;
-    static __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-    static __device__ __forceinline__ float value(const uint4& v, int i) {
-        const float2 f = __half22float2(as_pair<__half2>(word(v, i >> 1)));
-        return i & 1 ? f.y : f.x;
-    }
+    using Count = P;   // up to 4 for each vector of a batch
+    using Bound = P;
     static __device__ __forceinline__ float top(const uint4& v) {
-        const __half2 m = __hmax2_nan(__hmax2_nan(as_pair<__half2>(v.x), as_pair<__half2>(v.y)), __hmax2_nan(as_pair<__half2>(v.z), as_pair<__half2>(v.w)));
+        const P m = __hmax2_nan(__hmax2_nan(as_pair<P>(v.x), as_pair<P>(v.y)), __hmax2_nan(as_pair<P>(v.z), as_pair<P>(v.w)));
         return max_nan(__low2float(m), __high2float(m));
     }
-    static __device__ __forceinline__ int reach(const uint4& v, float bound) {
-        const __half2 b = __float2half2_rn(bound);   // a number of the type
-        const __half2 n = __hadd2(__hadd2(__hge2(as_pair<__half2>(v.x), b), __hge2(as_pair<__half2>(v.y), b)), __hadd2(__hge2(as_pair<__half2>(v.z), b), __hge2(as_pair<__half2>(v.w), b)));
-        return (int)(__low2float(n) + __high2float(n));
+    static __device__ __forceinline__ void reach(const uint4& v, Bound b, Count& n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n = __hadd2(n, __hge2(as_pair<P>(word_of(v, i)), b));
+    }
+    static __device__ __forceinline__ int count(Count n) { return (int)(__low2float(n) + __high2float(n)); }
+};
+template <>
+struct Vec<__half> : HalfVec<__half2> {
+    static __device__ __forceinline__ float value(const uint4& v, int i) {
+        const float2 f = __half22float2(as_pair<__half2>(word_of(v, i >> 1)));
+        return i & 1 ? f.y : f.x;
+    }
+    static constexpr float lowest = -65504.f;
+    static __device__ __forceinline__ Bound bound(float x) { return __float2half2_rn(x); }
+    static __device__ __forceinline__ Two two(const uint4& v, int i, Bound least) {
+        const float2 f = __half22float2(__hmax2(as_pair<__half2>(word_of(v, i)), least));
+        return Two{f.x, f.y};
     }
     static __device__ __forceinline__ float after(float x) {
         const unsigned short b = __half_as_ushort(__float2half_rn(x + 0.f));
@@ -85,22 +130,17 @@ struct Vec<__half> {
     }
 };
 template <>
-struct Vec<__nv_bfloat16> {
-    static constexpr int N = 8;
+struct Vec<__nv_bfloat16> : HalfVec<__nv_bfloat162> {
     static __device__ __forceinline__ float value(const uint4& v, int i) {
-        const uint32_t w = Vec<__half>::word(v, i >> 1);
+        const uint32_t w = word_of(v, i >> 1);
         return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     }
-    static __device__ __forceinline__ float top(const uint4& v) {
-        using P = __nv_bfloat162;
-        const P m = __hmax2_nan(__hmax2_nan(as_pair<P>(v.x), as_pair<P>(v.y)), __hmax2_nan(as_pair<P>(v.z), as_pair<P>(v.w)));
-        return max_nan(__low2float(m), __high2float(m));
-    }
-    static __device__ __forceinline__ int reach(const uint4& v, float bound) {
-        using P = __nv_bfloat162;
-        const P b = __float2bfloat162_rn(bound);
-        const P n = __hadd2(__hadd2(__hge2(as_pair<P>(v.x), b), __hge2(as_pair<P>(v.y), b)), __hadd2(__hge2(as_pair<P>(v.z), b), __hge2(as_pair<P>(v.w), b)));
-        return (int)(__low2float(n) + __high2float(n));
+    static constexpr float lowest = -3.3895313892515355e38f;
+    static __device__ __forceinline__ Bound bound(float x) { return __float2bfloat162_rn(x); }
+    static __device__ __forceinline__ Two two(const uint4& v, int i, Bound least) {
+        const __nv_bfloat162 m = __hmax2(as_pair<__nv_bfloat162>(word_of(v, i)), least);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+        return Two{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
     }
     static __device__ __forceinline__ float after(float x) {
         const uint32_t b = __float_as_uint(x + 0.f) >> 16;
@@ -312,54 +352,67 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     // tokens in front of the given one count where they reach its logit, those behind it where they exceed it; its own vector's are looked at one by one
     const float above = given ? Vec<T>::after(mine) : INFINITY;
     const int own_vector = given && token >= run.first ? (token - run.first) / N : -1;
+    const auto bound_mine = Vec<T>::bound(mine), bound_above = Vec<T>::bound(above), bound_none = Vec<T>::bound(INFINITY);
 
-    Sums my{-INFINITY, 0.f, 0.f, 0};
-    auto add = [&](float v, float m) {
-        const float d = v - m, e = ex2(d * kLog2e);
-        my.z += e;
-        my.zx = fmaf(e, fmaxf(d, -3e38f), my.zx);
+    Two z{0.f, 0.f}, zx{0.f, 0.f};
+    float m_run = -INFINITY;
+    int before = 0;
+    auto add = [&](Two v, Two minus_m) {
+        const Two d = v + minus_m, y = d * Two{kLog2e, kLog2e}, e{ex2(y.x), ex2(y.y)};
+        z = z + e;
+        zx = fma2(e, d, zx);
     };
     auto raise = [&](float top) {   // the maximum to at least `top`; what to subtract
-        const float m = max_nan(my.m, top);
-        if (m > my.m) {
-            const float d = fmaxf(my.m - m, -3e38f), f = ex2(d * kLog2e);
-            my.zx = f > 0.f ? f * fmaf(my.z, d, my.zx) : 0.f;
-            my.z *= f;
+        const float m = max_nan(m_run, top);
+        if (m > m_run) {
+            const float d = fmaxf(m_run - m, -3e38f), f = ex2(d * kLog2e);
+            zx = f > 0.f ? Two{f, f} * fma2(z, Two{d, d}, zx) : Two{0.f, 0.f};
+            z = z * Two{f, f};
         }
-        my.m = m;
+        m_run = m;
         return m == -INFINITY ? 0.f : m;
     };
-    for (int i0 = tid; i0 < run.vectors; i0 += kThreads * kBatch) {
+    // values whose weight is 0 anyway count as this far below the maximum: a weight of 0 times what is left of -inf would not be 0
+    auto least_of = [](float m) { return fmaxf(m - 300.f - fabsf(m), Vec<T>::lowest); };
+    auto batch = [&](int i0, auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
         uint4 v[kBatch];
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
-            if (i0 + k * kThreads < run.vectors) v[k] = run.vector(i0 + k * kThreads);
+            if (kWhole || i0 + k * kThreads < run.vectors) v[k] = run.vector(i0 + k * kThreads);
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
-            if (i0 + k * kThreads < run.vectors) top = max_nan(top, Vec<T>::top(v[k]));
+            if (kWhole || i0 + k * kThreads < run.vectors) top = max_nan(top, Vec<T>::top(v[k]));
         const float m = raise(top);
+        const auto least = Vec<T>::bound(least_of(m));
+        typename Vec<T>::Count n{};
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
             const int i = i0 + k * kThreads;
-            if (i >= run.vectors) break;
+            if (!kWhole && i >= run.vectors) break;
 #pragma unroll
-            for (int j = 0; j < N; ++j) add(Vec<T>::value(v[k], j), m);
-            my.before += Vec<T>::reach(v[k], i < own_vector ? mine : (i == own_vector ? INFINITY : above));
+            for (int j = 0; j < N / 2; ++j) add(Vec<T>::two(v[k], j, least), Two{-m, -m});
+            Vec<T>::reach(v[k], i < own_vector ? bound_mine : (i == own_vector ? bound_none : bound_above), n);
         }
-    }
+        before += Vec<T>::count(n);
+    };
+    int i0 = tid;
+    for (; i0 + (kBatch - 1) * kThreads < run.vectors; i0 += kThreads * kBatch) batch(i0, std::true_type{});
+    if (i0 < run.vectors) batch(i0, std::false_type{});
     {
         const int e = run.edge();
         if (e >= 0) {
-            const float v = (float)x[e];
-            add(v, raise(v));
-            if (given) my.before += e < token ? v >= mine : v >= above;
+            const float v = (float)x[e], m = raise(v);
+            add(Two{fmaxf(v, least_of(m)), -300.f}, Two{-m, 0.f});   // and nothing
+            if (given) before += e < token ? v >= mine : v >= above;
         }
         if (own_vector >= 0 && own_vector < run.vectors && tid < N) {
             const int e = run.first + own_vector * N + tid;
-            if (e != token) my.before += (float)x[e] >= (e < token ? mine : above) ? 1 : 0;
+            if (e != token) before += (float)x[e] >= (e < token ? mine : above) ? 1 : 0;
         }
     }
+    const Sums my{m_run, z.x + z.y, zx.x + zx.y, before};
     const float my_top = my.m;
     Sums all = my;
 #pragma unroll
