@@ -5,7 +5,6 @@
 // c_i stands for low + step c_i.  low is one of the values, so it needs no rounding; the step's is 2^-11 (f16) or 2^-8 (bf16) of it at most and moves no value by more than
 // L times that, and since the codes are made with the rounded step they are the nearest ones under it.  A group with a value, or a range, that is not finite reads as NaN throughout.
 #include "quantized_kv.h"
-#include "attention_math.cuh"
 #include <algorithm>
 
 namespace mk {
@@ -28,6 +27,10 @@ struct Two<__half> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
     static constexpr float largest = 65504.f;
+    using Pair = __half2;
+    static constexpr int kCodeBits = 8;               // of a code in numbers kOne + c of this type, c exact
+    static constexpr uint32_t kOne = 0x64006400u;     // 1024 + c
+    static __device__ __forceinline__ Pair minus_one() { return __float2half2_rn(-1024.f); }
 };
 template <>
 struct Two<__nv_bfloat16> {
@@ -37,7 +40,52 @@ struct Two<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
     static constexpr float largest = 3.3895313892515355e38f;
+    using Pair = __nv_bfloat162;
+    static constexpr int kCodeBits = 4;
+    static constexpr uint32_t kOne = 0x43004300u;     // 128 + c
+    static __device__ __forceinline__ Pair minus_one() { return __float2bfloat162_rn(-128.f); }
 };
+template <typename P>
+__device__ __forceinline__ P as_pair(uint32_t w) { return *reinterpret_cast<const P*>(&w); }
+template <typename P>
+__device__ __forceinline__ uint32_t word_of(P v) { return *reinterpret_cast<const uint32_t*>(&v); }
+
+// What eight codes stand for, as four words.  In numbers of the type themselves, a pair at a time, where they hold the codes (low + step c is rounded once either way), else in 32 bits.
+template <typename T, int BITS>
+__device__ __forceinline__ uint4 values_of(uint32_t pair, const uint32_t (&c)[BITS / 4]) {
+    using W = Two<T>;
+    uint32_t w[4];
+    const float2 sl = W::wide(pair);
+    if constexpr (BITS <= W::kCodeBits) {
+        const auto step = as_pair<typename W::Pair>(__byte_perm(pair, 0, 0x1010)), low = as_pair<typename W::Pair>(__byte_perm(pair, 0, 0x3232));
+        auto two = [&](uint32_t bits) { return word_of(__hfma2(__hadd2(as_pair<typename W::Pair>(bits), W::minus_one()), step, low)); };
+        if constexpr (BITS == 4) {   // pairs (0, 4), (1, 5), (2, 6), (3, 7), then neighbours
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = two((c[0] >> 4 * j & 0x000f000fu) | W::kOne);
+            w[0] = __byte_perm(u[0], u[1], 0x5410), w[1] = __byte_perm(u[2], u[3], 0x5410), w[2] = __byte_perm(u[0], u[1], 0x7632), w[3] = __byte_perm(u[2], u[3], 0x7632);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = two(__byte_perm(c[j >> 1], W::kOne, j & 1 ? 0x5352 : 0x5150));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)   // 2^23 + c by its bits
+                v[h] = fmaf(sl.x, __uint_as_float((c[j * 2 * BITS / 32] >> (j * 2 + h) * BITS % 32 & ((1u << BITS) - 1)) | 0x4b000000u) - 8388608.f, sl.y);
+            w[j] = W::pack(v[0], v[1]);
+        }
+    }
+    // a rounded step may lead beyond the largest number
+    if (fmaf(sl.x, (float)((1 << BITS) - 1), sl.y) > W::largest) {
+        const auto most = as_pair<typename W::Pair>(W::pack(W::largest, W::largest));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = word_of(__hmin2_nan(as_pair<typename W::Pair>(w[j]), most));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // The lane of row t, by a whole warp: the last one whose rows do not begin behind t, 32 of them looked at in each turn.  Whatever cu holds, the index is a lane's.
 __device__ __forceinline__ int lane_of_row(const QuantLanes& a, int t) {
@@ -94,24 +142,39 @@ __device__ __forceinline__ Place place_of_row(const QuantLanes& a, const QuantPo
     return r;
 }
 
-// Codes of eight values x under (step, low); step is positive.  The quotient by a reciprocal is off by 2^-22 of it, 2^-14 at most, so that it decides wherever it is not that near to a half.
+// Codes of eight values x under (step, low); step is positive.  A reciprocal gives the quotient to 2^-22 of it, 2^-14 at most, which decides wherever it is not that near to a half; there, as bf16 values
+// often are, the remainder does: d - c step is exact (c step has at most 19 bits), and twice that against the step says which code is nearer, or that both are and the even one is meant.
 template <int BITS>
 __device__ __forceinline__ void codes_of(const float (&x)[8], float low, float step, uint32_t (&word)[BITS / 4]) {
-    constexpr int L = (1 << BITS) - 1;
+    constexpr uint32_t L = (1u << BITS) - 1;
     constexpr float kWhole = 12582912.f;   // 2^23 + 2^22: sums keep whole numbers, in their lowest bits
     const float inv = 1.0f / step;
-    float off = inv < INFINITY ? 0.f : 1.f;
+    uint32_t c[8];
+    float off = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float q = (x[j] - low) * inv, c = fminf(q, (float)L) + kWhole;
-        off = fmaxf(off, fabsf(q - (c - kWhole)));
-        word[j * BITS / 32] = j * BITS % 32 == 0 ? __float_as_uint(c) & L : word[j * BITS / 32] | (__float_as_uint(c) & L) << (j * BITS % 32);
+        const float q = (x[j] - low) * inv, whole = fminf(q, (float)L) + kWhole;
+        off = fmaxf(off, fabsf(q - (whole - kWhole)));
+        c[j] = __float_as_uint(whole) & L;
     }
-    if (off < 0.4999f) return;
+    if (!(inv < INFINITY)) {   // steps below 2^-128
 #pragma unroll
-    for (int i = 0; i < BITS / 4; ++i) word[i] = 0;
+        for (int j = 0; j < 8; ++j) c[j] = min(L, (uint32_t)__float2int_rn(__fdiv_rn(x[j] - low, step)));
+    } else if (off >= 0.4999f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) word[j * BITS / 32] |= min((uint32_t)L, (uint32_t)__float2int_rn(__fdiv_rn(x[j] - low, step))) << (j * BITS % 32);
+        for (int j = 0; j < 8; ++j) {
+            const float rest = fmaf(-(float)c[j], step, x[j] - low), twice = 2.f * fabsf(rest);
+            const bool other = twice > step || (twice == step && (c[j] & 1u));
+            c[j] = other ? (rest > 0.f ? min(c[j] + 1u, L) : c[j] - 1u) : c[j];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) {
+        constexpr int N = 32 / BITS;
+        word[i] = c[i * N];
+#pragma unroll
+        for (int j = 1; j < N; ++j) word[i] |= c[i * N + j] << j * BITS;
+    }
 }
 
 // A warp has ROWS rows of K or V, and their places in as many threads; eight values to a thread, a group to eight threads, four of a thread's pieces on their way together.
@@ -145,27 +208,32 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_co
             for (int k = 0; k < kAhead; ++k) {
                 const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
                 if (i - lane >= n) break;
+                using P = typename Two<T>::Pair;
                 const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-                float x[8], low = INFINITY, high = -INFINITY;
+                // lowest and highest of the group, the latter as the lowest of what is turned round: one reduction for both
+                P lows = __hmin2_nan(__hmin2_nan(as_pair<P>(u[0]), as_pair<P>(u[1])), __hmin2_nan(as_pair<P>(u[2]), as_pair<P>(u[3])));
+                P highs = __hmax2_nan(__hmax2_nan(as_pair<P>(u[0]), as_pair<P>(u[1])), __hmax2_nan(as_pair<P>(u[2]), as_pair<P>(u[3])));
+                highs = __hneg2(highs);
+                P both = __hmin2_nan(as_pair<P>(__byte_perm(word_of(lows), word_of(highs), 0x5410)), as_pair<P>(__byte_perm(word_of(lows), word_of(highs), 0x7632)));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 v = Two<T>::wide(u[j]);
-                    x[2 * j] = v.x;
-                    x[2 * j + 1] = v.y;
-                    low = min_nan(low, min_nan(v.x, v.y));
-                    high = max_nan(high, max_nan(v.x, v.y));
-                }
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) {
-                    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
-                    high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
-                }
+                for (int o = 1; o < 8; o <<= 1) both = __hmin2_nan(both, as_pair<P>(__shfl_xor_sync(0xffffffffu, word_of(both), o)));
+                const float2 ends = Two<T>::wide(word_of(both));
+                const float low = ends.x, high = -ends.y;
                 const float range = high - low;
                 uint32_t pair = Two<T>::pack(__fdiv_rn(range, (float)L), low);
                 if (!isfinite(range)) pair = Two<T>::pack(NAN, NAN);
                 const float step = Two<T>::wide(pair).x;
                 uint32_t word[BITS / 4] = {};
-                if (step > 0.f) codes_of<BITS>(x, low, step, word);
+                if (step > 0.f) {
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 v = Two<T>::wide(u[j]);
+                        x[2 * j] = v.x;
+                        x[2 * j + 1] = v.y;
+                    }
+                    codes_of<BITS>(x, low, step, word);
+                }
                 if (i >= n) break;
                 const int64_t at = ((int64_t)head * p.block_tokens + in_page) << pieces_shift;   // in pieces
                 uint8_t* to = codes + (at + piece) * BITS;
@@ -195,17 +263,16 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const __grid_
         const uint8_t* codes = (keys ? p.k_codes : p.v_codes) + page * p.codes_stride;
         const uint32_t* scales = (keys ? p.k_scales : p.v_scales) + page * p.scales_stride;
         for (int i0 = lane; i0 < n; i0 += 32 * kAhead) {
-            uint32_t pair[kAhead], c[kAhead][2];
+            uint32_t pair[kAhead], c[kAhead][BITS / 4];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
-                pair[k] = c[k][0] = c[k][1] = 0u;
+                pair[k] = c[k][0] = c[k][BITS / 4 - 1] = 0u;
                 if (i >= n || page < 0) continue;
                 const int64_t at = (((int64_t)head * p.block_tokens + in_page) << pieces_shift) + piece;
                 pair[k] = scales[at >> 3];
                 if constexpr (BITS == 4) {
                     c[k][0] = *reinterpret_cast<const uint32_t*>(codes + at * 4);
-                    c[k][1] = c[k][0] >> 16;
                 } else {
                     const uint2 x = *reinterpret_cast<const uint2*>(codes + at * 8);
                     c[k][0] = x.x;
@@ -215,32 +282,18 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const __grid_
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const int i = i0 + 32 * k, head = i >> pieces_shift, piece = i & ((1 << pieces_shift) - 1);
-                if (i >= n) break;
-                const float2 sl = Two<T>::wide(pair[k]);
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // 2^23 + c by its bits
-                        const float code = __uint_as_float((c[k][j >> 1] >> (((j & 1) * 2 + h) * BITS) & ((1u << BITS) - 1)) | 0x4b000000u) - 8388608.f;
-                        v[h] = min_nan(fmaf(sl.x, code, sl.y), Two<T>::largest);
-                    }
-                    w[j] = Two<T>::pack(v[0], v[1]);
-                }
-                *reinterpret_cast<uint4*>(row + head * head_stride + piece * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (i < n) *reinterpret_cast<uint4*>(row + head * head_stride + piece * 8) = values_of<T, BITS>(pair[k], c[k]);
             }
         }
     }
 }
 
-// Rows of a warp: one where rows are few (a launch of 64 rows of 8 heads of 128 has 128 warps then), eight where there are many, so that looking up their places does not count.
+// Rows of a warp: one where rows are few (a launch of 64 rows of 8 heads of 128 has 128 warps then), four where there are many, so that looking up their places hardly counts (eight leave fewer warps: 12 contexts of 8000 tokens 88 us where four take 83).
 template <typename F>
 void with_types(const QuantRowsArgs& a, F&& f) {
-    const bool many = a.lanes.total >= 8 * 148 * 8;
+    const bool many = a.lanes.total >= 4 * 148 * 8;
     auto with_rows = [&](auto type, auto bits) {
-        constexpr int kFew = 1, kMany = 8;
+        constexpr int kFew = 1, kMany = 4;
         const int rows = many ? kMany : kFew, warps = kThreads / 32;
         const dim3 grid((unsigned)((a.lanes.total + warps * rows - 1) / (warps * rows)), 2);
         many ? f(type, bits, std::integral_constant<int, kMany>{}, grid) : f(type, bits, std::integral_constant<int, kFew>{}, grid);
