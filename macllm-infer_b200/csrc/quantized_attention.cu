@@ -1249,8 +1249,9 @@ QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bit
     p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
     p.cut.least = p.items > 16 ? 256 : 512;
     p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < (p.items > 16 ? 1 : 4) * want;
-    // a lane's last share is a part of one; CTAs of few items are many to an SM and may come in a second wave (48 lanes of 200 to 6000 tokens: 51 us where one wave of larger ones takes 56)
-    p.cut.want = (float)(p.items > 16 ? std::max(want / 2, want - lanes) : want);
+    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 41 us,
+    // with some of them in a second wave 50).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens: 51 us where one wave takes 56).
+    p.cut.want = (float)(p.items > 16 || lanes <= want / 4 ? std::max(want / 2, want - lanes) : want);
     p.slots = p.cut.split ? lanes + (int)std::min(want, (double)lanes * (double)table / p.cut.least) + 1 : lanes;   // a lane's last share is a part of one
     if (p.cut.split) p.bytes = (int64_t)p.slots * rows * q_heads * ((int64_t)d * 4 + 8);
     return p;

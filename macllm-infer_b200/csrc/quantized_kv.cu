@@ -288,15 +288,18 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const __grid_
     }
 }
 
-// Rows of a warp: one where rows are few (a launch of 64 rows of 8 heads of 128 has 128 warps then), four where there are many, so that looking up their places hardly counts (eight leave fewer warps: 12 contexts of 8000 tokens 88 us where four take 83).
+// Rows of a warp: one where rows are few (a launch of 64 rows of 8 heads of 128 has 128 warps then), four where there are many, so that looking up their places hardly counts (eight leave fewer warps: 12 contexts
+// of 8000 tokens 88 us where four take 83), two between (16383 rows written and read: 45 us, with four 48).
 template <typename F>
 void with_types(const QuantRowsArgs& a, F&& f) {
-    const bool many = a.lanes.total >= 4 * 148 * 8;
     auto with_rows = [&](auto type, auto bits) {
-        constexpr int kFew = 1, kMany = 4;
-        const int rows = many ? kMany : kFew, warps = kThreads / 32;
-        const dim3 grid((unsigned)((a.lanes.total + warps * rows - 1) / (warps * rows)), 2);
-        many ? f(type, bits, std::integral_constant<int, kMany>{}, grid) : f(type, bits, std::integral_constant<int, kFew>{}, grid);
+        auto run = [&](auto rows) {
+            constexpr int kEach = decltype(rows)::value * (kThreads / 32);
+            f(type, bits, rows, dim3((unsigned)((a.lanes.total + kEach - 1) / kEach), 2));
+        };
+        if (a.lanes.total < 4096) run(std::integral_constant<int, 1>{});
+        else if (a.lanes.total < 40000) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, 4>{});
     };
     using Four = std::integral_constant<int, 4>;
     using Eight = std::integral_constant<int, 8>;
