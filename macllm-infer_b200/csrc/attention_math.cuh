@@ -33,6 +33,36 @@ __device__ __forceinline__ float capped_wide(float v, float cap, float two_over_
     return y < 0.0625f ? v * fmaf(y, fmaf(y, fmaf(y, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f) : capped(v, cap, two_over_cap);
 }
 
+// FloatPair 32-bit numbers at once.
+struct FloatPair {
+    float x, y;
+    __device__ __forceinline__ uint64_t bits() const {
+        uint64_t b;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(x), "f"(y));
+        return b;
+    }
+    static __device__ __forceinline__ FloatPair of(uint64_t b) {
+        FloatPair t;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(t.x), "=f"(t.y) : "l"(b));
+        return t;
+    }
+};
+__device__ __forceinline__ FloatPair operator+(FloatPair a, FloatPair b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()));
+    return FloatPair::of(r);
+}
+__device__ __forceinline__ FloatPair operator*(FloatPair a, FloatPair b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()));
+    return FloatPair::of(r);
+}
+__device__ __forceinline__ FloatPair fma2(FloatPair a, FloatPair b, FloatPair c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()), "l"(c.bits()));
+    return FloatPair::of(r);
+}
+
 // The 8 x 8 tile of 16-bit numbers that a warp holds as (row lane / 4, columns 2 (lane % 4), + 1), transposed.
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t r;

@@ -77,23 +77,26 @@ __device__ __forceinline__ Piece piece_of(const QuantAttnArgs& a, const QuantAtt
     float total = (float)mine;
     for (int i = 32 + lane; i < n_lanes; i += 32) total += (float)keys_of(i);
     const float per_share = 1.0f / fmaxf((float)c.least, warp_sum(total) / c.want);
+    // lanes with shares of more than half the largest size first: what is left at the end of a call is short
     int before = 0;
-    for (int i0 = 0; i0 < n_lanes; i0 += 32) {
-        const int n = i0 == 0 ? mine : keys_of(i0 + lane), shares = i0 + lane < n_lanes ? max(1, (int)ceilf((float)n * per_share - 1e-3f)) : 0;   // roundings make no share
-        int upto = shares;
+    for (int small = 0; small < 2; ++small)
+        for (int i0 = 0; i0 < n_lanes; i0 += 32) {
+            const float n = (float)(i0 == 0 ? mine : keys_of(i0 + lane)) * per_share;   // in largest shares
+            const int shares = i0 + lane < n_lanes && (n < 0.5f) == (small != 0) ? max(1, (int)ceilf(n - 1e-3f)) : 0;   // roundings make no share
+            int upto = shares;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            upto += before;
+            const uint32_t hit = __ballot_sync(0xffffffffu, of_lane >= 0 ? shares > 0 && i0 + lane == of_lane : slot < upto);
+            if (hit != 0) {
+                const int at = __ffs(hit) - 1, its = __shfl_sync(0xffffffffu, shares, at), first = __shfl_sync(0xffffffffu, upto, at) - its;
+                return Piece{i0 + at, of_lane >= 0 ? 0 : slot - first, its, first};
+            }
+            before = __shfl_sync(0xffffffffu, upto, 31);
         }
-        upto += before;
-        const uint32_t hit = __ballot_sync(0xffffffffu, of_lane >= 0 ? i0 + lane == of_lane : slot < upto);
-        if (hit != 0) {
-            const int at = __ffs(hit) - 1, its = __shfl_sync(0xffffffffu, shares, at), first = __shfl_sync(0xffffffffu, upto, at) - its;
-            return Piece{i0 + at, of_lane >= 0 ? 0 : slot - first, its, first};
-        }
-        before = __shfl_sync(0xffffffffu, upto, 31);
-    }
     return Piece{-1, 0, 1, 0};
 }
 
@@ -1000,13 +1003,15 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 m_run = m_tile;
             }
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            FloatPair part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-            for (int j = 0; j < kKeyTile; ++j) {
-                s[j] = ex2(fmaf(s[j], u, -m_use));
-                part[j & 3] += s[j];
+            for (int j = 0; j < kKeyTile; j += 2) {
+                const FloatPair y = fma2(FloatPair{s[j], s[j + 1]}, FloatPair{u, u}, FloatPair{-m_use, -m_use}), e{ex2(y.x), ex2(y.y)};
+                s[j] = e.x;
+                s[j + 1] = e.y;
+                part[j >> 1 & 1] = part[j >> 1 & 1] + e;
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
             // exponents of the values: the largest so far for all
             ok = __all_sync(0xffffffffu, bar_wait(&v_full[t % VST], t / VST & 1));
             if (!ok) break;
@@ -1249,10 +1254,12 @@ QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bit
     p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
     p.cut.least = p.items > 16 ? 256 : 512;
     p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < (p.items > 16 ? 1 : 4) * want;
-    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 41 us,
-    // with some of them in a second wave 50).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens: 51 us where one wave takes 56).
-    p.cut.want = (float)(p.items > 16 || lanes <= want / 4 ? std::max(want / 2, want - lanes) : want);
-    p.slots = p.cut.split ? lanes + (int)std::min(want, (double)lanes * (double)table / p.cut.least) + 1 : lanes;   // a lane's last share is a part of one
+    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 40 us,
+    // with some of them in a second wave 50).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens: 47 us; shares of the largest size for one
+    // wave 56, half as large ones 52).
+    const double shares = p.items > 16 || lanes <= want / 4 ? std::max(want / 2, want - lanes) : 1.5 * want;
+    p.cut.want = (float)shares;
+    p.slots = p.cut.split ? lanes + (int)std::min(shares, (double)lanes * (double)table / p.cut.least) + 1 : lanes;
     if (p.cut.split) p.bytes = (int64_t)p.slots * rows * q_heads * ((int64_t)d * 4 + 8);
     return p;
 }

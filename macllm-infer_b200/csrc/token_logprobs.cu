@@ -41,36 +41,6 @@ __device__ __forceinline__ uint64_t key_of(float x, int token) { return (uint64_
 __device__ __forceinline__ int token_of(uint64_t key) { return 0xffffff - (int)(key & 0xffffff); }
 __device__ __forceinline__ float value_of(uint64_t key) { return of_ordered((uint32_t)(key >> 24)); }
 
-// Two 32-bit numbers at once.
-struct Two {
-    float x, y;
-    __device__ __forceinline__ uint64_t bits() const {
-        uint64_t b;
-        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(x), "f"(y));
-        return b;
-    }
-    static __device__ __forceinline__ Two of(uint64_t b) {
-        Two t;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(t.x), "=f"(t.y) : "l"(b));
-        return t;
-    }
-};
-__device__ __forceinline__ Two operator+(Two a, Two b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()));
-    return Two::of(r);
-}
-__device__ __forceinline__ Two operator*(Two a, Two b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()));
-    return Two::of(r);
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.bits()), "l"(b.bits()), "l"(c.bits()));
-    return Two::of(r);
-}
-
 // Vectors of 16 bytes: N values, taken two at a time with none below `least`; their maximum; and counts of those that reach a bound, in a form of the type's own that holds a batch's.
 template <typename T>
 struct Vec;
@@ -83,7 +53,7 @@ struct Vec<float> {
     static __device__ __forceinline__ float value(const uint4& v, int i) { return __uint_as_float(word_of(v, i)); }
     static constexpr float lowest = -3.4028234663852886e38f;
     static __device__ __forceinline__ Bound bound(float x) { return x; }
-    static __device__ __forceinline__ Two two(const uint4& v, int i, Bound least) { return Two{fmaxf(value(v, 2 * i), least), fmaxf(value(v, 2 * i + 1), least)}; }
+    static __device__ __forceinline__ FloatPair two(const uint4& v, int i, Bound least) { return FloatPair{fmaxf(value(v, 2 * i), least), fmaxf(value(v, 2 * i + 1), least)}; }
     static __device__ __forceinline__ float top(const uint4& v) { return max_nan(max_nan(value(v, 0), value(v, 1)), max_nan(value(v, 2), value(v, 3))); }
     static __device__ __forceinline__ void reach(const uint4& v, Bound b, Count& n) {
 #pragma unroll
@@ -120,9 +90,9 @@ struct Vec<__half> : HalfVec<__half2> {
     }
     static constexpr float lowest = -65504.f;
     static __device__ __forceinline__ Bound bound(float x) { return __float2half2_rn(x); }
-    static __device__ __forceinline__ Two two(const uint4& v, int i, Bound least) {
+    static __device__ __forceinline__ FloatPair two(const uint4& v, int i, Bound least) {
         const float2 f = __half22float2(__hmax2(as_pair<__half2>(word_of(v, i)), least));
-        return Two{f.x, f.y};
+        return FloatPair{f.x, f.y};
     }
     static __device__ __forceinline__ float after(float x) {
         const unsigned short b = __half_as_ushort(__float2half_rn(x + 0.f));
@@ -137,10 +107,10 @@ struct Vec<__nv_bfloat16> : HalfVec<__nv_bfloat162> {
     }
     static constexpr float lowest = -3.3895313892515355e38f;
     static __device__ __forceinline__ Bound bound(float x) { return __float2bfloat162_rn(x); }
-    static __device__ __forceinline__ Two two(const uint4& v, int i, Bound least) {
+    static __device__ __forceinline__ FloatPair two(const uint4& v, int i, Bound least) {
         const __nv_bfloat162 m = __hmax2(as_pair<__nv_bfloat162>(word_of(v, i)), least);
         const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
-        return Two{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+        return FloatPair{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
     }
     static __device__ __forceinline__ float after(float x) {
         const uint32_t b = __float_as_uint(x + 0.f) >> 16;
@@ -354,11 +324,11 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     const int own_vector = given && token >= run.first ? (token - run.first) / N : -1;
     const auto bound_mine = Vec<T>::bound(mine), bound_above = Vec<T>::bound(above), bound_none = Vec<T>::bound(INFINITY);
 
-    Two z{0.f, 0.f}, zx{0.f, 0.f};
+    FloatPair z{0.f, 0.f}, zx{0.f, 0.f};
     float m_run = -INFINITY;
     int before = 0;
-    auto add = [&](Two v, Two minus_m) {
-        const Two d = v + minus_m, y = d * Two{kLog2e, kLog2e}, e{ex2(y.x), ex2(y.y)};
+    auto add = [&](FloatPair v, FloatPair minus_m) {
+        const FloatPair d = v + minus_m, y = d * FloatPair{kLog2e, kLog2e}, e{ex2(y.x), ex2(y.y)};
         z = z + e;
         zx = fma2(e, d, zx);
     };
@@ -366,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
         const float m = max_nan(m_run, top);
         if (m > m_run) {
             const float d = fmaxf(m_run - m, -3e38f), f = ex2(d * kLog2e);
-            zx = f > 0.f ? Two{f, f} * fma2(z, Two{d, d}, zx) : Two{0.f, 0.f};
-            z = z * Two{f, f};
+            zx = f > 0.f ? FloatPair{f, f} * fma2(z, FloatPair{d, d}, zx) : FloatPair{0.f, 0.f};
+            z = z * FloatPair{f, f};
         }
         m_run = m;
         return m == -INFINITY ? 0.f : m;
@@ -392,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
             const int i = i0 + k * kThreads;
             if (!kWhole && i >= run.vectors) break;
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) add(Vec<T>::two(v[k], j, least), Two{-m, -m});
+            for (int j = 0; j < N / 2; ++j) add(Vec<T>::two(v[k], j, least), FloatPair{-m, -m});
             Vec<T>::reach(v[k], i < own_vector ? bound_mine : (i == own_vector ? bound_none : bound_above), n);
         }
         before += Vec<T>::count(n);
@@ -404,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
         const int e = run.edge();
         if (e >= 0) {
             const float v = (float)x[e], m = raise(v);
-            add(Two{fmaxf(v, least_of(m)), -300.f}, Two{-m, 0.f});   // and nothing
+            add(FloatPair{fmaxf(v, least_of(m)), -300.f}, FloatPair{-m, 0.f});   // and nothing
             if (given) before += e < token ? v >= mine : v >= above;
         }
         if (own_vector >= 0 && own_vector < run.vectors && tid < N) {

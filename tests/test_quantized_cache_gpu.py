@@ -459,6 +459,29 @@ def test_pools_beyond_four_gigabytes(dops):
         assert torch.equal(dops.quantized_attention(q, pools, tables, c.lengths, scale=0.06), dops.quantized_attention(q, c.pools, c.tables, c.lengths, scale=0.06))
 
 
+def spread_lengths(lanes, most, seed):
+    return [1 + (i * 7919 + seed * 131) % 97 * most // 96 * (1 if i % 5 else 0) + i % 3 for i in range(lanes)]
+
+
+@pytest.mark.parametrize("lanes, most", [(2, 9000), (31, 3000), (32, 2500), (33, 2500), (70, 2000), (130, 1500)])
+@pytest.mark.parametrize("dim, q_heads, kv_heads, window", [(64, 8, 2, 0), (128, 4, 1, 0), (128, 4, 4, 700), (256, 6, 2, 0)])
+def test_keys_of_many_lanes_are_shared_out(dops, lanes, most, dim, q_heads, kv_heads, window):
+    """Lanes of very different lengths, more of them than threads of a warp: which CTA has which keys is found on the device."""
+    c = Cache(F16, 4, kv_heads, dim, 64, spread_lengths(lanes, most, dim), 1, seed=18).fill()
+    q = queries(c, q_heads)
+    check_attention(c, q, attend(dops, c, q, window=window), window=window)
+
+
+@pytest.mark.parametrize("lanes, rows, most", [(3, 20, 5000), (33, 20, 1500), (40, 9, 1200), (260, 6, 100), (300, 33, 60)])
+@pytest.mark.parametrize("dim, kv_heads, dtype", [(64, 1, F16), (128, 2, BF16), (256, 1, BF16)])
+def test_lanes_of_many_rows(dops, lanes, rows, most, dim, kv_heads, dtype):
+    lengths = [rows + n for n in spread_lengths(lanes, most, rows)]
+    counts = [max(0, rows - i % 7 * rows // 4) for i in range(lanes)]
+    c = Cache(dtype, 4, kv_heads, dim, 16, lengths, counts, seed=19).fill()
+    q = queries(c, 4 * kv_heads)
+    check_attention(c, q, attend(dops, c, q))
+
+
 def test_repeated_calls_give_the_same_bits(dops):
     for rows, lengths in ((1, [5000, 300, 20000]), (60, [5000, 300, 2000])):
         c = Cache(F16, 4, 2, 128, 16, lengths, rows, seed=15).fill()
