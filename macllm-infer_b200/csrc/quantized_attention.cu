@@ -126,6 +126,9 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 // steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
 // Queries are brought to f16 by a power of two per item, weights by one for the largest step met so far; either is exact.  The running maximum follows only
 // when a score exceeds it by more than 2^kSlack, which a vote of the warp tells.
+// What bounds it is issue slots: about 340 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
+// 4 bits: 47 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 40 us, 2.7 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 123 us, 2.2 TB/s.  Codes by ordinary loads
+// a tile ahead: 62, 124 and 149 us before the keys were shared out by lengths; 32 keys a step do 1.1 times as well as 16, four CTAs on an SM with 128 registers no better than three.
 constexpr int kTile = 16, kHalves = 2, kStep = kHalves * kTile;
 constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;            // base-2 logarithm
@@ -600,10 +603,12 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 // ---- many items ----------------------------------------------------------------------------------------------------
 //
 // A CTA takes SUBS tiles of 128 (row, query head) items of a lane and KV head and walks the keys they see, or a share of them, in tiles of 64, on the fifth-generation tensor
-// cores: scores Q K^T (128 x 64, f32) into one of two areas of tensor memory per tile of items, O += P V with P as the A operand in tensor memory, over its scores.  Four warps bring
-// 16 keys each: bulk copies of codes and scales into a ring, as f16 numbers into the swizzled rows that the products read.  One warp issues the products; the others hold
-// an item to a thread.  Two tiles of items share the numbers made from the codes (about 90 clocks of issue slots per tile of keys and of items, where exponentials and products take 512 each), and
-// one's softmax runs under the other's products.
+// cores: scores Q K^T (128 x 64, f32) into one of two areas of tensor memory per tile of items, O += P V with P as the A operand in tensor memory, over its scores.  Four warps make
+// numbers of keys out of their codes, 16 keys each, four of values: codes into registers two tiles ahead, f16 numbers into the swizzled rows that the products read.  A warp for each tile of items issues its
+// products; four hold an item to a thread.  Two tiles of items share the numbers, and one's softmax runs under the other's products.
+// What bounds it is the chain of a tile's softmax: 2700 clocks for 256 items by 64 keys of heads of 128, half of them exponentials (two warps of a scheduler come to them together), where products take 1024: tensor pipe
+// 37 % busy.  4 portions of 1000 rows, 32 heads of 128 over 4, behind 2500 to 12000 tokens: 400 us, 721 TFLOP/s; 2048 rows of 32 heads over 8 behind 16384: 677 us, 761.  One thread issuing all products: 498 us;
+// codes through bulk copies and shared memory: 441; turns at the exponentials: 441; a fourth of the exponentials as polynomials on the other pipes: 401.
 // A code becomes 1024 + c by its bits, c by a subtraction, and low + step c by one fused multiply-add in f16: rounded once, to 11 bits, as a 16-bit cache would hold it; weights are
 // rounded to 11 bits for the second product.  Scales come with a power of two of their own for every 16 keys (multiples of 2^8, so that neighbours share one): scores are multiplied by the
 // keys', weights by the values' over the largest so far where they differ, so that bf16 caches of any range fit f16.  Values of a chunk of eight lie in the order in which the
@@ -679,7 +684,6 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     const int g = a.q_heads / p.kv_heads;
     // the longest lanes come first, and of each the last rows, which see the most keys: what is left at the end is short
     const int of_slot = p.kv_heads * blocks, slot = blockIdx.x / of_slot, rest = blockIdx.x - slot * of_slot, block = blocks - 1 - rest / p.kv_heads, kvh = rest % p.kv_heads;
-    pdl_trigger();
     const Piece piece = piece_of(a, cut, slot, -1);
     if (piece.lane < 0) return;
     const int lane_id = cut.split ? piece.lane : lane_of_rank(a.lanes, slot), share = piece.share, shares = piece.shares;
@@ -703,6 +707,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;
+    pdl_trigger();   // with the tensor memory taken: the next kernel may wait for some
 
     if (warp >= L::ITEM_WARPS && warp < L::MMA_WARP) {
         // ---- codes to numbers: 16 keys, or their values, of each tile

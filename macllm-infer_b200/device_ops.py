@@ -273,13 +273,19 @@ def dequantize_rows(pools, tables, lengths, total: int, *, cu_seqlens=None, k=No
     device = pools[0].get_device()
     dim, dtype, heads, cache = _quantized(pools, device)
     _, where = _lanes(tables, lengths, cu_seqlens, device)
-    shape = (total, heads, dim)
-    if k is None:
-        k = pools[2].new_empty(shape)
-    if v is None:
-        v = pools[2].new_empty(shape)
-    _run(device, capi.lib().mk_k_dequantize_rows_dev, *cache, *where, total, *_head_rows(k, shape, dtype, device, "k"), *_head_rows(v, shape, dtype, device, "v"),
-         _word(status, device))
+    if total < 0:
+        raise ValueError("total is not negative")
+    shape, row = (total, heads, dim), heads * dim
+    if k is None and v is None:
+        k, v = pools[2].new_empty((2, total, heads, dim)).unbind()
+        to_k, to_v = (k.data_ptr(), row, dim), (v.data_ptr(), row, dim)
+    else:
+        if k is None:
+            k = pools[2].new_empty(shape)
+        if v is None:
+            v = pools[2].new_empty(shape)
+        to_k, to_v = _head_rows(k, shape, dtype, device, "k"), _head_rows(v, shape, dtype, device, "v")
+    _run(device, capi.lib().mk_k_dequantize_rows_dev, *cache, *where, total, *to_k, *to_v, _word(status, device))
     return k, v
 
 

@@ -145,6 +145,8 @@ def test_wrappers_refuse_by_shape_type_and_place(dops):
             calls[0](**change)
     with pytest.raises(ValueError, match="v is"):
         calls[1](v=rows[:1])
+    with pytest.raises(ValueError, match="total"):
+        calls[1](total=-3)
     for change, message in ((dict(q=q.float()), "float16"), (dict(q=q[..., :32]), "64"), (dict(tables=tables[:2], lengths=lengths[:2]), "same number of rows"),
                             (dict(cu_seqlens=torch.zeros(4, dtype=torch.int32)), "max_rows"), (dict(out=q[:2]), "like q"), (dict(q=torch.zeros(3, 64, 8, dtype=F16).transpose(1, 2)[..., :64]), "64|dense")):
         with pytest.raises(ValueError, match=message):

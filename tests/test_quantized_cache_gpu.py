@@ -396,6 +396,17 @@ def test_what_a_row_does_not_see_may_be_anything(dops, rows):
     assert torch.isnan(got[rows:]).all() and torch.equal(torch.isnan(got[:rows]), torch.isnan(want))
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_pages_in_front_of_the_window_may_be_gone(dops, rows):
+    c = Cache(F16, 4, 2, 128, 16, [2000, 300], rows, seed=21).fill()
+    q = queries(c, 8)
+    want = attend(dops, c, q, window=200)
+    for lane, n in enumerate(c.lengths_list):
+        c.tables[lane, :(n - rows - 199) // 16] = -1
+    status = torch.zeros(1, dtype=INT, device="cuda")
+    assert torch.equal(attend(dops, c, q, window=200, status=status), want) and status.item() == 0
+
+
 def test_queries_that_are_not_finite(dops):
     for rows in (1, 40):
         c = Cache(BF16, 4, 2, 64, 16, [100, 100], rows, seed=11).fill()
@@ -526,6 +537,25 @@ def test_captured_and_on_two_streams(dops):
                     r.append(dops.quantized_attention(q, c.pools, c.tables, c.lengths, scale=0.1))
         torch.cuda.synchronize()
         assert all(torch.equal(a, out) for r in results for a in r)
+
+
+@pytest.mark.parametrize("bits, dim, dtype", [(4, 64, F16), (8, 128, BF16), (4, 256, BF16)])
+def test_a_thinned_context(dops, bits, dim, dtype):
+    """Kept tokens of a lane moved together, codes and scales alike: what is read back is what was there."""
+    c = Cache(dtype, bits, 2, dim, 16, [150, 70], 1, seed=20).fill()
+    keep = ints([[0, 1, 2, 17, 40, 41, 99, 149], [3, 5, 64, 69, -1, -1, -1, -1]])
+    counts, first = ints([8, 4]), ints([0, 2])
+    before = [[c.tokens(lane, kind, n) for kind in (0, 1)] for lane, n in enumerate(c.lengths_list)]
+    for k, v in ((c.pools[0], c.pools[1]), (c.pools[2].flatten(3), c.pools[3].flatten(3))):
+        dops.gather_tokens(k[None], v[None], c.tables, keep, counts, c.tables, first)
+    for lane, (n, f) in enumerate(zip((8, 4), (0, 2))):
+        for kind in (0, 1):
+            now = c.tokens(lane, kind, f + n)
+            assert torch.equal(now[f:], before[lane][kind][keep[lane, :n].long()])
+    got = dops.dequantize_rows(c.pools, c.tables, ints([8, 6]), 2)
+    for kind in (0, 1):
+        want = torch.stack([before[lane][kind][p] for lane, p in ((0, 149), (1, 69))])
+        assert ((got[kind].double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2 ** -10) + 2 ** -25).all()
 
 
 def test_a_text_behind_a_forked_prompt(dops):
