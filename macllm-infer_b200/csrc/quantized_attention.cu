@@ -129,6 +129,7 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 // What bounds it is issue slots: about 340 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
 // 4 bits: 47 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 40 us, 2.7 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 123 us, 2.2 TB/s.  Codes by ordinary loads
 // a tile ahead: 62, 124 and 149 us before the keys were shared out by lengths; 32 keys a step do 1.1 times as well as 16, four CTAs on an SM with 128 registers no better than three.
+constexpr int kFewItems = 32;            // of a lane and KV head: more go to the tall kernel
 constexpr int kTile = 16, kHalves = 2, kStep = kHalves * kTile;
 constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;            // base-2 logarithm
@@ -1250,7 +1251,9 @@ void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cud
 QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window) {
     QuantAttnPlan p;
     const int64_t items = (int64_t)rows * (q_heads / kv_heads);
-    p.items = items <= 8 || (items <= 16 && d == 256) ? 8 : (items <= 16 ? 16 : (d == 256 ? kItemTile : 2 * kItemTile));
+    // Up to 32 items go by blocks of 16 (heads of 256: of 8), each of which walks the keys, out of L2 but for the first: 24 lanes of 20 items, heads of 128, 129 us where the tall kernel takes 145; 8 lanes of 32 57 and 59;
+    // heads of 256, 12 lanes of 24, 103 and 125.  With 48 items it is the other way round: 88 and 61, 196 and 146, heads of 64 47 and 36.
+    p.items = items <= 8 || (items <= kFewItems && d == 256) ? 8 : (items <= kFewItems ? 16 : (d == 256 ? kItemTile : 2 * kItemTile));
     p.blocks = (int)std::max<int64_t>(1, (items + p.items - 1) / p.items);
     // one wave of CTAs
     const int ctas = p.items > 16 ? 1 : few_ctas(d, p.items / 8);

@@ -300,7 +300,8 @@ def quantized_attention(q, pools, tables, lengths, *, scale: float, cu_seqlens=N
     """Attention of a ragged batch over a cache in 4 or 8 bits, read as it is.
 
     q [total, q_heads, head_dim] of the scales' type; tables, lengths, cu_seqlens and ``max_rows`` as of ``shared_attention``: a lane's rows are the last of its tokens, whose
-    keys and values are in the pages already.  Returns [total, q_heads, head_dim]; a row that sees nothing becomes zeros, rows outside cu_seqlens are left as ``out`` had them."""
+    keys and values are in the pages already.  Pages wholly in front of every row's window need not be there.  Returns [total, q_heads, head_dim]; a row that sees nothing becomes zeros,
+    rows outside cu_seqlens are left as ``out`` had them."""
     device, shape = q.get_device(), q.shape
     dim, dtype, _, cache = _quantized(pools, device)
     if len(shape) != 3 or q.dtype is not dtype or shape[2] != dim:
