@@ -533,8 +533,13 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma_f16(o_acc[n][j][u], a0, a1, a2, a3, hi_b[n][j][0], hi_b[n][j][1]);
-                        mma_f16(o_acc[n][j][u], a0, a1, a2, a3, lo_b[n][j][0], lo_b[n][j][1]);
+                        // Products align their sums by exponent fields, which for subnormal codes are up to 2^10 above the value: a sum is cut at 2^-17 of it or so.  Over many tiles in one
+                        // accumulator that would add up, so that each tile's is added in 32 bits.
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_f16(part, a0, a1, a2, a3, hi_b[n][j][0], hi_b[n][j][1]);
+                        mma_f16(part, a0, a1, a2, a3, lo_b[n][j][0], lo_b[n][j][1]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o_acc[n][j][u][e] += part[e];
                     }
                 }
             }

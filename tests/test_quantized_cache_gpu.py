@@ -234,7 +234,9 @@ def check_attention(c, q, got, window=0, softcap=0.0, pools=None):
     """Against the definition in 64 bits.
 
     Rounded: the result, to the type (half = eps / 2).  In 32 bits: the products' sums, d of them at the largest intermediate value, which in the form step (q . c) + low sum(q) is
-    sum |q| (step c + |low|); 2^-21 for the exponential; a few 1e-7 of the cap.  Where a lane has many rows, keys, values and weights are rounded to f16 once each (2^-11): a
+    sum |q| (step c + |low|); values likewise, as step c and low
+    apart, where they cancel too; the tensor cores cut a product's sum by its exponent fields, which for codes as f16 subnormals are up to 2^10 above the value: 2^-14 of step c at the most.
+    2^-21 for the exponential; a few 1e-7 of the cap.  Where a lane has many rows, keys, values and weights are rounded to f16 once each (2^-11): a
     score moves by 2^-11 sum |q| |k|, a weight by as much (relative), twice, since the sum moves too.  Weights that underflow f16 are below 2^-24 of the largest."""
     dtype, scale = q.dtype, c.dim ** -0.5
     group = q.shape[1] // c.kv_heads
@@ -244,7 +246,7 @@ def check_attention(c, q, got, window=0, softcap=0.0, pools=None):
     for lane, (n, rows) in enumerate(zip(c.lengths_list, c.rows)):
         k, v = (c.tokens(lane, kind, n).transpose(0, 1).repeat_interleave(group, 0) for kind in (0, 1))
         ids = c.tables[lane, :-(-n // c.page)].long()
-        low = c.pools[2][ids][..., 1].double().repeat_interleave(64, -1).transpose(1, 2).flatten(0, 1)[:n].abs().transpose(0, 1).repeat_interleave(group, 0)
+        low, low_v = (c.pools[kind][ids][..., 1].double().repeat_interleave(64, -1).transpose(1, 2).flatten(0, 1)[:n].abs().transpose(0, 1).repeat_interleave(group, 0) for kind in (2, 3))
         x64 = q[at:at + rows].double().transpose(0, 1)
         p = torch.arange(n - rows, n, device="cuda")[:, None]
         key = torch.arange(n, device="cuda")[None]
@@ -253,10 +255,10 @@ def check_attention(c, q, got, window=0, softcap=0.0, pools=None):
         if softcap:
             x = softcap * torch.tanh(x / softcap)
         w = torch.softmax(x.masked_fill(hidden, -math.inf), -1).nan_to_num(0.0)
-        want, mean = w @ v, w @ v.abs()
+        want, mean, parts = w @ v, w @ v.abs(), w @ (v.abs() + 2 * low_v)
         size = (x64.abs() @ (k.abs() + 2 * low).transpose(1, 2) * scale).masked_fill(hidden, 0.0)
         score = (size.amax(-1, keepdim=True) if n else torch.zeros_like(mean[..., :1])) * ((c.dim + 8) * 2 ** -24 + (2 ** -11 if many else 0)) + 2 ** -21 + 1e-6 * softcap
-        bound = half * want.abs() * (1 + half) + (2 * score + (2 * 2 ** -11 if many else 2 ** -20)) * (mean + want.abs()) + 1e-7 * (dtype == F16)
+        bound = half * want.abs() * (1 + half) + (2 * score + (2 * 2 ** -11 if many else 0)) * (mean + want.abs()) + 2 ** -14 * parts + 1e-7 * (dtype == F16)
         off = (got[at:at + rows].double().transpose(0, 1) - want).abs()
         assert torch.isfinite(off).all(), lane
         assert (off <= bound).all(), (lane, float((off - bound).max()), float((off / bound.clamp_min(1e-30)).max()))
