@@ -126,8 +126,9 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 // steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
 // Queries are brought to f16 by a power of two per item, weights by one for the largest step met so far; either is exact.  The running maximum follows only
 // when a score exceeds it by more than 2^kSlack, which a vote of the warp tells.
-// What bounds it is issue slots: about 340 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
-// 4 bits: 47 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 40 us, 2.7 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 123 us, 2.2 TB/s.  Codes by ordinary loads
+// What bounds it is issue slots: about 370 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
+// 4 bits: 49 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 42 us, 2.6 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 144 us, 1.9 TB/s (outputs of all tiles in one accumulator: 47, 40 and
+// 123 us, but see there).  Codes by ordinary loads
 // a tile ahead: 62, 124 and 149 us before the keys were shared out by lengths; 32 keys a step do 1.1 times as well as 16, four CTAs on an SM with 128 registers no better than three.
 constexpr int kFewItems = 32;            // of a lane and KV head: more go to the tall kernel
 constexpr int kTile = 16, kHalves = 2, kStep = kHalves * kTile;
@@ -1256,8 +1257,8 @@ void launch(const QuantAttnArgs& a, const QuantAttnPlan& p, void* workspace, cud
 QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bits, int block_tokens, int width, int lanes, int rows, int total, int window) {
     QuantAttnPlan p;
     const int64_t items = (int64_t)rows * (q_heads / kv_heads);
-    // Up to 32 items go by blocks of 16 (heads of 256: of 8), each of which walks the keys, out of L2 but for the first: 24 lanes of 20 items, heads of 128, 129 us where the tall kernel takes 145; 8 lanes of 32 57 and 59;
-    // heads of 256, 12 lanes of 24, 103 and 125.  With 48 items it is the other way round: 88 and 61, 196 and 146, heads of 64 47 and 36.
+    // Up to 32 items go by blocks of 16 (heads of 256: of 8), each of which walks the keys, out of L2 but for the first: 24 lanes of 20 items, heads of 128, 137 us where the tall kernel takes 145; 8 lanes of 32 60 and 59;
+    // heads of 256, 12 lanes of 24, 111 and 125.  With 48 items it is the other way round: 88 and 61, 196 and 146, heads of 64 47 and 36.
     p.items = items <= 8 || (items <= kFewItems && d == 256) ? 8 : (items <= kFewItems ? 16 : (d == 256 ? kItemTile : 2 * kItemTile));
     p.blocks = (int)std::max<int64_t>(1, (items + p.items - 1) / p.items);
     // one wave of CTAs
@@ -1267,8 +1268,8 @@ QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bit
     p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
     p.cut.least = p.items > 16 ? 256 : 512;
     p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < (p.items > 16 ? 1 : 4) * want;
-    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 40 us,
-    // with some of them in a second wave 50).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens: 47 us; shares of the largest size for one
+    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 42 us,
+    // with some of them in a second wave about 10 more).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens, before outputs of tiles were added in 32 bits: 47 us; shares of the largest size for one
     // wave 56, half as large ones 52).
     const double shares = p.items > 16 || lanes <= want / 4 ? std::max(want / 2, want - lanes) : 1.5 * want;
     p.cut.want = (float)shares;
