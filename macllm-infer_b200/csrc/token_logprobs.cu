@@ -297,6 +297,25 @@ __device__ __forceinline__ void best_of_run(const Run<T>& run, float my_top, int
     if (tid == 0) s.n_best = min(n, top);
 }
 
+__device__ __forceinline__ void add_weights(FloatPair v, FloatPair minus_m, FloatPair& z, FloatPair& zx) {
+    const FloatPair d = v + minus_m, y = d * FloatPair{kLog2e, kLog2e}, e{ex2(y.x), ex2(y.y)};
+    z = z + e;
+    zx = fma2(e, d, zx);
+}
+// A maximum at the end of the type's numbers has none that far below it, so that -inf counted like the lowest of them: the thread's values once more, one by one, -inf left out.  (Where a larger one
+// came later, what was counted until then has vanished.)  Apart from the rest, which has 5 % more to do where these few lines are in line (2000 rows of bf16 logits 104.7 us, 99.6 so).
+template <typename T>
+__device__ __noinline__ float4 one_by_one(const T* row, int first, int vectors, int edge, float m) {
+    FloatPair z{0.f, 0.f}, zx{0.f, 0.f};
+    auto one = [&](float v) {
+        if (v > -INFINITY) add_weights(FloatPair{v, -300.f}, FloatPair{-m, 0.f}, z, zx);   // and nothing
+    };
+    for (int i = threadIdx.x; i < vectors; i += kThreads)
+        for (int j = 0; j < Vec<T>::N; ++j) one((float)row[first + i * Vec<T>::N + j]);
+    if (edge >= 0) one((float)row[edge]);
+    return make_float4(z.x, z.y, zx.x, zx.y);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     constexpr int N = Vec<T>::N;
@@ -329,11 +348,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     FloatPair z{0.f, 0.f}, zx{0.f, 0.f};
     float m_run = -INFINITY;
     int before = 0;
-    auto add = [&](FloatPair v, FloatPair minus_m) {
-        const FloatPair d = v + minus_m, y = d * FloatPair{kLog2e, kLog2e}, e{ex2(y.x), ex2(y.y)};
-        z = z + e;
-        zx = fma2(e, d, zx);
-    };
+    auto add = [&](FloatPair v, FloatPair minus_m) { add_weights(v, minus_m, z, zx); };
     auto raise = [&](float top) {   // the maximum to at least `top`; what to subtract
         const float m = max_nan(m_run, top);
         if (m > m_run) {
@@ -383,6 +398,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
             const int e = run.first + own_vector * N + tid;
             if (e != token) before += (float)x[e] >= (e < token ? mine : above) ? 1 : 0;
         }
+    }
+    if (m_run > -INFINITY && !(m_run - least_of(m_run) >= 150.f)) {
+        const float4 sums = one_by_one(run.row, run.first, run.vectors, run.edge(), m_run);
+        z = FloatPair{sums.x, sums.y}, zx = FloatPair{sums.z, sums.w};
     }
     const Sums my{m_run, z.x + z.y, zx.x + zx.y, before};
     const float my_top = my.m;
