@@ -725,7 +725,8 @@ int32_t mk_k_gather_tokens_dev(void* k_pool_dev, void* v_pool_dev, int64_t layer
  * Rows of keys and values [total][kv_heads][head_dim] (strides between rows and heads in values, multiples of 8) into the pages, and what the pages hold
  * back into rows, rounded to `type`, at most its largest value.  Lanes, tables and cu_seqlens are as of mk_k_shared_attention_dev: lane i has lengths[i] tokens
  * in the pages tables[i][..], and its rows are the last of them; cu_seqlens NULL: total / lanes rows each.  Rows in front of a lane's first token are
- * not written anywhere, and come back as zeros, as do rows whose page or length is out of range; rows that belong to no lane are left as they were.  No token is
+ * not written anywhere, and come back as zeros, as do rows whose page or length is out of range and those of a lane whose rows begin in front of the first
+ * or end behind the last (MK_DEV_BAD_RANGE); rows that belong to no lane are left as they were.  No token is
  * written by two rows of a call. */
 int32_t mk_k_quantize_rows_dev(const void* k_dev, int64_t k_row_stride, int64_t k_head_stride, const void* v_dev, int64_t v_row_stride, int64_t v_head_stride,
                                int32_t type, int32_t bits, void* k_codes_dev, void* v_codes_dev, void* k_scales_dev, void* v_scales_dev,

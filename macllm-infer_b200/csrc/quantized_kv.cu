@@ -123,10 +123,10 @@ __device__ __forceinline__ Place place_of_row(const QuantLanes& a, const QuantPo
         end = a.cu[lane + 1];
     }
     Place r{-2, 0};
-    if ((int)(threadIdx.x & 31) >= rows || t < begin || t >= end) return r;
+    if ((int)(threadIdx.x & 31) >= rows || t >= a.total || t < begin || t >= end) return r;   // a warp's last rows may lie behind the call's, wherever the list says that a lane ends
     r.page = -1;
     const int length = a.lengths[lane];
-    if (length < 0 || length > (int64_t)a.width << p.bt_shift) {
+    if (begin < 0 || end > a.total || length < 0 || length > (int64_t)a.width << p.bt_shift) {
         tell(a.status, kDevBadRange);
         return r;
     }
