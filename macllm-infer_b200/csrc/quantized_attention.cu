@@ -677,12 +677,12 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     using L = Many<D, BITS, SUBS>;
     constexpr int G = L::G, KST = L::K_STAGES, VST = L::V_STAGES;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 * KST + 2 * VST + 7 * SUBS];
+    __shared__ uint64_t bars[2 * KST + 2 * VST + 8 * SUBS];
     __shared__ uint32_t tmem_slot;
     __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 2; bit 0 tells of values' scales that are not finite
     __shared__ uint32_t odd_groups[4][kKeyTile];        // groups of a key's values whose scales are not finite, where the bit is set
     uint64_t *k_full = bars, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
-             *o_done = p_full + 2 * SUBS, *q_full = o_done + 2 * SUBS;
+             *o_done = p_full + 2 * SUBS, *q_full = o_done + 2 * SUBS, *drained = q_full + SUBS;
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ks = qs + SUBS * L::Q_BYTES;
     uint8_t* vs = ks + KST * L::TILE_BYTES;
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         for (int i = 0; i < KST; ++i) bar_init(&k_full[i], 4), bar_init(&k_empty[i], subs);
         for (int i = 0; i < VST; ++i) bar_init(&v_full[i], 4), bar_init(&v_empty[i], subs);
         for (int i = 0; i < 2 * SUBS; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], kItemTile), bar_init(&o_done[i], 1);
-        for (int i = 0; i < SUBS; ++i) bar_init(&q_full[i], kItemTile);
+        for (int i = 0; i < SUBS; ++i) bar_init(&q_full[i], kItemTile), bar_init(&drained[i], 1);
         bar_init_fence();
     }
     if (warp == L::MMA_WARP) tmem_alloc(&tmem_slot, 512);
@@ -905,6 +905,9 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 __syncwarp();
             }
             if (!ok && lane == 0) tell(a.lanes.status, kDevWait);
+            // products under way end before the memory of their operands and results is given back, whoever gave up a wait
+            if (issues) commit(&drained[sub]);
+            __all_sync(0xffffffffu, bar_wait(&drained[sub], 0));
         }
     } else if (warp < 4 * subs) {
         // ---- an item to a thread

@@ -1,0 +1,25 @@
+"""The kernels of caches in 4 and 8 bits as they are written: what no device can be made to show."""
+import re
+
+from test_dependent_launches import kernels
+
+
+def body_of(name):
+    return next(b for _, n, _, b in kernels() if n == name)
+
+
+def test_products_end_before_their_memory_is_given_back():
+    """Behind its loop, however that ended, a warp that issues products waits for all of them: for a barrier of its own, to which only the last commit arrives."""
+    body = body_of("many_items_kernel")
+    products = body[body.index("f16_idesc(kItemTile, kKeyTile, false)"):body.index("f16_idesc(kItemTile, D, true)")] + body[body.index("f16_idesc(kItemTile, D, true)"):]
+    products = products[:products.index("} else if (warp < 4 * subs)")]
+    assert products.count("commit(&drained[sub])") == 1 and products.count("bar_wait(&drained[sub], 0)") == 1
+    last = products[products.rindex("commit(&v_empty[st]);"):]
+    assert last.index("commit(&drained[sub])") < last.index("bar_wait(&drained[sub], 0)")
+    assert not re.search(r"if \(!?ok[^)]*\)\s*\{", last) and not re.search(r"if \(ok\) *(if|commit)", last)   # also where only the others gave up
+    assert re.search(r"bar_init\(&drained\[i\], 1\)", body)
+    # a barrier of each tile of items, behind the others
+    assert "bars[2 * KST + 2 * VST + 8 * SUBS]" in body and "*drained = q_full + SUBS" in body
+    # tensor memory is given back behind the barrier of all threads that follows
+    end = body[body.rindex("__syncthreads()"):]
+    assert "tmem_dealloc(tmem, 512)" in end and body.count("tmem_dealloc(") == 1
