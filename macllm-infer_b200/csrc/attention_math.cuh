@@ -22,10 +22,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)), which rounds in parts of the cap: 2^-14 and less up to kCapOfDifference.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// cap * tanh(v / cap) as cap - 2 cap / (1 + exp(2 v / cap)), which rounds in parts of the cap: 2^-14 and less up to kCapOfDifference; NaN of NaN.
 constexpr float kCapOfDifference = 256.f;
 __device__ __forceinline__ float capped(float v, float cap, float two_over_cap) {
-    return cap - __fdividef(2.0f * cap, 1.0f + __expf(fminf(v * two_over_cap, 80.0f)));
+    return cap - __fdividef(2.0f * cap, 1.0f + __expf(min_nan(v * two_over_cap, 80.0f)));
 }
 // For caps above, by kernels of their own (beside the other in one kernel it cost calls without any cap 1.5 %): with x = v / cap below 1/4 as v (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315), whose next term is 3.4e-7 of v; from there on the roundings above are less than 2^-20 of v.
 __device__ __forceinline__ float capped_wide(float v, float cap, float two_over_cap) {

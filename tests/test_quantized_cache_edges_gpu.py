@@ -6,7 +6,63 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_quantized_cache_gpu import BF16, F16, INT, Cache, codes_and_scales, dops, generator, ints  # noqa: E402, F401 (dops is a fixture)
+from test_quantized_cache_gpu import BF16, F16, INT, Cache, attend, codes_and_scales, dops, generator, ints, queries  # noqa: E402, F401 (dops is a fixture)
+
+
+# ---- what is not finite under a cap -------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("softcap", [50.0, 1000.0])
+def test_what_is_not_finite_stays_so_under_a_cap(dops, rows, softcap):  # noqa: F811
+    """A key or a query that is not a number has no score, capped or not; what a row does not see has no say."""
+    c = Cache(F16, 4, 2, 128, 16, [200, 90, 70], rows, seed=30).fill()
+    q = queries(c, 8)
+    c.pools[2][int(c.tables[0, 3])][0, 5, 1, 1] = math.nan          # a key of head 0 that every row of lane 0 sees
+    c.pools[3][int(c.tables[1, 1])][1, 2, 0, 0] = math.nan          # a value's first half, of head 1, lane 1
+    c.pools[2][int(c.tables[2, 69 // 16])][:, 69 % 16] = math.nan   # the last key of lane 2, which only its last row sees
+    if rows > 1:
+        q[2 * rows, 3, 7] = math.nan
+    got = attend(dops, c, q, softcap=softcap)
+    plain = attend(dops, c, q)
+    want = torch.zeros_like(got, dtype=torch.bool)
+    want[:rows, :4] = True
+    want[rows:2 * rows, 4:, :64] = True
+    want[3 * rows - 1] = True
+    if rows > 1:
+        want[2 * rows, 3] = True
+    assert torch.equal(torch.isnan(got), want) and torch.equal(torch.isnan(plain), want)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("softcap", [50.0, 1000.0])
+def test_infinite_scores_reach_the_cap(dops, rows, softcap):  # noqa: F811
+    """Scores far beyond the cap are the cap, of either sign."""
+    c = Cache(BF16, 8, 1, 64, 16, [40], rows, seed=31)
+    x = torch.ones(40, 1, 64, device="cuda", dtype=BF16)
+    x[::2] *= -1
+    dops.quantize_rows(x * 1e10, x, c.pools, c.tables, c.lengths, cu_seqlens=ints([0, 40]))
+    q = torch.full((c.total, 2, 64), 1e10, dtype=BF16, device="cuda")
+    got = attend(dops, c, q, softcap=softcap)
+    assert (got[-1] == 1).all()   # e^(-2 softcap) is nothing
+
+
+@pytest.mark.parametrize("own, rows, heads", [([40, 90], 1, (8, 2, 128)), ([700, 90], 1, (8, 2, 128)), ([300, 200], 40, (8, 2, 128)), ([300, 200], 40, (4, 1, 256)), ([500] * 40, 1, (8, 2, 64))])
+@pytest.mark.parametrize("softcap", [50.0, 1000.0])
+def test_keys_that_are_no_numbers_under_a_cap_in_16_bits(dops, own, rows, heads, softcap):  # noqa: F811
+    """The same of shared_attention, whose caps are the same function."""
+    from test_device_ops_gpu import Batch
+    for shared in (0, 256):
+        b = Batch(F16, *heads, 16, shared, own, rows, seed=32)
+        n = int(b.lengths[0])
+        place = (n - rows) // 2
+        b.pools[0][int(b.tables[0, place // 16])][:, place % 16] = math.nan
+        seen_by = [i for i in range(len(own)) if i == 0 or place < shared]
+        want = torch.zeros(len(own), rows, dtype=torch.bool, device="cuda")
+        want[seen_by] = True
+        for cap in (0.0, softcap):
+            got = torch.isnan(b.run(dops, softcap=cap)).flatten(1)
+            assert torch.equal(got.all(1), want.flatten()) and torch.equal(got.any(1), want.flatten())
 
 
 # ---- rows behind the last one -------------------------------------------------------------------------------------------------------------
