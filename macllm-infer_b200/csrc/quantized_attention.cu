@@ -1148,10 +1148,10 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Quant
                 float x[AHEAD][V], w[AHEAD];
 #pragma unroll
                 for (int s = 0; s < AHEAD; ++s) {
-                    w[s] = b + s < 32 ? __shfl_sync(0xffffffffu, f, b + s) : 0.f;   // 0 behind the last part
+                    w[s] = b + s < 32 ? __shfl_sync(0xffffffffu, f, b + s) : 0.f;
 #pragma unroll
                     for (int j = 0; j < V; ++j) x[s][j] = 0.f;
-                    if (w[s] == 0.f) continue;
+                    if (b + s >= parts) continue;   // not by its weight: one of 0 does not hide NaN
                     const float* src = part_o + ((s0 + b + s) * n_rows + row) * D + lane * V;
 #pragma unroll
                     for (int j = 0; j < V; j += 2) {

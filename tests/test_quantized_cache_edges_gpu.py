@@ -108,3 +108,23 @@ def test_rows_behind_the_last_are_left_alone(dops, bits, dtype, total):  # noqa:
         status.zero_()
         both(ints(wrong), ints([total + 9] * 4))
         assert status.item() & told == told
+
+
+# ---- shares -------------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("length", [60, 6000])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_value_that_is_not_finite_reaches_every_row_that_sees_it(dops, rows, length, dim):  # noqa: F811
+    """However small its weight is, and whether or not the lane's keys are shared out."""
+    c = Cache(BF16, 4, 1, dim, 16, [length + rows], rows, seed=34)
+    n = length + rows
+    x = torch.ones(n, 1, dim, dtype=BF16, device="cuda")
+    x[: n // 3] = -1   # keys whose scores are below the others' by 2 * 32 * dim^0.5, 2^-739 and less
+    v = torch.randn(n, 1, dim, generator=c.g, device="cuda").to(BF16)
+    v[5, 0, dim - 64:] = math.nan
+    dops.quantize_rows(x, v, c.pools, c.tables, c.lengths, cu_seqlens=ints([0, n]))
+    q = torch.full((c.total, 4, dim), 32.0, dtype=BF16, device="cuda")
+    got = attend(dops, c, q)
+    assert torch.isnan(got[..., dim - 64:]).all() and torch.isfinite(got[..., :dim - 64]).all()
