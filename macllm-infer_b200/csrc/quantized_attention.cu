@@ -76,13 +76,14 @@ __device__ __forceinline__ Piece piece_of(const QuantAttnArgs& a, const QuantAtt
     const int mine = keys_of(lane);
     float total = (float)mine;
     for (int i = 32 + lane; i < n_lanes; i += 32) total += (float)keys_of(i);
-    const float per_share = 1.0f / fmaxf((float)c.least, warp_sum(total) / c.want);
+    // The attention and the kernel that joins its shares count them each for itself: every rounding is spelled out, so that no compiler makes one of two in one kernel alone.
+    const float per_share = __frcp_rn(fmaxf((float)c.least, __fdiv_rn(warp_sum(total), c.want)));
     // lanes with shares of more than half the largest size first: what is left at the end of a call is short
     int before = 0;
     for (int small = 0; small < 2; ++small)
         for (int i0 = 0; i0 < n_lanes; i0 += 32) {
-            const float n = (float)(i0 == 0 ? mine : keys_of(i0 + lane)) * per_share;   // in largest shares
-            const int shares = i0 + lane < n_lanes && (n < 0.5f) == (small != 0) ? max(1, (int)ceilf(n - 1e-3f)) : 0;   // roundings make no share
+            const float n = __fmul_rn((float)(i0 == 0 ? mine : keys_of(i0 + lane)), per_share);   // in largest shares
+            const int shares = i0 + lane < n_lanes && (n < 0.5f) == (small != 0) ? max(1, (int)ceilf(__fsub_rn(n, 1e-3f))) : 0;   // roundings make no share
             int upto = shares;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {

@@ -1,7 +1,7 @@
 """The kernels of caches in 4 and 8 bits as they are written: what no device can be made to show."""
 import re
 
-from test_dependent_launches import kernels
+from test_dependent_launches import CSRC, kernels
 
 
 def body_of(name):
@@ -23,3 +23,15 @@ def test_products_end_before_their_memory_is_given_back():
     # tensor memory is given back behind the barrier of all threads that follows
     end = body[body.rindex("__syncthreads()"):]
     assert "tmem_dealloc(tmem, 512)" in end and body.count("tmem_dealloc(") == 1
+
+
+def test_shares_are_counted_alike_in_every_kernel():
+    """How many shares a lane has is found by the attention and by the kernel that joins them: from products, quotients and differences that are rounded where they stand, so that none is made
+    one with its neighbour in one kernel alone."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / "quantized_attention.cu").read_text())
+    text = text[text.index("Piece piece_of("):text.index("struct Shares")]
+    for wanted in ("__frcp_rn(", "__fdiv_rn(warp_sum(total), c.want)", "__fmul_rn(", "__fsub_rn(n, 1e-3f)"):
+        assert text.count(wanted) == 1, wanted
+    for wrong in ("* per_share", "/ c.want", "n - 1e", "1.0f /"):
+        assert wrong not in text, wrong
+    assert re.search(r"total \+= \(float\)keys_of", text)   # whole numbers, added
