@@ -142,9 +142,17 @@ __device__ __forceinline__ Place place_of_row(const QuantLanes& a, const QuantPo
     return r;
 }
 
+// The code of x, which is c or next to it, where the difference d of x and low may have lost something: x - low = d + lost (see below).
+__device__ __noinline__ uint32_t nearest(float x, float low, float step, uint32_t c, uint32_t most) {
+    const float d = x - low, of_low = d - x, lost = (x - (d - of_low)) - (low + of_low), rest = fmaf(-(float)c, step, d), twice = 2.f * fabsf(rest), beyond = rest > 0.f ? lost : -lost;
+    const bool other = twice > step || (twice == step && (beyond > 0.f || (beyond == 0.f && (c & 1u))));
+    return other ? (rest > 0.f ? min(c + 1u, most) : c - 1u) : c;
+}
 // Codes of eight values x under (step, low); step is positive.  A reciprocal gives the quotient to 2^-22 of it, 2^-14 at most, which decides wherever it is not that near to a half; there, as bf16 values
-// often are, the remainder does: d - c step is exact (c step has at most 19 bits), and twice that against the step says which code is nearer, or that both are and the even one is meant.
-template <int BITS>
+// often are, the remainder does: d - c step is exact for the 32-bit difference d = x - low (c step has at most 19 bits), and twice that against the step says which code is nearer.  Where they are equal,
+// what d lost in its rounding says it, and where it lost nothing the even code is meant; elsewhere the loss decides nothing, since twice the remainder is off the step by 2^-16 of it or more.  A difference
+// of numbers of m bits loses nothing unless one of them is below 2^(m - 24) of it, and that is looked for first: with the loss of each value found anyway 16383 rows written and read took 47.8 us, so 46.0, without 44.7.
+template <typename T, int BITS>
 __device__ __forceinline__ void codes_of(const float (&x)[8], float low, float step, uint32_t (&word)[BITS / 4]) {
     constexpr uint32_t L = (1u << BITS) - 1;
     constexpr float kWhole = 12582912.f;   // 2^23 + 2^22: sums keep whole numbers, in their lowest bits
@@ -161,11 +169,20 @@ __device__ __forceinline__ void codes_of(const float (&x)[8], float low, float s
 #pragma unroll
         for (int j = 0; j < 8; ++j) c[j] = min(L, (uint32_t)__float2int_rn(__fdiv_rn(x[j] - low, step)));
     } else if (off >= 0.4999f) {
+        constexpr float kLoses = (float)(L + 1) / (std::is_same_v<T, __half> ? 8192.f : 65536.f);
+        float least = low != 0.f ? fabsf(low) : INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float rest = fmaf(-(float)c[j], step, x[j] - low), twice = 2.f * fabsf(rest);
-            const bool other = twice > step || (twice == step && (c[j] & 1u));
-            c[j] = other ? (rest > 0.f ? min(c[j] + 1u, L) : c[j] - 1u) : c[j];
+        for (int j = 0; j < 8; j += 2) asm("{\n\t.reg .f32 a, b;\n\tabs.f32 a, %1;\n\tabs.f32 b, %2;\n\tmin.f32 %0, %0, a, b;\n\t}" : "+f"(least) : "f"(x[j]), "f"(x[j + 1]));
+        if (least > step * kLoses) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float rest = fmaf(-(float)c[j], step, x[j] - low), twice = 2.f * fabsf(rest);
+                const bool other = twice > step || (twice == step && (c[j] & 1u));
+                c[j] = other ? (rest > 0.f ? min(c[j] + 1u, L) : c[j] - 1u) : c[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = nearest(x[j], low, step, c[j], L);
         }
     }
 #pragma unroll
@@ -233,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_co
                         x[2 * j] = v.x;
                         x[2 * j + 1] = v.y;
                     }
-                    codes_of<BITS>(x, low, step, word);
+                    codes_of<T, BITS>(x, low, step, word);
                 }
                 if (i >= n) break;
                 const int64_t at = ((int64_t)head * p.block_tokens + in_page) << pieces_shift;   // in pieces

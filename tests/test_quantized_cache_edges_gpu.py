@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_quantized_cache_gpu import BF16, F16, INT, Cache, attend, codes_and_scales, dops, generator, ints, queries  # noqa: E402, F401 (dops is a fixture)
+from test_quantized_cache_gpu import BF16, F16, INT, Cache, attend, codes_and_scales, dops, generator, ints, queries, unpacked  # noqa: E402, F401 (dops is a fixture)
 
 
 # ---- what is not finite under a cap -------------------------------------------------------------------------------------------------------
@@ -128,3 +128,31 @@ def test_a_value_that_is_not_finite_reaches_every_row_that_sees_it(dops, rows, l
     q = torch.full((c.total, 4, dim), 32.0, dtype=BF16, device="cuda")
     got = attend(dops, c, q)
     assert torch.isnan(got[..., dim - 64:]).all() and torch.isfinite(got[..., :dim - 64]).all()
+
+
+# ---- codes --------------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_codes_are_the_nearest_where_sizes_are_far_apart(dops, dtype, bits):  # noqa: F811
+    """Values a hair above or below a half between two codes, where the lowest value is so far from them that 32 bits do not hold the difference."""
+    g = generator(41)
+    total, tiny = 300, 2.0 ** -24
+    step = 2.0 ** torch.randint(-2, 3, (total, 1, 1), generator=g, device="cuda").double()
+    # with low = -step / 2 (code 0) halves lie at 0 and at whole steps; the highest value makes the step a power of two
+    low = -step / 2
+    top = 2 ** bits - 1
+    high = low + step * top * (1 + 2.0 ** -9 if dtype is BF16 else 1)
+    half = step * torch.randint(0, 3, (total, 1, 64), generator=g, device="cuda").double()   # a code and a half
+    off = torch.randint(-1, 2, (total, 1, 64), generator=g, device="cuda").double() * tiny
+    x = torch.where(half == 0, off, half)
+    x[..., :1], x[..., 1:2] = low, high
+    x = x.to(dtype)
+    code, scale = codes_and_scales(x, bits)
+    c = Cache(dtype, bits, 1, 64, 16, [total], total, seed=41)
+    dops.quantize_rows(x, x, c.pools, c.tables, c.lengths)
+    for t, (page, at) in enumerate(c.slots()):
+        for kind in (0, 1):
+            assert torch.equal(unpacked(c.pools[kind][page][:, at], bits).double(), code[t]), (t, scale[t])
+            assert torch.equal(c.pools[2 + kind][page][:, at].double(), scale[t])
