@@ -37,6 +37,9 @@ __device__ __forceinline__ uint32_t narrow_pair(float x, float y) {
     }
 }
 
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }   // of a positive number
+
 // Where a lane's rows and keys are; whatever the arrays hold, rows stay inside [0, total) and keys inside the table.
 struct LaneRange {
     int first, n;       // rows
@@ -125,8 +128,10 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 // are the f16 number c 2^-24 (a subnormal, which the tensor cores take in full), so that it costs a mask and half a shift.  With steps and lowest values of the groups
 //   q . k = sum_g step_g (q_g . c_g) + low_g sum(q_g),   o = sum_j (w_j step_jg) c_j + sum_j w_j low_jg,
 // steps multiply 32-bit partial scores, and weights before they are rounded: to two f16 numbers, 22 bits, since a weight's rounding counts for the whole range of a group.
-// Queries are brought to f16 by a power of two per item, weights by one for the largest step met so far; either is exact.  The running maximum follows only
-// when a score exceeds it by more than 2^kSlack, which a vote of the warp tells.
+// Queries are brought to f16 by a power of two per item, weights times steps by one per item and group; either is exact.  The running maximum follows only
+// when a score exceeds it by more than 2^kSlack, which a vote of the warp tells, and the latter powers follow only when a step becomes too large for them, which the same vote tells: mostly they go by the
+// largest step, where sizes are far apart by the largest weight times step that the item sees.  So what an item does not see, or sees with little weight, and other groups' sizes leave its results as exact as
+// they are.  (One power of two for the largest step of all took ten bits off ordinary values' weights beside one of 6e4; it was faster by 2 % for single tokens at heads of 128, by 8 % at heads of 256.)
 // What bounds it is issue slots: about 370 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
 // 4 bits: 49 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 42 us, 2.6 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 144 us, 1.9 TB/s (outputs of all tiles in one accumulator: 47, 40 and
 // 123 us, but see there).  Codes by ordinary loads
@@ -135,7 +140,8 @@ constexpr int kFewItems = 32;            // of a lane and KV head: more go to th
 constexpr int kTile = 16, kHalves = 2, kStep = kHalves * kTile;
 constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;            // base-2 logarithm
-constexpr float kWeightScale = 128.f;    // weights up to 2^kSlack, times this, times a step over the largest: below f16's largest
+constexpr int kMostBy = 118;             // of the exponents by which weights times steps are brought to f16: times 2^kSlack they are still numbers
+constexpr float kStepLimit = 128.f;      // of steps brought to f16: times weights, 2^kSlack at most, they are below f16's largest
 
 // CTAs on an SM: what registers allow.
 __host__ __device__ constexpr int few_ctas(int d, int nt) { return d == 64 ? (nt == 1 ? 5 : 4) : (d == 128 ? (nt == 1 ? 3 : 2) : 2); }
@@ -347,7 +353,11 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 #pragma unroll
                 for (int s = 0; s < 4; ++s) query(n, j, s, q_reg[n][j][s][0], q_reg[n][j][s][1]);
     }
-    float cap_step = 0.f, to_step = 0.f;   // a power of two no step so far exceeds; kWeightScale over it
+    float by[NT][G][2];   // weights times steps of a group go into the second product by so much
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < G; ++j) by[n][j][0] = by[n][j][1] = power_of_two(kMostBy);
     const int key0 = key_of(gid), va = key_of(2 * tq), vb = key_of(2 * tq + 1);
 #pragma unroll 1
     for (int i = 0; i < my_steps; ++i) {
@@ -420,7 +430,6 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             }
         }
         bool up = false;
-        float top_step = 0.f;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
@@ -436,43 +445,97 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                     sc[h][n][e] = v;
                     up |= v > m_run[n][e & 1] + kSlack;   // also when there was none yet
                 }
-#pragma unroll
-            for (int j = 0; j < G; ++j) top_step = max3(top_step, v0[h][j].x, v1[h][j].x);
         }
-        up |= top_step > cap_step;
-        if (__any_sync(0xffffffffu, up)) {
-            const float largest = fmaxf(warp_max(top_step < INFINITY ? top_step : 0.f), cap_step);
-            // the next power of two, between those whose inverse is one too
-            const float cap_new = largest > 0.f ? __uint_as_float(min(max((__float_as_uint(largest) + 0x007fffffu) & 0x7f800000u, 8u << 23), 252u << 23)) : 0.f;
-            const float shrink = cap_new > 0.f ? cap_step / cap_new : 1.f;
-            cap_step = cap_new;
-            to_step = cap_new > 0.f ? kWeightScale / cap_new : 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float alpha[2];
+        for (int j = 0; j < G; ++j) {
+            float most = 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) most = max3(most, by[n][j][0], by[n][j][1]);
+            up |= max3(max3(v0[0][j].x, v1[0][j].x, v0[1][j].x), v1[1][j].x, 0.f) * most > kStepLimit;
+        }
+        if (__any_sync(0xffffffffu, up)) {
+            auto of_item = [](float top) {   // the largest of the threads that have the item
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                return fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            };
+            float less[NT][2];   // what the maximum has risen by, negative; 1: there was none
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float top = fmaxf(fmaxf(sc[0][n][c], sc[0][n][2 + c]), fmaxf(sc[1][n][c], sc[1][n][2 + c]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float m_new = fmaxf(m_run[n][c], top);
-                    alpha[c] = m_new == -INFINITY ? 1.f : ex2(m_run[n][c] - m_new);
+                    const float m_new = fmaxf(m_run[n][c], of_item(fmaxf(fmaxf(sc[0][n][c], sc[0][n][2 + c]), fmaxf(sc[1][n][c], sc[1][n][2 + c]))));
+                    less[n][c] = m_run[n][c] == -INFINITY ? 1.f : m_run[n][c] - m_new;
                     m_run[n][c] = m_new;
-                    l_run[n][c] *= alpha[c];
+                    if (less[n][c] == 0.f || less[n][c] == 1.f) continue;
+                    const float alpha = ex2(less[n][c]);
+                    l_run[n][c] *= alpha;
 #pragma unroll
-                    for (int j = 0; j < G; ++j) low_acc[n][j][c] *= alpha[c];
-                    alpha[c] *= shrink;
-                }
+                    for (int j = 0; j < G; ++j) {
+                        low_acc[n][j][c] *= alpha;
 #pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        o_acc[n][j][u][0] *= alpha[0];
-                        o_acc[n][j][u][1] *= alpha[1];
-                        o_acc[n][j][u][2] *= alpha[0];
-                        o_acc[n][j][u][3] *= alpha[1];
+                        for (int u = 0; u < 4; ++u) {
+                            o_acc[n][j][u][c] *= alpha;
+                            o_acc[n][j][u][2 + c] *= alpha;
+                        }
                     }
+                }
+            // as nearly always: steps of like size, for items that have met none or ones of that size
+            bool plain = true;
+            float largest[G];
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                float top = 0.f, least = INFINITY;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float step = k & 1 ? v1[k >> 1][j].x : v0[k >> 1][j].x;
+                    const int pos = pos0 + (k >> 1) * kTile + key0 + (k & 1) * 8;
+                    top = max_nan(top, step);
+                    if (whole || (pos >= lo && pos < hi)) least = fminf(least, step);
+                }
+                largest[j] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                plain = plain && largest[j] <= 256.f * __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) plain = plain && (less[n][c] == 1.f || (largest[j] * by[n][j][c] <= kStepLimit && largest[j] * by[n][j][c] >= 0x1p-4f));
+            }
+            if (__all_sync(0xffffffffu, plain)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < G; ++j)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (less[n][c] == 1.f) by[n][j][c] = power_of_two(min(4 - exponent(largest[j]), kMostBy));
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < G; ++j)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float m = m_run[n][c] == -INFINITY ? 0.f : m_run[n][c];
+                            float step = 0.f, x = 0.f;   // the largest that the item sees; the largest times its weight, 2^-10 of it
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float score = sc[k >> 1][n][(k & 1) * 2 + c], of_key = k & 1 ? v1[k >> 1][j].x : v0[k >> 1][j].x;
+                                if (!(score != -INFINITY && of_key < INFINITY)) continue;
+                                step = fmaxf(step, of_key);
+                                x = fmaxf(x, ex2(score - m - 10.f) * of_key);
+                            }
+                            step = of_item(step), x = of_item(x);
+                            // what came so far has become less by 2^more, so that what comes may count for that much more
+                            const int now = less[n][c] == 1.f ? kMostBy : exponent(by[n][j][c]), more = less[n][c] == 1.f ? 0 : min((int)fminf(-less[n][c], 240.f), kMostBy - now), e_step = exponent(step), e_x = exponent(x) + 10;
+                            const int then = min(now + more, step > 0.f ? min(x > 0.f ? (e_x >= e_step - 8 ? 4 - e_step : 3 - e_x) : kMostBy, 120 - e_step) : kMostBy);
+                            by[n][j][c] = power_of_two(then);
+                            const float factor = power_of_two(max(then - now, -126));
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                o_acc[n][j][u][c] *= factor;
+                                o_acc[n][j][u][2 + c] *= factor;
+                            }
+                        }
             }
         }
 #pragma unroll
@@ -492,18 +555,17 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
                     float x[4];
-                    const float step0 = v0[h][j].x * to_step, step1 = v1[h][j].x * to_step;
                     if (whole) {
                         low_acc[n][j][0] = fmaf(w[0], v0[h][j].y, fmaf(w[2], v1[h][j].y, low_acc[n][j][0]));
                         low_acc[n][j][1] = fmaf(w[1], v0[h][j].y, fmaf(w[3], v1[h][j].y, low_acc[n][j][1]));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = w[e] * (e < 2 ? step0 : step1);
+                        for (int e = 0; e < 4; ++e) x[e] = w[e] * (by[n][j][e & 1] * (e < 2 ? v0[h][j].x : v1[h][j].x));
                     } else {   // what an item does not see does not count, also where it is not finite
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const bool seen = sc[h][n][e] != -INFINITY;
                             low_acc[n][j][e & 1] += seen ? w[e] * (e < 2 ? v0[h][j].y : v1[h][j].y) : 0.f;
-                            x[e] = seen ? w[e] * (e < 2 ? step0 : step1) : 0.f;
+                            x[e] = seen ? w[e] * (by[n][j][e & 1] * (e < 2 ? v0[h][j].x : v1[h][j].x)) : 0.f;
                         }
                     }
 #pragma unroll
@@ -568,11 +630,12 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) low += __shfl_xor_sync(0xffffffffu, low, o);
                 low *= inv;
+                const float back = power_of_two(-exponent(by[n][j][h]));
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     // codes were c 2^-24, those of the second value 16 times that
-                    const float x = o_acc[n][j][u][h] * inv * (0x1p24f / kWeightScale), y = o_acc[n][j][u][2 + h] * inv * (BITS == 4 ? 0x1p20f / kWeightScale : 0x1p24f / kWeightScale);
-                    *reinterpret_cast<float2*>(mine + item * L::OP + j * kQuantGroup + gid * 8 + 2 * u) = make_float2(fmaf(x, cap_step, low), fmaf(y, cap_step, low));
+                    const float x = o_acc[n][j][u][h] * inv * 0x1p24f, y = o_acc[n][j][u][2 + h] * inv * (BITS == 4 ? 0x1p20f : 0x1p24f);
+                    *reinterpret_cast<float2*>(mine + item * L::OP + j * kQuantGroup + gid * 8 + 2 * u) = make_float2(fmaf(x, back, low), fmaf(y, back, low));
                 }
             }
         }
@@ -649,7 +712,6 @@ __device__ __forceinline__ int exponent_of(float bound, int before) {
     return e <= before && (e >= before - 16 || bound == 0.f) ? before : e;
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // The lane with the rank-th most tokens, the first of equals first, among up to kRanked lanes; more lanes keep their order.  All threads of the CTA.
 constexpr int kRanked = 256;
 __device__ __forceinline__ int lane_of_rank(const QuantLanes& l, int rank) {

@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_quantized_cache_gpu import BF16, F16, INT, Cache, attend, codes_and_scales, dops, generator, ints, queries, unpacked  # noqa: E402, F401 (dops is a fixture)
+from test_quantized_cache_gpu import BF16, F16, INT, Cache, attend, check_attention, codes_and_scales, dops, generator, ints, queries, unpacked  # noqa: E402, F401 (dops is a fixture)
 
 
 # ---- what is not finite under a cap -------------------------------------------------------------------------------------------------------
@@ -128,6 +128,125 @@ def test_a_value_that_is_not_finite_reaches_every_row_that_sees_it(dops, rows, l
     q = torch.full((c.total, 4, dim), 32.0, dtype=BF16, device="cuda")
     got = attend(dops, c, q)
     assert torch.isnan(got[..., dim - 64:]).all() and torch.isfinite(got[..., :dim - 64]).all()
+
+
+# ---- magnitudes far apart -----------------------------------------------------------------------------------------------------------------
+
+
+def put(c, lane, position, kind, x):
+    """One token's keys (kind 0) or values (1), [kv heads][dim], by the definition."""
+    code, scale = codes_and_scales(x.to(c.dtype), c.bits)
+    code = code.to(torch.uint8)
+    page, at = int(c.tables[lane, position // c.page]), position % c.page
+    c.pools[kind][page][:, at] = code[..., ::2] | code[..., 1::2] << 4 if c.bits == 4 else code
+    c.pools[2 + kind][page][:, at] = scale.to(c.dtype)
+
+
+HUGE = [(F16, 6e4), (BF16, 1e10), (BF16, 1e30)]
+
+
+@pytest.mark.parametrize("dtype, huge", HUGE)
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim, bits", [(64, 8), (128, 4), (256, 8)])
+@pytest.mark.parametrize("rows", [2, 5])
+def test_what_later_rows_see_has_no_say(dops, dtype, huge, kind, dim, bits, rows):  # noqa: F811
+    """A last token whose keys or values are far above all others': the rows before it, which do not see it, are as exact as ever."""
+    c = Cache(dtype, bits, 1, dim, 16, [rows + 60, rows + 1, 3 * rows], rows, seed=35).fill()
+    q = queries(c, 4)
+    for lane, n in enumerate(c.lengths_list):
+        x = torch.randn(1, dim, generator=c.g, device="cuda")
+        put(c, lane, n - 1, kind, x / x.abs().max() * huge)
+    got = attend(dops, c, q)
+    keep = [i for i in range(c.total) if (i + 1) % rows]   # all but each lane's last row
+    clean = Cache(dtype, bits, 1, dim, 16, [n - 1 for n in c.lengths_list], rows - 1, seed=35)
+    clean.pools, clean.tables = c.pools, c.tables
+    check_attention(clean, q[keep], got[keep])
+
+
+@pytest.mark.parametrize("dtype, huge", HUGE)
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim, bits", [(64, 4), (128, 8), (256, 4)])
+@pytest.mark.parametrize("rows", [1, 6])
+def test_what_is_in_front_of_the_window_has_no_say(dops, dtype, huge, kind, dim, bits, rows):  # noqa: F811
+    window = 100
+    c = Cache(dtype, bits, 1, dim, 16, [rows + 300, rows + 117], rows, seed=36).fill()
+    q = queries(c, 4)
+    for lane, n in enumerate(c.lengths_list):
+        for position in (n - rows - window - 9, n - rows - window):   # the latter is the last that no row sees
+            x = torch.randn(1, dim, generator=c.g, device="cuda")
+            put(c, lane, position, kind, x / x.abs().max() * huge)
+    check_attention(c, q, attend(dops, c, q, window=window), window=window)
+    x = torch.randn(1, dim, generator=c.g, device="cuda")
+    if rows > 1:   # the first row sees one more, the others do not
+        put(c, 0, c.lengths_list[0] - rows - window + 1, kind, x / x.abs().max() * huge)
+        got = attend(dops, c, q, window=window)
+        check_attention(Tail(c), q[1:rows], got[1:rows], window=window)
+
+
+class Tail(Cache):
+    """Lane 0 of a cache without its first row."""
+
+    def __init__(self, c):
+        self.__dict__.update(c.__dict__)
+        self.lengths_list, self.rows = c.lengths_list[:1], [c.rows[0] - 1]
+
+
+@pytest.mark.parametrize("dtype, huge", HUGE)
+@pytest.mark.parametrize("dim, bits", [(64, 4), (128, 8), (256, 8)])
+@pytest.mark.parametrize("rows, length", [(1, 90), (6, 1500)])
+def test_a_huge_value_with_no_weight_has_no_say(dops, dtype, huge, dim, bits, rows, length):  # noqa: F811
+    """Its weight times its size is far below what the others have, in front of them, among them and behind most."""
+    c = Cache(dtype, bits, 1, dim, 16, [length + rows], rows, seed=37).fill()
+    n = length + rows
+    q = torch.ones(c.total, 4, dim, dtype=dtype, device="cuda") + (0.5 * torch.randn(c.total, 4, dim, generator=c.g, device="cuda")).to(dtype)
+    low = torch.full((1, dim), -160.0 / dim ** 0.5, device="cuda")   # a score of about -160 where the others' are between -10 and 10
+    for position in (0, 3, n // 2, n - rows - 2):
+        put(c, 0, position, 0, low)
+        put(c, 0, position, 1, torch.linspace(-huge, huge, dim, device="cuda")[None])
+    check_attention(c, q, attend(dops, c, q))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("rows, ratio", [(1, 1e10), (7, 1e30)])
+def test_groups_of_one_head_far_apart(dops, bits, dim, rows, ratio):  # noqa: F811
+    """Values of one group of 64 channels far above another's: each channel is as exact as its own group allows.  Above 32 items numbers have 11 bits down to 2^-21 of a token's largest."""
+    c = Cache(BF16, bits, 2, dim, 16, [rows + 700, rows + 50], rows, seed=38).fill()
+    c.pools[3][..., 0, :] = (c.pools[3][..., 0, :].float() * ratio).to(BF16)
+    q = queries(c, 4 if rows < 40 else 8)
+    check_attention(c, q, attend(dops, c, q))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("rows", [1])
+def test_tokens_whose_sizes_rise_and_fall(dops, bits, dim, rows):  # noqa: F811
+    """Keys and values of every size from 2^-20 to 2^20 in one context, in runs and mixed."""
+    c = Cache(BF16, bits, 1, dim, 16, [rows + 1200, rows + 80], rows, seed=39).fill()
+    for kind in (2, 3):
+        by = torch.exp2(torch.randint(-20, 21, c.pools[kind].shape[:3], generator=c.g, device="cuda").float())
+        by[1::2] = by[1::2, :, :1]   # every other page: all of its tokens alike
+        if kind == 2:
+            by = by.clamp(max=1)
+        c.pools[kind].copy_((c.pools[kind].float() * by[..., None, None]).to(BF16))
+    q = queries(c, 4)
+    check_attention(c, q, attend(dops, c, q))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1])
+def test_many_light_keys_behind_a_heavy_one(dops, dtype, rows):  # noqa: F811
+    """One key has nearly all of the weight and a value of 0; 8000 have 2^-25.5 of it each and the value 1, and together the result."""
+    n = 8000 + rows
+    c = Cache(dtype, 4, 1, 64, 16, [n], rows, seed=40)
+    k = torch.full((n, 1, 64), -25.5 * math.log(2) / 8, device="cuda").to(dtype)
+    v = torch.ones(n, 1, 64, dtype=dtype, device="cuda")
+    k[3], v[3] = 0, 0
+    dops.quantize_rows(k, v, c.pools, c.tables, c.lengths, cu_seqlens=ints([0, n]))
+    q = torch.ones(c.total, 4, 64, dtype=dtype, device="cuda")
+    got = attend(dops, c, q)
+    check_attention(c, q, got)
+    assert (got > 2 ** -14).all()
 
 
 # ---- codes --------------------------------------------------------------------------------------------------------------------------------
