@@ -686,6 +686,9 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 // codes' masks give them; queries are laid out alike and results put back in order at the end.  Where a value's scales are not finite they count as zero, and the rows
 // that see the key get NaN for that group at the end: a weight of 0 does not hide NaN from a product.
 constexpr int kItemTile = 128, kKeyTile = 64, kCodeWarps = 8;   // four for keys, four for values
+// Base-2 logarithm of the weight of a score at the maximum, in sums and products alike: with 2^kSlack above it is below f16's largest, down to 2^-21 of the largest weights have 11 bits, and what f16 loses
+// of one is below 2^-32.  (With 0, thousands of weights of 2^-25 and less stayed in the sum alone.  It was 3.5 % faster, 677 us where 2048 rows behind 16384 take 702: products of numbers with few bits.)
+constexpr float kWeightBits = 7.f;
 
 template <int D, int BITS, int SUBS>
 struct Many {
@@ -1027,7 +1030,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16), my_o = my + sub * D;
         const float two_over_cap = CAP ? 2.0f / a.softcap : 0.f;
         const bool wide_cap = CAP && a.softcap > kCapOfDifference;
-        float m_run = -INFINITY, sum = 0.f;
+        float m_run = -INFINITY, sum = 0.f;   // the score whose weight is 1: kWeightBits below a maximum
         int e_run = -120;
         uint32_t odd = 0;
         bool ok = true;
@@ -1075,10 +1078,10 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
             const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * u;
             // exponents of the values: one for all that came so far
             float alpha = 1.f;
-            if (m_tile > m_run + kSlack) {   // also when there was none yet
-                alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - m_tile);
+            if (m_tile > m_run + (kSlack + kWeightBits)) {   // also when there was none yet
+                alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - (m_tile - kWeightBits));
                 sum *= alpha;
-                m_run = m_tile;
+                m_run = m_tile - kWeightBits;
             }
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             FloatPair part[2] = {{0.f, 0.f}, {0.f, 0.f}};

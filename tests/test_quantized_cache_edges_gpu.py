@@ -234,7 +234,7 @@ def test_tokens_whose_sizes_rise_and_fall(dops, bits, dim, rows):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("rows", [1])
+@pytest.mark.parametrize("rows", [1, 40])
 def test_many_light_keys_behind_a_heavy_one(dops, dtype, rows):  # noqa: F811
     """One key has nearly all of the weight and a value of 0; 8000 have 2^-25.5 of it each and the value 1, and together the result."""
     n = 8000 + rows
