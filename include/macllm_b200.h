@@ -740,7 +740,8 @@ int32_t mk_k_dequantize_rows_dev(int32_t type, int32_t bits, const void* k_codes
                                  int32_t* status_dev, void* cuda_stream);
 
 /* Attention over such pools.  Lanes, rows, window, scale and softcap are as of mk_k_shared_attention_dev; q, out [total] rows of q_heads x head_dim values of the
- * pools' type.  Keys and values are what their codes stand for; where `rows` times the query heads of a KV head is above 32, they and the weights are rounded to 11 bits each.
+ * pools' type.  Keys and values are what their codes stand for; where `rows` times the query heads of a KV head is above 32, they and the weights are rounded to 11 bits each (keys and values
+ * down to 2^-21 of the largest of their token and KV head, which is where fewer bits begin).
  * Queries are below 2^100 in size.  What a row does not see, behind it, in front of its window or behind the lane's length, may hold anything, and pages wholly in front of
  * every row's window need not be there. */
 int32_t mk_k_quantized_attention_workspace(int32_t bits, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_tokens, int32_t table_width, int32_t lanes,

@@ -682,12 +682,15 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 // codes through bulk copies and shared memory: 441; turns at the exponentials: 441; a fourth of the exponentials as polynomials on the other pipes: 401.
 // A code becomes 1024 + c by its bits, c by a subtraction, and low + step c by one fused multiply-add in f16: rounded once, to 11 bits, as a 16-bit cache would hold it; weights are
 // rounded to 11 bits for the second product.  Scales come with a power of two of their own for every 16 keys (multiples of 2^8, so that neighbours share one): scores are multiplied by the
-// keys', weights by the values' over the largest so far where they differ, so that bf16 caches of any range fit f16.  Values of a chunk of eight lie in the order in which the
+// keys', weights by the values' over the row's where they differ.  The row's goes by weights times sizes, so that values that it does not see, or sees with hardly any weight, take nothing off the others, whatever
+// their size.  Where groups among the 16 keys are so far apart that f16 would cut off the smaller ones' steps, each key has an exponent of its own below the 16 keys', and its numbers are made in 32 bits: they have 11 bits
+// down to 2^-21 of the key's largest.  (Exponents of 16 keys, and the largest of them for the weights, took all bits off a row's values beside an unseen one of 1e10.  Looking for such groups costs 4 % at heads of 256 in
+// 4 bits and for drafts, nothing elsewhere.)  Values of a chunk of eight lie in the order in which the
 // codes' masks give them; queries are laid out alike and results put back in order at the end.  Where a value's scales are not finite they count as zero, and the rows
 // that see the key get NaN for that group at the end: a weight of 0 does not hide NaN from a product.
 constexpr int kItemTile = 128, kKeyTile = 64, kCodeWarps = 8;   // four for keys, four for values
 // Base-2 logarithm of the weight of a score at the maximum, in sums and products alike: with 2^kSlack above it is below f16's largest, down to 2^-21 of the largest weights have 11 bits, and what f16 loses
-// of one is below 2^-32.  (With 0, thousands of weights of 2^-25 and less stayed in the sum alone.  It was 3.5 % faster, 677 us where 2048 rows behind 16384 take 702: products of numbers with few bits.)
+// of one is below 2^-32.  (With 0, thousands of weights of 2^-25 and less stayed in the sum alone; times are the same.)
 constexpr float kWeightBits = 7.f;
 
 template <int D, int BITS, int SUBS>
@@ -708,11 +711,11 @@ struct Many {
     static_assert(S_AT + SUBS * 2 * kKeyTile <= 512, "tensor memory");
 };
 
-// The exponent under which numbers up to `bound` are below 2^15, a multiple of eight; the one before stays while it leaves them above 2^-9, so that neighbours share one.
+// The exponent under which numbers up to `bound` are below 2^15, a multiple of eight; the one before stays while it leaves them above 2^-1, so that neighbours share one.
 __device__ __forceinline__ int exponent_of(float bound, int before) {
     const int above = (int)(__float_as_uint(bound) >> 23) - 126;   // bound < 2^above
     const int e = bound > 0.f ? min(max(((above - 15 + 1024 + 7) / 8 - 128) * 8, -120), 120) : -120;
-    return e <= before && (e >= before - 16 || bound == 0.f) ? before : e;
+    return e <= before && (e >= before - 8 || bound == 0.f) ? before : e;
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 // The lane with the rank-th most tokens, the first of equals first, among up to kRanked lanes; more lanes keep their order.  All threads of the CTA.
@@ -745,7 +748,9 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * KST + 2 * VST + 8 * SUBS];
     __shared__ uint32_t tmem_slot;
-    __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 2; bit 0 tells of values' scales that are not finite
+    __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 4; bit 0 tells of values' scales that are not finite, bit 1 of exponents for each key
+    __shared__ int key_exponents[2][4][kKeyTile];       // of keys and of values, where the bit is set: from the 16 keys' on down
+    __shared__ uint32_t key_bounds[kCodeWarps][kTile];
     __shared__ uint32_t odd_groups[4][kKeyTile];        // groups of a key's values whose scales are not finite, where the bit is set
     uint64_t *k_full = bars, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
              *o_done = p_full + 2 * SUBS, *q_full = o_done + 2 * SUBS, *drained = q_full + SUBS;
@@ -791,7 +796,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         const uint8_t* codes_of = (keys ? p.k_codes : p.v_codes) + (int64_t)kvh * p.block_tokens * L::ROW;
         const uint32_t* scales_of = (keys ? p.k_scales : p.v_scales) + (int64_t)kvh * p.block_tokens * G;
         auto there = [&](int t) { return t < n_tiles && begin + t * kKeyTile + w * kTile < hi; };
-        auto page_of = [&](int t) {
+        auto page_of = [&](int t) {   // the page of tile t's 16 keys
             if (!there(t)) return 0;
             const int32_t page = table[(begin + t * kKeyTile + w * kTile) >> p.bt_shift];
             if ((uint32_t)page < (uint64_t)p.pages) return page;
@@ -835,20 +840,29 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
         int stage = 0, e = -120;
         uint32_t empty_parity = 1;
         float by = power_of_two(120);
-        uint32_t most = 0, least = 1;   // bounds, as bits, for which the exponent stays
+        uint32_t most = 0, least = 1, fine = 1;   // bounds, as bits, for which the exponent stays; below which a group's numbers would have fewer than 11 bits
         auto make = [&](int t, const Raw& r) {
             const int pos0 = begin + t * kKeyTile + w * kTile;
             float2 sl[L::PASSES];
-            uint32_t bound = 0;   // of the numbers' absolute values, as bits: what is not finite is above all others
+            uint32_t bound = 0, small = UINT32_MAX;   // of the numbers' absolute values, as bits: what is not finite is above all others; the smallest group's, less one, so that zeros are above too
             auto bound_of = [](float2 v) { return max_nan(fabsf(v.y), fabsf(fmaf(v.x, (float)((1 << BITS) - 1), v.y))); };
 #pragma unroll
             for (int i = 0; i < L::PASSES; ++i) {
                 const int pos = pos0 + key_of_pass(i);
                 sl[i] = pos >= lo && pos < hi ? wide_pair<T>(r.scales[i]) : make_float2(0.f, 0.f);
-                bound = max(bound, __float_as_uint(bound_of(sl[i])));
+                const uint32_t b = __float_as_uint(bound_of(sl[i]));
+                bound = max(bound, b);
+                small = min(small, b - 1u);
             }
             bound = __reduce_max_sync(0xffffffffu, bound);
             uint32_t odd = 0;   // passes
+            auto follow = [&](int to) {
+                e = to;
+                by = power_of_two(-e);
+                most = min((uint32_t)(127 + 15 + e) << 23, 0x7f7fffffu);
+                least = (uint32_t)max(127 + 15 - 16 + e, 1) << 23;
+                fine = (uint32_t)max(127 - 6 + e, 1) << 23;
+            };
             if (bound > most || bound < least) {
                 if (bound >= 0x7f800000u) {   // the largest of the finite ones; values whose scales are not count as 0
                     float fine_bound = 0.f;
@@ -861,10 +875,13 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                     }
                     bound = __reduce_max_sync(0xffffffffu, __float_as_uint(fine_bound));
                 }
-                e = exponent_of(__uint_as_float(bound), e);
-                by = power_of_two(-e);
-                most = min((uint32_t)(127 + 15 + e) << 23, 0x7f7fffffu);
-                least = (uint32_t)max(127 + 15 - 24 + e, 1) << 23;
+                follow(exponent_of(__uint_as_float(bound), e));
+            }
+            // a group whose step, and with it its numbers, f16 would cut off: exponents for each key, unless the 16 keys' had only stayed above
+            bool apart = __any_sync(0xffffffffu, small < fine - 1u) != 0;
+            if (apart && exponent_of(__uint_as_float(bound), -120) < e) {
+                follow(exponent_of(__uint_as_float(bound), -120));
+                apart = __any_sync(0xffffffffu, small < fine - 1u) != 0;
             }
             const bool any_odd = !keys && __any_sync(0xffffffffu, odd != 0);
             if (!__all_sync(0xffffffffu, bar_wait(&mine_empty[stage], empty_parity))) return false;
@@ -875,8 +892,50 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 for (int i = 0; i < L::PASSES; ++i)
                     if (odd >> i & 1) atomicOr(&odd_groups[t & 3][w * kTile + key_of_pass(i)], 1u << (piece_of_pass(i) * 8 * L::CHUNKS / kQuantGroup));
             }
-            if (lane == 0) reinterpret_cast<int*>(keys ? &k_info[t & 3] : &v_info[t & 3])[w] = e * 2 | (any_odd ? 1 : 0);
+            if (lane == 0) reinterpret_cast<int*>(keys ? &k_info[t & 3] : &v_info[t & 3])[w] = e * 4 | (apart ? 2 : 0) | (any_odd ? 1 : 0);
             uint8_t* to = tiles + stage * L::TILE_BYTES;
+            if (apart) {   // numbers from 32 bits; rare, so that codes and scales are read again, one pass after the other
+                uint32_t* bounds = key_bounds[warp - L::ITEM_WARPS];
+                if (lane < kTile) bounds[lane] = 0;
+                __syncwarp();
+                const int64_t page = page_of(t);
+                const int row0 = pos0 & (p.block_tokens - 1);
+                const uint32_t* scales = scales_of + page * p.scales_stride + row0 * G;
+                auto scale_of = [&](int i) {
+                    const int key = key_of_pass(i);
+                    const float2 v = pos0 + key >= lo && pos0 + key < hi ? wide_pair<T>(scales[key * G + piece_of_pass(i) * 8 * L::CHUNKS / kQuantGroup]) : make_float2(0.f, 0.f);
+                    return keys || bound_of(v) < INFINITY ? v : make_float2(0.f, 0.f);
+                };
+#pragma unroll 1
+                for (int i = 0; i < L::PASSES; ++i) {
+                    const uint32_t b = __float_as_uint(bound_of(scale_of(i)));
+                    if (b < 0x7f800000u) atomicMax(&bounds[key_of_pass(i)], b);
+                }
+                __syncwarp();
+                if (lane < kTile) key_exponents[keys ? 0 : 1][t & 3][w * kTile + lane] = exponent_of(__uint_as_float(bounds[lane]), -120);
+#pragma unroll 1
+                for (int i = 0; i < L::PASSES; ++i) {
+                    const int key = key_of_pass(i), chunk0 = piece_of_pass(i) * L::CHUNKS;
+                    const float2 v = scale_of(i);
+                    const float by_key = power_of_two(-exponent_of(__uint_as_float(bounds[key]), -120)), step = v.x * by_key, low = v.y * by_key;
+                    const uint4 codes = *reinterpret_cast<const uint4*>(codes_of + page * p.codes_stride + (row0 + key) * L::ROW + piece_of_pass(i) * 16);
+                    const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+                    auto number = [&](uint32_t bits) { return narrow_pair<__half>(fmaf(step, (float)(bits & 0xffffu), low), fmaf(step, (float)(bits >> 16), low)); };
+                    uint8_t* row = to + (chunk0 >> 3) * L::PANEL + key * 128;
+#pragma unroll
+                    for (int j = 0; j < L::CHUNKS; ++j) {
+                        uint4 out;
+                        if constexpr (BITS == 4) {
+                            const uint32_t x = words[j];
+                            out = make_uint4(number(x & 0x000f000fu), number(x >> 4 & 0x000f000fu), number(x >> 8 & 0x000f000fu), number(x >> 12 & 0x000f000fu));
+                        } else {
+                            const uint32_t x = words[2 * j], y = words[2 * j + 1];
+                            out = make_uint4(number(x & 0x00ff00ffu), number(x >> 8 & 0x00ff00ffu), number(y & 0x00ff00ffu), number(y >> 8 & 0x00ff00ffu));
+                        }
+                        *reinterpret_cast<uint4*>(row + (((chunk0 + j & 7) ^ (key & 7)) << 4)) = out;
+                    }
+                }
+            } else
 #pragma unroll
             for (int i = 0; i < L::PASSES; ++i) {
                 const __half2 step = __float2half2_rn(sl[i].x * by), part = __hmul2(step, __float2half2_rn(0.0625f)), low = __float2half2_rn(sl[i].y * by);   // codes in bits 4 .. 7 are 16 times theirs
@@ -1045,17 +1104,26 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
             tmem_ld32(s_at, reinterpret_cast<uint32_t*>(s));
             tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s) + 32);
             const int4 ki = k_info[t & 3];
-            const int of[4] = {ki.x, ki.y, ki.z, ki.w};
             const int pos0 = begin + t * kKeyTile;
             tmem_wait_ld();
             // neither 0 nor infinite: where it would be, scores are 0 or overflow whatever it is
-            auto unit_of = [&](int info_of) { return fminf(fmaxf(factor * power_of_two(info_of >> 1), 1e-37f), 3e38f); };
-            float u = unit_of(of[0]);
-            const bool even = of[0] == of[1] && of[0] == of[2] && of[0] == of[3];
-            if (CAP || !even) {   // scores one by one; then they are what is exponentiated
+            auto unit_of = [&](int info) { return fminf(fmaxf(factor * power_of_two(info >> 2), 1e-37f), 3e38f); };
+            // what has exponents of its own for each key comes under that of the 16
+            auto under = [&](const int (&info)[4], const int* of_keys) {
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const float ub = unit_of(of[b]);
+                    if (!(info[b] & 2)) continue;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[b * 16 + j] *= power_of_two(max(of_keys[b * 16 + j] - (info[b] >> 2), -126));
+                }
+            };
+            float u = unit_of(ki.x);
+            if (CAP || ((ki.x ^ ki.y) | (ki.x ^ ki.z) | (ki.x ^ ki.w) | (ki.x & 2)) != 0) {   // scores one by one; then they are what is exponentiated
+                const int info[4] = {ki.x, ki.y, ki.z, ki.w};
+                if ((ki.x | ki.y | ki.z | ki.w) & 2) under(info, key_exponents[0][t & 3]);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float ub = unit_of(info[b]);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         float v = s[b * 16 + j] * ub;
@@ -1076,10 +1144,11 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 for (int k = 0; k < 4; ++k) top[k] = j + k + 4 < kKeyTile ? max3(top[k], s[j + k], s[j + k + 4]) : fmaxf(top[k], s[j + k]);
             }
             const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * u;
-            // exponents of the values: one for all that came so far
-            float alpha = 1.f;
+            const bool none = m_run == -INFINITY;
+            float less = 0.f, alpha = 1.f;   // what the maximum has risen by, negative
             if (m_tile > m_run + (kSlack + kWeightBits)) {   // also when there was none yet
-                alpha = m_run == -INFINITY ? 1.0f : ex2(m_run - (m_tile - kWeightBits));
+                less = none ? 0.f : m_run - (m_tile - kWeightBits);
+                alpha = ex2(less);
                 sum *= alpha;
                 m_run = m_tile - kWeightBits;
             }
@@ -1093,14 +1162,41 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 part[j >> 1 & 1] = part[j >> 1 & 1] + e;
             }
             sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-            // exponents of the values: the largest so far for all
             ok = __all_sync(0xffffffffu, bar_wait(&v_full[t % VST], t / VST & 1));
             if (!ok) break;
             const int4 vi = v_info[t & 3];
-            const int ev[4] = {vi.x, vi.y, vi.z, vi.w}, e_tile = max(max(ev[0] >> 1, ev[1] >> 1), max(ev[2] >> 1, ev[3] >> 1));
-            if (e_tile > e_run) {
-                alpha *= e_run - e_tile < -126 ? 0.f : power_of_two(e_run - e_tile);
-                e_run = e_tile;
+            // Exponents of the values: one for all, by which weights are scaled where a tile's differ.  It follows what the row's weights make of them, so that large values that it does not see, or
+            // sees with little weight, take nothing off the others.
+            if (none && ((vi.x ^ vi.y) | (vi.x ^ vi.z) | (vi.x ^ vi.w) | (vi.x & 3)) == 0) {
+                if (m_run != -INFINITY) e_run = vi.x >> 2;   // its largest weight is 2^kWeightBits
+            } else if (((vi.x ^ e_run * 4) | (vi.y ^ e_run * 4) | (vi.z ^ e_run * 4) | (vi.w ^ e_run * 4)) != 0) {
+                const int info[4] = {vi.x, vi.y, vi.z, vi.w}, ev[4] = {vi.x >> 2, vi.y >> 2, vi.z >> 2, vi.w >> 2};
+                if ((vi.x | vi.y | vi.z | vi.w) & 2) under(info, key_exponents[1][t & 3]);
+                int top = -1000;   // weights times 2^ev are below 2^top
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) most = fmaxf(most, s[b * 16 + j]);
+                    if (most > 0.f) top = max(top, ev[b] + exponent(fminf(most, 32767.f)) + 1);
+                }
+                const int low = max(e_run - (int)fminf(-less, 240.f), -120);   // what came so far has become less
+                const bool alike = ev[0] == ev[1] && ev[0] == ev[2] && ev[0] == ev[3];
+                const int e = alike && top >= ev[0] + 4 && top <= ev[0] + 15 && low <= ev[0] + 8 ? ev[0] : (top > low + 15 ? top - 8 : low);
+                alpha = ex2(less + (float)(e_run - e));
+                e_run = e;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float to = ev[b] - e < -126 ? 0.f : power_of_two(min(ev[b] - e, 126));
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[b * 16 + j] *= to;
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    if (!(info[b] & 1)) continue;
+                    for (int j = b * 16; j < b * 16 + 16; ++j)
+                        if (pos0 + j >= see_lo && pos0 + j < see_hi) odd |= odd_groups[t & 3][j];
+                }
             }
             if (t > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                 ok = __all_sync(0xffffffffu, bar_wait(&o_done[sub * 2 + (t - 1 & 1)], t - 1 >> 1 & 1));
@@ -1116,23 +1212,10 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                     tmem_st32(my_o + c, o);
                 }
             }
-            if (ev[0] >> 1 != e_run || ev[1] >> 1 != e_run || ev[2] >> 1 != e_run || ev[3] >> 1 != e_run) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int d = (ev[b] >> 1) - e_run;
-                    const float down = d < -126 ? 0.f : power_of_two(d);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) s[b * 16 + j] *= down;
-                }
-            }
             uint32_t w[kKeyTile / 2];
 #pragma unroll
             for (int j = 0; j < kKeyTile / 2; ++j) w[j] = narrow_pair<__half>(s[2 * j], s[2 * j + 1]);
             tmem_st32(s_at, w);
-            if ((ev[0] | ev[1] | ev[2] | ev[3]) & 1) {
-                for (int j = 0; j < kKeyTile; ++j)
-                    if (ev[j >> 4] & 1 && pos0 + j >= see_lo && pos0 + j < see_hi) odd |= odd_groups[t & 3][j];
-            }
             tmem_wait_st();
             fence_before();
             bar_arrive(&p_full[area]);

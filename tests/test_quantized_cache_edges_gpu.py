@@ -148,7 +148,7 @@ HUGE = [(F16, 6e4), (BF16, 1e10), (BF16, 1e30)]
 @pytest.mark.parametrize("dtype, huge", HUGE)
 @pytest.mark.parametrize("kind", [0, 1])
 @pytest.mark.parametrize("dim, bits", [(64, 8), (128, 4), (256, 8)])
-@pytest.mark.parametrize("rows", [2, 5])
+@pytest.mark.parametrize("rows", [2, 5, 12, 40, 90])
 def test_what_later_rows_see_has_no_say(dops, dtype, huge, kind, dim, bits, rows):  # noqa: F811
     """A last token whose keys or values are far above all others': the rows before it, which do not see it, are as exact as ever."""
     c = Cache(dtype, bits, 1, dim, 16, [rows + 60, rows + 1, 3 * rows], rows, seed=35).fill()
@@ -166,7 +166,7 @@ def test_what_later_rows_see_has_no_say(dops, dtype, huge, kind, dim, bits, rows
 @pytest.mark.parametrize("dtype, huge", HUGE)
 @pytest.mark.parametrize("kind", [0, 1])
 @pytest.mark.parametrize("dim, bits", [(64, 4), (128, 8), (256, 4)])
-@pytest.mark.parametrize("rows", [1, 6])
+@pytest.mark.parametrize("rows", [1, 6, 40])
 def test_what_is_in_front_of_the_window_has_no_say(dops, dtype, huge, kind, dim, bits, rows):  # noqa: F811
     window = 100
     c = Cache(dtype, bits, 1, dim, 16, [rows + 300, rows + 117], rows, seed=36).fill()
@@ -193,7 +193,7 @@ class Tail(Cache):
 
 @pytest.mark.parametrize("dtype, huge", HUGE)
 @pytest.mark.parametrize("dim, bits", [(64, 4), (128, 8), (256, 8)])
-@pytest.mark.parametrize("rows, length", [(1, 90), (6, 1500)])
+@pytest.mark.parametrize("rows, length", [(1, 90), (6, 1500), (40, 90), (40, 1500)])
 def test_a_huge_value_with_no_weight_has_no_say(dops, dtype, huge, dim, bits, rows, length):  # noqa: F811
     """Its weight times its size is far below what the others have, in front of them, among them and behind most."""
     c = Cache(dtype, bits, 1, dim, 16, [length + rows], rows, seed=37).fill()
@@ -208,7 +208,7 @@ def test_a_huge_value_with_no_weight_has_no_say(dops, dtype, huge, dim, bits, ro
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dim", [128, 256])
-@pytest.mark.parametrize("rows, ratio", [(1, 1e10), (7, 1e30)])
+@pytest.mark.parametrize("rows, ratio", [(1, 1e10), (7, 1e30), (40, 1e5)])
 def test_groups_of_one_head_far_apart(dops, bits, dim, rows, ratio):  # noqa: F811
     """Values of one group of 64 channels far above another's: each channel is as exact as its own group allows.  Above 32 items numbers have 11 bits down to 2^-21 of a token's largest."""
     c = Cache(BF16, bits, 2, dim, 16, [rows + 700, rows + 50], rows, seed=38).fill()
@@ -219,7 +219,7 @@ def test_groups_of_one_head_far_apart(dops, bits, dim, rows, ratio):  # noqa: F8
 
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dim", [64, 256])
-@pytest.mark.parametrize("rows", [1])
+@pytest.mark.parametrize("rows", [1, 40])
 def test_tokens_whose_sizes_rise_and_fall(dops, bits, dim, rows):  # noqa: F811
     """Keys and values of every size from 2^-20 to 2^20 in one context, in runs and mixed."""
     c = Cache(BF16, bits, 1, dim, 16, [rows + 1200, rows + 80], rows, seed=39).fill()
