@@ -41,6 +41,13 @@ def _rows(t, lanes, device, what: str):
     return t.data_ptr(), t.stride(0) if lanes > 1 else max(shape[1], 1), shape[1]
 
 
+def _int(n: int, what: str) -> int:
+    """n as the entry points take it: a larger number would lose its upper bits on the way."""
+    if n > 0x7fffffff:
+        raise ValueError(f"{what} is at most 2^31 - 1: got {n}")
+    return n
+
+
 def _run(device: int, fn, *args) -> None:
     """fn(..., the device's current stream), with that device current."""
     if device < 0:
@@ -117,7 +124,7 @@ def shared_attention(q, k_pool, v_pool, tables, lengths, shared_len: int, *, sca
                 or (total and out_strides[1:] != (dim, 1) and (heads != 1 or out_strides[2] != 1))):
             raise ValueError("out is like q, the heads of a row dense")
         out_stride = out_strides[0] if total > 1 else heads * dim
-    need = _attention_workspace(heads, kv_heads, dim, page, width, lanes, rows, total, shared_len, window)
+    need = _attention_workspace(heads, kv_heads, dim, page, width, lanes, _int(rows, "max_rows"), total, _int(shared_len, "shared_len"), _int(window, "window"))
     space = q.new_empty(need // 2) if need else None
     _run(device, capi.lib().mk_k_shared_attention_dev, _TYPES[dtype], q.data_ptr(), q_strides[0] if total > 1 else heads * dim, k_pool.data_ptr(), v_pool.data_ptr(), pages,
          strides[0] if pages > 1 else kv_heads * page * dim, heads, kv_heads, dim, page, table, table_stride, width, _dense(lengths, _I32, (lanes,), device, "lengths"), cu, lanes, rows,
@@ -261,7 +268,7 @@ def quantize_rows(k, v, pools, tables, lengths, *, cu_seqlens=None, status=None)
     device = k.get_device()
     dim, dtype, heads, cache = _quantized(pools, device)
     _, where = _lanes(tables, lengths, cu_seqlens, device)
-    shape = (k.shape[0] if k.dim() else 0, heads, dim)
+    shape = (_int(k.shape[0], "the number of rows") if k.dim() else 0, heads, dim)
     _run(device, capi.lib().mk_k_quantize_rows_dev, *_head_rows(k, shape, dtype, device, "k"), *_head_rows(v, shape, dtype, device, "v"), *cache, *where, shape[0],
          _word(status, device))
 
@@ -275,7 +282,7 @@ def dequantize_rows(pools, tables, lengths, total: int, *, cu_seqlens=None, k=No
     _, where = _lanes(tables, lengths, cu_seqlens, device)
     if total < 0:
         raise ValueError("total is not negative")
-    shape, row = (total, heads, dim), heads * dim
+    shape, row = (_int(total, "total"), heads, dim), heads * dim
     if k is None and v is None:
         k, v = pools[2].new_empty((2, total, heads, dim)).unbind()
         to_k, to_v = (k.data_ptr(), row, dim), (v.data_ptr(), row, dim)
@@ -327,7 +334,7 @@ def quantized_attention(q, pools, tables, lengths, *, scale: float, cu_seqlens=N
                 or (total and out_strides[1:] != (dim, 1) and (heads != 1 or out_strides[2] != 1))):
             raise ValueError("out is like q, the heads of a row dense")
         out_stride = out_strides[0] if total > 1 else heads * dim
-    need = _quantized_workspace(cache[1], heads, *cache[9:], where[2], lanes, rows, total, window)
+    need = _quantized_workspace(cache[1], heads, *cache[9:], where[2], lanes, _int(rows, "max_rows"), total, _int(window, "window"))
     space = q.new_empty(need // 2) if need else None
     _run(device, capi.lib().mk_k_quantized_attention_dev, q.data_ptr(), q_strides[0] if total > 1 else heads * dim, heads, *cache, *where, rows, total, scale, softcap, window,
          out.data_ptr(), out_stride, space.data_ptr() if need else None, need, _word(status, device))

@@ -1,5 +1,8 @@
 """The kernels of caches in 4 and 8 bits as they are written: what no device can be made to show."""
+import importlib
 import re
+
+import pytest
 
 from test_dependent_launches import CSRC, kernels
 
@@ -35,3 +38,26 @@ def test_shares_are_counted_alike_in_every_kernel():
     for wrong in ("* per_share", "/ c.want", "n - 1e", "1.0f /"):
         assert wrong not in text, wrong
     assert re.search(r"total \+= \(float\)keys_of", text)   # whole numbers, added
+
+
+@pytest.mark.parametrize("beyond", [1 << 31, (1 << 32) + 5, (1 << 63) + 7])
+def test_numbers_that_lose_their_upper_bits_on_the_way_are_refused(mk, beyond):
+    """A window of 2^32 + 5 was one of 5."""
+    torch = pytest.importorskip("torch")
+    dops = importlib.import_module("macllm_infer_b200.device_ops")
+    pools = dops.quantized_pools(10, 2, 16, 64, device="cpu")
+    pool = torch.zeros(10, 2, 16, 64, dtype=torch.float16)
+    q, row = torch.zeros(3, 8, 64, dtype=torch.float16), torch.zeros(1, 2, 64, dtype=torch.float16)
+    tables, lengths, cu = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    calls = [lambda: dops.quantized_attention(q, pools, tables, lengths, scale=1.0, window=beyond),
+             lambda: dops.quantized_attention(q, pools, tables, lengths, scale=1.0, cu_seqlens=cu, max_rows=beyond),
+             lambda: dops.shared_attention(q, pool, pool, tables, lengths, 0, scale=1.0, window=beyond),
+             lambda: dops.shared_attention(q, pool, pool, tables, lengths, 0, scale=1.0, cu_seqlens=cu, max_rows=beyond),
+             lambda: dops.shared_attention(q, pool, pool, tables, lengths, beyond, scale=1.0),
+             lambda: dops.dequantize_rows(pools, tables, lengths, beyond, cu_seqlens=cu)]
+    if beyond < 1 << 40:
+        many = row.expand(beyond, 2, 64)
+        calls.append(lambda: dops.quantize_rows(many, many, pools, tables, lengths, cu_seqlens=cu))
+    for call in calls:
+        with pytest.raises(ValueError, match="at most 2\\^31 - 1"):
+            call()
