@@ -131,7 +131,8 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 // Queries are brought to f16 by a power of two per item, weights times steps by one per item and group; either is exact.  The running maximum follows only
 // when a score exceeds it by more than 2^kSlack, which a vote of the warp tells, and the latter powers follow only when a step becomes too large for them, which the same vote tells: mostly they go by the
 // largest step, where sizes are far apart by the largest weight times step that the item sees.  So what an item does not see, or sees with little weight, and other groups' sizes leave its results as exact as
-// they are.  (One power of two for the largest step of all took ten bits off ordinary values' weights beside one of 6e4; it was faster by 2 % for single tokens at heads of 128, by 8 % at heads of 256.)
+// they are.  (One power of two for the largest step of all took ten bits off ordinary values' weights beside one of 6e4; it was faster by 2 % for single tokens at heads of 128, by 6 % for drafts at
+// heads of 256.)
 // What bounds it is issue slots: about 370 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
 // 4 bits: 49 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 42 us, 2.6 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 144 us, 1.9 TB/s (outputs of all tiles in one accumulator: 47, 40 and
 // 123 us, but see there).  Codes by ordinary loads
@@ -192,6 +193,31 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
+__device__ __forceinline__ float of_item(float top) {   // the largest of the threads that have the item
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    return fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+}
+// The exponent by which weights times steps go into the second product where sizes are far apart: by the largest step that the item sees or, where its weight is small, by the largest weight times step.  The
+// scores and steps of the thread's four keys, the maximum, what it has risen by (negative; 1: there was none), the exponent until now.  Apart from the kernel, whose loop it slowed by 1 to 2 % in line.
+__device__ __noinline__ int careful_exponent(float4 score, float4 of_key, float maximum, float less, int now) {
+    const float m = maximum == -INFINITY ? 0.f : maximum;
+    float step = 0.f, x = 0.f;   // the largest that the item sees; the largest times its weight, 2^-10 of it
+    auto key = [&](float score, float of_key) {
+        if (!(score != -INFINITY && of_key < INFINITY)) return;
+        step = fmaxf(step, of_key);
+        x = fmaxf(x, ex2(score - m - 10.f) * of_key);
+    };
+    key(score.x, of_key.x);
+    key(score.y, of_key.y);
+    key(score.z, of_key.z);
+    key(score.w, of_key.w);
+    step = of_item(step), x = of_item(x);
+    // what came so far has become less by 2^more, so that what comes may count for that much more
+    const int more = less == 1.f ? 0 : min((int)fminf(-less, 240.f), kMostBy - now), e_step = exponent(step), e_x = exponent(x) + 10;
+    return min(now + more, step > 0.f ? min(x > 0.f ? (e_x >= e_step - 8 ? 4 - e_step : 3 - e_x) : kMostBy, 120 - e_step) : kMostBy);
+}
+
 template <typename T, int D, int BITS, int NT, int CAP>
 __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items_kernel(const __grid_constant__ QuantAttnArgs a, const __grid_constant__ QuantAttnCut cut, float* part_o, float2* part_ml) {
     using L = Few<D, BITS, NT>;
@@ -454,11 +480,6 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
             up |= max3(max3(v0[0][j].x, v1[0][j].x, v0[1][j].x), v1[1][j].x, 0.f) * most > kStepLimit;
         }
         if (__any_sync(0xffffffffu, up)) {
-            auto of_item = [](float top) {   // the largest of the threads that have the item
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                return fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            };
             float less[NT][2];   // what the maximum has risen by, negative; 1: there was none
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -515,19 +536,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                     for (int j = 0; j < G; ++j)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float m = m_run[n][c] == -INFINITY ? 0.f : m_run[n][c];
-                            float step = 0.f, x = 0.f;   // the largest that the item sees; the largest times its weight, 2^-10 of it
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float score = sc[k >> 1][n][(k & 1) * 2 + c], of_key = k & 1 ? v1[k >> 1][j].x : v0[k >> 1][j].x;
-                                if (!(score != -INFINITY && of_key < INFINITY)) continue;
-                                step = fmaxf(step, of_key);
-                                x = fmaxf(x, ex2(score - m - 10.f) * of_key);
-                            }
-                            step = of_item(step), x = of_item(x);
-                            // what came so far has become less by 2^more, so that what comes may count for that much more
-                            const int now = less[n][c] == 1.f ? kMostBy : exponent(by[n][j][c]), more = less[n][c] == 1.f ? 0 : min((int)fminf(-less[n][c], 240.f), kMostBy - now), e_step = exponent(step), e_x = exponent(x) + 10;
-                            const int then = min(now + more, step > 0.f ? min(x > 0.f ? (e_x >= e_step - 8 ? 4 - e_step : 3 - e_x) : kMostBy, 120 - e_step) : kMostBy);
+                            const int now = less[n][c] == 1.f ? kMostBy : exponent(by[n][j][c]);
+                            const int then = careful_exponent(make_float4(sc[0][n][c], sc[0][n][2 + c], sc[1][n][c], sc[1][n][2 + c]), make_float4(v0[0][j].x, v1[0][j].x, v0[1][j].x, v1[1][j].x), m_run[n][c], less[n][c], now);
                             by[n][j][c] = power_of_two(then);
                             const float factor = power_of_two(max(then - now, -126));
 #pragma unroll
