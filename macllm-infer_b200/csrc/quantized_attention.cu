@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                     if (whole || (pos >= lo && pos < hi)) least = fminf(least, step);
                 }
                 largest[j] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                plain = plain && largest[j] <= 256.f * __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+                const float smallest = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));   // the whole warp, whatever its threads have found so far
+                plain = plain && largest[j] <= 256.f * smallest;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll

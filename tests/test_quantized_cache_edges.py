@@ -40,6 +40,18 @@ def test_shares_are_counted_alike_in_every_kernel():
     assert re.search(r"total \+= \(float\)keys_of", text)   # whole numbers, added
 
 
+def test_whole_warps_exchange_what_they_have():
+    """An exchange among all threads of a warp stands behind nothing that some of them may find and others not: a thread that leaves it out leaves the others waiting."""
+    uniform = ("!keys &&", "t > 0 &&", "ok && n_tiles > 0", "n_tiles > 0 &&")   # known to whole warps alike
+    for name in ("quantized_attention.cu", "quantized_kv.cu", "token_logprobs.cu"):
+        text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+        for statement in re.split(r"[;{}]", text):
+            first = re.search(r"&&|\|\|", statement)
+            exchange = r"_sync\(|\bwarp_max\(|\bwarp_sum\(|\bof_item\("
+            if first and re.search(exchange, statement[first.end():]) and not re.search(exchange, statement[:first.start()]):
+                assert any(u in statement for u in uniform), (name, statement.strip())
+
+
 @pytest.mark.parametrize("beyond", [1 << 31, (1 << 32) + 5, (1 << 63) + 7])
 def test_numbers_that_lose_their_upper_bits_on_the_way_are_refused(mk, beyond):
     """A window of 2^32 + 5 was one of 5."""

@@ -233,6 +233,22 @@ def test_tokens_whose_sizes_rise_and_fall(dops, bits, dim, rows):  # noqa: F811
     check_attention(c, q, attend(dops, c, q))
 
 
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim, dtype, span", [(128, F16, 6), (128, BF16, 30), (256, BF16, 12)])
+@pytest.mark.parametrize("rows, window", [(1, 1000), (3, 0)])
+def test_a_few_tokens_of_other_sizes(dops, dim, dtype, span, bits, rows, window, seed):  # noqa: F811
+    """One token in fifty, and groups, of other sizes: the items of a warp have met different ones when the next come, so that its threads judge them differently."""
+    c = Cache(dtype, bits, 3, dim, 32, [501, 1433, 90], rows, seed=43 + seed).fill()
+    for kind in (2, 3):
+        scales = c.pools[kind]
+        f = torch.randint(-span, span + 1, scales.shape[:3], generator=c.g, device="cuda").float() * (torch.rand(scales.shape[:3], generator=c.g, device="cuda") < 0.02)
+        f = f[..., None] + torch.randint(-3, 4, scales.shape[:4], generator=c.g, device="cuda").float()
+        scales.copy_((scales.float() * torch.exp2(f.clamp(max=0) if kind == 2 else f)[..., None]).to(dtype))
+    q = queries(c, 15)
+    check_attention(c, q, attend(dops, c, q, window=window), window=window)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("rows", [1, 40])
 def test_many_light_keys_behind_a_heavy_one(dops, dtype, rows):  # noqa: F811
