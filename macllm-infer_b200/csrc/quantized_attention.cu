@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
     __shared__ uint64_t bars[2 * KST + 2 * VST + 8 * SUBS];
     __shared__ uint32_t tmem_slot;
     __shared__ int4 k_info[4], v_info[4];               // exponents of each 16 keys and values of a tile, times 4; bit 0 tells of values' scales that are not finite, bit 1 of exponents for each key
-    __shared__ int key_exponents[2][4][kKeyTile];       // of keys and of values, where the bit is set: from the 16 keys' on down
+    __shared__ int key_exponents[2][4][kKeyTile];       // of keys and of values, where the bit is set
     __shared__ uint32_t key_bounds[kCodeWarps][kTile];
     __shared__ uint32_t odd_groups[4][kKeyTile];        // groups of a key's values whose scales are not finite, where the bit is set
     uint64_t *k_full = bars, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST, *p_full = s_full + 2 * SUBS,
@@ -1118,28 +1118,26 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
             const int pos0 = begin + t * kKeyTile;
             tmem_wait_ld();
             // neither 0 nor infinite: where it would be, scores are 0 or overflow whatever it is
-            auto unit_of = [&](int info) { return fminf(fmaxf(factor * power_of_two(info >> 2), 1e-37f), 3e38f); };
-            // what has exponents of its own for each key comes under that of the 16
-            auto under = [&](const int (&info)[4], const int* of_keys) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    if (!(info[b] & 2)) continue;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) s[b * 16 + j] *= power_of_two(max(of_keys[b * 16 + j] - (info[b] >> 2), -126));
-                }
-            };
-            float u = unit_of(ki.x);
+            auto unit_of = [&](int e) { return fminf(fmaxf(factor * power_of_two(e), 1e-37f), 3e38f); };
+            float u = unit_of(ki.x >> 2);
             if (CAP || ((ki.x ^ ki.y) | (ki.x ^ ki.z) | (ki.x ^ ki.w) | (ki.x & 2)) != 0) {   // scores one by one; then they are what is exponentiated
                 const int info[4] = {ki.x, ki.y, ki.z, ki.w};
-                if ((ki.x | ki.y | ki.z | ki.w) & 2) under(info, key_exponents[0][t & 3]);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const float ub = unit_of(info[b]);
+                    const float ub = unit_of(info[b] >> 2);
+                    if (info[b] & 2) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        float v = s[b * 16 + j] * ub;
-                        if (CAP) v = (wide_cap ? capped_wide(v, a.softcap, two_over_cap) : capped(v, a.softcap, two_over_cap)) * kLog2e;
-                        s[b * 16 + j] = v;
+                        for (int j = 0; j < 16; ++j) s[b * 16 + j] *= unit_of(key_exponents[0][t & 3][b * 16 + j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[b * 16 + j] *= ub;
+                    }
+                    if (CAP) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float v = s[b * 16 + j];
+                            s[b * 16 + j] = (wide_cap ? capped_wide(v, a.softcap, two_over_cap) : capped(v, a.softcap, two_over_cap)) * kLog2e;
+                        }
                     }
                 }
                 u = 1.f;
@@ -1182,25 +1180,37 @@ __global__ void __launch_bounds__(Many<D, BITS, SUBS>::THREADS, 1) many_items_ke
                 if (m_run != -INFINITY) e_run = vi.x >> 2;   // its largest weight is 2^kWeightBits
             } else if (((vi.x ^ e_run * 4) | (vi.y ^ e_run * 4) | (vi.z ^ e_run * 4) | (vi.w ^ e_run * 4)) != 0) {
                 const int info[4] = {vi.x, vi.y, vi.z, vi.w}, ev[4] = {vi.x >> 2, vi.y >> 2, vi.z >> 2, vi.w >> 2};
-                if ((vi.x | vi.y | vi.z | vi.w) & 2) under(info, key_exponents[1][t & 3]);
-                int top = -1000;   // weights times 2^ev are below 2^top
+                const int* of_keys = key_exponents[1][t & 3];
+                int top = -1000;   // weights times 2^e are below 2^top
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    float most = 0.f;
+                    if (info[b] & 2) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) most = fmaxf(most, s[b * 16 + j]);
-                    if (most > 0.f) top = max(top, ev[b] + exponent(fminf(most, 32767.f)) + 1);
+                        for (int j = 0; j < 16; ++j)
+                            if (s[b * 16 + j] > 0.f) top = max(top, of_keys[b * 16 + j] + exponent(fminf(s[b * 16 + j], 32767.f)) + 1);
+                    } else {
+                        float most = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) most = fmaxf(most, s[b * 16 + j]);
+                        if (most > 0.f) top = max(top, ev[b] + exponent(fminf(most, 32767.f)) + 1);
+                    }
                 }
                 const int low = max(e_run - (int)fminf(-less, 240.f), -120);   // what came so far has become less
-                const bool alike = ev[0] == ev[1] && ev[0] == ev[2] && ev[0] == ev[3];
+                const bool alike = ev[0] == ev[1] && ev[0] == ev[2] && ev[0] == ev[3] && ((vi.x | vi.y | vi.z | vi.w) & 2) == 0;
                 const int e = alike && top >= ev[0] + 4 && top <= ev[0] + 15 && low <= ev[0] + 8 ? ev[0] : (top > low + 15 ? top - 8 : low);
                 alpha = ex2(less + (float)(e_run - e));
                 e_run = e;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const float to = ev[b] - e < -126 ? 0.f : power_of_two(min(ev[b] - e, 126));
+                    auto to = [&](int from) { return from - e < -126 ? 0.f : power_of_two(min(from - e, 126)); };
+                    const float all = to(ev[b]);
+                    if (info[b] & 2) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) s[b * 16 + j] *= to;
+                        for (int j = 0; j < 16; ++j) s[b * 16 + j] *= to(of_keys[b * 16 + j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[b * 16 + j] *= all;
+                    }
                 }
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {

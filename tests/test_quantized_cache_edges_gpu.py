@@ -163,6 +163,26 @@ def test_what_later_rows_see_has_no_say(dops, dtype, huge, kind, dim, bits, rows
     check_attention(clean, q[keep], got[keep])
 
 
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim, bits", [(64, 4), (128, 8), (256, 8)])
+@pytest.mark.parametrize("rows", [2, 12, 40])
+def test_sizes_at_both_ends_of_the_type(dops, kind, dim, bits, rows):  # noqa: F811
+    """Keys or values of 1e-20 beside ones of 1e30 that only later rows see."""
+    c = Cache(BF16, bits, 1, dim, 16, [rows + 60, rows + 1, 3 * rows], rows, seed=42).fill()
+    c.pools[2 + kind].copy_((c.pools[2 + kind].float() * 2.0 ** -66).to(BF16))
+    q = queries(c, 4)
+    if kind == 0:
+        q *= 2.0 ** 66
+    for lane, n in enumerate(c.lengths_list):
+        x = torch.randn(1, dim, generator=c.g, device="cuda")
+        put(c, lane, n - 1, kind, x / x.abs().max() * 1e30)
+    got = attend(dops, c, q)
+    keep = [i for i in range(c.total) if (i + 1) % rows]
+    clean = Cache(BF16, bits, 1, dim, 16, [n - 1 for n in c.lengths_list], rows - 1, seed=42)
+    clean.pools, clean.tables = c.pools, c.tables
+    check_attention(clean, q[keep], got[keep])
+
+
 @pytest.mark.parametrize("dtype, huge", HUGE)
 @pytest.mark.parametrize("kind", [0, 1])
 @pytest.mark.parametrize("dim, bits", [(64, 4), (128, 8), (256, 4)])
