@@ -38,7 +38,7 @@ __device__ __forceinline__ float capped_wide(float v, float cap, float two_over_
     return y < 0.0625f ? v * fmaf(y, fmaf(y, fmaf(y, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f) : capped(v, cap, two_over_cap);
 }
 
-// FloatPair 32-bit numbers at once.
+// Two 32-bit numbers at once.
 struct FloatPair {
     float x, y;
     __device__ __forceinline__ uint64_t bits() const {

@@ -133,9 +133,11 @@ __device__ __forceinline__ Shares shares_of(const QuantAttnArgs& a, const LaneRa
 // largest step, where sizes are far apart by the largest weight times step that the item sees.  So what an item does not see, or sees with little weight, and other groups' sizes leave its results as exact as
 // they are.  (One power of two for the largest step of all took ten bits off ordinary values' weights beside one of 6e4; it was faster by 2 % for single tokens at heads of 128, by 6 % for drafts at
 // heads of 256.)
+// The tensor cores cut a sum by its operands' exponent fields, which for subnormals are above the values: in 4 bits a score is off by 2^-22.0 of sum |q| |k| (root mean square, heads of 64).  With codes made normal
+// numbers, an instruction more for each two, it is 2^-22.6, as in 8 bits either way; that takes 8 % longer for single tokens at heads of 128, 11 % for drafts at heads of 256.
 // What bounds it is issue slots: about 370 instructions of a warp for 16 keys of heads of 128 (4096 values), half of the slots taken with twelve warps on an SM.  48 lanes of 200 to 6000 tokens, 32 heads of 128 over 8,
-// 4 bits: 49 us, 2.0 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 42 us, 2.6 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 144 us, 1.9 TB/s (outputs of all tiles in one accumulator: 47, 40 and
-// 123 us, but see there).  Codes by ordinary loads
+// 4 bits: 49.9 us, 1.9 TB/s; 3 contexts of up to 120001 tokens, 16 heads over 4: 42.4 us, 2.6 TB/s; 20 lanes of up to five rows, heads of 256, 8 bits: 152 us, 1.8 TB/s.  Before each item and group had a
+// power of two of its own: 49, 42 and 144 us, with outputs of all tiles in one accumulator (but see there) 47, 40 and 123; codes by ordinary loads
 // a tile ahead: 62, 124 and 149 us before the keys were shared out by lengths; 32 keys a step do 1.1 times as well as 16, four CTAs on an SM with 128 registers no better than three.
 constexpr int kFewItems = 32;            // of a lane and KV head: more go to the tall kernel
 constexpr int kTile = 16, kHalves = 2, kStep = kHalves * kTile;
@@ -608,8 +610,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        // Products align their sums by exponent fields, which for subnormal codes are up to 2^10 above the value: a sum is cut at 2^-17 of it or so.  Over many tiles in one
-                        // accumulator that would add up, so that each tile's is added in 32 bits.
+                        // Products align their sums by exponent fields, which for subnormal codes are up to 2^10 above the value: a sum is cut at 2^-14 of the largest weight's step at the most.  Over many
+                        // tiles in one accumulator that would add up, so that each tile's is added in 32 bits: over 2048 keys results are off by 2^-20.8 of the mean of |v| in 4 bits, by 2^-22.4 in 8 (root mean squares).
                         float part[4] = {0.f, 0.f, 0.f, 0.f};
                         mma_f16(part, a0, a1, a2, a3, hi_b[n][j][0], hi_b[n][j][1]);
                         mma_f16(part, a0, a1, a2, a3, lo_b[n][j][0], lo_b[n][j][1]);
@@ -689,8 +691,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few<D, BITS, NT>::CTAS) few_items
 // numbers of keys out of their codes, 16 keys each, four of values: codes into registers two tiles ahead, f16 numbers into the swizzled rows that the products read.  A warp for each tile of items issues its
 // products; four hold an item to a thread.  Two tiles of items share the numbers, and one's softmax runs under the other's products.
 // What bounds it is the chain of a tile's softmax: 2700 clocks for 256 items by 64 keys of heads of 128, half of them exponentials (two warps of a scheduler come to them together), where products take 1024: tensor pipe
-// 37 % busy.  4 portions of 1000 rows, 32 heads of 128 over 4, behind 2500 to 12000 tokens: 400 us, 721 TFLOP/s; 2048 rows of 32 heads over 8 behind 16384: 677 us, 761.  One thread issuing all products: 498 us;
-// codes through bulk copies and shared memory: 441; turns at the exponentials: 441; a fourth of the exponentials as polynomials on the other pipes: 401.
+// 37 % busy.  4 portions of 1000 rows, 32 heads of 128 over 4, behind 2500 to 12000 tokens: 395 us, 729 TFLOP/s; 2048 rows of 32 heads over 8 behind 16384: 666 us, 774.  Where it took 400,
+// one thread issuing all products took 498, codes through bulk copies and shared memory 441, turns at the exponentials 441, a fourth of the exponentials as polynomials on the other pipes 401.
 // A code becomes 1024 + c by its bits, c by a subtraction, and low + step c by one fused multiply-add in f16: rounded once, to 11 bits, as a 16-bit cache would hold it; weights are
 // rounded to 11 bits for the second product.  Scales come with a power of two of their own for every 16 keys (multiples of 2^8, so that neighbours share one): scores are multiplied by the
 // keys', weights by the values' over the row's where they differ.  The row's goes by weights times sizes, so that values that it does not see, or sees with hardly any weight, take nothing off the others, whatever
@@ -1440,10 +1442,13 @@ QuantAttnPlan quantized_attention_plan(int q_heads, int kv_heads, int d, int bit
     const int64_t table = (int64_t)width * block_tokens, window_keys = (int64_t)window + rows + 16;
     p.cut.window_keys = (int)std::min<int64_t>(window_keys, INT32_MAX);
     p.cut.least = p.items > 16 ? 256 : 512;
+    // Lanes that fill the SMs by themselves, or four times over where they have few items, are not shared out: 4 portions of 375 to 875 rows take 395 us so and 469 shared out, 24 lanes of 12 rows 149 and 163.  The
+    // bound does not look at the lengths, which are the device's, and one lane far longer than the others pays for that: 19 lanes of 64 items, one of 12000 tokens among ones of 300, take 207 us and would take 45
+    // (18 lanes, which are shared out, 55); 222 single tokens, one of 40000 among ones of 300, 433 and would take 111.
     p.cut.split = (window > 0 ? std::min(table, window_keys) : table) > p.cut.least && lanes < (p.items > 16 ? 1 : 4) * want;
-    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 42 us,
-    // with some of them in a second wave about 10 more).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens, before outputs of tiles were added in 32 bits: 47 us; shares of the largest size for one
-    // wave 56, half as large ones 52).
+    // A lane's last share is a part of one, so `want` less the lanes is one wave: CTAs of many items are alone on an SM, and few lanes' CTAs all last as long (3 contexts of up to 120001 tokens: 42.3 us,
+    // with half as many more shares 52.5).  Many lanes' differ, and a second wave of smaller ones evens them out (48 lanes of 200 to 6000 tokens: 49.9 us; shares of the largest size for one
+    // wave 54.9, 2.5 times as many 54.2; 20 lanes of up to five rows, heads of 256: 152, 158 and 149).
     const double shares = p.items > 16 || lanes <= want / 4 ? std::max(want / 2, want - lanes) : 1.5 * want;
     p.cut.want = (float)shares;
     p.slots = p.cut.split ? lanes + (int)std::min(shares, (double)lanes * (double)table / p.cut.least) + 1 : lanes;

@@ -195,7 +195,7 @@ __device__ __forceinline__ void codes_of(const float (&x)[8], float low, float s
 }
 
 // A warp has ROWS rows of K or V, and their places in as many threads; eight values to a thread, a group to eight threads, four of a thread's pieces on their way together.
-// What bounds it is instructions, about 16 for a value: 16383 rows of 8 heads of 128, K and V, bf16 into 4 bits (86 MB read and written): 31 us, 2.8 TB/s.  With a division for each value 38 us.
+// What bounds it is instructions, about 16 for a value: 16383 rows of 8 heads of 128, K and V, bf16 into 4 bits (86 MB read and written): 32.3 us, 2.7 TB/s.  With a division for each value 38 us where it took 31.
 constexpr int kAhead = 4;
 
 template <typename T, int BITS, int ROWS>

@@ -9,8 +9,8 @@
 // The likeliest `top` of a run: the top-th best of the threads' maxima is a bound that at least `top` values reach and few more do, only the vectors of threads that reach it are
 // looked at again (in L2), and the candidates are ranked by counting.  Where too many reach it - thousands of equal logits, or most of them masked - a radix select over (value, token) finds the
 // top-th key exactly, in up to seven more passes.  The leader of a cluster merges the sorted lists by binary search.
-// What bounds it is HBM and, for 16-bit logits, instructions beside it (8 for a value): 2000 rows of 128256 bf16 logits 99 us, 5.2 TB/s (117 with sums of single numbers and bounds checked for each
-// vector); 40 rows of 151936 f32 with 20 alternatives 16.9 us, 6 of them the alternatives; 5 rows of 32000 with 5 alternatives 9.0, of which 3.
+// What bounds it is HBM and, for 16-bit logits, instructions beside it (8 for a value): 2000 rows of 128256 bf16 logits 99.6 us, 5.2 TB/s (117 with sums of single numbers and bounds checked for each
+// vector); 40 rows of 151936 f32 with 20 alternatives 17.1 us, 6 of them the alternatives; 5 rows of 32000 with 5 alternatives 9.1, of which 3.
 #include "token_logprobs.h"
 #include "attention_math.cuh"
 #include <cuda_bf16.h>
