@@ -107,6 +107,7 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
         const float2 ml = s0 + lane < parts ? __ldcg(a.part_ml + (s0 + lane) * n_rows + row) : make_float2(-INFINITY, 0.f);
         const float m_new = fmaxf(m, warp_max(ml.x)), m_use = m_new == -INFINITY ? 0.f : m_new;
         const float old = ex2(m - m_use), f = ml.y == 0.f ? 0.f : ex2(ml.x - m_use);
+        const uint32_t wrote = __ballot_sync(0xffffffffu, ml.y != 0.f);   // not by weights: one of 0 does not hide NaN
         l = l * old + warp_sum(ml.y * f);
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] *= old;
@@ -121,7 +122,7 @@ __device__ __forceinline__ void add_parts(const SharedAttnArgs& a, int64_t row, 
                 w[s] = b + s < 32 ? __shfl_sync(0xffffffffu, f, b + s) : 0.f;
 #pragma unroll
                 for (int j = 0; j < V; ++j) x[s][j] = 0.f;
-                if (w[s] == 0.f) continue;
+                if (b + s >= 32 || !(wrote >> (b + s) & 1u)) continue;
                 const float* src = a.part_o + ((s0 + b + s) * n_rows + row) * D + lane * V;
                 if constexpr (V == 2) {
                     const float2 y = __ldcg(reinterpret_cast<const float2*>(src));

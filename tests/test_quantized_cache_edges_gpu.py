@@ -130,6 +130,23 @@ def test_a_value_that_is_not_finite_reaches_every_row_that_sees_it(dops, rows, l
     assert torch.isnan(got[..., dim - 64:]).all() and torch.isfinite(got[..., :dim - 64]).all()
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("shared", [0, 256])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128), (4, 1, 256)])
+def test_a_value_that_is_not_finite_reaches_every_row_that_sees_it_in_16_bits(dops, rows, shared, heads):  # noqa: F811
+    """The same of shared_attention, whose lanes are shared out alike."""
+    from test_device_ops_gpu import Batch
+    b = Batch(F16, *heads, 16, shared, [5000, 90], rows, seed=44)
+    n = int(b.lengths[0])
+    ids = b.tables[0, :-(-n // 16)].long()
+    b.pools[0][ids] = 1.0
+    b.pools[0][b.tables[0, :n // 48].long()] = -1.0   # keys whose scores are below the others' by 2 * 32 * dim^0.5, 2^-739 and less
+    b.pools[1][int(b.tables[0, 0])][:, 5, :heads[2] // 2] = math.nan
+    b.q.fill_(32.0)
+    got = torch.isnan(b.run(dops))
+    assert got[:rows, :, :heads[2] // 2].all() and not got[:rows, :, heads[2] // 2:].any()
+
+
 # ---- magnitudes far apart -----------------------------------------------------------------------------------------------------------------
 
 
